@@ -64,7 +64,9 @@
 extern "C" {
 #endif
 
-enum msa_dtype { MSA_F32 = 0, MSA_BF16 = 1, MSA_F16 = 2 };
+/* MSA_I8 and MSA_FP8 (OCP e4m3) are types of cache rows only: codes with one
+ * fp32 scale per row (msa_cache_write). */
+enum msa_dtype { MSA_F32 = 0, MSA_BF16 = 1, MSA_F16 = 2, MSA_I8 = 3, MSA_FP8 = 4 };
 
 enum msa_status {
   MSA_OK = 0,
@@ -215,6 +217,56 @@ int msa_decode_noalloc(const void* q, int64_t q_sb, int64_t q_sh,
                        const void* vcache, int64_t v_sb, int64_t v_st, int64_t v_sh,
                        int B, int H, int D, int dtype, int cache_len, int cache_cap, int window_hint,
                        const float* r, const float* w, float eps, void* y, void* stream);
+
+/*
+ * Key/value cache rows written in one launch, and read back.  No counterpart
+ * in the reference (its generate has no cache, model.py:111-141).
+ *   k, v     : rows (B, Tx, H, D) of type dtype, the projections' view as in
+ *              msa_fwd.
+ *   kcache, vcache : (B, cache_cap, H, D) rows of type cache_dtype, strides in
+ *              elements, unit stride over D; every row 16-byte aligned.
+ *              cache_dtype is dtype (a copy), MSA_I8 or MSA_FP8.
+ *   kscale, vscale : quantised caches: fp32 (B, cache_cap, H) with strides (sb,
+ *              st, sh); else null.  A row x is kept as the codes nearest to
+ *              TOP x / A (ties to the even code, decided exactly), A = max|x|,
+ *              TOP = 127 or 448, and the scale A / TOP; code * scale is its value.
+ *              A row of zeros has scale 0, a row with an infinity or a NaN codes
+ *              0 and scale NaN.
+ *   rows     : null, or a device int64 (B, T): row t is taken from row
+ *              rows[b, t] of k and v (outside [0, Tx): not written).  Null: row
+ *              t, and T = Tx.
+ *   count    : null, or a device int64 (B): rows t < count[b] only.
+ *   start    : null, or device int64 positions, one (start_n = 1) or one per
+ *              sequence (start_n = B): row t goes to position start + t.  Null:
+ *              start0.  Rows at positions outside the cache are not written.
+ * Positions and rows of one sequence must not repeat.  Everything else of the
+ * cache is left as it was.
+ */
+int msa_cache_write(const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh,
+                    const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                    int B, int T, int Tx, int H, int D, int dtype,
+                    const int64_t* rows, const int64_t* count,
+                    const int64_t* start, int start_n, int64_t start0,
+                    void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_sh,
+                    void* vcache, int64_t vc_sb, int64_t vc_st, int64_t vc_sh,
+                    int cache_cap, int cache_dtype,
+                    float* kscale, int64_t ks_sb, int64_t ks_st, int64_t ks_sh,
+                    float* vscale, int64_t vs_sb, int64_t vs_st, int64_t vs_sh, void* stream);
+
+/*
+ * The values of positions start .. start + T - 1 (as msa_cache_write takes
+ * them) into contiguous k, v (B, T, H, D) of type dtype: code * scale, rounded
+ * once; a copy where cache_dtype is dtype.  Positions outside the cache read
+ * as zeros.
+ */
+int msa_cache_read(const void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_sh,
+                   const void* vcache, int64_t vc_sb, int64_t vc_st, int64_t vc_sh,
+                   int cache_cap, int cache_dtype,
+                   const float* kscale, int64_t ks_sb, int64_t ks_st, int64_t ks_sh,
+                   const float* vscale, int64_t vs_sb, int64_t vs_st, int64_t vs_sh,
+                   int B, int T, int H, int D, int dtype,
+                   const int64_t* start, int start_n, int64_t start0,
+                   void* k, void* v, void* stream);
 
 /* Kernel timing for measurement.  After msa_timer_arm(kernel, n) the next n
  * launches of that kernel (any entry point) each record a HIP event pair on

@@ -1,0 +1,207 @@
+// Key/value cache rows: written in the model's type or as 8-bit codes with one
+// scale per row, and read back (gfx950).
+//
+// A quantised row x of D values is kept as D codes and the fp32 scale A/TOP,
+// A = max|x| and TOP the type's largest code (127; 448 for e4m3).  A code is the
+// nearest one to TOP x / A, ties to the even one, exactly: the fp32 quotient
+// decides unless a border lies within its error, and 64 bits decide then.  So
+// the codes depend on nothing but the row: a row written twice, or moved, has
+// the same codes.  A row of zeros has scale 0; a row that holds an infinity or
+// a NaN has scale NaN and codes 0, and reads back as NaN.
+//
+// Both kernels are bound by their bytes (a row in its type and its D + 4 bytes
+// of code and scale); D/VEC lanes share a row (16 bytes of it each), so the row
+// is read once, its maximum is a lane-group reduction and nothing is staged.
+// The rows of a block are consecutive positions of one head, whose codes are
+// contiguous in head-major storage.
+#include "msa_device.h"
+#include "msa_internal.h"
+
+namespace msa {
+
+// 16 bytes of a row in its type.
+template <typename T> struct RowVec;
+template <> struct RowVec<bf16> { typedef bf16x8 type; static constexpr int N = 8; };
+template <> struct RowVec<f16> { typedef f16x8 type; static constexpr int N = 8; };
+template <> struct RowVec<float> { typedef f32x4 type; static constexpr int N = 4; };
+
+// The largest x of aligned groups of G lanes (non-negative integers).
+template <int G>
+__device__ inline uint32_t group_max_u32(uint32_t x) {
+#pragma unroll
+  for (int o = 1; o < G; o <<= 1) {
+    const uint32_t y = (uint32_t)__shfl_xor((int)x, o);
+    x = y > x ? y : x;
+  }
+  return x;
+}
+
+template <typename C> struct CodeTop { static constexpr float v = 1.0f; };
+template <> struct CodeTop<int8_t> { static constexpr float v = 127.0f; };
+template <> struct CodeTop<fp8> { static constexpr float v = 448.0f; };
+
+// The code of x in a row of largest magnitude `top`, inv = TOP/top in fp32.
+// t = x inv is within 2^-22 of the quotient; where both ends of t (1 +- 2^-21)
+// have one code, it is the quotient's.
+template <typename C>
+__device__ inline uint32_t code_of(float x, float inv, float top) {
+  const float t = x * inv;
+  constexpr float e = 4.76837158203125e-7f;  // 2^-21
+  if constexpr (__is_same(C, int8_t)) {
+    const float lo = rintf(fmaf(-e, t, t)), hi = rintf(fmaf(e, t, t));
+    if (lo == hi) return (uint32_t)(int)lo & 0xffu;
+    return (uint32_t)(int)rint(127.0 * (double)x / (double)top) & 0xffu;
+  } else {
+    const uint32_t two = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(fmaf(-e, t, t), fmaf(e, t, t), 0, false);
+    if (((two ^ (two >> 8)) & 0xffu) == 0u) return two & 0xffu;
+    // rounded to odd on the way to fp32, so that the second rounding sees on
+    // which side of a border the quotient lies
+    const double d = 448.0 * (double)x / (double)top;
+    float f = (float)d;
+    if ((double)f != d) {
+      uint32_t b = __float_as_uint(f);
+      if (fabs((double)f) > fabs(d)) b -= 1u;
+      f = __uint_as_float(b | 1u);
+    }
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f, f, 0, false) & 0xffu;
+  }
+}
+
+// Values of four codes.
+__device__ inline void decode4(uint32_t c, float (&v)[4], int8_t) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (float)(int8_t)(c >> (8 * e));
+}
+__device__ inline void decode4(uint32_t c, float (&v)[4], fp8) {
+  const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false);
+  const auto b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+  v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1];
+}
+
+// Cache position of row t of sequence b, or -1 if it lies outside the cache.
+__device__ inline int cache_position(const CacheCall& a, int b, int t) {
+  int64_t s = a.start != nullptr ? a.start[(int64_t)b * a.start_step] : a.start0;
+  if (s < -(int64_t)a.T || s >= (int64_t)a.cap) return -1;
+  s += t;
+  return s >= 0 && s < a.cap ? (int)s : -1;
+}
+
+// Block (x, y, z): 256 / LPR rows from row x 256/LPR on of head y = b H + h, of
+// k (z = 0) or v.
+template <typename T, typename C, int D>
+__global__ __launch_bounds__(256) void cache_write_kernel(CacheCall a) {
+  using vec = typename RowVec<T>::type;
+  constexpr int VEC = RowVec<T>::N, LPR = D / VEC;
+  const int z = blockIdx.z, b = blockIdx.y / a.H, h = blockIdx.y % a.H;
+  const int t = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, d0 = (threadIdx.x % LPR) * VEC;
+  int64_t src = t;
+  int pos = -1;
+  if (t < a.T && (a.count == nullptr || t < a.count[b])) {
+    if (a.rows != nullptr) src = a.rows[(int64_t)b * a.T + t];
+    if (src >= 0 && src < a.Tx) pos = cache_position(a, b, t);
+  }
+  vec x;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) x[e] = from_f<T>(0.0f);
+  const Strides3 xs = a.xs[z], cs = a.cs[z], ss = a.ss[z];
+  if (pos >= 0) x = *reinterpret_cast<const vec*>((const T*)a.x[z] + b * xs.sb + src * xs.st + h * xs.sh + d0);
+  char* row = (char*)a.c[z] + (b * cs.sb + (int64_t)pos * cs.st + h * cs.sh + d0) * (int64_t)sizeof(C);
+  if constexpr (sizeof(C) > 1) {
+    if (pos >= 0) *reinterpret_cast<vec*>(row) = x;
+  } else {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const uint32_t y = __float_as_uint(to_f(x[e])) & 0x7fffffffu;
+      m = y > m ? y : m;
+    }
+    m = group_max_u32<LPR>(m);  // a NaN's magnitude is above an infinity's
+    if (pos < 0) return;
+    const bool finite = m < 0x7f800000u;
+    const float top = __uint_as_float(m);
+    uint32_t code[VEC / 4];
+    if (finite && m != 0u) {
+      // below 2^-118 TOP/top may leave fp32's range: scaled by a power of two
+      const float up = m < 0x04800000u ? 1.0633823966279327e37f : 1.0f;  // 2^123
+      const float inv = CodeTop<C>::v / (top * up);
+#pragma unroll
+      for (int w = 0; w < VEC / 4; ++w) {
+        code[w] = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) code[w] |= code_of<C>(to_f(x[4 * w + e]) * up, inv, top * up) << (8 * e);
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < VEC / 4; ++w) code[w] = 0u;
+    }
+    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(row) = make_uint2(code[0], code[1]);
+    else *reinterpret_cast<uint32_t*>(row) = code[0];
+    if (d0 == 0)
+      a.s[z][b * ss.sb + (int64_t)pos * ss.st + h * ss.sh] = finite ? top / CodeTop<C>::v : __uint_as_float(0x7fc00000u);
+  }
+}
+
+// The same block shape; rows outside the cache read as zeros.
+template <typename T, typename C, int D>
+__global__ __launch_bounds__(256) void cache_read_kernel(CacheCall a) {
+  using vec = typename RowVec<T>::type;
+  constexpr int VEC = RowVec<T>::N, LPR = D / VEC;
+  const int z = blockIdx.z, b = blockIdx.y / a.H, h = blockIdx.y % a.H;
+  const int t = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, d0 = (threadIdx.x % LPR) * VEC;
+  if (t >= a.T) return;
+  const int pos = cache_position(a, b, t);
+  const Strides3 xs = a.xs[z], cs = a.cs[z], ss = a.ss[z];
+  vec x;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) x[e] = from_f<T>(0.0f);
+  if (pos >= 0) {
+    const char* row = (const char*)a.c[z] + (b * cs.sb + (int64_t)pos * cs.st + h * cs.sh + d0) * (int64_t)sizeof(C);
+    if constexpr (sizeof(C) > 1) {
+      x = *reinterpret_cast<const vec*>(row);
+    } else {
+      const float sc = a.s[z][b * ss.sb + (int64_t)pos * ss.st + h * ss.sh];
+#pragma unroll
+      for (int w = 0; w < VEC / 4; ++w) {
+        float v[4];
+        decode4(reinterpret_cast<const uint32_t*>(row)[w], v, C{});
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * w + e] = from_f<T>(v[e] * sc);
+      }
+    }
+  }
+  *reinterpret_cast<vec*>((T*)const_cast<void*>(a.x[z]) + b * xs.sb + (int64_t)t * xs.st + h * xs.sh + d0) = x;
+}
+
+template <typename T, typename C, int D>
+static hipError_t launch_cache_t(const CacheCall& c) {
+  constexpr int rows = 256 / (D / RowVec<T>::N);
+  const dim3 grid((unsigned)((c.T + rows - 1) / rows), (unsigned)(c.B * c.H), 2u);
+  if (c.read) hipLaunchKernelGGL((cache_read_kernel<T, C, D>), grid, dim3(256), 0, c.stream, c);
+  else hipLaunchKernelGGL((cache_write_kernel<T, C, D>), grid, dim3(256), 0, c.stream, c);
+  return hipGetLastError();
+}
+
+template <typename T, typename C>
+static hipError_t launch_cache_d(const CacheCall& c) {
+  switch (c.D) {
+    case 16: return launch_cache_t<T, C, 16>(c);
+    case 32: return launch_cache_t<T, C, 32>(c);
+    case 64: return launch_cache_t<T, C, 64>(c);
+    default: return launch_cache_t<T, C, 128>(c);
+  }
+}
+
+template <typename T>
+static hipError_t launch_cache_c(const CacheCall& c) {
+  if (c.cache_dtype == kInt8) return launch_cache_d<T, int8_t>(c);
+  if (c.cache_dtype == kFp8) return launch_cache_d<T, fp8>(c);
+  return launch_cache_d<T, T>(c);
+}
+
+hipError_t launch_cache(const CacheCall& c) {
+  if (c.dtype == 1) return launch_cache_c<bf16>(c);
+  if (c.dtype == 2) return launch_cache_c<f16>(c);
+  return launch_cache_c<float>(c);
+}
+
+}  // namespace msa

@@ -439,6 +439,94 @@ int msa_decode_noalloc(const void* q, int64_t q_sb, int64_t q_sh, const void* kc
   return hip_status(msa::launch_decode(c), "msa_decode_noalloc launch");
 }
 
+// Shapes, types and cache tensors shared by the cache entry points.
+static int check_cache(int B, int T, int H, int D, int dtype, const void* kcache, int64_t kc_sb, int64_t kc_st,
+                       int64_t kc_sh, const void* vcache, int64_t vc_sb, int64_t vc_st, int64_t vc_sh, int cache_cap,
+                       int cache_dtype, const float* kscale, int64_t ks_sb, int64_t ks_st, int64_t ks_sh,
+                       const float* vscale, int64_t vs_sb, int64_t vs_st, int64_t vs_sh) {
+  msa::Geometry g;
+  int rc = check_geometry(B, H, T, cache_cap, D, dtype, 1, &g);
+  if (rc != MSA_OK) return rc;
+  const bool codes = cache_dtype == MSA_I8 || cache_dtype == MSA_FP8;
+  if (!codes && cache_dtype != dtype)
+    return fail(MSA_ERR_INVALID, "cache_dtype must be the rows' dtype, MSA_I8 or MSA_FP8");
+  const int m = codes ? 16 : (dtype == MSA_F32 ? 4 : 8);
+  const int64_t st[2][3] = {{kc_sb, kc_st, kc_sh}, {vc_sb, vc_st, vc_sh}};
+  const int64_t sc[2][3] = {{ks_sb, ks_st, ks_sh}, {vs_sb, vs_st, vs_sh}};
+  const void* c[2] = {kcache, vcache};
+  const float* s[2] = {kscale, vscale};
+  for (int z = 0; z < 2; ++z) {
+    const char* name = z == 0 ? "kcache" : "vcache";
+    if ((rc = check_out(name, c[z])) != MSA_OK) return rc;
+    for (int e = 0; e < 3; ++e)
+      if (st[z][e] < 0 || st[z][e] % m)
+        return fail(MSA_ERR_INVALID, "%s strides must be non-negative multiples of %d elements", name, m);
+    if (!codes) continue;
+    if (s[z] == nullptr) return fail(MSA_ERR_INVALID, "%s of 8-bit codes needs its scales", name);
+    if (((uintptr_t)s[z] & 3u) != 0 || sc[z][0] < 0 || sc[z][1] < 0 || sc[z][2] < 0)
+      return fail(MSA_ERR_INVALID, "%s scales must be fp32 with non-negative strides", name);
+  }
+  return MSA_OK;
+}
+
+static int check_start(const int64_t* start, int start_n, int B) {
+  if (start != nullptr && start_n != 1 && start_n != B)
+    return fail(MSA_ERR_INVALID, "start holds %d positions, 1 or B=%d needed", start_n, B);
+  return MSA_OK;
+}
+
+int msa_cache_write(const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st,
+                    int64_t v_sh, int B, int T, int Tx, int H, int D, int dtype, const int64_t* rows,
+                    const int64_t* count, const int64_t* start, int start_n, int64_t start0, void* kcache,
+                    int64_t kc_sb, int64_t kc_st, int64_t kc_sh, void* vcache, int64_t vc_sb, int64_t vc_st,
+                    int64_t vc_sh, int cache_cap, int cache_dtype, float* kscale, int64_t ks_sb, int64_t ks_st,
+                    int64_t ks_sh, float* vscale, int64_t vs_sb, int64_t vs_st, int64_t vs_sh, void* stream) {
+  int rc = check_cache(B, T, H, D, dtype, kcache, kc_sb, kc_st, kc_sh, vcache, vc_sb, vc_st, vc_sh, cache_cap,
+                       cache_dtype, kscale, ks_sb, ks_st, ks_sh, vscale, vs_sb, vs_st, vs_sh);
+  if (rc != MSA_OK) return rc;
+  if (Tx < 0 || Tx > kMaxT || (rows == nullptr && T > Tx))
+    return fail(MSA_ERR_INVALID, "k and v hold %d rows, %d asked for", Tx, T);
+  if ((rc = check_start(start, start_n, B)) != MSA_OK) return rc;
+  if (B == 0 || T == 0 || Tx == 0) return ok();
+  if ((rc = check_tensor("k", k, k_sb, k_st, k_sh, dtype)) != MSA_OK) return rc;
+  if ((rc = check_tensor("v", v, v_sb, v_st, v_sh, dtype)) != MSA_OK) return rc;
+  msa::CacheCall c;
+  c.x[0] = k; c.x[1] = v; c.xs[0] = {k_sb, k_st, k_sh}; c.xs[1] = {v_sb, v_st, v_sh};
+  c.c[0] = kcache; c.c[1] = vcache; c.cs[0] = {kc_sb, kc_st, kc_sh}; c.cs[1] = {vc_sb, vc_st, vc_sh};
+  c.s[0] = kscale; c.s[1] = vscale; c.ss[0] = {ks_sb, ks_st, ks_sh}; c.ss[1] = {vs_sb, vs_st, vs_sh};
+  c.rows = rows; c.count = count; c.start = start; c.start_step = start_n == 1 ? 0 : 1; c.start0 = start0;
+  c.B = B; c.T = T; c.Tx = Tx; c.H = H; c.D = D; c.cap = cache_cap; c.dtype = dtype; c.cache_dtype = cache_dtype;
+  c.read = 0;
+  c.stream = (hipStream_t)stream;
+  return hip_status(msa::launch_cache(c), "msa_cache_write launch");
+}
+
+int msa_cache_read(const void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_sh, const void* vcache, int64_t vc_sb,
+                   int64_t vc_st, int64_t vc_sh, int cache_cap, int cache_dtype, const float* kscale, int64_t ks_sb,
+                   int64_t ks_st, int64_t ks_sh, const float* vscale, int64_t vs_sb, int64_t vs_st, int64_t vs_sh,
+                   int B, int T, int H, int D, int dtype, const int64_t* start, int start_n, int64_t start0, void* k,
+                   void* v, void* stream) {
+  int rc = check_cache(B, T, H, D, dtype, kcache, kc_sb, kc_st, kc_sh, vcache, vc_sb, vc_st, vc_sh, cache_cap,
+                       cache_dtype, kscale, ks_sb, ks_st, ks_sh, vscale, vs_sb, vs_st, vs_sh);
+  if (rc != MSA_OK) return rc;
+  if ((rc = check_start(start, start_n, B)) != MSA_OK) return rc;
+  if (B == 0 || T == 0) return ok();
+  if ((rc = check_out("k", k)) != MSA_OK) return rc;
+  if ((rc = check_out("v", v)) != MSA_OK) return rc;
+  msa::CacheCall c;
+  const int64_t sh = D, st = (int64_t)H * D, sb = st * T;
+  c.x[0] = k; c.x[1] = v; c.xs[0] = c.xs[1] = {sb, st, sh};
+  c.c[0] = const_cast<void*>(kcache); c.c[1] = const_cast<void*>(vcache);
+  c.cs[0] = {kc_sb, kc_st, kc_sh}; c.cs[1] = {vc_sb, vc_st, vc_sh};
+  c.s[0] = const_cast<float*>(kscale); c.s[1] = const_cast<float*>(vscale);
+  c.ss[0] = {ks_sb, ks_st, ks_sh}; c.ss[1] = {vs_sb, vs_st, vs_sh};
+  c.rows = nullptr; c.count = nullptr; c.start = start; c.start_step = start_n == 1 ? 0 : 1; c.start0 = start0;
+  c.B = B; c.T = T; c.Tx = T; c.H = H; c.D = D; c.cap = cache_cap; c.dtype = dtype; c.cache_dtype = cache_dtype;
+  c.read = 1;
+  c.stream = (hipStream_t)stream;
+  return hip_status(msa::launch_cache(c), "msa_cache_read launch");
+}
+
 int msa_selftest_mfma(const float* a16, const float* b16, float* out16, const float* a2, const float* b2,
                       float* out2, void* stream) {
   if (!a16 || !b16 || !out16 || !a2 || !b2 || !out2) return fail(MSA_ERR_INVALID, "null pointer");

@@ -104,6 +104,23 @@ int decode_chunk_keys();
 int decode_max_chunks(int max_len);
 hipError_t launch_decode(const DecodeCall& c);
 
+// Types of cache rows beside the input types 0..2 (msa.h's msa_dtype).
+constexpr int kInt8 = 3, kFp8 = 4;
+
+// Rows of a cache written or read back; index 0 is k, 1 is v.
+struct CacheCall {
+  const void* x[2]; Strides3 xs[2];  // the rows in the model's type: read by a write, written by a read
+  void* c[2]; Strides3 cs[2];        // the cache
+  float* s[2]; Strides3 ss[2];       // its scales (quantised caches)
+  const int64_t* rows;               // (B, T) which row of x each written row is, or null: row t
+  const int64_t* count;              // (B) rows written of each sequence, or null: T
+  const int64_t* start; int start_step;  // first position of each sequence (step 0: of all), or null: start0
+  int64_t start0;
+  int B, T, Tx, H, D, cap, dtype, cache_dtype, read;
+  hipStream_t stream;
+};
+hipError_t launch_cache(const CacheCall& c);
+
 // Waves that share a row (32-query or 32-key unit) in the live, dq and dK/dV
 // passes: launches with few rows split each row's units, so that about 2048
 // waves (2-byte types) or 4096 (fp32, whose rows take several times as long)

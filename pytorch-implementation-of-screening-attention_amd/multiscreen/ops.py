@@ -18,6 +18,8 @@ kernels, so their backward is too.
 GPU tensors only: a CPU tensor, or a missing libmsa.so, raises.
 """
 
+import contextlib
+
 import torch
 
 from . import _native
@@ -241,3 +243,138 @@ def decode_step_at(q, kcache, vcache, last_pos, r, w, eps=1e-8, workspace=None, 
                          _stream_ptr(dev))
     _native.check(rc, "msa_decode_at")
     return y
+
+
+# ---------------------------------------------------------------------------
+# Caches of 8-bit codes, several new tokens at once, and drafted tokens
+# ---------------------------------------------------------------------------
+_CACHE_DTYPES = {**_DTYPES, torch.int8: _native.MSA_I8, torch.float8_e4m3fn: _native.MSA_FP8}
+CODE_DTYPES = (torch.int8, torch.float8_e4m3fn)
+
+
+def _on(dev):
+    """Launches go to the tensors' device, whichever is current."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _check_gpu(what, **tensors):
+    """Every tensor given is on one GPU; returns it."""
+    dev = None
+    for name, x in tensors.items():
+        if x is None:
+            continue
+        if not x.is_cuda:
+            raise RuntimeError(f"{what} runs on the GPU only ({name} is a CPU tensor)")
+        if dev is not None and x.device != dev:
+            raise RuntimeError(f"{what}: {name} is on {x.device}, other tensors on {dev}")
+        dev = x.device
+    return dev
+
+
+def _index(x, name, *shapes):
+    """An int64 tensor of one of the shapes, contiguous."""
+    if x.dtype != torch.int64 or tuple(x.shape) not in shapes:
+        raise ValueError(f"{name} must be int64 of shape {' or '.join(map(str, shapes))}, got {x.dtype} {tuple(x.shape)}")
+    return x.contiguous()
+
+
+def _cache_args(what, kcache, vcache, kscale, vscale, dtype):
+    """Checks a cache pair (B, cap, H, D) and its scales (B, cap, H) against the rows' type; returns the C arguments
+    of the codes and of the scales."""
+    if kcache.dim() != 4 or kcache.shape != vcache.shape or kcache.dtype != vcache.dtype:
+        raise ValueError(f"{what}: the caches must be (B, cap, H, D) of one shape and type, got {kcache.dtype} "
+                         f"{tuple(kcache.shape)}, {vcache.dtype} {tuple(vcache.shape)}")
+    codes = kcache.dtype in CODE_DTYPES
+    if not codes and kcache.dtype != dtype:
+        raise TypeError(f"{what}: a cache of {kcache.dtype} does not hold rows of {dtype}")
+    mult = 16 // kcache.element_size()
+    args, scales = [], []
+    for name, c, s in (("kcache", kcache, kscale), ("vcache", vcache, vscale)):
+        if c.stride(3) != 1 or any(x % mult for x in c.stride()[:3]) or c.data_ptr() % 16:
+            raise ValueError(f"{what}: {name} needs unit stride over D and 16-byte aligned rows, got strides {c.stride()}")
+        if codes != (s is not None):
+            raise ValueError(f"{what}: {name} of {c.dtype} {'needs its scales' if codes else 'takes no scales'}")
+        if codes and (s.dtype != torch.float32 or s.shape != c.shape[:3]):
+            raise ValueError(f"{what}: the scales of {name} must be float32 {tuple(c.shape[:3])}, got {s.dtype} "
+                             f"{tuple(s.shape)}")
+        args += _args_bthd(c)
+        scales += (s.data_ptr(), *s.stride()) if codes else (None, 0, 0, 0)
+    return args, scales
+
+
+def _start_args(start, B, dev):
+    """(pointer or None, count, host value, tensor to keep) of an int or int64 device tensor."""
+    if not torch.is_tensor(start):
+        return None, 0, int(start), None
+    start = _index(start, "start", (1,), (B,))
+    return start.data_ptr(), start.numel(), 0, start
+
+
+def cache_write(k, v, kcache, vcache, start, kscale=None, vscale=None, rows=None, count=None):
+    """Writes rows k, v (B, T, H, D) to positions start, start + 1, ... of a cache.
+
+    kcache, vcache (B, cap, H, D): of k's type (copied), or torch.int8 /
+    torch.float8_e4m3fn codes with kscale, vscale float32 (B, cap, H): a row is
+    kept as the codes nearest to TOP x / max|x| (TOP = 127 or 448, ties to the
+    even code) and the scale max|x| / TOP.  Rows of zeros have scale 0; rows with
+    an infinity or a NaN read back as NaN.
+    start: an int (then all rows must fit), or an int64 CUDA tensor of 1 or B
+    elements (rows that would lie outside the cache are not written).
+    rows (B, T') int64, count (B) int64: row rows[b, t] of k and v goes to
+    position start + t, for t < count[b] only: the accepted path of
+    verify_drafts.  Rows outside k are not written.
+    The rest of the cache is left as it was.  No gradient flows through it.
+    """
+    L = _native.lib()
+    dev = _check_gpu("cache_write", k=k, v=v, kcache=kcache, vcache=vcache, kscale=kscale, vscale=vscale, rows=rows,
+                     count=count, start=start if torch.is_tensor(start) else None)
+    if k.dtype not in _DTYPES or v.dtype != k.dtype or k.shape != v.shape:
+        raise TypeError(f"cache_write: k and v must share shape and dtype float32, bfloat16 or float16, got {k.dtype} "
+                        f"{tuple(k.shape)}, {v.dtype} {tuple(v.shape)}")
+    es = k.element_size()
+    k, v = _as_bthd(k, "k", es), _as_bthd(v, "v", es)
+    B, Tx, H, D = k.shape
+    if kcache.dim() != 4 or (kcache.shape[0], *kcache.shape[2:]) != (B, H, D):
+        raise ValueError(f"cache_write: cache {tuple(kcache.shape)} does not match rows {tuple(k.shape)}")
+    codes, scales = _cache_args("cache_write", kcache, vcache, kscale, vscale, k.dtype)
+    cap = int(kcache.shape[1])
+    T = Tx
+    if rows is not None:
+        T = int(rows.shape[-1])
+        rows = _index(rows, "rows", (B, T))
+    if count is not None:
+        count = _index(count, "count", (B,))
+    ptr, n, host, keep = _start_args(start, B, dev)
+    if ptr is None and (host < 0 or host + (T if count is None else 0) > cap):
+        raise IndexError(f"KV cache capacity {cap} exceeded at position {host + T}")
+    with _on(dev):
+        rc = L.msa_cache_write(*_args_bthd(k), *_args_bthd(v), B, T, Tx, H, D, _DTYPES[k.dtype],
+                               rows.data_ptr() if rows is not None else None,
+                               count.data_ptr() if count is not None else None, ptr, n, host,
+                               *codes, cap, _CACHE_DTYPES[kcache.dtype], *scales, _stream_ptr(dev))
+    _native.check(rc, "msa_cache_write")
+
+
+def cache_read(kcache, vcache, kscale, vscale, start, length, dtype):
+    """The rows at positions start .. start + length - 1 of a cache (as
+    cache_write takes it) in `dtype`: code * scale, rounded once; (k, v), each
+    contiguous (B, length, H, D).  With a device `start`, positions outside the
+    cache read as zeros."""
+    L = _native.lib()
+    dev = _check_gpu("cache_read", kcache=kcache, vcache=vcache, kscale=kscale, vscale=vscale,
+                     start=start if torch.is_tensor(start) else None)
+    if dtype not in _DTYPES:
+        raise TypeError(f"cache_read: dtype must be float32, bfloat16 or float16, got {dtype}")
+    codes, scales = _cache_args("cache_read", kcache, vcache, kscale, vscale, dtype)
+    B, cap, H, D = kcache.shape
+    length = int(length)
+    ptr, n, host, keep = _start_args(start, B, dev)
+    if length < 0 or (ptr is None and (host < 0 or host + length > cap)):
+        raise IndexError(f"positions {host} .. {host + length} are outside the KV cache's capacity {cap}")
+    k = torch.empty((B, length, H, D), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    with _on(dev):
+        rc = L.msa_cache_read(*codes, cap, _CACHE_DTYPES[kcache.dtype], *scales, B, length, H, D, _DTYPES[dtype],
+                              ptr, n, host, k.data_ptr(), v.data_ptr(), _stream_ptr(dev))
+    _native.check(rc, "msa_cache_read")
+    return k, v
