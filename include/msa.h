@@ -268,6 +268,43 @@ int msa_cache_read(const void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_
                    const int64_t* start, int start_n, int64_t start0,
                    void* k, void* v, void* stream);
 
+/*
+ * Screening attention of a tree of N <= MSA_TREE_MAX drafted tokens per
+ * sequence over a cache; N = 1 decodes one token.  No counterpart in the
+ * reference (its generate re-runs the prefix for every token,
+ * model.py:111-141).
+ *   q        : (B, N, H, D) raw query projections, strides (sb, sn, sh), unit D.
+ *   kcache, vcache, kscale, vscale : as msa_cache_write leaves them;
+ *              cache_dtype is dtype, MSA_I8 or MSA_FP8.  The cache holds sequence b's
+ *              committed rows at positions [0, n_b) and its nodes' own rows at
+ *              n_b .. n_b + N - 1 (so n_b is clamped to [0, cache_cap - N]).
+ *   lengths  : device int64 n_b, one (lengths_n = 1) or one per sequence.
+ *   parents  : device int64, node i of sequence b continues node parents[b *
+ *              par_sb + i] < i, or is a root (any other value); null: a chain.
+ * Node i stands at position n_b + depth_i (a root's depth is 0) and sees the
+ * committed keys of its window (pos - w, pos], and of the drafted rows its own
+ * and its ancestors' within the window.  y (B, N, H, D) contiguous, of type
+ * dtype.  A key row that is not finite is never live; a value row that is not
+ * finite makes the nodes that a live pair brings it to NaN, and no others.
+ * window_hint as in msa_decode: it sizes the launch.  How a head's keys are
+ * split over blocks (the sums' order, so y's rounding) depends on it and on
+ * the shapes only: equal calls give bitwise equal y.
+ * workspace: msa_tree_workspace_bytes of the same sizes (0 where one block
+ * takes a head's keys), scratch of this call.
+ */
+#define MSA_TREE_MAX 64
+size_t msa_tree_workspace_bytes(int B, int H, int N, int D, int cache_cap, int window_hint);
+int msa_tree_decode(const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh,
+                    const void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_sh,
+                    const void* vcache, int64_t vc_sb, int64_t vc_st, int64_t vc_sh,
+                    int cache_cap, int cache_dtype,
+                    const float* kscale, int64_t ks_sb, int64_t ks_st, int64_t ks_sh,
+                    const float* vscale, int64_t vs_sb, int64_t vs_st, int64_t vs_sh,
+                    int B, int N, int H, int D, int dtype,
+                    const int64_t* lengths, int lengths_n, const int64_t* parents, int64_t par_sb, int window_hint,
+                    const float* r, const float* w, float eps,
+                    void* y, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Kernel timing for measurement.  After msa_timer_arm(kernel, n) the next n
  * launches of that kernel (any entry point) each record a HIP event pair on
  * their stream around the launch; several kernels can be armed at once.

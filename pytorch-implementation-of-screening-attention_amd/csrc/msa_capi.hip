@@ -450,6 +450,7 @@ static int check_cache(int B, int T, int H, int D, int dtype, const void* kcache
   const bool codes = cache_dtype == MSA_I8 || cache_dtype == MSA_FP8;
   if (!codes && cache_dtype != dtype)
     return fail(MSA_ERR_INVALID, "cache_dtype must be the rows' dtype, MSA_I8 or MSA_FP8");
+  if (B == 0 || T == 0) return MSA_OK;  // an empty call touches no tensor
   const int m = codes ? 16 : (dtype == MSA_F32 ? 4 : 8);
   const int64_t st[2][3] = {{kc_sb, kc_st, kc_sh}, {vc_sb, vc_st, vc_sh}};
   const int64_t sc[2][3] = {{ks_sb, ks_st, ks_sh}, {vs_sb, vs_st, vs_sh}};
@@ -525,6 +526,54 @@ int msa_cache_read(const void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_
   c.read = 1;
   c.stream = (hipStream_t)stream;
   return hip_status(msa::launch_cache(c), "msa_cache_read launch");
+}
+
+static int tree_blocks_of(int B, int H, int N, int cache_cap, int window_hint) {
+  return msa::tree_blocks(B, H, N, window_hint > 0 && window_hint < cache_cap ? window_hint : cache_cap);
+}
+
+size_t msa_tree_workspace_bytes(int B, int H, int N, int D, int cache_cap, int window_hint) {
+  if (B <= 0 || H <= 0 || N <= 0 || N > MSA_TREE_MAX || cache_cap <= 0 || cache_cap > kMaxT || (int64_t)B * H > 65535 ||
+      !(D == 16 || D == 32 || D == 64 || D == 128))
+    return 0;
+  const int blocks = tree_blocks_of(B, H, N, cache_cap, window_hint);
+  return blocks == 1 ? 0 : (size_t)B * H * blocks * N * D * sizeof(float);
+}
+
+int msa_tree_decode(const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const void* kcache, int64_t kc_sb,
+                    int64_t kc_st, int64_t kc_sh, const void* vcache, int64_t vc_sb, int64_t vc_st, int64_t vc_sh,
+                    int cache_cap, int cache_dtype, const float* kscale, int64_t ks_sb, int64_t ks_st, int64_t ks_sh,
+                    const float* vscale, int64_t vs_sb, int64_t vs_st, int64_t vs_sh, int B, int N, int H, int D,
+                    int dtype, const int64_t* lengths, int lengths_n, const int64_t* parents, int64_t par_sb,
+                    int window_hint, const float* r, const float* w, float eps, void* y, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  int rc = check_cache(B, N, H, D, dtype, kcache, kc_sb, kc_st, kc_sh, vcache, vc_sb, vc_st, vc_sh, cache_cap,
+                       cache_dtype, kscale, ks_sb, ks_st, ks_sh, vscale, vs_sb, vs_st, vs_sh);
+  if (rc != MSA_OK) return rc;
+  if (N > MSA_TREE_MAX) return fail(MSA_ERR_INVALID, "a tree holds at most %d nodes, got %d", MSA_TREE_MAX, N);
+  if (B == 0 || N == 0) return ok();
+  if (N > cache_cap) return fail(MSA_ERR_INVALID, "the cache's %d positions do not hold %d nodes", cache_cap, N);
+  if (!(eps > 0.0f)) return fail(MSA_ERR_INVALID, "eps must be positive");
+  if (lengths == nullptr || (lengths_n != 1 && lengths_n != B))
+    return fail(MSA_ERR_INVALID, "lengths must be 1 or B=%d device int64", B);
+  if (par_sb < 0) return fail(MSA_ERR_INVALID, "parents stride must not be negative");
+  if ((rc = check_tensor("q", q, q_sb, q_sn, q_sh, dtype)) != MSA_OK) return rc;
+  if (r == nullptr || w == nullptr) return fail(MSA_ERR_INVALID, "r and w must be device arrays of H floats");
+  if ((rc = check_out("y", y)) != MSA_OK) return rc;
+  const size_t need = msa_tree_workspace_bytes(B, H, N, D, cache_cap, window_hint);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(MSA_ERR_WORKSPACE, "tree workspace holds %zu bytes, %zu needed", workspace_bytes, need);
+  if (need > 0 && !aligned16(workspace)) return fail(MSA_ERR_INVALID, "workspace is not 16-byte aligned");
+  msa::TreeCall c;
+  c.B = B; c.H = H; c.N = N; c.D = D; c.q_dtype = dtype; c.cache_dtype = cache_dtype; c.cap = cache_cap;
+  c.q = q; c.q_sb = q_sb; c.q_sn = q_sn; c.q_sh = q_sh;
+  c.kc = kcache; c.ks = {kc_sb, kc_st, kc_sh}; c.vc = vcache; c.vs = {vc_sb, vc_st, vc_sh};
+  c.kscale = kscale; c.kss = {ks_sb, ks_st, ks_sh}; c.vscale = vscale; c.vss = {vs_sb, vs_st, vs_sh};
+  c.lengths = lengths; c.len_step = lengths_n == 1 ? 0 : 1; c.parents = parents; c.par_sb = par_sb;
+  c.r = r; c.w = w; c.eps = eps; c.part = (float*)workspace; c.y = y;
+  c.blocks = tree_blocks_of(B, H, N, cache_cap, window_hint);
+  c.stream = (hipStream_t)stream;
+  return hip_status(msa::launch_tree(c), "msa_tree_decode launch");
 }
 
 int msa_selftest_mfma(const float* a16, const float* b16, float* out16, const float* a2, const float* b2,

@@ -121,6 +121,26 @@ struct CacheCall {
 };
 hipError_t launch_cache(const CacheCall& c);
 
+// Screening attention of a tree of N nodes per sequence over a cache.
+struct TreeCall {
+  int B, H, N, D, q_dtype, cache_dtype, cap;
+  const void* q; int64_t q_sb, q_sn, q_sh;
+  const void* kc; Strides3 ks;
+  const void* vc; Strides3 vs;
+  const float* kscale; Strides3 kss;  // 8-bit caches
+  const float* vscale; Strides3 vss;
+  const int64_t* lengths; int len_step;       // committed positions, one (step 0) or per sequence
+  const int64_t* parents; int64_t par_sb;     // parents of a sequence's nodes, or null: a chain
+  const float* r; const float* w; float eps;
+  float* part;  // [b*H + h][block][node][D] sums, where blocks > 1
+  void* y;
+  int blocks;   // blocks that share a head's keys
+  hipStream_t stream;
+};
+int tree_max_nodes();
+int tree_blocks(int B, int H, int N, int span);
+hipError_t launch_tree(const TreeCall& c);
+
 // Waves that share a row (32-query or 32-key unit) in the live, dq and dK/dV
 // passes: launches with few rows split each row's units, so that about 2048
 // waves (2-byte types) or 4096 (fp32, whose rows take several times as long)

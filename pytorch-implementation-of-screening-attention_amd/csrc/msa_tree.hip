@@ -1,0 +1,653 @@
+// Screening attention of a tree of drafted tokens over a key/value cache
+// (gfx950): N <= 64 nodes per sequence, over caches of the input type or of
+// 8-bit codes with a scale per row.  N = 1 is the decode of one token.
+//
+// Sequence b's cache holds its committed tokens at positions [0, n) and the
+// nodes' own rows at n, n + 1, ...; node i stands at position n + depth_i and
+// sees the committed keys of its window and, of the drafted rows, its own and
+// its ancestors':
+//   s = q^.k^,  a = max(1 - r(1 - s), 0),  m = (cos(pi d/w) + 1)/2 for 0 <= d < w
+//   y = TanhNorm(sum a^2 m v^)
+// There is no softmax, so partial sums over any split of the keys just add.
+//
+// One wave takes 32 nodes (the columns of a product) and walks 32-key units of
+// the window: S = K Q^T on the matrix cores, a vote on the threshold, and only
+// for a unit with a live pair the weights, V (through LDS, transposed on the
+// way out) and h^T += V^T P^T.  Every key row is thus read once for 32 nodes;
+// the nodes' operand and the sums stay in registers.
+//
+// Operands: rows of the input type enter as they are, 1/|x| multiplies the
+// fp32 results.  Codes enter as fp16, which holds every code of both types
+// exactly; the nodes' rows are scaled to fp16's range by a power of two (an
+// fp32 row as the sum of two fp16 rows, 22 bits).  Pair weights are rounded to
+// two terms of the operand's type (16 or 22 bits), in fp16 after a power of two
+// that keeps small weights clear of its subnormals.
+#include "msa_device.h"
+#include "msa_internal.h"
+
+namespace msa {
+
+constexpr int kTreeMax = 64;   // nodes of a tree: one lane each
+constexpr int kTreeWaves = 4;  // waves of a block
+// Fewest units of a block, so that a block's sums stay small beside its keys.
+constexpr int kTreeMinUnits = 8;
+
+// How a cache row of type C enters the products.
+template <typename C> struct TreeRow {
+  typedef C comp;  // operand type
+  static constexpr bool kCodes = false;
+};
+template <> struct TreeRow<int8_t> { typedef f16 comp; static constexpr bool kCodes = true; };
+template <> struct TreeRow<fp8> { typedef f16 comp; static constexpr bool kCodes = true; };
+
+// Power of two on the pair weights (fp16 operands only): a^2 m <= 1 times the
+// row factor, at most 2 for fp16 rows scaled to [1/2, 1), at most 1/64 for codes.
+template <typename C> constexpr float kWeightUp = 1.0f;
+template <> constexpr float kWeightUp<f16> = 16384.0f;
+template <> constexpr float kWeightUp<int8_t> = 2097152.0f;
+template <> constexpr float kWeightUp<fp8> = 2097152.0f;
+
+typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t u32x4;
+typedef __attribute__((__vector_size__(2 * sizeof(uint32_t)))) uint32_t u32x2;
+typedef __attribute__((__vector_size__(2 * sizeof(_Float16)))) _Float16 f16x2;
+
+// Four codes as fp16.  int8: the code + 128 in the low bits of 1024 is the
+// fp16 number 1152 + code; the subtraction is exact.
+__device__ inline void decode_f16(uint32_t c, int8_t, f16* o) {
+  const uint32_t u = c ^ 0x80808080u;
+  const f16x2 off = {(f16)1152.0f, (f16)1152.0f};
+  const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off;
+  const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off;
+  o[0] = a[0]; o[1] = a[1]; o[2] = b[0]; o[3] = b[1];
+}
+__device__ inline void decode_f16(uint32_t c, fp8, f16* o) {
+  const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false);
+  const auto b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+  o[0] = (f16)a[0]; o[1] = (f16)a[1]; o[2] = (f16)b[0]; o[3] = (f16)b[1];
+}
+template <typename C>
+__device__ inline f16x8 decode8(uint32_t c0, uint32_t c1) {
+  f16 o[8];
+  decode_f16(c0, C{}, o);
+  decode_f16(c1, C{}, o + 4);
+  f16x8 f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = o[e];
+  return f;
+}
+
+// Waits that keep a run's A/B fragments and its result's registers apart from
+// later writes (guard_run, for any number of fragments).
+template <typename F, int N>
+__device__ inline void guard_all(const F (&f)[N], const f32x16& c) {
+  if constexpr (__is_same(F, f32x4)) {
+    const int x = __builtin_amdgcn_readfirstlane(__float_as_int(c[15]));
+#pragma unroll
+    for (int k = 0; k < N; ++k) asm volatile("" ::"v"(f[k]), "s"(x));
+  } else {
+    asm volatile(MSA_NOP16 ::"v"(c[15]));
+#pragma unroll
+    for (int k = 0; k < N; ++k) asm volatile("" ::"v"(f[k]));
+  }
+}
+
+// The key operand of a unit: lane l holds row perm_row(l % 32), slots in the
+// column order col() below.
+template <typename C, int D>
+struct KeyRows {
+  using comp = typename TreeRow<C>::comp;
+  using M = Mma<comp>;
+  using frag = typename M::frag;
+  static constexpr bool kCodes = TreeRow<C>::kCodes;
+  static constexpr int NKS = D / M::KS;
+  static constexpr int LB = kCodes && D == 16 ? 8 : 16;            // bytes of a load
+  static constexpr int NL = D * (int)sizeof(C) / (2 * LB);         // loads of a lane
+  u32x4 raw[NL];
+  float scale;
+
+  // Column of slot e of fragment ks in a lane of half `half`.
+  __device__ static constexpr int col(int ks, int half) {
+    if constexpr (!kCodes) return M::KS * ks + M::PER * half;
+    else if constexpr (D == 16) return 8 * half;
+    else return 32 * (ks / 2) + 16 * half + 8 * (ks & 1);
+  }
+  __device__ inline void load(const char* row, const float* sc, int half) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const char* p = row + (2 * i + half) * LB;
+      if constexpr (LB == 8) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+        raw[i] = u32x4{x[0], x[1], 0u, 0u};
+      } else {
+        raw[i] = *reinterpret_cast<const u32x4*>(p);
+      }
+    }
+    if constexpr (kCodes) scale = *sc;
+  }
+  __device__ inline void frags(frag (&f)[NKS]) const {
+    if constexpr (!kCodes) {
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) f[ks] = __builtin_bit_cast(frag, raw[ks]);
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks)
+        f[ks] = decode8<C>(raw[D == 16 ? 0 : ks / 2][2 * (ks & 1)], raw[D == 16 ? 0 : ks / 2][2 * (ks & 1) + 1]);
+    }
+  }
+  // 1/max(|k|, eps) of the row, times the code's scale.  A row that is not
+  // finite gives 0 or NaN: its pairs are not live.
+  __device__ inline float factor(const frag (&f)[NKS], float eps) const {
+    if constexpr (__is_same(C, int8_t)) {
+      int ss = 0;
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+#pragma unroll
+        for (int e = 0; e < LB / 4; ++e) ss = __builtin_amdgcn_sdot4((int)raw[i][e], (int)raw[i][e], ss, false);
+      return code_factor(half_sum((float)ss), scale, eps);
+    } else if constexpr (kCodes) {
+      return code_factor(half_sum(row_dot<comp>(f, f)), scale, eps);
+    } else {
+      return inv_len_of<C>(half_sum(row_dot<comp>(f, f)), eps);
+    }
+  }
+  // min(1/|c|, scale/eps): the factor that takes a row of codes c with this
+  // scale to its unit row (0 for a row of zeros, NaN for one that is not finite).
+  __device__ static inline float code_factor(float ss, float scale, float eps) {
+    const float f = fminf(inv_len_of<float>(ss, 1e-30f), scale / eps);
+    return scale == scale ? f : scale;
+  }
+};
+
+// The nodes' operand: lane l holds node row l % 32 in the key rows' column
+// order; PARTS terms whose sum is the row (scaled for codes).
+template <typename C, int D, int PARTS>
+struct NodeRows {
+  using K = KeyRows<C, D>;
+  using frag = typename K::frag;
+  frag f[PARTS][K::NKS];
+  float inv;  // 1/max(|q|, eps), over the scaling
+  template <typename T>
+  __device__ inline void load(const T* row, bool ok, float eps, int half) {
+    constexpr int PER = K::M::PER;
+    float x[K::NKS][PER];
+    float ss = 0.0f, mx = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < K::NKS; ++ks)
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        x[ks][e] = ok ? to_f(row[K::col(ks, half) + e]) : 0.0f;
+        ss = fmaf(x[ks][e], x[ks][e], ss);
+        mx = fmaxf(mx, fabsf(x[ks][e]));
+      }
+    const float p = TreeRow<C>::kCodes ? row_pow2(half_max(mx)) : 1.0f;
+    inv = inv_len_of<float>(half_sum(ss), eps) / p;
+#pragma unroll
+    for (int ks = 0; ks < K::NKS; ++ks)
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        float rest = x[ks][e] * p;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+          const auto part = from_f<typename K::comp>(rest);
+          f[i][ks][e] = part;
+          rest -= to_f(part);
+        }
+      }
+  }
+};
+
+// V of a unit on its way to LDS: coalesced 16-byte loads (a row's CPR lanes are
+// neighbours), then the operand rows in UnitTile's layout and each row's factor.
+template <typename C, int D>
+struct ValueRows {
+  using comp = typename TreeRow<C>::comp;
+  static constexpr bool kCodes = TreeRow<C>::kCodes;
+  static constexpr int DP = D < 32 ? 32 : D;
+  using Tile = UnitTile<comp, DP>;
+  static constexpr int CPR = D * (int)sizeof(C) / 16;
+  static constexpr int NV = (kUnit * CPR + 63) / 64;
+  u32x4 raw[NV];
+  float scale[kCodes ? NV : 1];
+
+  __device__ static inline int row_of(int i, int lane) { return ((i * 64 + lane) / CPR) & (kUnit - 1); }
+  // `row(r)`: address of unit row r; `sc(r)`: of its scale.
+  template <typename RowFn, typename ScaleFn>
+  __device__ inline void load(RowFn row, ScaleFn sc, int lane) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int r = row_of(i, lane);
+      raw[i] = *reinterpret_cast<const u32x4*>(row(r) + 16 * (lane % CPR));
+      if constexpr (kCodes) scale[i] = *sc(r);
+    }
+  }
+  // A row that is not finite is staged as zeros; its factor is NaN, so that a
+  // live pair still sees it and a masked one does not.  (A finite row whose
+  // length overflows has factor 0.)
+  __device__ inline void stage(char* tile, float* fac, float eps, int lane) const {
+    typedef typename Mma<comp>::frag vec;  // 16 bytes of an operand row
+    constexpr int N = 16 / (int)sizeof(comp);
+    constexpr int W = kCodes ? 2 : 1;      // operand chunks of a load
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      vec x[W];
+      if constexpr (kCodes) {
+        x[0] = decode8<C>(raw[i][0], raw[i][1]);
+        x[W - 1] = decode8<C>(raw[i][2], raw[i][3]);
+      } else {
+        x[0] = __builtin_bit_cast(vec, raw[i]);
+      }
+      float ss = 0.0f;
+#pragma unroll
+      for (int u = 0; u < W; ++u) {
+        if constexpr (sizeof(comp) == 2) ss = frag_dot(x[u], x[u], ss);
+        else
+#pragma unroll
+          for (int e = 0; e < N; ++e) ss = fmaf(x[u][e], x[u][e], ss);
+      }
+      ss = group_sum<CPR>(ss);
+      const bool finite = ss < INFINITY;
+      float f;
+      if constexpr (kCodes) f = KeyRows<C, D>::code_factor(ss, scale[i], eps);
+      else f = inv_len_of<C>(ss, eps);
+      if (__ballot(!finite) != 0ull) {
+        float bad = 0.0f;  // an element that is not finite, and not only their squares' sum
+#pragma unroll
+        for (int u = 0; u < W; ++u)
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+            if (!(fabsf(to_f(x[u][e])) < INFINITY)) bad = 1.0f;
+        bad = group_sum<CPR>(bad);
+        if (!finite) {
+          f = bad > 0.0f ? __uint_as_float(0x7fc00000u) : 0.0f;
+#pragma unroll
+          for (int u = 0; u < W; ++u) x[u] = Mma<comp>::zero();
+        }
+      }
+      if constexpr (kCodes) {
+        // cache_write's rows reach the type's largest code, so |codes| >= 127 and the
+        // factor is at most 1/127; rows of smaller codes (an e4m3 code is 2^-9 at
+        // least) are scaled up to a length of 64
+        const bool small = ss < 16129.0f;
+        if (__ballot(small) != 0ull && small) {
+          const float up = ss > 0.0f ? Pow2Split::recip(__uint_as_float(__float_as_uint(sqrtf(ss)) & 0x7f800000u)) * 64.0f : 1.0f;
+#pragma unroll
+          for (int u = 0; u < W; ++u)
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[u][e] *= (f16)up;
+          f = ss > 0.0f ? f / up : 0.0f;
+        }
+      }
+      if constexpr (__is_same(C, f16)) {  // |v| to [1/2, 1) by a power of two, the rest in the factor
+        if (finite) {
+          const Pow2Split sp(f);
+#pragma unroll
+          for (int e = 0; e < N; ++e) x[0][e] = (f16)(to_f(x[0][e]) * sp.c1 * sp.c2);
+          f = sp.w;
+        }
+      }
+      const int r = row_of(i, lane), ch = W * (lane % CPR);
+      const bool mine = kUnit * CPR >= 64 || lane < kUnit * CPR;
+      if (mine) {
+#pragma unroll
+        for (int u = 0; u < W; ++u)
+          *reinterpret_cast<vec*>(tile + r * Tile::ROWB + (((ch + u) ^ Tile::swz(r)) << 4)) = x[u];
+        if (lane % CPR == 0) fac[r] = f;
+      }
+    }
+  }
+};
+
+// Where a C block's registers (rows = tcol-ordered columns) go: groups of
+// consecutive columns of one row.
+template <typename COMP, typename OUT, int D, typename Fn>
+__device__ inline void store_row(OUT* row, int half, Fn fn) {
+  constexpr int NDH = (D + 31) / 32;
+  if constexpr (sizeof(COMP) == 2) {
+#pragma unroll
+    for (int dblk = 0; dblk < NDH; ++dblk)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int d0 = 32 * dblk + 16 * g + 8 * half;
+        if (d0 < D) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = fn(dblk, 8 * g + e);
+          store8(row + d0, v);
+        }
+      }
+  } else {
+#pragma unroll
+    for (int dblk = 0; dblk < NDH; ++dblk)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d0 = 32 * dblk + 8 * g + 4 * half;
+        if (d0 < D) store4(row + d0, fn(dblk, 4 * g), fn(dblk, 4 * g + 1), fn(dblk, 4 * g + 2), fn(dblk, 4 * g + 3));
+      }
+  }
+}
+template <typename COMP, int D, typename Fn>
+__device__ inline void store_row_as(void* y, int64_t off, int dtype, int half, Fn fn) {
+  if (dtype == 1) store_row<COMP, bf16, D>((bf16*)y + off, half, fn);
+  else if (dtype == 2) store_row<COMP, f16, D>((f16*)y + off, half, fn);
+  else store_row<COMP, float, D>((float*)y + off, half, fn);
+}
+
+// What a wave knows of the tree: each lane's node, its depth and the bitmap of
+// the nodes on its way up (itself among them).  A parent that is no earlier
+// node makes the node a root.
+struct Tree {
+  int depth;
+  unsigned long long above;
+  __device__ Tree(const int64_t* parents, int N, int lane) {
+    if (parents == nullptr) {  // a chain
+      depth = lane;
+      above = ~0ull >> (63 - lane);
+      return;
+    }
+    int64_t p64 = lane < N ? parents[lane] : -1;
+    int p = p64 >= 0 && p64 < lane ? (int)p64 : -1;
+    above = 1ull << lane;
+    depth = p >= 0 ? 1 : 0;
+    // each step doubles the way that `above` covers: p is the first node past it
+#pragma unroll
+    for (int k = 0; k < 6; ++k) {
+      const int at = p < 0 ? lane : p;
+      const unsigned long long up =
+          ((unsigned long long)(uint32_t)__shfl((int)(above >> 32), at) << 32) | (uint32_t)__shfl((int)above, at);
+      const int d = __shfl(depth, at), q = __shfl(p, at);
+      if (p >= 0) {
+        above |= up;
+        depth += d;
+        p = q;
+      }
+    }
+  }
+};
+
+// Committed length of sequence b, and head h's key units: keys lo, lo + 1, ...,
+// n + N - 1 in units of 32 (none for an empty window).
+struct TreeSpan {
+  int n, lo, units;
+  __device__ TreeSpan(const TreeCall& a, int b, const HeadParams& hp) {
+    int64_t x = a.lengths[(int64_t)b * a.len_step];
+    x = x > a.cap - a.N ? a.cap - a.N : x;
+    n = x < 0 ? 0 : (int)x;
+    lo = n - hp.wc + 1;
+    lo = lo < 0 ? 0 : lo;
+    units = hp.wc == 0 ? 0 : (n + a.N - lo + kUnit - 1) / kUnit;
+  }
+  // Units of each of the at most `blocks` blocks that share them.
+  __device__ int per(int blocks) const {
+    const int p = (units + blocks - 1) / blocks;
+    return p < kTreeMinUnits ? kTreeMinUnits : p;
+  }
+};
+
+// Block (x, y): units [x per, (x + 1) per) of head y.  Waves w and w + WPT, ...
+// of a node tile take every WPT-th unit.
+template <typename C, int D, int PARTS>
+__global__ __launch_bounds__(256) void tree_kernel(TreeCall a) {
+  using K = KeyRows<C, D>;
+  using V = ValueRows<C, D>;
+  using comp = typename K::comp;
+  using frag = typename K::frag;
+  using M = Mma<comp>;
+  using Tile = typename V::Tile;
+  constexpr int NDH = Tile::NDH, NC = Tile::NC;
+  constexpr bool kTwo = sizeof(comp) == 2;  // weights as two terms
+  constexpr int kRed = kUnit * V::DP * 4;   // a wave's sums
+  constexpr int kLds = kTreeWaves * Tile::BYTES > 2 * kRed ? kTreeWaves * Tile::BYTES : 2 * kRed;
+  __shared__ __align__(16) char lds[kLds];
+  __shared__ __align__(16) float kfac[kTreeWaves][kUnit], vfac[kTreeWaves][kUnit], mtab[kTreeWaves][128];
+  __shared__ int dtab[kTreeWaves][kTreeMax];
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
+  const int b = blockIdx.y / a.H, h = blockIdx.y % a.H;
+  const int tiles = (a.N + 31) / 32, wpt = kTreeWaves / tiles, tile = wave / wpt, kw = wave % wpt;
+  const HeadParams hp = head_params(a.r, a.w, h, true);
+  const TreeSpan sp(a, b, hp);
+  const int per = sp.per(gridDim.x);
+  const int u0 = blockIdx.x * per, u1 = u0 + per < sp.units ? u0 + per : sp.units;
+  if (gridDim.x > 1 && u0 >= sp.units) return;
+
+  const Tree tree(a.parents == nullptr ? nullptr : a.parents + b * a.par_sb, a.N, lane);
+  dtab[wave][lane] = tree.depth;
+  const int node = 32 * tile + l32;
+  const int depth = __shfl(tree.depth, node);
+  const unsigned long long above =
+      ((unsigned long long)(uint32_t)__shfl((int)(tree.above >> 32), node) << 32) | (uint32_t)__shfl((int)tree.above, node);
+
+  NodeRows<C, D, PARTS> q;
+  {
+    const bool ok = node < a.N;
+    const int64_t off = b * a.q_sb + (int64_t)(ok ? node : 0) * a.q_sn + h * a.q_sh;
+    if (a.q_dtype == 1) q.load((const bf16*)a.q + off, ok, a.eps, half);
+    else if (a.q_dtype == 2) q.load((const f16*)a.q + off, ok, a.eps, half);
+    else q.load((const float*)a.q + off, ok, a.eps, half);
+  }
+
+  const char* kb = (const char*)a.kc + (b * a.ks.sb + h * a.ks.sh) * (int64_t)sizeof(C);
+  const char* vb = (const char*)a.vc + (b * a.vs.sb + h * a.vs.sh) * (int64_t)sizeof(C);
+  const int64_t kst = a.ks.st * (int64_t)sizeof(C), vst = a.vs.st * (int64_t)sizeof(C);
+  const float* ksc = a.kscale + b * a.kss.sb + h * a.kss.sh;
+  const float* vsc = a.vscale + b * a.vss.sb + h * a.vss.sh;
+  const int last = sp.n + a.N - 1;  // last key row
+
+  char* vt = lds + wave * Tile::BYTES;
+  if constexpr (D < V::DP) {  // the columns past D
+#pragma unroll
+    for (int i = 0; i < Tile::BYTES / 1024; ++i)
+      *reinterpret_cast<u32x4*>(vt + i * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+  }
+  const uint32_t cbase = Tile::col_base(lane);
+  f32x16 acc[NDH];
+#pragma unroll
+  for (int d = 0; d < NDH; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
+
+  for (int u = u0 + kw; u < u1; u += wpt) {
+    const int k0 = sp.lo + u * kUnit;  // position of the unit's first row (a drafted row: n + its node)
+    K key;
+    {
+      const int j = k0 + perm_row(l32) < last ? k0 + perm_row(l32) : last;
+      key.load(kb + j * kst, ksc + j * a.kss.st, half);
+    }
+    frag kf[K::NKS];
+    key.frags(kf);
+    const float f = key.factor(kf, a.eps);
+    if (half == 0) kfac[wave][perm_row(l32)] = f;
+    f32x16 s = unit_product<comp, K::NKS>(kf, q.f[0]);
+    if constexpr (PARTS == 2) {
+      const f32x16 s2 = unit_product<comp, K::NKS>(kf, q.f[1]);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] += s2[r];
+    }
+    guard_all(kf, s);
+    wave_lds_sync();
+    float x[16];
+    read_row_scales(kfac[wave], half, x);
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] *= x[r];
+      top = fmaxf(top, s[r]);
+    }
+    if (__ballot(top * q.inv > hp.thr) == 0ull) continue;
+
+    // a^2 m of every pair: register r is key row 16 (r/8) + 8 half + r%8
+    bool live = false;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = 16 * (r >> 3) + 8 * half + (r & 7), j = k0 + row - sp.n;  // j >= 0: drafted
+      const bool draft = j >= 0;
+      const int dd = depth - (draft ? dtab[wave][j & (kTreeMax - 1)] : j);
+      const bool seen = draft ? j < a.N && ((above >> j) & 1ull) != 0ull : true;
+      const float av = fmaxf(fmaf(-hp.r, fmaf(-s[r], q.inv, 1.0f), 1.0f), 0.0f);
+      const bool on = seen && in_window(dd, hp) && av > 0.0f && node < a.N;
+      s[r] = on ? av * av * mask_fast(dd, hp.w, hp.iw) : 0.0f;
+      live = live || s[r] > 0.0f;
+    }
+    if (__ballot(live) == 0ull) continue;
+
+    V val;
+    val.load([&](int r) { return vb + (int64_t)(k0 + r < last ? k0 + r : last) * vst; },
+             [&](int r) { return vsc + (int64_t)(k0 + r < last ? k0 + r : last) * a.vss.st; }, lane);
+    val.stage(vt, vfac[wave], a.eps, lane);
+    wave_lds_sync();
+    read_row_scales(vfac[wave], half, x);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = s[r] > 0.0f ? s[r] * x[r] * kWeightUp<C> : 0.0f;
+    frag hi[NC], lo[kTwo ? NC : 1];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      hi[c] = M::pack(s, M::PER * c);
+      if constexpr (kTwo) {
+#pragma unroll
+        for (int e = 0; e < M::PER; ++e) s[M::PER * c + e] -= M::get(hi[c], e);
+        lo[c] = M::pack(s, M::PER * c);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < NDH; ++d) {
+      frag vf[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) vf[c] = Tile::col_frag(vt, cbase, d, c);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        acc[d] = M::mma_ng(vf[c], hi[c], acc[d]);
+        if constexpr (kTwo) acc[d] = M::mma_ng(vf[c], lo[c], acc[d]);
+      }
+      guard_all(vf, acc[d]);
+    }
+    guard_all(hi, acc[NDH - 1]);
+    guard_all(lo, acc[NDH - 1]);
+  }
+
+  // the waves of a tile: w += w + 2 (one tile), then w += w + 1
+  __syncthreads();
+  char* red = lds + (tiles == 1 ? wave & 1 : tile) * kRed;
+  auto put = [&] {
+#pragma unroll
+    for (int d = 0; d < NDH; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(red + (4 * d + g) * 1024 + lane * 16) =
+            f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+  };
+  auto add = [&] {
+#pragma unroll
+    for (int d = 0; d < NDH; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(red + (4 * d + g) * 1024 + lane * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[d][4 * g + e] += x[e];
+      }
+  };
+  if (tiles == 1) {
+    if (wave >= 2) put();
+    __syncthreads();
+    if (wave < 2) add();
+    __syncthreads();
+    red = lds;
+  }
+  if (kw == 1) put();
+  __syncthreads();
+  if (kw != 0) return;
+  add();
+  if (node >= a.N) return;  // lanes l and l + 32 share a node
+  constexpr float down = 1.0f / kWeightUp<C>;
+  if (gridDim.x > 1) {
+    float* p = a.part + ((int64_t)(blockIdx.y * gridDim.x + blockIdx.x) * a.N + node) * D;
+    store_row<comp, float, D>(p, half, [&](int d, int r) { return acc[d][r] * down; });
+    return;
+  }
+  float ss = 0.0f;
+#pragma unroll
+  for (int d = 0; d < NDH; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      acc[d][r] *= down;
+      ss = fmaf(acc[d][r], acc[d][r], ss);
+    }
+  const float nc = fmaxf(sqrtf(half_sum(ss)), a.eps), fy = tanhf(nc) / nc;
+  store_row_as<comp, D>(a.y, (((int64_t)b * a.N + node) * a.H + h) * D, a.q_dtype, half,
+                        [&](int d, int r) { return acc[d][r] * fy; });
+}
+
+// Sum of a node's block sums, in block order, and TanhNorm.  Block per (node,
+// b, h).
+template <int D>
+__global__ __launch_bounds__(256) void tree_reduce_kernel(TreeCall a, int blocks) {
+  constexpr int G = 256 / D;
+  __shared__ float red[256];
+  __shared__ float sq[D];
+  const int node = blockIdx.x, b = blockIdx.y / a.H, h = blockIdx.y % a.H;
+  const int t = threadIdx.x, d = t % D, g = t / D;
+  const HeadParams hp = head_params(a.r, a.w, h, true);
+  const TreeSpan sp(a, b, hp);
+  const int per = sp.per(blocks), used = (sp.units + per - 1) / per;
+  const float* p = a.part + ((int64_t)blockIdx.y * blocks * a.N + node) * D + d;
+  float x = 0.0f;
+#pragma unroll 4
+  for (int c = g; c < used; c += G) x += p[(int64_t)c * a.N * D];
+  red[t] = x;
+  __syncthreads();
+  x = 0.0f;
+  if (t < D) {
+#pragma unroll
+    for (int k = 0; k < G; ++k) x += red[k * D + t];
+    sq[t] = x * x;
+  }
+  __syncthreads();
+  for (int s = D / 2; s > 0; s >>= 1) {
+    if (t < s) sq[t] += sq[t + s];
+    __syncthreads();
+  }
+  const float nc = fmaxf(sqrtf(sq[0]), a.eps), fy = tanhf(nc) / nc;
+  if (t >= D) return;
+  const int64_t at = (((int64_t)b * a.N + node) * a.H + h) * D + t;
+  if (a.q_dtype == 1) ((bf16*)a.y)[at] = (bf16)(x * fy);
+  else if (a.q_dtype == 2) ((f16*)a.y)[at] = (f16)(x * fy);
+  else ((float*)a.y)[at] = x * fy;
+}
+
+int tree_max_nodes() { return kTreeMax; }
+// Blocks that share a head's units: about four per CU in all, each with at
+// least kTreeMinUnits of the longest window's.
+int tree_blocks(int B, int H, int N, int span) {
+  const int64_t units = ((int64_t)span + N + kUnit - 1) / kUnit;
+  int64_t most = (units + kTreeMinUnits - 1) / kTreeMinUnits;
+  const int64_t want = (1024 + (int64_t)B * H - 1) / ((int64_t)B * H);
+  most = most < want ? most : want;
+  return (int)(most < 1 ? 1 : most);
+}
+
+template <typename C, int D, int PARTS>
+static hipError_t launch_tree_t(const TreeCall& c) {
+  hipLaunchKernelGGL((tree_kernel<C, D, PARTS>), dim3((unsigned)c.blocks, (unsigned)(c.B * c.H)), dim3(256), 0, c.stream, c);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || c.blocks == 1) return e;
+  hipLaunchKernelGGL((tree_reduce_kernel<D>), dim3((unsigned)c.N, (unsigned)(c.B * c.H)), dim3(256), 0, c.stream, c, c.blocks);
+  return hipGetLastError();
+}
+template <typename C, int PARTS>
+static hipError_t launch_tree_d(const TreeCall& c) {
+  switch (c.D) {
+    case 16: return launch_tree_t<C, 16, PARTS>(c);
+    case 32: return launch_tree_t<C, 32, PARTS>(c);
+    case 64: return launch_tree_t<C, 64, PARTS>(c);
+    default: return launch_tree_t<C, 128, PARTS>(c);
+  }
+}
+hipError_t launch_tree(const TreeCall& c) {
+  // an fp32 query over codes is two fp16 rows
+  if (c.cache_dtype == kInt8) return c.q_dtype == 0 ? launch_tree_d<int8_t, 2>(c) : launch_tree_d<int8_t, 1>(c);
+  if (c.cache_dtype == kFp8) return c.q_dtype == 0 ? launch_tree_d<fp8, 2>(c) : launch_tree_d<fp8, 1>(c);
+  if (c.cache_dtype == 1) return launch_tree_d<bf16, 1>(c);
+  if (c.cache_dtype == 2) return launch_tree_d<f16, 1>(c);
+  return launch_tree_d<float, 1>(c);
+}
+
+}  // namespace msa

@@ -16,6 +16,8 @@ MSA_F16 = 2
 MSA_I8 = 3   # cache rows only
 MSA_FP8 = 4  # cache rows only (OCP e4m3)
 
+TREE_MAX = 64  # MSA_TREE_MAX: nodes of a tree
+
 # kernel ids for msa_timer_arm (include/msa.h)
 K_PREP_K, K_FWD_SCREEN, K_FWD_LIVE, K_DKDV, K_DQ, K_DECODE = 1, 2, 3, 4, 5, 7
 
@@ -54,6 +56,10 @@ _SIGS = {
                              _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p]),
     "msa_cache_read": (_i, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i,
                             _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i, _i, _i, _i, _p, _i, _i64, _p, _p, _p]),
+    "msa_tree_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "msa_tree_decode": (_i, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i,
+                             _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i, _i, _i, _i,
+                             _p, _i, _p, _i64, _i, _p, _p, _f, _p, _p, _sz, _p]),
     "msa_timer_arm": (_i, [_i, _i]),
     "msa_timer_arm_every": (_i, [_i, _i, _i]),
     "msa_timer_read": (_i, [_i, ctypes.POINTER(ctypes.c_float), _i]),

@@ -378,3 +378,63 @@ def cache_read(kcache, vcache, kscale, vscale, start, length, dtype):
                               ptr, n, host, k.data_ptr(), v.data_ptr(), _stream_ptr(dev))
     _native.check(rc, "msa_cache_read")
     return k, v
+
+
+def _parents_arg(parents, B, N):
+    """(pointer or None, stride over sequences, tensor to keep) of parents (N,) or (B, N), or None: a chain."""
+    if parents is None:
+        return None, 0, None
+    parents = _index(parents, "parents", (N,), (B, N))
+    return parents.data_ptr(), N if parents.dim() == 2 else 0, parents
+
+
+def tree_decode(q, kcache, vcache, lengths, parents, r, w, eps=1e-8, kscale=None, vscale=None, workspace=None,
+                window_hint=0):
+    """Screening attention of a tree of N <= 64 drafted tokens per sequence
+    over a cache (N = 1: of one new token).
+
+    q (B, N, H, D) raw query projections.  kcache, vcache (B, cap, H, D), with
+    kscale, vscale (B, cap, H) where they hold codes (as cache_write leaves
+    them): sequence b's committed rows at positions [0, n_b), its nodes' own
+    rows at n_b .. n_b + N - 1.  lengths: int64 CUDA tensor of 1 or B elements,
+    the n_b (clamped to [0, cap - N]).
+    parents: int64 (N,) or (B, N), parents[i] < i the node that node i
+    continues, any other value for a root; None for a chain.  Node i stands at
+    position n_b + depth_i and sees the committed keys of its window, itself
+    and its ancestors.
+    window_hint: 0, or a bound on ceil(w) over the heads (sizes the launch).
+    Returns y (B, N, H, D) = TanhNorm(h), in q's dtype; no gradient.
+    """
+    L = _native.lib()
+    dev = _check_gpu("tree_decode", q=q, kcache=kcache, vcache=vcache, kscale=kscale, vscale=vscale, lengths=lengths,
+                     parents=parents, workspace=workspace)
+    if q.dtype not in _DTYPES:
+        raise TypeError(f"tree_decode: q must be float32, bfloat16 or float16, got {q.dtype}")
+    q = _as_bthd(q, "q", q.element_size())
+    B, N, H, D = q.shape
+    if N > _native.TREE_MAX:
+        raise ValueError(f"tree_decode: a tree holds at most {_native.TREE_MAX} nodes, got {N}")
+    codes, scales = _cache_args("tree_decode", kcache, vcache, kscale, vscale, q.dtype)
+    if (kcache.shape[0], *kcache.shape[2:]) != (B, H, D):
+        raise ValueError(f"tree_decode: cache {tuple(kcache.shape)} does not match q {tuple(q.shape)}")
+    cap = int(kcache.shape[1])
+    if N > cap:
+        raise IndexError(f"KV cache capacity {cap} is below {N} nodes")
+    if r.shape != (H,) or w.shape != (H,):
+        raise ValueError(f"r and w must have shape ({H},)")
+    lengths = _index(lengths, "lengths", (1,), (B,))
+    par, par_sb, parents = _parents_arg(parents, B, N)
+    r32 = r.detach().to(device=dev, dtype=torch.float32).contiguous()
+    w32 = w.detach().to(device=dev, dtype=torch.float32).contiguous()
+    hint = max(0, int(window_hint))
+    y = torch.empty((B, N, H, D), dtype=q.dtype, device=dev)
+    need = int(L.msa_tree_workspace_bytes(B, H, N, D, cap, hint))
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty((need,), dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = L.msa_tree_decode(*_args_bthd(q), *codes, cap, _CACHE_DTYPES[kcache.dtype], *scales, B, N, H, D,
+                               _DTYPES[q.dtype], lengths.data_ptr(), lengths.numel(), par, par_sb, hint,
+                               r32.data_ptr(), w32.data_ptr(), float(eps), y.data_ptr(),
+                               workspace.data_ptr() if need else None, need, _stream_ptr(dev))
+    _native.check(rc, "msa_tree_decode")
+    return y
