@@ -305,6 +305,43 @@ int msa_tree_decode(const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh,
                     const float* r, const float* w, float eps,
                     void* y, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Verification of drafted tokens.  No counterpart in the reference.  Sequence
+ * b's tree has M <= MSA_TREE_MAX nodes; node 0 is its last committed token.
+ *   target   : (B, M, V) of type dtype, strides (t_sb, t_sn), unit stride over
+ *              V: row i is the target's distribution after node i.
+ *              Probabilities, or any scores where uniforms is null.
+ *   tokens   : device int64 (B, M) contiguous, the nodes' tokens (tokens[b, 0]
+ *              is not read).  A token outside [0, V) is never accepted.
+ *   parents  : device int64, node i >= 1 continues node parents[b * par_sb + i]
+ *              in [0, i), any other value: the node is never reached; null: a
+ *              chain.
+ *   uniforms : device fp32 (B, M) contiguous in [0, 1); null: greedy.
+ *   draft    : null, or probabilities (B, M - 1, V) of type dtype, strides
+ *              (d_sb, d_sn): row i is the distribution that token i + 1 was
+ *              drawn from.  Drafts are then a chain: a node whose parent is not
+ *              the node before it is never reached.  Needs uniforms.
+ * From node 0 the walk goes on to the first child in index order that is
+ * accepted: child i with token x of a node with row p
+ *   greedy : x is p's largest entry (the first of equal ones, NaN the largest)
+ *   draft  : u_i q(x) < p(x)
+ *   else   : u_i (1 - sum p of the siblings before it) < p(x), equal tokens
+ *            counted once and accepted at the first of them only
+ * in 64-bit arithmetic.  Outputs, device int64: path (B, M) the nodes walked,
+ * node 0 first, -1 behind them; count (B) their number (>= 1); token (B) the
+ * token after the last of them: greedy: its row's largest entry; else the
+ * first v with weight and cumulated weight > u_0 * total, the weights (negative
+ * and NaN entries count as 0) p without the refused children's tokens, max(p -
+ * q, 0) where a draft was refused, p itself behind a chain's last node or
+ * where no weight is left (token 0 if p has none).
+ * workspace: msa_verify_workspace_bytes (greedy; 0 with uniforms).
+ */
+size_t msa_verify_workspace_bytes(int B, int M, int64_t V, int greedy);
+int msa_verify(const void* target, int64_t t_sb, int64_t t_sn, const void* draft, int64_t d_sb, int64_t d_sn,
+               const int64_t* tokens, const int64_t* parents, int64_t par_sb, const float* uniforms,
+               int B, int M, int64_t V, int dtype, int64_t* path, int64_t* count, int64_t* token,
+               void* workspace, size_t workspace_bytes, void* stream);
+
 /* Kernel timing for measurement.  After msa_timer_arm(kernel, n) the next n
  * launches of that kernel (any entry point) each record a HIP event pair on
  * their stream around the launch; several kernels can be armed at once.

@@ -576,6 +576,44 @@ int msa_tree_decode(const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh, con
   return hip_status(msa::launch_tree(c), "msa_tree_decode launch");
 }
 
+size_t msa_verify_workspace_bytes(int B, int M, int64_t V, int greedy) {
+  if (!greedy || B <= 0 || M <= 0 || M > MSA_TREE_MAX || V <= 0 || V > 0x7fffffff) return 0;
+  return (size_t)B * M * msa::verify_parts(B, M, (int)V) * sizeof(unsigned long long);
+}
+
+int msa_verify(const void* target, int64_t t_sb, int64_t t_sn, const void* draft, int64_t d_sb, int64_t d_sn,
+               const int64_t* tokens, const int64_t* parents, int64_t par_sb, const float* uniforms, int B, int M,
+               int64_t V, int dtype, int64_t* path, int64_t* count, int64_t* token, void* workspace,
+               size_t workspace_bytes, void* stream) {
+  if (dtype != MSA_F32 && dtype != MSA_BF16 && dtype != MSA_F16)
+    return fail(MSA_ERR_INVALID, "dtype must be MSA_F32, MSA_BF16 or MSA_F16");
+  if (B < 0 || B > (1 << 24) || M < 1 || M > MSA_TREE_MAX)
+    return fail(MSA_ERR_INVALID, "a tree holds 1 to %d nodes and a batch at most 2^24 sequences, got M=%d, B=%d",
+                MSA_TREE_MAX, M, B);
+  if (V < 1 || V > 0x7fffffff) return fail(MSA_ERR_INVALID, "the vocabulary must hold 1 to 2^31 - 1 tokens");
+  if (draft != nullptr && uniforms == nullptr) return fail(MSA_ERR_INVALID, "draft probabilities need uniforms");
+  if (B == 0) return ok();
+  const uintptr_t es = dtype == MSA_F32 ? 4 : 2;
+  if (target == nullptr || tokens == nullptr) return fail(MSA_ERR_INVALID, "target or tokens is null");
+  if ((uintptr_t)target % es != 0 || (uintptr_t)draft % es != 0)
+    return fail(MSA_ERR_INVALID, "target and draft must be aligned to their type");
+  if (t_sb < 0 || t_sn < 0 || d_sb < 0 || d_sn < 0 || par_sb < 0)
+    return fail(MSA_ERR_INVALID, "strides must not be negative");
+  if (path == nullptr || count == nullptr || token == nullptr)
+    return fail(MSA_ERR_INVALID, "path, count or token is null");
+  const size_t need = msa_verify_workspace_bytes(B, M, V, uniforms == nullptr);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(MSA_ERR_WORKSPACE, "verify workspace holds %zu bytes, %zu needed", workspace_bytes, need);
+  if (need > 0 && !aligned16(workspace)) return fail(MSA_ERR_INVALID, "workspace is not 16-byte aligned");
+  msa::VerifyCall c;
+  c.B = B; c.M = M; c.V = V; c.dtype = dtype;
+  c.target = target; c.t_sb = t_sb; c.t_sn = t_sn; c.draft = draft; c.d_sb = d_sb; c.d_sn = d_sn;
+  c.tokens = tokens; c.parents = parents; c.par_sb = par_sb; c.uniforms = uniforms;
+  c.path = path; c.count = count; c.token = token; c.best = (unsigned long long*)workspace;
+  c.stream = (hipStream_t)stream;
+  return hip_status(msa::launch_verify(c), "msa_verify launch");
+}
+
 int msa_selftest_mfma(const float* a16, const float* b16, float* out16, const float* a2, const float* b2,
                       float* out2, void* stream) {
   if (!a16 || !b16 || !out16 || !a2 || !b2 || !out2) return fail(MSA_ERR_INVALID, "null pointer");

@@ -141,6 +141,22 @@ int tree_max_nodes();
 int tree_blocks(int B, int H, int N, int span);
 hipError_t launch_tree(const TreeCall& c);
 
+// Drafted tokens against the target's rows.
+struct VerifyCall {
+  int B, M, dtype;
+  int64_t V;
+  const void* target; int64_t t_sb, t_sn;  // (B, M, V)
+  const void* draft; int64_t d_sb, d_sn;   // (B, M - 1, V), or null
+  const int64_t* tokens;                   // (B, M)
+  const int64_t* parents; int64_t par_sb;  // or null: a chain
+  const float* uniforms;                   // (B, M), or null: greedy
+  int64_t* path; int64_t* count; int64_t* token;
+  unsigned long long* best;                // greedy: [b*M + i][part] keys
+  hipStream_t stream;
+};
+int verify_parts(int B, int M, int V);
+hipError_t launch_verify(const VerifyCall& c);
+
 // Waves that share a row (32-query or 32-key unit) in the live, dq and dK/dV
 // passes: launches with few rows split each row's units, so that about 2048
 // waves (2-byte types) or 4096 (fp32, whose rows take several times as long)

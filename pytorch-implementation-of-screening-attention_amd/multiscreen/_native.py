@@ -60,6 +60,8 @@ _SIGS = {
     "msa_tree_decode": (_i, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i,
                              _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i, _i, _i, _i,
                              _p, _i, _p, _i64, _i, _p, _p, _f, _p, _p, _sz, _p]),
+    "msa_verify_workspace_bytes": (_sz, [_i, _i, _i64, _i]),
+    "msa_verify": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _i, _i, _i64, _i, _p, _p, _p, _p, _sz, _p]),
     "msa_timer_arm": (_i, [_i, _i]),
     "msa_timer_arm_every": (_i, [_i, _i, _i]),
     "msa_timer_read": (_i, [_i, ctypes.POINTER(ctypes.c_float), _i]),

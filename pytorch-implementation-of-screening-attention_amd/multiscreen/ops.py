@@ -438,3 +438,64 @@ def tree_decode(q, kcache, vcache, lengths, parents, r, w, eps=1e-8, kscale=None
                                workspace.data_ptr() if need else None, need, _stream_ptr(dev))
     _native.check(rc, "msa_tree_decode")
     return y
+
+
+def verify_drafts(target, tokens, parents=None, uniforms=None, draft=None):
+    """Which drafted tokens the target model accepts, and its next token.
+
+    A tree of M <= 64 nodes per sequence; node 0 is the last committed token,
+    node i >= 1 continues node parents[i] in [0, i) (any other value: it is never
+    reached).  parents int64 (M,) or (B, M), or None for a chain; tokens int64
+    (B, M).
+    target (B, M, V) float32, bfloat16 or float16: row i is the target's
+    distribution after node i: probabilities, or any scores where uniforms is
+    None.
+    uniforms float32 (B, M) in [0, 1), or None for greedy decoding.
+    draft (B, M - 1, V) probabilities in target's dtype, or None: row i is what
+    token i + 1 was drawn from; the drafts are then a chain.
+
+    From node 0 the walk goes on to the first child, in index order, that is
+    accepted: with `draft` if u_i q(x) < p(x), without if u_i (1 - the p of the
+    siblings refused before it) < p(x), greedily if x is the row's largest entry.
+    Behind the last node the next token is drawn with u_0 from what is left of p
+    (max(p - q, 0), or p without the refused tokens), so that the tokens are
+    distributed as the target's own samples.  Sums are in 64 bits.
+    Returns int64 path (B, M), the nodes walked, node 0 first, -1 behind them;
+    count (B), how many; token (B), the next token.  The count[b] rows path[b]
+    are what cache_write takes as `rows` and `count`.
+    """
+    L = _native.lib()
+    dev = _check_gpu("verify_drafts", target=target, tokens=tokens, parents=parents, uniforms=uniforms, draft=draft)
+    if target.dim() != 3 or target.dtype not in _DTYPES:
+        raise TypeError(f"verify_drafts: target must be (B, M, V) float32, bfloat16 or float16, got {target.dtype} "
+                        f"{tuple(target.shape)}")
+    B, M, V = target.shape
+    if not 1 <= M <= _native.TREE_MAX:
+        raise ValueError(f"verify_drafts: a tree holds 1 to {_native.TREE_MAX} nodes, got {M}")
+    tokens = _index(tokens, "tokens", (B, M))
+    par, par_sb, parents = _parents_arg(parents, B, M)
+    if uniforms is not None:
+        if uniforms.dtype != torch.float32 or uniforms.shape != (B, M):
+            raise ValueError(f"uniforms must be float32 ({B}, {M}), got {uniforms.dtype} {tuple(uniforms.shape)}")
+        uniforms = uniforms.contiguous()
+    if draft is not None:
+        if uniforms is None:
+            raise ValueError("verify_drafts: draft probabilities need uniforms")
+        if draft.dtype != target.dtype or draft.shape != (B, M - 1, V):
+            raise ValueError(f"draft must be {target.dtype} ({B}, {M - 1}, {V}), got {draft.dtype} {tuple(draft.shape)}")
+        draft = draft if draft.stride(2) == 1 else draft.contiguous()
+    target = target if target.stride(2) == 1 else target.contiguous()
+    path = torch.empty((B, M), dtype=torch.int64, device=dev)
+    count, token = torch.empty((2, B), dtype=torch.int64, device=dev)
+    need = int(L.msa_verify_workspace_bytes(B, M, V, int(uniforms is None)))
+    workspace = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    with _on(dev):
+        # a chain of one node has no draft rows: nothing can be refused
+        rc = L.msa_verify(target.data_ptr(), target.stride(0), target.stride(1),
+                          draft.data_ptr() if draft is not None and M > 1 else None,
+                          *(draft.stride()[:2] if draft is not None else (0, 0)), tokens.data_ptr(), par, par_sb,
+                          uniforms.data_ptr() if uniforms is not None else None, B, M, V, _DTYPES[target.dtype],
+                          path.data_ptr(), count.data_ptr(), token.data_ptr(),
+                          workspace.data_ptr() if need else None, need, _stream_ptr(dev))
+    _native.check(rc, "msa_verify")
+    return path, count, token
