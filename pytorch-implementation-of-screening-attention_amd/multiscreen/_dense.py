@@ -45,3 +45,113 @@ def screening_core_dense(q, k, v, r, w, causal=True, eps=1e-8, key_padding_mask=
     n = torch.linalg.vector_norm(h, dim=-1, keepdim=True).clamp(min=eps)
     y = h * (torch.tanh(n) / n)
     return y.transpose(1, 2)                                  # (B,Tq,H,D)
+
+
+# ---------------------------------------------------------------------------
+# Serving on the host: the forms of ops.cache_write, ops.tree_decode and
+# ops.verify_drafts that CPU tensors take.
+# ---------------------------------------------------------------------------
+CODE_TOP = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+
+
+def quantise_rows(x, dtype):
+    """(codes, float32 scales) of rows x (..., D): the codes nearest to TOP x / max|x|,
+    ties to the even code; decided in float64."""
+    top = x.double().abs().amax(-1, keepdim=True)
+    some = torch.isfinite(top) & (top > 0)
+    t = torch.where(some, CODE_TOP[dtype] * x.double() / torch.where(some, top, 1.0), 0.0)
+    if dtype == torch.int8:
+        t = t.round()
+    else:  # 4 significant bits, spaced 2^-9 below 2^-6
+        step = torch.exp2(torch.frexp(t).exponent.double() - 4).clamp(min=2.0 ** -9)
+        t = (t / step).round() * step
+    scale = torch.where(torch.isfinite(top), top.float() / CODE_TOP[dtype], math.nan)
+    return t.float().to(dtype), scale.squeeze(-1)
+
+
+def tree_relations(parents):
+    """(above, depth) of parents (B, M): above[b, i, j], whether node j is node i or one
+    of its ancestors, and the nodes' depths.  A parent outside [0, i) makes a root."""
+    B, M = parents.shape
+    at = torch.arange(M, device=parents.device)
+    up = torch.where((parents >= 0) & (parents < at), parents, -1)
+    above = torch.eye(M, dtype=torch.bool, device=parents.device).expand(B, M, M)
+    step = 1
+    while step < M:  # `up` is the first node that `above` does not cover yet
+        on = (up >= 0).unsqueeze(-1)
+        to = up.clamp(min=0)
+        above = above | (on & above.gather(1, to.unsqueeze(-1).expand(B, M, M)))
+        up = torch.where(up >= 0, up.gather(1, to), -1)
+        step *= 2
+    return above, above.sum(-1) - 1
+
+
+def tree_dense(q, k, v, lengths, parents, r, w, eps=1e-8):
+    """Screening of a tree of drafted rows: q (B, M, H, D) over values k, v (B, cap, H, D) of
+    a cache that holds sequence b's committed rows below lengths[b] and its nodes' rows from there on."""
+    B, M, H, D = q.shape
+    cap = k.shape[1]
+    n = lengths.clamp(0, cap - M).view(-1, 1).expand(B, 1)
+    above, depth = tree_relations(parents)
+    j = torch.arange(cap).expand(B, cap)
+    node = (j - n).clamp(0, M - 1)
+    drafted = (j >= n) & (j < n + M)
+    kpos = torch.where(drafted, n + depth.gather(1, node), j)
+    dist = ((n + depth).unsqueeze(-1) - kpos.unsqueeze(1)).unsqueeze(1).float()          # (B, 1, M, cap)
+    seen = torch.where(drafted.unsqueeze(1), above.gather(2, node.unsqueeze(1).expand(B, M, cap)), (j < n).unsqueeze(1))
+    wh = w.float().view(1, H, 1, 1)
+    m = torch.where(seen.unsqueeze(1) & (dist >= 0) & (dist < wh), 0.5 * (torch.cos(math.pi * dist / wh) + 1.0), 0.0)
+    qn, kn, vn = (F.normalize(x.transpose(1, 2).float(), dim=-1, eps=eps) for x in (q, k, v))
+    a = torch.relu(1.0 - r.float().view(1, H, 1, 1) * (1.0 - qn @ kn.transpose(-2, -1)))
+    p = torch.where(m > 0, a * a * m, 0.0)
+    h = p @ torch.where((p > 0).any(2, keepdim=True).transpose(2, 3), vn, 0.0)
+    size = torch.linalg.vector_norm(h, dim=-1, keepdim=True).clamp(min=eps)
+    return (h * (torch.tanh(size) / size)).transpose(1, 2).to(q.dtype)
+
+
+def verify_dense(target, tokens, parents=None, uniforms=None, draft=None):
+    """ops.verify_drafts on the host, sequence by sequence."""
+    B, M, V = target.shape
+    path, count, token = torch.full((B, M), -1), torch.ones(B, dtype=torch.int64), torch.zeros(B, dtype=torch.int64)
+    for b in range(B):
+        up = list(range(-1, M - 1)) if parents is None else (parents[b] if parents.dim() == 2 else parents).tolist()
+        node, length = 0, 0
+        while True:
+            path[b, length] = node
+            length += 1
+            row = target[b, node].double()
+            row = row if uniforms is None else row.nan_to_num(0.0).clamp(min=0.0)
+            best = int((row == row.amax()).nonzero()[0]) if uniforms is None else -1
+            rest, left, refused, taken = row.clone(), 1.0, False, -1
+            for c in range(max(1, node + 1), M):
+                x = int(tokens[b, c])
+                if up[c] != node or not 0 <= x < V or (draft is not None and c != node + 1):
+                    continue
+                if uniforms is None:
+                    hit = x == best
+                elif draft is not None:
+                    hit = float(uniforms[b, c]) * float(draft[b, node, x]) < float(row[x])
+                else:
+                    hit = float(uniforms[b, c]) * left < float(rest[x])
+                if hit:
+                    taken = c
+                    break
+                refused = True
+                if draft is None and uniforms is not None:
+                    left -= float(rest[x])
+                    rest[x] = 0.0
+            if taken < 0:
+                break
+            node = taken
+        count[b] = length
+        if uniforms is None:
+            token[b] = best
+            continue
+        if draft is not None and node < M - 1:
+            rest = (row - draft[b, node].double()).clamp(min=0.0)
+        rest = rest if float(rest.sum()) > 0 else row
+        below = rest.cumsum(0)
+        over = ((below > float(uniforms[b, 0]) * float(below[-1])) & (rest > 0)).nonzero()
+        some = (rest > 0).nonzero()
+        token[b] = int(over[0]) if len(over) else int(some[-1]) if len(some) else 0
+    return path, count, token

@@ -27,7 +27,7 @@ import torch.nn.functional as F
 
 from .norm import TanhNorm
 from . import ops
-from ._dense import screening_core_dense
+from ._dense import CODE_TOP, quantise_rows, screening_core_dense, tree_dense
 
 
 class ScreeningAttention(nn.Module):
@@ -167,6 +167,12 @@ class ScreeningAttention(nn.Module):
         if not self.causal:
             raise RuntimeError("KV-cache decode is defined for causal self-attention only")
         B = x.shape[0]
+        if cache.k_scale is not None:  # 8-bit rows: a tree of one node
+            if not torch.is_tensor(pos):
+                if pos + 1 > cache.k.shape[1]:
+                    raise IndexError(f"KV cache capacity {cache.k.shape[1]} exceeded at position {pos + 1}")
+                pos = torch.full((1,), pos, dtype=torch.int64, device=x.device)
+            return self.tree_step(x, cache, pos, None, rw)[0]
         q, k, v = self.project_qkv(x, x, x)
         r, w = rw if rw is not None else (self.sharpness(), self.window())
         if torch.is_tensor(pos):
@@ -185,6 +191,29 @@ class ScreeningAttention(nn.Module):
             y = screening_core_dense(q, kc, vc, r, w, True, self.eps, q_offset=pos)[:, 0]
         return self.out_proj(y.reshape(B, 1, self.d_model))
 
+    def tree_step(self, x: torch.Tensor, cache, lengths: torch.Tensor, parents=None, rw=None):
+        """x (B, M, d): the M <= 64 nodes of a tree of drafted tokens that follows sequence b's
+        lengths[b] cached positions (lengths int64, 1 or B elements; parents as in
+        ops.tree_decode, None for a chain).  Writes the nodes' k and v behind the committed rows and
+        returns the attention output (B, M, d), node i seeing the sequence and its own ancestors,
+        and (k, v), from which KVCache.store_rows keeps an accepted path."""
+        if not self.causal:
+            raise RuntimeError("KV-cache decode is defined for causal self-attention only")
+        B, M, _ = x.shape
+        q, k, v = self.project_qkv(x, x, x)
+        if cache.k_scale is None:
+            q, k, v = (t.to(cache.k.dtype) for t in (q, k, v))
+        cache.store_rows(k, v, lengths)
+        r, w = rw if rw is not None else (self.sharpness(), self.window())
+        if x.is_cuda:
+            y = ops.tree_decode(q, cache.k, cache.v, lengths, parents, r, w, self.eps, cache.k_scale, cache.v_scale,
+                                None, cache.window_hint)
+        else:
+            up = torch.arange(-1, M - 1) if parents is None else parents
+            kc, vc = cache.read(0, cache.k.shape[1], q.dtype)
+            y = tree_dense(q, kc, vc, lengths, up.expand(B, M), r, w, self.eps)
+        return self.out_proj(y.to(x.dtype).reshape(B, M, self.d_model)), (k, v)
+
 
 class KVCache:
     """Raw k/v projections of one attention layer.
@@ -192,7 +221,12 @@ class KVCache:
     Stored head-major, (B, H, capacity, D), so that one head's window is one
     contiguous stream for the decode kernel; `k` and `v` are the (B, capacity,
     H, D) views of that storage, the layout of the projections, in the model's
-    dtype (float32, bfloat16 or float16)."""
+    dtype (float32, bfloat16 or float16).
+
+    With dtype torch.int8 or torch.float8_e4m3fn the cache holds 8-bit codes and
+    `k_scale`, `v_scale` (B, capacity, H) a float32 scale per row, as
+    ops.cache_write leaves them: a half or a quarter of the bytes to keep and
+    to read per token."""
 
     def __init__(self, batch, capacity, num_heads, head_dim, dtype, device, window_hint=0):
         # 0, or a bound on ceil(w) over the layer's heads: sizes the decode
@@ -202,8 +236,12 @@ class KVCache:
         self._v = torch.zeros_like(self._k)
         self.k = self._k.permute(0, 2, 1, 3)
         self.v = self._v.permute(0, 2, 1, 3)
+        self.k_scale = self.v_scale = None
+        if dtype in CODE_TOP:
+            self.k_scale, self.v_scale = (torch.zeros((batch, num_heads, capacity), device=device).transpose(1, 2)
+                                          for _ in range(2))
         self.workspace = None
-        if self.k.is_cuda:
+        if self.k.is_cuda and self.k_scale is None:
             from . import _native
             nbytes = int(_native.lib().msa_decode_workspace_bytes(batch, num_heads, head_dim, capacity))
             self.workspace = torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=device)
@@ -212,11 +250,56 @@ class KVCache:
         T = k.shape[1]
         if pos + T > self.k.shape[1]:
             raise IndexError(f"KV cache capacity {self.k.shape[1]} exceeded at position {pos + T}")
+        if self.k_scale is not None:
+            if self.k.is_cuda:
+                ops.cache_write(k, v, self.k, self.v, pos, self.k_scale, self.v_scale)
+            else:
+                self.store_rows(k, v, torch.tensor([pos]))
+            return
         self.k[:, pos:pos + T] = k.to(self.k.dtype)
         self.v[:, pos:pos + T] = v.to(self.v.dtype)
 
     def store_at(self, k, v, pos):
         """k, v (B,1,H,D) at the position held by the device int64 tensor pos
         (one element).  The caller keeps pos below the capacity."""
+        if self.k_scale is not None:
+            self.store_rows(k, v, pos)
+            return
         self._k.index_copy_(2, pos, k.permute(0, 2, 1, 3).to(self._k.dtype))
         self._v.index_copy_(2, pos, v.permute(0, 2, 1, 3).to(self._v.dtype))
+
+    def store_rows(self, k, v, start, rows=None, count=None):
+        """k, v (B, T, H, D) at positions start[b], start[b] + 1, ... (start int64, 1 or B
+        elements); with rows (B, T') and count (B), row rows[b, t] of k and v at start[b] + t for t <
+        count[b] (an accepted path of ops.verify_drafts).  Positions outside the cache are not
+        written."""
+        if self.k_scale is None:
+            k, v = k.to(self.k.dtype), v.to(self.v.dtype)
+        if self.k.is_cuda:
+            ops.cache_write(k, v, self.k, self.v, start, self.k_scale, self.v_scale, rows, count)
+            return
+        B, T = k.shape[:2] if rows is None else rows.shape
+        src = torch.arange(T).expand(B, T) if rows is None else rows
+        at = start.view(-1, 1) + torch.arange(T).expand(B, T)
+        keep = (at >= 0) & (at < self.k.shape[1]) & (src >= 0) & (src < k.shape[1])
+        if count is not None:
+            keep &= torch.arange(T) < count.view(-1, 1)
+        b, t = keep.nonzero(as_tuple=True)
+        for x, c, s in ((k, self.k, self.k_scale), (v, self.v, self.v_scale)):
+            x = x[b, src[b, t]]
+            if s is not None:
+                x, s[b, at[b, t]] = quantise_rows(x, c.dtype)
+                x, c = x.view(torch.uint8), c.view(torch.uint8)
+            c[b, at[b, t]] = x
+
+    def read(self, start, length, dtype):
+        """Rows start .. start + length - 1 as (k, v) of `dtype`, (B, length, H, D)."""
+        if self.k_scale is not None and self.k.is_cuda:
+            return ops.cache_read(self.k, self.v, self.k_scale, self.v_scale, start, length, dtype)
+        if not 0 <= start <= start + length <= self.k.shape[1]:
+            raise IndexError(f"positions {start} .. {start + length} are outside the KV cache's capacity {self.k.shape[1]}")
+        part = slice(start, start + length)
+        if self.k_scale is None:
+            return self.k[:, part].to(dtype), self.v[:, part].to(dtype)
+        return tuple((c[:, part].float() * s[:, part].unsqueeze(-1)).to(dtype)
+                     for c, s in ((self.k, self.k_scale), (self.v, self.v_scale)))

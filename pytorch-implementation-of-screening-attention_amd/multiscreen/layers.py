@@ -9,8 +9,8 @@ so state_dicts are interchangeable:
         x = x + self_attn(norm1(x));  x = x + cross_attn(norm2(x), memory)
         x = x + ffn(norm3(x))
 
-MultiscreenBlock additionally exposes prefill/decode steps over a KV cache,
-used by MultiscreenLM.generate.
+MultiscreenBlock additionally exposes prefill, decode and tree steps over a KV
+cache, used by MultiscreenLM.generate and generate_speculative.
 """
 
 import torch
@@ -56,6 +56,13 @@ class MultiscreenBlock(nn.Module):
         normed = self.norm1(x)
         x = x + self.attn.decode(normed, cache, pos, rw)
         return x + self.ffn(self.norm2(x))
+
+    def tree_step(self, x: torch.Tensor, cache, lengths, parents=None, rw=None):
+        """The nodes x (B, M, d) of a tree of drafted tokens (ScreeningAttention.tree_step); returns
+        their outputs and the layer's (k, v)."""
+        y, kv = self.attn.tree_step(self.norm1(x), cache, lengths, parents, rw)
+        x = x + y
+        return x + self.ffn(self.norm2(x)), kv
 
 
 class MultiscreenDecoderLayer(nn.Module):

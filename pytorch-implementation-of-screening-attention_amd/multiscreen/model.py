@@ -11,6 +11,11 @@ generate() differs only in cost: instead of re-running forward() over the
 whole prefix for every new token, it prefills a per-layer KV cache once and
 then runs one single-query decode step per token (the HIP decode kernel on
 GPU), which computes the same last-position logits.
+
+Beyond the reference: caches of 8-bit rows (cache_dtype=torch.int8 or
+torch.float8_e4m3fn), steps over several tokens or a tree of drafts at once
+(tree_step, accept) and generation with a smaller model that drafts
+(generate_speculative).
 """
 
 import math
@@ -19,6 +24,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import ops
+from ._dense import tree_relations, verify_dense
 from .attention import KVCache
 from .layers import MultiscreenBlock
 
@@ -83,7 +90,8 @@ class MultiscreenLM(nn.Module):
     def new_cache(self, batch: int, capacity: int, dtype: torch.dtype, device) -> list:
         """One KVCache per block.  Each carries its layer's widest window
         (ceil(max_h w_h), read once here) so that decode launches only the
-        blocks the windows need."""
+        blocks the windows need.  dtype torch.int8 or torch.float8_e4m3fn: 8-bit
+        rows with a scale each (KVCache)."""
         caches = []
         for block in self.blocks:
             attn = block.attn
@@ -116,18 +124,126 @@ class MultiscreenLM(nn.Module):
         return self._head(x)[:, 0]
 
     @torch.no_grad()
-    def generate_greedy(self, input_ids: torch.Tensor, max_new_tokens: int = 100) -> torch.Tensor:
+    def tree_step(self, tokens: torch.Tensor, caches: list, lengths: torch.Tensor, parents=None, rws=None):
+        """One step over a tree of M <= 64 tokens per sequence: tokens (B, M), node 0 the last
+        committed token at position lengths[b] (int64, 1 or B elements), the others drafted
+        continuations (parents as in ops.tree_decode; None: a chain).  Writes the nodes' rows into
+        the caches from position lengths[b] on.  Positions past the last position embedding take
+        the last one.
+        Returns the logits (B, M, vocab) and per layer (k, v), for accept()."""
+        B, M = tokens.shape
+        if parents is None:
+            depth = torch.arange(M, device=tokens.device)
+        else:
+            parents = parents.expand(B, M)
+            depth = tree_relations(parents)[1]
+        pos = (lengths.view(-1, 1) + depth).clamp(max=self.pos_emb.num_embeddings - 1)
+        x = self.emb_dropout(self.token_emb(tokens) + self.pos_emb(pos))
+        kvs = []
+        for i, (block, cache) in enumerate(zip(self.blocks, caches)):
+            x, kv = block.tree_step(x, cache, lengths, parents, None if rws is None else rws[i])
+            kvs.append(kv)
+        return self._head(x), kvs
+
+    @torch.no_grad()
+    def accept(self, caches: list, kvs: list, path: torch.Tensor, count: torch.Tensor, lengths: torch.Tensor):
+        """Keeps an accepted path of a tree_step (path, count of ops.verify_drafts): its rows move
+        to positions lengths[b], lengths[b] + 1, ... of every layer's cache.  Returns lengths + count.
+        (A chain's path is where it belongs already: lengths + count is all it needs.)"""
+        for cache, (k, v) in zip(caches, kvs):
+            cache.store_rows(k, v, lengths, path, count)
+        return lengths + count
+
+    @torch.no_grad()
+    def generate_speculative(self, input_ids: torch.Tensor, draft: "MultiscreenLM", max_new_tokens: int = 100,
+                             num_drafts: int = 4, temperature: float = 1.0, top_k: int | None = None,
+                             cache_dtype: torch.dtype | None = None) -> torch.Tensor:
+        """generate() with `draft`, a smaller model of the same vocabulary: it drafts num_drafts tokens
+        one by one, this model scores them in one step (tree_step), and ops.verify_drafts keeps those
+        that leave the tokens distributed as generate()'s own.  temperature 0 is greedy: the tokens
+        of generate_greedy, up to the rounding of logits that nearly tie.
+
+        cache_dtype: as in generate().  Returns (B, T + max_new_tokens) token ids.
+        """
+        self.eval()
+        draft.eval()
+        B, T = input_ids.shape
+        if not 1 <= num_drafts <= 63:
+            raise ValueError(f"num_drafts must be in 1 .. 63, got {num_drafts}")
+        if max_new_tokens <= 0:
+            return input_ids
+        end = T + max_new_tokens
+        for m in (self, draft):
+            if end > m.pos_emb.num_embeddings:
+                raise IndexError(f"{end} positions exceed the model's {m.pos_emb.num_embeddings}")
+        if draft.lm_head.out_features != self.lm_head.out_features:
+            raise ValueError("the draft model's vocabulary differs")
+        dev = input_ids.device
+        # room for the drafts behind the last position of a sequence that is done
+        both = [(m, m.new_cache(B, end + num_drafts + 1, m._cache_dtype(dev, cache_dtype), dev)) for m in (self, draft)]
+        logits = [m.prefill(input_ids, caches) for m, caches in both][0]
+        out = torch.cat((input_ids, input_ids.new_zeros(B, max_new_tokens + num_drafts + 1)), 1)
+        lengths = torch.full((B,), T, dtype=torch.int64, device=dev)
+        token = self._pick(_probabilities(logits, temperature, top_k))
+        out[:, T] = token.squeeze(1)
+        at = torch.arange(num_drafts + 1, device=dev)
+        verify = ops.verify_drafts if input_ids.is_cuda else verify_dense
+        for _ in range(max_new_tokens - 1):
+            # the draft's rows of the last two tokens (it has not seen the last accepted one), then on from there
+            nodes, probs = [token], []
+            step = torch.cat((out.gather(1, lengths.unsqueeze(1) - 1), token), 1)
+            for i in range(num_drafts):
+                logits, _ = draft.tree_step(step, both[1][1], lengths - 1 if i == 0 else lengths + i)
+                probs.append(_probabilities(logits[:, -1], temperature, top_k))
+                step = self._pick(probs[-1])
+                nodes.append(step)
+            nodes = torch.cat(nodes, 1)
+            logits, _ = self.tree_step(nodes, both[0][1], lengths)
+            if temperature == 0:
+                _, count, token = verify(logits, nodes)
+            else:
+                _, count, token = verify(_probabilities(logits, temperature, top_k), nodes, None,
+                                         torch.rand(B, num_drafts + 1, device=dev), torch.stack(probs, 1))
+            # the accepted drafts and the token after them; a sequence that is done stays at its last position
+            count = torch.where(lengths + 1 < end, count, 0)
+            place = lengths.unsqueeze(1) + at
+            out.scatter_(1, place, torch.where(at < count.unsqueeze(1), nodes, out.gather(1, place)))
+            place = (lengths + count).unsqueeze(1)
+            out.scatter_(1, place, torch.where(count.unsqueeze(1) > 0, token.unsqueeze(1), out.gather(1, place)))
+            lengths = (lengths + count).clamp(max=end - 1)
+            token = out.gather(1, lengths.unsqueeze(1))
+            if int(lengths.min()) + 1 >= end:
+                break
+        return out[:, :end]
+
+    @staticmethod
+    def _pick(probs: torch.Tensor) -> torch.Tensor:
+        """A token (B, 1) of what _probabilities gives for one row per sequence."""
+        return torch.multinomial(probs, num_samples=1) if probs.dtype.is_floating_point else probs
+
+    def _cache_dtype(self, device, cache_dtype=None) -> torch.dtype:
+        """The type generate() keeps its rows in: cache_dtype, else the model's (autocast's under it)."""
+        if cache_dtype is not None:
+            return cache_dtype
+        if device.type == "cuda" and torch.is_autocast_enabled("cuda"):
+            return torch.get_autocast_dtype("cuda")
+        return self.blocks[0].attn.q_proj.weight.dtype
+
+    @torch.no_grad()
+    def generate_greedy(self, input_ids: torch.Tensor, max_new_tokens: int = 100,
+                        cache_dtype: torch.dtype | None = None) -> torch.Tensor:
         """Greedy decoding (the argmax token; among equal logits the first).
 
         On GPU the per-token decode step runs as one replayed HIP graph
         (GraphDecoder); on CPU it is the eager loop.  Returns
         (B, T + max_new_tokens) token ids.  generate(top_k=1) samples the same
-        distribution but breaks exact ties at random, as the reference does."""
+        distribution but breaks exact ties at random, as the reference does.
+        cache_dtype: as in generate()."""
         self.eval()
         B, T = input_ids.shape
         if max_new_tokens <= 0:
             return input_ids
-        dtype = self.blocks[0].attn.q_proj.weight.dtype
+        dtype = cache_dtype or self.blocks[0].attn.q_proj.weight.dtype
         caches = self.new_cache(B, T + max_new_tokens, dtype, input_ids.device)
         logits = self.prefill(input_ids, caches)
         first = logits.argmax(-1, keepdim=True)
@@ -144,19 +260,18 @@ class MultiscreenLM(nn.Module):
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int = 100, temperature: float = 1.0,
-                 top_k: int | None = None) -> torch.Tensor:
+                 top_k: int | None = None, cache_dtype: torch.dtype | None = None) -> torch.Tensor:
         """Temperature / top-k sampling (top_k=1 is greedy).
 
+        cache_dtype: type of the cached rows; None: the model's own; torch.int8 or
+        torch.float8_e4m3fn: 8-bit codes (KVCache).
         Returns (B, T + max_new_tokens) token ids.
         """
         self.eval()
         B, T = input_ids.shape
         if max_new_tokens <= 0:
             return input_ids
-        dtype = self.blocks[0].attn.q_proj.weight.dtype
-        if input_ids.is_cuda and torch.is_autocast_enabled("cuda"):
-            dtype = torch.get_autocast_dtype("cuda")
-        caches = self.new_cache(B, T + max_new_tokens, dtype, input_ids.device)
+        caches = self.new_cache(B, T + max_new_tokens, self._cache_dtype(input_ids.device, cache_dtype), input_ids.device)
         logits = self.prefill(input_ids, caches)
         out = [input_ids]
         pos = T
@@ -172,6 +287,18 @@ class MultiscreenLM(nn.Module):
                 logits = self.decode_step(next_token, caches, pos)
                 pos += 1
         return torch.cat(out, dim=1)
+
+
+def _probabilities(logits, temperature, top_k):
+    """Sampling probabilities (float32) of logits (..., vocab) as generate() forms them; at temperature 0
+    the first largest entry's index (..., 1)."""
+    if temperature == 0:
+        return logits.argmax(-1, keepdim=True)
+    logits = logits / temperature
+    if top_k is not None:
+        values, _ = torch.topk(logits, top_k)
+        logits = logits.masked_fill(logits < values[..., -1:], float("-inf"))
+    return F.softmax(logits.float(), dim=-1)
 
 
 class GraphDecoder:
