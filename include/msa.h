@@ -286,14 +286,15 @@ int msa_cache_read(const void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_
  * and its ancestors' within the window.  y (B, N, H, D) contiguous, of type
  * dtype.  A key row that is not finite is never live; a value row that is not
  * finite makes the nodes that a live pair brings it to NaN, and no others.
- * window_hint as in msa_decode: it sizes the launch.  How a head's keys are
- * split over blocks (the sums' order, so y's rounding) depends on it and on
- * the shapes only: equal calls give bitwise equal y.
+ * window_hint as in msa_decode: it sizes the launch.  How the keys are split
+ * over blocks (the sums' order, so y's rounding) depends on it, the shapes, the
+ * length and the windows: equal calls give bitwise equal y.
  * workspace: msa_tree_workspace_bytes of the same sizes (0 where one block
  * takes a head's keys), scratch of this call.
  */
 #define MSA_TREE_MAX 64
-size_t msa_tree_workspace_bytes(int B, int H, int N, int D, int cache_cap, int window_hint);
+size_t msa_tree_workspace_bytes(int B, int H, int N, int D, int dtype, int cache_dtype, int cache_cap,
+                                int window_hint);
 int msa_tree_decode(const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh,
                     const void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_sh,
                     const void* vcache, int64_t vc_sb, int64_t vc_st, int64_t vc_sh,

@@ -528,16 +528,18 @@ int msa_cache_read(const void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_
   return hip_status(msa::launch_cache(c), "msa_cache_read launch");
 }
 
-static int tree_blocks_of(int B, int H, int N, int cache_cap, int window_hint) {
-  return msa::tree_blocks(B, H, N, window_hint > 0 && window_hint < cache_cap ? window_hint : cache_cap);
+static int tree_blocks_of(int B, int H, int N, int D, int dtype, int cache_dtype, int cache_cap, int window_hint) {
+  return msa::tree_blocks(B, H, N, D, dtype, cache_dtype,
+                          window_hint > 0 && window_hint < cache_cap ? window_hint : cache_cap);
 }
 
-size_t msa_tree_workspace_bytes(int B, int H, int N, int D, int cache_cap, int window_hint) {
+size_t msa_tree_workspace_bytes(int B, int H, int N, int D, int dtype, int cache_dtype, int cache_cap,
+                                int window_hint) {
   if (B <= 0 || H <= 0 || N <= 0 || N > MSA_TREE_MAX || cache_cap <= 0 || cache_cap > kMaxT || (int64_t)B * H > 65535 ||
       !(D == 16 || D == 32 || D == 64 || D == 128))
     return 0;
-  const int blocks = tree_blocks_of(B, H, N, cache_cap, window_hint);
-  return blocks == 1 ? 0 : (size_t)B * H * blocks * N * D * sizeof(float);
+  const int blocks = tree_blocks_of(B, H, N, D, dtype, cache_dtype, cache_cap, window_hint);
+  return blocks == H ? 0 : (size_t)B * blocks * N * D * sizeof(float);
 }
 
 int msa_tree_decode(const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const void* kcache, int64_t kc_sb,
@@ -553,6 +555,8 @@ int msa_tree_decode(const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh, con
   if (N > MSA_TREE_MAX) return fail(MSA_ERR_INVALID, "a tree holds at most %d nodes, got %d", MSA_TREE_MAX, N);
   if (B == 0 || N == 0) return ok();
   if (N > cache_cap) return fail(MSA_ERR_INVALID, "the cache's %d positions do not hold %d nodes", cache_cap, N);
+  if ((int64_t)H * cache_cap > (int64_t)1 << 35)  // a sequence's key units are counted in 32 bits
+    return fail(MSA_ERR_INVALID, "H * cache_cap = %lld exceeds 2^35", (long long)H * cache_cap);
   if (!(eps > 0.0f)) return fail(MSA_ERR_INVALID, "eps must be positive");
   if (lengths == nullptr || (lengths_n != 1 && lengths_n != B))
     return fail(MSA_ERR_INVALID, "lengths must be 1 or B=%d device int64", B);
@@ -560,7 +564,7 @@ int msa_tree_decode(const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh, con
   if ((rc = check_tensor("q", q, q_sb, q_sn, q_sh, dtype)) != MSA_OK) return rc;
   if (r == nullptr || w == nullptr) return fail(MSA_ERR_INVALID, "r and w must be device arrays of H floats");
   if ((rc = check_out("y", y)) != MSA_OK) return rc;
-  const size_t need = msa_tree_workspace_bytes(B, H, N, D, cache_cap, window_hint);
+  const size_t need = msa_tree_workspace_bytes(B, H, N, D, dtype, cache_dtype, cache_cap, window_hint);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(MSA_ERR_WORKSPACE, "tree workspace holds %zu bytes, %zu needed", workspace_bytes, need);
   if (need > 0 && !aligned16(workspace)) return fail(MSA_ERR_INVALID, "workspace is not 16-byte aligned");
@@ -571,7 +575,7 @@ int msa_tree_decode(const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh, con
   c.kscale = kscale; c.kss = {ks_sb, ks_st, ks_sh}; c.vscale = vscale; c.vss = {vs_sb, vs_st, vs_sh};
   c.lengths = lengths; c.len_step = lengths_n == 1 ? 0 : 1; c.parents = parents; c.par_sb = par_sb;
   c.r = r; c.w = w; c.eps = eps; c.part = (float*)workspace; c.y = y;
-  c.blocks = tree_blocks_of(B, H, N, cache_cap, window_hint);
+  c.blocks = tree_blocks_of(B, H, N, D, dtype, cache_dtype, cache_cap, window_hint);
   c.stream = (hipStream_t)stream;
   return hip_status(msa::launch_tree(c), "msa_tree_decode launch");
 }

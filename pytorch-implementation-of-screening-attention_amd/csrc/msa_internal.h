@@ -132,13 +132,13 @@ struct TreeCall {
   const int64_t* lengths; int len_step;       // committed positions, one (step 0) or per sequence
   const int64_t* parents; int64_t par_sb;     // parents of a sequence's nodes, or null: a chain
   const float* r; const float* w; float eps;
-  float* part;  // [b*H + h][block][node][D] sums, where blocks > 1
+  float* part;  // [b][block][node][D] sums, where blocks != H
   void* y;
-  int blocks;   // blocks that share a head's keys
+  int blocks;   // blocks that share a sequence's keys; H: a block per head
   hipStream_t stream;
 };
 int tree_max_nodes();
-int tree_blocks(int B, int H, int N, int span);
+int tree_blocks(int B, int H, int N, int D, int q_dtype, int cache_dtype, int span);
 hipError_t launch_tree(const TreeCall& c);
 
 // Drafted tokens against the target's rows.

@@ -28,9 +28,27 @@
 namespace msa {
 
 constexpr int kTreeMax = 64;   // nodes of a tree: one lane each
-constexpr int kTreeWaves = 4;  // waves of a block
+#ifndef WAVES
+#define WAVES 4
+#endif
+constexpr int kTreeWaves = WAVES;  // waves of a block
 // Fewest units of a block, so that a block's sums stay small beside its keys.
-constexpr int kTreeMinUnits = 8;
+// Fewest units of a block, so that a block's sums stay small beside its keys;
+// a head of at most kTreeSmall units is one block's (no sums to join).
+constexpr int kTreeMinUnits = 8, kTreeSmall = 16;
+
+// Waves per SIMD that the kernel's registers are budgeted for.
+#ifndef O64
+#define O64 3
+#define O128 2
+#define O256 2
+#endif
+#ifndef AHEAD
+#define AHEAD 64
+#endif
+constexpr int tree_occupancy(int D, int row_bytes, int parts) {
+  return row_bytes * parts <= 64 ? O64 : (row_bytes <= 128 && D < 128 ? O128 : row_bytes <= 256 ? O256 : 1);
+}
 
 // How a cache row of type C enters the products.
 template <typename C> struct TreeRow {
@@ -168,14 +186,23 @@ struct NodeRows {
   float inv;  // 1/max(|q|, eps), over the scaling
   template <typename T>
   __device__ inline void load(const T* row, bool ok, float eps, int half) {
-    constexpr int PER = K::M::PER;
+    constexpr int PER = K::M::PER, VEC = 16 / (int)sizeof(T);  // PER is a multiple of 4, VEC 4 or 8
+    constexpr int W = PER < VEC ? PER : VEC;
     float x[K::NKS][PER];
     float ss = 0.0f, mx = 0.0f;
 #pragma unroll
     for (int ks = 0; ks < K::NKS; ++ks)
 #pragma unroll
+      for (int e0 = 0; e0 < PER; e0 += W) {
+        typedef __attribute__((__vector_size__(W * sizeof(T)))) T vec;
+        const vec v = *reinterpret_cast<const vec*>(row + K::col(ks, half) + e0);
+#pragma unroll
+        for (int e = 0; e < W; ++e) x[ks][e0 + e] = ok ? to_f(v[e]) : 0.0f;
+      }
+#pragma unroll
+    for (int ks = 0; ks < K::NKS; ++ks)
+#pragma unroll
       for (int e = 0; e < PER; ++e) {
-        x[ks][e] = ok ? to_f(row[K::col(ks, half) + e]) : 0.0f;
         ss = fmaf(x[ks][e], x[ks][e], ss);
         mx = fmaxf(mx, fabsf(x[ks][e]));
       }
@@ -332,6 +359,15 @@ __device__ inline void store_row_as(void* y, int64_t off, int dtype, int half, F
   else store_row<COMP, float, D>((float*)y + off, half, fn);
 }
 
+__device__ inline int wave_max(int x) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_xor(x, o);
+    x = y > x ? y : x;
+  }
+  return x;
+}
+
 // What a wave knows of the tree: each lane's node, its depth and the bitmap of
 // the nodes on its way up (itself among them).  A parent that is no earlier
 // node makes the node a root.
@@ -364,29 +400,83 @@ struct Tree {
   }
 };
 
-// Committed length of sequence b, and head h's key units: keys lo, lo + 1, ...,
-// n + N - 1 in units of 32 (none for an empty window).
+// Committed length of sequence b; head h's key units: keys lo, lo + 1, ..., n +
+// N - 1 in units of 32 (none for an empty window).
 struct TreeSpan {
-  int n, lo, units;
-  __device__ TreeSpan(const TreeCall& a, int b, const HeadParams& hp) {
+  int n;
+  __device__ TreeSpan(const TreeCall& a, int b) {
     int64_t x = a.lengths[(int64_t)b * a.len_step];
     x = x > a.cap - a.N ? a.cap - a.N : x;
     n = x < 0 ? 0 : (int)x;
-    lo = n - hp.wc + 1;
-    lo = lo < 0 ? 0 : lo;
-    units = hp.wc == 0 ? 0 : (n + a.N - lo + kUnit - 1) / kUnit;
   }
-  // Units of each of the at most `blocks` blocks that share them.
-  __device__ int per(int blocks) const {
-    const int p = (units + blocks - 1) / blocks;
-    return p < kTreeMinUnits ? kTreeMinUnits : p;
+  __device__ int lo(int wc) const { return n - wc + 1 < 0 ? 0 : n - wc + 1; }
+  __device__ int units(const TreeCall& a, int wc) const {
+    return wc == 0 ? 0 : (n + a.N - lo(wc) + kUnit - 1) / kUnit;
   }
 };
 
-// Block (x, y): units [x per, (x + 1) per) of head y.  Waves w and w + WPT, ...
-// of a node tile take every WPT-th unit.
+// How the blocks of a sequence share its heads' units: head h's are cut into
+// pieces of `per`, the heads' pieces numbered one after the other, a block
+// each; `per` is the least (in steps of an eighth) for which the blocks
+// suffice.  Windows differ by orders of magnitude between heads, and blocks per
+// head would leave most of the card to the widest.  Wave-uniform.
+struct TreeMap {
+  int per;
+  __device__ static int units_of(const TreeCall& a, const TreeSpan& sp, int h) {
+    return h < a.H ? sp.units(a, head_params(a.r, a.w, h, true).wc) : 0;
+  }
+  __device__ static int sum(int x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+    return x;
+  }
+  __device__ TreeMap(const TreeCall& a, const TreeSpan& sp, int lane) {
+    const int first = units_of(a, sp, lane);
+    int all = sum(first);
+    for (int h = 64; h < a.H; h += 64) all += sum(units_of(a, sp, h + lane));
+    per = (all + a.blocks - 1) / a.blocks;
+    per = per < kTreeMinUnits ? kTreeMinUnits : per;
+    for (;; per += per / 8) {  // ends: one piece a head fits
+      int pieces = sum((first + per - 1) / per);
+      for (int h = 64; h < a.H; h += 64) pieces += sum((units_of(a, sp, h + lane) + per - 1) / per);
+      if (pieces <= a.blocks) return;
+    }
+  }
+  // The head of piece i, or -1; its first piece.
+  __device__ int head_of(const TreeCall& a, const TreeSpan& sp, int lane, int i, int& piece0) const {
+    int carry = 0;
+    for (int h = 0; h < a.H; h += 64) {
+      const int c = (units_of(a, sp, h + lane) + per - 1) / per;
+      int incl = c;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(incl, o);
+        if (lane >= o) incl += y;
+      }
+      incl += carry;
+      const unsigned long long past = __ballot(incl > i);
+      if (past != 0ull) {
+        const int l = (int)__builtin_ctzll(past);
+        piece0 = __shfl(incl - c, l);
+        return h + l;
+      }
+      carry = __shfl(incl, 63);
+    }
+    return -1;
+  }
+  // First piece of head h and how many it has.
+  __device__ int pieces_of(const TreeCall& a, const TreeSpan& sp, int lane, int h, int& piece0) const {
+    int before = 0;
+    for (int g = 0; g <= h; g += 64) before += sum(g + lane < h ? (units_of(a, sp, g + lane) + per - 1) / per : 0);
+    piece0 = before;
+    return (units_of(a, sp, h) + per - 1) / per;
+  }
+};
+
+// Block (x, y): piece x of sequence y, or all of head x.  The waves of a node
+// tile take every WPT-th unit of it.
 template <typename C, int D, int PARTS>
-__global__ __launch_bounds__(256) void tree_kernel(TreeCall a) {
+__global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D, D * (int)sizeof(C), PARTS)) void tree_kernel(TreeCall a) {
   using K = KeyRows<C, D>;
   using V = ValueRows<C, D>;
   using comp = typename K::comp;
@@ -395,20 +485,54 @@ __global__ __launch_bounds__(256) void tree_kernel(TreeCall a) {
   using Tile = typename V::Tile;
   constexpr int NDH = Tile::NDH, NC = Tile::NC;
   constexpr bool kTwo = sizeof(comp) == 2;  // weights as two terms
+  constexpr bool kAhead = D * sizeof(C) <= AHEAD;  // registers for a unit of values in flight
   constexpr int kRed = kUnit * V::DP * 4;   // a wave's sums
-  constexpr int kLds = kTreeWaves * Tile::BYTES > 2 * kRed ? kTreeWaves * Tile::BYTES : 2 * kRed;
+  constexpr int kLds = kTreeWaves * (Tile::BYTES > kRed / 2 ? Tile::BYTES : kRed / 2);
   __shared__ __align__(16) char lds[kLds];
   __shared__ __align__(16) float kfac[kTreeWaves][kUnit], vfac[kTreeWaves][kUnit], mtab[kTreeWaves][128];
   __shared__ int dtab[kTreeWaves][kTreeMax];
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
-  const int b = blockIdx.y / a.H, h = blockIdx.y % a.H;
+  const int b = blockIdx.y;
   const int tiles = (a.N + 31) / 32, wpt = kTreeWaves / tiles, tile = wave / wpt, kw = wave % wpt;
+  const TreeSpan sp(a, b);
+  int h = blockIdx.x, u0 = 0, per = 0;
+  if (a.blocks != a.H) {
+    const TreeMap map(a, sp, lane);
+    int piece0 = 0;
+    h = map.head_of(a, sp, lane, blockIdx.x, piece0);
+    if (h < 0) return;
+    per = map.per;
+    u0 = ((int)blockIdx.x - piece0) * per;
+  }
   const HeadParams hp = head_params(a.r, a.w, h, true);
-  const TreeSpan sp(a, b, hp);
-  const int per = sp.per(gridDim.x);
-  const int u0 = blockIdx.x * per, u1 = u0 + per < sp.units ? u0 + per : sp.units;
-  if (gridDim.x > 1 && u0 >= sp.units) return;
+  const int units = sp.units(a, hp.wc), lo_key = sp.lo(hp.wc);
+  if (per == 0) per = units;
+  const int u1 = u0 + per < units ? u0 + per : units;
+
+  const char* kb = (const char*)a.kc + (b * a.ks.sb + h * a.ks.sh) * (int64_t)sizeof(C);
+  const char* vb = (const char*)a.vc + (b * a.vs.sb + h * a.vs.sh) * (int64_t)sizeof(C);
+  const int64_t kst = a.ks.st * (int64_t)sizeof(C), vst = a.vs.st * (int64_t)sizeof(C);
+  const float* ksc = a.kscale + b * a.kss.sb + h * a.kss.sh;
+  const float* vsc = a.vscale + b * a.vss.sb + h * a.vss.sh;
+  const int last = sp.n + a.N - 1;  // last key row
+
+  auto load_keys = [&](K& key, int u) {
+    const int j = lo_key + u * kUnit + perm_row(l32), c = j < last ? j : last;
+    key.load(kb + c * kst, ksc + c * a.kss.st, half);
+  };
+  auto load_values = [&](V& val, int u) {
+    const int k0 = lo_key + u * kUnit;
+    val.load([&](int r) { return vb + (int64_t)(k0 + r < last ? k0 + r : last) * vst; },
+             [&](int r) { return vsc + (int64_t)(k0 + r < last ? k0 + r : last) * a.vss.st; }, lane);
+  };
+  // rows in flight: the next unit's keys, and its values where the last unit
+  // had a live pair (a head's first units are taken to be live if it has few)
+  K key_next;
+  V val_next;
+  bool ahead = kAhead && per <= 4 * wpt, issued = ahead && u0 + kw < u1;
+  if (u0 + kw < u1) load_keys(key_next, u0 + kw);
+  if (issued) load_values(val_next, u0 + kw);
 
   const Tree tree(a.parents == nullptr ? nullptr : a.parents + b * a.par_sb, a.N, lane);
   dtab[wave][lane] = tree.depth;
@@ -426,13 +550,6 @@ __global__ __launch_bounds__(256) void tree_kernel(TreeCall a) {
     else q.load((const float*)a.q + off, ok, a.eps, half);
   }
 
-  const char* kb = (const char*)a.kc + (b * a.ks.sb + h * a.ks.sh) * (int64_t)sizeof(C);
-  const char* vb = (const char*)a.vc + (b * a.vs.sb + h * a.vs.sh) * (int64_t)sizeof(C);
-  const int64_t kst = a.ks.st * (int64_t)sizeof(C), vst = a.vs.st * (int64_t)sizeof(C);
-  const float* ksc = a.kscale + b * a.kss.sb + h * a.kss.sh;
-  const float* vsc = a.vscale + b * a.vss.sb + h * a.vss.sh;
-  const int last = sp.n + a.N - 1;  // last key row
-
   char* vt = lds + wave * Tile::BYTES;
   if constexpr (D < V::DP) {  // the columns past D
 #pragma unroll
@@ -446,13 +563,15 @@ __global__ __launch_bounds__(256) void tree_kernel(TreeCall a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
 
+  const int depth_max = a.parents == nullptr ? a.N - 1 : wave_max(tree.depth);
   for (int u = u0 + kw; u < u1; u += wpt) {
-    const int k0 = sp.lo + u * kUnit;  // position of the unit's first row (a drafted row: n + its node)
-    K key;
-    {
-      const int j = k0 + perm_row(l32) < last ? k0 + perm_row(l32) : last;
-      key.load(kb + j * kst, ksc + j * a.kss.st, half);
-    }
+    const int k0 = lo_key + u * kUnit;  // position of the unit's first row (a drafted row: n + its node)
+    const K key = key_next;
+    V val = val_next;
+    const bool have = issued;
+    issued = ahead && u + wpt < u1;
+    if (u + wpt < u1) load_keys(key_next, u + wpt);
+    if (issued) load_values(val_next, u + wpt);
     frag kf[K::NKS];
     key.frags(kf);
     const float f = key.factor(kf, a.eps);
@@ -473,26 +592,40 @@ __global__ __launch_bounds__(256) void tree_kernel(TreeCall a) {
       s[r] *= x[r];
       top = fmaxf(top, s[r]);
     }
+    ahead = false;
     if (__ballot(top * q.inv > hp.thr) == 0ull) continue;
 
     // a^2 m of every pair: register r is key row 16 (r/8) + 8 half + r%8
-    bool live = false;
+    float any = 0.0f;
+    if (k0 + kUnit <= sp.n) {
+      // committed keys: m from a table over depth - row (entry e: distance n - k0 - 31 + e)
+      const int dmin = sp.n - k0 - 31;
+      for (int e = lane; e < 32 + depth_max; e += 64)
+        mtab[wave][e] = in_window(dmin + e, hp) ? mask_fast(dmin + e, hp.w, hp.iw) : 0.0f;
+      wave_lds_sync();
+      const float* mt = mtab[wave] + (depth + 8 - 8 * half);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int row = 16 * (r >> 3) + 8 * half + (r & 7), j = k0 + row - sp.n;  // j >= 0: drafted
-      const bool draft = j >= 0;
-      const int dd = depth - (draft ? dtab[wave][j & (kTreeMax - 1)] : j);
-      const bool seen = draft ? j < a.N && ((above >> j) & 1ull) != 0ull : true;
-      const float av = fmaxf(fmaf(-hp.r, fmaf(-s[r], q.inv, 1.0f), 1.0f), 0.0f);
-      const bool on = seen && in_window(dd, hp) && av > 0.0f && node < a.N;
-      s[r] = on ? av * av * mask_fast(dd, hp.w, hp.iw) : 0.0f;
-      live = live || s[r] > 0.0f;
+      for (int r = 0; r < 16; ++r) {
+        const float av = fmaxf(fmaf(-hp.r, fmaf(-s[r], q.inv, 1.0f), 1.0f), 0.0f);
+        s[r] = av * av * mt[23 - 16 * (r >> 3) - (r & 7)];
+        any = fmaxf(any, s[r]);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = 16 * (r >> 3) + 8 * half + (r & 7), j = k0 + row - sp.n;  // j >= 0: drafted
+        const bool draft = j >= 0;
+        const int dd = depth - (draft ? dtab[wave][j & (kTreeMax - 1)] : j);
+        const bool seen = draft ? j < a.N && ((above >> j) & 1ull) != 0ull : true;
+        const float av = fmaxf(fmaf(-hp.r, fmaf(-s[r], q.inv, 1.0f), 1.0f), 0.0f);
+        s[r] = seen && in_window(dd, hp) ? av * av * mask_fast(dd, hp.w, hp.iw) : 0.0f;
+        any = fmaxf(any, s[r]);
+      }
     }
-    if (__ballot(live) == 0ull) continue;
+    if (__ballot(any > 0.0f) == 0ull) continue;
 
-    V val;
-    val.load([&](int r) { return vb + (int64_t)(k0 + r < last ? k0 + r : last) * vst; },
-             [&](int r) { return vsc + (int64_t)(k0 + r < last ? k0 + r : last) * a.vss.st; }, lane);
+    ahead = kAhead;
+    if (!have) load_values(val, u);
     val.stage(vt, vfac[wave], a.eps, lane);
     wave_lds_sync();
     read_row_scales(vfac[wave], half, x);
@@ -524,9 +657,8 @@ __global__ __launch_bounds__(256) void tree_kernel(TreeCall a) {
     guard_all(lo, acc[NDH - 1]);
   }
 
-  // the waves of a tile: w += w + 2 (one tile), then w += w + 1
-  __syncthreads();
-  char* red = lds + (tiles == 1 ? wave & 1 : tile) * kRed;
+  // the waves of a tile, the upper half of them into the lower, until one has all
+  char* red = nullptr;
   auto put = [&] {
 #pragma unroll
     for (int d = 0; d < NDH; ++d)
@@ -545,21 +677,18 @@ __global__ __launch_bounds__(256) void tree_kernel(TreeCall a) {
         for (int e = 0; e < 4; ++e) acc[d][4 * g + e] += x[e];
       }
   };
-  if (tiles == 1) {
-    if (wave >= 2) put();
+  for (int step = wpt / 2; step >= 1; step /= 2) {
+    red = lds + (tile * step + kw % step) * kRed;
     __syncthreads();
-    if (wave < 2) add();
+    if (kw >= step && kw < 2 * step) put();
     __syncthreads();
-    red = lds;
+    if (kw < step) add();
   }
-  if (kw == 1) put();
-  __syncthreads();
   if (kw != 0) return;
-  add();
   if (node >= a.N) return;  // lanes l and l + 32 share a node
   constexpr float down = 1.0f / kWeightUp<C>;
-  if (gridDim.x > 1) {
-    float* p = a.part + ((int64_t)(blockIdx.y * gridDim.x + blockIdx.x) * a.N + node) * D;
+  if (a.blocks != a.H) {
+    float* p = a.part + (((int64_t)b * a.blocks + blockIdx.x) * a.N + node) * D;
     store_row<comp, float, D>(p, half, [&](int d, int r) { return acc[d][r] * down; });
     return;
   }
@@ -576,60 +705,55 @@ __global__ __launch_bounds__(256) void tree_kernel(TreeCall a) {
                         [&](int d, int r) { return acc[d][r] * fy; });
 }
 
-// Sum of a node's block sums, in block order, and TanhNorm.  Block per (node,
-// b, h).
+// Sum of a node's block sums and TanhNorm: a wave per node, D/4 lanes for a
+// block's sums and 256/D blocks at a time.
 template <int D>
-__global__ __launch_bounds__(256) void tree_reduce_kernel(TreeCall a, int blocks) {
-  constexpr int G = 256 / D;
-  __shared__ float red[256];
-  __shared__ float sq[D];
-  const int node = blockIdx.x, b = blockIdx.y / a.H, h = blockIdx.y % a.H;
-  const int t = threadIdx.x, d = t % D, g = t / D;
-  const HeadParams hp = head_params(a.r, a.w, h, true);
-  const TreeSpan sp(a, b, hp);
-  const int per = sp.per(blocks), used = (sp.units + per - 1) / per;
-  const float* p = a.part + ((int64_t)blockIdx.y * blocks * a.N + node) * D + d;
-  float x = 0.0f;
+__global__ __launch_bounds__(256) void tree_reduce_kernel(TreeCall a) {
+  constexpr int L = D / 4, G = 64 / L;
+  const int lane = threadIdx.x & 63, node = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int b = blockIdx.y / a.H, h = blockIdx.y % a.H;
+  if (node >= a.N) return;
+  const TreeSpan sp(a, b);
+  const TreeMap map(a, sp, lane);
+  int piece0;
+  const int used = map.pieces_of(a, sp, lane, h, piece0);
+  const float* p = a.part + (((int64_t)b * a.blocks + piece0) * a.N + node) * D + 4 * (lane % L);
+  f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-  for (int c = g; c < used; c += G) x += p[(int64_t)c * a.N * D];
-  red[t] = x;
-  __syncthreads();
-  x = 0.0f;
-  if (t < D) {
+  for (int c = lane / L; c < used; c += G) x += *reinterpret_cast<const f32x4*>(p + (int64_t)c * a.N * D);
 #pragma unroll
-    for (int k = 0; k < G; ++k) x += red[k * D + t];
-    sq[t] = x * x;
-  }
-  __syncthreads();
-  for (int s = D / 2; s > 0; s >>= 1) {
-    if (t < s) sq[t] += sq[t + s];
-    __syncthreads();
-  }
-  const float nc = fmaxf(sqrtf(sq[0]), a.eps), fy = tanhf(nc) / nc;
-  if (t >= D) return;
-  const int64_t at = (((int64_t)b * a.N + node) * a.H + h) * D + t;
-  if (a.q_dtype == 1) ((bf16*)a.y)[at] = (bf16)(x * fy);
-  else if (a.q_dtype == 2) ((f16*)a.y)[at] = (f16)(x * fy);
-  else ((float*)a.y)[at] = x * fy;
+  for (int o = L; o < 64; o <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], o);
+  const float ss = group_sum<L>(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
+  const float nc = fmaxf(sqrtf(ss), a.eps), fy = tanhf(nc) / nc;
+  if (lane >= L) return;
+  const int64_t at = (((int64_t)b * a.N + node) * a.H + h) * D + 4 * lane;
+  if (a.q_dtype == 1) store4((bf16*)a.y + at, x[0] * fy, x[1] * fy, x[2] * fy, x[3] * fy);
+  else if (a.q_dtype == 2) store4((f16*)a.y + at, x[0] * fy, x[1] * fy, x[2] * fy, x[3] * fy);
+  else store4((float*)a.y + at, x[0] * fy, x[1] * fy, x[2] * fy, x[3] * fy);
 }
 
 int tree_max_nodes() { return kTreeMax; }
-// Blocks that share a head's units: about four per CU in all, each with at
-// least kTreeMinUnits of the longest window's.
-int tree_blocks(int B, int H, int N, int span) {
+// Blocks of a sequence: as many as run at one time on the card's 256 CUs share
+// its heads' keys; one a head (H) where heads are short, or the batch alone
+// fills the card several times over with heads that are not long.
+int tree_blocks(int B, int H, int N, int D, int q_dtype, int cache_dtype, int span) {
   const int64_t units = ((int64_t)span + N + kUnit - 1) / kUnit;
-  int64_t most = (units + kTreeMinUnits - 1) / kTreeMinUnits;
-  const int64_t want = (1024 + (int64_t)B * H - 1) / ((int64_t)B * H);
-  most = most < want ? most : want;
-  return (int)(most < 1 ? 1 : most);
+  const bool codes = cache_dtype == kInt8 || cache_dtype == kFp8;
+  const int row = D * (codes ? 1 : cache_dtype == 0 ? 4 : 2);
+  const int slots = 256 * tree_occupancy(D, row, codes && q_dtype == 0 ? 2 : 1);
+  if (units <= kTreeSmall || ((int64_t)B * H >= 2 * slots && units <= 4 * kTreeSmall)) return H;
+  const int each = slots / B;
+  return each < 2 * H ? 2 * H : each;
 }
 
 template <typename C, int D, int PARTS>
 static hipError_t launch_tree_t(const TreeCall& c) {
-  hipLaunchKernelGGL((tree_kernel<C, D, PARTS>), dim3((unsigned)c.blocks, (unsigned)(c.B * c.H)), dim3(256), 0, c.stream, c);
+  hipLaunchKernelGGL((tree_kernel<C, D, PARTS>), dim3((unsigned)c.blocks, (unsigned)c.B), dim3(64 * kTreeWaves), 0, c.stream, c);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || c.blocks == 1) return e;
-  hipLaunchKernelGGL((tree_reduce_kernel<D>), dim3((unsigned)c.N, (unsigned)(c.B * c.H)), dim3(256), 0, c.stream, c, c.blocks);
+  if (e != hipSuccess || c.blocks == c.H) return e;
+  hipLaunchKernelGGL((tree_reduce_kernel<D>), dim3((unsigned)((c.N + 3) / 4), (unsigned)(c.B * c.H)), dim3(256), 0, c.stream, c);
   return hipGetLastError();
 }
 template <typename C, int PARTS>

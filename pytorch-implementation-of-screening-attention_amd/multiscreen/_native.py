@@ -56,7 +56,7 @@ _SIGS = {
                              _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p]),
     "msa_cache_read": (_i, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i,
                             _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i, _i, _i, _i, _p, _i, _i64, _p, _p, _p]),
-    "msa_tree_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "msa_tree_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
     "msa_tree_decode": (_i, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i,
                              _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i, _i, _i, _i,
                              _p, _i, _p, _i64, _i, _p, _p, _f, _p, _p, _sz, _p]),

@@ -18,8 +18,6 @@ kernels, so their backward is too.
 GPU tensors only: a CPU tensor, or a missing libmsa.so, raises.
 """
 
-import contextlib
-
 import torch
 
 from . import _native
@@ -246,68 +244,94 @@ def decode_step_at(q, kcache, vcache, last_pos, r, w, eps=1e-8, workspace=None, 
 
 
 # ---------------------------------------------------------------------------
-# Caches of 8-bit codes, several new tokens at once, and drafted tokens
+# Caches of 8-bit codes, several new tokens at once, and drafted tokens.  These
+# calls are short (a decode step's rows, a few hundred keys), so their checks
+# look at each tensor once and build messages only for a call that is refused.
 # ---------------------------------------------------------------------------
 _CACHE_DTYPES = {**_DTYPES, torch.int8: _native.MSA_I8, torch.float8_e4m3fn: _native.MSA_FP8}
 CODE_DTYPES = (torch.int8, torch.float8_e4m3fn)
+_NO_SCALES = (None, 0, 0, 0)
 
 
-def _on(dev):
-    """Launches go to the tensors' device, whichever is current."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+def _launch(what, fn, index, args):
+    """Calls fn(*args, stream) for tensors of GPU `index`, whichever device is current."""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        _native.check(rc, what)
 
 
-def _check_gpu(what, **tensors):
-    """Every tensor given is on one GPU; returns it."""
-    dev = None
-    for name, x in tensors.items():
-        if x is None:
-            continue
-        if not x.is_cuda:
-            raise RuntimeError(f"{what} runs on the GPU only ({name} is a CPU tensor)")
-        if dev is not None and x.device != dev:
-            raise RuntimeError(f"{what}: {name} is on {x.device}, other tensors on {dev}")
-        dev = x.device
-    return dev
+def _one_gpu(what, first, **others):
+    """The index of the GPU that every tensor given is on."""
+    index = first.get_device()
+    if index < 0:
+        raise RuntimeError(f"{what} runs on the GPU only (got a CPU tensor)")
+    for name, x in others.items():
+        if x is not None and x.get_device() != index:
+            raise RuntimeError(f"{what} runs on one GPU: {name} is on {x.device}, not on {first.device}")
+    return index
 
 
 def _index(x, name, *shapes):
     """An int64 tensor of one of the shapes, contiguous."""
-    if x.dtype != torch.int64 or tuple(x.shape) not in shapes:
+    if x.dtype != torch.int64 or x.shape not in shapes:
         raise ValueError(f"{name} must be int64 of shape {' or '.join(map(str, shapes))}, got {x.dtype} {tuple(x.shape)}")
     return x.contiguous()
 
 
+def _float32(x):
+    """r or w as the kernels take it."""
+    if x.dtype != torch.float32 or not x.is_contiguous():
+        x = x.detach().to(torch.float32).contiguous()
+    return x
+
+
+def _rows_bthd(x, name):
+    """x (B, T, H, D) as the kernels read it, its pointer and its first three strides."""
+    if x.dim() == 4:
+        sb, st, sh, sd = x.stride()
+        p = x.data_ptr()
+        if sd == 1 and not ((sb | st | sh) * x.element_size() | p) & 15:
+            return x, (p, sb, st, sh)
+    x = _as_bthd(x, name, x.element_size())
+    return x, _args_bthd(x)
+
+
 def _cache_args(what, kcache, vcache, kscale, vscale, dtype):
-    """Checks a cache pair (B, cap, H, D) and its scales (B, cap, H) against the rows' type; returns the C arguments
-    of the codes and of the scales."""
+    """The C arguments of a cache pair (B, cap, H, D) and of its scales (B, cap, H), checked against the
+    rows' type."""
     if kcache.dim() != 4 or kcache.shape != vcache.shape or kcache.dtype != vcache.dtype:
         raise ValueError(f"{what}: the caches must be (B, cap, H, D) of one shape and type, got {kcache.dtype} "
                          f"{tuple(kcache.shape)}, {vcache.dtype} {tuple(vcache.shape)}")
-    codes = kcache.dtype in CODE_DTYPES
-    if not codes and kcache.dtype != dtype:
-        raise TypeError(f"{what}: a cache of {kcache.dtype} does not hold rows of {dtype}")
-    mult = 16 // kcache.element_size()
-    args, scales = [], []
-    for name, c, s in (("kcache", kcache, kscale), ("vcache", vcache, vscale)):
-        if c.stride(3) != 1 or any(x % mult for x in c.stride()[:3]) or c.data_ptr() % 16:
-            raise ValueError(f"{what}: {name} needs unit stride over D and 16-byte aligned rows, got strides {c.stride()}")
-        if codes != (s is not None):
-            raise ValueError(f"{what}: {name} of {c.dtype} {'needs its scales' if codes else 'takes no scales'}")
-        if codes and (s.dtype != torch.float32 or s.shape != c.shape[:3]):
-            raise ValueError(f"{what}: the scales of {name} must be float32 {tuple(c.shape[:3])}, got {s.dtype} "
-                             f"{tuple(s.shape)}")
-        args += _args_bthd(c)
-        scales += (s.data_ptr(), *s.stride()) if codes else (None, 0, 0, 0)
-    return args, scales
+    kb, kt, kh, kd = kcache.stride()
+    vb, vt, vh, vd = vcache.stride()
+    kp, vp = kcache.data_ptr(), vcache.data_ptr()
+    if kd != 1 or vd != 1 or ((kb | kt | kh | vb | vt | vh) * kcache.element_size() | kp | vp) & 15:
+        raise ValueError(f"{what}: the caches need unit stride over D and 16-byte aligned rows, got strides "
+                         f"{kcache.stride()}, {vcache.stride()}")
+    pair = (kp, kb, kt, kh, vp, vb, vt, vh)
+    if kcache.dtype not in CODE_DTYPES:
+        if kcache.dtype != dtype:
+            raise TypeError(f"{what}: a cache of {kcache.dtype} does not hold rows of {dtype}")
+        if kscale is not None or vscale is not None:
+            raise ValueError(f"{what}: a cache of {kcache.dtype} takes no scales")
+        return pair, _NO_SCALES + _NO_SCALES
+    shape = kcache.shape[:3]
+    if kscale is None or vscale is None or kscale.dtype != torch.float32 or vscale.dtype != torch.float32 \
+            or kscale.shape != shape or vscale.shape != shape:
+        raise ValueError(f"{what}: a cache of {kcache.dtype} needs kscale and vscale, float32 {tuple(shape)}")
+    return pair, (kscale.data_ptr(), *kscale.stride(), vscale.data_ptr(), *vscale.stride())
 
 
-def _start_args(start, B, dev):
+def _start_args(start, B):
     """(pointer or None, count, host value, tensor to keep) of an int or int64 device tensor."""
     if not torch.is_tensor(start):
         return None, 0, int(start), None
     start = _index(start, "start", (1,), (B,))
-    return start.data_ptr(), start.numel(), 0, start
+    return start.data_ptr(), start.shape[0], 0, start
 
 
 def cache_write(k, v, kcache, vcache, start, kscale=None, vscale=None, rows=None, count=None):
@@ -325,34 +349,33 @@ def cache_write(k, v, kcache, vcache, start, kscale=None, vscale=None, rows=None
     verify_drafts.  Rows outside k are not written.
     The rest of the cache is left as it was.  No gradient flows through it.
     """
-    L = _native.lib()
-    dev = _check_gpu("cache_write", k=k, v=v, kcache=kcache, vcache=vcache, kscale=kscale, vscale=vscale, rows=rows,
+    index = _one_gpu("cache_write", k, v=v, kcache=kcache, vcache=vcache, kscale=kscale, vscale=vscale, rows=rows,
                      count=count, start=start if torch.is_tensor(start) else None)
-    if k.dtype not in _DTYPES or v.dtype != k.dtype or k.shape != v.shape:
+    dtype = k.dtype
+    if dtype not in _DTYPES or v.dtype != dtype or k.shape != v.shape:
         raise TypeError(f"cache_write: k and v must share shape and dtype float32, bfloat16 or float16, got {k.dtype} "
                         f"{tuple(k.shape)}, {v.dtype} {tuple(v.shape)}")
-    es = k.element_size()
-    k, v = _as_bthd(k, "k", es), _as_bthd(v, "v", es)
+    k, kargs = _rows_bthd(k, "k")
+    v, vargs = _rows_bthd(v, "v")
     B, Tx, H, D = k.shape
-    if kcache.dim() != 4 or (kcache.shape[0], *kcache.shape[2:]) != (B, H, D):
+    pair, scales = _cache_args("cache_write", kcache, vcache, kscale, vscale, dtype)
+    Bc, cap, Hc, Dc = kcache.shape
+    if Bc != B or Hc != H or Dc != D:
         raise ValueError(f"cache_write: cache {tuple(kcache.shape)} does not match rows {tuple(k.shape)}")
-    codes, scales = _cache_args("cache_write", kcache, vcache, kscale, vscale, k.dtype)
-    cap = int(kcache.shape[1])
-    T = Tx
+    T, rp, cp = Tx, None, None
     if rows is not None:
-        T = int(rows.shape[-1])
+        T = rows.shape[-1]
         rows = _index(rows, "rows", (B, T))
+        rp = rows.data_ptr()
     if count is not None:
         count = _index(count, "count", (B,))
-    ptr, n, host, keep = _start_args(start, B, dev)
-    if ptr is None and (host < 0 or host + (T if count is None else 0) > cap):
+        cp = count.data_ptr()
+    sp, n, host, start = _start_args(start, B)
+    if sp is None and (host < 0 or host + (T if count is None else 0) > cap):
         raise IndexError(f"KV cache capacity {cap} exceeded at position {host + T}")
-    with _on(dev):
-        rc = L.msa_cache_write(*_args_bthd(k), *_args_bthd(v), B, T, Tx, H, D, _DTYPES[k.dtype],
-                               rows.data_ptr() if rows is not None else None,
-                               count.data_ptr() if count is not None else None, ptr, n, host,
-                               *codes, cap, _CACHE_DTYPES[kcache.dtype], *scales, _stream_ptr(dev))
-    _native.check(rc, "msa_cache_write")
+    _launch("msa_cache_write", _native.lib().msa_cache_write, index,
+            (*kargs, *vargs, B, T, Tx, H, D, _DTYPES[dtype], rp, cp, sp, n, host, *pair, cap,
+             _CACHE_DTYPES[kcache.dtype], *scales))
 
 
 def cache_read(kcache, vcache, kscale, vscale, start, length, dtype):
@@ -360,23 +383,21 @@ def cache_read(kcache, vcache, kscale, vscale, start, length, dtype):
     cache_write takes it) in `dtype`: code * scale, rounded once; (k, v), each
     contiguous (B, length, H, D).  With a device `start`, positions outside the
     cache read as zeros."""
-    L = _native.lib()
-    dev = _check_gpu("cache_read", kcache=kcache, vcache=vcache, kscale=kscale, vscale=vscale,
+    index = _one_gpu("cache_read", kcache, vcache=vcache, kscale=kscale, vscale=vscale,
                      start=start if torch.is_tensor(start) else None)
     if dtype not in _DTYPES:
         raise TypeError(f"cache_read: dtype must be float32, bfloat16 or float16, got {dtype}")
-    codes, scales = _cache_args("cache_read", kcache, vcache, kscale, vscale, dtype)
+    pair, scales = _cache_args("cache_read", kcache, vcache, kscale, vscale, dtype)
     B, cap, H, D = kcache.shape
     length = int(length)
-    ptr, n, host, keep = _start_args(start, B, dev)
-    if length < 0 or (ptr is None and (host < 0 or host + length > cap)):
+    sp, n, host, start = _start_args(start, B)
+    if length < 0 or (sp is None and (host < 0 or host + length > cap)):
         raise IndexError(f"positions {host} .. {host + length} are outside the KV cache's capacity {cap}")
-    k = torch.empty((B, length, H, D), dtype=dtype, device=dev)
+    k = torch.empty((B, length, H, D), dtype=dtype, device=kcache.device)
     v = torch.empty_like(k)
-    with _on(dev):
-        rc = L.msa_cache_read(*codes, cap, _CACHE_DTYPES[kcache.dtype], *scales, B, length, H, D, _DTYPES[dtype],
-                              ptr, n, host, k.data_ptr(), v.data_ptr(), _stream_ptr(dev))
-    _native.check(rc, "msa_cache_read")
+    _launch("msa_cache_read", _native.lib().msa_cache_read, index,
+            (*pair, cap, _CACHE_DTYPES[kcache.dtype], *scales, B, length, H, D, _DTYPES[dtype], sp, n, host,
+             k.data_ptr(), v.data_ptr()))
     return k, v
 
 
@@ -384,7 +405,7 @@ def _parents_arg(parents, B, N):
     """(pointer or None, stride over sequences, tensor to keep) of parents (N,) or (B, N), or None: a chain."""
     if parents is None:
         return None, 0, None
-    parents = _index(parents, "parents", (N,), (B, N))
+    parents = _index(parents, "parents", (B, N), (N,))
     return parents.data_ptr(), N if parents.dim() == 2 else 0, parents
 
 
@@ -405,38 +426,37 @@ def tree_decode(q, kcache, vcache, lengths, parents, r, w, eps=1e-8, kscale=None
     window_hint: 0, or a bound on ceil(w) over the heads (sizes the launch).
     Returns y (B, N, H, D) = TanhNorm(h), in q's dtype; no gradient.
     """
-    L = _native.lib()
-    dev = _check_gpu("tree_decode", q=q, kcache=kcache, vcache=vcache, kscale=kscale, vscale=vscale, lengths=lengths,
-                     parents=parents, workspace=workspace)
-    if q.dtype not in _DTYPES:
+    index = _one_gpu("tree_decode", q, kcache=kcache, vcache=vcache, kscale=kscale, vscale=vscale, lengths=lengths,
+                     parents=parents, r=r, w=w, workspace=workspace)
+    dtype = q.dtype
+    if dtype not in _DTYPES:
         raise TypeError(f"tree_decode: q must be float32, bfloat16 or float16, got {q.dtype}")
-    q = _as_bthd(q, "q", q.element_size())
+    q, qargs = _rows_bthd(q, "q")
     B, N, H, D = q.shape
     if N > _native.TREE_MAX:
         raise ValueError(f"tree_decode: a tree holds at most {_native.TREE_MAX} nodes, got {N}")
-    codes, scales = _cache_args("tree_decode", kcache, vcache, kscale, vscale, q.dtype)
-    if (kcache.shape[0], *kcache.shape[2:]) != (B, H, D):
+    pair, scales = _cache_args("tree_decode", kcache, vcache, kscale, vscale, dtype)
+    Bc, cap, Hc, Dc = kcache.shape
+    if Bc != B or Hc != H or Dc != D:
         raise ValueError(f"tree_decode: cache {tuple(kcache.shape)} does not match q {tuple(q.shape)}")
-    cap = int(kcache.shape[1])
     if N > cap:
         raise IndexError(f"KV cache capacity {cap} is below {N} nodes")
     if r.shape != (H,) or w.shape != (H,):
         raise ValueError(f"r and w must have shape ({H},)")
-    lengths = _index(lengths, "lengths", (1,), (B,))
+    lengths = _index(lengths, "lengths", (B,), (1,))
     par, par_sb, parents = _parents_arg(parents, B, N)
-    r32 = r.detach().to(device=dev, dtype=torch.float32).contiguous()
-    w32 = w.detach().to(device=dev, dtype=torch.float32).contiguous()
+    r, w = _float32(r), _float32(w)
     hint = max(0, int(window_hint))
-    y = torch.empty((B, N, H, D), dtype=q.dtype, device=dev)
-    need = int(L.msa_tree_workspace_bytes(B, H, N, D, cap, hint))
+    L = _native.lib()
+    y = torch.empty((B, N, H, D), dtype=dtype, device=q.device)
+    qt, ct = _DTYPES[dtype], _CACHE_DTYPES[kcache.dtype]
+    need = L.msa_tree_workspace_bytes(B, H, N, D, qt, ct, cap, hint)
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty((need,), dtype=torch.uint8, device=dev)
-    with _on(dev):
-        rc = L.msa_tree_decode(*_args_bthd(q), *codes, cap, _CACHE_DTYPES[kcache.dtype], *scales, B, N, H, D,
-                               _DTYPES[q.dtype], lengths.data_ptr(), lengths.numel(), par, par_sb, hint,
-                               r32.data_ptr(), w32.data_ptr(), float(eps), y.data_ptr(),
-                               workspace.data_ptr() if need else None, need, _stream_ptr(dev))
-    _native.check(rc, "msa_tree_decode")
+        workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
+    _launch("msa_tree_decode", L.msa_tree_decode, index,
+            (*qargs, *pair, cap, ct, *scales, B, N, H, D, qt, lengths.data_ptr(), lengths.shape[0], par, par_sb, hint,
+             r.data_ptr(), w.data_ptr(), float(eps), y.data_ptr(),
+             workspace.data_ptr() if need else None, need))
     return y
 
 
@@ -464,9 +484,9 @@ def verify_drafts(target, tokens, parents=None, uniforms=None, draft=None):
     count (B), how many; token (B), the next token.  The count[b] rows path[b]
     are what cache_write takes as `rows` and `count`.
     """
-    L = _native.lib()
-    dev = _check_gpu("verify_drafts", target=target, tokens=tokens, parents=parents, uniforms=uniforms, draft=draft)
-    if target.dim() != 3 or target.dtype not in _DTYPES:
+    index = _one_gpu("verify_drafts", target, tokens=tokens, parents=parents, uniforms=uniforms, draft=draft)
+    dtype = target.dtype
+    if target.dim() != 3 or dtype not in _DTYPES:
         raise TypeError(f"verify_drafts: target must be (B, M, V) float32, bfloat16 or float16, got {target.dtype} "
                         f"{tuple(target.shape)}")
     B, M, V = target.shape
@@ -474,28 +494,32 @@ def verify_drafts(target, tokens, parents=None, uniforms=None, draft=None):
         raise ValueError(f"verify_drafts: a tree holds 1 to {_native.TREE_MAX} nodes, got {M}")
     tokens = _index(tokens, "tokens", (B, M))
     par, par_sb, parents = _parents_arg(parents, B, M)
+    up = dp = None
+    d_sb = d_sn = 0
     if uniforms is not None:
         if uniforms.dtype != torch.float32 or uniforms.shape != (B, M):
             raise ValueError(f"uniforms must be float32 ({B}, {M}), got {uniforms.dtype} {tuple(uniforms.shape)}")
         uniforms = uniforms.contiguous()
+        up = uniforms.data_ptr()
     if draft is not None:
         if uniforms is None:
             raise ValueError("verify_drafts: draft probabilities need uniforms")
-        if draft.dtype != target.dtype or draft.shape != (B, M - 1, V):
-            raise ValueError(f"draft must be {target.dtype} ({B}, {M - 1}, {V}), got {draft.dtype} {tuple(draft.shape)}")
+        if draft.dtype != dtype or draft.shape != (B, M - 1, V):
+            raise ValueError(f"draft must be {dtype} ({B}, {M - 1}, {V}), got {draft.dtype} {tuple(draft.shape)}")
         draft = draft if draft.stride(2) == 1 else draft.contiguous()
+        d_sb, d_sn, _ = draft.stride()
+        dp = draft.data_ptr() if M > 1 else None  # a chain of one node has no draft rows: nothing can be refused
     target = target if target.stride(2) == 1 else target.contiguous()
-    path = torch.empty((B, M), dtype=torch.int64, device=dev)
-    count, token = torch.empty((2, B), dtype=torch.int64, device=dev)
-    need = int(L.msa_verify_workspace_bytes(B, M, V, int(uniforms is None)))
-    workspace = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-    with _on(dev):
-        # a chain of one node has no draft rows: nothing can be refused
-        rc = L.msa_verify(target.data_ptr(), target.stride(0), target.stride(1),
-                          draft.data_ptr() if draft is not None and M > 1 else None,
-                          *(draft.stride()[:2] if draft is not None else (0, 0)), tokens.data_ptr(), par, par_sb,
-                          uniforms.data_ptr() if uniforms is not None else None, B, M, V, _DTYPES[target.dtype],
-                          path.data_ptr(), count.data_ptr(), token.data_ptr(),
-                          workspace.data_ptr() if need else None, need, _stream_ptr(dev))
-    _native.check(rc, "msa_verify")
+    t_sb, t_sn, _ = target.stride()
+    L = _native.lib()
+    path = torch.empty((B, M), dtype=torch.int64, device=target.device)
+    count = torch.empty((B,), dtype=torch.int64, device=target.device)
+    token = torch.empty_like(count)
+    need, workspace = 0, None
+    if uniforms is None:
+        need = L.msa_verify_workspace_bytes(B, M, V, 1)
+        workspace = torch.empty((need,), dtype=torch.uint8, device=target.device)
+    _launch("msa_verify", L.msa_verify, index,
+            (target.data_ptr(), t_sb, t_sn, dp, d_sb, d_sn, tokens.data_ptr(), par, par_sb, up, B, M, V, _DTYPES[dtype],
+             path.data_ptr(), count.data_ptr(), token.data_ptr(), workspace.data_ptr() if need else None, need))
     return path, count, token

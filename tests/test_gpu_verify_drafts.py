@@ -277,7 +277,10 @@ def test_refusals():
 
 
 def test_c_entry_refuses_bad_arguments():
-    """Argument checks run before any device work, so these run without a GPU."""
+    """Argument checks run before any device work.  The pointers are no addresses, so this runs only where no
+    kernel could start."""
+    if torch.cuda.is_available():
+        pytest.skip("a call that is not refused would start a kernel")
     from multiscreen import _native
     L = _native.lib()
 
