@@ -462,6 +462,9 @@ static int check_cache(int B, int T, int H, int D, int dtype, const void* kcache
     for (int e = 0; e < 3; ++e)
       if (st[z][e] < 0 || st[z][e] % m)
         return fail(MSA_ERR_INVALID, "%s strides must be non-negative multiples of %d elements", name, m);
+    // kernels address the rows of a 32-row unit by 32-bit byte offsets
+    if (st[z][1] * 64 * (codes ? 1 : dtype == MSA_F32 ? 4 : 2) >= (int64_t)1 << 32 || (codes && sc[z][1] * 256 >= (int64_t)1 << 32))
+      return fail(MSA_ERR_INVALID, "%s time stride is too large (64 rows must span < 4 GiB)", name);
     if (!codes) continue;
     if (s[z] == nullptr) return fail(MSA_ERR_INVALID, "%s of 8-bit codes needs its scales", name);
     if (((uintptr_t)s[z] & 3u) != 0 || sc[z][0] < 0 || sc[z][1] < 0 || sc[z][2] < 0)

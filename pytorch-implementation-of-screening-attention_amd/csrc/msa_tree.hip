@@ -28,26 +28,15 @@
 namespace msa {
 
 constexpr int kTreeMax = 64;   // nodes of a tree: one lane each
-#ifndef WAVES
-#define WAVES 4
-#endif
-constexpr int kTreeWaves = WAVES;  // waves of a block
+constexpr int kTreeWaves = 4;  // waves of a block
 // Fewest units of a block, so that a block's sums stay small beside its keys.
 // Fewest units of a block, so that a block's sums stay small beside its keys;
 // a head of at most kTreeSmall units is one block's (no sums to join).
 constexpr int kTreeMinUnits = 8, kTreeSmall = 16;
 
 // Waves per SIMD that the kernel's registers are budgeted for.
-#ifndef O64
-#define O64 3
-#define O128 2
-#define O256 2
-#endif
-#ifndef AHEAD
-#define AHEAD 64
-#endif
-constexpr int tree_occupancy(int D, int row_bytes, int parts) {
-  return row_bytes * parts <= 64 ? O64 : (row_bytes <= 128 && D < 128 ? O128 : row_bytes <= 256 ? O256 : 1);
+constexpr int tree_occupancy(int row_bytes, int parts) {
+  return row_bytes * parts <= 64 ? 3 : row_bytes <= 256 ? 2 : 1;
 }
 
 // How a cache row of type C enters the products.
@@ -129,10 +118,12 @@ struct KeyRows {
     else if constexpr (D == 16) return 8 * half;
     else return 32 * (ks / 2) + 16 * half + 8 * (ks & 1);
   }
-  __device__ inline void load(const char* row, const float* sc, int half) {
+  // `off`: the lane's row and half in bytes from the wave-uniform address
+  // `rows`, `soff` its scale's.
+  __device__ inline void load(const char* rows, uint32_t off, const char* scales, uint32_t soff) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const char* p = row + (2 * i + half) * LB;
+      const char* p = rows + off + 2 * i * LB;
       if constexpr (LB == 8) {
         const u32x2 x = *reinterpret_cast<const u32x2*>(p);
         raw[i] = u32x4{x[0], x[1], 0u, 0u};
@@ -140,7 +131,7 @@ struct KeyRows {
         raw[i] = *reinterpret_cast<const u32x4*>(p);
       }
     }
-    if constexpr (kCodes) scale = *sc;
+    if constexpr (kCodes) scale = *reinterpret_cast<const float*>(scales + soff);
   }
   __device__ inline void frags(frag (&f)[NKS]) const {
     if constexpr (!kCodes) {
@@ -236,24 +227,35 @@ struct ValueRows {
   u32x4 raw[NV];
   float scale[kCodes ? NV : 1];
 
-  __device__ static inline int row_of(int i, int lane) { return ((i * 64 + lane) / CPR) & (kUnit - 1); }
-  // `row(r)`: address of unit row r; `sc(r)`: of its scale.
-  template <typename RowFn, typename ScaleFn>
-  __device__ inline void load(RowFn row, ScaleFn sc, int lane) {
+  static constexpr int RPI = CPR > 2 ? 64 / CPR : kUnit;  // rows of a load (CPR 1: the upper lanes repeat them)
+
+  // `rows`: wave-uniform address of the unit's first row, rows `st` bytes apart,
+  // `lim` the last of them that exists (later ones read it); the scales alike.
+  __device__ inline void load(const char* rows, uint32_t st, const char* scales, uint32_t sst, int lim, int lane) {
+    const int r0 = (lane / CPR) & (kUnit - 1);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int r = row_of(i, lane);
-      raw[i] = *reinterpret_cast<const u32x4*>(row(r) + 16 * (lane % CPR));
-      if constexpr (kCodes) scale[i] = *sc(r);
+      int r = r0 + i * RPI;
+      if (lim < kUnit - 1) r = r < lim ? r : lim;
+      raw[i] = *reinterpret_cast<const u32x4*>(rows + (uint32_t)r * st + 16 * (lane % CPR));
+      if constexpr (kCodes) scale[i] = *reinterpret_cast<const float*>(scales + (uint32_t)r * sst);
     }
   }
   // A row that is not finite is staged as zeros; its factor is NaN, so that a
-  // live pair still sees it and a masked one does not.  (A finite row whose
-  // length overflows has factor 0.)
-  __device__ inline void stage(char* tile, float* fac, float eps, int lane) const {
+  // live pair still sees it and a masked one does not; then the result is true.
+  // (A finite row whose length overflows has factor 0.)  The factors are times
+  // kWeightUp.
+  __device__ inline bool stage(char* tile, float* fac, float eps, int lane) const {
     typedef typename Mma<comp>::frag vec;  // 16 bytes of an operand row
     constexpr int N = 16 / (int)sizeof(comp);
     constexpr int W = kCodes ? 2 : 1;      // operand chunks of a load
+    const int r0 = (lane / CPR) & (kUnit - 1), ch = W * (lane % CPR);
+    // lds_swz is linear over the row's bits, and r0 < RPI: the rows of load i
+    // differ from r0's place by constants
+    uint32_t at[W];
+#pragma unroll
+    for (int u = 0; u < W; ++u) at[u] = (uint32_t)(r0 * Tile::ROWB + (((ch + u) ^ Tile::swz(r0)) << 4));
+    bool odd = false;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       vec x[W];
@@ -272,18 +274,21 @@ struct ValueRows {
           for (int e = 0; e < N; ++e) ss = fmaf(x[u][e], x[u][e], ss);
       }
       ss = group_sum<CPR>(ss);
-      const bool finite = ss < INFINITY;
+      bool finite = ss < INFINITY;
+      if constexpr (kCodes) finite = finite && scale[i] == scale[i];
       float f;
       if constexpr (kCodes) f = KeyRows<C, D>::code_factor(ss, scale[i], eps);
       else f = inv_len_of<C>(ss, eps);
       if (__ballot(!finite) != 0ull) {
-        float bad = 0.0f;  // an element that is not finite, and not only their squares' sum
+        float bad = 0.0f;  // an element (or its scale) that is not finite, and not only the squares' sum
+        if constexpr (kCodes) bad = scale[i] == scale[i] ? 0.0f : 1.0f;
 #pragma unroll
         for (int u = 0; u < W; ++u)
 #pragma unroll
           for (int e = 0; e < N; ++e)
             if (!(fabsf(to_f(x[u][e])) < INFINITY)) bad = 1.0f;
         bad = group_sum<CPR>(bad);
+        odd = true;
         if (!finite) {
           f = bad > 0.0f ? __uint_as_float(0x7fc00000u) : 0.0f;
 #pragma unroll
@@ -312,15 +317,15 @@ struct ValueRows {
           f = sp.w;
         }
       }
-      const int r = row_of(i, lane), ch = W * (lane % CPR);
       const bool mine = kUnit * CPR >= 64 || lane < kUnit * CPR;
       if (mine) {
 #pragma unroll
         for (int u = 0; u < W; ++u)
-          *reinterpret_cast<vec*>(tile + r * Tile::ROWB + (((ch + u) ^ Tile::swz(r)) << 4)) = x[u];
-        if (lane % CPR == 0) fac[r] = f;
+          *reinterpret_cast<vec*>(tile + (at[u] ^ (uint32_t)(Tile::swz((i * RPI) & (kUnit - 1)) << 4)) + i * RPI * Tile::ROWB) = x[u];
+        if (lane % CPR == 0) fac[r0 + i * RPI] = f * kWeightUp<C>;
       }
     }
+    return odd;
   }
 };
 
@@ -475,8 +480,8 @@ struct TreeMap {
 
 // Block (x, y): piece x of sequence y, or all of head x.  The waves of a node
 // tile take every WPT-th unit of it.
-template <typename C, int D, int PARTS>
-__global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D, D * (int)sizeof(C), PARTS)) void tree_kernel(TreeCall a) {
+template <typename C, int D, int PARTS, int T>
+__global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C), PARTS * T)) void tree_kernel(TreeCall a) {
   using K = KeyRows<C, D>;
   using V = ValueRows<C, D>;
   using comp = typename K::comp;
@@ -484,17 +489,22 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D, D * (int)sizeof(
   using M = Mma<comp>;
   using Tile = typename V::Tile;
   constexpr int NDH = Tile::NDH, NC = Tile::NC;
-  constexpr bool kTwo = sizeof(comp) == 2;  // weights as two terms
-  constexpr bool kAhead = D * sizeof(C) <= AHEAD;  // registers for a unit of values in flight
-  constexpr int kRed = kUnit * V::DP * 4;   // a wave's sums
-  constexpr int kLds = kTreeWaves * (Tile::BYTES > kRed / 2 ? Tile::BYTES : kRed / 2);
+  constexpr bool kTwo = sizeof(comp) == 2;
+  // Weights as two terms of the operand's type.  One fp16 term (2^-12) is enough
+  // beside a result in bf16 (2^-9).
+  const bool two = kTwo && !(TreeRow<C>::kCodes && PARTS == 1 && a.q_dtype == 1);
+  constexpr bool kAhead = D * sizeof(C) * T <= 64;  // registers for a unit of values in flight
+  constexpr int kRed = kUnit * V::DP * 4;   // a wave's sums of a node tile
+  constexpr int kLds = kTreeWaves * (Tile::BYTES > T * kRed / 2 ? Tile::BYTES : T * kRed / 2);
   __shared__ __align__(16) char lds[kLds];
   __shared__ __align__(16) float kfac[kTreeWaves][kUnit], vfac[kTreeWaves][kUnit], mtab[kTreeWaves][128];
   __shared__ int dtab[kTreeWaves][kTreeMax];
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
+  const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.y;
-  const int tiles = (a.N + 31) / 32, wpt = kTreeWaves / tiles, tile = wave / wpt, kw = wave % wpt;
+  // T = 1: the block's waves share its node tiles, wpt of them to each
+  const int tiles = T == 2 ? 1 : (a.N + 31) / 32, wpt = kTreeWaves / tiles, tile = wave / wpt, kw = wave % wpt;
   const TreeSpan sp(a, b);
   int h = blockIdx.x, u0 = 0, per = 0;
   if (a.blocks != a.H) {
@@ -510,21 +520,22 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D, D * (int)sizeof(
   if (per == 0) per = units;
   const int u1 = u0 + per < units ? u0 + per : units;
 
-  const char* kb = (const char*)a.kc + (b * a.ks.sb + h * a.ks.sh) * (int64_t)sizeof(C);
-  const char* vb = (const char*)a.vc + (b * a.vs.sb + h * a.vs.sh) * (int64_t)sizeof(C);
   const int64_t kst = a.ks.st * (int64_t)sizeof(C), vst = a.vs.st * (int64_t)sizeof(C);
-  const float* ksc = a.kscale + b * a.kss.sb + h * a.kss.sh;
-  const float* vsc = a.vscale + b * a.vss.sb + h * a.vss.sh;
-  const int last = sp.n + a.N - 1;  // last key row
-
+  const char* kb = (const char*)a.kc + (b * a.ks.sb + h * a.ks.sh) * (int64_t)sizeof(C) + lo_key * kst;
+  const char* vb = (const char*)a.vc + (b * a.vs.sb + h * a.vs.sh) * (int64_t)sizeof(C) + lo_key * vst;
+  const char* ksc = (const char*)(a.kscale + b * a.kss.sb + h * a.kss.sh + lo_key * a.kss.st);
+  const char* vsc = (const char*)(a.vscale + b * a.vss.sb + h * a.vss.sh + lo_key * a.vss.st);
+  const int last = sp.n + a.N - 1 - lo_key;  // last key row, from the window's first
   auto load_keys = [&](K& key, int u) {
-    const int j = lo_key + u * kUnit + perm_row(l32), c = j < last ? j : last;
-    key.load(kb + c * kst, ksc + c * a.kss.st, half);
+    int r = perm_row(l32);
+    const int lim = last - u * kUnit;
+    if (lim < kUnit - 1) r = r < lim ? r : lim;
+    key.load(kb + (int64_t)u * kUnit * kst, (uint32_t)r * (uint32_t)kst + half * K::LB,
+             ksc + (int64_t)u * kUnit * a.kss.st * 4, (uint32_t)r * (uint32_t)(a.kss.st * 4));
   };
   auto load_values = [&](V& val, int u) {
-    const int k0 = lo_key + u * kUnit;
-    val.load([&](int r) { return vb + (int64_t)(k0 + r < last ? k0 + r : last) * vst; },
-             [&](int r) { return vsc + (int64_t)(k0 + r < last ? k0 + r : last) * a.vss.st; }, lane);
+    val.load(vb + (int64_t)u * kUnit * vst, (uint32_t)vst, vsc + (int64_t)u * kUnit * a.vss.st * 4,
+             (uint32_t)(a.vss.st * 4), last - u * kUnit, lane);
   };
   // rows in flight: the next unit's keys, and its values where the last unit
   // had a live pair (a head's first units are taken to be live if it has few)
@@ -536,18 +547,20 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D, D * (int)sizeof(
 
   const Tree tree(a.parents == nullptr ? nullptr : a.parents + b * a.par_sb, a.N, lane);
   dtab[wave][lane] = tree.depth;
-  const int node = 32 * tile + l32;
-  const int depth = __shfl(tree.depth, node);
-  const unsigned long long above =
-      ((unsigned long long)(uint32_t)__shfl((int)(tree.above >> 32), node) << 32) | (uint32_t)__shfl((int)tree.above, node);
-
-  NodeRows<C, D, PARTS> q;
-  {
-    const bool ok = node < a.N;
-    const int64_t off = b * a.q_sb + (int64_t)(ok ? node : 0) * a.q_sn + h * a.q_sh;
-    if (a.q_dtype == 1) q.load((const bf16*)a.q + off, ok, a.eps, half);
-    else if (a.q_dtype == 2) q.load((const f16*)a.q + off, ok, a.eps, half);
-    else q.load((const float*)a.q + off, ok, a.eps, half);
+  int node[T], depth[T];
+  unsigned long long above[T];
+  NodeRows<C, D, PARTS> q[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    node[t] = 32 * (T == 2 ? t : tile) + l32;
+    depth[t] = __shfl(tree.depth, node[t]);
+    above[t] = ((unsigned long long)(uint32_t)__shfl((int)(tree.above >> 32), node[t]) << 32) |
+               (uint32_t)__shfl((int)tree.above, node[t]);
+    const bool ok = node[t] < a.N;
+    const int64_t off = b * a.q_sb + (int64_t)(ok ? node[t] : 0) * a.q_sn + h * a.q_sh;
+    if (a.q_dtype == 1) q[t].load((const bf16*)a.q + off, ok, a.eps, half);
+    else if (a.q_dtype == 2) q[t].load((const f16*)a.q + off, ok, a.eps, half);
+    else q[t].load((const float*)a.q + off, ok, a.eps, half);
   }
 
   char* vt = lds + wave * Tile::BYTES;
@@ -557,11 +570,13 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D, D * (int)sizeof(
       *reinterpret_cast<u32x4*>(vt + i * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
   }
   const uint32_t cbase = Tile::col_base(lane);
-  f32x16 acc[NDH];
+  f32x16 acc[T][NDH];
 #pragma unroll
-  for (int d = 0; d < NDH; ++d)
+  for (int t = 0; t < T; ++t)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
+    for (int d = 0; d < NDH; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[t][d][r] = 0.0f;
 
   const int depth_max = a.parents == nullptr ? a.N - 1 : wave_max(tree.depth);
   for (int u = u0 + kw; u < u1; u += wpt) {
@@ -576,26 +591,36 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D, D * (int)sizeof(
     key.frags(kf);
     const float f = key.factor(kf, a.eps);
     if (half == 0) kfac[wave][perm_row(l32)] = f;
-    f32x16 s = unit_product<comp, K::NKS>(kf, q.f[0]);
-    if constexpr (PARTS == 2) {
-      const f32x16 s2 = unit_product<comp, K::NKS>(kf, q.f[1]);
+    f32x16 s[T];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] += s2[r];
+    for (int t = 0; t < T; ++t) {
+      s[t] = unit_product<comp, K::NKS>(kf, q[t].f[0]);
+      if constexpr (PARTS == 2) {
+        const f32x16 s2 = unit_product<comp, K::NKS>(kf, q[t].f[1]);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] += s2[r];
+      }
     }
-    guard_all(kf, s);
+    guard_all(kf, s[T - 1]);
     wave_lds_sync();
     float x[16];
     read_row_scales(kfac[wave], half, x);
-    float top = -INFINITY;
+    bool vote = false;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] *= x[r];
-      top = fmaxf(top, s[r]);
+    for (int t = 0; t < T; ++t) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[t][r] *= x[r];
+        top = fmaxf(top, s[t][r]);
+      }
+      vote = vote || top * q[t].inv > hp.thr;
     }
     ahead = false;
-    if (__ballot(top * q.inv > hp.thr) == 0ull) continue;
+    if (__ballot(vote) == 0ull) continue;
 
-    // a^2 m of every pair: register r is key row 16 (r/8) + 8 half + r%8
+    // a^2 m of every pair: register r is key row 16 (r/8) + 8 half + r%8 (the
+    // clamp takes a NaN to 0)
     float any = 0.0f;
     if (k0 + kUnit <= sp.n) {
       // committed keys: m from a table over depth - row (entry e: distance n - k0 - 31 + e)
@@ -603,42 +628,63 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D, D * (int)sizeof(
       for (int e = lane; e < 32 + depth_max; e += 64)
         mtab[wave][e] = in_window(dmin + e, hp) ? mask_fast(dmin + e, hp.w, hp.iw) : 0.0f;
       wave_lds_sync();
-      const float* mt = mtab[wave] + (depth + 8 - 8 * half);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float av = fmaxf(fmaf(-hp.r, fmaf(-s[r], q.inv, 1.0f), 1.0f), 0.0f);
-        s[r] = av * av * mt[23 - 16 * (r >> 3) - (r & 7)];
-        any = fmaxf(any, s[r]);
+      for (int t = 0; t < T; ++t) {
+        const float* mt = mtab[wave] + (depth[t] + 8 - 8 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float av = __builtin_amdgcn_fmed3f(fmaf(-hp.r, fmaf(-s[t][r], q[t].inv, 1.0f), 1.0f), 0.0f, 1.0f);
+          s[t][r] = av * av * mt[23 - 16 * (r >> 3) - (r & 7)];
+          any = fmaxf(any, s[t][r]);
+        }
       }
     } else {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = 16 * (r >> 3) + 8 * half + (r & 7), j = k0 + row - sp.n;  // j >= 0: drafted
-        const bool draft = j >= 0;
-        const int dd = depth - (draft ? dtab[wave][j & (kTreeMax - 1)] : j);
-        const bool seen = draft ? j < a.N && ((above >> j) & 1ull) != 0ull : true;
-        const float av = fmaxf(fmaf(-hp.r, fmaf(-s[r], q.inv, 1.0f), 1.0f), 0.0f);
-        s[r] = seen && in_window(dd, hp) ? av * av * mask_fast(dd, hp.w, hp.iw) : 0.0f;
-        any = fmaxf(any, s[r]);
-      }
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = 16 * (r >> 3) + 8 * half + (r & 7), j = k0 + row - sp.n;  // j >= 0: drafted
+          const bool draft = j >= 0;
+          const int dd = depth[t] - (draft ? dtab[wave][j & (kTreeMax - 1)] : j);
+          const bool seen = draft ? j < a.N && ((above[t] >> (j & 63)) & 1ull) != 0ull : true;
+          const float av = __builtin_amdgcn_fmed3f(fmaf(-hp.r, fmaf(-s[t][r], q[t].inv, 1.0f), 1.0f), 0.0f, 1.0f);
+          s[t][r] = seen && in_window(dd, hp) ? av * av * mask_fast(dd, hp.w, hp.iw) : 0.0f;
+          any = fmaxf(any, s[t][r]);
+        }
     }
     if (__ballot(any > 0.0f) == 0ull) continue;
 
     ahead = kAhead;
     if (!have) load_values(val, u);
-    val.stage(vt, vfac[wave], a.eps, lane);
+    const bool odd = val.stage(vt, vfac[wave], a.eps, lane);
     wave_lds_sync();
     read_row_scales(vfac[wave], half, x);
+    frag hi[T][NC], lo[T][kTwo ? NC : 1];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = s[r] > 0.0f ? s[r] * x[r] * kWeightUp<C> : 0.0f;
-    frag hi[NC], lo[kTwo ? NC : 1];
+    for (int t = 0; t < T; ++t) {
+      if (odd) {  // a NaN factor reaches live pairs only
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      hi[c] = M::pack(s, M::PER * c);
-      if constexpr (kTwo) {
+        for (int r = 0; r < 16; ++r) s[t][r] = s[t][r] > 0.0f ? s[t][r] * x[r] : 0.0f;
+      } else {
 #pragma unroll
-        for (int e = 0; e < M::PER; ++e) s[M::PER * c + e] -= M::get(hi[c], e);
-        lo[c] = M::pack(s, M::PER * c);
+        for (int r = 0; r < 16; ++r) s[t][r] *= x[r];
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        hi[t][c] = M::pack(s[t], M::PER * c);
+        // one rounding for both uses below: formed anew from the factors it may be
+        // rounded once instead of twice, and the second term would not be its rest
+        asm volatile("" : "+v"(hi[t][c]));
+      }
+      if (two) {
+        if constexpr (kTwo) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+#pragma unroll
+            for (int e = 0; e < M::PER; ++e) s[t][M::PER * c + e] -= M::get(hi[t][c], e);
+            lo[t][c] = M::pack(s[t], M::PER * c);
+          }
+        }
       }
     }
 #pragma unroll
@@ -647,62 +693,77 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D, D * (int)sizeof(
 #pragma unroll
       for (int c = 0; c < NC; ++c) vf[c] = Tile::col_frag(vt, cbase, d, c);
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        acc[d] = M::mma_ng(vf[c], hi[c], acc[d]);
-        if constexpr (kTwo) acc[d] = M::mma_ng(vf[c], lo[c], acc[d]);
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int t = 0; t < T; ++t) acc[t][d] = M::mma_ng(vf[c], hi[t][c], acc[t][d]);
+      if (two) {
+        if constexpr (kTwo) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int t = 0; t < T; ++t) acc[t][d] = M::mma_ng(vf[c], lo[t][c], acc[t][d]);
+        }
       }
-      guard_all(vf, acc[d]);
+#pragma unroll
+      for (int t = 0; t < T; ++t) guard_all(vf, acc[t][d]);
     }
-    guard_all(hi, acc[NDH - 1]);
-    guard_all(lo, acc[NDH - 1]);
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      guard_all(hi[t], acc[t][NDH - 1]);
+      if constexpr (kTwo) guard_all(lo[t], acc[t][NDH - 1]);
+    }
   }
 
   // the waves of a tile, the upper half of them into the lower, until one has all
-  char* red = nullptr;
-  auto put = [&] {
-#pragma unroll
-    for (int d = 0; d < NDH; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(red + (4 * d + g) * 1024 + lane * 16) =
-            f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
-  };
-  auto add = [&] {
-#pragma unroll
-    for (int d = 0; d < NDH; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(red + (4 * d + g) * 1024 + lane * 16);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[d][4 * g + e] += x[e];
-      }
-  };
   for (int step = wpt / 2; step >= 1; step /= 2) {
-    red = lds + (tile * step + kw % step) * kRed;
+    char* red = lds + (tile * step + kw % step) * (T * kRed) + lane * 16;
     __syncthreads();
-    if (kw >= step && kw < 2 * step) put();
+    if (kw >= step && kw < 2 * step) {
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int d = 0; d < NDH; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4*>(red + ((t * NDH + d) * 4 + g) * 1024) =
+                f32x4{acc[t][d][4 * g], acc[t][d][4 * g + 1], acc[t][d][4 * g + 2], acc[t][d][4 * g + 3]};
+    }
     __syncthreads();
-    if (kw < step) add();
+    if (kw < step) {
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int d = 0; d < NDH; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x4 y = *reinterpret_cast<const f32x4*>(red + ((t * NDH + d) * 4 + g) * 1024);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[t][d][4 * g + e] += y[e];
+          }
+    }
   }
   if (kw != 0) return;
-  if (node >= a.N) return;  // lanes l and l + 32 share a node
   constexpr float down = 1.0f / kWeightUp<C>;
-  if (a.blocks != a.H) {
-    float* p = a.part + (((int64_t)b * a.blocks + blockIdx.x) * a.N + node) * D;
-    store_row<comp, float, D>(p, half, [&](int d, int r) { return acc[d][r] * down; });
-    return;
-  }
-  float ss = 0.0f;
 #pragma unroll
-  for (int d = 0; d < NDH; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      acc[d][r] *= down;
-      ss = fmaf(acc[d][r], acc[d][r], ss);
+  for (int t = 0; t < T; ++t) {
+    if (node[t] >= a.N) continue;  // lanes l and l + 32 share a node
+    if (a.blocks != a.H) {
+      float* p = a.part + (((int64_t)b * a.blocks + blockIdx.x) * a.N + node[t]) * D;
+      store_row<comp, float, D>(p, half, [&](int d, int r) { return acc[t][d][r] * down; });
+      continue;
     }
-  const float nc = fmaxf(sqrtf(half_sum(ss)), a.eps), fy = tanhf(nc) / nc;
-  store_row_as<comp, D>(a.y, (((int64_t)b * a.N + node) * a.H + h) * D, a.q_dtype, half,
-                        [&](int d, int r) { return acc[d][r] * fy; });
+    float ss = 0.0f;
+#pragma unroll
+    for (int d = 0; d < NDH; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        acc[t][d][r] *= down;
+        ss = fmaf(acc[t][d][r], acc[t][d][r], ss);
+      }
+    const float nc = fmaxf(sqrtf(half_sum(ss)), a.eps), fy = tanhf(nc) / nc;
+    store_row_as<comp, D>(a.y, (((int64_t)b * a.N + node[t]) * a.H + h) * D, a.q_dtype, half,
+                          [&](int d, int r) { return acc[t][d][r] * fy; });
+  }
 }
 
 // Sum of a node's block sums and TanhNorm: a wave per node, D/4 lanes for a
@@ -735,6 +796,9 @@ __global__ __launch_bounds__(256) void tree_reduce_kernel(TreeCall a) {
 }
 
 int tree_max_nodes() { return kTreeMax; }
+// Whether a wave takes all of more than 32 nodes: its registers hold two tiles'
+// operands and sums for rows of at most 64 values in 2-byte operands.
+bool tree_both(int N, int D, bool f32) { return N > 32 && D <= 64 && !f32; }
 // Blocks of a sequence: as many as run at one time on the card's 256 CUs share
 // its heads' keys; one a head (H) where heads are short, or the batch alone
 // fills the card several times over with heads that are not long.
@@ -742,27 +806,35 @@ int tree_blocks(int B, int H, int N, int D, int q_dtype, int cache_dtype, int sp
   const int64_t units = ((int64_t)span + N + kUnit - 1) / kUnit;
   const bool codes = cache_dtype == kInt8 || cache_dtype == kFp8;
   const int row = D * (codes ? 1 : cache_dtype == 0 ? 4 : 2);
-  const int slots = 256 * tree_occupancy(D, row, codes && q_dtype == 0 ? 2 : 1);
+  const bool f32 = codes ? q_dtype == 0 : cache_dtype == 0;
+  const int slots = 256 * tree_occupancy(row, codes && q_dtype == 0 ? 2 : tree_both(N, D, f32) ? 2 : 1);
   if (units <= kTreeSmall || ((int64_t)B * H >= 2 * slots && units <= 4 * kTreeSmall)) return H;
   const int each = slots / B;
   return each < 2 * H ? 2 * H : each;
 }
 
-template <typename C, int D, int PARTS>
+template <typename C, int D, int PARTS, int T>
 static hipError_t launch_tree_t(const TreeCall& c) {
-  hipLaunchKernelGGL((tree_kernel<C, D, PARTS>), dim3((unsigned)c.blocks, (unsigned)c.B), dim3(64 * kTreeWaves), 0, c.stream, c);
+  hipLaunchKernelGGL((tree_kernel<C, D, PARTS, T>), dim3((unsigned)c.blocks, (unsigned)c.B), dim3(64 * kTreeWaves), 0, c.stream, c);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || c.blocks == c.H) return e;
   hipLaunchKernelGGL((tree_reduce_kernel<D>), dim3((unsigned)((c.N + 3) / 4), (unsigned)(c.B * c.H)), dim3(256), 0, c.stream, c);
   return hipGetLastError();
 }
+template <typename C, int D, int PARTS>
+static hipError_t launch_tree_n(const TreeCall& c) {
+  constexpr bool f32 = PARTS == 2 || __is_same(C, float);
+  if constexpr (D <= 64 && !f32)
+    if (tree_both(c.N, D, f32)) return launch_tree_t<C, D, PARTS, 2>(c);
+  return launch_tree_t<C, D, PARTS, 1>(c);
+}
 template <typename C, int PARTS>
 static hipError_t launch_tree_d(const TreeCall& c) {
   switch (c.D) {
-    case 16: return launch_tree_t<C, 16, PARTS>(c);
-    case 32: return launch_tree_t<C, 32, PARTS>(c);
-    case 64: return launch_tree_t<C, 64, PARTS>(c);
-    default: return launch_tree_t<C, 128, PARTS>(c);
+    case 16: return launch_tree_n<C, 16, PARTS>(c);
+    case 32: return launch_tree_n<C, 32, PARTS>(c);
+    case 64: return launch_tree_n<C, 64, PARTS>(c);
+    default: return launch_tree_n<C, 128, PARTS>(c);
   }
 }
 hipError_t launch_tree(const TreeCall& c) {
