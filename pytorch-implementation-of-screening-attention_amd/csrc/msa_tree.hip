@@ -493,7 +493,6 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C),
   // Weights as two terms of the operand's type.  One fp16 term (2^-12) is enough
   // beside a result in bf16 (2^-9).
   const bool two = kTwo && !(TreeRow<C>::kCodes && PARTS == 1 && a.q_dtype == 1);
-  constexpr bool kAhead = D * sizeof(C) * T <= 64;  // registers for a unit of values in flight
   constexpr int kRed = kUnit * V::DP * 4;   // a wave's sums of a node tile
   constexpr int kLds = kTreeWaves * (Tile::BYTES > T * kRed / 2 ? Tile::BYTES : T * kRed / 2);
   __shared__ __align__(16) char lds[kLds];
@@ -537,13 +536,12 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C),
     val.load(vb + (int64_t)u * kUnit * vst, (uint32_t)vst, vsc + (int64_t)u * kUnit * a.vss.st * 4,
              (uint32_t)(a.vss.st * 4), last - u * kUnit, lane);
   };
-  // rows in flight: the next unit's keys, and its values where the last unit
-  // had a live pair (a head's first units are taken to be live if it has few)
+  // Keys are in flight a unit ahead; values are asked for once the vote has
+  // found a live pair and arrive behind its weights.  (Asked for with the keys
+  // where the last unit was live, they cost registers: 4 x 64 nodes over 30K bf16
+  // 106 instead of 70 us, chain of 8 over 16K int8 53 instead of 50.)
   K key_next;
-  V val_next;
-  bool ahead = kAhead && per <= 4 * wpt, issued = ahead && u0 + kw < u1;
   if (u0 + kw < u1) load_keys(key_next, u0 + kw);
-  if (issued) load_values(val_next, u0 + kw);
 
   const Tree tree(a.parents == nullptr ? nullptr : a.parents + b * a.par_sb, a.N, lane);
   dtab[wave][lane] = tree.depth;
@@ -582,11 +580,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C),
   for (int u = u0 + kw; u < u1; u += wpt) {
     const int k0 = lo_key + u * kUnit;  // position of the unit's first row (a drafted row: n + its node)
     const K key = key_next;
-    V val = val_next;
-    const bool have = issued;
-    issued = ahead && u + wpt < u1;
     if (u + wpt < u1) load_keys(key_next, u + wpt);
-    if (issued) load_values(val_next, u + wpt);
     frag kf[K::NKS];
     key.frags(kf);
     const float f = key.factor(kf, a.eps);
@@ -616,8 +610,9 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C),
       }
       vote = vote || top * q[t].inv > hp.thr;
     }
-    ahead = false;
     if (__ballot(vote) == 0ull) continue;
+    V val;
+    load_values(val, u);
 
     // a^2 m of every pair: register r is key row 16 (r/8) + 8 half + r%8 (the
     // clamp takes a NaN to 0)
@@ -654,8 +649,6 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C),
     }
     if (__ballot(any > 0.0f) == 0ull) continue;
 
-    ahead = kAhead;
-    if (!have) load_values(val, u);
     const bool odd = val.stage(vt, vfac[wave], a.eps, lane);
     wave_lds_sync();
     read_row_scales(vfac[wave], half, x);
