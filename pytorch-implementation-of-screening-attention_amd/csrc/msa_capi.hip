@@ -585,7 +585,7 @@ int msa_tree_decode(const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh, con
 
 size_t msa_verify_workspace_bytes(int B, int M, int64_t V, int greedy) {
   if (!greedy || B <= 0 || M <= 0 || M > MSA_TREE_MAX || V <= 0 || V > 0x7fffffff) return 0;
-  return (size_t)B * M * msa::verify_parts(B, M, (int)V) * sizeof(unsigned long long);
+  return (size_t)B * M * msa::verify_parts(V) * sizeof(unsigned long long);
 }
 
 int msa_verify(const void* target, int64_t t_sb, int64_t t_sn, const void* draft, int64_t d_sb, int64_t d_sn,

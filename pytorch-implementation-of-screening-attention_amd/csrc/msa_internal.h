@@ -154,7 +154,7 @@ struct VerifyCall {
   unsigned long long* best;                // greedy: [b*M + i][part] keys
   hipStream_t stream;
 };
-int verify_parts(int B, int M, int V);
+int verify_parts(int64_t V);
 hipError_t launch_verify(const VerifyCall& c);
 
 // Waves that share a row (32-query or 32-key unit) in the live, dq and dK/dV

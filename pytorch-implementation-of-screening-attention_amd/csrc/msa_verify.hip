@@ -23,6 +23,7 @@
 
 namespace msa {
 
+constexpr int kPart = 8192;  // entries of a block of the greedy pass
 constexpr int kVerifyThreads = 1024, kVerifyWaves = kVerifyThreads / 64;
 
 // VEC consecutive entries of a row as fp32, from an address of any alignment
@@ -74,33 +75,61 @@ __device__ inline double shfl_d(double x, int l) {
                                           (uint32_t)__shfl((int)b, l)));
 }
 
-// The largest entry of part blockIdx.y of row blockIdx.x = b M + i.
+// The largest entry of part blockIdx.y (kPart entries) of row blockIdx.x = b M +
+// i.  A thread holds its entries in registers: their maximum first (NaN noted
+// apart), and once the block's is known, its place in the threads that have it.
 template <typename T>
 __global__ __launch_bounds__(256) void argmax_kernel(VerifyCall a) {
-  constexpr int N = RowLoad<T>::N;
+  constexpr int N = RowLoad<T>::N, U = kPart / (256 * N);
   __shared__ unsigned long long red[4];
   const int b = blockIdx.x / a.M, i = blockIdx.x % a.M;
   const T* row = (const T*)a.target + b * a.t_sb + i * a.t_sn;
-  const int64_t len = ((a.V + gridDim.y - 1) / gridDim.y + N - 1) / N * N;
-  const int64_t lo = len * blockIdx.y, hi = lo + len < a.V ? lo + len : a.V;
-  unsigned long long best = 0ull;
-  for (int64_t v = lo + threadIdx.x * N; v < hi; v += 256 * N) {
-    float x[N];
-    load_row(row, v, a.V, x, 0.0f);
+  const int64_t v0 = (int64_t)blockIdx.y * kPart + threadIdx.x * N;
+  float x[U][N];
+  if ((int64_t)(blockIdx.y + 1) * kPart <= a.V) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const auto y = *reinterpret_cast<const typename RowLoad<T>::vec*>(row + v0 + u * 256 * N);
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[u][e] = (float)y[e];
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_row(row, v0 + u * 256 * N, a.V, x[u], -INFINITY);
+  }
+  float top = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const unsigned long long k = v + e < a.V ? arg_key(x[e], (uint32_t)(v + e)) : 0ull;
-      best = k > best ? k : best;
+      top = fmaxf(top, x[u][e]);
+      nan = nan || x[u][e] != x[u][e];
     }
+  float m = nan ? NAN : top;
+  // the wave's, then the first place of it in the wave
+  bool wnan = __ballot(nan) != 0ull;
+  float wtop = top;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) wtop = fmaxf(wtop, __shfl_xor(wtop, o));
+  uint32_t at = 0xffffffffu;
+  if (wnan ? nan : m == wtop) {
+#pragma unroll
+    for (int u = U - 1; u >= 0; --u)
+#pragma unroll
+      for (int e = N - 1; e >= 0; --e)
+        if (wnan ? x[u][e] != x[u][e] : x[u][e] == wtop) at = (uint32_t)(v0 + u * 256 * N + e);
+    if (at >= a.V) at = 0xffffffffu;  // behind the row (all of its entries are -inf)
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const unsigned long long k = shfl_xor64(best, o);
-    best = k > best ? k : best;
+    const uint32_t y = (uint32_t)__shfl_xor((int)at, o);
+    at = y < at ? y : at;
   }
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = best;
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = at == 0xffffffffu ? 0ull : arg_key(wnan ? NAN : wtop, at);
   __syncthreads();
   if (threadIdx.x == 0) {
+    unsigned long long best = red[0];
 #pragma unroll
     for (int w = 1; w < 4; ++w) best = red[w] > best ? red[w] : best;
     a.best[(int64_t)blockIdx.x * gridDim.y + blockIdx.y] = best;
@@ -119,7 +148,22 @@ struct Nodes {
     const int64_t p = a.parents == nullptr ? lane - 1 : (in ? a.parents[b * a.par_sb + lane] : -1);
     parent = in && p >= 0 && p < lane ? (int)p : -1;
   }
+  // The nodes before this one under the same parent (nodes without one: none),
+  // by the bits of the parents.
+  __device__ unsigned long long before(int lane) const {
+    unsigned long long m = __ballot(parent >= 0);
+#pragma unroll
+    for (int k = 0; k < 6; ++k) {
+      const bool bit = ((parent >> k) & 1) != 0;
+      const unsigned long long on = __ballot(bit);
+      m &= bit ? on : ~on;
+    }
+    return parent >= 0 ? m & ((1ull << lane) - 1ull) : 0ull;
+  }
 };
+__device__ inline int64_t shfl_i64(int64_t x, int l) {
+  return ((int64_t)__shfl((int)(x >> 32), l) << 32) | (uint32_t)__shfl((int)x, l);
+}
 
 // The way down from node 0 over nodes taken (at most one child of each), into
 // path (-1 behind it) and count.  Returns the last node.  Wave-wide.
@@ -143,6 +187,7 @@ __global__ __launch_bounds__(64) void greedy_walk_kernel(VerifyCall a, int parts
   const Nodes n(a, b, lane);
   unsigned long long best = 0ull;
   if (lane < a.M)
+#pragma unroll 8
     for (int s = 0; s < parts; ++s) {
       const unsigned long long k = a.best[((int64_t)b * a.M + lane) * parts + s];
       best = k > best ? k : best;
@@ -150,12 +195,7 @@ __global__ __launch_bounds__(64) void greedy_walk_kernel(VerifyCall a, int parts
   const int top = (int)(0xffffffffu - (uint32_t)best);  // V <= 2^31
   const int want = __shfl(top, n.parent < 0 ? 0 : n.parent);
   bool taken = n.parent >= 0 && n.token == want;
-  const unsigned long long hit = __ballot(taken);
-  // the first of the siblings that have the token
-  for (int j = 0; j < a.M; ++j) {
-    const int p = __builtin_amdgcn_readlane(n.parent, j);
-    if (j < lane && p == n.parent && ((hit >> j) & 1ull) != 0ull) taken = false;
-  }
+  if ((__ballot(taken) & n.before(lane)) != 0ull) taken = false;  // the first of the siblings that have the token
   const int last = walk(a, b, lane, n, taken);
   const int tok = __shfl(top, last);
   if (lane == 0) a.token[b] = tok;
@@ -171,8 +211,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyCall a) {
   __shared__ int last_s, gone_s;
   __shared__ unsigned long long first_s, tail_s;
   const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  int shift = 0;
-  while ((a.V >> shift) > 4096) ++shift;
+  const double u0 = (double)a.uniforms[(int64_t)b * a.M];
+  int shift = 3;  // a stretch holds whole loads
+  while ((a.V >> shift) > 4095) ++shift;
   if (t < 128) bins[t] = 0u;
   if (t == 0) {
     first_s = ~0ull;
@@ -192,19 +233,16 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyCall a) {
       taken = on && (double)u * q < p;
     } else {
       if (!(p > 0.0)) p = 0.0;
+      const unsigned long long before = asked ? n.before(lane) : 0ull;
+      // a token that an earlier sibling had counts once
+      for (unsigned long long m = before; __ballot(m != 0ull) != 0ull; m &= m - 1ull) {
+        const int64_t tok = shfl_i64(n.token, m != 0ull ? (int)__builtin_ctzll(m) : lane);
+        if (m != 0ull && tok == n.token) p = 0.0;
+      }
       double left = 1.0;
-      unsigned long long before = 0ull;  // earlier siblings
-      for (int j = 1; j < a.M; ++j) {
-        const int pj = __builtin_amdgcn_readlane(n.parent, j);
-        if (pj < 0) continue;
-        const int64_t tj = ((int64_t)__builtin_amdgcn_readlane((int)(n.token >> 32), j) << 32) |
-                           (uint32_t)__builtin_amdgcn_readlane((int)n.token, j);
-        const double share = shfl_d(p, j);
-        if (j < lane && pj == n.parent) {
-          before |= 1ull << j;
-          if (tj == n.token) p = 0.0;
-          else left -= share;
-        }
+      for (unsigned long long m = before; __ballot(m != 0ull) != 0ull; m &= m - 1ull) {
+        const double share = shfl_d(p, m != 0ull ? (int)__builtin_ctzll(m) : lane);
+        if (m != 0ull) left -= share;
       }
       taken = asked && (double)u * left < p;
       if ((__ballot(taken) & before) != 0ull) taken = false;
@@ -228,34 +266,35 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyCall a) {
   const T* qrow = kChain && last < a.M - 1 ? (const T*)a.draft + b * a.d_sb + (int64_t)last * a.d_sn : nullptr;
   bool plain = false;  // the second time, if nothing is left: p itself
 
-  // weights of entries v .. v + N - 1 (0 behind the row)
-  auto weights = [&](int64_t v, double (&x)[N]) {
-    float p[N];
-    load_row(prow, v, a.V, p, 0.0f);
-#pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = p[e] > 0.0f ? (double)p[e] : 0.0;
-    if (plain) return;
-    if constexpr (kChain) {
-      if (qrow == nullptr) return;
-      float q[N];
-      load_row(qrow, v, a.V, q, 0.0f);
+  typedef typename RowLoad<T>::vec vec;
+  // weights of entries v .. v + N - 1 (v a multiple of N) with probabilities p
+  // (and the draft's q)
+  auto weigh = [&](int64_t v, const float (&p)[N], const float (&q)[N], double (&x)[N]) {
+    if (kChain && qrow != nullptr && !plain) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const double d = (double)p[e] - (double)q[e];
         x[e] = d > 0.0 ? d : 0.0;
       }
-    } else {
-      const uint32_t b0 = (uint32_t)(v >> shift), b1 = (uint32_t)((v + N - 1) >> shift);
-      bool some = false;
-      for (uint32_t c = b0; c <= b1 && c < 4096u; ++c) some = some || ((bins[c >> 5] >> (c & 31u)) & 1u) != 0u;
-      if (some)
-        for (int j = 0; j < ngone; ++j) {
-          const int64_t g = gone[j];
-#pragma unroll
-          for (int e = 0; e < N; ++e)
-            if (v + e == g) x[e] = 0.0;
-        }
+      return;
     }
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = (double)fmaxf(p[e], 0.0f);  // a NaN counts as 0
+    if (kChain || plain) return;
+    const uint32_t bin = (uint32_t)(v >> shift);
+    if (((bins[bin >> 5] >> (bin & 31u)) & 1u) != 0u)
+      for (int j = 0; j < ngone; ++j) {
+        const int64_t g = gone[j];
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (v + e == g) x[e] = 0.0;
+      }
+  };
+  auto weights = [&](int64_t v, double (&x)[N]) {  // the row ends at V
+    float p[N], q[N];
+    load_row(prow, v, a.V, p, 0.0f);
+    if (kChain && qrow != nullptr) load_row(qrow, v, a.V, q, 0.0f);
+    weigh(v, p, q, x);
   };
 
   // sums of the row's sixteenths, one a wave
@@ -265,9 +304,36 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyCall a) {
     plain = pass == 1;
     const int64_t lo = len * wave, hi = lo + len < a.V ? lo + len : a.V;
     double s = 0.0;
-    for (int64_t v = lo + lane * N; v < hi; v += 64 * N) {
+    constexpr int U = 32 / N;  // loads in flight
+    for (int64_t v0 = lo + lane * N; v0 < hi; v0 += U * 64 * N) {
+      vec p[U], q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t v = v0 + u * 64 * N;
+        p[u] = q[u] = vec(0);
+        if (v + N <= hi) {
+          p[u] = *reinterpret_cast<const vec*>(prow + v);
+          if (kChain && qrow != nullptr) q[u] = *reinterpret_cast<const vec*>(qrow + v);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float pf[N], qf[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          pf[e] = (float)p[u][e];
+          qf[e] = (float)q[u][e];
+        }
+        double x[N];
+        weigh(v0 + u * 64 * N, pf, qf, x);
+#pragma unroll
+        for (int e = 0; e < N; ++e) s += x[e];
+      }
+    }
+    const int64_t rest = lo + (hi - lo) / N * N;  // the row's last entries, fewer than a load
+    if (lane == 0 && rest < hi) {
       double x[N];
-      weights(v, x);
+      weights(rest, x);
 #pragma unroll
       for (int e = 0; e < N; ++e) s += x[e];
     }
@@ -284,7 +350,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyCall a) {
     for (int w = 0; w < kVerifyWaves; ++w) total += seg[w];
     if (total > 0.0) break;
   }
-  const double want = (double)a.uniforms[(int64_t)b * a.M] * total;
+  const double want = u0 * total;
   // the first sixteenth whose sums pass `want`, else the last with any weight
   int at = -1;
   double base = 0.0, run = 0.0;
@@ -335,26 +401,21 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyCall a) {
         tail = (unsigned long long)(v + e) + 1ull;
       }
   }
-  if (first != ~0ull) atomicMin(&first_s, first);
-  if (tail != 0ull) atomicMax(&tail_s, tail);
+  // entries grow with the lanes: the wave's first and last
+  const unsigned long long some = __ballot(first != ~0ull), rest = __ballot(tail != 0ull);
+  if (some != 0ull && lane == (int)__builtin_ctzll(some)) atomicMin(&first_s, first);
+  if (rest != 0ull && lane == 63 - (int)__builtin_clzll(rest)) atomicMax(&tail_s, tail);
   __syncthreads();
   if (t == 0) a.token[b] = first_s != ~0ull ? (int64_t)first_s : (int64_t)tail_s - 1;
 }
 
-// Parts of a row in the greedy pass: about four blocks per CU in all, each with
-// 4096 entries at least.
-int verify_parts(int B, int M, int V) {
-  const int64_t rows = (int64_t)B * M;
-  int64_t p = (1024 + rows - 1) / rows;
-  const int64_t most = (V + 4095) / 4096;
-  p = p < most ? p : most;
-  return (int)(p < 1 ? 1 : p);
-}
+// Parts of a row in the greedy pass.
+int verify_parts(int64_t V) { return (int)((V + kPart - 1) / kPart); }
 
 template <typename T>
 static hipError_t launch_verify_t(const VerifyCall& c) {
   if (c.uniforms == nullptr) {
-    const int parts = verify_parts(c.B, c.M, (int)c.V);
+    const int parts = verify_parts(c.V);
     hipLaunchKernelGGL((argmax_kernel<T>), dim3((unsigned)(c.B * c.M), (unsigned)parts), dim3(256), 0, c.stream, c);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
