@@ -3,8 +3,7 @@
 //
 // A quantised row x of D values is kept as D codes and the fp32 scale A/TOP,
 // A = max|x| and TOP the type's largest code (127; 448 for e4m3).  A code is the
-// nearest one to TOP x / A, ties to the even one, exactly: the fp32 quotient
-// decides unless a border lies within its error, and 64 bits decide then.  So
+// nearest one to TOP x / A, ties to the even one, exactly (codes_of).  So
 // the codes depend on nothing but the row: a row written twice, or moved, has
 // the same codes.  A row of zeros has scale 0; a row that holds an infinity or
 // a NaN has scale NaN and codes 0, and reads back as NaN.
@@ -40,23 +39,15 @@ template <typename C> struct CodeTop { static constexpr float v = 1.0f; };
 template <> struct CodeTop<int8_t> { static constexpr float v = 127.0f; };
 template <> struct CodeTop<fp8> { static constexpr float v = 448.0f; };
 
-// The code of x in a row of largest magnitude `top`, inv = TOP/top in fp32.
-// t = x inv is within 2^-22 of the quotient; where both ends of t (1 +- 2^-21)
-// have one code, it is the quotient's.
+// The code of x in a row of largest magnitude `top`, by 64 bits.
 template <typename C>
-__device__ inline uint32_t code_of(float x, float inv, float top) {
-  const float t = x * inv;
-  constexpr float e = 4.76837158203125e-7f;  // 2^-21
+__device__ inline uint32_t exact_code(float x, float top) {
+  const double d = (double)CodeTop<C>::v * (double)x / (double)top;
   if constexpr (__is_same(C, int8_t)) {
-    const float lo = rintf(fmaf(-e, t, t)), hi = rintf(fmaf(e, t, t));
-    if (lo == hi) return (uint32_t)(int)lo & 0xffu;
-    return (uint32_t)(int)rint(127.0 * (double)x / (double)top) & 0xffu;
+    return (uint32_t)(int)rint(d) & 0xffu;
   } else {
-    const uint32_t two = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(fmaf(-e, t, t), fmaf(e, t, t), 0, false);
-    if (((two ^ (two >> 8)) & 0xffu) == 0u) return two & 0xffu;
     // rounded to odd on the way to fp32, so that the second rounding sees on
     // which side of a border the quotient lies
-    const double d = 448.0 * (double)x / (double)top;
     float f = (float)d;
     if ((double)f != d) {
       uint32_t b = __float_as_uint(f);
@@ -64,6 +55,63 @@ __device__ inline uint32_t code_of(float x, float inv, float top) {
       f = __uint_as_float(b | 1u);
     }
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f, f, 0, false) & 0xffu;
+  }
+}
+
+// The codes nearest to x f, four to a word.  int8 rounds in the addition of
+// 1.5 2^23 (the sum's low byte is the code).
+__device__ inline uint32_t codes4(const float* x, float f, int8_t) {
+  constexpr float magic = 12582912.0f;
+  const uint32_t a = __float_as_uint(fmaf(x[0], f, magic)), b = __float_as_uint(fmaf(x[1], f, magic));
+  const uint32_t c = __float_as_uint(fmaf(x[2], f, magic)), d = __float_as_uint(fmaf(x[3], f, magic));
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u),
+                               0x05040100u);
+}
+__device__ inline uint32_t codes4(const float* x, float f, fp8) {
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * f, x[1] * f, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * f, x[3] * f, lo, true);
+}
+
+// Codes of N values of a row of largest magnitude `top`, of type T.
+//
+// The quotient TOP x / top lies between x inv (1 - 2^-21) and x inv (1 + 2^-21),
+// inv = TOP/top in fp32; where both ends have one code, it is the quotient's.
+// Else fp32 rows take 64 bits.  2-byte rows have X 2^i and P 2^j for x and top
+// with X, P < 2^11, and TOP = N 2^n (N = 127 or 7): a quotient that is not on a
+// border M 2^m (M < 2^8, or 2^5) is at least 1/(M P) or 1/(N X) > 2^-19 of it
+// away, so the fp32 quotient, rounded once, decides.
+//
+// int8 codes of 2-byte rows need only the upper end: 2^-21 crosses no border,
+// and of those hit exactly, 63.5 (x = top/2, in every sixth row of 64 values)
+// goes up to the even 64.  Others, (n + 1/2) P = 127 X 2^k, need a P that 127
+// divides: such rows take the quotient.
+template <typename T, typename C, int N>
+__device__ inline void codes_of(const float (&x)[N], float top, uint32_t (&code)[N / 4]) {
+  const float inv = CodeTop<C>::v / top;
+  constexpr float e = 4.76837158203125e-7f;  // 2^-21
+  const float lo = fmaf(-e, inv, inv), hi = fmaf(e, inv, inv);
+  bool differ = false;
+#pragma unroll
+  for (int w = 0; w < N / 4; ++w) code[w] = codes4(x + 4 * w, hi, C{});
+  if constexpr (sizeof(T) == 2 && __is_same(C, int8_t)) {
+    differ = ((__float_as_uint(top) & 0x7fffffu) | 0x800000u) % 127u == 0u;
+  } else {
+#pragma unroll
+    for (int w = 0; w < N / 4; ++w) differ = differ || code[w] != codes4(x + 4 * w, lo, C{});
+  }
+  if (!differ) return;
+#pragma unroll
+  for (int w = 0; w < N / 4; ++w) {
+    if constexpr (sizeof(T) == 2) {
+      float q[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) q[k] = CodeTop<C>::v * x[4 * w + k] / top;
+      code[w] = codes4(q, 1.0f, C{});
+    } else {
+      code[w] = 0u;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) code[w] |= exact_code<C>(x[4 * w + k], top) << (8 * k);
+    }
   }
 }
 
@@ -87,7 +135,8 @@ __device__ inline int cache_position(const CacheCall& a, int b, int t) {
 }
 
 // Block (x, y, z): 256 / LPR rows from row x 256/LPR on of head y = b H + h, of
-// k (z = 0) or v.
+// k (z = 0) or v.  (Blocks over several heads of the same positions, so that
+// each reads whole lines of a stacked projection, were no faster.)
 template <typename T, typename C, int D>
 __global__ __launch_bounds__(256) void cache_write_kernel(CacheCall a) {
   using vec = typename RowVec<T>::type;
@@ -119,20 +168,14 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheCall a) {
     if (pos < 0) return;
     const bool finite = m < 0x7f800000u;
     const float top = __uint_as_float(m);
-    uint32_t code[VEC / 4];
+    uint32_t code[VEC / 4] = {};
     if (finite && m != 0u) {
       // below 2^-118 TOP/top may leave fp32's range: scaled by a power of two
       const float up = m < 0x04800000u ? 1.0633823966279327e37f : 1.0f;  // 2^123
-      const float inv = CodeTop<C>::v / (top * up);
+      float f[VEC];
 #pragma unroll
-      for (int w = 0; w < VEC / 4; ++w) {
-        code[w] = 0u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) code[w] |= code_of<C>(to_f(x[4 * w + e]) * up, inv, top * up) << (8 * e);
-      }
-    } else {
-#pragma unroll
-      for (int w = 0; w < VEC / 4; ++w) code[w] = 0u;
+      for (int e = 0; e < VEC; ++e) f[e] = to_f(x[e]) * up;
+      codes_of<T, C, VEC>(f, top * up, code);
     }
     if constexpr (VEC == 8) *reinterpret_cast<uint2*>(row) = make_uint2(code[0], code[1]);
     else *reinterpret_cast<uint32_t*>(row) = code[0];
