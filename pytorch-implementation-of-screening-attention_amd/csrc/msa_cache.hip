@@ -134,14 +134,15 @@ __device__ inline int cache_position(const CacheCall& a, int b, int t) {
   return s >= 0 && s < a.cap ? (int)s : -1;
 }
 
-// Block (x, y, z): 256 / LPR rows from row x 256/LPR on of head y = b H + h, of
-// k (z = 0) or v.  (Blocks over several heads of the same positions, so that
-// each reads whole lines of a stacked projection, were no faster.)
+// Block (x, y): rows x 256/LPR, ... of head y = b H + h, of k and of v: their
+// loads are in flight together and the positions are found once.  (Blocks over
+// several heads of the same positions, so that each reads whole lines of a
+// stacked projection, were no faster.)
 template <typename T, typename C, int D>
 __global__ __launch_bounds__(256) void cache_write_kernel(CacheCall a) {
   using vec = typename RowVec<T>::type;
   constexpr int VEC = RowVec<T>::N, LPR = D / VEC;
-  const int z = blockIdx.z, b = blockIdx.y / a.H, h = blockIdx.y % a.H;
+  const int b = blockIdx.y / a.H, h = blockIdx.y % a.H;
   const int t = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, d0 = (threadIdx.x % LPR) * VEC;
   int64_t src = t;
   int pos = -1;
@@ -149,38 +150,45 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheCall a) {
     if (a.rows != nullptr) src = a.rows[(int64_t)b * a.T + t];
     if (src >= 0 && src < a.Tx) pos = cache_position(a, b, t);
   }
-  vec x;
+  vec x[2];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) x[e] = from_f<T>(0.0f);
-  const Strides3 xs = a.xs[z], cs = a.cs[z], ss = a.ss[z];
-  if (pos >= 0) x = *reinterpret_cast<const vec*>((const T*)a.x[z] + b * xs.sb + src * xs.st + h * xs.sh + d0);
-  char* row = (char*)a.c[z] + (b * cs.sb + (int64_t)pos * cs.st + h * cs.sh + d0) * (int64_t)sizeof(C);
-  if constexpr (sizeof(C) > 1) {
-    if (pos >= 0) *reinterpret_cast<vec*>(row) = x;
-  } else {
-    uint32_t m = 0u;
+  for (int z = 0; z < 2; ++z) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const uint32_t y = __float_as_uint(to_f(x[e])) & 0x7fffffffu;
-      m = y > m ? y : m;
+    for (int e = 0; e < VEC; ++e) x[z][e] = from_f<T>(0.0f);
+    const Strides3 xs = a.xs[z];
+    if (pos >= 0) x[z] = *reinterpret_cast<const vec*>((const T*)a.x[z] + b * xs.sb + src * xs.st + h * xs.sh + d0);
+  }
+#pragma unroll
+  for (int z = 0; z < 2; ++z) {
+    const Strides3 cs = a.cs[z], ss = a.ss[z];
+    char* row = (char*)a.c[z] + (b * cs.sb + (int64_t)pos * cs.st + h * cs.sh + d0) * (int64_t)sizeof(C);
+    if constexpr (sizeof(C) > 1) {
+      if (pos >= 0) *reinterpret_cast<vec*>(row) = x[z];
+    } else {
+      uint32_t m = 0u;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const uint32_t y = __float_as_uint(to_f(x[z][e])) & 0x7fffffffu;
+        m = y > m ? y : m;
+      }
+      m = group_max_u32<LPR>(m);  // a NaN's magnitude is above an infinity's
+      if (pos < 0) continue;
+      const bool finite = m < 0x7f800000u;
+      const float top = __uint_as_float(m);
+      uint32_t code[VEC / 4] = {};
+      if (finite && m != 0u) {
+        // below 2^-118 TOP/top may leave fp32's range: scaled by a power of two
+        const float up = m < 0x04800000u ? 1.0633823966279327e37f : 1.0f;  // 2^123
+        float f[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] = to_f(x[z][e]) * up;
+        codes_of<T, C, VEC>(f, top * up, code);
+      }
+      if constexpr (VEC == 8) *reinterpret_cast<uint2*>(row) = make_uint2(code[0], code[1]);
+      else *reinterpret_cast<uint32_t*>(row) = code[0];
+      if (d0 == 0)
+        a.s[z][b * ss.sb + (int64_t)pos * ss.st + h * ss.sh] = finite ? top / CodeTop<C>::v : __uint_as_float(0x7fc00000u);
     }
-    m = group_max_u32<LPR>(m);  // a NaN's magnitude is above an infinity's
-    if (pos < 0) return;
-    const bool finite = m < 0x7f800000u;
-    const float top = __uint_as_float(m);
-    uint32_t code[VEC / 4] = {};
-    if (finite && m != 0u) {
-      // below 2^-118 TOP/top may leave fp32's range: scaled by a power of two
-      const float up = m < 0x04800000u ? 1.0633823966279327e37f : 1.0f;  // 2^123
-      float f[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) f[e] = to_f(x[e]) * up;
-      codes_of<T, C, VEC>(f, top * up, code);
-    }
-    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(row) = make_uint2(code[0], code[1]);
-    else *reinterpret_cast<uint32_t*>(row) = code[0];
-    if (d0 == 0)
-      a.s[z][b * ss.sb + (int64_t)pos * ss.st + h * ss.sh] = finite ? top / CodeTop<C>::v : __uint_as_float(0x7fc00000u);
   }
 }
 
@@ -189,36 +197,51 @@ template <typename T, typename C, int D>
 __global__ __launch_bounds__(256) void cache_read_kernel(CacheCall a) {
   using vec = typename RowVec<T>::type;
   constexpr int VEC = RowVec<T>::N, LPR = D / VEC;
-  const int z = blockIdx.z, b = blockIdx.y / a.H, h = blockIdx.y % a.H;
+  const int b = blockIdx.y / a.H, h = blockIdx.y % a.H;
   const int t = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, d0 = (threadIdx.x % LPR) * VEC;
   if (t >= a.T) return;
   const int pos = cache_position(a, b, t);
-  const Strides3 xs = a.xs[z], cs = a.cs[z], ss = a.ss[z];
-  vec x;
+  vec x[2];
+  uint32_t code[2][VEC / 4];
+  float sc[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) x[e] = from_f<T>(0.0f);
-  if (pos >= 0) {
+  for (int z = 0; z < 2; ++z) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) x[z][e] = from_f<T>(0.0f);
+    const Strides3 cs = a.cs[z], ss = a.ss[z];
     const char* row = (const char*)a.c[z] + (b * cs.sb + (int64_t)pos * cs.st + h * cs.sh + d0) * (int64_t)sizeof(C);
-    if constexpr (sizeof(C) > 1) {
-      x = *reinterpret_cast<const vec*>(row);
-    } else {
-      const float sc = a.s[z][b * ss.sb + (int64_t)pos * ss.st + h * ss.sh];
+    if (pos >= 0) {
+      if constexpr (sizeof(C) > 1) {
+        x[z] = *reinterpret_cast<const vec*>(row);
+      } else {
 #pragma unroll
-      for (int w = 0; w < VEC / 4; ++w) {
-        float v[4];
-        decode4(reinterpret_cast<const uint32_t*>(row)[w], v, C{});
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * w + e] = from_f<T>(v[e] * sc);
+        for (int w = 0; w < VEC / 4; ++w) code[z][w] = reinterpret_cast<const uint32_t*>(row)[w];
+        sc[z] = a.s[z][b * ss.sb + (int64_t)pos * ss.st + h * ss.sh];
       }
     }
   }
-  *reinterpret_cast<vec*>((T*)const_cast<void*>(a.x[z]) + b * xs.sb + (int64_t)t * xs.st + h * xs.sh + d0) = x;
+#pragma unroll
+  for (int z = 0; z < 2; ++z) {
+    if constexpr (sizeof(C) == 1) {
+      if (pos >= 0) {
+#pragma unroll
+        for (int w = 0; w < VEC / 4; ++w) {
+          float v[4];
+          decode4(code[z][w], v, C{});
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[z][4 * w + e] = from_f<T>(v[e] * sc[z]);
+        }
+      }
+    }
+    const Strides3 xs = a.xs[z];
+    *reinterpret_cast<vec*>((T*)const_cast<void*>(a.x[z]) + b * xs.sb + (int64_t)t * xs.st + h * xs.sh + d0) = x[z];
+  }
 }
 
 template <typename T, typename C, int D>
 static hipError_t launch_cache_t(const CacheCall& c) {
   constexpr int rows = 256 / (D / RowVec<T>::N);
-  const dim3 grid((unsigned)((c.T + rows - 1) / rows), (unsigned)(c.B * c.H), 2u);
+  const dim3 grid((unsigned)((c.T + rows - 1) / rows), (unsigned)(c.B * c.H));
   if (c.read) hipLaunchKernelGGL((cache_read_kernel<T, C, D>), grid, dim3(256), 0, c.stream, c);
   else hipLaunchKernelGGL((cache_write_kernel<T, C, D>), grid, dim3(256), 0, c.stream, c);
   return hipGetLastError();
