@@ -219,61 +219,61 @@ int msa_decode_noalloc(const void* q, int64_t q_sb, int64_t q_sh,
                        const float* r, const float* w, float eps, void* y, void* stream);
 
 /*
+ * The entry points below take their arguments in one struct (every field 8
+ * bytes wide, so a binding can pack it without knowing paddings): converting
+ * some forty arguments one by one costs a Python caller as much as the launch.
+ * The struct is read during the call only.
+ *
+ * A (B, T, H, D) tensor: strides in elements, unit stride over D, rows 16-byte
+ * aligned.  Scales of cache rows: fp32 (B, T, H).
+ */
+typedef struct { void* p; int64_t sb, st, sh; } msa_tensor;
+
+/*
  * Key/value cache rows written in one launch, and read back.  No counterpart
  * in the reference (its generate has no cache, model.py:111-141).
  *   k, v     : rows (B, Tx, H, D) of type dtype, the projections' view as in
  *              msa_fwd.
- *   kcache, vcache : (B, cache_cap, H, D) rows of type cache_dtype, strides in
- *              elements, unit stride over D; every row 16-byte aligned.
- *              cache_dtype is dtype (a copy), MSA_I8 or MSA_FP8.
- *   kscale, vscale : quantised caches: fp32 (B, cache_cap, H) with strides (sb,
- *              st, sh); else null.  A row x is kept as the codes nearest to
+ *   kcache, vcache : (B, cache_cap, H, D) rows of type cache_dtype: dtype (a
+ *              copy), MSA_I8 or MSA_FP8.
+ *   kscale, vscale : quantised caches: fp32 (B, cache_cap, H); else null.  A row x is kept as the codes nearest to
  *              TOP x / A (ties to the even code, decided exactly), A = max|x|,
  *              TOP = 127 or 448, and the scale A / TOP; code * scale is its value.
  *              A row of zeros has scale 0, a row with an infinity or a NaN codes
  *              0 and scale NaN.
  *   rows     : null, or a device int64 (B, T): row t is taken from row
  *              rows[b, t] of k and v (outside [0, Tx): not written).  Null: row
- *              t, and T = Tx.
+ *              t, and T <= Tx.
  *   count    : null, or a device int64 (B): rows t < count[b] only.
  *   start    : null, or device int64 positions, one (start_n = 1) or one per
  *              sequence (start_n = B): row t goes to position start + t.  Null:
  *              start0.  Rows at positions outside the cache are not written.
- * Positions and rows of one sequence must not repeat.  Everything else of the
- * cache is left as it was.
+ * Positions of one sequence must not repeat.  Everything else of the cache is
+ * left as it was.
+ *
+ * msa_cache_read takes the same struct: the values of positions start .. start
+ * + T - 1 go to k, v (B, T, H, D) of type dtype: code * scale, rounded once; a
+ * copy where cache_dtype is dtype.  Positions outside the cache read as zeros.
+ * rows and count must be null.
  */
-int msa_cache_write(const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh,
-                    const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh,
-                    int B, int T, int Tx, int H, int D, int dtype,
-                    const int64_t* rows, const int64_t* count,
-                    const int64_t* start, int start_n, int64_t start0,
-                    void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_sh,
-                    void* vcache, int64_t vc_sb, int64_t vc_st, int64_t vc_sh,
-                    int cache_cap, int cache_dtype,
-                    float* kscale, int64_t ks_sb, int64_t ks_st, int64_t ks_sh,
-                    float* vscale, int64_t vs_sb, int64_t vs_st, int64_t vs_sh, void* stream);
-
-/*
- * The values of positions start .. start + T - 1 (as msa_cache_write takes
- * them) into contiguous k, v (B, T, H, D) of type dtype: code * scale, rounded
- * once; a copy where cache_dtype is dtype.  Positions outside the cache read
- * as zeros.
- */
-int msa_cache_read(const void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_sh,
-                   const void* vcache, int64_t vc_sb, int64_t vc_st, int64_t vc_sh,
-                   int cache_cap, int cache_dtype,
-                   const float* kscale, int64_t ks_sb, int64_t ks_st, int64_t ks_sh,
-                   const float* vscale, int64_t vs_sb, int64_t vs_st, int64_t vs_sh,
-                   int B, int T, int H, int D, int dtype,
-                   const int64_t* start, int start_n, int64_t start0,
-                   void* k, void* v, void* stream);
+typedef struct {
+  msa_tensor k, v, kcache, vcache, kscale, vscale;
+  const int64_t* rows;
+  const int64_t* count;
+  const int64_t* start;
+  int64_t start_n, start0;
+  int64_t B, T, Tx, H, D, dtype, cache_cap, cache_dtype;
+} msa_cache_args;
+int msa_cache_write(const msa_cache_args* args, void* stream);
+int msa_cache_read(const msa_cache_args* args, void* stream);
 
 /*
  * Screening attention of a tree of N <= MSA_TREE_MAX drafted tokens per
  * sequence over a cache; N = 1 decodes one token.  No counterpart in the
  * reference (its generate re-runs the prefix for every token,
  * model.py:111-141).
- *   q        : (B, N, H, D) raw query projections, strides (sb, sn, sh), unit D.
+ *   q        : (B, N, H, D) raw query projections of type dtype (st: the
+ *              stride over nodes).
  *   kcache, vcache, kscale, vscale : as msa_cache_write leaves them;
  *              cache_dtype is dtype, MSA_I8 or MSA_FP8.  The cache holds sequence b's
  *              committed rows at positions [0, n_b) and its nodes' own rows at
@@ -281,6 +281,7 @@ int msa_cache_read(const void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_
  *   lengths  : device int64 n_b, one (lengths_n = 1) or one per sequence.
  *   parents  : device int64, node i of sequence b continues node parents[b *
  *              par_sb + i] < i, or is a root (any other value); null: a chain.
+ *   r, w     : fp32 (H,), as in msa_fwd.
  * Node i stands at position n_b + depth_i (a root's depth is 0) and sees the
  * committed keys of its window (pos - w, pos], and of the drafted rows its own
  * and its ancestors' within the window.  y (B, N, H, D) contiguous, of type
@@ -290,21 +291,25 @@ int msa_cache_read(const void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_
  * over blocks (the sums' order, so y's rounding) depends on it, the shapes, the
  * length and the windows: equal calls give bitwise equal y.
  * workspace: msa_tree_workspace_bytes of the same sizes (0 where one block
- * takes a head's keys), scratch of this call.
+ * takes a head's keys), scratch of this call.  H * cache_cap <= 2^35.
  */
 #define MSA_TREE_MAX 64
+typedef struct {
+  msa_tensor q, kcache, vcache, kscale, vscale;
+  const int64_t* lengths;
+  const int64_t* parents;
+  const float* r;
+  const float* w;
+  void* y;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t lengths_n, par_sb;
+  int64_t B, N, H, D, dtype, cache_cap, cache_dtype, window_hint;
+  double eps;
+} msa_tree_args;
 size_t msa_tree_workspace_bytes(int B, int H, int N, int D, int dtype, int cache_dtype, int cache_cap,
                                 int window_hint);
-int msa_tree_decode(const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh,
-                    const void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_sh,
-                    const void* vcache, int64_t vc_sb, int64_t vc_st, int64_t vc_sh,
-                    int cache_cap, int cache_dtype,
-                    const float* kscale, int64_t ks_sb, int64_t ks_st, int64_t ks_sh,
-                    const float* vscale, int64_t vs_sb, int64_t vs_st, int64_t vs_sh,
-                    int B, int N, int H, int D, int dtype,
-                    const int64_t* lengths, int lengths_n, const int64_t* parents, int64_t par_sb, int window_hint,
-                    const float* r, const float* w, float eps,
-                    void* y, void* workspace, size_t workspace_bytes, void* stream);
+int msa_tree_decode(const msa_tree_args* args, void* stream);
 
 /*
  * Verification of drafted tokens.  No counterpart in the reference.  Sequence
@@ -337,11 +342,24 @@ int msa_tree_decode(const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh,
  * where no weight is left (token 0 if p has none).
  * workspace: msa_verify_workspace_bytes (greedy; 0 with uniforms).
  */
+typedef struct {
+  const void* target;
+  int64_t t_sb, t_sn;
+  const void* draft;
+  int64_t d_sb, d_sn;
+  const int64_t* tokens;
+  const int64_t* parents;
+  int64_t par_sb;
+  const float* uniforms;
+  int64_t* path;
+  int64_t* count;
+  int64_t* token;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t B, M, V, dtype;
+} msa_verify_args;
 size_t msa_verify_workspace_bytes(int B, int M, int64_t V, int greedy);
-int msa_verify(const void* target, int64_t t_sb, int64_t t_sn, const void* draft, int64_t d_sb, int64_t d_sn,
-               const int64_t* tokens, const int64_t* parents, int64_t par_sb, const float* uniforms,
-               int B, int M, int64_t V, int dtype, int64_t* path, int64_t* count, int64_t* token,
-               void* workspace, size_t workspace_bytes, void* stream);
+int msa_verify(const msa_verify_args* args, void* stream);
 
 /* Kernel timing for measurement.  After msa_timer_arm(kernel, n) the next n
  * launches of that kernel (any entry point) each record a HIP event pair on

@@ -439,11 +439,14 @@ int msa_decode_noalloc(const void* q, int64_t q_sb, int64_t q_sh, const void* kc
   return hip_status(msa::launch_decode(c), "msa_decode_noalloc launch");
 }
 
+// A size as the kernels take it; what does not fit becomes -1, which no check
+// passes.
+static int size_of(int64_t x) { return x < 0 || x > 0x7fffffff ? -1 : (int)x; }
+static msa::Strides3 strides_of(const msa_tensor& t) { return {t.sb, t.st, t.sh}; }
+
 // Shapes, types and cache tensors shared by the cache entry points.
-static int check_cache(int B, int T, int H, int D, int dtype, const void* kcache, int64_t kc_sb, int64_t kc_st,
-                       int64_t kc_sh, const void* vcache, int64_t vc_sb, int64_t vc_st, int64_t vc_sh, int cache_cap,
-                       int cache_dtype, const float* kscale, int64_t ks_sb, int64_t ks_st, int64_t ks_sh,
-                       const float* vscale, int64_t vs_sb, int64_t vs_st, int64_t vs_sh) {
+static int check_cache(int B, int T, int H, int D, int dtype, int cache_cap, int cache_dtype, const msa_tensor& kcache,
+                       const msa_tensor& vcache, const msa_tensor& kscale, const msa_tensor& vscale) {
   msa::Geometry g;
   int rc = check_geometry(B, H, T, cache_cap, D, dtype, 1, &g);
   if (rc != MSA_OK) return rc;
@@ -452,83 +455,56 @@ static int check_cache(int B, int T, int H, int D, int dtype, const void* kcache
     return fail(MSA_ERR_INVALID, "cache_dtype must be the rows' dtype, MSA_I8 or MSA_FP8");
   if (B == 0 || T == 0) return MSA_OK;  // an empty call touches no tensor
   const int m = codes ? 16 : (dtype == MSA_F32 ? 4 : 8);
-  const int64_t st[2][3] = {{kc_sb, kc_st, kc_sh}, {vc_sb, vc_st, vc_sh}};
-  const int64_t sc[2][3] = {{ks_sb, ks_st, ks_sh}, {vs_sb, vs_st, vs_sh}};
-  const void* c[2] = {kcache, vcache};
-  const float* s[2] = {kscale, vscale};
+  const msa_tensor* c[2] = {&kcache, &vcache};
+  const msa_tensor* s[2] = {&kscale, &vscale};
   for (int z = 0; z < 2; ++z) {
     const char* name = z == 0 ? "kcache" : "vcache";
-    if ((rc = check_out(name, c[z])) != MSA_OK) return rc;
-    for (int e = 0; e < 3; ++e)
-      if (st[z][e] < 0 || st[z][e] % m)
-        return fail(MSA_ERR_INVALID, "%s strides must be non-negative multiples of %d elements", name, m);
+    if ((rc = check_out(name, c[z]->p)) != MSA_OK) return rc;
+    if (c[z]->sb < 0 || c[z]->st < 0 || c[z]->sh < 0 || c[z]->sb % m || c[z]->st % m || c[z]->sh % m)
+      return fail(MSA_ERR_INVALID, "%s strides must be non-negative multiples of %d elements", name, m);
     // kernels address the rows of a 32-row unit by 32-bit byte offsets
-    if (st[z][1] * 64 * (codes ? 1 : dtype == MSA_F32 ? 4 : 2) >= (int64_t)1 << 32 || (codes && sc[z][1] * 256 >= (int64_t)1 << 32))
+    if (c[z]->st >= ((int64_t)1 << 26) / (codes ? 1 : dtype == MSA_F32 ? 4 : 2) || (codes && s[z]->st >= (int64_t)1 << 24))
       return fail(MSA_ERR_INVALID, "%s time stride is too large (64 rows must span < 4 GiB)", name);
     if (!codes) continue;
-    if (s[z] == nullptr) return fail(MSA_ERR_INVALID, "%s of 8-bit codes needs its scales", name);
-    if (((uintptr_t)s[z] & 3u) != 0 || sc[z][0] < 0 || sc[z][1] < 0 || sc[z][2] < 0)
+    if (s[z]->p == nullptr) return fail(MSA_ERR_INVALID, "%s of 8-bit codes needs its scales", name);
+    if (((uintptr_t)s[z]->p & 3u) != 0 || s[z]->sb < 0 || s[z]->st < 0 || s[z]->sh < 0)
       return fail(MSA_ERR_INVALID, "%s scales must be fp32 with non-negative strides", name);
   }
   return MSA_OK;
 }
 
-static int check_start(const int64_t* start, int start_n, int B) {
-  if (start != nullptr && start_n != 1 && start_n != B)
-    return fail(MSA_ERR_INVALID, "start holds %d positions, 1 or B=%d needed", start_n, B);
-  return MSA_OK;
+// Both directions of msa_cache_args.
+static int cache_call(const msa_cache_args* a, int read, void* stream, const char* what) {
+  if (a == nullptr) return fail(MSA_ERR_INVALID, "args is null");
+  msa::CacheCall c;
+  c.B = size_of(a->B); c.T = size_of(a->T); c.Tx = size_of(a->Tx); c.H = size_of(a->H); c.D = size_of(a->D);
+  c.cap = size_of(a->cache_cap); c.dtype = size_of(a->dtype); c.cache_dtype = size_of(a->cache_dtype);
+  int rc = check_cache(c.B, c.T, c.H, c.D, c.dtype, c.cap, c.cache_dtype, a->kcache, a->vcache, a->kscale, a->vscale);
+  if (rc != MSA_OK) return rc;
+  if (c.Tx < 0 || c.Tx > kMaxT || (a->rows == nullptr && c.T > c.Tx))
+    return fail(MSA_ERR_INVALID, "k and v hold %d rows, %d asked for", c.Tx, c.T);
+  if (read && (a->rows != nullptr || a->count != nullptr))
+    return fail(MSA_ERR_INVALID, "msa_cache_read takes no rows or count");
+  if (a->start != nullptr && a->start_n != 1 && a->start_n != a->B)
+    return fail(MSA_ERR_INVALID, "start holds %lld positions, 1 or B=%d needed", (long long)a->start_n, c.B);
+  if (c.B == 0 || c.T == 0 || c.Tx == 0) return ok();
+  if ((rc = check_tensor("k", a->k.p, a->k.sb, a->k.st, a->k.sh, c.dtype)) != MSA_OK) return rc;
+  if ((rc = check_tensor("v", a->v.p, a->v.sb, a->v.st, a->v.sh, c.dtype)) != MSA_OK) return rc;
+  c.x[0] = a->k.p; c.x[1] = a->v.p; c.xs[0] = strides_of(a->k); c.xs[1] = strides_of(a->v);
+  c.c[0] = a->kcache.p; c.c[1] = a->vcache.p; c.cs[0] = strides_of(a->kcache); c.cs[1] = strides_of(a->vcache);
+  c.s[0] = (float*)a->kscale.p; c.s[1] = (float*)a->vscale.p;
+  c.ss[0] = strides_of(a->kscale); c.ss[1] = strides_of(a->vscale);
+  c.rows = a->rows; c.count = a->count; c.start = a->start; c.start_step = a->start_n == 1 ? 0 : 1; c.start0 = a->start0;
+  c.read = read;
+  c.stream = (hipStream_t)stream;
+  return hip_status(msa::launch_cache(c), what);
 }
 
-int msa_cache_write(const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st,
-                    int64_t v_sh, int B, int T, int Tx, int H, int D, int dtype, const int64_t* rows,
-                    const int64_t* count, const int64_t* start, int start_n, int64_t start0, void* kcache,
-                    int64_t kc_sb, int64_t kc_st, int64_t kc_sh, void* vcache, int64_t vc_sb, int64_t vc_st,
-                    int64_t vc_sh, int cache_cap, int cache_dtype, float* kscale, int64_t ks_sb, int64_t ks_st,
-                    int64_t ks_sh, float* vscale, int64_t vs_sb, int64_t vs_st, int64_t vs_sh, void* stream) {
-  int rc = check_cache(B, T, H, D, dtype, kcache, kc_sb, kc_st, kc_sh, vcache, vc_sb, vc_st, vc_sh, cache_cap,
-                       cache_dtype, kscale, ks_sb, ks_st, ks_sh, vscale, vs_sb, vs_st, vs_sh);
-  if (rc != MSA_OK) return rc;
-  if (Tx < 0 || Tx > kMaxT || (rows == nullptr && T > Tx))
-    return fail(MSA_ERR_INVALID, "k and v hold %d rows, %d asked for", Tx, T);
-  if ((rc = check_start(start, start_n, B)) != MSA_OK) return rc;
-  if (B == 0 || T == 0 || Tx == 0) return ok();
-  if ((rc = check_tensor("k", k, k_sb, k_st, k_sh, dtype)) != MSA_OK) return rc;
-  if ((rc = check_tensor("v", v, v_sb, v_st, v_sh, dtype)) != MSA_OK) return rc;
-  msa::CacheCall c;
-  c.x[0] = k; c.x[1] = v; c.xs[0] = {k_sb, k_st, k_sh}; c.xs[1] = {v_sb, v_st, v_sh};
-  c.c[0] = kcache; c.c[1] = vcache; c.cs[0] = {kc_sb, kc_st, kc_sh}; c.cs[1] = {vc_sb, vc_st, vc_sh};
-  c.s[0] = kscale; c.s[1] = vscale; c.ss[0] = {ks_sb, ks_st, ks_sh}; c.ss[1] = {vs_sb, vs_st, vs_sh};
-  c.rows = rows; c.count = count; c.start = start; c.start_step = start_n == 1 ? 0 : 1; c.start0 = start0;
-  c.B = B; c.T = T; c.Tx = Tx; c.H = H; c.D = D; c.cap = cache_cap; c.dtype = dtype; c.cache_dtype = cache_dtype;
-  c.read = 0;
-  c.stream = (hipStream_t)stream;
-  return hip_status(msa::launch_cache(c), "msa_cache_write launch");
+int msa_cache_write(const msa_cache_args* args, void* stream) {
+  return cache_call(args, 0, stream, "msa_cache_write launch");
 }
-
-int msa_cache_read(const void* kcache, int64_t kc_sb, int64_t kc_st, int64_t kc_sh, const void* vcache, int64_t vc_sb,
-                   int64_t vc_st, int64_t vc_sh, int cache_cap, int cache_dtype, const float* kscale, int64_t ks_sb,
-                   int64_t ks_st, int64_t ks_sh, const float* vscale, int64_t vs_sb, int64_t vs_st, int64_t vs_sh,
-                   int B, int T, int H, int D, int dtype, const int64_t* start, int start_n, int64_t start0, void* k,
-                   void* v, void* stream) {
-  int rc = check_cache(B, T, H, D, dtype, kcache, kc_sb, kc_st, kc_sh, vcache, vc_sb, vc_st, vc_sh, cache_cap,
-                       cache_dtype, kscale, ks_sb, ks_st, ks_sh, vscale, vs_sb, vs_st, vs_sh);
-  if (rc != MSA_OK) return rc;
-  if ((rc = check_start(start, start_n, B)) != MSA_OK) return rc;
-  if (B == 0 || T == 0) return ok();
-  if ((rc = check_out("k", k)) != MSA_OK) return rc;
-  if ((rc = check_out("v", v)) != MSA_OK) return rc;
-  msa::CacheCall c;
-  const int64_t sh = D, st = (int64_t)H * D, sb = st * T;
-  c.x[0] = k; c.x[1] = v; c.xs[0] = c.xs[1] = {sb, st, sh};
-  c.c[0] = const_cast<void*>(kcache); c.c[1] = const_cast<void*>(vcache);
-  c.cs[0] = {kc_sb, kc_st, kc_sh}; c.cs[1] = {vc_sb, vc_st, vc_sh};
-  c.s[0] = const_cast<float*>(kscale); c.s[1] = const_cast<float*>(vscale);
-  c.ss[0] = {ks_sb, ks_st, ks_sh}; c.ss[1] = {vs_sb, vs_st, vs_sh};
-  c.rows = nullptr; c.count = nullptr; c.start = start; c.start_step = start_n == 1 ? 0 : 1; c.start0 = start0;
-  c.B = B; c.T = T; c.Tx = T; c.H = H; c.D = D; c.cap = cache_cap; c.dtype = dtype; c.cache_dtype = cache_dtype;
-  c.read = 1;
-  c.stream = (hipStream_t)stream;
-  return hip_status(msa::launch_cache(c), "msa_cache_read launch");
+int msa_cache_read(const msa_cache_args* args, void* stream) {
+  return cache_call(args, 1, stream, "msa_cache_read launch");
 }
 
 static int tree_blocks_of(int B, int H, int N, int D, int dtype, int cache_dtype, int cache_cap, int window_hint) {
@@ -545,40 +521,37 @@ size_t msa_tree_workspace_bytes(int B, int H, int N, int D, int dtype, int cache
   return blocks == H ? 0 : (size_t)B * blocks * N * D * sizeof(float);
 }
 
-int msa_tree_decode(const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const void* kcache, int64_t kc_sb,
-                    int64_t kc_st, int64_t kc_sh, const void* vcache, int64_t vc_sb, int64_t vc_st, int64_t vc_sh,
-                    int cache_cap, int cache_dtype, const float* kscale, int64_t ks_sb, int64_t ks_st, int64_t ks_sh,
-                    const float* vscale, int64_t vs_sb, int64_t vs_st, int64_t vs_sh, int B, int N, int H, int D,
-                    int dtype, const int64_t* lengths, int lengths_n, const int64_t* parents, int64_t par_sb,
-                    int window_hint, const float* r, const float* w, float eps, void* y, void* workspace,
-                    size_t workspace_bytes, void* stream) {
-  int rc = check_cache(B, N, H, D, dtype, kcache, kc_sb, kc_st, kc_sh, vcache, vc_sb, vc_st, vc_sh, cache_cap,
-                       cache_dtype, kscale, ks_sb, ks_st, ks_sh, vscale, vs_sb, vs_st, vs_sh);
-  if (rc != MSA_OK) return rc;
-  if (N > MSA_TREE_MAX) return fail(MSA_ERR_INVALID, "a tree holds at most %d nodes, got %d", MSA_TREE_MAX, N);
-  if (B == 0 || N == 0) return ok();
-  if (N > cache_cap) return fail(MSA_ERR_INVALID, "the cache's %d positions do not hold %d nodes", cache_cap, N);
-  if ((int64_t)H * cache_cap > (int64_t)1 << 35)  // a sequence's key units are counted in 32 bits
-    return fail(MSA_ERR_INVALID, "H * cache_cap = %lld exceeds 2^35", (long long)H * cache_cap);
-  if (!(eps > 0.0f)) return fail(MSA_ERR_INVALID, "eps must be positive");
-  if (lengths == nullptr || (lengths_n != 1 && lengths_n != B))
-    return fail(MSA_ERR_INVALID, "lengths must be 1 or B=%d device int64", B);
-  if (par_sb < 0) return fail(MSA_ERR_INVALID, "parents stride must not be negative");
-  if ((rc = check_tensor("q", q, q_sb, q_sn, q_sh, dtype)) != MSA_OK) return rc;
-  if (r == nullptr || w == nullptr) return fail(MSA_ERR_INVALID, "r and w must be device arrays of H floats");
-  if ((rc = check_out("y", y)) != MSA_OK) return rc;
-  const size_t need = msa_tree_workspace_bytes(B, H, N, D, dtype, cache_dtype, cache_cap, window_hint);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
-    return fail(MSA_ERR_WORKSPACE, "tree workspace holds %zu bytes, %zu needed", workspace_bytes, need);
-  if (need > 0 && !aligned16(workspace)) return fail(MSA_ERR_INVALID, "workspace is not 16-byte aligned");
+int msa_tree_decode(const msa_tree_args* a, void* stream) {
+  if (a == nullptr) return fail(MSA_ERR_INVALID, "args is null");
   msa::TreeCall c;
-  c.B = B; c.H = H; c.N = N; c.D = D; c.q_dtype = dtype; c.cache_dtype = cache_dtype; c.cap = cache_cap;
-  c.q = q; c.q_sb = q_sb; c.q_sn = q_sn; c.q_sh = q_sh;
-  c.kc = kcache; c.ks = {kc_sb, kc_st, kc_sh}; c.vc = vcache; c.vs = {vc_sb, vc_st, vc_sh};
-  c.kscale = kscale; c.kss = {ks_sb, ks_st, ks_sh}; c.vscale = vscale; c.vss = {vs_sb, vs_st, vs_sh};
-  c.lengths = lengths; c.len_step = lengths_n == 1 ? 0 : 1; c.parents = parents; c.par_sb = par_sb;
-  c.r = r; c.w = w; c.eps = eps; c.part = (float*)workspace; c.y = y;
-  c.blocks = tree_blocks_of(B, H, N, D, dtype, cache_dtype, cache_cap, window_hint);
+  c.B = size_of(a->B); c.N = size_of(a->N); c.H = size_of(a->H); c.D = size_of(a->D); c.cap = size_of(a->cache_cap);
+  c.q_dtype = size_of(a->dtype); c.cache_dtype = size_of(a->cache_dtype); c.eps = (float)a->eps;
+  int rc = check_cache(c.B, c.N, c.H, c.D, c.q_dtype, c.cap, c.cache_dtype, a->kcache, a->vcache, a->kscale, a->vscale);
+  if (rc != MSA_OK) return rc;
+  if (c.N > MSA_TREE_MAX) return fail(MSA_ERR_INVALID, "a tree holds at most %d nodes, got %d", MSA_TREE_MAX, c.N);
+  if (c.B == 0 || c.N == 0) return ok();
+  if (c.N > c.cap) return fail(MSA_ERR_INVALID, "the cache's %d positions do not hold %d nodes", c.cap, c.N);
+  if ((int64_t)c.H * c.cap > (int64_t)1 << 35)  // a sequence's key units are counted in 32 bits
+    return fail(MSA_ERR_INVALID, "H * cache_cap = %lld exceeds 2^35", (long long)c.H * c.cap);
+  if (!(c.eps > 0.0f)) return fail(MSA_ERR_INVALID, "eps must be positive");
+  if (a->lengths == nullptr || (a->lengths_n != 1 && a->lengths_n != a->B))
+    return fail(MSA_ERR_INVALID, "lengths must be 1 or B=%d device int64", c.B);
+  if (a->par_sb < 0) return fail(MSA_ERR_INVALID, "parents stride must not be negative");
+  if ((rc = check_tensor("q", a->q.p, a->q.sb, a->q.st, a->q.sh, c.q_dtype)) != MSA_OK) return rc;
+  if (a->r == nullptr || a->w == nullptr) return fail(MSA_ERR_INVALID, "r and w must be device arrays of H floats");
+  if ((rc = check_out("y", a->y)) != MSA_OK) return rc;
+  const int hint = size_of(a->window_hint) < 0 ? 0 : (int)a->window_hint;
+  const size_t need = msa_tree_workspace_bytes(c.B, c.H, c.N, c.D, c.q_dtype, c.cache_dtype, c.cap, hint);
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need))
+    return fail(MSA_ERR_WORKSPACE, "tree workspace holds %zu bytes, %zu needed", (size_t)a->workspace_bytes, need);
+  if (need > 0 && !aligned16(a->workspace)) return fail(MSA_ERR_INVALID, "workspace is not 16-byte aligned");
+  c.q = a->q.p; c.q_sb = a->q.sb; c.q_sn = a->q.st; c.q_sh = a->q.sh;
+  c.kc = a->kcache.p; c.ks = strides_of(a->kcache); c.vc = a->vcache.p; c.vs = strides_of(a->vcache);
+  c.kscale = (const float*)a->kscale.p; c.kss = strides_of(a->kscale);
+  c.vscale = (const float*)a->vscale.p; c.vss = strides_of(a->vscale);
+  c.lengths = a->lengths; c.len_step = a->lengths_n == 1 ? 0 : 1; c.parents = a->parents; c.par_sb = a->par_sb;
+  c.r = a->r; c.w = a->w; c.part = (float*)a->workspace; c.y = a->y;
+  c.blocks = tree_blocks_of(c.B, c.H, c.N, c.D, c.q_dtype, c.cache_dtype, c.cap, hint);
   c.stream = (hipStream_t)stream;
   return hip_status(msa::launch_tree(c), "msa_tree_decode launch");
 }
@@ -588,35 +561,34 @@ size_t msa_verify_workspace_bytes(int B, int M, int64_t V, int greedy) {
   return (size_t)B * M * msa::verify_parts(V) * sizeof(unsigned long long);
 }
 
-int msa_verify(const void* target, int64_t t_sb, int64_t t_sn, const void* draft, int64_t d_sb, int64_t d_sn,
-               const int64_t* tokens, const int64_t* parents, int64_t par_sb, const float* uniforms, int B, int M,
-               int64_t V, int dtype, int64_t* path, int64_t* count, int64_t* token, void* workspace,
-               size_t workspace_bytes, void* stream) {
+int msa_verify(const msa_verify_args* a, void* stream) {
+  if (a == nullptr) return fail(MSA_ERR_INVALID, "args is null");
+  const int B = size_of(a->B), M = size_of(a->M), dtype = size_of(a->dtype);
   if (dtype != MSA_F32 && dtype != MSA_BF16 && dtype != MSA_F16)
     return fail(MSA_ERR_INVALID, "dtype must be MSA_F32, MSA_BF16 or MSA_F16");
   if (B < 0 || B > (1 << 24) || M < 1 || M > MSA_TREE_MAX)
     return fail(MSA_ERR_INVALID, "a tree holds 1 to %d nodes and a batch at most 2^24 sequences, got M=%d, B=%d",
                 MSA_TREE_MAX, M, B);
-  if (V < 1 || V > 0x7fffffff) return fail(MSA_ERR_INVALID, "the vocabulary must hold 1 to 2^31 - 1 tokens");
-  if (draft != nullptr && uniforms == nullptr) return fail(MSA_ERR_INVALID, "draft probabilities need uniforms");
+  if (a->V < 1 || a->V > 0x7fffffff) return fail(MSA_ERR_INVALID, "the vocabulary must hold 1 to 2^31 - 1 tokens");
+  if (a->draft != nullptr && a->uniforms == nullptr) return fail(MSA_ERR_INVALID, "draft probabilities need uniforms");
   if (B == 0) return ok();
   const uintptr_t es = dtype == MSA_F32 ? 4 : 2;
-  if (target == nullptr || tokens == nullptr) return fail(MSA_ERR_INVALID, "target or tokens is null");
-  if ((uintptr_t)target % es != 0 || (uintptr_t)draft % es != 0)
+  if (a->target == nullptr || a->tokens == nullptr) return fail(MSA_ERR_INVALID, "target or tokens is null");
+  if ((uintptr_t)a->target % es != 0 || (uintptr_t)a->draft % es != 0)
     return fail(MSA_ERR_INVALID, "target and draft must be aligned to their type");
-  if (t_sb < 0 || t_sn < 0 || d_sb < 0 || d_sn < 0 || par_sb < 0)
+  if (a->t_sb < 0 || a->t_sn < 0 || a->d_sb < 0 || a->d_sn < 0 || a->par_sb < 0)
     return fail(MSA_ERR_INVALID, "strides must not be negative");
-  if (path == nullptr || count == nullptr || token == nullptr)
+  if (a->path == nullptr || a->count == nullptr || a->token == nullptr)
     return fail(MSA_ERR_INVALID, "path, count or token is null");
-  const size_t need = msa_verify_workspace_bytes(B, M, V, uniforms == nullptr);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
-    return fail(MSA_ERR_WORKSPACE, "verify workspace holds %zu bytes, %zu needed", workspace_bytes, need);
-  if (need > 0 && !aligned16(workspace)) return fail(MSA_ERR_INVALID, "workspace is not 16-byte aligned");
+  const size_t need = msa_verify_workspace_bytes(B, M, a->V, a->uniforms == nullptr);
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need))
+    return fail(MSA_ERR_WORKSPACE, "verify workspace holds %zu bytes, %zu needed", (size_t)a->workspace_bytes, need);
+  if (need > 0 && !aligned16(a->workspace)) return fail(MSA_ERR_INVALID, "workspace is not 16-byte aligned");
   msa::VerifyCall c;
-  c.B = B; c.M = M; c.V = V; c.dtype = dtype;
-  c.target = target; c.t_sb = t_sb; c.t_sn = t_sn; c.draft = draft; c.d_sb = d_sb; c.d_sn = d_sn;
-  c.tokens = tokens; c.parents = parents; c.par_sb = par_sb; c.uniforms = uniforms;
-  c.path = path; c.count = count; c.token = token; c.best = (unsigned long long*)workspace;
+  c.B = B; c.M = M; c.V = a->V; c.dtype = dtype;
+  c.target = a->target; c.t_sb = a->t_sb; c.t_sn = a->t_sn; c.draft = a->draft; c.d_sb = a->d_sb; c.d_sn = a->d_sn;
+  c.tokens = a->tokens; c.parents = a->parents; c.par_sb = a->par_sb; c.uniforms = a->uniforms;
+  c.path = a->path; c.count = a->count; c.token = a->token; c.best = (unsigned long long*)a->workspace;
   c.stream = (hipStream_t)stream;
   return hip_status(msa::launch_verify(c), "msa_verify launch");
 }

@@ -6,6 +6,7 @@ fails loudly (RuntimeError) when it is missing: there is no other GPU path.
 
 import ctypes
 import os
+import struct
 import threading
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmsa.so")
@@ -31,6 +32,13 @@ _f = ctypes.c_float
 _u64 = ctypes.c_uint64
 _sz = ctypes.c_size_t
 
+# Argument structs of include/msa.h, packed to bytes (every field 8 wide): msa_cache_args and msa_verify_args
+# are integers and pointers, msa_tree_args ends with its eps.
+_args = ctypes.c_char_p
+pack_cache_args = struct.Struct("=37q").pack
+pack_tree_args = struct.Struct("=37qd").pack
+pack_verify_args = struct.Struct("=19q").pack
+
 _SIGS = {
     "msa_version": (_i, []),
     "msa_last_error": (ctypes.c_char_p, []),
@@ -51,17 +59,12 @@ _SIGS = {
                            _i, _i, _i, _i, _p, _i, _i, _p, _p, _f, _p, _p, _sz, _p]),
     "msa_decode_noalloc": (_i, [_p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
                                 _i, _i, _i, _i, _i, _i, _i, _p, _p, _f, _p, _p]),
-    "msa_cache_write": (_i, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i, _i, _i, _i, _i, _p, _p, _p, _i, _i64,
-                             _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i,
-                             _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p]),
-    "msa_cache_read": (_i, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i,
-                            _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i, _i, _i, _i, _p, _i, _i64, _p, _p, _p]),
+    "msa_cache_write": (_i, [_args, _p]),
+    "msa_cache_read": (_i, [_args, _p]),
     "msa_tree_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
-    "msa_tree_decode": (_i, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i,
-                             _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i, _i, _i, _i,
-                             _p, _i, _p, _i64, _i, _p, _p, _f, _p, _p, _sz, _p]),
+    "msa_tree_decode": (_i, [_args, _p]),
     "msa_verify_workspace_bytes": (_sz, [_i, _i, _i64, _i]),
-    "msa_verify": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _i, _i, _i64, _i, _p, _p, _p, _p, _sz, _p]),
+    "msa_verify": (_i, [_args, _p]),
     "msa_timer_arm": (_i, [_i, _i]),
     "msa_timer_arm_every": (_i, [_i, _i, _i]),
     "msa_timer_read": (_i, [_i, ctypes.POINTER(ctypes.c_float), _i]),

@@ -250,16 +250,16 @@ def decode_step_at(q, kcache, vcache, last_pos, r, w, eps=1e-8, workspace=None, 
 # ---------------------------------------------------------------------------
 _CACHE_DTYPES = {**_DTYPES, torch.int8: _native.MSA_I8, torch.float8_e4m3fn: _native.MSA_FP8}
 CODE_DTYPES = (torch.int8, torch.float8_e4m3fn)
-_NO_SCALES = (None, 0, 0, 0)
+_NO_SCALES = (0, 0, 0, 0)
 
 
 def _launch(what, fn, index, args):
-    """Calls fn(*args, stream) for tensors of GPU `index`, whichever device is current."""
+    """Calls fn(args, stream) for tensors of GPU `index`, whichever device is current."""
     if torch.cuda.current_device() == index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
     if rc != 0:
         _native.check(rc, what)
 
@@ -319,17 +319,17 @@ def _cache_args(what, kcache, vcache, kscale, vscale, dtype):
         if kscale is not None or vscale is not None:
             raise ValueError(f"{what}: a cache of {kcache.dtype} takes no scales")
         return pair, _NO_SCALES + _NO_SCALES
-    shape = kcache.shape[:3]
+    B, cap, H, _ = kcache.shape
     if kscale is None or vscale is None or kscale.dtype != torch.float32 or vscale.dtype != torch.float32 \
-            or kscale.shape != shape or vscale.shape != shape:
-        raise ValueError(f"{what}: a cache of {kcache.dtype} needs kscale and vscale, float32 {tuple(shape)}")
+            or kscale.shape != (B, cap, H) or vscale.shape != (B, cap, H):
+        raise ValueError(f"{what}: a cache of {kcache.dtype} needs kscale and vscale, float32 ({B}, {cap}, {H})")
     return pair, (kscale.data_ptr(), *kscale.stride(), vscale.data_ptr(), *vscale.stride())
 
 
 def _start_args(start, B):
-    """(pointer or None, count, host value, tensor to keep) of an int or int64 device tensor."""
+    """(pointer or 0, count, host value, tensor to keep) of an int or int64 device tensor."""
     if not torch.is_tensor(start):
-        return None, 0, int(start), None
+        return 0, 0, int(start), None
     start = _index(start, "start", (1,), (B,))
     return start.data_ptr(), start.shape[0], 0, start
 
@@ -362,7 +362,7 @@ def cache_write(k, v, kcache, vcache, start, kscale=None, vscale=None, rows=None
     Bc, cap, Hc, Dc = kcache.shape
     if Bc != B or Hc != H or Dc != D:
         raise ValueError(f"cache_write: cache {tuple(kcache.shape)} does not match rows {tuple(k.shape)}")
-    T, rp, cp = Tx, None, None
+    T, rp, cp = Tx, 0, 0
     if rows is not None:
         T = rows.shape[-1]
         rows = _index(rows, "rows", (B, T))
@@ -371,11 +371,11 @@ def cache_write(k, v, kcache, vcache, start, kscale=None, vscale=None, rows=None
         count = _index(count, "count", (B,))
         cp = count.data_ptr()
     sp, n, host, start = _start_args(start, B)
-    if sp is None and (host < 0 or host + (T if count is None else 0) > cap):
+    if not sp and (host < 0 or host + (T if count is None else 0) > cap):
         raise IndexError(f"KV cache capacity {cap} exceeded at position {host + T}")
     _launch("msa_cache_write", _native.lib().msa_cache_write, index,
-            (*kargs, *vargs, B, T, Tx, H, D, _DTYPES[dtype], rp, cp, sp, n, host, *pair, cap,
-             _CACHE_DTYPES[kcache.dtype], *scales))
+            _native.pack_cache_args(*kargs, *vargs, *pair, *scales, rp, cp, sp, n, host, B, T, Tx, H, D, _DTYPES[dtype],
+                                    cap, _CACHE_DTYPES[kcache.dtype]))
 
 
 def cache_read(kcache, vcache, kscale, vscale, start, length, dtype):
@@ -391,20 +391,21 @@ def cache_read(kcache, vcache, kscale, vscale, start, length, dtype):
     B, cap, H, D = kcache.shape
     length = int(length)
     sp, n, host, start = _start_args(start, B)
-    if length < 0 or (sp is None and (host < 0 or host + length > cap)):
+    if length < 0 or (not sp and (host < 0 or host + length > cap)):
         raise IndexError(f"positions {host} .. {host + length} are outside the KV cache's capacity {cap}")
     k = torch.empty((B, length, H, D), dtype=dtype, device=kcache.device)
     v = torch.empty_like(k)
     _launch("msa_cache_read", _native.lib().msa_cache_read, index,
-            (*pair, cap, _CACHE_DTYPES[kcache.dtype], *scales, B, length, H, D, _DTYPES[dtype], sp, n, host,
-             k.data_ptr(), v.data_ptr()))
+            _native.pack_cache_args(k.data_ptr(), length * H * D, H * D, D, v.data_ptr(), length * H * D, H * D, D, *pair,
+                                    *scales, 0, 0, sp, n, host, B, length, length, H, D, _DTYPES[dtype], cap,
+                                    _CACHE_DTYPES[kcache.dtype]))
     return k, v
 
 
 def _parents_arg(parents, B, N):
-    """(pointer or None, stride over sequences, tensor to keep) of parents (N,) or (B, N), or None: a chain."""
+    """(pointer or 0, stride over sequences, tensor to keep) of parents (N,) or (B, N), or None: a chain."""
     if parents is None:
-        return None, 0, None
+        return 0, 0, None
     parents = _index(parents, "parents", (B, N), (N,))
     return parents.data_ptr(), N if parents.dim() == 2 else 0, parents
 
@@ -454,9 +455,9 @@ def tree_decode(q, kcache, vcache, lengths, parents, r, w, eps=1e-8, kscale=None
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
         workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
     _launch("msa_tree_decode", L.msa_tree_decode, index,
-            (*qargs, *pair, cap, ct, *scales, B, N, H, D, qt, lengths.data_ptr(), lengths.shape[0], par, par_sb, hint,
-             r.data_ptr(), w.data_ptr(), float(eps), y.data_ptr(),
-             workspace.data_ptr() if need else None, need))
+            _native.pack_tree_args(*qargs, *pair, *scales, lengths.data_ptr(), par, r.data_ptr(), w.data_ptr(), y.data_ptr(),
+                                   workspace.data_ptr() if need else 0, need, lengths.shape[0], par_sb, B, N, H, D, qt,
+                                   cap, ct, hint, float(eps)))
     return y
 
 
@@ -494,7 +495,7 @@ def verify_drafts(target, tokens, parents=None, uniforms=None, draft=None):
         raise ValueError(f"verify_drafts: a tree holds 1 to {_native.TREE_MAX} nodes, got {M}")
     tokens = _index(tokens, "tokens", (B, M))
     par, par_sb, parents = _parents_arg(parents, B, M)
-    up = dp = None
+    up = dp = 0
     d_sb = d_sn = 0
     if uniforms is not None:
         if uniforms.dtype != torch.float32 or uniforms.shape != (B, M):
@@ -508,7 +509,7 @@ def verify_drafts(target, tokens, parents=None, uniforms=None, draft=None):
             raise ValueError(f"draft must be {dtype} ({B}, {M - 1}, {V}), got {draft.dtype} {tuple(draft.shape)}")
         draft = draft if draft.stride(2) == 1 else draft.contiguous()
         d_sb, d_sn, _ = draft.stride()
-        dp = draft.data_ptr() if M > 1 else None  # a chain of one node has no draft rows: nothing can be refused
+        dp = draft.data_ptr() if M > 1 else 0  # a chain of one node has no draft rows: nothing can be refused
     target = target if target.stride(2) == 1 else target.contiguous()
     t_sb, t_sn, _ = target.stride()
     L = _native.lib()
@@ -520,6 +521,7 @@ def verify_drafts(target, tokens, parents=None, uniforms=None, draft=None):
         need = L.msa_verify_workspace_bytes(B, M, V, 1)
         workspace = torch.empty((need,), dtype=torch.uint8, device=target.device)
     _launch("msa_verify", L.msa_verify, index,
-            (target.data_ptr(), t_sb, t_sn, dp, d_sb, d_sn, tokens.data_ptr(), par, par_sb, up, B, M, V, _DTYPES[dtype],
-             path.data_ptr(), count.data_ptr(), token.data_ptr(), workspace.data_ptr() if need else None, need))
+            _native.pack_verify_args(target.data_ptr(), t_sb, t_sn, dp, d_sb, d_sn, tokens.data_ptr(), par, par_sb, up,
+                                     path.data_ptr(), count.data_ptr(), token.data_ptr(),
+                                     workspace.data_ptr() if need else 0, need, B, M, V, _DTYPES[dtype]))
     return path, count, token

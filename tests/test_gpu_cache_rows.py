@@ -262,21 +262,25 @@ def test_c_entries_refuse_bad_arguments():
     from multiscreen import _native
     L = _native.lib()
 
-    def write(**kw):
-        a = dict(k=16, ks=(512, 128, 64), B=2, T=3, Tx=3, H=2, D=64, dt=1, rows=None, count=None, start=None, n=0, s0=0,
+    def pack(**kw):
+        a = dict(k=16, ks=(512, 128, 64), B=2, T=3, Tx=3, H=2, D=64, dt=1, rows=0, count=0, start=0, n=0, s0=0,
                  c=16, cs=(1024, 64, 512), cap=8, ct=3, sc=16, ss=(16, 1, 8))
         a.update(kw)
-        return L.msa_cache_write(a["k"], *a["ks"], a["k"], *a["ks"], a["B"], a["T"], a["Tx"], a["H"], a["D"], a["dt"],
-                                 a["rows"], a["count"], a["start"], a["n"], a["s0"], a["c"], *a["cs"], a["c"], *a["cs"],
-                                 a["cap"], a["ct"], a["sc"], *a["ss"], a["sc"], *a["ss"], None)
+        pair, cpair, spair = (a["k"], *a["ks"]), (a["c"], *a["cs"]), (a["sc"], *a["ss"])
+        return _native.pack_cache_args(*pair, *pair, *cpair, *cpair, *spair, *spair, a["rows"], a["count"], a["start"], a["n"],
+                                       a["s0"], a["B"], a["T"], a["Tx"], a["H"], a["D"], a["dt"], a["cap"], a["ct"])
+
+    def write(**kw):
+        return L.msa_cache_write(pack(**kw), None)
 
     for kw, msg in ((dict(D=48), "head_dim"), (dict(dt=3), "dtype"), (dict(ct=2), "cache_dtype"), (dict(ct=5), "cache_dtype"),
-                    (dict(sc=None), "scales"), (dict(c=None), "null"), (dict(c=8), "aligned"), (dict(cs=(1024, 8, 512)), "multiples"),
-                    (dict(k=None), "null"), (dict(ks=(512, 4, 64)), "strides"), (dict(T=4), "rows"), (dict(start=16, n=3), "start"),
-                    (dict(ss=(16, -1, 8)), "strides"), (dict(B=70000, H=1), "B*H")):
+                    (dict(sc=0), "scales"), (dict(c=0), "null"), (dict(c=8), "aligned"), (dict(cs=(1024, 8, 512)), "multiples"),
+                    (dict(k=0), "null"), (dict(ks=(512, 4, 64)), "strides"), (dict(T=4), "rows"), (dict(start=16, n=3), "start"),
+                    (dict(ss=(16, -1, 8)), "strides"), (dict(B=70000, H=1), "B*H"), (dict(B=-1), "size"), (dict(T=2 ** 40), "size"), (dict(cs=(1024, 2 ** 26, 512)), "span")):
         assert write(**kw) == 1, kw
         assert msg in L.msa_last_error().decode(), (kw, L.msa_last_error())
     assert write(B=0) == 0 and write(T=0) == 0
-    rc = L.msa_cache_read(16, 1024, 64, 512, 16, 1024, 64, 512, 8, 3, 16, 16, 1, 8, 16, 16, 1, 8, 2, 3, 2, 64, 1,
-                          None, 0, 0, None, 16, None)
-    assert rc == 1 and "k is null" in L.msa_last_error().decode()
+    for kw, msg in ((dict(k=0), "k is null"), (dict(rows=16), "no rows"), (dict(count=16), "no rows"), (dict(T=4), "rows")):
+        assert L.msa_cache_read(pack(**kw), None) == 1, kw
+        assert msg in L.msa_last_error().decode(), (kw, L.msa_last_error())
+    assert L.msa_cache_write(None, None) == 1 and b"args is null" in L.msa_last_error()

@@ -407,18 +407,20 @@ def test_c_entry_refuses_bad_arguments():
     L = _native.lib()
 
     def tree(**kw):
-        a = dict(q=16, qs=(512, 128, 64), c=16, cs=(25600000, 64, 12800000), cap=200000, ct=3, s=16, ss=(400000, 1, 200000), B=2, N=4, H=2, D=64,
-                 dt=1, n=16, nn=2, par=None, psb=0, hint=0, r=16, w=16, eps=1e-8, y=16, ws=16, wsb=1 << 30)
+        a = dict(q=16, qs=(512, 128, 64), c=16, cs=(25600000, 64, 12800000), cap=200000, ct=3, s=16, ss=(400000, 1, 200000), B=2, N=4,
+                 H=2, D=64, dt=1, n=16, nn=2, par=0, psb=0, hint=0, r=16, w=16, eps=1e-8, y=16, ws=16, wsb=1 << 30)
         a.update(kw)
-        return L.msa_tree_decode(a["q"], *a["qs"], a["c"], *a["cs"], a["c"], *a["cs"], a["cap"], a["ct"], a["s"], *a["ss"],
-                                 a["s"], *a["ss"], a["B"], a["N"], a["H"], a["D"], a["dt"], a["n"], a["nn"], a["par"], a["psb"],
-                                 a["hint"], a["r"], a["w"], a["eps"], a["y"], a["ws"], a["wsb"], None)
+        c, s = (a["c"], *a["cs"]), (a["s"], *a["ss"])
+        return L.msa_tree_decode(_native.pack_tree_args(a["q"], *a["qs"], *c, *c, *s, *s, a["n"], a["par"], a["r"], a["w"], a["y"],
+                                                        a["ws"], a["wsb"], a["nn"], a["psb"], a["B"], a["N"], a["H"], a["D"], a["dt"],
+                                                        a["cap"], a["ct"], a["hint"], a["eps"]), None)
 
     for kw, code, msg in ((dict(N=65), 1, "at most 64"), (dict(N=4, cap=3), 1, "do not hold"), (dict(D=48), 1, "head_dim"),
-                          (dict(ct=0), 1, "cache_dtype"), (dict(q=None), 1, "q is null"), (dict(qs=(512, 4, 64)), 1, "strides"),
-                          (dict(n=None), 1, "lengths"), (dict(nn=3), 1, "lengths"), (dict(r=None), 1, "r and w"),
-                          (dict(eps=0.0), 1, "eps"), (dict(y=8), 1, "aligned"), (dict(s=None), 1, "scales"),
-                          (dict(wsb=16), 2, "tree workspace"), (dict(ws=None), 2, "tree workspace"), (dict(psb=-1), 1, "parents")):
+                          (dict(ct=0), 1, "cache_dtype"), (dict(q=0), 1, "q is null"), (dict(qs=(512, 4, 64)), 1, "strides"),
+                          (dict(n=0), 1, "lengths"), (dict(nn=3), 1, "lengths"), (dict(r=0), 1, "r and w"),
+                          (dict(eps=0.0), 1, "eps"), (dict(y=8), 1, "aligned"), (dict(s=0), 1, "scales"),
+                          (dict(wsb=16), 2, "tree workspace"), (dict(ws=0), 2, "tree workspace"), (dict(psb=-1), 1, "parents"),
+                          (dict(H=32768, B=1, cap=2 ** 22), 1, "2^35"), (dict(N=2 ** 33), 1, "size")):
         assert tree(**kw) == code, kw
         assert msg in L.msa_last_error().decode(), (kw, L.msa_last_error())
     assert tree(B=0) == 0 and tree(N=0) == 0

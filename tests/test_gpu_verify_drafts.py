@@ -285,15 +285,15 @@ def test_c_entry_refuses_bad_arguments():
     L = _native.lib()
 
     def verify(**kw):
-        a = dict(t=16, d=None, tok=16, par=None, psb=0, u=16, B=2, M=4, V=100, dt=0, path=16, count=16, token=16, ws=None, wsb=0)
+        a = dict(t=16, d=0, tok=16, par=0, psb=0, u=16, B=2, M=4, V=100, dt=0, path=16, count=16, token=16, ws=0, wsb=0)
         a.update(kw)
-        return L.msa_verify(a["t"], 400, 100, a["d"], 300, 100, a["tok"], a["par"], a["psb"], a["u"], a["B"], a["M"], a["V"], a["dt"],
-                            a["path"], a["count"], a["token"], a["ws"], a["wsb"], None)
+        return L.msa_verify(_native.pack_verify_args(a["t"], 400, 100, a["d"], 300, 100, a["tok"], a["par"], a["psb"], a["u"], a["path"],
+                                                     a["count"], a["token"], a["ws"], a["wsb"], a["B"], a["M"], a["V"], a["dt"]), None)
 
     for kw, code, msg in ((dict(dt=3), 1, "dtype"), (dict(M=65), 1, "nodes"), (dict(M=0), 1, "nodes"), (dict(V=0), 1, "vocabulary"),
-                          (dict(V=1 << 31), 1, "vocabulary"), (dict(u=None, d=16), 1, "uniforms"), (dict(t=None), 1, "null"),
-                          (dict(t=18), 1, "aligned"), (dict(path=None), 1, "null"), (dict(psb=-1), 1, "strides"),
-                          (dict(u=None), 2, "verify workspace")):
+                          (dict(V=1 << 31), 1, "vocabulary"), (dict(u=0, d=16), 1, "uniforms"), (dict(t=0), 1, "null"),
+                          (dict(t=18), 1, "aligned"), (dict(path=0), 1, "null"), (dict(psb=-1), 1, "strides"),
+                          (dict(u=0), 2, "verify workspace")):
         assert verify(**kw) == code, kw
         assert msg in L.msa_last_error().decode(), (kw, L.msa_last_error())
     assert verify(B=0) == 0
