@@ -38,6 +38,14 @@ constexpr int kTreeMinUnits = 8, kTreeSmall = 16;
 constexpr int tree_occupancy(int row_bytes, int parts) {
   return row_bytes * parts <= 64 ? 3 : row_bytes <= 256 ? 2 : 1;
 }
+#ifndef O16A
+#define O16A 4
+#define O16B 3
+#define O16C 2
+#endif
+constexpr int tree_occupancy16(int row_bytes, int parts) {  // the same of tree16_kernel
+  return row_bytes * parts <= 64 ? O16A : row_bytes * parts <= 128 ? O16B : O16C;
+}
 
 // How a cache row of type C enters the products.
 template <typename C> struct TreeRow {
@@ -329,6 +337,15 @@ struct ValueRows {
   }
 };
 
+// The values of unit u of a window whose rows (of `st` bytes) and scales start
+// at `rows` and `scales` and end with row `last`.
+template <typename C, int D>
+__device__ inline void load_values_at(ValueRows<C, D>& val, const char* rows, int64_t st, const char* scales,
+                                      int64_t scale_st, int u, int last, int lane) {
+  val.load(rows + (int64_t)u * kUnit * st, (uint32_t)st, scales + (int64_t)u * kUnit * scale_st * 4,
+           (uint32_t)(scale_st * 4), last - u * kUnit, lane);
+}
+
 // Where a C block's registers (rows = tcol-ordered columns) go: groups of
 // consecutive columns of one row.
 template <typename COMP, typename OUT, int D, typename Fn>
@@ -532,10 +549,6 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C),
     key.load(kb + (int64_t)u * kUnit * kst, (uint32_t)r * (uint32_t)kst + half * K::LB,
              ksc + (int64_t)u * kUnit * a.kss.st * 4, (uint32_t)r * (uint32_t)(a.kss.st * 4));
   };
-  auto load_values = [&](V& val, int u) {
-    val.load(vb + (int64_t)u * kUnit * vst, (uint32_t)vst, vsc + (int64_t)u * kUnit * a.vss.st * 4,
-             (uint32_t)(a.vss.st * 4), last - u * kUnit, lane);
-  };
   // Keys are in flight a unit ahead; values are asked for once the vote has
   // found a live pair and arrive behind its weights.  (Asked for with the keys
   // where the last unit was live, they cost registers: 4 x 64 nodes over 30K bf16
@@ -612,7 +625,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C),
     }
     if (__ballot(vote) == 0ull) continue;
     V val;
-    load_values(val, u);
+    load_values_at<C, D>(val, vb, vst, vsc, a.vss.st, u, last, lane);
 
     // a^2 m of every pair: register r is key row 16 (r/8) + 8 half + r%8 (the
     // clamp takes a NaN to 0)
@@ -759,6 +772,381 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C),
   }
 }
 
+// ---------------------------------------------------------------------------
+// Trees of at most 16 nodes: the same walk on the 16x16x32 product, whose block
+// of 16 columns halves the per-pair work (and the sums' registers) that 32
+// columns would spend on absent nodes.  2-byte operands only.
+//
+//   Operands: lane l supplies row (A) / column (B) l%16 and the 8 contraction
+//   slots of group l/16.  C block: lane l, register r -> row 4 (l/16) + r, column
+//   l%16.
+// A unit's keys are two row blocks t; block row m holds unit row 8 (m/4) + 4 t +
+// m%4, so that a lane's registers (t, r) are unit rows 8 (l/16) + 4 t + r: the
+// eight slots it supplies to the value product.  The value columns of block d
+// likewise: row m holds column 32 (d/2) + 8 (m/4) + 4 (d%2) + m%4, and a lane's
+// registers of two blocks are 8 consecutive columns.
+// ---------------------------------------------------------------------------
+template <typename T> struct Mma16;
+template <> struct Mma16<bf16> {
+  __device__ static inline f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct Mma16<f16> {
+  __device__ static inline f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <typename F, int N>
+__device__ inline void guard_all16(const F (&f)[N], const f32x4& c) {
+  asm volatile(MSA_NOP16 ::"v"(c[3]));
+#pragma unroll
+  for (int k = 0; k < N; ++k) asm volatile("" ::"v"(f[k]));
+}
+// Sum over the four lanes l%16 + 16 i.
+__device__ inline float quarter_sum(float x) { return half_sum(x + __shfl_xor(x, 16)); }
+__device__ inline float quarter_max(float x) { return half_max(fmaxf(x, __shfl_xor(x, 16))); }
+
+template <typename C, int D>
+struct KeyRows16 {
+  using comp = typename TreeRow<C>::comp;
+  typedef typename Mma<comp>::frag frag;
+  static constexpr bool kCodes = TreeRow<C>::kCodes;
+  static constexpr int NKS = D < 32 ? 1 : D / 32;
+  static constexpr int LB = kCodes && D <= 32 ? 8 : 16;                      // bytes of a load
+  static constexpr int NL = D < 32 ? 1 : D * (int)sizeof(C) / (4 * LB);      // loads of a lane and block
+  static constexpr bool kHalf = D < 32;                                      // groups 2, 3 hold no columns
+  u32x4 raw[2][NL];
+  float scale[2];
+
+  __device__ static inline int row(int t, int lane) { return 8 * ((lane & 15) >> 2) + 4 * t + (lane & 3); }
+  __device__ static constexpr int col(int ks, int g) {
+    if constexpr (kCodes && D >= 64) return 64 * (ks / 2) + 16 * g + 8 * (ks & 1);
+    else return 32 * ks + 8 * (kHalf ? g & 1 : g);
+  }
+  // `off[t]`: block t's row of this lane and its group's first bytes.
+  __device__ inline void load(const char* rows, const uint32_t (&off)[2], const char* scales, const uint32_t (&soff)[2]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const char* p = rows + off[t] + 4 * i * LB;
+        if constexpr (LB == 8) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+          raw[t][i] = u32x4{x[0], x[1], 0u, 0u};
+        } else {
+          raw[t][i] = *reinterpret_cast<const u32x4*>(p);
+        }
+      }
+      if constexpr (kCodes) scale[t] = *reinterpret_cast<const float*>(scales + soff[t]);
+    }
+  }
+  __device__ inline void frags(int t, int lane, frag (&f)[NKS]) const {
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      if constexpr (!kCodes) f[ks] = __builtin_bit_cast(frag, raw[t][ks]);
+      else if constexpr (D >= 64) f[ks] = decode8<C>(raw[t][ks / 2][2 * (ks & 1)], raw[t][ks / 2][2 * (ks & 1) + 1]);
+      else f[ks] = decode8<C>(raw[t][0][0], raw[t][0][1]);
+      if (kHalf && lane >= 32) f[ks] = Mma<comp>::zero();
+    }
+  }
+  __device__ inline float factor(int t, const frag (&f)[NKS], float eps) const {
+    const float ss = quarter_sum(row_dot<comp>(f, f));
+    if constexpr (kCodes) return KeyRows<C, D>::code_factor(ss, scale[t], eps);
+    else return inv_len_of<C>(ss, eps);
+  }
+};
+
+template <typename C, int D, int PARTS>
+struct NodeRows16 {
+  using K = KeyRows16<C, D>;
+  typename K::frag f[PARTS][K::NKS];
+  float inv;
+  template <typename T>
+  __device__ inline void load(const T* row, bool ok, float eps, int g) {
+    constexpr int VEC = 16 / (int)sizeof(T);
+    float x[K::NKS][8];
+    float ss = 0.0f, mx = 0.0f;
+    ok = ok && !(K::kHalf && g >= 2);
+#pragma unroll
+    for (int ks = 0; ks < K::NKS; ++ks)
+#pragma unroll
+      for (int e0 = 0; e0 < 8; e0 += VEC) {
+        typedef __attribute__((__vector_size__(16))) T vec;
+        const vec v = *reinterpret_cast<const vec*>(row + K::col(ks, g) + e0);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[ks][e0 + e] = ok ? to_f(v[e]) : 0.0f;
+      }
+#pragma unroll
+    for (int ks = 0; ks < K::NKS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        ss = fmaf(x[ks][e], x[ks][e], ss);
+        mx = fmaxf(mx, fabsf(x[ks][e]));
+      }
+    const float p = TreeRow<C>::kCodes ? row_pow2(quarter_max(mx)) : 1.0f;
+    inv = inv_len_of<float>(quarter_sum(ss), eps) / p;
+#pragma unroll
+    for (int ks = 0; ks < K::NKS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float rest = x[ks][e] * p;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+          const auto part = from_f<typename K::comp>(rest);
+          f[i][ks][e] = part;
+          rest -= to_f(part);
+        }
+      }
+  }
+};
+
+template <typename C, int D, int PARTS>
+__global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy16(D * (int)sizeof(C), PARTS)) void tree16_kernel(TreeCall a) {
+  using K = KeyRows16<C, D>;
+  using V = ValueRows<C, D>;
+  using comp = typename K::comp;
+  using frag = typename K::frag;
+  using Tile = typename V::Tile;
+  constexpr int NDT = V::DP / 16;
+  constexpr int kRed = NDT * 1024;
+  constexpr int kLds = kTreeWaves * (Tile::BYTES > kRed / 2 ? Tile::BYTES : kRed / 2);
+  const bool two = !(TreeRow<C>::kCodes && PARTS == 1 && a.q_dtype == 1);
+  __shared__ __align__(16) char lds[kLds];
+  __shared__ __align__(16) float kfac[kTreeWaves][kUnit], vfac[kTreeWaves][kUnit], mtab[kTreeWaves][64];
+  __shared__ int dtab[kTreeWaves][kTreeMax];
+
+  const int lane = threadIdx.x & 63, g = lane >> 4, node = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.y;
+  const TreeSpan sp(a, b);
+  int h = blockIdx.x, u0 = 0, per = 0;
+  if (a.blocks != a.H) {
+    const TreeMap map(a, sp, lane);
+    int piece0 = 0;
+    h = map.head_of(a, sp, lane, blockIdx.x, piece0);
+    if (h < 0) return;
+    per = map.per;
+    u0 = ((int)blockIdx.x - piece0) * per;
+  }
+  const HeadParams hp = head_params(a.r, a.w, h, true);
+  const int units = sp.units(a, hp.wc), lo_key = sp.lo(hp.wc);
+  if (per == 0) per = units;
+  const int u1 = u0 + per < units ? u0 + per : units;
+
+  const int64_t kst = a.ks.st * (int64_t)sizeof(C), vst = a.vs.st * (int64_t)sizeof(C);
+  const char* kb = (const char*)a.kc + (b * a.ks.sb + h * a.ks.sh) * (int64_t)sizeof(C) + lo_key * kst;
+  const char* vb = (const char*)a.vc + (b * a.vs.sb + h * a.vs.sh) * (int64_t)sizeof(C) + lo_key * vst;
+  const char* ksc = (const char*)(a.kscale + b * a.kss.sb + h * a.kss.sh + lo_key * a.kss.st);
+  const char* vsc = (const char*)(a.vscale + b * a.vss.sb + h * a.vss.sh + lo_key * a.vss.st);
+  const int last = sp.n + a.N - 1 - lo_key;  // last key row, from the window's first
+  auto load_keys = [&](K& key, int u) {
+    const int lim = last - u * kUnit;
+    uint32_t off[2], soff[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      int r = K::row(t, lane);
+      if (lim < kUnit - 1) r = r < lim ? r : lim;
+      off[t] = (uint32_t)r * (uint32_t)kst + (K::kHalf ? g & 1 : g) * K::LB;
+      soff[t] = (uint32_t)r * (uint32_t)(a.kss.st * 4);
+    }
+    key.load(kb + (int64_t)u * kUnit * kst, off, ksc + (int64_t)u * kUnit * a.kss.st * 4, soff);
+  };
+  K key_next;
+  if (u0 + wave < u1) load_keys(key_next, u0 + wave);
+
+  const Tree tree(a.parents == nullptr ? nullptr : a.parents + b * a.par_sb, a.N, lane);
+  dtab[wave][lane] = tree.depth;
+  const int depth = __shfl(tree.depth, node);
+  const uint32_t above = (uint32_t)__shfl((int)tree.above, node);
+  NodeRows16<C, D, PARTS> q;
+  {
+    const bool ok = node < a.N;
+    const int64_t off = b * a.q_sb + (int64_t)(ok ? node : 0) * a.q_sn + h * a.q_sh;
+    if (a.q_dtype == 1) q.load((const bf16*)a.q + off, ok, a.eps, g);
+    else if (a.q_dtype == 2) q.load((const f16*)a.q + off, ok, a.eps, g);
+    else q.load((const float*)a.q + off, ok, a.eps, g);
+  }
+  char* vt = lds + wave * Tile::BYTES;
+  if constexpr (D < V::DP) {  // the columns past D
+#pragma unroll
+    for (int i = 0; i < Tile::BYTES / 1024; ++i)
+      *reinterpret_cast<u32x4*>(vt + i * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+  }
+  // value column operands: a 16-lane group transposes 4 rows x 16 columns; lane
+  // 4 k + q gives row k's columns 8 q + 4 (d%2) .. of block d
+  const int cr = 8 * g + ((lane & 15) >> 2), cq = lane & 3;
+  const uint32_t cbase = (uint32_t)(cr * Tile::ROWB + ((cq ^ Tile::swz(cr)) << 4));
+  auto value_frag = [&](int d) {
+    typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4;
+    typedef __attribute__((__vector_size__(8 * sizeof(short)))) short s16x8;
+    s16x8 v;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const char* p = vt + (cbase ^ (uint32_t)((Tile::swz(4 * j) ^ (4 * (d >> 1))) << 4)) + 4 * j * Tile::ROWB + 8 * (d & 1);
+      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)const_cast<char*>(p));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * j + e] = x[e];
+    }
+    return __builtin_bit_cast(frag, v);
+  };
+  f32x4 acc[NDT];
+#pragma unroll
+  for (int d = 0; d < NDT; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const int depth_max = a.parents == nullptr ? a.N - 1 : wave_max(tree.depth);
+
+  for (int u = u0 + wave; u < u1; u += kTreeWaves) {
+    const int k0 = lo_key + u * kUnit;
+    const K key = key_next;
+    if (u + kTreeWaves < u1) load_keys(key_next, u + kTreeWaves);
+    float s[8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      frag kf[K::NKS];
+      key.frags(t, lane, kf);
+      const float f = key.factor(t, kf, a.eps);
+      if (g == 0) kfac[wave][K::row(t, lane)] = f;
+      f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = PARTS - 1; i >= 0; --i)
+#pragma unroll
+        for (int ks = 0; ks < K::NKS; ++ks) c = Mma16<comp>::mma(kf[ks], q.f[i][ks], c);
+      guard_all16(kf, c);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[4 * t + r] = c[r];
+    }
+    wave_lds_sync();
+    float x[8];
+    auto read8 = [&](const float* p) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(p + 8 * g + 4 * t);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[4 * t + r] = v[r];
+      }
+    };
+    read8(kfac[wave]);
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      s[r] *= x[r];
+      top = fmaxf(top, s[r]);
+    }
+    if (__ballot(top * q.inv > hp.thr) == 0ull) continue;
+    V val;
+    load_values_at<C, D>(val, vb, vst, vsc, a.vss.st, u, last, lane);
+
+    float any = 0.0f;
+    if (k0 + kUnit <= sp.n) {
+      const int dmin = sp.n - k0 - 31, e = lane;  // entries 0 .. 31 + 15
+      if (e < 32 + depth_max) mtab[wave][e] = in_window(dmin + e, hp) ? mask_fast(dmin + e, hp.w, hp.iw) : 0.0f;
+      wave_lds_sync();
+      const float* mt = mtab[wave] + (depth + 24 - 8 * g);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const float av = __builtin_amdgcn_fmed3f(fmaf(-hp.r, fmaf(-s[r], q.inv, 1.0f), 1.0f), 0.0f, 1.0f);
+        s[r] = av * av * mt[7 - r];
+        any = fmaxf(any, s[r]);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const int j = k0 + 8 * g + r - sp.n;  // j >= 0: drafted
+        const bool draft = j >= 0;
+        const int dd = depth - (draft ? dtab[wave][j & (kTreeMax - 1)] : j);
+        const bool seen = draft ? j < a.N && ((above >> (j & 31)) & 1u) != 0u : true;
+        const float av = __builtin_amdgcn_fmed3f(fmaf(-hp.r, fmaf(-s[r], q.inv, 1.0f), 1.0f), 0.0f, 1.0f);
+        s[r] = seen && in_window(dd, hp) ? av * av * mask_fast(dd, hp.w, hp.iw) : 0.0f;
+        any = fmaxf(any, s[r]);
+      }
+    }
+    if (__ballot(any > 0.0f) == 0ull) continue;
+
+    const bool odd = val.stage(vt, vfac[wave], a.eps, lane);
+    wave_lds_sync();
+    read8(vfac[wave]);
+    if (odd) {  // a NaN factor reaches live pairs only
+#pragma unroll
+      for (int r = 0; r < 8; ++r) s[r] = s[r] > 0.0f ? s[r] * x[r] : 0.0f;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) s[r] *= x[r];
+    }
+    frag w[2];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[0][e] = from_f<comp>(s[e]);
+    asm volatile("" : "+v"(w[0]));  // one rounding for both its uses (tree_kernel)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[1][e] = two ? from_f<comp>(s[e] - to_f(w[0][e])) : from_f<comp>(0.0f);
+    frag vf[NDT];
+#pragma unroll
+    for (int d = 0; d < NDT; ++d) vf[d] = value_frag(d);
+#pragma unroll
+    for (int d = 0; d < NDT; ++d) acc[d] = Mma16<comp>::mma(vf[d], w[0], acc[d]);
+    if (two) {
+#pragma unroll
+      for (int d = 0; d < NDT; ++d) acc[d] = Mma16<comp>::mma(vf[d], w[1], acc[d]);
+    }
+    guard_all16(vf, acc[NDT - 1]);
+    guard_all16(w, acc[NDT - 1]);
+  }
+
+  // the waves' sums, the upper half of them into the lower, until one has all
+  for (int step = kTreeWaves / 2; step >= 1; step /= 2) {
+    char* red = lds + (wave % step) * kRed + lane * 16;
+    __syncthreads();
+    if (wave >= step && wave < 2 * step) {
+#pragma unroll
+      for (int d = 0; d < NDT; ++d) *reinterpret_cast<f32x4*>(red + d * 1024) = acc[d];
+    }
+    __syncthreads();
+    if (wave < step) {
+#pragma unroll
+      for (int d = 0; d < NDT; ++d) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(red + d * 1024);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[d][e] += y[e];
+      }
+    }
+  }
+  if (wave != 0) return;
+  constexpr float down = 1.0f / kWeightUp<C>;
+  float fy = down;
+  if (a.blocks == a.H) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int d = 0; d < NDT; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) ss = fmaf(acc[d][r] * down, acc[d][r] * down, ss);
+    const float nc = fmaxf(sqrtf(quarter_sum(ss)), a.eps);
+    fy = down * (tanhf(nc) / nc);
+  }
+  if (node >= a.N) return;
+  auto store = [&](auto* row) {
+#pragma unroll
+    for (int j = 0; j < NDT / 2; ++j) {
+      const int d0 = 32 * j + 8 * g;
+      if (d0 < D) {
+        float v[8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          v[r] = acc[2 * j][r] * fy;
+          v[4 + r] = acc[2 * j + 1][r] * fy;
+        }
+        store8(row + d0, v);
+      }
+    }
+  };
+  if (a.blocks != a.H) {
+    store(a.part + (((int64_t)b * a.blocks + blockIdx.x) * a.N + node) * D);
+    return;
+  }
+  const int64_t at = (((int64_t)b * a.N + node) * a.H + h) * D;
+  if (a.q_dtype == 1) store((bf16*)a.y + at);
+  else if (a.q_dtype == 2) store((f16*)a.y + at);
+  else store((float*)a.y + at);
+}
+
 // Sum of a node's block sums and TanhNorm: a wave per node, D/4 lanes for a
 // block's sums and 256/D blocks at a time.
 template <int D>
@@ -792,6 +1180,8 @@ int tree_max_nodes() { return kTreeMax; }
 // Whether a wave takes all of more than 32 nodes: its registers hold two tiles'
 // operands and sums for rows of at most 64 values in 2-byte operands.
 bool tree_both(int N, int D, bool f32) { return N > 32 && D <= 64 && !f32; }
+// Whether a tree takes the 16-column form.
+bool tree_few(int N, bool f32_operands) { return N <= 16 && !f32_operands; }
 // Blocks of a sequence: as many as run at one time on the card's 256 CUs share
 // its heads' keys; one a head (H) where heads are short, or the batch alone
 // fills the card several times over with heads that are not long.
@@ -800,7 +1190,9 @@ int tree_blocks(int B, int H, int N, int D, int q_dtype, int cache_dtype, int sp
   const bool codes = cache_dtype == kInt8 || cache_dtype == kFp8;
   const int row = D * (codes ? 1 : cache_dtype == 0 ? 4 : 2);
   const bool f32 = codes ? q_dtype == 0 : cache_dtype == 0;
-  const int slots = 256 * tree_occupancy(row, codes && q_dtype == 0 ? 2 : tree_both(N, D, f32) ? 2 : 1);
+  const int parts = codes && q_dtype == 0 ? 2 : 1;
+  const int slots = 256 * (tree_few(N, !codes && f32) ? tree_occupancy16(row, parts)
+                                                      : tree_occupancy(row, tree_both(N, D, f32) ? 2 : parts));
   if (units <= kTreeSmall || ((int64_t)B * H >= 2 * slots && units <= 4 * kTreeSmall)) return H;
   const int each = slots / B;
   return each < 2 * H ? 2 * H : each;
@@ -808,7 +1200,9 @@ int tree_blocks(int B, int H, int N, int D, int q_dtype, int cache_dtype, int sp
 
 template <typename C, int D, int PARTS, int T>
 static hipError_t launch_tree_t(const TreeCall& c) {
-  hipLaunchKernelGGL((tree_kernel<C, D, PARTS, T>), dim3((unsigned)c.blocks, (unsigned)c.B), dim3(64 * kTreeWaves), 0, c.stream, c);
+  const dim3 grid((unsigned)c.blocks, (unsigned)c.B), block(64 * kTreeWaves);
+  if constexpr (T == 0) hipLaunchKernelGGL((tree16_kernel<C, D, PARTS>), grid, block, 0, c.stream, c);
+  else hipLaunchKernelGGL((tree_kernel<C, D, PARTS, T>), grid, block, 0, c.stream, c);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || c.blocks == c.H) return e;
   hipLaunchKernelGGL((tree_reduce_kernel<D>), dim3((unsigned)((c.N + 3) / 4), (unsigned)(c.B * c.H)), dim3(256), 0, c.stream, c);
@@ -817,6 +1211,8 @@ static hipError_t launch_tree_t(const TreeCall& c) {
 template <typename C, int D, int PARTS>
 static hipError_t launch_tree_n(const TreeCall& c) {
   constexpr bool f32 = PARTS == 2 || __is_same(C, float);
+  if constexpr (!__is_same(C, float))
+    if (tree_few(c.N, false)) return launch_tree_t<C, D, PARTS, 0>(c);
   if constexpr (D <= 64 && !f32)
     if (tree_both(c.N, D, f32)) return launch_tree_t<C, D, PARTS, 2>(c);
   return launch_tree_t<C, D, PARTS, 1>(c);

@@ -148,6 +148,19 @@ def test_types_and_head_sizes(dt, ct, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,ct", PAIRS, ids=PAIR_IDS)
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+def test_small_trees(dt, ct, D):
+    """Up to 16 nodes and one more, over short and split windows."""
+    for M, kind, lengths in ((2, "chain", [31, 1]), (9, "roots", [64, 130]), (15, "tree", [0, 250]), (16, "tree", [40, 97]),
+                             (17, "tree", [40, 97])):
+        check_case = Case(2, M, 2, D, dt, ct, lengths, kind, w=(40.0, 200.0), seed=7 * D + M)
+        check(check_case, check_case.run())
+    case = Case(1, 12, 3, D, dt, ct, [3000], "tree", w=(500.0, 4000.0), r=1.3, seed=D)
+    check(case, case.run())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["chain", "star", "roots", "tree"])
 @pytest.mark.parametrize("M", [1, 2, 5, 31, 32, 33, 63, 64])
 def test_trees(M, kind):
