@@ -488,6 +488,10 @@ static int cache_call(const msa_cache_args* a, int read, void* stream, const cha
   if (a->start != nullptr && a->start_n != 1 && a->start_n != a->B)
     return fail(MSA_ERR_INVALID, "start holds %lld positions, 1 or B=%d needed", (long long)a->start_n, c.B);
   if (c.B == 0 || c.T == 0 || c.Tx == 0) return ok();
+  const msa_tensor* out[4] = {read ? &a->k : &a->kcache, read ? &a->v : &a->vcache, &a->kscale, &a->vscale};
+  for (int z = 0; z < (read || c.cache_dtype == c.dtype ? 2 : 4); ++z)
+    if ((c.B > 1 && out[z]->sb == 0) || (c.T > 1 && out[z]->st == 0) || (c.H > 1 && out[z]->sh == 0))
+      return fail(MSA_ERR_INVALID, "rows that are written must not share memory (a stride is 0)");
   if ((rc = check_tensor("k", a->k.p, a->k.sb, a->k.st, a->k.sh, c.dtype)) != MSA_OK) return rc;
   if ((rc = check_tensor("v", a->v.p, a->v.sb, a->v.st, a->v.sh, c.dtype)) != MSA_OK) return rc;
   c.x[0] = a->k.p; c.x[1] = a->v.p; c.xs[0] = strides_of(a->k); c.xs[1] = strides_of(a->v);

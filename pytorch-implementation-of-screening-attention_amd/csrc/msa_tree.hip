@@ -38,13 +38,8 @@ constexpr int kTreeMinUnits = 8, kTreeSmall = 16;
 constexpr int tree_occupancy(int row_bytes, int parts) {
   return row_bytes * parts <= 64 ? 3 : row_bytes <= 256 ? 2 : 1;
 }
-#ifndef O16A
-#define O16A 4
-#define O16B 3
-#define O16C 2
-#endif
 constexpr int tree_occupancy16(int row_bytes, int parts) {  // the same of tree16_kernel
-  return row_bytes * parts <= 64 ? O16A : row_bytes * parts <= 128 ? O16B : O16C;
+  return row_bytes * parts <= 128 ? 3 : 2;
 }
 
 // How a cache row of type C enters the products.

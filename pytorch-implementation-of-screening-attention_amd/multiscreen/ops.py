@@ -342,8 +342,9 @@ def cache_write(k, v, kcache, vcache, start, kscale=None, vscale=None, rows=None
     kept as the codes nearest to TOP x / max|x| (TOP = 127 or 448, ties to the
     even code) and the scale max|x| / TOP.  Rows of zeros have scale 0; rows with
     an infinity or a NaN read back as NaN.
-    start: an int (then all rows must fit), or an int64 CUDA tensor of 1 or B
-    elements (rows that would lie outside the cache are not written).
+    start: an int (then all rows must fit, unless `count` is given), or an int64
+    CUDA tensor of 1 or B elements; rows that would lie outside the cache are
+    not written.
     rows (B, T') int64, count (B) int64: row rows[b, t] of k and v goes to
     position start + t, for t < count[b] only: the accepted path of
     verify_drafts.  Rows outside k are not written.

@@ -239,6 +239,13 @@ def test_refusals():
     odd = torch.zeros(2, 8, 2, 72, dtype=torch.int8, device=DEV)[..., :64]
     with pytest.raises(ValueError):
         ops.cache_write(x, x, odd, odd, 0, ks, vs)
+    shared = kc[:1].expand(2, 8, 2, 64)
+    with pytest.raises(_native_error()):  # two sequences would write one row
+        ops.cache_write(x, x, shared, shared, 0, ks, vs)
+    with pytest.raises(_native_error()):
+        ops.cache_write(x, x, kc, vc, 0, ks[:1].expand(2, 8, 2), vs)
+    # reading such a cache is fine
+    assert ops.cache_read(shared, shared, ks, vs, 0, 8, torch.bfloat16)[0].shape == (2, 8, 2, 64)
     with pytest.raises(_native_error()):
         y = torch.zeros(2, 3, 2, 48, dtype=torch.bfloat16, device=DEV)
         c = torch.zeros(2, 8, 2, 48, dtype=torch.int8, device=DEV)
@@ -276,7 +283,7 @@ def test_c_entries_refuse_bad_arguments():
     for kw, msg in ((dict(D=48), "head_dim"), (dict(dt=3), "dtype"), (dict(ct=2), "cache_dtype"), (dict(ct=5), "cache_dtype"),
                     (dict(sc=0), "scales"), (dict(c=0), "null"), (dict(c=8), "aligned"), (dict(cs=(1024, 8, 512)), "multiples"),
                     (dict(k=0), "null"), (dict(ks=(512, 4, 64)), "strides"), (dict(T=4), "rows"), (dict(start=16, n=3), "start"),
-                    (dict(ss=(16, -1, 8)), "strides"), (dict(B=70000, H=1), "B*H"), (dict(B=-1), "size"), (dict(T=2 ** 40), "size"), (dict(cs=(1024, 2 ** 26, 512)), "span")):
+                    (dict(ss=(16, -1, 8)), "strides"), (dict(cs=(0, 64, 512)), "share memory"), (dict(ss=(16, 0, 8)), "share memory"), (dict(B=70000, H=1), "B*H"), (dict(B=-1), "size"), (dict(T=2 ** 40), "size"), (dict(cs=(1024, 2 ** 26, 512)), "span")):
         assert write(**kw) == 1, kw
         assert msg in L.msa_last_error().decode(), (kw, L.msa_last_error())
     assert write(B=0) == 0 and write(T=0) == 0
