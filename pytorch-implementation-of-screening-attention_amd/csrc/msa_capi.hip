@@ -511,6 +511,8 @@ int msa_cache_read(const msa_cache_args* args, void* stream) {
   return cache_call(args, 1, stream, "msa_cache_read launch");
 }
 
+static size_t tree_table_bytes(int B, int H) { return (size_t)msa::round_up((int64_t)B * H * sizeof(int2), 256); }
+
 static int tree_blocks_of(int B, int H, int N, int D, int dtype, int cache_dtype, int cache_cap, int window_hint) {
   return msa::tree_blocks(B, H, N, D, dtype, cache_dtype,
                           window_hint > 0 && window_hint < cache_cap ? window_hint : cache_cap);
@@ -522,7 +524,7 @@ size_t msa_tree_workspace_bytes(int B, int H, int N, int D, int dtype, int cache
       !(D == 16 || D == 32 || D == 64 || D == 128))
     return 0;
   const int blocks = tree_blocks_of(B, H, N, D, dtype, cache_dtype, cache_cap, window_hint);
-  return blocks == H ? 0 : (size_t)B * blocks * N * D * sizeof(float);
+  return blocks == H ? 0 : tree_table_bytes(B, H) + (size_t)B * blocks * N * D * sizeof(float);
 }
 
 int msa_tree_decode(const msa_tree_args* a, void* stream) {
@@ -554,7 +556,8 @@ int msa_tree_decode(const msa_tree_args* a, void* stream) {
   c.kscale = (const float*)a->kscale.p; c.kss = strides_of(a->kscale);
   c.vscale = (const float*)a->vscale.p; c.vss = strides_of(a->vscale);
   c.lengths = a->lengths; c.len_step = a->lengths_n == 1 ? 0 : 1; c.parents = a->parents; c.par_sb = a->par_sb;
-  c.r = a->r; c.w = a->w; c.part = (float*)a->workspace; c.y = a->y;
+  c.r = a->r; c.w = a->w; c.y = a->y;
+  c.table = (int2*)a->workspace; c.part = need > 0 ? (float*)((char*)a->workspace + tree_table_bytes(c.B, c.H)) : nullptr;
   c.blocks = tree_blocks_of(c.B, c.H, c.N, c.D, c.q_dtype, c.cache_dtype, c.cap, hint);
   c.stream = (hipStream_t)stream;
   return hip_status(msa::launch_tree(c), "msa_tree_decode launch");

@@ -132,6 +132,7 @@ struct TreeCall {
   const int64_t* lengths; int len_step;       // committed positions, one (step 0) or per sequence
   const int64_t* parents; int64_t par_sb;     // parents of a sequence's nodes, or null: a chain
   const float* r; const float* w; float eps;
+  int2* table;  // [b][h] first piece and number of pieces of the head, where blocks != H
   float* part;  // [b][block][node][D] sums, where blocks != H
   void* y;
   int blocks;   // blocks that share a sequence's keys; H: a block per head

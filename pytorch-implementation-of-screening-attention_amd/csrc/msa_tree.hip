@@ -434,7 +434,7 @@ struct TreeSpan {
 
 // How the blocks of a sequence share its heads' units: head h's are cut into
 // pieces of `per`, the heads' pieces numbered one after the other, a block
-// each; `per` is the least (in steps of an eighth) for which the blocks
+// each; `per` is the least (in steps of about an eighth) for which the blocks
 // suffice.  Windows differ by orders of magnitude between heads, and blocks per
 // head would leave most of the card to the widest.  Wave-uniform.
 struct TreeMap {
@@ -453,7 +453,7 @@ struct TreeMap {
     for (int h = 64; h < a.H; h += 64) all += sum(units_of(a, sp, h + lane));
     per = (all + a.blocks - 1) / a.blocks;
     per = per < kTreeMinUnits ? kTreeMinUnits : per;
-    for (;; per += per / 8) {  // ends: one piece a head fits
+    for (;; per += per / 8 + 1) {  // ends: one piece a head fits
       int pieces = sum((first + per - 1) / per);
       for (int h = 64; h < a.H; h += 64) pieces += sum((units_of(a, sp, h + lane) + per - 1) / per);
       if (pieces <= a.blocks) return;
@@ -481,12 +481,22 @@ struct TreeMap {
     }
     return -1;
   }
-  // First piece of head h and how many it has.
-  __device__ int pieces_of(const TreeCall& a, const TreeSpan& sp, int lane, int h, int& piece0) const {
-    int before = 0;
-    for (int g = 0; g <= h; g += 64) before += sum(g + lane < h ? (units_of(a, sp, g + lane) + per - 1) / per : 0);
-    piece0 = before;
-    return (units_of(a, sp, h) + per - 1) / per;
+  // Every head's first piece and how many it has, for the sums' reduction (one
+  // wave of a sequence's first block).
+  __device__ void write(const TreeCall& a, const TreeSpan& sp, int lane, int2* table) const {
+    int carry = 0;
+    for (int h = 0; h < a.H; h += 64) {
+      const int c = (units_of(a, sp, h + lane) + per - 1) / per;
+      int incl = c;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(incl, o);
+        if (lane >= o) incl += y;
+      }
+      incl += carry;
+      if (h + lane < a.H) table[h + lane] = make_int2(incl - c, c);
+      carry = __shfl(incl, 63);
+    }
   }
 };
 
@@ -521,6 +531,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C),
   if (a.blocks != a.H) {
     const TreeMap map(a, sp, lane);
     int piece0 = 0;
+    if (blockIdx.x == 0 && wave == 0) map.write(a, sp, lane, a.table + (int64_t)b * a.H);
     h = map.head_of(a, sp, lane, blockIdx.x, piece0);
     if (h < 0) return;
     per = map.per;
@@ -919,6 +930,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy16(D * (int)sizeof(C
   if (a.blocks != a.H) {
     const TreeMap map(a, sp, lane);
     int piece0 = 0;
+    if (blockIdx.x == 0 && wave == 0) map.write(a, sp, lane, a.table + (int64_t)b * a.H);
     h = map.head_of(a, sp, lane, blockIdx.x, piece0);
     if (h < 0) return;
     per = map.per;
@@ -1150,11 +1162,9 @@ __global__ __launch_bounds__(256) void tree_reduce_kernel(TreeCall a) {
   const int lane = threadIdx.x & 63, node = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int b = blockIdx.y / a.H, h = blockIdx.y % a.H;
   if (node >= a.N) return;
-  const TreeSpan sp(a, b);
-  const TreeMap map(a, sp, lane);
-  int piece0;
-  const int used = map.pieces_of(a, sp, lane, h, piece0);
-  const float* p = a.part + (((int64_t)b * a.blocks + piece0) * a.N + node) * D + 4 * (lane % L);
+  const int2 at_pieces = a.table[blockIdx.y];  // first piece of the head, and how many
+  const int used = at_pieces.y;
+  const float* p = a.part + (((int64_t)b * a.blocks + at_pieces.x) * a.N + node) * D + 4 * (lane % L);
   f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
   for (int c = lane / L; c < used; c += G) x += *reinterpret_cast<const f32x4*>(p + (int64_t)c * a.N * D);
