@@ -22,6 +22,13 @@
 // fp32 row as the sum of two fp16 rows, 22 bits).  Pair weights are rounded to
 // two terms of the operand's type (16 or 22 bits), in fp16 after a power of two
 // that keeps small weights clear of its subnormals.
+//
+// What bounds it: long windows of few nodes the cache's bytes (one token of 16
+// sequences over 100K int8 positions: 143 us, 6.1 TB/s); many nodes or live units
+// the vector instructions of a unit (about 570 for 64 nodes of bf16, 375 for the
+// 16-column form: 56 and 41 us at 3 to 4 waves a SIMD, 65% of the issue slots);
+// short windows the latency of the call (12 us at 9 units a head, of which the
+// launch and the tree take 4 and a unit's way through a wave 2 to 3).
 #include "msa_device.h"
 #include "msa_internal.h"
 
@@ -30,9 +37,16 @@ namespace msa {
 constexpr int kTreeMax = 64;   // nodes of a tree: one lane each
 constexpr int kTreeWaves = 4;  // waves of a block
 // Fewest units of a block, so that a block's sums stay small beside its keys.
-// Fewest units of a block, so that a block's sums stay small beside its keys;
-// a head of at most kTreeSmall units is one block's (no sums to join).
-constexpr int kTreeMinUnits = 8, kTreeSmall = 16;
+// Fewest units of a block, so that a block's sums stay small beside its keys (16
+// instead of 8: 21 nodes over 5001 e4m3 rows of D = 128 24 -> 30 us, 40 over 6000
+// fp32 of D = 32 27 -> 39; 4: no gain).
+constexpr int kTreeMinUnits = 8;
+// Heads of at most kTreeSmall units are a block each, with no sums to join: at 9
+// units one block 12.8 us, two 18.5; at 22 units 14.0 and 14.5; at 41 units 22.0
+// and 17.4.  A batch that fills the card twice with heads of at most kTreeLong
+// units likewise (256 x 8 heads of 38 units bf16: 130 us, shared 159; of windows
+// 2 .. 1500 int8 84, shared 82).
+constexpr int kTreeSmall = 24, kTreeLong = 64;
 
 // Waves per SIMD that the kernel's registers are budgeted for.
 constexpr int tree_occupancy(int row_bytes, int parts) {
@@ -1183,9 +1197,14 @@ __global__ __launch_bounds__(256) void tree_reduce_kernel(TreeCall a) {
 
 int tree_max_nodes() { return kTreeMax; }
 // Whether a wave takes all of more than 32 nodes: its registers hold two tiles'
-// operands and sums for rows of at most 64 values in 2-byte operands.
+// operands and sums for rows of at most 64 values in 2-byte operands.  A wave a
+// tile converts, votes on and stages every unit twice: 4 x 64 nodes over 30K bf16
+// 88 us, together 75; before training 48, together 42.
 bool tree_both(int N, int D, bool f32) { return N > 32 && D <= 64 && !f32; }
-// Whether a tree takes the 16-column form.
+// Whether a tree takes the 16-column form: 8 nodes over 16K int8 49 -> 46 us, fp32
+// queries 53 -> 45 (D = 128: 85 -> 71), one node at windows 2 .. 256 10.1 -> 8.6,
+// 16 nodes over 8K bf16 of D = 128 61 -> 59; one node over 100K int8, which its
+// bytes bound, 157 and 160.
 bool tree_few(int N, bool f32_operands) { return N <= 16 && !f32_operands; }
 // Blocks of a sequence: as many as run at one time on the card's 256 CUs share
 // its heads' keys; one a head (H) where heads are short, or the batch alone
@@ -1198,7 +1217,7 @@ int tree_blocks(int B, int H, int N, int D, int q_dtype, int cache_dtype, int sp
   const int parts = codes && q_dtype == 0 ? 2 : 1;
   const int slots = 256 * (tree_few(N, !codes && f32) ? tree_occupancy16(row, parts)
                                                       : tree_occupancy(row, tree_both(N, D, f32) ? 2 : parts));
-  if (units <= kTreeSmall || ((int64_t)B * H >= 2 * slots && units <= 4 * kTreeSmall)) return H;
+  if (units <= kTreeSmall || ((int64_t)B * H >= 2 * slots && units <= kTreeLong)) return H;
   const int each = slots / B;
   return each < 2 * H ? 2 * H : each;
 }
