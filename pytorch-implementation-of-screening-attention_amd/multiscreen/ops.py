@@ -250,7 +250,6 @@ def decode_step_at(q, kcache, vcache, last_pos, r, w, eps=1e-8, workspace=None, 
 # ---------------------------------------------------------------------------
 _CACHE_DTYPES = {**_DTYPES, torch.int8: _native.MSA_I8, torch.float8_e4m3fn: _native.MSA_FP8}
 CODE_DTYPES = (torch.int8, torch.float8_e4m3fn)
-_NO_SCALES = (0, 0, 0, 0)
 
 
 def _launch(what, fn, index, args):
@@ -264,15 +263,13 @@ def _launch(what, fn, index, args):
         _native.check(rc, what)
 
 
-def _one_gpu(what, first, **others):
-    """The index of the GPU that every tensor given is on."""
-    index = first.get_device()
+def _one_gpu(what, index, *tensors):
+    """Raises unless every tensor given is on GPU `index`."""
     if index < 0:
         raise RuntimeError(f"{what} runs on the GPU only (got a CPU tensor)")
-    for name, x in others.items():
+    for x in tensors:
         if x is not None and x.get_device() != index:
-            raise RuntimeError(f"{what} runs on one GPU: {name} is on {x.device}, not on {first.device}")
-    return index
+            raise RuntimeError(f"{what} runs on one GPU: got a tensor on {x.device} beside cuda:{index}")
 
 
 def _index(x, name, *shapes):
@@ -301,34 +298,36 @@ def _rows_bthd(x, name):
 
 
 def _cache_args(what, kcache, vcache, kscale, vscale, dtype):
-    """The C arguments of a cache pair (B, cap, H, D) and of its scales (B, cap, H), checked against the
-    rows' type."""
-    if kcache.dim() != 4 or kcache.shape != vcache.shape or kcache.dtype != vcache.dtype:
+    """The type and the C arguments of a cache pair (B, cap, H, D) and its scales (B, cap, H), checked against
+    the rows' type."""
+    shape = kcache.shape
+    if len(shape) != 4 or vcache.shape != shape or vcache.dtype != kcache.dtype:
         raise ValueError(f"{what}: the caches must be (B, cap, H, D) of one shape and type, got {kcache.dtype} "
                          f"{tuple(kcache.shape)}, {vcache.dtype} {tuple(vcache.shape)}")
+    ct = _CACHE_DTYPES.get(kcache.dtype, -1)
+    codes = ct >= _native.MSA_I8
+    if not codes and kcache.dtype != dtype:
+        raise TypeError(f"{what}: a cache of {kcache.dtype} does not hold rows of {dtype}")
     kb, kt, kh, kd = kcache.stride()
     vb, vt, vh, vd = vcache.stride()
     kp, vp = kcache.data_ptr(), vcache.data_ptr()
-    if kd != 1 or vd != 1 or ((kb | kt | kh | vb | vt | vh) * kcache.element_size() | kp | vp) & 15:
+    if kd != 1 or vd != 1 or ((kb | kt | kh | vb | vt | vh) * (1 if codes else kcache.element_size()) | kp | vp) & 15:
         raise ValueError(f"{what}: the caches need unit stride over D and 16-byte aligned rows, got strides "
                          f"{kcache.stride()}, {vcache.stride()}")
-    pair = (kp, kb, kt, kh, vp, vb, vt, vh)
-    if kcache.dtype not in CODE_DTYPES:
-        if kcache.dtype != dtype:
-            raise TypeError(f"{what}: a cache of {kcache.dtype} does not hold rows of {dtype}")
+    if not codes:
         if kscale is not None or vscale is not None:
             raise ValueError(f"{what}: a cache of {kcache.dtype} takes no scales")
-        return pair, _NO_SCALES + _NO_SCALES
-    B, cap, H, _ = kcache.shape
-    if kscale is None or vscale is None or kscale.dtype != torch.float32 or vscale.dtype != torch.float32 \
-            or kscale.shape != (B, cap, H) or vscale.shape != (B, cap, H):
-        raise ValueError(f"{what}: a cache of {kcache.dtype} needs kscale and vscale, float32 ({B}, {cap}, {H})")
-    return pair, (kscale.data_ptr(), *kscale.stride(), vscale.data_ptr(), *vscale.stride())
+        return ct, (kp, kb, kt, kh, vp, vb, vt, vh, 0, 0, 0, 0, 0, 0, 0, 0)
+    rows = shape[:3]
+    if kscale is None or vscale is None or kscale.shape != rows or vscale.shape != rows \
+            or kscale.dtype != torch.float32 or vscale.dtype != torch.float32:
+        raise ValueError(f"{what}: a cache of {kcache.dtype} needs kscale and vscale, float32 {tuple(rows)}")
+    return ct, (kp, kb, kt, kh, vp, vb, vt, vh, kscale.data_ptr(), *kscale.stride(), vscale.data_ptr(), *vscale.stride())
 
 
 def _start_args(start, B):
     """(pointer or 0, count, host value, tensor to keep) of an int or int64 device tensor."""
-    if not torch.is_tensor(start):
+    if not isinstance(start, torch.Tensor):
         return 0, 0, int(start), None
     start = _index(start, "start", (1,), (B,))
     return start.data_ptr(), start.shape[0], 0, start
@@ -350,8 +349,9 @@ def cache_write(k, v, kcache, vcache, start, kscale=None, vscale=None, rows=None
     verify_drafts.  Rows outside k are not written.
     The rest of the cache is left as it was.  No gradient flows through it.
     """
-    index = _one_gpu("cache_write", k, v=v, kcache=kcache, vcache=vcache, kscale=kscale, vscale=vscale, rows=rows,
-                     count=count, start=start if torch.is_tensor(start) else None)
+    index = k.get_device()
+    _one_gpu("cache_write", index, v, kcache, vcache, kscale, vscale, rows, count,
+             start if isinstance(start, torch.Tensor) else None)
     dtype = k.dtype
     if dtype not in _DTYPES or v.dtype != dtype or k.shape != v.shape:
         raise TypeError(f"cache_write: k and v must share shape and dtype float32, bfloat16 or float16, got {k.dtype} "
@@ -359,7 +359,7 @@ def cache_write(k, v, kcache, vcache, start, kscale=None, vscale=None, rows=None
     k, kargs = _rows_bthd(k, "k")
     v, vargs = _rows_bthd(v, "v")
     B, Tx, H, D = k.shape
-    pair, scales = _cache_args("cache_write", kcache, vcache, kscale, vscale, dtype)
+    ct, cache = _cache_args("cache_write", kcache, vcache, kscale, vscale, dtype)
     Bc, cap, Hc, Dc = kcache.shape
     if Bc != B or Hc != H or Dc != D:
         raise ValueError(f"cache_write: cache {tuple(kcache.shape)} does not match rows {tuple(k.shape)}")
@@ -375,8 +375,7 @@ def cache_write(k, v, kcache, vcache, start, kscale=None, vscale=None, rows=None
     if not sp and (host < 0 or host + (T if count is None else 0) > cap):
         raise IndexError(f"KV cache capacity {cap} exceeded at position {host + T}")
     _launch("msa_cache_write", _native.lib().msa_cache_write, index,
-            _native.pack_cache_args(*kargs, *vargs, *pair, *scales, rp, cp, sp, n, host, B, T, Tx, H, D, _DTYPES[dtype],
-                                    cap, _CACHE_DTYPES[kcache.dtype]))
+            _native.pack_cache_args(*kargs, *vargs, *cache, rp, cp, sp, n, host, B, T, Tx, H, D, _DTYPES[dtype], cap, ct))
 
 
 def cache_read(kcache, vcache, kscale, vscale, start, length, dtype):
@@ -384,11 +383,11 @@ def cache_read(kcache, vcache, kscale, vscale, start, length, dtype):
     cache_write takes it) in `dtype`: code * scale, rounded once; (k, v), each
     contiguous (B, length, H, D).  With a device `start`, positions outside the
     cache read as zeros."""
-    index = _one_gpu("cache_read", kcache, vcache=vcache, kscale=kscale, vscale=vscale,
-                     start=start if torch.is_tensor(start) else None)
+    index = kcache.get_device()
+    _one_gpu("cache_read", index, vcache, kscale, vscale, start if isinstance(start, torch.Tensor) else None)
     if dtype not in _DTYPES:
         raise TypeError(f"cache_read: dtype must be float32, bfloat16 or float16, got {dtype}")
-    pair, scales = _cache_args("cache_read", kcache, vcache, kscale, vscale, dtype)
+    ct, cache = _cache_args("cache_read", kcache, vcache, kscale, vscale, dtype)
     B, cap, H, D = kcache.shape
     length = int(length)
     sp, n, host, start = _start_args(start, B)
@@ -396,10 +395,11 @@ def cache_read(kcache, vcache, kscale, vscale, start, length, dtype):
         raise IndexError(f"positions {host} .. {host + length} are outside the KV cache's capacity {cap}")
     k = torch.empty((B, length, H, D), dtype=dtype, device=kcache.device)
     v = torch.empty_like(k)
+    st = H * D
+    sb = length * st
     _launch("msa_cache_read", _native.lib().msa_cache_read, index,
-            _native.pack_cache_args(k.data_ptr(), length * H * D, H * D, D, v.data_ptr(), length * H * D, H * D, D, *pair,
-                                    *scales, 0, 0, sp, n, host, B, length, length, H, D, _DTYPES[dtype], cap,
-                                    _CACHE_DTYPES[kcache.dtype]))
+            _native.pack_cache_args(k.data_ptr(), sb, st, D, v.data_ptr(), sb, st, D, *cache, 0, 0, sp, n, host, B, length,
+                                    length, H, D, _DTYPES[dtype], cap, ct))
     return k, v
 
 
@@ -428,8 +428,8 @@ def tree_decode(q, kcache, vcache, lengths, parents, r, w, eps=1e-8, kscale=None
     window_hint: 0, or a bound on ceil(w) over the heads (sizes the launch).
     Returns y (B, N, H, D) = TanhNorm(h), in q's dtype; no gradient.
     """
-    index = _one_gpu("tree_decode", q, kcache=kcache, vcache=vcache, kscale=kscale, vscale=vscale, lengths=lengths,
-                     parents=parents, r=r, w=w, workspace=workspace)
+    index = q.get_device()
+    _one_gpu("tree_decode", index, kcache, vcache, kscale, vscale, lengths, parents, r, w, workspace)
     dtype = q.dtype
     if dtype not in _DTYPES:
         raise TypeError(f"tree_decode: q must be float32, bfloat16 or float16, got {q.dtype}")
@@ -437,7 +437,7 @@ def tree_decode(q, kcache, vcache, lengths, parents, r, w, eps=1e-8, kscale=None
     B, N, H, D = q.shape
     if N > _native.TREE_MAX:
         raise ValueError(f"tree_decode: a tree holds at most {_native.TREE_MAX} nodes, got {N}")
-    pair, scales = _cache_args("tree_decode", kcache, vcache, kscale, vscale, dtype)
+    ct, cache = _cache_args("tree_decode", kcache, vcache, kscale, vscale, dtype)
     Bc, cap, Hc, Dc = kcache.shape
     if Bc != B or Hc != H or Dc != D:
         raise ValueError(f"tree_decode: cache {tuple(kcache.shape)} does not match q {tuple(q.shape)}")
@@ -450,13 +450,13 @@ def tree_decode(q, kcache, vcache, lengths, parents, r, w, eps=1e-8, kscale=None
     r, w = _float32(r), _float32(w)
     hint = max(0, int(window_hint))
     L = _native.lib()
-    y = torch.empty((B, N, H, D), dtype=dtype, device=q.device)
-    qt, ct = _DTYPES[dtype], _CACHE_DTYPES[kcache.dtype]
+    y = torch.empty((B, N, H, D), dtype=dtype, device=q.device) if not q.is_contiguous() else torch.empty_like(q)
+    qt = _DTYPES[dtype]
     need = L.msa_tree_workspace_bytes(B, H, N, D, qt, ct, cap, hint)
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
         workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
     _launch("msa_tree_decode", L.msa_tree_decode, index,
-            _native.pack_tree_args(*qargs, *pair, *scales, lengths.data_ptr(), par, r.data_ptr(), w.data_ptr(), y.data_ptr(),
+            _native.pack_tree_args(*qargs, *cache, lengths.data_ptr(), par, r.data_ptr(), w.data_ptr(), y.data_ptr(),
                                    workspace.data_ptr() if need else 0, need, lengths.shape[0], par_sb, B, N, H, D, qt,
                                    cap, ct, hint, float(eps)))
     return y
@@ -486,7 +486,8 @@ def verify_drafts(target, tokens, parents=None, uniforms=None, draft=None):
     count (B), how many; token (B), the next token.  The count[b] rows path[b]
     are what cache_write takes as `rows` and `count`.
     """
-    index = _one_gpu("verify_drafts", target, tokens=tokens, parents=parents, uniforms=uniforms, draft=draft)
+    index = target.get_device()
+    _one_gpu("verify_drafts", index, tokens, parents, uniforms, draft)
     dtype = target.dtype
     if target.dim() != 3 or dtype not in _DTYPES:
         raise TypeError(f"verify_drafts: target must be (B, M, V) float32, bfloat16 or float16, got {target.dtype} "
@@ -514,7 +515,7 @@ def verify_drafts(target, tokens, parents=None, uniforms=None, draft=None):
     target = target if target.stride(2) == 1 else target.contiguous()
     t_sb, t_sn, _ = target.stride()
     L = _native.lib()
-    path = torch.empty((B, M), dtype=torch.int64, device=target.device)
+    path = torch.empty_like(tokens)
     count = torch.empty((B,), dtype=torch.int64, device=target.device)
     token = torch.empty_like(count)
     need, workspace = 0, None
