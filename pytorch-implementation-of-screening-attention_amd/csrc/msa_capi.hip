@@ -531,7 +531,7 @@ int msa_tree_decode(const msa_tree_args* a, void* stream) {
   if (a == nullptr) return fail(MSA_ERR_INVALID, "args is null");
   msa::TreeCall c;
   c.B = size_of(a->B); c.N = size_of(a->N); c.H = size_of(a->H); c.D = size_of(a->D); c.cap = size_of(a->cache_cap);
-  c.q_dtype = size_of(a->dtype); c.cache_dtype = size_of(a->cache_dtype); c.eps = (float)a->eps;
+  c.q_dtype = size_of(a->dtype); c.cache_dtype = size_of(a->cache_dtype); c.eps = (float)a->eps; c.inv_eps = fminf(1.0f / c.eps, 3.4e38f);
   int rc = check_cache(c.B, c.N, c.H, c.D, c.q_dtype, c.cap, c.cache_dtype, a->kcache, a->vcache, a->kscale, a->vscale);
   if (rc != MSA_OK) return rc;
   if (c.N > MSA_TREE_MAX) return fail(MSA_ERR_INVALID, "a tree holds at most %d nodes, got %d", MSA_TREE_MAX, c.N);

@@ -131,7 +131,7 @@ struct TreeCall {
   const float* vscale; Strides3 vss;
   const int64_t* lengths; int len_step;       // committed positions, one (step 0) or per sequence
   const int64_t* parents; int64_t par_sb;     // parents of a sequence's nodes, or null: a chain
-  const float* r; const float* w; float eps;
+  const float* r; const float* w; float eps, inv_eps;
   int2* table;  // [b][h] first piece and number of pieces of the head, where blocks != H
   float* part;  // [b][block][node][D] sums, where blocks != H
   void* y;

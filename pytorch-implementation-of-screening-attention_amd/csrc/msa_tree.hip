@@ -100,6 +100,15 @@ __device__ inline f16x8 decode8(uint32_t c0, uint32_t c1) {
   return f;
 }
 
+// Sum of squares of the int8 codes in N words.
+template <int N>
+__device__ inline int code_dot(const u32x4& c) {
+  int s = 0;
+#pragma unroll
+  for (int e = 0; e < N; ++e) s = __builtin_amdgcn_sdot4((int)c[e], (int)c[e], s, false);
+  return s;
+}
+
 // Waits that keep a run's A/B fragments and its result's registers apart from
 // later writes (guard_run, for any number of fragments).
 template <typename F, int N>
@@ -162,24 +171,22 @@ struct KeyRows {
   }
   // 1/max(|k|, eps) of the row, times the code's scale.  A row that is not
   // finite gives 0 or NaN: its pairs are not live.
-  __device__ inline float factor(const frag (&f)[NKS], float eps) const {
+  __device__ inline float factor(const frag (&f)[NKS], float eps, float inv_eps) const {
     if constexpr (__is_same(C, int8_t)) {
       int ss = 0;
 #pragma unroll
-      for (int i = 0; i < NL; ++i)
-#pragma unroll
-        for (int e = 0; e < LB / 4; ++e) ss = __builtin_amdgcn_sdot4((int)raw[i][e], (int)raw[i][e], ss, false);
-      return code_factor(half_sum((float)ss), scale, eps);
+      for (int i = 0; i < NL; ++i) ss += code_dot<LB / 4>(raw[i]);
+      return code_factor(half_sum((float)ss), scale, inv_eps);
     } else if constexpr (kCodes) {
-      return code_factor(half_sum(row_dot<comp>(f, f)), scale, eps);
+      return code_factor(half_sum(row_dot<comp>(f, f)), scale, inv_eps);
     } else {
       return inv_len_of<C>(half_sum(row_dot<comp>(f, f)), eps);
     }
   }
   // min(1/|c|, scale/eps): the factor that takes a row of codes c with this
   // scale to its unit row (0 for a row of zeros, NaN for one that is not finite).
-  __device__ static inline float code_factor(float ss, float scale, float eps) {
-    const float f = fminf(inv_len_of<float>(ss, 1e-30f), scale / eps);
+  __device__ static inline float code_factor(float ss, float scale, float inv_eps) {
+    const float f = fminf(inv_len_of<float>(ss, 1e-30f), scale * inv_eps);
     return scale == scale ? f : scale;
   }
 };
@@ -262,7 +269,7 @@ struct ValueRows {
   // live pair still sees it and a masked one does not; then the result is true.
   // (A finite row whose length overflows has factor 0.)  The factors are times
   // kWeightUp.
-  __device__ inline bool stage(char* tile, float* fac, float eps, int lane) const {
+  __device__ inline bool stage(char* tile, float* fac, float eps, float inv_eps, int lane) const {
     typedef typename Mma<comp>::frag vec;  // 16 bytes of an operand row
     constexpr int N = 16 / (int)sizeof(comp);
     constexpr int W = kCodes ? 2 : 1;      // operand chunks of a load
@@ -283,6 +290,8 @@ struct ValueRows {
         x[0] = __builtin_bit_cast(vec, raw[i]);
       }
       float ss = 0.0f;
+      if constexpr (__is_same(C, int8_t)) ss = (float)code_dot<4>(raw[i]);
+      else
 #pragma unroll
       for (int u = 0; u < W; ++u) {
         if constexpr (sizeof(comp) == 2) ss = frag_dot(x[u], x[u], ss);
@@ -294,7 +303,7 @@ struct ValueRows {
       bool finite = ss < INFINITY;
       if constexpr (kCodes) finite = finite && scale[i] == scale[i];
       float f;
-      if constexpr (kCodes) f = KeyRows<C, D>::code_factor(ss, scale[i], eps);
+      if constexpr (kCodes) f = KeyRows<C, D>::code_factor(ss, scale[i], inv_eps);
       else f = inv_len_of<C>(ss, eps);
       if (__ballot(!finite) != 0ull) {
         float bad = 0.0f;  // an element (or its scale) that is not finite, and not only the squares' sum
@@ -616,7 +625,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C),
     if (u + wpt < u1) load_keys(key_next, u + wpt);
     frag kf[K::NKS];
     key.frags(kf);
-    const float f = key.factor(kf, a.eps);
+    const float f = key.factor(kf, a.eps, a.inv_eps);
     if (half == 0) kfac[wave][perm_row(l32)] = f;
     f32x16 s[T];
 #pragma unroll
@@ -682,7 +691,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C),
     }
     if (__ballot(any > 0.0f) == 0ull) continue;
 
-    const bool odd = val.stage(vt, vfac[wave], a.eps, lane);
+    const bool odd = val.stage(vt, vfac[wave], a.eps, a.inv_eps, lane);
     wave_lds_sync();
     read_row_scales(vfac[wave], half, x);
     frag hi[T][NC], lo[T][kTwo ? NC : 1];
@@ -870,9 +879,18 @@ struct KeyRows16 {
       if (kHalf && lane >= 32) f[ks] = Mma<comp>::zero();
     }
   }
-  __device__ inline float factor(int t, const frag (&f)[NKS], float eps) const {
-    const float ss = quarter_sum(row_dot<comp>(f, f));
-    if constexpr (kCodes) return KeyRows<C, D>::code_factor(ss, scale[t], eps);
+  __device__ inline float factor(int t, const frag (&f)[NKS], float eps, float inv_eps) const {
+    float ss = 0.0f;
+    if constexpr (__is_same(C, int8_t)) {
+      int si = 0;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) si += code_dot<LB / 4>(raw[t][i]);
+      ss = kHalf && (threadIdx.x & 32) != 0 ? 0.0f : (float)si;
+    } else {
+      ss = row_dot<comp>(f, f);
+    }
+    ss = quarter_sum(ss);
+    if constexpr (kCodes) return KeyRows<C, D>::code_factor(ss, scale[t], inv_eps);
     else return inv_len_of<C>(ss, eps);
   }
 };
@@ -1025,7 +1043,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy16(D * (int)sizeof(C
     for (int t = 0; t < 2; ++t) {
       frag kf[K::NKS];
       key.frags(t, lane, kf);
-      const float f = key.factor(t, kf, a.eps);
+      const float f = key.factor(t, kf, a.eps, a.inv_eps);
       if (g == 0) kfac[wave][K::row(t, lane)] = f;
       f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -1083,7 +1101,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy16(D * (int)sizeof(C
     }
     if (__ballot(any > 0.0f) == 0ull) continue;
 
-    const bool odd = val.stage(vt, vfac[wave], a.eps, lane);
+    const bool odd = val.stage(vt, vfac[wave], a.eps, a.inv_eps, lane);
     wave_lds_sync();
     read8(vfac[wave]);
     if (odd) {  // a NaN factor reaches live pairs only
