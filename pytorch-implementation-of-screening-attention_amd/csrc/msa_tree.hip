@@ -24,11 +24,11 @@
 // that keeps small weights clear of its subnormals.
 //
 // What bounds it: long windows of few nodes the cache's bytes (one token of 16
-// sequences over 100K int8 positions: 143 us, 6.1 TB/s); many nodes or live units
-// the vector instructions of a unit (about 570 for 64 nodes of bf16, 375 for the
-// 16-column form: 56 and 41 us at 3 to 4 waves a SIMD, 65% of the issue slots);
-// short windows the latency of the call (12 us at 9 units a head, of which the
-// launch and the tree take 4 and a unit's way through a wave 2 to 3).
+// sequences over 100K int8 positions: 140 us, 6.2 TB/s); many nodes or live units
+// the vector instructions of a unit (about 570 for 64 nodes of bf16, 350 for the
+// 16-column form: 56 and 37 us, half to two thirds of the issue slots); short
+// windows the latency of the call (12 us at 9 units a head, of which the launch
+// and the tree take 4 and a unit's way through a wave 2 to 3).
 #include "msa_device.h"
 #include "msa_internal.h"
 
@@ -1222,7 +1222,8 @@ bool tree_both(int N, int D, bool f32) { return N > 32 && D <= 64 && !f32; }
 // Whether a tree takes the 16-column form: 8 nodes over 16K int8 49 -> 46 us, fp32
 // queries 53 -> 45 (D = 128: 85 -> 71), one node at windows 2 .. 256 10.1 -> 8.6,
 // 16 nodes over 8K bf16 of D = 128 61 -> 59; one node over 100K int8, which its
-// bytes bound, 157 and 160.
+// bytes bound, the same.  (The transposed reads of natural column blocks, 16 d +
+// 0 .. 15, spread over twice the banks and were no faster.)
 bool tree_few(int N, bool f32_operands) { return N <= 16 && !f32_operands; }
 // Blocks of a sequence: as many as run at one time on the card's 256 CUs share
 // its heads' keys; one a head (H) where heads are short, or the batch alone

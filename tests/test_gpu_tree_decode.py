@@ -407,6 +407,35 @@ def test_other_stream_and_graph_replays():
 
 
 @pytest.mark.gpu
+def test_calls_at_the_same_time():
+    """Split calls on two streams, each with its own scratch, interleaved with writes to other caches."""
+    ops = _ops()
+    cases = [Case(2, 20, 4, 64, torch.bfloat16, torch.int8, [4000, 3500], "tree", w=(100.0, 4000.0), seed=20),
+             Case(1, 5, 6, 64, torch.bfloat16, torch.bfloat16, [6000], "chain", w=(50.0, 6000.0), seed=21)]
+    args = [[x if x is None else x.to(DEV) for x in (c.q, c.kc, c.vc, c.ks, c.vs, c.r, c.w, torch.tensor(c.lengths), c.parents)]
+            for c in cases]
+
+    def call(d):
+        return ops.tree_decode(d[0], d[1], d[2], d[7], d[8], d[5], d[6], EPS, d[3], d[4])
+
+    base = [call(d) for d in args]
+    for c, y in zip(cases, base):
+        check(c, y)
+    streams = [torch.cuda.Stream() for _ in args]
+    spare = empty_cache(1, 64, 6, 64, torch.int8)
+    x = torch.randn(1, 64, 6, 64, device=DEV, dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (d, st) in enumerate(zip(args, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(call(d))
+        ops.cache_write(x, x, spare[0], spare[1], 0, spare[2], spare[3])
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, b) for ys, b in zip(got, base) for y in ys)
+
+
+@pytest.mark.gpu
 def test_empty_batch_and_refusals():
     ops = _ops()
     case = Case(2, 4, 2, 32, torch.bfloat16, torch.int8, [20, 9], "chain", seed=1)
