@@ -253,3 +253,18 @@ def test_under_autocast():
             out = lm.generate(prompt, 6, top_k=1, cache_dtype=ct)
             spec = lm.generate_speculative(prompt, lm, 6, 3, 0.7, cache_dtype=ct)
             assert out.shape == spec.shape == (2, 18)
+
+
+def test_packed_arguments_have_the_headers_fields():
+    """Every field of the argument structs is 8 bytes wide, so a count of the header's fields is the packed size."""
+    import re
+    from conftest import ROOT
+    from multiscreen import _native
+    text = re.sub(r"/\*.*?\*/", "", open(f"{ROOT}/include/msa.h").read(), flags=re.S)
+    for name, pack, values in (("msa_cache_args", _native.pack_cache_args, [0] * 37),
+                               ("msa_tree_args", _native.pack_tree_args, [0] * 37 + [1.0]),
+                               ("msa_verify_args", _native.pack_verify_args, [0] * 19)):
+        body = re.search(r"typedef struct \{([^{}]*)\} " + name, text).group(1)
+        fields = sum(len(part.split(",")) * (4 if part.split()[0] == "msa_tensor" else 1)
+                     for part in body.split(";") if part.strip())
+        assert len(pack(*values)) == 8 * fields, name
