@@ -326,7 +326,8 @@ int msa_tree_decode(const msa_tree_args* args, void* stream);
  *   draft    : null, or probabilities (B, M - 1, V) of type dtype, strides
  *              (d_sb, d_sn): row i is the distribution that token i + 1 was
  *              drawn from.  Drafts are then a chain: a node whose parent is not
- *              the node before it is never reached.  Needs uniforms.
+ *              the node before it is never reached.  The chain ends before such
+ *              a node and before a token outside [0, V).  Needs uniforms.
  * From node 0 the walk goes on to the first child in index order that is
  * accepted: child i with token x of a node with row p
  *   greedy : x is p's largest entry (the first of equal ones, NaN the largest)

@@ -9,7 +9,7 @@
 //   chain   u_i q(x_i) < p(x_i), q the row that the token was drawn from
 // and where none is, one token more: the row's largest entry, or with u_0 from
 // p without the refused children, from max(p - q, 0), or, past a chain's last
-// node, from p: the first v with weight and cumulated weight > u_0 total.  The
+// node or before one without a token, from p: the first v with weight and cumulated weight > u_0 total.  The
 // tokens so produced are distributed as the target's own.
 // All sums and comparisons are in 64 bits: probabilities of fp32 or fewer bits
 // are exact there and so is u q, and the borders between tokens move by 1e-16.
@@ -229,8 +229,8 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyCall a) {
     const int up = asked ? n.parent : 0;
     double p = asked ? (double)to_f(((const T*)a.target + b * a.t_sb + (int64_t)up * a.t_sn)[n.token]) : 0.0;
     bool taken;
+    const bool on = asked && (!kChain || n.parent == lane - 1);  // a draft that the walk may ask
     if constexpr (kChain) {
-      const bool on = asked && n.parent == lane - 1;
       const double q = on ? (double)to_f(((const T*)a.draft + b * a.d_sb + (int64_t)up * a.d_sn)[n.token]) : 0.0;
       taken = on && (double)u * q < p;
     } else {
@@ -250,9 +250,10 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyCall a) {
       if ((__ballot(taken) & before) != 0ull) taken = false;
     }
     const int last = walk(a, b, lane, n, taken);
-    // the children of the last node, none of them taken
-    const unsigned long long out = __ballot(!kChain && asked && n.parent == last);
-    if (((out >> lane) & 1ull) != 0ull) {
+    // the children of the last node, none of them taken; a chain whose next node
+    // is missing or holds no token of the vocabulary has refused nothing there
+    const unsigned long long out = __ballot(on && n.parent == last);
+    if (!kChain && ((out >> lane) & 1ull) != 0ull) {
       gone[__builtin_popcountll(out & ((1ull << lane) - 1ull))] = n.token;
       const uint32_t bin = (uint32_t)(n.token >> shift);
       atomicOr(&bins[bin >> 5], 1u << (bin & 31u));
@@ -265,7 +266,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyCall a) {
   __syncthreads();
   const int last = last_s, ngone = gone_s;
   const T* prow = (const T*)a.target + b * a.t_sb + (int64_t)last * a.t_sn;
-  const T* qrow = kChain && last < a.M - 1 ? (const T*)a.draft + b * a.d_sb + (int64_t)last * a.d_sn : nullptr;
+  const T* qrow = kChain && ngone > 0 ? (const T*)a.draft + b * a.d_sb + (int64_t)last * a.d_sn : nullptr;
   bool plain = false;  // the second time, if nothing is left: p itself
 
   typedef typename RowLoad<T>::vec vec;

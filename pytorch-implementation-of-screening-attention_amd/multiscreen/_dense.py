@@ -147,7 +147,7 @@ def verify_dense(target, tokens, parents=None, uniforms=None, draft=None):
         if uniforms is None:
             token[b] = best
             continue
-        if draft is not None and node < M - 1:
+        if draft is not None and refused:
             rest = (row - draft[b, node].double()).clamp(min=0.0)
         rest = rest if float(rest.sum()) > 0 else row
         below = rest.cumsum(0)

@@ -474,7 +474,8 @@ def verify_drafts(target, tokens, parents=None, uniforms=None, draft=None):
     None.
     uniforms float32 (B, M) in [0, 1), or None for greedy decoding.
     draft (B, M - 1, V) probabilities in target's dtype, or None: row i is what
-    token i + 1 was drawn from; the drafts are then a chain.
+    token i + 1 was drawn from; the drafts are then a chain, which ends before
+    the first token outside [0, V) (so -1 pads a sequence with fewer drafts).
 
     From node 0 the walk goes on to the first child, in index order, that is
     accepted: with `draft` if u_i q(x) < p(x), without if u_i (1 - the p of the

@@ -43,7 +43,7 @@ def rule(target, tokens, parents, uniforms, draft):
         return walk, largest(row)
     p = [x if x > 0 else 0.0 for x in row]
     weight = [0.0 if v in out else x for v, x in enumerate(p)]
-    if draft is not None and node < M - 1:
+    if draft is not None and any(0 <= int(tokens[c]) < V for c in children):
         weight = [max(x - y, 0.0) if x - y > 0 else 0.0 for x, y in zip(row, draft[node].double().tolist())]
     if not math.fsum(weight) > 0:
         weight = p
@@ -207,6 +207,34 @@ def test_tokens_are_distributed_as_the_target(mode):
     sigma = (p.double() * (1 - p.double()) / B).sqrt()
     assert ((share - p.double()).abs() < 5 * sigma).all(), share.tolist()
     assert 0.2 < float((count > 1).double().mean()) < 0.9
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", FLOATS, ids=_name)
+@pytest.mark.parametrize("pad", [-1, 37, 2 ** 40])
+def test_a_padded_chain_is_the_shorter_chain(dt, pad):
+    """Sequences with fewer drafts than the batch holds: behind them stand tokens outside the vocabulary, or parents that
+    are none, with draft rows of any content."""
+    V, B, M = 37, 64, 6
+    g = torch.Generator().manual_seed(5)
+    logits = 2 * torch.randn(B, M, V, generator=g)
+    p = torch.softmax(logits, -1).to(dt)
+    q = torch.softmax(logits[:, :M - 1] + 0.3 * torch.randn(B, M - 1, V, generator=g), -1).to(dt)
+    tokens = torch.cat((torch.zeros(B, 1), torch.multinomial(q.float().flatten(0, 1), 1, generator=g).view(B, M - 1)), 1).long()
+    u = torch.rand(B, M, generator=g)
+    short = torch.arange(B) % M + 1  # nodes of each sequence
+    behind = torch.arange(M) >= short.unsqueeze(1)
+    padded = torch.where(behind, pad, tokens)
+    parents = torch.where(behind, -1, torch.arange(-1, M - 1))
+    for t, par in ((padded, None), (tokens, parents), (padded, parents)):
+        check(p, t, par, u, q)
+        out = [x.cpu() for x in _ops().verify_drafts(p.to(DEV), t.to(DEV), None if par is None else par.to(DEV), u.to(DEV), q.to(DEV))]
+        for b in range(B):
+            n = int(short[b])
+            one = _ops().verify_drafts(*(x[b:b + 1, :m].contiguous().to(DEV) if x is not None else None
+                                         for x, m in ((p, n), (tokens, n), (None, 0), (u, n), (q, n - 1))))
+            assert out[0][b, :n].tolist() == one[0][0].tolist() and (out[0][b, n:] == -1).all()
+            assert int(out[1][b]) == int(one[1]) and int(out[2][b]) == int(one[2]), b
 
 
 @pytest.mark.gpu

@@ -96,6 +96,21 @@ def test_dense_verify():
                 assert path[b].tolist() == walk + [-1] * (M - len(walk)) and int(count[b]) == len(walk) and int(token[b]) == t
 
 
+def test_dense_verify_of_a_padded_chain():
+    """Behind a sequence's drafts stand tokens outside the vocabulary: the result is the shorter chain's."""
+    g = torch.Generator().manual_seed(1)
+    p, q = (torch.softmax(2 * torch.randn(64, n, 11, generator=g), -1) for n in (4, 3))
+    tok, u = torch.randint(0, 11, (64, 4), generator=g), torch.rand(64, 4, generator=g)
+    for b in range(64):
+        n = b % 4 + 1
+        line = torch.where(torch.arange(4) < n, tok[b], -1)
+        path, count, token = verify_dense(p[b:b + 1], line[None], None, u[b:b + 1], q[b:b + 1])
+        short = verify_dense(p[b:b + 1, :n], tok[b:b + 1, :n], None, u[b:b + 1, :n], q[b:b + 1, :n - 1])
+        assert (int(count), int(token)) == (int(short[1]), int(short[2]))
+        assert path[0].tolist() == short[0][0].tolist() + [-1] * (4 - n)
+        assert rule(p[b], line, [-1, 0, 1, 2], u[b], q[b])[1] == int(token)
+
+
 # ---------------------------------------------------------------------------
 # The model, on both
 # ---------------------------------------------------------------------------
