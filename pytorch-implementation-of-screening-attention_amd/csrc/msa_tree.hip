@@ -36,7 +36,6 @@ namespace msa {
 
 constexpr int kTreeMax = 64;   // nodes of a tree: one lane each
 constexpr int kTreeWaves = 4;  // waves of a block
-// Fewest units of a block, so that a block's sums stay small beside its keys.
 // Fewest units of a block, so that a block's sums stay small beside its keys (16
 // instead of 8: 21 nodes over 5001 e4m3 rows of D = 128 24 -> 30 us, 40 over 6000
 // fp32 of D = 32 27 -> 39; 4: no gain).
