@@ -534,9 +534,6 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C),
   using Tile = typename V::Tile;
   constexpr int NDH = Tile::NDH, NC = Tile::NC;
   constexpr bool kTwo = sizeof(comp) == 2;
-  // Weights as two terms of the operand's type.  One fp16 term (2^-12) is enough
-  // beside a result in bf16 (2^-9).
-  const bool two = kTwo && !(TreeRow<C>::kCodes && PARTS == 1 && a.q_dtype == 1);
   constexpr int kRed = kUnit * V::DP * 4;   // a wave's sums of a node tile
   constexpr int kLds = kTreeWaves * (Tile::BYTES > T * kRed / 2 ? Tile::BYTES : T * kRed / 2);
   __shared__ __align__(16) char lds[kLds];
@@ -710,14 +707,12 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C),
         // rounded once instead of twice, and the second term would not be its rest
         asm volatile("" : "+v"(hi[t][c]));
       }
-      if (two) {
-        if constexpr (kTwo) {
+      if constexpr (kTwo) {
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
+        for (int c = 0; c < NC; ++c) {
 #pragma unroll
-            for (int e = 0; e < M::PER; ++e) s[t][M::PER * c + e] -= M::get(hi[t][c], e);
-            lo[t][c] = M::pack(s[t], M::PER * c);
-          }
+          for (int e = 0; e < M::PER; ++e) s[t][M::PER * c + e] -= M::get(hi[t][c], e);
+          lo[t][c] = M::pack(s[t], M::PER * c);
         }
       }
     }
@@ -730,13 +725,11 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy(D * (int)sizeof(C),
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int t = 0; t < T; ++t) acc[t][d] = M::mma_ng(vf[c], hi[t][c], acc[t][d]);
-      if (two) {
-        if constexpr (kTwo) {
+      if constexpr (kTwo) {
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int t = 0; t < T; ++t) acc[t][d] = M::mma_ng(vf[c], lo[t][c], acc[t][d]);
-        }
+          for (int t = 0; t < T; ++t) acc[t][d] = M::mma_ng(vf[c], lo[t][c], acc[t][d]);
       }
 #pragma unroll
       for (int t = 0; t < T; ++t) guard_all(vf, acc[t][d]);
@@ -948,7 +941,6 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy16(D * (int)sizeof(C
   constexpr int NDT = V::DP / 16;
   constexpr int kRed = NDT * 1024;
   constexpr int kLds = kTreeWaves * (Tile::BYTES > kRed / 2 ? Tile::BYTES : kRed / 2);
-  const bool two = !(TreeRow<C>::kCodes && PARTS == 1 && a.q_dtype == 1);
   __shared__ __align__(16) char lds[kLds];
   __shared__ __align__(16) float kfac[kTreeWaves][kUnit], vfac[kTreeWaves][kUnit], mtab[kTreeWaves][64];
   __shared__ int dtab[kTreeWaves][kTreeMax];
@@ -1115,16 +1107,14 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_occupancy16(D * (int)sizeof(C
     for (int e = 0; e < 8; ++e) w[0][e] = from_f<comp>(s[e]);
     asm volatile("" : "+v"(w[0]));  // one rounding for both its uses (tree_kernel)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[1][e] = two ? from_f<comp>(s[e] - to_f(w[0][e])) : from_f<comp>(0.0f);
+    for (int e = 0; e < 8; ++e) w[1][e] = from_f<comp>(s[e] - to_f(w[0][e]));
     frag vf[NDT];
 #pragma unroll
     for (int d = 0; d < NDT; ++d) vf[d] = value_frag(d);
 #pragma unroll
     for (int d = 0; d < NDT; ++d) acc[d] = Mma16<comp>::mma(vf[d], w[0], acc[d]);
-    if (two) {
 #pragma unroll
-      for (int d = 0; d < NDT; ++d) acc[d] = Mma16<comp>::mma(vf[d], w[1], acc[d]);
-    }
+    for (int d = 0; d < NDT; ++d) acc[d] = Mma16<comp>::mma(vf[d], w[1], acc[d]);
     guard_all16(vf, acc[NDT - 1]);
     guard_all16(w, acc[NDT - 1]);
   }
