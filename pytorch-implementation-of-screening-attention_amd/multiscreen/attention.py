@@ -169,10 +169,10 @@ class ScreeningAttention(nn.Module):
         B = x.shape[0]
         if cache.k_scale is not None:  # 8-bit rows: a tree of one node
             if not torch.is_tensor(pos):
-                if pos + 1 > cache.k.shape[1]:
+                if not 0 <= pos < cache.k.shape[1]:
                     raise IndexError(f"KV cache capacity {cache.k.shape[1]} exceeded at position {pos + 1}")
                 pos = torch.full((1,), pos, dtype=torch.int64, device=x.device)
-            return self.tree_step(x, cache, pos, None, rw)[0]
+            return self.tree_step(x, cache, pos, None, rw, checked=True)[0]
         q, k, v = self.project_qkv(x, x, x)
         r, w = rw if rw is not None else (self.sharpness(), self.window())
         if torch.is_tensor(pos):
@@ -191,15 +191,20 @@ class ScreeningAttention(nn.Module):
             y = screening_core_dense(q, kc, vc, r, w, True, self.eps, q_offset=pos)[:, 0]
         return self.out_proj(y.reshape(B, 1, self.d_model))
 
-    def tree_step(self, x: torch.Tensor, cache, lengths: torch.Tensor, parents=None, rw=None):
+    def tree_step(self, x: torch.Tensor, cache, lengths: torch.Tensor, parents=None, rw=None, checked=False):
         """x (B, M, d): the M <= 64 nodes of a tree of drafted tokens that follows sequence b's
         lengths[b] cached positions (lengths int64, 1 or B elements; parents as in
         ops.tree_decode, None for a chain).  Writes the nodes' k and v behind the committed rows and
         returns the attention output (B, M, d), node i seeing the sequence and its own ancestors,
-        and (k, v), from which KVCache.store_rows keeps an accepted path."""
+        and (k, v), from which KVCache.store_rows keeps an accepted path.
+        A sequence needs 0 <= lengths[b] <= capacity - M: on the CPU others raise IndexError; on the
+        GPU, where the host does not see them, their output is NaN (checked=True: the caller sees to
+        it, and theirs is meaningless)."""
         if not self.causal:
             raise RuntimeError("KV-cache decode is defined for causal self-attention only")
         B, M, _ = x.shape
+        if not x.is_cuda and not bool(cache.has_room(lengths, M).all()):
+            raise IndexError(f"KV cache capacity {cache.k.shape[1]} exceeded by {M} nodes behind positions {lengths.tolist()}")
         q, k, v = self.project_qkv(x, x, x)
         if cache.k_scale is None:
             q, k, v = (t.to(cache.k.dtype) for t in (q, k, v))
@@ -212,7 +217,10 @@ class ScreeningAttention(nn.Module):
             up = torch.arange(-1, M - 1) if parents is None else parents
             kc, vc = cache.read(0, cache.k.shape[1], q.dtype)
             y = tree_dense(q, kc, vc, lengths, up.expand(B, M), r, w, self.eps)
-        return self.out_proj(y.to(x.dtype).reshape(B, M, self.d_model)), (k, v)
+        y = self.out_proj(y.to(x.dtype).reshape(B, M, self.d_model))
+        if x.is_cuda and not checked:
+            y = torch.where(cache.has_room(lengths, M).view(-1, 1, 1), y, math.nan)
+        return y, (k, v)
 
 
 class KVCache:
@@ -245,6 +253,10 @@ class KVCache:
             from . import _native
             nbytes = int(_native.lib().msa_decode_workspace_bytes(batch, num_heads, head_dim, capacity))
             self.workspace = torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=device)
+
+    def has_room(self, lengths, rows):
+        """Of each element of lengths (int64): whether `rows` positions from there on lie in the cache."""
+        return lengths == lengths.clamp(0, self.k.shape[1] - rows)
 
     def store(self, k, v, pos):
         T = k.shape[1]

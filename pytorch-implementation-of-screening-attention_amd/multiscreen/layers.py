@@ -57,10 +57,10 @@ class MultiscreenBlock(nn.Module):
         x = x + self.attn.decode(normed, cache, pos, rw)
         return x + self.ffn(self.norm2(x))
 
-    def tree_step(self, x: torch.Tensor, cache, lengths, parents=None, rw=None):
+    def tree_step(self, x: torch.Tensor, cache, lengths, parents=None, rw=None, checked=False):
         """The nodes x (B, M, d) of a tree of drafted tokens (ScreeningAttention.tree_step); returns
         their outputs and the layer's (k, v)."""
-        y, kv = self.attn.tree_step(self.norm1(x), cache, lengths, parents, rw)
+        y, kv = self.attn.tree_step(self.norm1(x), cache, lengths, parents, rw, checked)
         x = x + y
         return x + self.ffn(self.norm2(x)), kv
 

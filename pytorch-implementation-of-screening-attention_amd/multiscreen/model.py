@@ -129,7 +129,8 @@ class MultiscreenLM(nn.Module):
         committed token at position lengths[b] (int64, 1 or B elements), the others drafted
         continuations (parents as in ops.tree_decode; None: a chain).  Writes the nodes' rows into
         the caches from position lengths[b] on.  Positions past the last position embedding take
-        the last one.
+        the last one.  0 <= lengths[b] <= capacity - M: others raise IndexError on the CPU; on the GPU
+        the logits of their sequences are NaN.
         Returns the logits (B, M, vocab) and per layer (k, v), for accept()."""
         B, M = tokens.shape
         if parents is None:
@@ -137,12 +138,14 @@ class MultiscreenLM(nn.Module):
         else:
             parents = parents.expand(B, M)
             depth = tree_relations(parents)[1]
-        pos = (lengths.view(-1, 1) + depth).clamp(max=self.pos_emb.num_embeddings - 1)
+        pos = (lengths.view(-1, 1) + depth).clamp(0, self.pos_emb.num_embeddings - 1)
         x = self.emb_dropout(self.token_emb(tokens) + self.pos_emb(pos))
         kvs = []
         for i, (block, cache) in enumerate(zip(self.blocks, caches)):
-            x, kv = block.tree_step(x, cache, lengths, parents, None if rws is None else rws[i])
+            x, kv = block.tree_step(x, cache, lengths, parents, None if rws is None else rws[i], checked=True)
             kvs.append(kv)
+        if x.is_cuda and caches:  # once, for all layers
+            x = torch.where(caches[0].has_room(lengths, M).view(-1, 1, 1), x, math.nan)
         return self._head(x), kvs
 
     @torch.no_grad()
