@@ -285,8 +285,8 @@ int msa_cache_read(const msa_cache_args* args, void* stream);
  * Node i stands at position n_b + depth_i (a root's depth is 0) and sees the
  * committed keys of its window (pos - w, pos], and of the drafted rows its own
  * and its ancestors' within the window.  y (B, N, H, D) contiguous, of type
- * dtype.  A key row that is not finite is never live; a value row that is not
- * finite makes the nodes that a live pair brings it to NaN, and no others.
+ * dtype.  A key or query row that is not finite is never live; a value row that
+ * is not finite makes the nodes that a live pair brings it to NaN, and no others.
  * window_hint as in msa_decode: it sizes the launch.  How the keys are split
  * over blocks (the sums' order, so y's rounding) depends on it, the shapes, the
  * length and the windows: equal calls give bitwise equal y.

@@ -103,8 +103,11 @@ def tree_dense(q, k, v, lengths, parents, r, w, eps=1e-8):
     m = torch.where(seen.unsqueeze(1) & (dist >= 0) & (dist < wh), 0.5 * (torch.cos(math.pi * dist / wh) + 1.0), 0.0)
     qn, kn, vn = (F.normalize(x.transpose(1, 2).float(), dim=-1, eps=eps) for x in (q, k, v))
     a = torch.relu(1.0 - r.float().view(1, H, 1, 1) * (1.0 - qn @ kn.transpose(-2, -1)))
-    p = torch.where(m > 0, a * a * m, 0.0)
-    h = p @ torch.where((p > 0).any(2, keepdim=True).transpose(2, 3), vn, 0.0)
+    p = a * a * m
+    p = torch.where(p > 0, p, 0.0)  # a NaN, of a q or k row that is not finite, is not live
+    odd = ~torch.isfinite(v).all(-1).transpose(1, 2).unsqueeze(2)                         # (B, H, 1, cap)
+    h = p @ torch.where(odd.transpose(2, 3), 0.0, vn)
+    h = torch.where((odd & (p > 0)).any(-1, keepdim=True), math.nan, h)  # a live pair brings NaN to its node alone
     size = torch.linalg.vector_norm(h, dim=-1, keepdim=True).clamp(min=eps)
     return (h * (torch.tanh(size) / size)).transpose(1, 2).to(q.dtype)
 
