@@ -123,8 +123,12 @@ def verify_dense(target, tokens, parents=None, uniforms=None, draft=None):
             path[b, length] = node
             length += 1
             row = target[b, node].double()
-            row = row if uniforms is None else row.nan_to_num(0.0).clamp(min=0.0)
-            best = int((row == row.amax()).nonzero()[0]) if uniforms is None else -1
+            best = -1
+            if uniforms is None:  # a NaN is the largest entry
+                top = row.isnan() if row.isnan().any() else row == row.amax()
+                best = int(top.nonzero()[0])
+            else:
+                row = row.nan_to_num(0.0).clamp(min=0.0)
             rest, left, refused, taken = row.clone(), 1.0, False, -1
             for c in range(max(1, node + 1), M):
                 x = int(tokens[b, c])
