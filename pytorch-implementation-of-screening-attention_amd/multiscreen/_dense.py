@@ -127,9 +127,8 @@ def verify_dense(target, tokens, parents=None, uniforms=None, draft=None):
             if uniforms is None:  # a NaN is the largest entry
                 top = row.isnan() if row.isnan().any() else row == row.amax()
                 best = int(top.nonzero()[0])
-            else:
-                row = row.nan_to_num(0.0).clamp(min=0.0)
-            rest, left, refused, taken = row.clone(), 1.0, False, -1
+            p = torch.where(row > 0, row, 0.0)  # entries that are negative or NaN count as 0
+            rest, left, refused, taken = p.clone(), 1.0, False, -1
             for c in range(max(1, node + 1), M):
                 x = int(tokens[b, c])
                 if up[c] != node or not 0 <= x < V or (draft is not None and c != node + 1):
@@ -155,8 +154,9 @@ def verify_dense(target, tokens, parents=None, uniforms=None, draft=None):
             token[b] = best
             continue
         if draft is not None and refused:
-            rest = (row - draft[b, node].double()).clamp(min=0.0)
-        rest = rest if float(rest.sum()) > 0 else row
+            more = row - draft[b, node].double()
+            rest = torch.where(more > 0, more, 0.0)
+        rest = rest if float(rest.sum()) > 0 else p
         below = rest.cumsum(0)
         over = ((below > float(uniforms[b, 0]) * float(below[-1])) & (rest > 0)).nonzero()
         some = (rest > 0).nonzero()

@@ -8,7 +8,7 @@ import torch
 
 from multiscreen._dense import verify_dense
 from test_gpu_cache_rows import FLOATS, _name
-from test_gpu_verify_drafts import rule
+from test_gpu_verify_drafts import check as check_kernel, rule
 
 
 def check(target, tokens, parents, uniforms, draft):
@@ -51,3 +51,33 @@ def test_borders(dt):
                 q = torch.zeros(1, 1, V)
                 q[0, 0, tok], q[0, 0, (tok + 1) % V] = 0.25, 0.75
                 check(p.to(dt), t, None, u, q.to(dt))
+
+
+@pytest.mark.parametrize("check", [check, pytest.param(check_kernel, marks=pytest.mark.gpu)], ids=["cpu", "cuda"])
+def test_odd_entries(check):
+    """NaN, negative and infinite entries of the target's and the draft's rows count as the operator has it."""
+    V = 60
+    g = torch.Generator().manual_seed(1)
+    odd = torch.softmax(torch.randn(1, 4, V, generator=g), -1)
+    odd[0, :, 3], odd[0, :, 4] = math.nan, -0.5
+    par = torch.tensor([[-1, 0, 0, 0]])
+    for u in ([0.001, 0.0, 0.0, 0.9], [0.9, 0.5, 0.9, 0.99]):
+        check(odd, torch.tensor([[0, 3, 4, 8]]), par, torch.tensor([u]), None)
+    draft = torch.softmax(torch.randn(1, 3, V, generator=g), -1)
+    for column, value in ((8, math.nan), (40, math.nan), (40, math.inf), (8, math.inf)):
+        q = draft.clone()
+        q[0, :, column] = value
+        for u0 in (0.0, 0.3, 0.99):
+            check(odd, torch.tensor([[0, 8, 9, 10]]), None, torch.tensor([[u0, 0.99, 0.99, 0.99]]), q)
+    high = odd.clone()
+    high[0, :, 20] = math.inf
+    for u0 in (0.0, 0.3, 0.99):
+        check(high, torch.tensor([[0, 8, 9, 10]]), par, torch.tensor([[u0, 0.99, 0.99, 0.99]]), None)
+        check(high, torch.tensor([[0, 20, 9, 10]]), None, torch.tensor([[u0, 0.99, 0.99, 0.99]]), draft)
+    zero = torch.zeros(1, 2, V)
+    u = torch.tensor([[0.3, 0.9]])
+    check(zero, torch.tensor([[0, 5]]), None, u, None)
+    check(zero, torch.tensor([[0, 5]]), None, u, zero[:, :1])
+    few = zero.clone()
+    few[0, 0, 5] = 0.25
+    check(few, torch.tensor([[0, 5]]), None, u, few[:, :1] * 2 + 0.5)  # the draft above the target everywhere
