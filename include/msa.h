@@ -248,8 +248,10 @@ typedef struct { void* p; int64_t sb, st, sh; } msa_tensor;
  *   start    : null, or device int64 positions, one (start_n = 1) or one per
  *              sequence (start_n = B): row t goes to position start + t.  Null:
  *              start0.  Rows at positions outside the cache are not written.
- * k and v must not overlap the caches (rows move through a copy, as their order
- * is open).  Everything else of the cache is left as it was.
+ * No two rows of the caches and their scales may share memory (refused, also
+ * where strides of two tensors interleave too finely to tell).  k and v must not
+ * overlap the caches (rows move through a copy, as their order is open).
+ * Everything else of the cache is left as it was.
  *
  * msa_cache_read takes the same struct: the values of positions start .. start
  * + T - 1 go to k, v (B, T, H, D) of type dtype: code * scale, rounded once; a

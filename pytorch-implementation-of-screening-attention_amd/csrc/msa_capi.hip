@@ -473,6 +473,54 @@ static int check_cache(int B, int T, int H, int D, int dtype, int cache_cap, int
   return MSA_OK;
 }
 
+// Rows of a tensor that a kernel writes: `bytes` each, strides in bytes, the
+// dimensions of more than one from the largest stride down.
+struct RowSet {
+  __int128 at;
+  int n = 0;
+  int dim[3];
+  __int128 count[3], stride[3], bytes;
+  RowSet(const msa_tensor& t, const int (&counts)[3], int64_t elements, int64_t es) : at((uintptr_t)t.p), bytes(elements * es) {
+    const int64_t st[3] = {t.sb, t.st, t.sh};
+    for (int d = 0; d < 3; ++d) {
+      if (counts[d] <= 1) continue;
+      int i = n++;
+      for (; i > 0 && stride[i - 1] < (__int128)st[d] * es; --i) {
+        dim[i] = dim[i - 1]; count[i] = count[i - 1]; stride[i] = stride[i - 1];
+      }
+      dim[i] = d; count[i] = counts[d]; stride[i] = (__int128)st[d] * es;
+    }
+  }
+  // Bytes from the first row to the end of the last, of the dimensions from i on.
+  __int128 extent(int i) const {
+    __int128 e = bytes;
+    for (; i < n; ++i) e += (count[i] - 1) * stride[i];
+    return e;
+  }
+  // Whether no two rows share memory: each stride passes what lies inside it
+  // (layouts of interleaved dimensions count as shared).
+  bool separate() const {
+    for (int i = 0; i < n; ++i)
+      if (stride[i] < extent(i + 1)) return false;
+    return true;
+  }
+};
+
+// Whether rows of a and b, both separate, share memory; b's first row stands x
+// bytes behind a's, and dimensions before i are settled.  Exact down to the first
+// dimension in which the layouts differ, then by the ranges that are left.
+static bool rows_meet(const RowSet& a, const RowSet& b, __int128 x, int i = 0) {
+  if (x >= a.extent(i) || -x >= b.extent(i)) return false;
+  if (i == a.n || i == b.n || a.dim[i] != b.dim[i] || a.stride[i] != b.stride[i]) return true;
+  // rows `steps` apart in this dimension; those less than a stride apart may meet
+  const __int128 s = a.stride[i], steps = x >= 0 ? x / s : -((-x + s - 1) / s);
+  for (int e = 0; e < 2; ++e) {
+    const __int128 d = steps + e;
+    if (d < a.count[i] && -d < a.count[i] && rows_meet(a, b, x - d * s, i + 1)) return true;
+  }
+  return false;
+}
+
 // Both directions of msa_cache_args.
 static int cache_call(const msa_cache_args* a, int read, void* stream, const char* what) {
   if (a == nullptr) return fail(MSA_ERR_INVALID, "args is null");
@@ -488,12 +536,19 @@ static int cache_call(const msa_cache_args* a, int read, void* stream, const cha
   if (a->start != nullptr && a->start_n != 1 && a->start_n != a->B)
     return fail(MSA_ERR_INVALID, "start holds %lld positions, 1 or B=%d needed", (long long)a->start_n, c.B);
   if (c.B == 0 || c.T == 0 || c.Tx == 0) return ok();
-  const msa_tensor* out[4] = {read ? &a->k : &a->kcache, read ? &a->v : &a->vcache, &a->kscale, &a->vscale};
-  for (int z = 0; z < (read || c.cache_dtype == c.dtype ? 2 : 4); ++z)
-    if ((c.B > 1 && out[z]->sb == 0) || (c.T > 1 && out[z]->st == 0) || (c.H > 1 && out[z]->sh == 0))
-      return fail(MSA_ERR_INVALID, "rows that are written must not share memory (a stride is 0)");
   if ((rc = check_tensor("k", a->k.p, a->k.sb, a->k.st, a->k.sh, c.dtype)) != MSA_OK) return rc;
   if ((rc = check_tensor("v", a->v.p, a->v.sb, a->v.st, a->v.sh, c.dtype)) != MSA_OK) return rc;
+  // what is written: k and v by a read; the caches' rows, at any position, and their scales by a write
+  const int64_t es = c.dtype == MSA_F32 ? 4 : 2, ces = c.cache_dtype == c.dtype ? es : 1;
+  const int counts[3] = {c.B, read ? c.T : c.cap, c.H};
+  const RowSet out[4] = {{read ? a->k : a->kcache, counts, c.D, read ? es : ces}, {read ? a->v : a->vcache, counts, c.D, read ? es : ces},
+                         {a->kscale, counts, 1, 4}, {a->vscale, counts, 1, 4}};
+  const int outs = read || c.cache_dtype == c.dtype ? 2 : 4;
+  for (int i = 0; i < outs; ++i) {
+    bool shared = !out[i].separate();
+    for (int j = 0; j < i; ++j) shared = shared || rows_meet(out[j], out[i], out[i].at - out[j].at);
+    if (shared) return fail(MSA_ERR_INVALID, "rows that are written must not share memory (strides or tensors overlap)");
+  }
   c.x[0] = a->k.p; c.x[1] = a->v.p; c.xs[0] = strides_of(a->k); c.xs[1] = strides_of(a->v);
   c.c[0] = a->kcache.p; c.c[1] = a->vcache.p; c.cs[0] = strides_of(a->kcache); c.cs[1] = strides_of(a->vcache);
   c.s[0] = (float*)a->kscale.p; c.s[1] = (float*)a->vscale.p;

@@ -347,8 +347,9 @@ def cache_write(k, v, kcache, vcache, start, kscale=None, vscale=None, rows=None
     rows (B, T') int64, count (B) int64: row rows[b, t] of k and v goes to
     position start + t, for t < count[b] only: the accepted path of
     verify_drafts.  Rows outside k are not written.
-    k and v must not overlap the caches, as the order of the rows is open.  The
-    rest of the cache is left as it was.  No gradient flows through it.
+    The caches' rows and scales must not share memory (refused).  k and v must not
+    overlap the caches, as the order of the rows is open.  The rest of the cache
+    is left as it was.  No gradient flows through it.
     """
     index = k.get_device()
     _one_gpu("cache_write", index, v, kcache, vcache, kscale, vscale, rows, count,
