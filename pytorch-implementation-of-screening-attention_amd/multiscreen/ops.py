@@ -185,11 +185,15 @@ def _decode_args(q, kcache, vcache, r, w):
     return q, kcache, vcache, r32, w32
 
 
-def _decode_workspace(L, workspace, B, H, D, length, dev):
-    need = int(L.msa_decode_workspace_bytes(B, H, D, int(length)))
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty((max(need, 16),), dtype=torch.uint8, device=dev)
+def _scratch(workspace, need, device):
+    """The caller's workspace if it holds `need` bytes in one piece, else one of this call's own."""
+    if workspace is None or not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty((need,), dtype=torch.uint8, device=device)
     return workspace
+
+
+def _decode_workspace(L, workspace, B, H, D, length, dev):
+    return _scratch(workspace, max(int(L.msa_decode_workspace_bytes(B, H, D, int(length))), 16), dev)
 
 
 def decode_step(q, kcache, vcache, cache_len, r, w, eps=1e-8, workspace=None, window_hint=0):
@@ -428,6 +432,8 @@ def tree_decode(q, kcache, vcache, lengths, parents, r, w, eps=1e-8, kscale=None
     position n_b + depth_i and sees the committed keys of its window, itself
     and its ancestors.
     window_hint: 0, or a bound on ceil(w) over the heads (sizes the launch).
+    workspace: scratch of this call on q's GPU; where it is None, too small or not
+    contiguous the call allocates its own.
     Returns y (B, N, H, D) = TanhNorm(h), in q's dtype; no gradient.
     """
     index = q.get_device()
@@ -455,8 +461,8 @@ def tree_decode(q, kcache, vcache, lengths, parents, r, w, eps=1e-8, kscale=None
     y = torch.empty((B, N, H, D), dtype=dtype, device=q.device) if not q.is_contiguous() else torch.empty_like(q)
     qt = _DTYPES[dtype]
     need = L.msa_tree_workspace_bytes(B, H, N, D, qt, ct, cap, hint)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
+    if need:
+        workspace = _scratch(workspace, need, q.device)
     _launch("msa_tree_decode", L.msa_tree_decode, index,
             _native.pack_tree_args(*qargs, *cache, lengths.data_ptr(), par, r.data_ptr(), w.data_ptr(), y.data_ptr(),
                                    workspace.data_ptr() if need else 0, need, lengths.shape[0], par_sb, B, N, H, D, qt,
