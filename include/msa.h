@@ -344,6 +344,7 @@ int msa_tree_decode(const msa_tree_args* args, void* stream);
  * q, 0) where a draft was refused, p itself behind a chain's last node or
  * where no weight is left (token 0 if p has none).
  * workspace: msa_verify_workspace_bytes (greedy; 0 with uniforms).
+ * With uniforms B < 2^22; greedy B * M < 2^24 and V <= 65535 * 8192.
  */
 typedef struct {
   const void* target;

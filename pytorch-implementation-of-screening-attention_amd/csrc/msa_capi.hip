@@ -628,10 +628,13 @@ int msa_verify(const msa_verify_args* a, void* stream) {
   const int B = size_of(a->B), M = size_of(a->M), dtype = size_of(a->dtype);
   if (dtype != MSA_F32 && dtype != MSA_BF16 && dtype != MSA_F16)
     return fail(MSA_ERR_INVALID, "dtype must be MSA_F32, MSA_BF16 or MSA_F16");
-  if (B < 0 || B > (1 << 24) || M < 1 || M > MSA_TREE_MAX)
-    return fail(MSA_ERR_INVALID, "a tree holds 1 to %d nodes and a batch at most 2^24 sequences, got M=%d, B=%d",
-                MSA_TREE_MAX, M, B);
+  if (B < 0 || M < 1 || M > MSA_TREE_MAX)
+    return fail(MSA_ERR_INVALID, "a tree holds 1 to %d nodes, got M=%d, B=%d", MSA_TREE_MAX, M, B);
   if (a->V < 1 || a->V > 0x7fffffff) return fail(MSA_ERR_INVALID, "the vocabulary must hold 1 to 2^31 - 1 tokens");
+  // a grid has fewer than 2^32 threads along x and at most 65535 blocks along y
+  if (a->uniforms == nullptr ? (int64_t)B * M >= 1 << 24 || msa::verify_parts(a->V) > 65535 : B >= 1 << 22)
+    return fail(MSA_ERR_INVALID, "at most 2^22 - 1 sequences; greedy: 2^24 - 1 rows of at most 65535 * 8192 tokens, got B=%d, M=%d, V=%lld",
+                B, M, (long long)a->V);
   if (a->draft != nullptr && a->uniforms == nullptr) return fail(MSA_ERR_INVALID, "draft probabilities need uniforms");
   if (B == 0) return ok();
   const uintptr_t es = dtype == MSA_F32 ? 4 : 2;
