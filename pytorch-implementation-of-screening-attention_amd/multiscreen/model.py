@@ -175,6 +175,8 @@ class MultiscreenLM(nn.Module):
             raise ValueError(f"num_drafts must be in 1 .. 63, got {num_drafts}")
         if max_new_tokens <= 0:
             return input_ids
+        if B == 0:
+            return input_ids.new_zeros(0, T + max_new_tokens, dtype=torch.int64)
         end = T + max_new_tokens
         for m in (self, draft):
             if end > m.pos_emb.num_embeddings:
