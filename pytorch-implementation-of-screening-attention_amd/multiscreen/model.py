@@ -187,7 +187,7 @@ class MultiscreenLM(nn.Module):
         # room for the drafts behind the last position of a sequence that is done
         both = [(m, m.new_cache(B, end + num_drafts + 1, m._cache_dtype(dev, cache_dtype), dev)) for m in (self, draft)]
         logits = [m.prefill(input_ids, caches) for m, caches in both][0]
-        out = torch.cat((input_ids, input_ids.new_zeros(B, max_new_tokens + num_drafts + 1)), 1)
+        out = torch.cat((input_ids.long(), input_ids.new_zeros(B, max_new_tokens + num_drafts + 1, dtype=torch.int64)), 1)
         lengths = torch.full((B,), T, dtype=torch.int64, device=dev)
         token = self._pick(_probabilities(logits, temperature, top_k))
         out[:, T] = token.squeeze(1)

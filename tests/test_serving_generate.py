@@ -14,3 +14,16 @@ def test_an_empty_batch(dev):
     for t in (0, 1.0):
         got = lm.generate_speculative(none, lm, 4, temperature=t)
         assert got.shape == (0, 9) and got.dtype == lm.generate(none, 4).dtype
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_prompts_of_32_bit_tokens(dev):
+    lm, small = lm_of(dev), lm_of(dev, seed=5, layers=1)
+    prompt = prompt_of(2, 9, VOCAB, dev)
+    got = lm.generate_speculative(prompt.int(), small, 12, 3, temperature=0)
+    assert got.dtype == lm.generate(prompt.int(), 2).dtype == torch.int64
+    assert torch.equal(got, lm.generate_greedy(prompt, 12))
+    torch.manual_seed(3)
+    a = lm.generate_speculative(prompt.int(), small, 12, 3)
+    torch.manual_seed(3)
+    assert torch.equal(a, lm.generate_speculative(prompt, small, 12, 3))
