@@ -179,8 +179,8 @@ class MultiscreenLM(nn.Module):
             return input_ids.new_zeros(0, T + max_new_tokens, dtype=torch.int64)
         end = T + max_new_tokens
         for m in (self, draft):
-            if end > m.pos_emb.num_embeddings:
-                raise IndexError(f"{end} positions exceed the model's {m.pos_emb.num_embeddings}")
+            if end - 1 > m.pos_emb.num_embeddings:  # the last token is not read again
+                raise IndexError(f"{end - 1} positions exceed the model's {m.pos_emb.num_embeddings}")
         if draft.lm_head.out_features != self.lm_head.out_features:
             raise ValueError("the draft model's vocabulary differs")
         dev = input_ids.device
