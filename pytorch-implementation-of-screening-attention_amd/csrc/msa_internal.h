@@ -138,7 +138,6 @@ struct TreeCall {
   int blocks;   // blocks that share a sequence's keys; H: a block per head
   hipStream_t stream;
 };
-int tree_max_nodes();
 int tree_blocks(int B, int H, int N, int D, int q_dtype, int cache_dtype, int span);
 hipError_t launch_tree(const TreeCall& c);
 

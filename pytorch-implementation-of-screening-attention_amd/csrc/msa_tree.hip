@@ -29,12 +29,14 @@
 // 16-column form: 56 and 37 us, half to two thirds of the issue slots); short
 // windows the latency of the call (12 us at 9 units a head, of which the launch
 // and the tree take 4 and a unit's way through a wave 2 to 3).
+#include "../../include/msa.h"
 #include "msa_device.h"
 #include "msa_internal.h"
 
 namespace msa {
 
 constexpr int kTreeMax = 64;   // nodes of a tree: one lane each
+static_assert(kTreeMax == MSA_TREE_MAX);
 constexpr int kTreeWaves = 4;  // waves of a block
 // Fewest units of a block, so that a block's sums stay small beside its keys (16
 // instead of 8: 21 nodes over 5001 e4m3 rows of D = 128 24 -> 30 us, 40 over 6000
@@ -1202,7 +1204,6 @@ __global__ __launch_bounds__(256) void tree_reduce_kernel(TreeCall a) {
   else store4((float*)a.y + at, x[0] * fy, x[1] * fy, x[2] * fy, x[3] * fy);
 }
 
-int tree_max_nodes() { return kTreeMax; }
 // Whether a wave takes all of more than 32 nodes: its registers hold two tiles'
 // operands and sums for rows of at most 64 values in 2-byte operands.  A wave a
 // tile converts, votes on and stages every unit twice: 4 x 64 nodes over 30K bf16
