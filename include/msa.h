@@ -254,8 +254,8 @@ typedef struct { void* p; int64_t sb, st, sh; } msa_tensor;
  * Everything else of the cache is left as it was.
  *
  * msa_cache_read takes the same struct: the values of positions start .. start
- * + T - 1 go to k, v (B, T, H, D) of type dtype: code * scale, rounded once; a
- * copy where cache_dtype is dtype.  Positions outside the cache read as zeros.
+ * + T - 1 go to k, v (B, T, H, D) of type dtype: the fp32 product code * scale,
+ * rounded to dtype; a copy where cache_dtype is dtype.  Positions outside the cache read as zeros.
  * rows and count must be null.
  */
 typedef struct {

@@ -386,8 +386,8 @@ def cache_write(k, v, kcache, vcache, start, kscale=None, vscale=None, rows=None
 
 def cache_read(kcache, vcache, kscale, vscale, start, length, dtype):
     """The rows at positions start .. start + length - 1 of a cache (as
-    cache_write takes it) in `dtype`: code * scale, rounded once; (k, v), each
-    contiguous (B, length, H, D).  With a device `start`, positions outside the
+    cache_write takes it) in `dtype`: the float32 product code * scale, rounded to
+    dtype; (k, v), each contiguous (B, length, H, D).  With a device `start`, positions outside the
     cache read as zeros."""
     index = kcache.get_device()
     _one_gpu("cache_read", index, vcache, kscale, vscale, start if isinstance(start, torch.Tensor) else None)
