@@ -187,8 +187,14 @@ class ScreeningAttention(nn.Module):
             y = ops.decode_step(q[:, 0].to(cache.k.dtype), cache.k, cache.v, pos + 1, r, w, self.eps,
                                 cache.workspace, cache.window_hint).to(x.dtype)
         else:
-            kc, vc = cache.k[:, :pos + 1], cache.v[:, :pos + 1]
-            y = screening_core_dense(q, kc, vc, r, w, True, self.eps, q_offset=pos)[:, 0]
+            rows = (q, cache.k[:, :pos + 1], cache.v[:, :pos + 1])
+            ct = cache.k.dtype
+            if ct != q.dtype and not torch.is_autocast_enabled("cpu"):
+                # the cache's type is the query's and the result's too, as on the GPU
+                rows = tuple(t.to(ct).to(torch.promote_types(q.dtype, ct)) for t in rows)
+            y = screening_core_dense(*rows, r, w, True, self.eps, q_offset=pos)[:, 0]
+            if rows[0] is not q:
+                y = y.to(ct).to(x.dtype)
         return self.out_proj(y.reshape(B, 1, self.d_model))
 
     def tree_step(self, x: torch.Tensor, cache, lengths: torch.Tensor, parents=None, rw=None, checked=False):

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from test_serving import CODES, DEVICES, prompt_of
-from test_serving_attention import VOCAB, lm_of
+from test_serving_attention import VOCAB, apart, blind, lm_of
 
 
 @pytest.mark.parametrize("dev", DEVICES)
@@ -41,3 +41,22 @@ def test_up_to_the_last_position(dev, ct):
             assert torch.equal(lm.generate_speculative(prompt, drafter, new, drafts, temperature=0, cache_dtype=ct), want)
     with pytest.raises(IndexError):
         lm.generate_speculative(prompt, small, 20)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("ct", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_caches_of_another_floating_type(dev, dt, ct):
+    """A token decoded over rows of ct is a tree of one node over them."""
+    lm, T = lm_of(dev).to(dt), 20
+    prompt, token = prompt_of(2, T, VOCAB, dev), prompt_of(2, 1, VOCAB, dev, seed=2)
+    one, two, full = (lm.new_cache(2, 32, t, dev) for t in (ct, ct, dt))
+    for c in (one, two, full):
+        lm.prefill(prompt, c)
+    got, ref = lm.decode_step(token, one, T), lm.tree_step(token, two, torch.tensor([T], device=dev))[0][:, 0]
+    # roundings of the narrower type through two layers: 2^-8 of every activation, some ten of them a layer
+    coarse = torch.bfloat16 in (dt, ct)
+    assert apart(got, ref) < (0.1 if coarse else 2e-2) and apart(got, lm.decode_step(token, full, T)) < (0.1 if coarse else 2e-2)
+    assert apart(blind(lm).decode_step(token, full, T), got) > 0.4
+    assert all(c.k.dtype == ct for c in one)
+    assert lm.generate_greedy(prompt, 4, cache_dtype=ct).shape == lm.generate(prompt, 4, cache_dtype=ct).shape == (2, T + 4)
