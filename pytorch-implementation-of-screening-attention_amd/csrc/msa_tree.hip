@@ -24,11 +24,11 @@
 // that keeps small weights clear of its subnormals.
 //
 // What bounds it: long windows of few nodes the cache's bytes (one token of 16
-// sequences over 100K int8 positions: 140 us, 6.2 TB/s); many nodes or live units
-// the vector instructions of a unit (about 570 for 64 nodes of bf16, 350 for the
-// 16-column form: 56 and 37 us, half to two thirds of the issue slots); short
-// windows the latency of the call (12 us at 9 units a head, of which the launch
-// and the tree take 4 and a unit's way through a wave 2 to 3).
+// sequences over 94K int8 positions on average, 819 MB: 140 us, 5.9 TB/s); many
+// nodes or live units the vector instructions of a unit (about 570 for 64 nodes of
+// bf16, 340 for the 16-column form: 56 and 37 to 41 us, half to two thirds of the
+// issue slots); short windows the latency of the call (12 us at 9 units a head, of
+// which the launch and the tree take 4 and a unit's way through a wave 2 to 3).
 #include "../../include/msa.h"
 #include "msa_device.h"
 #include "msa_internal.h"
@@ -49,7 +49,11 @@ constexpr int kTreeMinUnits = 8;
 // 2 .. 1500 int8 84, shared 82).
 constexpr int kTreeSmall = 24, kTreeLong = 64;
 
-// Waves per SIMD that the kernel's registers are budgeted for.
+// Waves per SIMD that the kernel's registers are budgeted for, by the bytes of
+// the stored row.  Operands of 8-bit rows are fp16, so <int8 or fp8, 32, 1, 2>
+// spill 12 and 37 registers at 3 and the D = 128 ones 3 to 6; most 2-byte and 8-bit
+// instances of one tile need fewer than they are given, and one or two more of
+// their waves fit.
 constexpr int tree_occupancy(int row_bytes, int parts) {
   return row_bytes * parts <= 64 ? 3 : row_bytes <= 256 ? 2 : 1;
 }
@@ -1215,8 +1219,8 @@ bool tree_both(int N, int D, bool f32) { return N > 32 && D <= 64 && !f32; }
 // bytes bound, the same.  (The transposed reads of natural column blocks, 16 d +
 // 0 .. 15, spread over twice the banks and were no faster.)
 bool tree_few(int N, bool f32_operands) { return N <= 16 && !f32_operands; }
-// Blocks of a sequence: as many as run at one time on the card's 256 CUs share
-// its heads' keys; one a head (H) where heads are short, or the batch alone
+// Blocks of a sequence: as many as run at one time on the card's 256 CUs by the
+// waves budgeted above (more fit of some instances) share its heads' keys; one a head (H) where heads are short, or the batch alone
 // fills the card several times over with heads that are not long.
 int tree_blocks(int B, int H, int N, int D, int q_dtype, int cache_dtype, int span) {
   const int64_t units = ((int64_t)span + N + kUnit - 1) / kUnit;

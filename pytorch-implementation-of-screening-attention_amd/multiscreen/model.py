@@ -164,7 +164,8 @@ class MultiscreenLM(nn.Module):
         """generate() with `draft`, a smaller model of the same vocabulary: it drafts num_drafts tokens
         one by one, this model scores them in one step (tree_step), and ops.verify_drafts keeps those
         that leave the tokens distributed as generate()'s own.  temperature 0 is greedy: the tokens
-        of generate_greedy, up to the rounding of logits that nearly tie.
+        of generate_greedy, up to the rounding of logits that nearly tie.  The steps are eager: a
+        round takes as long as num_drafts + 1 of generate()'s steps of the two models.
 
         cache_dtype: as in generate().  Returns (B, T + max_new_tokens) token ids.
         """
