@@ -365,6 +365,110 @@ typedef struct {
 size_t msa_verify_workspace_bytes(int B, int M, int64_t V, int greedy);
 int msa_verify(const msa_verify_args* args, void* stream);
 
+/*
+ * Losses of rows against a vocabulary, straight from the rows: no logits are
+ * kept.  The reference forms them all (its loss is F.cross_entropy of lm_head's
+ * output, model.py:101-106); its distillation has no counterpart.
+ *   hidden   : (N, d) of type dtype, unit stride over d, hidden_ld elements
+ *              from row to row (any alignment: rows that count are copied).
+ *   weight   : (V, d) of type dtype, unit stride over d, weight_ld from row to
+ *              row.  Used in place where its rows are 16-byte aligned, d % 32
+ *              == 0 and dtype is not MSA_F32; else copied once a call.
+ *   ids      : device int64 (N, K), ids_ld from row to row.
+ *   teacher  : null: cross entropy, K = 1, z = hidden . weight^T,
+ *                L_n = ln sum_v exp z_nv - z_n,ids(n)
+ *              and rows with ids(n) == ignore_index do not count.
+ *              Else (N, K) of type teacher_dtype, teacher_ld from row to row, 1
+ *              <= K <= MSA_HEAD_MAX_K: the row's largest logits of a teacher and
+ *              the tokens ids that they belong to.  With p = softmax(teacher /
+ *              T) over the row's entries and q = softmax(z / T)
+ *                L_n = T^2 sum_k p_k (ln p_k - ln q_ids(n,k)).
+ *              Entries with a negative id or a logit of -inf are none; rows
+ *              without an entry do not count.  A token that is named twice is
+ *              two entries.
+ *   reduction: 0: loss (N) fp32, rows that do not count 0; 1: their mean over
+ *              the rows that count (NaN if none does); 2: their sum.
+ * A row that counts and names a token outside [0, V) has loss NaN and gradient
+ * NaN.  Rows that do not count are not read beyond their ids (and teacher): their
+ * hidden may hold anything, and their gradient is 0.
+ * msa_head_bwd takes the same arguments, state as msa_head_fwd left it (its pass
+ * only writes the header's scales there) and dloss, fp32: (N) for reduction 0,
+ * one value else.  dhidden (N, d) and dweight (V, d) contiguous, of type dtype;
+ * either may be null.  The gradient of the logits is formed in pieces of the
+ * vocabulary, rounded to dtype (fp32: to two fp16 terms, 22 bits) and multiplied
+ * with fp32 sums.
+ * state: msa_head_state_bytes, kept from forward to backward.  workspace:
+ * msa_head_workspace_bytes of the same arguments (backward 0 or 1; state,
+ * loss, dloss and workspace are not looked at), scratch of the call.
+ * 1 <= d <= 65536, V < 2^26, N <= 2^24, N K < 2^32, N d <= 2^38, V d <= 2^37, (N / 128)
+ * (V / 128) < 2^24.  No atomics on sums: equal calls give bitwise equal results.
+ */
+#define MSA_HEAD_MAX_K 256
+typedef struct {
+  const void* hidden;
+  int64_t hidden_ld;
+  const void* weight;
+  int64_t weight_ld;
+  const int64_t* ids;
+  int64_t ids_ld;
+  const void* teacher;
+  int64_t teacher_ld;
+  void* state;
+  uint64_t state_bytes;
+  float* loss;
+  const float* dloss;
+  void* dhidden;
+  void* dweight;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t N, d, V, K, dtype, teacher_dtype, reduction, ignore_index;
+  double temperature;
+} msa_head_args;
+size_t msa_head_state_bytes(int64_t N, int64_t K);
+size_t msa_head_workspace_bytes(const msa_head_args* args, int backward);
+int msa_head_fwd(const msa_head_args* args, void* stream);
+int msa_head_bwd(const msa_head_args* args, void* stream);
+
+/*
+ * Gated feed-forward: h = act(x Wg^T) * (x Wu^T), the first half of a gated
+ * block in one kernel.  No counterpart in the reference (its feed-forward is
+ * Linear, GELU, Linear, layers.py:52-58).
+ *   x        : (N, d) of type dtype, unit stride over d, x_ld from row to row.
+ *   gate, up : (F, d) of type dtype, likewise.
+ *   act      : 0: silu, g / (1 + exp(-g)); 1: gelu, g (1 + erf(g / sqrt 2)) / 2.
+ *   h        : (N, F) contiguous, of type dtype: act and product in fp32, rounded
+ *              once.
+ * msa_gated_bwd: dh (N, F), unit stride over F, dh_ld from row to row; dx (N, d),
+ * dgate, dup (F, d) contiguous, of type dtype.  dx may be null, or dgate and dup
+ * both.  The gradients of x Wg^T and x Wu^T are formed in pieces of the features,
+ * rounded to dtype behind a power of two (fp32: to two fp16 terms), sums are
+ * fp32.
+ * Operands are used in place under the conditions of msa_head_args' weight.
+ * workspace: msa_gated_workspace_bytes of the same arguments.  1 <= d <= 65536, 1 <= F
+ * <= 2^24, N <= 2^24, N d <= 2^38, F d <= 2^37, (N / 128) (F / 128) < 2^24.  Equal calls
+ * give bitwise equal results.
+ */
+typedef struct {
+  const void* x;
+  int64_t x_ld;
+  const void* gate;
+  int64_t gate_ld;
+  const void* up;
+  int64_t up_ld;
+  void* h;
+  const void* dh;
+  int64_t dh_ld;
+  void* dx;
+  void* dgate;
+  void* dup;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t N, d, F, dtype, act;
+} msa_gated_args;
+size_t msa_gated_workspace_bytes(const msa_gated_args* args, int backward);
+int msa_gated_fwd(const msa_gated_args* args, void* stream);
+int msa_gated_bwd(const msa_gated_args* args, void* stream);
+
 /* Kernel timing for measurement.  After msa_timer_arm(kernel, n) the next n
  * launches of that kernel (any entry point) each record a HIP event pair on
  * their stream around the launch; several kernels can be armed at once.

@@ -658,6 +658,127 @@ int msa_verify(const msa_verify_args* a, void* stream) {
   return hip_status(msa::launch_verify(c), "msa_verify launch");
 }
 
+// Shared checks of the wide products' sizes.
+static int check_wide(const char* what, int64_t N, int64_t d, int64_t rows, int64_t most, int64_t dtype) {
+  if (dtype != MSA_F32 && dtype != MSA_BF16 && dtype != MSA_F16)
+    return fail(MSA_ERR_INVALID, "dtype must be MSA_F32, MSA_BF16 or MSA_F16");
+  if (N < 0 || N > (int64_t)1 << 24) return fail(MSA_ERR_INVALID, "%s: 0 to 2^24 rows, got %lld", what, (long long)N);
+  if (d < 1 || d > 65536) return fail(MSA_ERR_INVALID, "%s: rows of 1 to 65536 columns, got %lld", what, (long long)d);
+  if (rows < 1 || rows > most)
+    return fail(MSA_ERR_INVALID, "%s: 1 to %lld weight rows, got %lld", what, (long long)most, (long long)rows);
+  // a grid has fewer than 2^32 threads along x: 2^24 blocks of 256
+  if (((N + 127) / 128) * ((rows + 127) / 128) >= (int64_t)1 << 24 || N * d > (int64_t)1 << 38 || rows * d > (int64_t)1 << 37)
+    return fail(MSA_ERR_INVALID, "%s: %lld rows by %lld weight rows of %lld columns are too many for a launch", what, (long long)N,
+                (long long)rows, (long long)d);
+  return MSA_OK;
+}
+
+static int check_rows(const char* name, const void* p, int64_t ld, int64_t cols, int64_t dtype) {
+  if (p == nullptr) return fail(MSA_ERR_INVALID, "%s is null", name);
+  if ((uintptr_t)p % (dtype == MSA_F32 ? 4 : 2) != 0) return fail(MSA_ERR_INVALID, "%s is not aligned to its type", name);
+  if (ld < 0 || ld > (int64_t)1 << 40) return fail(MSA_ERR_INVALID, "%s has a row stride of %lld", name, (long long)ld);
+  return MSA_OK;
+}
+
+static int head_call(const msa_head_args* a, msa::HeadCall* c) {
+  if (a == nullptr) return fail(MSA_ERR_INVALID, "args is null");
+  int rc = check_wide("head", a->N, a->d, a->V, ((int64_t)1 << 26) - 1, a->dtype);
+  if (rc != MSA_OK) return rc;
+  if (a->teacher == nullptr ? a->K != 1 : a->K < 1 || a->K > MSA_HEAD_MAX_K)
+    return fail(MSA_ERR_INVALID, "K must be 1 without a teacher and 1 to %d with one, got %lld", MSA_HEAD_MAX_K, (long long)a->K);
+  if (a->teacher != nullptr && a->teacher_dtype != MSA_F32 && a->teacher_dtype != MSA_BF16 && a->teacher_dtype != MSA_F16)
+    return fail(MSA_ERR_INVALID, "teacher_dtype must be MSA_F32, MSA_BF16 or MSA_F16");
+  if (a->N * a->K >= (int64_t)1 << 32) return fail(MSA_ERR_INVALID, "N * K = %lld exceeds 2^32 - 1", (long long)(a->N * a->K));
+  if (a->reduction < 0 || a->reduction > 2) return fail(MSA_ERR_INVALID, "reduction must be 0, 1 or 2");
+  if (!(a->temperature > 0.0) || !((float)a->temperature > 1e-30f) || !((float)a->temperature < 1e30f))
+    return fail(MSA_ERR_INVALID, "temperature must be positive and finite");
+  if (a->N > 0) {
+    if ((rc = check_rows("hidden", a->hidden, a->hidden_ld, a->d, a->dtype)) != MSA_OK) return rc;
+    if ((rc = check_rows("ids", a->ids, a->ids_ld, a->K, MSA_F32)) != MSA_OK) return rc;
+    if (a->teacher != nullptr && (rc = check_rows("teacher", a->teacher, a->teacher_ld, a->K, a->teacher_dtype)) != MSA_OK) return rc;
+  }
+  if ((rc = check_rows("weight", a->weight, a->weight_ld, a->d, a->dtype)) != MSA_OK) return rc;
+  c->N = a->N; c->V = a->V; c->d = (int)a->d; c->K = (int)a->K; c->dtype = (int)a->dtype; c->teacher_dtype = (int)a->teacher_dtype;
+  c->reduction = (int)a->reduction; c->temperature = (float)a->temperature; c->ignore_index = a->ignore_index;
+  c->x = a->hidden; c->x_ld = a->hidden_ld; c->w = a->weight; c->w_ld = a->weight_ld; c->ids = a->ids; c->ids_ld = a->ids_ld;
+  c->teacher = a->teacher; c->teacher_ld = a->teacher_ld; c->state = a->state; c->loss = a->loss; c->dloss = a->dloss;
+  c->dx = a->dhidden; c->dw = a->dweight; c->workspace = nullptr; c->stream = nullptr;
+  return MSA_OK;
+}
+
+size_t msa_head_state_bytes(int64_t N, int64_t K) {
+  return N < 0 || N > (int64_t)1 << 24 || K < 1 || K > MSA_HEAD_MAX_K ? 0 : msa::head_state_bytes(N, (int)K);
+}
+
+size_t msa_head_workspace_bytes(const msa_head_args* a, int backward) {
+  msa::HeadCall c;
+  return head_call(a, &c) != MSA_OK ? 0 : msa::head_workspace_bytes(c, backward != 0);
+}
+
+static int head_run(const msa_head_args* a, int backward, void* stream) {
+  msa::HeadCall c;
+  const int rc = head_call(a, &c);
+  if (rc != MSA_OK) return rc;
+  if (a->state == nullptr || a->state_bytes < msa::head_state_bytes(c.N, c.K))
+    return fail(MSA_ERR_WORKSPACE, "head state holds %zu bytes, %zu needed", (size_t)a->state_bytes, msa::head_state_bytes(c.N, c.K));
+  const size_t need = msa::head_workspace_bytes(c, backward);
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need))
+    return fail(MSA_ERR_WORKSPACE, "head workspace holds %zu bytes, %zu needed", (size_t)a->workspace_bytes, need);
+  if (!aligned16(a->state) || !aligned16(a->workspace)) return fail(MSA_ERR_INVALID, "state or workspace is not 16-byte aligned");
+  const bool empty = c.N == 0 && c.reduction == 0;  // a loss of no rows has no address
+  if (!empty && (backward ? a->dloss == nullptr : a->loss == nullptr)) return fail(MSA_ERR_INVALID, backward ? "dloss is null" : "loss is null");
+  if (!aligned16(a->dhidden) || !aligned16(a->dweight)) return fail(MSA_ERR_INVALID, "dhidden or dweight is not 16-byte aligned");
+  c.workspace = a->workspace;
+  c.stream = (hipStream_t)stream;
+  return hip_status(backward ? msa::launch_head_bwd(c) : msa::launch_head_fwd(c), backward ? "msa_head_bwd launch" : "msa_head_fwd launch");
+}
+
+int msa_head_fwd(const msa_head_args* a, void* stream) { return head_run(a, 0, stream); }
+int msa_head_bwd(const msa_head_args* a, void* stream) { return head_run(a, 1, stream); }
+
+static int gated_call(const msa_gated_args* a, int backward, msa::GatedCall* c) {
+  if (a == nullptr) return fail(MSA_ERR_INVALID, "args is null");
+  int rc = check_wide("gated", a->N, a->d, a->F, (int64_t)1 << 24, a->dtype);
+  if (rc != MSA_OK) return rc;
+  if (a->act != 0 && a->act != 1) return fail(MSA_ERR_INVALID, "act must be 0 (silu) or 1 (gelu)");
+  if (a->N > 0 && (rc = check_rows("x", a->x, a->x_ld, a->d, a->dtype)) != MSA_OK) return rc;
+  if ((rc = check_rows("gate", a->gate, a->gate_ld, a->d, a->dtype)) != MSA_OK) return rc;
+  if ((rc = check_rows("up", a->up, a->up_ld, a->d, a->dtype)) != MSA_OK) return rc;
+  if (backward) {
+    if (a->N > 0 && (rc = check_rows("dh", a->dh, a->dh_ld, a->F, a->dtype)) != MSA_OK) return rc;
+    if ((a->dgate == nullptr) != (a->dup == nullptr)) return fail(MSA_ERR_INVALID, "dgate and dup come together");
+  }
+  c->N = a->N; c->d = (int)a->d; c->F = (int)a->F; c->dtype = (int)a->dtype; c->act = (int)a->act;
+  c->x = a->x; c->x_ld = a->x_ld; c->w[0] = a->gate; c->w[1] = a->up; c->w_ld[0] = a->gate_ld; c->w_ld[1] = a->up_ld;
+  c->h = a->h; c->dh = a->dh; c->dh_ld = a->dh_ld; c->dx = a->dx; c->dw[0] = a->dgate; c->dw[1] = a->dup;
+  c->workspace = nullptr; c->stream = nullptr;
+  return MSA_OK;
+}
+
+size_t msa_gated_workspace_bytes(const msa_gated_args* a, int backward) {
+  msa::GatedCall c;
+  return gated_call(a, backward, &c) != MSA_OK ? 0 : msa::gated_workspace_bytes(c, backward != 0);
+}
+
+static int gated_run(const msa_gated_args* a, int backward, void* stream) {
+  msa::GatedCall c;
+  const int rc = gated_call(a, backward, &c);
+  if (rc != MSA_OK) return rc;
+  const size_t need = msa::gated_workspace_bytes(c, backward);
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need))
+    return fail(MSA_ERR_WORKSPACE, "gated workspace holds %zu bytes, %zu needed", (size_t)a->workspace_bytes, need);
+  if (!aligned16(a->workspace)) return fail(MSA_ERR_INVALID, "workspace is not 16-byte aligned");
+  if (!backward && a->N > 0 && a->h == nullptr) return fail(MSA_ERR_INVALID, "h is null");
+  if (!aligned16(a->h) || !aligned16(a->dx) || !aligned16(a->dgate) || !aligned16(a->dup))
+    return fail(MSA_ERR_INVALID, "h, dx, dgate or dup is not 16-byte aligned");
+  c.workspace = a->workspace;
+  c.stream = (hipStream_t)stream;
+  return hip_status(backward ? msa::launch_gated_bwd(c) : msa::launch_gated_fwd(c), backward ? "msa_gated_bwd launch" : "msa_gated_fwd launch");
+}
+
+int msa_gated_fwd(const msa_gated_args* a, void* stream) { return gated_run(a, 0, stream); }
+int msa_gated_bwd(const msa_gated_args* a, void* stream) { return gated_run(a, 1, stream); }
+
 int msa_selftest_mfma(const float* a16, const float* b16, float* out16, const float* a2, const float* b2,
                       float* out2, void* stream) {
   if (!a16 || !b16 || !out16 || !a2 || !b2 || !out2) return fail(MSA_ERR_INVALID, "null pointer");

@@ -1,0 +1,320 @@
+// Gated feed-forward: h = act(x Wg^T) * (x Wu^T) in one kernel, and its gradients.
+//   dg = dh u act'(g), du = dh act(g);  dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x
+// A tile's A rows alternate between the two weights by 64, so that a wave holds a feature's g and u of the same token
+// and the activation and the product happen in registers: h is written once, g and u never.  The backward pass forms g
+// and u again (keeping them rounded would cost 4 N F bytes and a rounding), in pieces of the features (256 MB of dg and
+// du, or 256 features), then takes the two products of msa_wide.hip.
+#include "msa_wide.h"
+
+namespace msa {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int64_t kPieceBytes = (int64_t)256 << 20;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// act(g) and act'(g): silu g / (1 + e^-g); gelu g (1 + erf(g / sqrt 2)) / 2, with erfc(x) = (a1 t + ... + a5 t^5) e^-x^2,
+// t = 1 / (1 + p x), x >= 0 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26: within 1.5e-7): no
+// branches, e^-x^2 also makes the slope, and the lower tail is not a difference.  slope of both kinds is c + what
+// multiplies g in c'.
+template <int ACT>
+__device__ inline void act_slope(float g, float& a, float& s) {
+  if constexpr (ACT == 0) {
+    const float c = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));
+    a = g * c;
+    s = fmaf(c, g - a, c);
+  } else {
+    const float e = __builtin_amdgcn_exp2f(-0.5f * kLog2e * g * g);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(g), 1.0f));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    const float tail = 0.5f * e * (p * t);  // erfc(|g| / sqrt 2) / 2
+    const float c = g < 0.0f ? tail : 1.0f - tail;
+    a = g * c;
+    s = fmaf(g * 0.3989422804014327f, e, c);
+  }
+}
+template <int ACT>
+__device__ inline float act_of(float g) {
+  float a, s;
+  act_slope<ACT>(g, a, s);
+  return a;
+}
+
+struct GatedArgs {
+  const char* x; int64_t x_ld; int64_t N, n_pad;
+  const char* w; int64_t w_ld, up;  // the gate's first row of the piece; from there to the other weight's
+  int cols;                         // features of the piece
+  MmSegs segs;
+  int ksteps, tiles_f, tiles_n;
+  const WideHdr* hdr;
+  void* h; int64_t h_ld; int vec;   // forward
+  const void* dh; int64_t dh_ld;    // backward: the piece's first column
+  char* g; int64_t C, plane, half;
+};
+
+template <typename T, int ACT, bool BWD>
+__global__ void __launch_bounds__(kThreads, 2) gated_kernel(GatedArgs a) {
+  using E = typename Wide<T>::E;
+  using Tl = MmTile<E, 256, 128, 2, 2, false, false, true, 3>;
+  __shared__ char smem[Tl::LDS];
+  LdsChar* lds = (LdsChar*)smem;
+  int tf, tn;
+  patch_order(xcd_order(blockIdx.x, gridDim.x), a.tiles_f, a.tiles_n, 8, tf, tn);
+  const int64_t n0 = (int64_t)tn * 128;
+  const int f0 = tf * 128;
+  typename Tl::Acc acc;
+  Tl::clear(acc);
+  const int fleft = a.cols - f0 < 128 ? a.cols - f0 : 128;
+  const int rows = (int)(a.N - n0 < 128 ? a.N - n0 : 128);
+  const typename Tl::Side A{a.w + f0 * a.w_ld, fleft, a.w_ld, 0, a.up};
+  const typename Tl::Side B{a.x + n0 * a.x_ld, rows, a.x_ld, 0, 0};
+  Tl::run(acc, lds, A, B, a.segs, 0, a.ksteps);
+  float f1 = 1.0f, f2 = 1.0f;
+  if constexpr (Wide<T>::P == 2) {
+    f1 = 1.0f / scale_x<T>(a.hdr);
+    f2 = 1.0f / scale_w<T>(a.hdr);
+  }
+  if constexpr (!BWD) {
+    T* out = (T*)a.h + n0 * a.h_ld + f0;
+    Tl::template store_rows<T, false, 2>(lds, out, a.h_ld, rows, fleft, a.vec != 0, [&](int i, int j, int q) {
+      return quad<T>([&](int e) { return act_of<ACT>(acc[i][j][4 * q + e] * f1 * f2) * (acc[i + 2][j][4 * q + e] * f1 * f2); });
+    });
+  } else {
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
+    const float sg = scale_g<T>(a.hdr, 1);
+    // dh goes through LDS in whole rows, 32 tokens of each wave at a time; places outside are zeros, so that dg and du
+    // are zeros there.
+    constexpr int PER = 16 / (int)sizeof(T), CPR = 128 / PER, ROW = 128 * (int)sizeof(T) + 16;
+    static_assert(64 * ROW <= Tl::LDS, "the staged rows of dh fit the tile's LDS");
+    typedef __attribute__((__vector_size__(16))) T TV;
+    typedef __attribute__((address_space(3))) TV LdsTV;
+    typedef typename Quad<T>::V T4;
+    typedef __attribute__((address_space(3))) T4 LdsT4;
+    const T* dh = (const T*)a.dh + n0 * a.dh_ld + f0;
+#pragma unroll
+    for (int j = 0; j < Tl::NB; ++j) {
+#pragma unroll 4
+      for (int c = (int)threadIdx.x; c < 64 * CPR; c += kThreads) {
+        const int row = c / CPR, f = (c - row * CPR) * PER, n = (row >> 5) * 64 + 32 * j + (row & 31);
+        TV v;
+        if (a.vec && n < rows && f + PER <= fleft) {
+          v = *reinterpret_cast<const TV*>(dh + n * a.dh_ld + f);
+        } else {
+#pragma unroll
+          for (int e = 0; e < PER; ++e) v[e] = n < rows && f + e < fleft ? dh[n * a.dh_ld + f + e] : (T)0.0f;
+        }
+        *reinterpret_cast<LdsTV*>(lds + row * ROW + f * (int)sizeof(T)) = v;
+      }
+      __syncthreads();
+      typename Quad<E>::V grads[2][Wide<T>::P][8];  // [dg, du][term], rounded as they are made
+      const LdsChar* at = lds + (wn * 32 + (lane & 31)) * ROW + (wm * 64 + 4 * (lane >> 5)) * (int)sizeof(T);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const T4 d = *reinterpret_cast<const LdsT4*>(at + 8 * q * (int)sizeof(T));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = q >> 2, r = 4 * (q & 3) + e;
+          const float g = acc[i][j][r] * f1 * f2, u = acc[i + 2][j][r] * f1 * f2;
+          float act, slope;
+          act_slope<ACT>(g, act, slope);
+          const float ds = (float)d[e] * sg;
+          const float v[2] = {ds * u * slope, ds * act};
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if constexpr (Wide<T>::P == 2) {
+              const Terms<float> t(v[half]);
+              grads[half][0][q][e] = t.h;
+              grads[half][1][q][e] = t.l;
+            } else {
+              grads[half][0][q][e] = (E)v[half];
+            }
+          }
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int t = 0; t < Wide<T>::P; ++t)
+          Tl::template store_tokens<E, false, 2>(lds, reinterpret_cast<E*>(a.g + half * a.half + t * a.plane) + n0 * a.C + f0, a.C,
+                                                 128, 128, true, j, [&](int i, int q) { return grads[half][t][4 * i + q]; });
+    }
+  }
+}
+
+__global__ void zero_kernel(uint16_t* p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) p[i] = 0;
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+int64_t es_of(int dtype) { return dtype == 0 ? 4 : 2; }
+bool direct(const GatedCall& c, const void* p, int64_t ld) {
+  return c.dtype != 0 && c.d % 32 == 0 && ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld * 2 * 256 < ((int64_t)1 << 32);
+}
+
+struct GatedPlan {
+  int64_t n_pad, dp, x_plane, w_plane, C, g_plane;
+  int planes, dx_split, dw_split;
+  char *x, *w, *g;
+  float *dx_part, *dw_part;
+  WideHdr* hdr;
+  size_t bytes;
+  GatedPlan(const GatedCall& c, int backward) {
+    planes = c.dtype == 0 ? 2 : 1;
+    n_pad = round_up(c.N > 0 ? c.N : 1, 128);
+    dp = wide_dp(c.d);
+    x_plane = round_up(n_pad * dp * 2, 256);
+    w_plane = round_up((int64_t)c.F * dp * 2, 256);
+    char* p = (char*)c.workspace;
+    size_t o = 0;
+    auto take = [&](int64_t bytes) { char* q = p + o; o += (size_t)round_up(bytes, 256); return q; };
+    hdr = (WideHdr*)take(256);
+    x = direct(c, c.x, c.x_ld) ? nullptr : take(planes * x_plane);
+    w = direct(c, c.w[0], c.w_ld[0]) && direct(c, c.w[1], c.w_ld[1]) && c.w_ld[0] == c.w_ld[1] ? nullptr : take(2 * planes * w_plane);
+    C = g_plane = 0;
+    dx_split = dw_split = 1;
+    g = nullptr; dx_part = dw_part = nullptr;
+    if (backward) {
+      C = kPieceBytes / (2 * planes * 2 * n_pad) / 256 * 256;
+      C = C < 256 ? 256 : C;
+      const int64_t all = round_up(c.F, 256);
+      C = C > all ? all : C;
+      const int64_t pieces = (all + C - 1) / C;
+      C = round_up((all + pieces - 1) / pieces, 256);
+      g_plane = round_up(n_pad * C * 2, 256);
+      g = take(2 * planes * g_plane);
+      wide_splits(c.N, c.d, C, 2, c.dx != nullptr, c.dw[0] != nullptr, &dx_split, &dw_split);
+      if (c.dx != nullptr) dx_part = (float*)take((int64_t)dx_split * n_pad * dp * 4);
+      if (c.dw[0] != nullptr && dw_split > 1) dw_part = (float*)take((int64_t)dw_split * 2 * C * dp * 4);
+    }
+    bytes = o;
+  }
+};
+
+#define GATED_TRY(call) do { const hipError_t e_ = (call); if (e_ != hipSuccess) return e_; } while (0)
+
+struct GatedOperands { const char *x, *w[2]; int64_t x_ld, w_ld; int x_rows; MmSegs segs; };
+
+hipError_t operands(const GatedCall& c, const GatedPlan& p, int backward, GatedOperands* o) {
+  RowsCopy x{c.x, c.x_ld, c.N, c.d, c.dtype, p.x, p.x_plane, nullptr, p.hdr, 0};
+  RowsCopy w[2];
+  for (int i = 0; i < 2; ++i)
+    w[i] = RowsCopy{c.w[i], c.w_ld[i], c.F, c.d, c.dtype, p.w + (p.w == nullptr ? 0 : i * p.planes * p.w_plane), p.w_plane, nullptr, p.hdr, 1};
+  if (p.planes == 2 || (backward && c.dtype == 2)) {  // scales of the operands, and of dg and du
+    GATED_TRY(launch_hdr_clear(p.hdr, c.stream));
+    GATED_TRY(launch_rows_max(x, backward, c.stream));
+    GATED_TRY(launch_rows_max(w[0], backward, c.stream));
+    GATED_TRY(launch_rows_max(w[1], backward, c.stream));
+    if (backward) {
+      const RowsCopy dh{c.dh, c.dh_ld, c.N, c.F, c.dtype, nullptr, 0, nullptr, p.hdr, 2};
+      GATED_TRY(launch_rows_max(dh, 0, c.stream));
+    }
+  }
+  if (p.x != nullptr) GATED_TRY(launch_rows_copy(x, c.stream));
+  if (p.w != nullptr) {
+    GATED_TRY(launch_rows_copy(w[0], c.stream));
+    GATED_TRY(launch_rows_copy(w[1], c.stream));
+  }
+  o->x = p.x != nullptr ? p.x : (const char*)c.x;
+  o->x_ld = p.x != nullptr ? p.dp * 2 : c.x_ld * 2;
+  o->x_rows = (int)c.N;
+  o->w[0] = p.w != nullptr ? p.w : (const char*)c.w[0];
+  o->w[1] = p.w != nullptr ? p.w + p.planes * p.w_plane : (const char*)c.w[1];
+  o->w_ld = p.w != nullptr ? p.dp * 2 : c.w_ld[0] * 2;
+  o->segs = MmSegs{};
+  if (p.planes == 2) {
+    o->segs.b[0] = p.x_plane;
+    o->segs.a[1] = p.w_plane;
+    o->segs.n = 3;
+    o->segs.low = 2;
+  } else {
+    o->segs.n = 1;
+  }
+  return hipSuccess;
+}
+
+GatedArgs args_of(const GatedCall& c, const GatedPlan& p, const GatedOperands& o, int64_t f0, int cols) {
+  GatedArgs a = {};
+  a.x = o.x; a.x_ld = o.x_ld; a.N = c.N; a.n_pad = p.n_pad;
+  a.w = o.w[0] + f0 * o.w_ld; a.w_ld = o.w_ld; a.up = o.w[1] - o.w[0]; a.cols = cols;
+  a.segs = o.segs; a.ksteps = (int)(p.dp / 32); a.tiles_f = (cols + 127) / 128; a.tiles_n = (int)(p.n_pad / 128);
+  a.hdr = p.hdr;
+  return a;
+}
+
+template <typename T, bool BWD>
+hipError_t launch(const GatedArgs& a, int act, hipStream_t s) {
+  auto* k = act == 0 ? gated_kernel<T, 0, BWD> : gated_kernel<T, 1, BWD>;
+  hipLaunchKernelGGL(k, dim3((unsigned)((int64_t)a.tiles_f * a.tiles_n)), dim3(kThreads), 0, s, a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t gated_fwd(const GatedCall& c) {
+  if (c.N == 0) return hipSuccess;
+  const GatedPlan p(c, 0);
+  GatedOperands o;
+  GATED_TRY(operands(c, p, 0, &o));
+  GatedArgs a = args_of(c, p, o, 0, c.F);
+  a.h = c.h; a.h_ld = c.F;
+  a.vec = (int64_t)c.F * sizeof(T) % 16 == 0 && ((uintptr_t)c.h & 15) == 0;
+  return launch<T, false>(a, c.act, c.stream);
+}
+
+template <typename T>
+hipError_t gated_bwd(const GatedCall& c) {
+  if (c.N == 0) {
+    for (int i = 0; i < 2; ++i)
+      if (c.dw[i] != nullptr) {
+        hipLaunchKernelGGL(zero_kernel, dim3(1024), dim3(kThreads), 0, c.stream, (uint16_t*)c.dw[i], (int64_t)c.F * c.d * es_of(c.dtype) / 2);
+        GATED_TRY(hipGetLastError());
+      }
+    return hipSuccess;
+  }
+  const GatedPlan p(c, 1);
+  GatedOperands o;
+  GATED_TRY(operands(c, p, 1, &o));
+  for (int64_t f0 = 0; f0 < c.F; f0 += p.C) {
+    const int cols = (int)(c.F - f0 < p.C ? c.F - f0 : p.C);
+    GatedArgs a = args_of(c, p, o, f0, cols);
+    a.dh = (const T*)c.dh + f0; a.dh_ld = c.dh_ld;
+    a.vec = c.dh_ld * sizeof(T) % 16 == 0 && ((uintptr_t)c.dh & 15) == 0;
+    a.g = p.g; a.C = p.C; a.plane = p.g_plane; a.half = p.planes * p.g_plane;
+    GATED_TRY((launch<T, true>(a, c.act, c.stream)));
+    WideProducts q = {};
+    q.dtype = c.dtype; q.gated = 1; q.N = c.N; q.n_pad = p.n_pad; q.d = c.d; q.dp = p.dp; q.halves = 2; q.cols = cols; q.C = p.C;
+    q.x = o.x; q.x_ld = o.x_ld; q.x_plane = p.x_plane; q.x_rows = o.x_rows;
+    for (int i = 0; i < 2; ++i) {
+      q.w[i] = o.w[i] + f0 * o.w_ld;
+      q.dw[i] = c.dw[i] == nullptr ? nullptr : (char*)c.dw[i] + f0 * c.d * es_of(c.dtype);
+    }
+    q.w_ld = o.w_ld; q.w_plane = p.w_plane; q.w_rows = (int)(c.F - f0);
+    q.g = p.g; q.g_plane = p.g_plane; q.g_half = p.planes * p.g_plane;
+    q.dx_part = p.dx_part; q.dx_add = f0 > 0; q.dw_part = p.dw_part;
+    q.dx_split = p.dx_split; q.dw_split = p.dw_split; q.hdr = p.hdr; q.use_live = 0;
+    GATED_TRY(launch_wide_products(q, c.stream));
+  }
+  if (c.dx != nullptr) {
+    const WideFinish f{c.dtype, 1, c.N, p.n_pad, c.d, p.dp, p.dx_split, p.dx_part, nullptr, p.hdr, c.dx};
+    GATED_TRY(launch_wide_finish(f, c.stream));
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+size_t gated_workspace_bytes(const GatedCall& c, int backward) { return GatedPlan(c, backward).bytes; }
+
+hipError_t launch_gated_fwd(const GatedCall& c) {
+  return c.dtype == 0 ? gated_fwd<float>(c) : c.dtype == 1 ? gated_fwd<bf16>(c) : gated_fwd<f16>(c);
+}
+hipError_t launch_gated_bwd(const GatedCall& c) {
+  return c.dtype == 0 ? gated_bwd<float>(c) : c.dtype == 1 ? gated_bwd<bf16>(c) : gated_bwd<f16>(c);
+}
+
+}  // namespace msa

@@ -1,0 +1,654 @@
+// Losses of rows against a vocabulary without its logits: softmax cross entropy and the divergence from a teacher's
+// largest logits.  With z2_nv = log2(e) x_n . W_v / T and lse2_n = log2 sum_v 2^z2_nv:
+//   cross entropy  L_n = ln2 (lse2_n - z2_n,y)
+//   distillation   L_n = T^2 (sum_k p_k ln p_k - ln2 sum_k p_k (z2_n,id(k) - lse2_n)),  p = softmax of the row's entries
+//   both           dL_n/dz_nv = T (2^(z2_nv - lse2_n) - sum_{k: id(k) = v} p_k)        (z: logits before 1/T)
+// Forward: one product over all of the vocabulary whose tiles leave each row's maximum and sum; a row's own logits are
+// K dot products.  Backward, in pieces of the vocabulary: the product again, now with lse2 known, gives the piece's
+// gradient G in the operand type (256 MB at most, or 256 columns); then dx += G W and dW = G^T x (msa_wide.hip).
+// Rows that do not count are taken out before the products: their x may hold anything.
+#include "msa_wide.h"
+
+namespace msa {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kHeadMaxK = 256;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int64_t kPieceBytes = (int64_t)256 << 20;
+
+// What the backward pass needs: header, pos[N] (row of the operand, -1: does not count), lse2[N rows of the operand],
+// t[N][K]: 2^(z2 - lse2) - p of the targets (p summed over equal ids).
+struct HeadState {
+  WideHdr* hdr;
+  int* pos;
+  float* lse2;
+  float* t;
+  size_t bytes;
+  HeadState(void* p, int64_t N, int K) {
+    char* c = (char*)p;
+    size_t o = 256;
+    hdr = (WideHdr*)c;
+    pos = (int*)(c + o); o += (size_t)round_up(N * 4, 256);
+    lse2 = (float*)(c + o); o += (size_t)round_up(round_up(N, 128) * 4, 256);
+    t = (float*)(c + o); o += (size_t)round_up(N * K * 4, 256);
+    bytes = o;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Which rows count
+// ---------------------------------------------------------------------------
+// One block: pos[n] = how many rows before n count, or -1.  A thread takes neighbouring rows twice: to count and to
+// number them.  32768 rows take about 10 us beside products of milliseconds.
+template <typename Fn>
+__device__ inline int number_rows(int64_t N, int* pos, Fn counts) {
+  __shared__ int sums[16];
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t per = (N + 1023) / 1024, from = tid * per, to = from + per < N ? from + per : N;
+  int c = 0;
+  for (int64_t n = from; n < to; ++n) c += counts(n) ? 1 : 0;
+  int incl = c;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 63) sums[wave] = incl;
+  __syncthreads();
+  int before = 0, total = 0;
+  for (int w = 0; w < 16; ++w) {
+    if (w < wave) before += sums[w];
+    total += sums[w];
+  }
+  int at = before + incl - c;
+  for (int64_t n = from; n < to; ++n) pos[n] = counts(n) ? at++ : -1;
+  return total;
+}
+
+__global__ void __launch_bounds__(1024) plan_kernel(const int64_t* ids, int64_t ids_ld, int64_t ignore,
+                                                    const uint8_t* live, int64_t N, int* pos, WideHdr* hdr) {
+  const int total = live != nullptr ? number_rows(N, pos, [&](int64_t n) { return live[n] != 0; })
+                                    : number_rows(N, pos, [&](int64_t n) { return ids[n * ids_ld] != ignore; });
+  if (threadIdx.x == 0) {
+    *hdr = WideHdr{};
+    hdr->live = total;
+    hdr->cmax = 1.0f;
+  }
+}
+
+// A teacher's record of a row: entries with an id >= 0 and a logit above -inf; p = their softmax at 1/T.  A wave per
+// row.  tp[n][k] = (p, p summed over the row's entries of the same id); ent[n] = sum p ln p.  NaN logits, or +inf, give NaN.
+template <typename L>
+__global__ void __launch_bounds__(kThreads) teacher_kernel(const L* logits, int64_t lld, const int64_t* ids,
+                                                           int64_t ids_ld, int64_t N, int K, float inv_t, float2* tp,
+                                                           float* ent, uint8_t* live) {
+  constexpr int R = kHeadMaxK / 64;
+  __shared__ int64_t sid[4][kHeadMaxK];
+  __shared__ float sp[4][kHeadMaxK];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  const int64_t n = (int64_t)blockIdx.x * 4 + wave;
+  if (n < N) {
+    float t[R];
+    int64_t id[R];
+    float mx = -INFINITY;
+    bool any = false;
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const int k = q * 64 + lane;
+      id[q] = k < K ? ids[n * ids_ld + k] : -1;
+      t[q] = id[q] >= 0 ? to_f(logits[n * lld + k]) * inv_t : -INFINITY;
+      any = any || !(t[q] == -INFINITY);
+      mx = fmaxf(mx, t[q]);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    any = __ballot(any) != 0ull;
+    float sum = 0.0f;
+#pragma unroll
+    for (int q = 0; q < R; ++q) sum += t[q] == -INFINITY ? 0.0f : exp2f((t[q] - mx) * kLog2e);
+    sum = wave_sum(sum);
+    const float ls = logf(sum);
+    float h = 0.0f;
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const int k = q * 64 + lane;
+      const float lp = t[q] - mx - ls, p = t[q] == -INFINITY ? 0.0f : expf(lp);
+      h += p > 0.0f ? p * lp : p;  // 0 ln 0 = 0; NaN stays
+      t[q] = p;
+      sid[wave][k] = id[q];
+      sp[wave][k] = p;
+    }
+    h = wave_sum(h);
+    wave_lds_sync();
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const int k = q * 64 + lane;
+      if (q * 64 >= K) break;
+      float all = 0.0f;
+      for (int o = 0; o < K; ++o) all += sid[wave][o] == id[q] ? sp[wave][o] : 0.0f;
+      if (k < K) tp[n * K + k] = float2{t[q], all};
+    }
+    if (lane == 0) {
+      ent[n] = h;
+      live[n] = any ? 1 : 0;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The product's maxima and sums
+// ---------------------------------------------------------------------------
+struct StatsArgs {
+  const char* x; int64_t x_ld; int64_t n_pad;
+  const char* w; int64_t w_ld; int64_t V;
+  MmSegs segs;
+  int ksteps, tiles_v, tiles_n;
+  float to_log2;  // log2(e) / T
+  const WideHdr* hdr;
+  float2* part;  // [tiles_v][n_pad]
+};
+
+// Features from `left` on become v: only the last tile along the vocabulary pays for the comparisons.
+template <typename Tl>
+__device__ inline void mask_features(typename Tl::Acc& acc, int left, int wm, int lane, float v) {
+#pragma unroll
+  for (int i = 0; i < Tl::MB; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const bool out = Tl::m_of(wm, lane, i, r >> 2) + (r & 3) >= left;
+#pragma unroll
+      for (int j = 0; j < Tl::NB; ++j) acc[i][j][r] = out ? v : acc[i][j][r];
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) stats_kernel(StatsArgs a) {
+  using E = typename Wide<T>::E;
+  using Tl = MmTile<E, 256, 128, 2, 2, false, false, false, 3>;
+  __shared__ char smem[Tl::LDS];
+  LdsChar* lds = (LdsChar*)smem;
+  int tv, tn;
+  patch_order(xcd_order(blockIdx.x, gridDim.x), a.tiles_v, a.tiles_n, 8, tv, tn);
+  const int64_t v0 = (int64_t)tv * 256, n0 = (int64_t)tn * 128;
+  if (n0 >= a.hdr->live) return;
+  typename Tl::Acc acc;
+  Tl::clear(acc);
+  const int vleft = (int)(a.V - v0 < 256 ? a.V - v0 : 256);
+  const typename Tl::Side A{a.w + v0 * a.w_ld, vleft, a.w_ld, 0, 0};
+  const typename Tl::Side B{a.x + n0 * a.x_ld, (int)(a.n_pad - n0 < 128 ? a.n_pad - n0 : 128), a.x_ld, 0, 0};
+  Tl::run(acc, lds, A, B, a.segs, 0, a.ksteps);
+  const float f = a.to_log2 / scale_x<T>(a.hdr) / scale_w<T>(a.hdr);
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
+  __shared__ float2 red[2][128];
+  if (vleft < 256) mask_features<Tl>(acc, vleft, wm, lane, -INFINITY);
+#pragma unroll
+  for (int j = 0; j < Tl::NB; ++j) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < Tl::MB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        acc[i][j][r] *= f;
+        mx = fmaxf(mx, acc[i][j][r]);
+      }
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const float at = mx == -INFINITY ? 0.0f : mx;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < Tl::MB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(acc[i][j][r] - at);
+    s += __shfl_xor(s, 32);
+    if (lane < 32) red[wm][Tl::n_of(wn, lane, j)] = float2{mx, s};
+  }
+  __syncthreads();
+  if (threadIdx.x < 128) {
+    const float2 p = red[0][threadIdx.x], q = red[1][threadIdx.x];
+    const float m = fmaxf(p.x, q.x), at = m == -INFINITY ? 0.0f : m;
+    a.part[(int64_t)tv * a.n_pad + n0 + threadIdx.x] =
+        float2{m, p.y * __builtin_amdgcn_exp2f(p.x - at) + q.y * __builtin_amdgcn_exp2f(q.x - at)};
+  }
+}
+
+// ---------------------------------------------------------------------------
+// A row's sum over the tiles, its targets' logits and its loss.  A block takes 8 rows: first 32 groups of 8 lanes
+// share the tiles, then a wave takes a target at a time (a dot product of d terms).
+// ---------------------------------------------------------------------------
+struct RowsArgs {
+  const void* x; int64_t x_ld;
+  const void* w; int64_t w_ld;
+  const int64_t* ids; int64_t ids_ld;
+  const float2* tp;  // null: cross entropy
+  const float* ent;
+  const float2* part; int64_t part_ld; int tiles;
+  int64_t N, V; int d, K, vec;
+  float temperature;
+  const int* pos;
+  float* lse2; float* t; float* loss;
+};
+
+// x . w in one order of the sum however the rows are aligned.
+template <typename T>
+__device__ inline float row_dot_of(const T* x, const T* w, int d, int vec, int lane) {
+  constexpr int PER = 16 / (int)sizeof(T);
+  typedef __attribute__((__vector_size__(16))) T TV;
+  float s = 0.0f;
+  for (int c = lane * PER; c < d; c += 64 * PER) {
+    TV a, b;
+    if (vec) {
+      a = *reinterpret_cast<const TV*>(x + c);
+      b = *reinterpret_cast<const TV*>(w + c);
+    } else {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const int at = c + e < d ? c + e : d - 1;
+        a[e] = c + e < d ? x[at] : (T)0.0f;
+        b[e] = c + e < d ? w[at] : (T)0.0f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < PER; ++e) s = fmaf((float)a[e], (float)b[e], s);
+  }
+  return wave_sum(s);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
+  __shared__ float2 red[32][8];
+  __shared__ float2 stat[8];     // the row's maximum and log2 of its sum
+  __shared__ float part_loss[8][4];
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t first = (int64_t)blockIdx.x * 8;
+  {
+    const int r = tid & 7, g = tid >> 3;
+    const int at = first + r < a.N ? a.pos[first + r] : -1;
+    float m = -INFINITY, s = 0.0f;
+    if (at >= 0)
+      for (int t = g; t < a.tiles; t += 32) {
+        const float2 p = a.part[(int64_t)t * a.part_ld + at];
+        const float mn = fmaxf(m, p.x), b = mn == -INFINITY ? 0.0f : mn;
+        s = s * __builtin_amdgcn_exp2f(m - b) + p.y * __builtin_amdgcn_exp2f(p.x - b);
+        m = mn;
+      }
+    red[g][r] = float2{m, s};
+    __syncthreads();
+    if (tid < 8) {
+      float mm = -INFINITY, ss = 0.0f;
+      for (int q = 0; q < 32; ++q) mm = fmaxf(mm, red[q][tid].x);
+      const float b = mm == -INFINITY ? 0.0f : mm;
+      for (int q = 0; q < 32; ++q) ss += red[q][tid].y * __builtin_amdgcn_exp2f(red[q][tid].x - b);
+      stat[tid] = float2{mm, log2f(ss)};
+    }
+    __syncthreads();
+  }
+  const float to_log2 = kLog2e / a.temperature;
+  for (int r = 0; r < 8; ++r) {
+    const int64_t n = first + r;
+    const int at = n < a.N ? a.pos[n] : -1;
+    float sum = 0.0f;
+    if (at >= 0) {
+      const float2 st = stat[r];
+      for (int k = wave; k < a.K; k += 4) {
+        const int64_t id = a.ids[n * a.ids_ld + k];
+        const float2 p = a.tp == nullptr ? float2{1.0f, 1.0f} : a.tp[n * a.K + k];
+        const bool none = a.tp != nullptr && id < 0;
+        float t = 0.0f, part = 0.0f;
+        if (!none) {
+          if (id >= 0 && id < a.V) {
+            const float z2 = to_log2 * row_dot_of((const T*)a.x + n * a.x_ld, (const T*)a.w + id * a.w_ld, a.d, a.vec, lane);
+            const float away = (st.x - z2) + st.y;  // lse2 - z2
+            t = __builtin_amdgcn_exp2f(-away) - p.y;
+            part = p.x > 0.0f || !(p.x == p.x) ? p.x * away : 0.0f;
+          } else {
+            t = part = NAN;
+          }
+        }
+        sum += part;
+        if (lane == 0) a.t[n * a.K + k] = t;
+      }
+    }
+    if (lane == 0) part_loss[r][wave] = sum;
+  }
+  __syncthreads();
+  if (tid < 8) {
+    const int64_t n = first + tid;
+    if (n < a.N) {
+      const int at = a.pos[n];
+      const float away = (part_loss[tid][0] + part_loss[tid][1]) + (part_loss[tid][2] + part_loss[tid][3]);
+      float loss = kLn2 * away;
+      if (a.tp != nullptr && at >= 0) loss = a.temperature * a.temperature * (loss + a.ent[n]);
+      a.loss[n] = at >= 0 ? loss : 0.0f;
+      // a target outside the vocabulary makes the row NaN, its gradient too
+      if (at >= 0) a.lse2[at] = away == away ? stat[tid].x + stat[tid].y : NAN;
+    }
+  }
+}
+
+// One block: the mean or the sum of the rows' losses, in 64 bits.
+__global__ void __launch_bounds__(1024) total_kernel(const float* rows, int64_t N, const WideHdr* hdr, int mean, float* out) {
+  __shared__ double sums[1024];
+  double s = 0.0;
+  for (int64_t n = threadIdx.x; n < N; n += 1024) s += (double)rows[n];
+  sums[threadIdx.x] = s;
+  __syncthreads();
+  for (int o = 512; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) sums[threadIdx.x] += sums[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) out[0] = (float)(mean ? sums[0] / (double)hdr->live : sums[0]);
+}
+
+// ---------------------------------------------------------------------------
+// Backward
+// ---------------------------------------------------------------------------
+// One block: coefficients of the rows of the operand, as g_n / cmax; zero behind the last row up to the next multiple
+// of 128.  A mean or a sum has one coefficient: cmax is it and every row's is 1, so that G is rounded from the
+// probabilities themselves.  Else cmax is a power of two, at least the largest finite |g_n|.
+__global__ void __launch_bounds__(1024) coef_kernel(const float* dloss, int reduction, float factor, int64_t N, int64_t n_pad,
+                                                    const int* pos, WideHdr* hdr, float* coef) {
+  const int tid = (int)threadIdx.x;
+  const int live = hdr->live;
+  if (reduction != 0) {
+    if (tid == 0) hdr->cmax = reduction == 1 ? dloss[0] * factor / (float)live : dloss[0] * factor;
+    for (int64_t i = tid; i < n_pad; i += 1024) coef[i] = i < live ? 1.0f : 0.0f;
+    return;
+  }
+  __shared__ float red[16];
+  float mx = 0.0f;
+  for (int64_t n = tid; n < N; n += 1024) {
+    const float g = pos[n] >= 0 ? fabsf(dloss[n] * factor) : 0.0f;
+    if (g < INFINITY) mx = fmaxf(mx, g);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+  if ((tid & 63) == 0) red[tid >> 6] = mx;
+  __syncthreads();
+  for (int w = 0; w < 16; ++w) mx = fmaxf(mx, red[w]);
+  const float inv = pow2_to(mx, 0);  // mx inv in [0.5, 1)
+  if (tid == 0) hdr->cmax = 1.0f / inv;
+  for (int64_t n = tid; n < N; n += 1024)
+    if (pos[n] >= 0) coef[pos[n]] = dloss[n] * factor * inv;
+  for (int64_t i = live + tid; i < n_pad; i += 1024) coef[i] = 0.0f;
+}
+
+struct GradArgs {
+  const char* x; int64_t x_ld; int64_t n_pad;
+  const char* w; int64_t w_ld;  // the piece's first row
+  int cols;                     // its rows
+  MmSegs segs;
+  int ksteps, tiles_v, tiles_n;
+  float to_log2;
+  const WideHdr* hdr;
+  const float* lse2; const float* coef;
+  char* g; int64_t C, plane;
+};
+
+// G of one tile: c_n 2^(z2 - lse2), without the targets, which scatter_kernel puts in their place.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
+  using E = typename Wide<T>::E;
+  using Tl = MmTile<E, 256, 128, 2, 2, false, false, false, 3>;
+  __shared__ char smem[Tl::LDS];
+  LdsChar* lds = (LdsChar*)smem;
+  int tv, tn;
+  patch_order(xcd_order(blockIdx.x, gridDim.x), a.tiles_v, a.tiles_n, 8, tv, tn);
+  const int64_t v0 = (int64_t)tv * 256, n0 = (int64_t)tn * 128;
+  const int64_t live = a.hdr->live;
+  if (n0 >= live) return;
+  typename Tl::Acc acc;
+  Tl::clear(acc);
+  const int vleft = (int)(a.cols - v0 < 256 ? a.cols - v0 : 256);
+  const typename Tl::Side A{a.w + v0 * a.w_ld, vleft, a.w_ld, 0, 0};
+  const typename Tl::Side B{a.x + n0 * a.x_ld, (int)(a.n_pad - n0 < 128 ? a.n_pad - n0 : 128), a.x_ld, 0, 0};
+  Tl::run(acc, lds, A, B, a.segs, 0, a.ksteps);
+  const float f = a.to_log2 / scale_x<T>(a.hdr) / scale_w<T>(a.hdr), sg = scale_g<T>(a.hdr, 0);
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
+  if (vleft < 256) mask_features<Tl>(acc, vleft, wm, lane, -INFINITY);
+#pragma unroll
+  for (int j = 0; j < Tl::NB; ++j) {
+    const int64_t n = n0 + Tl::n_of(wn, lane, j);
+    const bool ok = n < live;
+    // a row behind the last one has an operand of zeros, lse2 of infinity and so a gradient of zeros
+    const float l = ok ? a.lse2[n] : INFINITY, c = ok ? a.coef[n] * sg : 0.0f;
+#pragma unroll
+    for (int i = 0; i < Tl::MB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        acc[i][j][r] = c * __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], f, -l));
+      }
+  }
+  E* out = reinterpret_cast<E*>(a.g) + n0 * a.C + v0;
+  if constexpr (Wide<T>::P == 2) {
+    Tl::template store_rows<E, false>(lds, out, a.C, 128, 256, true, [&](int i, int j, int g) {
+      return quad<E>([&](int e) { return (float)Terms<float>(acc[i][j][4 * g + e]).h; });
+    });
+    Tl::renew(acc);
+    Tl::template store_rows<E, false>(lds, reinterpret_cast<E*>(reinterpret_cast<char*>(out) + a.plane), a.C, 128, 256, true,
+                                      [&](int i, int j, int g) {
+                                        return quad<E>([&](int e) { return (float)Terms<float>(acc[i][j][4 * g + e]).l; });
+                                      });
+  } else {
+    Tl::template store_rows<E, false>(lds, out, a.C, 128, 256, true, [&](int i, int j, int g) {
+      return quad<E>([&](int e) { return acc[i][j][4 * g + e]; });
+    });
+  }
+}
+
+// The targets' entries of a piece's G.  Entries of equal ids write equal values.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) scatter_kernel(const int64_t* ids, int64_t ids_ld, int64_t N, int K, const int* pos,
+                                                           const float* t, const float* coef, const WideHdr* hdr, int64_t v0,
+                                                           int cols, char* g, int64_t C, int64_t plane) {
+  using E = typename Wide<T>::E;
+  const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t n = e / K;
+  if (n >= N) return;
+  const int at = pos[n];
+  const int64_t v = ids[n * ids_ld + (e - n * K)] - v0;
+  if (at < 0 || v < 0 || v >= cols) return;
+  const float x = t[e] * coef[at] * scale_g<T>(hdr, 0);
+  E* p = reinterpret_cast<E*>(g) + (int64_t)at * C + v;
+  if constexpr (Wide<T>::P == 2) {
+    const Terms<float> w(x);
+    *p = w.h;
+    *reinterpret_cast<E*>(reinterpret_cast<char*>(p) + plane) = w.l;
+  } else {
+    *p = (E)x;
+  }
+}
+
+__global__ void zero_kernel(uint16_t* p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) p[i] = 0;
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+int64_t es_of(int dtype) { return dtype == 0 ? 4 : 2; }
+bool w_direct(const HeadCall& c) {
+  return c.dtype != 0 && c.d % 32 == 0 && ((uintptr_t)c.w & 15) == 0 && c.w_ld % 8 == 0 && c.w_ld * 2 * 256 < ((int64_t)1 << 32);
+}
+bool rows_vec(const HeadCall& c) {
+  const int64_t per = 16 / es_of(c.dtype);
+  return c.d % per == 0 && c.x_ld % per == 0 && c.w_ld % per == 0 && (((uintptr_t)c.x | (uintptr_t)c.w) & 15) == 0;
+}
+
+struct HeadPlan {
+  int64_t n_pad, dp, x_plane, w_plane, C, g_plane;
+  int planes, tiles_n, tiles_v, dx_split, dw_split;
+  bool distill;
+  char *x, *w, *g;
+  float2 *part, *tp;
+  float *ent, *rows, *coef, *dx_part, *dw_part;
+  uint8_t* live;
+  size_t bytes;
+  HeadPlan(const HeadCall& c, int backward) {
+    distill = c.teacher != nullptr;
+    planes = c.dtype == 0 ? 2 : 1;
+    n_pad = round_up(c.N > 0 ? c.N : 1, 128);
+    dp = wide_dp(c.d);
+    x_plane = round_up(n_pad * dp * 2, 256);
+    w_plane = round_up(c.V * dp * 2, 256);
+    tiles_n = (int)(n_pad / 128);
+    tiles_v = (int)((c.V + 255) / 256);
+    char* p = (char*)c.workspace;
+    size_t o = 0;
+    auto take = [&](int64_t bytes) { char* q = p + o; o += (size_t)round_up(bytes, 256); return q; };
+    x = take(planes * x_plane);
+    w = w_direct(c) ? nullptr : take(planes * w_plane);
+    C = g_plane = 0;
+    dx_split = dw_split = 1;
+    part = tp = nullptr; ent = rows = coef = dx_part = dw_part = nullptr; live = nullptr; g = nullptr;
+    if (!backward) {
+      part = (float2*)take((int64_t)tiles_v * n_pad * 8);
+      if (c.reduction != 0) rows = (float*)take(c.N * 4);
+      if (distill) {
+        tp = (float2*)take(c.N * c.K * 8);
+        ent = (float*)take(c.N * 4);
+        live = (uint8_t*)take(c.N);
+      }
+    } else {
+      C = kPieceBytes / (planes * 2 * n_pad) / 256 * 256;
+      C = C < 256 ? 256 : C;
+      const int64_t all = round_up(c.V, 256);
+      C = C > all ? all : C;
+      const int64_t pieces = (all + C - 1) / C;  // of equal size
+      C = round_up((all + pieces - 1) / pieces, 256);
+      g_plane = round_up(n_pad * C * 2, 256);
+      g = take(planes * g_plane);
+      coef = (float*)take(n_pad * 4);
+      wide_splits(c.N, c.d, C, 1, c.dx != nullptr, c.dw != nullptr, &dx_split, &dw_split);
+      if (c.dx != nullptr) dx_part = (float*)take((int64_t)dx_split * n_pad * dp * 4);
+      if (c.dw != nullptr && dw_split > 1) dw_part = (float*)take((int64_t)dw_split * C * dp * 4);
+    }
+    bytes = o;
+  }
+  MmSegs logits() const {
+    MmSegs s = {};
+    if (planes == 2) {
+      s.b[0] = x_plane;
+      s.a[1] = w_plane;
+      s.n = 3;
+      s.low = 2;
+    } else {
+      s.n = 1;
+    }
+    return s;
+  }
+};
+
+#define HEAD_TRY(call) do { const hipError_t e_ = (call); if (e_ != hipSuccess) return e_; } while (0)
+
+// hidden's counting rows and the weight as operands
+template <typename T>
+hipError_t operands(const HeadCall& c, const HeadPlan& p, const HeadState& st) {
+  RowsCopy x{c.x, c.x_ld, c.N, c.d, c.dtype, p.x, p.x_plane, st.pos, st.hdr, 0};
+  RowsCopy w{c.w, c.w_ld, c.V, c.d, c.dtype, p.w, p.w_plane, nullptr, st.hdr, 1};
+  if (p.planes == 2) {
+    HEAD_TRY(launch_rows_max(x, 0, c.stream));
+    HEAD_TRY(launch_rows_max(w, 0, c.stream));
+  }
+  HEAD_TRY(launch_rows_copy(x, c.stream));
+  if (p.w != nullptr) HEAD_TRY(launch_rows_copy(w, c.stream));
+  return hipSuccess;
+}
+
+template <typename T>
+hipError_t head_fwd(const HeadCall& c) {
+  const HeadPlan p(c, 0);
+  const HeadState st(c.state, c.N, c.K);
+  const unsigned row_blocks = (unsigned)((c.N + 3) / 4);
+  const float inv_t = 1.0f / c.temperature;
+  if (p.distill && c.N > 0) {
+    if (c.teacher_dtype == 0)
+      hipLaunchKernelGGL(teacher_kernel<float>, dim3(row_blocks), dim3(kThreads), 0, c.stream, (const float*)c.teacher, c.teacher_ld, c.ids, c.ids_ld, c.N, c.K, inv_t, p.tp, p.ent, p.live);
+    else if (c.teacher_dtype == 1)
+      hipLaunchKernelGGL(teacher_kernel<bf16>, dim3(row_blocks), dim3(kThreads), 0, c.stream, (const bf16*)c.teacher, c.teacher_ld, c.ids, c.ids_ld, c.N, c.K, inv_t, p.tp, p.ent, p.live);
+    else
+      hipLaunchKernelGGL(teacher_kernel<f16>, dim3(row_blocks), dim3(kThreads), 0, c.stream, (const f16*)c.teacher, c.teacher_ld, c.ids, c.ids_ld, c.N, c.K, inv_t, p.tp, p.ent, p.live);
+    HEAD_TRY(hipGetLastError());
+  }
+  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, c.stream, c.ids, c.ids_ld, c.ignore_index, p.live, c.N, st.pos, st.hdr);
+  HEAD_TRY(hipGetLastError());
+  float* rows = c.reduction == 0 ? c.loss : p.rows;
+  if (c.N > 0) {
+    HEAD_TRY(operands<T>(c, p, st));
+    StatsArgs a;
+    a.x = p.x; a.x_ld = p.dp * 2; a.n_pad = p.n_pad;
+    a.w = p.w != nullptr ? p.w : (const char*)c.w; a.w_ld = p.w != nullptr ? p.dp * 2 : c.w_ld * 2; a.V = c.V;
+    a.segs = p.logits(); a.ksteps = (int)(p.dp / 32); a.tiles_v = p.tiles_v; a.tiles_n = p.tiles_n;
+    a.to_log2 = kLog2e / c.temperature; a.hdr = st.hdr; a.part = p.part;
+    hipLaunchKernelGGL(stats_kernel<T>, dim3((unsigned)((int64_t)p.tiles_v * p.tiles_n)), dim3(kThreads), 0, c.stream, a);
+    HEAD_TRY(hipGetLastError());
+    RowsArgs r;
+    r.x = c.x; r.x_ld = c.x_ld; r.w = c.w; r.w_ld = c.w_ld; r.ids = c.ids; r.ids_ld = c.ids_ld; r.tp = p.tp; r.ent = p.ent;
+    r.part = p.part; r.part_ld = p.n_pad; r.tiles = p.tiles_v; r.N = c.N; r.V = c.V; r.d = c.d; r.K = c.K; r.vec = rows_vec(c);
+    r.temperature = c.temperature; r.pos = st.pos; r.lse2 = st.lse2; r.t = st.t; r.loss = rows;
+    hipLaunchKernelGGL(rows_kernel<T>, dim3((unsigned)((c.N + 7) / 8)), dim3(kThreads), 0, c.stream, r);
+    HEAD_TRY(hipGetLastError());
+  }
+  if (c.reduction != 0) {
+    hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, c.stream, rows, c.N, st.hdr, c.reduction == 1, c.loss);
+    HEAD_TRY(hipGetLastError());
+  }
+  return hipSuccess;
+}
+
+template <typename T>
+hipError_t head_bwd(const HeadCall& c) {
+  const HeadPlan p(c, 1);
+  const HeadState st(c.state, c.N, c.K);
+  if (c.N == 0) {
+    if (c.dw != nullptr)
+      hipLaunchKernelGGL(zero_kernel, dim3(1024), dim3(kThreads), 0, c.stream, (uint16_t*)c.dw, c.V * c.d * es_of(c.dtype) / 2);
+    return hipGetLastError();
+  }
+  const float factor = p.distill ? c.temperature : 1.0f;  // T^2 of the loss, 1/T of z
+  hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, c.stream, c.dloss, c.reduction, factor, c.N, p.n_pad, st.pos, st.hdr, p.coef);
+  HEAD_TRY(hipGetLastError());
+  HEAD_TRY(operands<T>(c, p, st));
+  const char* w = p.w != nullptr ? p.w : (const char*)c.w;
+  const int64_t w_ld = p.w != nullptr ? p.dp * 2 : c.w_ld * 2;
+  for (int64_t v0 = 0; v0 < c.V; v0 += p.C) {
+    const int cols = (int)(c.V - v0 < p.C ? c.V - v0 : p.C);
+    GradArgs a;
+    a.x = p.x; a.x_ld = p.dp * 2; a.n_pad = p.n_pad; a.w = w + v0 * w_ld; a.w_ld = w_ld; a.cols = cols;
+    a.segs = p.logits(); a.ksteps = (int)(p.dp / 32); a.tiles_v = (int)(round_up(cols, 256) / 256); a.tiles_n = p.tiles_n;
+    a.to_log2 = kLog2e / c.temperature; a.hdr = st.hdr; a.lse2 = st.lse2; a.coef = p.coef; a.g = p.g; a.C = p.C; a.plane = p.g_plane;
+    hipLaunchKernelGGL(grad_kernel<T>, dim3((unsigned)((int64_t)a.tiles_v * a.tiles_n)), dim3(kThreads), 0, c.stream, a);
+    HEAD_TRY(hipGetLastError());
+    hipLaunchKernelGGL(scatter_kernel<T>, dim3((unsigned)((c.N * c.K + kThreads - 1) / kThreads)), dim3(kThreads), 0, c.stream,
+                       c.ids, c.ids_ld, c.N, c.K, st.pos, st.t, p.coef, st.hdr, v0, cols, p.g, p.C, p.g_plane);
+    HEAD_TRY(hipGetLastError());
+    WideProducts q = {};
+    q.dtype = c.dtype; q.gated = 0; q.N = c.N; q.n_pad = p.n_pad; q.d = c.d; q.dp = p.dp; q.halves = 1; q.cols = cols;
+    q.C = p.C;
+    q.x = p.x; q.x_ld = p.dp * 2; q.x_plane = p.x_plane; q.x_rows = (int)p.n_pad;
+    q.w[0] = w + v0 * w_ld; q.w_ld = w_ld; q.w_plane = p.w_plane; q.w_rows = (int)(c.V - v0);
+    q.g = p.g; q.g_plane = p.g_plane; q.g_half = 0;
+    q.dx_part = p.dx_part; q.dx_add = v0 > 0;
+    q.dw[0] = c.dw == nullptr ? nullptr : (char*)c.dw + v0 * c.d * es_of(c.dtype); q.dw_part = p.dw_part;
+    q.dx_split = p.dx_split; q.dw_split = p.dw_split; q.hdr = st.hdr; q.use_live = 1;
+    HEAD_TRY(launch_wide_products(q, c.stream));
+  }
+  if (c.dx != nullptr) {
+    const WideFinish f{c.dtype, 0, c.N, p.n_pad, c.d, p.dp, p.dx_split, p.dx_part, st.pos, st.hdr, c.dx};
+    HEAD_TRY(launch_wide_finish(f, c.stream));
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+size_t head_state_bytes(int64_t N, int K) { return HeadState(nullptr, N, K).bytes; }
+size_t head_workspace_bytes(const HeadCall& c, int backward) { return HeadPlan(c, backward).bytes; }
+
+hipError_t launch_head_fwd(const HeadCall& c) {
+  return c.dtype == 0 ? head_fwd<float>(c) : c.dtype == 1 ? head_fwd<bf16>(c) : head_fwd<f16>(c);
+}
+hipError_t launch_head_bwd(const HeadCall& c) {
+  return c.dtype == 0 ? head_bwd<float>(c) : c.dtype == 1 ? head_bwd<bf16>(c) : head_bwd<f16>(c);
+}
+
+}  // namespace msa

@@ -157,6 +157,43 @@ struct VerifyCall {
 int verify_parts(int64_t V);
 hipError_t launch_verify(const VerifyCall& c);
 
+// Losses of rows against a vocabulary, straight from the rows: z = hidden weight^T / temperature, cross entropy
+// (teacher null, K = 1) or the divergence from a teacher's K largest logits.
+struct HeadCall {
+  int64_t N, V; int d, K, dtype, teacher_dtype, reduction;  // reduction 0: a loss per row, 1: their mean, 2: their sum
+  float temperature;
+  int64_t ignore_index;
+  const void* x; int64_t x_ld;
+  const void* w; int64_t w_ld;
+  const int64_t* ids; int64_t ids_ld;
+  const void* teacher; int64_t teacher_ld;
+  void* state;
+  float* loss;
+  const float* dloss;
+  void* dx; void* dw;
+  void* workspace;
+  hipStream_t stream;
+};
+size_t head_state_bytes(int64_t N, int K);
+size_t head_workspace_bytes(const HeadCall& c, int backward);
+hipError_t launch_head_fwd(const HeadCall& c);
+hipError_t launch_head_bwd(const HeadCall& c);
+
+// h = act(x w[0]^T) * (x w[1]^T) and its gradients.
+struct GatedCall {
+  int64_t N; int d, F, dtype, act;  // act 0: silu, 1: gelu (erf)
+  const void* x; int64_t x_ld;
+  const void* w[2]; int64_t w_ld[2];
+  void* h;
+  const void* dh; int64_t dh_ld;
+  void* dx; void* dw[2];
+  void* workspace;
+  hipStream_t stream;
+};
+size_t gated_workspace_bytes(const GatedCall& c, int backward);
+hipError_t launch_gated_fwd(const GatedCall& c);
+hipError_t launch_gated_bwd(const GatedCall& c);
+
 // Waves that share a row (32-query or 32-key unit) in the live, dq and dK/dV
 // passes: launches with few rows split each row's units, so that about 2048
 // waves (2-byte types) or 4096 (fp32, whose rows take several times as long)

@@ -1,0 +1,347 @@
+// Matrix products on gfx950 for the kernels whose work is a product with a fused epilogue (the vocabulary head's
+// losses, the gated feed-forward): a block computes one tile C[m][n] = sum_k A[m][k] B[n][k] of 16-bit operands in
+// fp32 registers, the caller's epilogue does the rest.
+//
+// Feature rows (weights, or the columns of an output) are the m side and tokens the n side, so that a lane holds
+// many features of few tokens: sums over a token's features need no shuffles, and four registers are four
+// neighbours of an output row.
+//
+// Each operand lies in memory with either its k contiguous (rows of A or B) or its m or n contiguous (k rows), and
+// is staged in that order; MFMA fragments come by ds_read_b128 or, transposed, by ds_read_b64_tr_b16.
+#pragma once
+
+#include "msa_device.h"
+
+namespace msa {
+
+constexpr int kMmK = 32;      // k of a stage
+constexpr int kMmSegs = 6;    // products that one tile adds up
+
+// A sum over up to kMmSegs operand pairs of the same shape (byte offsets to A and B).  fp32 operands enter as two
+// fp16 terms, x s = h + 2^-11 l with a power of two s: three products h l + l h, then 2^-11 of their sum, then h h.
+struct MmSegs {
+  int64_t a[kMmSegs], b[kMmSegs];
+  int n, low;  // products; the first `low` are of order 2^-11 (0: none)
+};
+constexpr float kLowTerm = 1.0f / 2048.0f;
+
+// Starts the copy of 16 bytes a lane from base (uniform) + off to LDS at `to` (uniform) + 16 lane.  Written out because
+// the compiler waits for every copy in flight before it reads any of the array that one goes to, which would undo the
+// stages; the loop waits for the stage that it reads (MmTile::arrive).  M0 takes a wait state before its use.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // M0 is reserved: the clobber still tells the compiler that it changed
+__device__ inline void mm_copy(const char* base, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// Four neighbours of an output row.
+template <typename O> struct Quad { typedef __attribute__((__vector_size__(4 * sizeof(O)))) O V; };
+template <typename O, typename Fn>
+__device__ inline typename Quad<O>::V quad(Fn fn) {
+  typename Quad<O>::V v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = from_f<O>(fn(e));
+  return v;
+}
+
+// E: operand type.  BM x BN: the block's tile; WM x WN waves share it.  AMN, BMN: the operand's m or n is
+// contiguous.  DUAL: A is two matrices, whose rows alternate by 64 (m = 128 i + j: row 64 i + j of the first for j <
+// 64, row 64 i + j - 64 of the second above).  NST: stages.
+template <typename E, int BM, int BN, int WM, int WN, bool AMN, bool BMN, bool DUAL, int NST>
+struct MmTile {
+  using M = Mma<E>;
+  using frag = typename M::frag;
+  static constexpr int NT = 64 * WM * WN;                    // threads
+  static constexpr int MB = BM / WM / 32, NB = BN / WN / 32;  // 32x32 blocks of a wave
+  static constexpr int ABYTES = BM * kMmK * 2, BBYTES = BN * kMmK * 2, STAGE = ABYTES + BBYTES;
+  static constexpr int LDS = NST * STAGE;
+  static constexpr int NWAVES = WM * WN;
+  static constexpr int AI = ABYTES / 1024 / NWAVES, BI = BBYTES / 1024 / NWAVES;  // copies of 1 KiB a wave issues
+  static_assert(AI * NWAVES * 1024 == ABYTES && BI * NWAVES * 1024 == BBYTES, "a stage is whole copies of every wave");
+  static_assert(!DUAL || (!AMN && NWAVES == 4 && BM % 128 == 0), "alternating rows are laid out for four waves");
+
+  typedef f32x16 Acc[MB][NB];
+
+  // One operand's copies.  K-contiguous: rows of 64 bytes, a copy is 16 rows; the 16-byte chunks of row R are
+  // XOR-swizzled by (R >> 1) & 3.  Otherwise: k rows of W columns; chunks are swizzled by (k & 3) << 1, so that the
+  // four rows that a transposed read takes lie in different banks.
+  template <bool MN, int W, int NI, bool ALT>
+  struct Loader {
+    uint32_t off[NI];
+    uint32_t ld;   // bytes from row to row
+    int rows, r0;  // MN: k rows of the matrix (later ones read the last), the lane's row of copy 0
+    static constexpr int CPR = W / 8;            // MN: chunks of a row
+    static constexpr int RPI = 64 / CPR;         // MN: rows of a copy (W <= 512)
+    // first: the tile's first row (K-contiguous) or column (MN); count: rows or columns of the matrix from there on.
+    // ALT: count of each of the two matrices.
+    __device__ inline void init(int64_t stride_bytes, int count, int wave, int lane, int krows) {
+      ld = (uint32_t)stride_bytes;
+      rows = krows;
+      if constexpr (!MN) {
+        const int lr = lane >> 2, chunk = (lane & 3) ^ ((lane >> 3) & 3);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          int r = ALT ? (j >> 1) * 64 + 16 * wave + lr : (j * NWAVES + wave) * 16 + lr;
+          r = r < count ? r : count - 1;
+          off[j] = (uint32_t)r * ld + (uint32_t)chunk * 16u;
+        }
+      } else {
+        static_assert(64 % CPR == 0, "a copy is whole rows");
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          const int p = (j * NWAVES + wave) * 64 + lane, k = p / CPR;
+          int col = ((p % CPR) ^ ((k & 3) << 1)) * 8;
+          col = col < count ? col : count - 8;  // count is a multiple of 8
+          off[j] = (uint32_t)k * ld + (uint32_t)col * 2u;
+        }
+        r0 = wave * RPI + lane / CPR;
+      }
+    }
+    // Starts the copies of the stage whose k begins at k0; base points to (first row, k0) or (k0, first column).
+    __device__ inline void issue(const char* base, int64_t alt, LdsChar* lds, int wave, int k0) const {
+      // k rows behind the last one read it again (their other operand is zero); all of this is block-uniform
+      const bool cut = MN && k0 + kMmK > rows;
+      int last = 0;
+      if (cut) {
+        const int from = k0 < rows ? k0 : rows - 1;
+        base -= (int64_t)(k0 - from) * ld;
+        last = rows - 1 - from;
+      }
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        uint32_t o = off[j];
+        if constexpr (MN) {
+          if (cut) {
+            const int k = r0 + j * NWAVES * RPI;
+            if (k > last) o -= (uint32_t)(k - last) * ld;
+          }
+        }
+        const char* b = ALT && (j & 1) ? base + alt : base;
+        mm_copy(b, o, (uint32_t)(uintptr_t)lds + (uint32_t)((j * NWAVES + wave) * 1024));
+      }
+    }
+  };
+
+  // The lane's fragment address in a staged operand: block i of 32 rows or columns from `first`, half c of the k.
+  template <bool MN, int W>
+  struct Reader {
+    uint32_t at;
+    __device__ inline void init(int first, int lane) {
+      const int half = lane >> 5;
+      if constexpr (!MN) {
+        const int R = lane & 31;
+        at = (uint32_t)((first + R) * 64 + ((half ^ ((R >> 1) & 3)) << 4));
+      } else {
+        const int kk = (lane & 15) >> 2, q = lane & 3, gg = (lane >> 4) & 1;
+        at = (uint32_t)((8 * half + kk) * (W * 2) + first * 2 + (((2 * gg + (q >> 1)) ^ (kk << 1)) << 4) + 8 * (q & 1));
+      }
+    }
+    __device__ inline frag read(const LdsChar* tile, int i, int c) const {
+      if constexpr (!MN) {
+        return *reinterpret_cast<const __attribute__((address_space(3))) frag*>(tile + (at ^ (uint32_t)(c << 5)) + i * 2048);
+      } else {
+        typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4;
+        typedef __attribute__((__vector_size__(8 * sizeof(short)))) short s16x8;
+        s16x8 v;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const LdsChar* p = tile + (at ^ (uint32_t)((i & 1) << 6)) + (i >> 1) * 128 + (16 * c + 4 * j) * (W * 2);
+          const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)const_cast<LdsChar*>(p));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * j + e] = x[e];
+        }
+        return __builtin_bit_cast(frag, v);
+      }
+    }
+  };
+
+  // The tile's operands: where (first row or column, k = 0) lies, rows or columns there are from it on, bytes from
+  // row to row, bytes that 32 k advance, k rows (MN).
+  struct Side {
+    const char* p;
+    int count;
+    int64_t ld;
+    int krows;
+    int64_t alt;  // DUAL: to the second matrix
+  };
+
+  // acc += the tile's product over k in [k0, k0 + 32 steps).  Every thread of the block calls it with the same
+  // arguments.  lds: LDS bytes of the block's own, free on entry; on return every wave is past its last read.
+  __device__ static inline void run(Acc& acc, LdsChar* lds, const Side& A, const Side& B, const MmSegs& segs, int k0,
+                                    int steps) {
+    const int tid = (int)threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave % WM, wn = wave / WM;
+    Loader<AMN, BM, AI, DUAL> la;
+    Loader<BMN, BN, BI, false> lb;
+    la.init(A.ld, A.count, wave, lane, A.krows);
+    lb.init(B.ld, B.count, wave, lane, B.krows);
+    Reader<AMN, BM> ra;
+    Reader<BMN, BN> rb;
+    ra.init(wm * (BM / WM), lane);
+    rb.init(wn * (BN / WN), lane);
+    const int64_t astep = AMN ? A.ld * kMmK : kMmK * 2, bstep = BMN ? B.ld * kMmK : kMmK * 2;
+    const char* const a0 = A.p + (AMN ? A.ld * k0 : (int64_t)k0 * 2);
+    const char* const b0 = B.p + (BMN ? B.ld * k0 : (int64_t)k0 * 2);
+
+    const int total = steps * segs.n;
+    int iseg = 0, istep = 0;  // the next stage to copy
+    const char* ia = a0 + segs.a[0];
+    const char* ib = b0 + segs.b[0];
+    auto issue = [&](int slot) {
+      LdsChar* s = lds + slot * STAGE;
+      la.issue(ia, A.alt, s, wave, k0 + istep * kMmK);
+      lb.issue(ib, 0, s + ABYTES, wave, k0 + istep * kMmK);
+      ia += astep;
+      ib += bstep;
+      if (++istep == steps) {
+        istep = 0;
+        if (++iseg < segs.n) {
+          ia = a0 + segs.a[iseg];
+          ib = b0 + segs.b[iseg];
+        }
+      }
+    };
+    int filled = 0;
+#pragma unroll
+    for (int u = 0; u < NST - 1; ++u)
+      if (u < total) { issue(u); ++filled; }
+    const int low = steps * segs.low;
+    int rs = 0, ws = NST - 1;
+    for (int t = 0; t < total; ++t) {
+      // stage t has landed once only the younger ones are outstanding
+      if (filled - t > NST - 2) arrive<(NST - 2) * (AI + BI)>();
+      else if (NST > 3 && filled - t == NST - 2) arrive<(NST > 3 ? NST - 3 : 0) * (AI + BI)>();
+      else arrive<0>();
+      if (filled < total) { issue(ws); ++filled; }
+      const LdsChar* at = lds + rs * STAGE;
+      const LdsChar* bt = at + ABYTES;
+      rs = rs + 1 == NST ? 0 : rs + 1;
+      ws = ws + 1 == NST ? 0 : ws + 1;
+      if (low != 0 && t == low) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] *= kLowTerm;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        frag a[MB], b[NB];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) a[i] = ra.read(at, i, c);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) b[j] = rb.read(bt, j, c);
+        // MB * NB independent sums: an accumulator comes again only after all the others, so no MFMA waits for the
+        // one before it and none reads its operands late (see the source-operand guard in msa_device.h)
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int j = 0; j < NB; ++j) acc[i][j] = M::mma_ng(a[i], b[j], acc[i][j]);
+        if constexpr (MB * NB < 4) {
+#pragma unroll
+          for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) asm volatile(MSA_NOP16 : "+v"(a[i]), "+v"(b[j]));
+        }
+      }
+    }
+    arrive<0>();
+  }
+
+  // The block's barrier, with this wave's LDS reads done and at most N of its copies outstanding.
+  template <int N>
+  __device__ static inline void arrive() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+  }
+
+  // Writes rows of an output: dst[n ld + m .. + 3] = fn(i, j, g) of registers 4 g .. 4 g + 3 of blocks (i, j), i < MS, for
+  // n < rows and m < cols; ADD: added to what is there (O float).  A wave's MS blocks are neighbours (MS = MB: the tile itself).  vec:
+  // dst and ld allow 16-byte accesses.  The values go through the block's LDS (free on entry and on return), 32
+  // tokens of each wave at a time, so that a wave writes whole rows.
+  template <typename O, bool ADD, int MS = MB, typename Fn>
+  __device__ static inline void store_rows(LdsChar* lds, O* dst, int64_t ld, int rows, int cols, bool vec, Fn fn) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      store_tokens<O, ADD, MS>(lds, dst, ld, rows, cols, vec, j, [&](int i, int g) { return fn(i, j, g); });
+  }
+  // The part of it for the tokens of blocks (., j).
+  template <typename O, bool ADD, int MS, typename Fn>
+  __device__ static inline void store_tokens(LdsChar* lds, O* dst, int64_t ld, int rows, int cols, bool vec, int j, Fn fn) {
+    constexpr int W = 32 * MS * WM;
+    constexpr int ROW = W * (int)sizeof(O) + 16, PER = 16 / (int)sizeof(O), CPR = W / PER, R = 32 * WN;
+    static_assert(R * ROW <= LDS, "the staged rows fit the tile's LDS");
+    typedef __attribute__((address_space(3))) typename Quad<O>::V LdsQuad;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave % WM, wn = wave / WM;
+    LdsChar* to = lds + (wn * 32 + (lane & 31)) * ROW + (wm * 32 * MS + 4 * (lane >> 5)) * (int)sizeof(O);
+#pragma unroll
+    for (int i = 0; i < MS; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const typename Quad<O>::V v = fn(i, g);
+        *reinterpret_cast<LdsQuad*>(to + (32 * i + 8 * g) * (int)sizeof(O)) = v;
+      }
+    __syncthreads();
+#pragma unroll 4
+    for (int u = tid; u < R * CPR; u += NT) {
+      const int r = u / CPR, c = (u - r * CPR) * PER, n = (r >> 5) * (BN / WN) + 32 * j + (r & 31);
+      if (n < rows && c < cols) {
+        typedef __attribute__((__vector_size__(16))) O OV;
+        OV v = *reinterpret_cast<const __attribute__((address_space(3))) OV*>(lds + r * ROW + c * (int)sizeof(O));
+        O* p = dst + (int64_t)n * ld + c;
+        if (vec && c + PER <= cols) {
+          if constexpr (ADD) v += *reinterpret_cast<const OV*>(p);
+          *reinterpret_cast<OV*>(p) = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < PER; ++e)
+            if (c + e < cols) p[e] = ADD ? (O)((float)p[e] + (float)v[e]) : v[e];
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  // Hides the values from the compiler, which would otherwise keep what it formed from them for a second use.
+  __device__ static inline void renew(Acc& acc) {
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) asm volatile("" : "+v"(acc[i][j]));
+  }
+
+  __device__ static inline void clear(Acc& acc) {
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+  }
+
+  // Place of a lane's registers in the tile: register 4 g + e of block (i, j) is C[m(i, g) + e][n(j)].
+  __device__ static inline int m_of(int wm, int lane, int i, int g) { return wm * (BM / WM) + 32 * i + 8 * g + 4 * (lane >> 5); }
+  __device__ static inline int n_of(int wn, int lane, int j) { return wn * (BN / WN) + 32 * j + (lane & 31); }
+};
+
+// Blocks of a grid go to the eight XCDs in turn, each with an L2 of its own: block id -> position in an order whose
+// consecutive eighths are an XCD's.
+__device__ inline int64_t xcd_order(int64_t id, int64_t total) {
+  const int64_t x = id & 7, i = id >> 3, q = total >> 3, r = total & 7;
+  return x * q + (x < r ? x : r) + i;
+}
+
+// Tile (tm, tn) at position t of an order that walks patches of G m-tiles by all n-tiles, m first: the tiles in flight
+// on an XCD then share few rows of both operands.
+__device__ inline void patch_order(int64_t t, int tiles_m, int tiles_n, int G, int& tm, int& tn) {
+  const int64_t per = (int64_t)G * tiles_n;
+  const int g = (int)(t / per), in = (int)(t - g * per);
+  const int w = tiles_m - g * G < G ? tiles_m - g * G : G;
+  tn = in / w;
+  tm = g * G + (in - tn * w);
+}
+
+}  // namespace msa

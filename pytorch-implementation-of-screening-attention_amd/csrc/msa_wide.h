@@ -1,0 +1,114 @@
+// What the kernels around wide products share (msa_head.hip, msa_gated.hip): operands laid out for the matrix core,
+// power-of-two scales, and the two products of a backward pass, dx = G W and dW = G^T x.
+//
+// Types: bf16 and fp16 rows are operands as they are (copied only where their rows are not 16-byte aligned or their
+// width is no multiple of 32).  fp32 rows become two fp16 terms, x s = h + 2^-11 l, with a power of two s for the whole
+// matrix that brings its largest entry to [2^14, 2^15): 22 bits of every entry down to 2^-28 of the largest, and three
+// MFMA products where the fp32 MFMA would take sixteen times as long.
+#pragma once
+
+#include "msa_internal.h"
+#include "msa_matmul.h"
+
+namespace msa {
+
+// Operand type of an input type, and its number of terms.
+template <typename T> struct Wide { typedef T E; static constexpr int P = 1; };
+template <> struct Wide<float> { typedef f16 E; static constexpr int P = 2; };
+
+// Device-side facts of a call.  max_*: bits of the largest finite |entry| (of counting rows), norm_*: of the largest
+// finite squared row norm; floats of one sign compare as integers, so atomicMax gives the same whatever the order.
+struct WideHdr {
+  int live;  // rows that count
+  uint32_t max_x, max_w, max_dh, norm_x, norm_w;
+  float cmax;  // what the rows' gradient coefficients are divided by: their common value, or a power of two
+  int pad[9];
+};
+static_assert(sizeof(WideHdr) == 64, "header size");
+
+__device__ inline float pow2_to(float mx, int top) {  // p with mx p in [2^(top-1), 2^top); 1 for 0
+  if (!(mx > 0.0f)) return 1.0f;
+  int ex;
+  (void)frexpf(mx, &ex);
+  int e = top - ex;
+  e = e > 120 ? 120 : (e < -120 ? -120 : e);
+  return ldexpf(1.0f, e);
+}
+__device__ inline float finite_max(uint32_t bits) { return __uint_as_float(bits); }
+
+// Scales of the operands.  fp16 gradients of logits lie in [-1, 1] and are kept times 2^15; those of the gated
+// projections are bounded by max|dh| 1.13 max|x| max|w| (|act(g)| <= |g|, |act'| < 1.13).
+template <typename T> __device__ inline float scale_x(const WideHdr* h) { return Wide<T>::P == 2 ? pow2_to(finite_max(h->max_x), 15) : 1.0f; }
+template <typename T> __device__ inline float scale_w(const WideHdr* h) { return Wide<T>::P == 2 ? pow2_to(finite_max(h->max_w), 15) : 1.0f; }
+template <typename T> __device__ inline float scale_g(const WideHdr* h, int gated) {
+  if constexpr (__is_same(T, bf16)) return 1.0f;
+  if (!gated) return 32768.0f;
+  return pow2_to(1.15f * finite_max(h->max_dh) * sqrtf(finite_max(h->norm_x)) * sqrtf(finite_max(h->norm_w)), 15);
+}
+
+// The terms of v (already scaled).  v is held in a register first: formed inside, a product that makes v may be rounded
+// to h straight from its exact value in one place and from the rounded one in another, and l belongs to one h only.
+template <typename T> struct Terms;
+template <> struct Terms<float> {
+  f16 h, l;
+  __device__ explicit Terms(float v) {
+    asm("" : "+v"(v));
+    h = (f16)v;
+    l = (f16)((v - (float)h) * 2048.0f);
+  }
+};
+
+inline int64_t wide_dp(int64_t d) { return round_up(d, 32); }
+
+// Rows of a matrix (rows x d, type dtype) as operand rows of dp columns: `planes` matrices of plane_bytes each.
+// pos: null, or which row of the operand each row becomes (-1: none); rows from *live up to the next multiple of 128
+// are then zeroed.  hdr, slot (0: x, 1: w): fp32's scale.
+struct RowsCopy {
+  const void* src; int64_t ld; int64_t rows; int d, dtype;
+  char* dst; int64_t plane_bytes;
+  const int* pos; WideHdr* hdr; int slot;
+};
+hipError_t launch_rows_copy(const RowsCopy& c, hipStream_t s);
+// max|entry| and, with `norms`, the largest squared row norm of a matrix into hdr (slot 0: x, 1: w, 2: dh).
+hipError_t launch_rows_max(const RowsCopy& c, int norms, hipStream_t s);
+hipError_t launch_hdr_clear(WideHdr* hdr, hipStream_t s);
+
+// The backward products of one piece of the weight's rows.
+struct WideProducts {
+  int dtype, gated;
+  int64_t N, n_pad;  // tokens (operand rows), as padded in g
+  int d;
+  int64_t dp;
+  int halves;        // weights: 1, or 2 (gate and up)
+  int cols;          // weight rows of the piece
+  int64_t C;         // columns of g: cols rounded up to 256
+  const char* x; int64_t x_ld, x_plane; int x_rows;           // bytes from row to row, to the second term; readable rows
+  const char* w[2]; int64_t w_ld, w_plane; int w_rows;        // the piece's first rows; readable rows from there
+  const char* g; int64_t g_plane, g_half;                     // [half][term][n_pad][C]
+  float* dx_part; int dx_add;                                 // [dx_split][n_pad][dp], or null: no dx
+  void* dw[2];                                                // the piece's rows of the gradients, or null
+  float* dw_part;                                             // [dw_split][halves][C][dp] where dw_split > 1
+  int dx_split, dw_split;
+  const WideHdr* hdr;
+  int use_live;  // tokens are hdr->live
+};
+hipError_t launch_wide_products(const WideProducts& p, hipStream_t s);
+
+// Blocks that share the k of each tile, for tiles of 256 x 128 of which a CU holds two.
+void wide_splits(int64_t N, int d, int64_t C, int halves, bool dx, bool dw, int* dx_split, int* dw_split);
+
+// dx[n] = factor * sum of the parts' rows pos[n] (pos null: n); rows with pos < 0 are zero.
+struct WideFinish {
+  int dtype, gated;
+  int64_t N, n_pad;
+  int d;
+  int64_t dp;
+  int split;
+  const float* part;
+  const int* pos;
+  const WideHdr* hdr;
+  void* dx;
+};
+hipError_t launch_wide_finish(const WideFinish& f, hipStream_t s);
+
+}  // namespace msa

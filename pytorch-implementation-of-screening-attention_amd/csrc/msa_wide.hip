@@ -1,0 +1,327 @@
+// Operand rows, scales and the backward products of the wide layers (msa_wide.h).
+#include "msa_wide.h"
+
+namespace msa {
+namespace {
+
+constexpr int kThreads = 256;
+
+__global__ void hdr_clear_kernel(WideHdr* h) {
+  if (threadIdx.x < sizeof(WideHdr) / 4) reinterpret_cast<uint32_t*>(h)[threadIdx.x] = 0u;
+}
+
+template <typename T>
+__device__ inline void atomic_max_finite(uint32_t* slot, float v) {
+  v = fabsf(v);
+  if (v < INFINITY && v > 0.0f) atomicMax(slot, __float_as_uint(v));
+}
+
+// A wave per row, rows in turn.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) rows_max_kernel(const T* src, int64_t ld, int64_t rows, int d, const int* pos,
+                                                            uint32_t* mslot, uint32_t* nslot) {
+  const int lane = (int)threadIdx.x & 63;
+  float mx = 0.0f, nx = 0.0f;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
+    if (pos != nullptr && pos[r] < 0) continue;
+    const T* p = src + r * ld;
+    float ss = 0.0f;
+    for (int c = lane; c < d; c += 64) {
+      const float v = fabsf(to_f(p[c]));
+      if (v < INFINITY) {
+        mx = fmaxf(mx, v);
+        ss = fmaf(v, v, ss);
+      }
+    }
+    if (nslot != nullptr) {
+      ss = wave_sum(ss);
+      if (ss < INFINITY) nx = fmaxf(nx, ss);
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+  __shared__ float sm[4], sn[4];
+  if (lane == 0) { sm[threadIdx.x >> 6] = mx; sn[threadIdx.x >> 6] = nx; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    atomic_max_finite<T>(mslot, fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])));
+    if (nslot != nullptr) atomic_max_finite<T>(nslot, fmaxf(fmaxf(sn[0], sn[1]), fmaxf(sn[2], sn[3])));
+  }
+}
+
+// Rows to operand rows.  A wave per row, 8 columns a lane; the last blocks zero the rows behind the last one that
+// counts, up to the next multiple of 128.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads) rows_copy_kernel(const T* src, int64_t ld, int64_t rows, int d, int dp,
+                                                             char* dst, int64_t plane, const int* pos,
+                                                             const WideHdr* hdr, int slot) {
+  using E = typename Wide<T>::E;
+  const int lane = (int)threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  int64_t to = r;
+  bool zero = false;
+  if (r >= rows) {
+    if (pos == nullptr) return;
+    const int64_t live = hdr->live;
+    to = live + (r - rows);
+    if (to >= (live + 127) / 128 * 128) return;
+    zero = true;
+  } else if (pos != nullptr) {
+    to = pos[r];
+    if (to < 0) return;
+  }
+  float s = 1.0f;
+  if constexpr (Wide<T>::P == 2) s = slot == 0 ? scale_x<T>(hdr) : scale_w<T>(hdr);
+  E* out = reinterpret_cast<E*>(dst) + to * dp;
+  const T* in = src + r * ld;
+  typedef __attribute__((__vector_size__(16))) E E8;
+  for (int c = lane * 8; c < dp; c += 512) {
+    T x[8];
+    if (VEC && !zero && c + 8 <= d) {
+      typedef __attribute__((__vector_size__(16))) T T16;
+      constexpr int PER = 16 / (int)sizeof(T);
+#pragma unroll
+      for (int q = 0; q < 8 / PER; ++q) {
+        const T16 t = *reinterpret_cast<const T16*>(in + c + q * PER);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x[q * PER + e] = t[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = !zero && c + e < d ? in[c + e] : (T)0.0f;
+    }
+    E8 h;
+    if constexpr (Wide<T>::P == 2) {
+      E8 l;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const Terms<float> t(x[e] * s);
+        h[e] = t.h;
+        l[e] = t.l;
+      }
+      *reinterpret_cast<E8*>(reinterpret_cast<char*>(out + c) + plane) = l;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] = x[e];
+    }
+    *reinterpret_cast<E8*>(out + c) = h;
+  }
+}
+
+struct ProductArgs {
+  int64_t N, n_pad;
+  int d;
+  int64_t dp;
+  int dx_tm, dx_tn, dx_split, dw_tm, dw_tn, dw_split, halves, cols;
+  int dx_blocks;
+  int64_t C;
+  MmSegs dx_segs, dw_segs;
+  const char* x; int64_t x_ld; int x_rows;
+  const char* w; int64_t w_ld; int w_rows;
+  const char* g; int64_t g_half;
+  float* dx_part; int dx_add;
+  void* dw0; void* dw1;
+  float* dw_part;
+  const WideHdr* hdr;
+  int use_live, gated, vec;
+};
+
+// A block per tile and split: the first dx_blocks take dx[n][m] = sum_v G[n][v] W[v][m], the others dW[v][m] = sum_n
+// G[n][v] x[n][m].  Both in one launch, so that neither leaves CUs idle at its end.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) products_kernel(ProductArgs p) {
+  using E = typename Wide<T>::E;
+  using TX = MmTile<E, 256, 128, 2, 2, true, false, false, 3>;
+  using TW = MmTile<E, 256, 128, 2, 2, true, true, false, 3>;
+  __shared__ char smem[TX::LDS];
+  LdsChar* lds = (LdsChar*)smem;
+  const int64_t N = p.use_live ? p.hdr->live : p.N;
+  const bool is_dx = (int)blockIdx.x < p.dx_blocks;
+  const float out_g = (p.gated ? 1.0f : p.hdr->cmax) / scale_g<T>(p.hdr, p.gated);
+  if (is_dx) {
+    int64_t t = xcd_order(blockIdx.x, p.dx_blocks);
+    const int split = (int)(t % p.dx_split);
+    t /= p.dx_split;
+    const int tm = (int)(t % p.dx_tm), tn = (int)(t / p.dx_tm);
+    const int n0 = tn * 128, m0 = tm * 256;
+    if (n0 >= N) return;
+    const int steps = (p.cols + 127) / 128 * 4, from = (int)((int64_t)steps * split / p.dx_split),
+              to = (int)((int64_t)steps * (split + 1) / p.dx_split);
+    typename TX::Acc acc;
+    TX::clear(acc);
+    const typename TX::Side A{p.w + (int64_t)m0 * 2, (int)(p.dp - m0), p.w_ld, p.w_rows, 0};
+    const typename TX::Side B{p.g + (int64_t)n0 * p.C * 2, (int)(p.n_pad - n0), p.C * 2, 0, 0};
+    TX::run(acc, lds, A, B, p.dx_segs, from * 32, to - from);
+    float* out = p.dx_part + ((int64_t)split * p.n_pad + n0) * p.dp + m0;
+    auto fn = [&](int i, int j, int g) { return quad<float>([&](int e) { return acc[i][j][4 * g + e]; }); };
+    const int rows = (int)(N - n0 < 128 ? N - n0 : 128);
+    if (p.dx_add) TX::template store_rows<float, true>(lds, out, p.dp, rows, (int)(p.dp - m0), true, fn);
+    else TX::template store_rows<float, false>(lds, out, p.dp, rows, (int)(p.dp - m0), true, fn);
+  } else {
+    int64_t t = xcd_order((int64_t)blockIdx.x - p.dx_blocks, (int64_t)gridDim.x - p.dx_blocks);
+    const int split = (int)(t % p.dw_split);
+    t /= p.dw_split;
+    const int tm = (int)(t % p.dw_tm);
+    t /= p.dw_tm;
+    const int tn = (int)(t % p.dw_tn), half = (int)(t / p.dw_tn);
+    const int n0 = tn * 128, m0 = tm * 256;
+    const int steps = (int)((N + 31) / 32), from = (int)((int64_t)steps * split / p.dw_split),
+              to = (int)((int64_t)steps * (split + 1) / p.dw_split);
+    typename TW::Acc acc;
+    TW::clear(acc);
+    const typename TW::Side A{p.x + (int64_t)m0 * 2, (int)(p.dp - m0), p.x_ld, p.x_rows, 0};
+    const typename TW::Side B{p.g + half * p.g_half + (int64_t)n0 * 2, (int)(p.C - n0), p.C * 2, (int)p.n_pad, 0};
+    if (to > from) TW::run(acc, lds, A, B, p.dw_segs, from * 32, to - from);
+    const int rows = p.cols - n0 < 128 ? p.cols - n0 : 128;
+    const float f = out_g, fx = 1.0f / scale_x<T>(p.hdr);
+    if (p.dw_split > 1) {
+      float* out = p.dw_part + (((int64_t)split * p.halves + half) * p.C + n0) * p.dp + m0;
+      TW::template store_rows<float, false>(lds, out, p.dp, rows, (int)(p.dp - m0), true,
+                                            [&](int i, int j, int g) { return quad<float>([&](int e) { return acc[i][j][4 * g + e]; }); });
+    } else {
+      T* out = (T*)(half ? p.dw1 : p.dw0) + (int64_t)n0 * p.d + m0;
+      TW::template store_rows<T, false>(lds, out, p.d, rows, p.d - m0, p.vec != 0,
+                                        [&](int i, int j, int g) { return quad<T>([&](int e) { return acc[i][j][4 * g + e] * f * fx; }); });
+    }
+  }
+}
+
+// Sums of split tiles in split order, scaled, as rows of T.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) parts_kernel(const float* part, int64_t part_stride, int split, int64_t rows,
+                                                         int d, int dp, const int* pos, const WideHdr* hdr, int gated,
+                                                         int by_x, T* out) {
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const int64_t at = pos == nullptr ? r : pos[r];
+  const float f = (gated ? 1.0f : hdr->cmax) / scale_g<T>(hdr, gated), f2 = 1.0f / (by_x ? scale_x<T>(hdr) : scale_w<T>(hdr));
+  for (int c = ((int)threadIdx.x & 63) * 4; c < d; c += 256) {
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (at >= 0) {
+      for (int s = 0; s < split; ++s) v += *reinterpret_cast<const f32x4*>(part + s * part_stride + at * dp + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = v[e] * f * f2;
+    }
+    T* o = out + r * d + c;
+    if (c + 4 <= d && d % 4 == 0) store4(o, v[0], v[1], v[2], v[3]);
+    else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < d) o[e] = from_f<T>(v[e]);
+    }
+  }
+}
+
+template <typename T>
+hipError_t rows_copy(const RowsCopy& c, hipStream_t s) {
+  const bool vec = ((uintptr_t)c.src & 15) == 0 && c.ld * (int64_t)sizeof(T) % 16 == 0;
+  const int64_t blocks = (c.rows + (c.pos != nullptr ? 128 : 0) + 3) / 4;
+  if (blocks == 0) return hipSuccess;
+  auto* k = vec ? rows_copy_kernel<T, true> : rows_copy_kernel<T, false>;
+  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(kThreads), 0, s, (const T*)c.src, c.ld, c.rows, c.d,
+                     (int)wide_dp(c.d), c.dst, c.plane_bytes, c.pos, c.hdr, c.slot);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t rows_max(const RowsCopy& c, int norms, hipStream_t s) {
+  const int64_t blocks = (c.rows + 3) / 4 < 1024 ? (c.rows + 3) / 4 : 1024;
+  if (blocks == 0) return hipSuccess;
+  uint32_t* m = c.slot == 0 ? &c.hdr->max_x : c.slot == 1 ? &c.hdr->max_w : &c.hdr->max_dh;
+  uint32_t* n = !norms ? nullptr : c.slot == 0 ? &c.hdr->norm_x : &c.hdr->norm_w;
+  hipLaunchKernelGGL(rows_max_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, s, (const T*)c.src, c.ld, c.rows,
+                     c.d, c.pos, m, n);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t products(const WideProducts& p, hipStream_t s) {
+  constexpr int P = Wide<T>::P;
+  ProductArgs a;
+  a.N = p.N; a.n_pad = p.n_pad; a.d = p.d; a.dp = p.dp;
+  a.dx_tm = (int)((p.dp + 255) / 256); a.dx_tn = (int)(p.n_pad / 128); a.dx_split = p.dx_split;
+  a.dw_tm = a.dx_tm; a.dw_tn = (p.cols + 127) / 128; a.dw_split = p.dw_split; a.halves = p.halves; a.cols = p.cols;
+  a.dx_blocks = p.dx_part != nullptr ? a.dx_tm * a.dx_tn * p.dx_split : 0;
+  a.C = p.C;
+  // (first, second) terms: low ones first
+  int n = 0;
+  for (int t = P - 1; t >= 0; --t)
+    for (int half = 0; half < p.halves; ++half) {
+      const int64_t wh = half ? p.w[1] - p.w[0] : 0, gh = half * p.g_half;
+      if (t == 1) {
+        a.dx_segs.a[n] = wh; a.dx_segs.b[n++] = gh + p.g_plane;
+        a.dx_segs.a[n] = wh + p.w_plane; a.dx_segs.b[n++] = gh;
+      } else {
+        a.dx_segs.a[n] = wh; a.dx_segs.b[n++] = gh;
+      }
+    }
+  a.dx_segs.n = n; a.dx_segs.low = n - p.halves;
+  n = 0;
+  if (P == 2) {
+    a.dw_segs.a[n] = 0; a.dw_segs.b[n++] = p.g_plane;
+    a.dw_segs.a[n] = p.x_plane; a.dw_segs.b[n++] = 0;
+  }
+  a.dw_segs.a[n] = 0; a.dw_segs.b[n++] = 0;
+  a.dw_segs.n = n; a.dw_segs.low = n - 1;
+  a.x = p.x; a.x_ld = p.x_ld; a.x_rows = p.x_rows;
+  a.w = p.w[0]; a.w_ld = p.w_ld; a.w_rows = p.w_rows;
+  a.g = p.g; a.g_half = p.g_half;
+  a.dx_part = p.dx_part; a.dx_add = p.dx_add;
+  a.dw0 = p.dw[0]; a.dw1 = p.dw[1]; a.dw_part = p.dw_part;
+  a.hdr = p.hdr; a.use_live = p.use_live; a.gated = p.gated;
+  a.vec = (int64_t)p.d * sizeof(T) % 16 == 0 && ((uintptr_t)p.dw[0] & 15) == 0 && ((uintptr_t)p.dw[1] & 15) == 0;
+  const int64_t dw_blocks = p.dw[0] != nullptr ? (int64_t)a.dw_tm * a.dw_tn * p.dw_split * p.halves : 0;
+  const int64_t blocks = a.dx_blocks + dw_blocks;
+  if (blocks == 0) return hipSuccess;
+  hipLaunchKernelGGL(products_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || dw_blocks == 0 || p.dw_split == 1) return e;
+  for (int half = 0; half < p.halves; ++half) {
+    hipLaunchKernelGGL(parts_kernel<T>, dim3((unsigned)((p.cols + 3) / 4)), dim3(kThreads), 0, s,
+                       p.dw_part + (int64_t)half * p.C * p.dp, (int64_t)p.halves * p.C * p.dp, p.dw_split, (int64_t)p.cols, p.d,
+                       (int)p.dp, (const int*)nullptr, p.hdr, p.gated, 1, (T*)p.dw[half]);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+template <typename T>
+hipError_t finish(const WideFinish& f, hipStream_t s) {
+  if (f.N == 0) return hipSuccess;
+  hipLaunchKernelGGL(parts_kernel<T>, dim3((unsigned)((f.N + 3) / 4)), dim3(kThreads), 0, s, f.part, f.n_pad * f.dp,
+                     f.split, f.N, f.d, (int)f.dp, f.pos, f.hdr, f.gated, 0, (T*)f.dx);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_hdr_clear(WideHdr* hdr, hipStream_t s) {
+  hipLaunchKernelGGL(hdr_clear_kernel, dim3(1), dim3(64), 0, s, hdr);
+  return hipGetLastError();
+}
+hipError_t launch_rows_copy(const RowsCopy& c, hipStream_t s) {
+  return c.dtype == 0 ? rows_copy<float>(c, s) : c.dtype == 1 ? rows_copy<bf16>(c, s) : rows_copy<f16>(c, s);
+}
+hipError_t launch_rows_max(const RowsCopy& c, int norms, hipStream_t s) {
+  return c.dtype == 0 ? rows_max<float>(c, norms, s) : c.dtype == 1 ? rows_max<bf16>(c, norms, s) : rows_max<f16>(c, norms, s);
+}
+hipError_t launch_wide_products(const WideProducts& p, hipStream_t s) {
+  return p.dtype == 0 ? products<float>(p, s) : p.dtype == 1 ? products<bf16>(p, s) : products<f16>(p, s);
+}
+hipError_t launch_wide_finish(const WideFinish& f, hipStream_t s) {
+  return f.dtype == 0 ? finish<float>(f, s) : f.dtype == 1 ? finish<bf16>(f, s) : finish<f16>(f, s);
+}
+
+void wide_splits(int64_t N, int d, int64_t C, int halves, bool dx, bool dw, int* dx_split, int* dw_split) {
+  const int64_t tm = (wide_dp(d) + 255) / 256;
+  const int64_t bx = dx ? tm * ((N + 127) / 128) : 0, bw = dw ? tm * (C / 128) * halves : 0;
+  // k of the products in steps of 32, shared so that about 512 blocks have equal parts of at least 8 steps
+  const int64_t kx = halves * (C / 32), kw = (N + 31) / 32;
+  int64_t each = (bx * kx + bw * kw) / 512;
+  if (each < 8) each = 8;
+  const int64_t sx = (kx + each / 2) / each, sw = (kw + each / 2) / each;
+  *dx_split = (int)(sx < 1 ? 1 : sx > 16 ? 16 : sx);
+  *dw_split = (int)(sw < 1 ? 1 : sw > 16 ? 16 : sw);
+}
+
+}  // namespace msa

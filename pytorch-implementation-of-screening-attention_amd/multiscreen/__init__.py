@@ -7,7 +7,7 @@ build_lib.py); `ops` exposes the operator boundary and the decode step.
 """
 
 from .attention import ScreeningAttention, KVCache
-from .layers import MultiscreenBlock, MultiscreenDecoderLayer
+from .layers import GatedFFN, MultiscreenBlock, MultiscreenDecoderLayer
 from .model import MultiscreenLM
 from .norm import TanhNorm
 from . import ops
@@ -18,6 +18,7 @@ __all__ = [
     "MultiscreenDecoderLayer",
     "MultiscreenLM",
     "TanhNorm",
+    "GatedFFN",
 ]
 
 __version__ = "0.1.0"

@@ -162,3 +162,55 @@ def verify_dense(target, tokens, parents=None, uniforms=None, draft=None):
         some = (rest > 0).nonzero()
         token[b] = int(over[0]) if len(over) else int(some[-1]) if len(some) else 0
     return path, count, token
+
+
+# ---------------------------------------------------------------------------
+# The vocabulary head's losses and the gated feed-forward for CPU tensors, by
+# autograd over the products that the GPU does not keep: the rules of ops.linear_cross_entropy,
+# ops.linear_distillation and ops.gated_linear.  A token outside the vocabulary raises here.
+# ---------------------------------------------------------------------------
+def _reduce_rows(loss, live, reduction):
+    if reduction not in ("none", "mean", "sum"):
+        raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
+    if reduction == "none":
+        return loss
+    total = loss.double().sum()
+    return (total / live.sum() if reduction == "mean" else total).float()
+
+
+def _check_tokens(ids, V):
+    if bool((ids >= V).any()) or bool((ids < 0).any()):
+        raise IndexError(f"token ids must be in [0, {V})")
+
+
+def linear_cross_entropy_dense(hidden, weight, labels, ignore_index=-100, reduction="mean"):
+    live = labels != ignore_index
+    _check_tokens(labels[live], weight.shape[0])
+    rows = torch.where(live.unsqueeze(-1), hidden, 0.0).float()  # rows that do not count may hold anything
+    z = rows @ weight.float().T
+    at = torch.where(live, labels, 0).unsqueeze(-1)
+    loss = torch.logsumexp(z, -1) - z.gather(-1, at).squeeze(-1)
+    return _reduce_rows(torch.where(live, loss, 0.0), live, reduction)
+
+
+def linear_distillation_dense(hidden, weight, teacher_logits, teacher_ids, temperature=1.0, reduction="mean"):
+    if not 0.0 < temperature < math.inf:
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    t = teacher_logits.detach().float() / temperature
+    held = (teacher_ids >= 0) & (t != -math.inf)
+    _check_tokens(teacher_ids[held], weight.shape[0])
+    live = held.any(-1)
+    t = torch.where(held, t, -math.inf)
+    log_p = torch.log_softmax(torch.where(live.unsqueeze(-1), t, 0.0), -1)
+    p = torch.where(held, log_p.exp(), 0.0)
+    rows = torch.where(live.unsqueeze(-1), hidden, 0.0).float()
+    log_q = torch.log_softmax(rows @ weight.float().T / temperature, -1).gather(-1, torch.where(held, teacher_ids, 0))
+    loss = temperature ** 2 * torch.where(p > 0, p * (log_p - log_q), p).sum(-1)
+    return _reduce_rows(torch.where(live, loss, 0.0), live, reduction)
+
+
+def gated_linear_dense(x, w_gate, w_up, activation="silu"):
+    if activation not in ("silu", "gelu"):
+        raise ValueError(f"activation must be 'silu' or 'gelu', got {activation!r}")
+    g, u = x.float() @ w_gate.float().T, x.float() @ w_up.float().T
+    return ((F.silu(g) if activation == "silu" else F.gelu(g)) * u).to(x.dtype)

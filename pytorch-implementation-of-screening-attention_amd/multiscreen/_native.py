@@ -38,6 +38,10 @@ _args = ctypes.c_char_p
 pack_cache_args = struct.Struct("=37q").pack
 pack_tree_args = struct.Struct("=37qd").pack
 pack_verify_args = struct.Struct("=19q").pack
+pack_head_args = struct.Struct("=24qd").pack   # msa_head_args: ends with its temperature
+pack_gated_args = struct.Struct("=19q").pack   # msa_gated_args
+
+HEAD_MAX_K = 256  # MSA_HEAD_MAX_K: a teacher's logits of a row
 
 _SIGS = {
     "msa_version": (_i, []),
@@ -65,6 +69,13 @@ _SIGS = {
     "msa_tree_decode": (_i, [_args, _p]),
     "msa_verify_workspace_bytes": (_sz, [_i, _i, _i64, _i]),
     "msa_verify": (_i, [_args, _p]),
+    "msa_head_state_bytes": (_sz, [_i64, _i64]),
+    "msa_head_workspace_bytes": (_sz, [_args, _i]),
+    "msa_head_fwd": (_i, [_args, _p]),
+    "msa_head_bwd": (_i, [_args, _p]),
+    "msa_gated_workspace_bytes": (_sz, [_args, _i]),
+    "msa_gated_fwd": (_i, [_args, _p]),
+    "msa_gated_bwd": (_i, [_args, _p]),
     "msa_timer_arm": (_i, [_i, _i]),
     "msa_timer_arm_every": (_i, [_i, _i, _i]),
     "msa_timer_read": (_i, [_i, ctypes.POINTER(ctypes.c_float), _i]),

@@ -3,11 +3,14 @@
 Same constructors, submodule names and forward signatures as the reference,
 so state_dicts are interchangeable:
 
-    MultiscreenBlock(d_model, num_heads, ffn_dim=None, dropout=0.0, causal=True)
+    MultiscreenBlock(d_model, num_heads, ffn_dim=None, dropout=0.0, causal=True, ffn="gelu")
         x = x + attn(norm1(x));  x = x + ffn(norm2(x))
-    MultiscreenDecoderLayer(d_model, num_heads, ffn_dim=None, dropout=0.0)
+    MultiscreenDecoderLayer(d_model, num_heads, ffn_dim=None, dropout=0.0, ffn="gelu")
         x = x + self_attn(norm1(x));  x = x + cross_attn(norm2(x), memory)
         x = x + ffn(norm3(x))
+
+ffn="gelu" is the reference's feed-forward; "swiglu" and "geglu" are gated ones
+(GatedFFN), beyond the reference.
 
 MultiscreenBlock additionally exposes prefill, decode and tree steps over a KV
 cache, used by MultiscreenLM.generate and generate_speculative.
@@ -16,10 +19,36 @@ cache, used by MultiscreenLM.generate and generate_speculative.
 import torch
 import torch.nn as nn
 
+from . import ops
+from ._dense import gated_linear_dense
 from .attention import ScreeningAttention
 
+_GATED = {"swiglu": "silu", "geglu": "gelu"}
 
-def _ffn(d_model, ffn_dim, dropout):
+
+class GatedFFN(nn.Module):
+    """down(dropout(act(gate(x)) * up(x))), dropout behind it: both products, the
+    activation and their product are one kernel on the GPU (ops.gated_linear)."""
+
+    def __init__(self, d_model: int, ffn_dim: int, dropout: float = 0.0, activation: str = "silu"):
+        super().__init__()
+        self.gate = nn.Linear(d_model, ffn_dim, bias=False)
+        self.up = nn.Linear(d_model, ffn_dim, bias=False)
+        self.down = nn.Linear(ffn_dim, d_model, bias=False)
+        self.dropout = nn.Dropout(dropout)
+        self.activation = activation
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        gated = ops.gated_linear if x.is_cuda else gated_linear_dense
+        h = gated(x, self.gate.weight, self.up.weight, self.activation)
+        return self.dropout(self.down(self.dropout(h)))
+
+
+def _ffn(d_model, ffn_dim, dropout, kind="gelu"):
+    if kind in _GATED:
+        return GatedFFN(d_model, ffn_dim, dropout, _GATED[kind])
+    if kind != "gelu":
+        raise ValueError(f"ffn must be 'gelu', 'swiglu' or 'geglu', got {kind!r}")
     return nn.Sequential(
         nn.Linear(d_model, ffn_dim, bias=False),
         nn.GELU(),
@@ -31,14 +60,14 @@ def _ffn(d_model, ffn_dim, dropout):
 
 class MultiscreenBlock(nn.Module):
     def __init__(self, d_model: int, num_heads: int, ffn_dim: int | None = None,
-                 dropout: float = 0.0, causal: bool = True):
+                 dropout: float = 0.0, causal: bool = True, ffn: str = "gelu"):
         super().__init__()
         ffn_dim = ffn_dim or 4 * d_model
         self.norm1 = nn.RMSNorm(d_model)
         self.norm2 = nn.RMSNorm(d_model)
         self.attn = ScreeningAttention(d_model=d_model, num_heads=num_heads, dropout=dropout,
                                        causal=causal)
-        self.ffn = _ffn(d_model, ffn_dim, dropout)
+        self.ffn = _ffn(d_model, ffn_dim, dropout, ffn)
 
     def forward(self, x: torch.Tensor, key_padding_mask: torch.Tensor | None = None) -> torch.Tensor:
         normed = self.norm1(x)
@@ -67,7 +96,7 @@ class MultiscreenBlock(nn.Module):
 
 class MultiscreenDecoderLayer(nn.Module):
     def __init__(self, d_model: int, num_heads: int, ffn_dim: int | None = None,
-                 dropout: float = 0.0):
+                 dropout: float = 0.0, ffn: str = "gelu"):
         super().__init__()
         ffn_dim = ffn_dim or 4 * d_model
         self.norm1 = nn.RMSNorm(d_model)
@@ -77,7 +106,7 @@ class MultiscreenDecoderLayer(nn.Module):
                                             causal=True)
         self.cross_attn = ScreeningAttention(d_model=d_model, num_heads=num_heads, dropout=dropout,
                                              causal=False)
-        self.ffn = _ffn(d_model, ffn_dim, dropout)
+        self.ffn = _ffn(d_model, ffn_dim, dropout, ffn)
 
     def forward(self, x: torch.Tensor, memory: torch.Tensor,
                 tgt_key_padding_mask: torch.Tensor | None = None,

@@ -7,12 +7,16 @@ an un-shifted cross-entropy with ignore_index=-100, model.py:101-106) and
 generate() signature and sampling (temperature, optional top-k, multinomial,
 model.py:111-141).
 
+Beyond the reference: loss() and distillation_loss() train without forming the
+logits, top_logits() is what a teacher passes to the latter, and ffn="swiglu" or
+"geglu" takes gated feed-forwards.
+
 generate() differs only in cost: instead of re-running forward() over the
 whole prefix for every new token, it prefills a per-layer KV cache once and
 then runs one single-query decode step per token (the HIP decode kernel on
 GPU), which computes the same last-position logits.
 
-Beyond the reference: caches of 8-bit rows (cache_dtype=torch.int8 or
+Also beyond the reference: caches of 8-bit rows (cache_dtype=torch.int8 or
 torch.float8_e4m3fn), steps over several tokens or a tree of drafts at once
 (tree_step, accept) and generation with a smaller model that drafts
 (generate_speculative).
@@ -25,7 +29,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import ops
-from ._dense import tree_relations, verify_dense
+from ._dense import linear_cross_entropy_dense, linear_distillation_dense, tree_relations, verify_dense
 from .attention import KVCache
 from .layers import MultiscreenBlock
 
@@ -33,7 +37,7 @@ from .layers import MultiscreenBlock
 class MultiscreenLM(nn.Module):
     def __init__(self, vocab_size: int, d_model: int = 512, num_heads: int = 8, num_layers: int = 6,
                  ffn_dim: int | None = None, max_seq_len: int = 2048, dropout: float = 0.0,
-                 tie_weights: bool = True):
+                 tie_weights: bool = True, ffn: str = "gelu"):
         super().__init__()
         self.d_model = d_model
         self.token_emb = nn.Embedding(vocab_size, d_model)
@@ -41,7 +45,7 @@ class MultiscreenLM(nn.Module):
         self.emb_dropout = nn.Dropout(dropout)
         self.blocks = nn.ModuleList([
             MultiscreenBlock(d_model=d_model, num_heads=num_heads, ffn_dim=ffn_dim, dropout=dropout,
-                             causal=True)
+                             causal=True, ffn=ffn)
             for _ in range(num_layers)
         ])
         self.norm = nn.RMSNorm(d_model)
@@ -77,15 +81,49 @@ class MultiscreenLM(nn.Module):
         Returns:
             {'logits': (B, T, vocab)} plus 'loss' when labels are given.
         """
-        x = self.embed(input_ids)
-        for block in self.blocks:
-            x = block(x, key_padding_mask=key_padding_mask)
-        logits = self.lm_head(self.norm(x))
+        logits = self.lm_head(self.hidden_states(input_ids, key_padding_mask))
         result = {"logits": logits}
         if labels is not None:
             result["loss"] = F.cross_entropy(logits.view(-1, logits.size(-1)), labels.view(-1),
                                              ignore_index=-100)
         return result
+
+    def hidden_states(self, input_ids: torch.Tensor, key_padding_mask: torch.Tensor | None = None) -> torch.Tensor:
+        """The head's input (B, T, d_model): forward() without lm_head."""
+        x = self.embed(input_ids)
+        for block in self.blocks:
+            x = block(x, key_padding_mask=key_padding_mask)
+        return self.norm(x)
+
+    def loss(self, input_ids: torch.Tensor, labels: torch.Tensor, key_padding_mask: torch.Tensor | None = None,
+             reduction: str = "mean") -> torch.Tensor:
+        """forward()'s loss (un-shifted, -100 ignored) without its (B, T, vocab) logits
+        (ops.linear_cross_entropy).  float32; reduction "none": (B, T), each token's
+        score with its sign changed."""
+        fn = ops.linear_cross_entropy if input_ids.is_cuda else linear_cross_entropy_dense
+        return fn(self.hidden_states(input_ids, key_padding_mask), self.lm_head.weight, labels, -100, reduction)
+
+    def distillation_loss(self, input_ids: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
+                          temperature: float = 1.0, key_padding_mask: torch.Tensor | None = None,
+                          reduction: str = "mean") -> torch.Tensor:
+        """Divergence from a teacher of the same vocabulary that gave teacher_logits,
+        teacher_ids (B, T, K) = teacher.top_logits(input_ids, K): what a drafting model
+        learns for generate_speculative (ops.linear_distillation).  Positions whose ids
+        are all -1 do not count."""
+        fn = ops.linear_distillation if input_ids.is_cuda else linear_distillation_dense
+        return fn(self.hidden_states(input_ids, key_padding_mask), self.lm_head.weight, teacher_logits, teacher_ids,
+                  temperature, reduction)
+
+    @torch.no_grad()
+    def top_logits(self, input_ids: torch.Tensor, k: int, key_padding_mask: torch.Tensor | None = None):
+        """The k largest logits of each position and their tokens, (B, T, k) each; 1024
+        positions' logits exist at a time."""
+        rows = self.hidden_states(input_ids, key_padding_mask).flatten(0, 1)
+        parts = [self.lm_head(x).topk(k, -1) for x in rows.split(1024)]
+        if not parts:
+            parts = [self.lm_head(rows).topk(k, -1)]
+        values, ids = (torch.cat(p).view(*input_ids.shape, k) for p in zip(*parts))
+        return values, ids
 
     def new_cache(self, batch: int, capacity: int, dtype: torch.dtype, device) -> list:
         """One KVCache per block.  Each carries its layer's widest window

@@ -19,6 +19,7 @@ GPU tensors only: a CPU tensor, or a missing libmsa.so, raises.
 """
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -536,3 +537,220 @@ def verify_drafts(target, tokens, parents=None, uniforms=None, draft=None):
                                      path.data_ptr(), count.data_ptr(), token.data_ptr(),
                                      workspace.data_ptr() if need else 0, need, B, M, V, _DTYPES[dtype]))
     return path, count, token
+
+
+# ---------------------------------------------------------------------------
+# The wide products of a language model: the vocabulary head's losses, straight
+# from its input, and the gated feed-forward.
+# ---------------------------------------------------------------------------
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+_ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def _autocast(*tensors):
+    """The tensors in autocast's type where it is on for the GPU, as torch's linear layers take them."""
+    if torch.is_autocast_enabled("cuda") and tensors[0].is_cuda:
+        dtype = torch.get_autocast_dtype("cuda")
+        if dtype in _DTYPES:
+            return tuple(x.to(dtype) for x in tensors)
+    return tensors
+
+
+def _rows_2d(x):
+    """x (..., n) as rows with unit stride: the 2-D tensor, its pointer and its row stride."""
+    x = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if x.stride(1) != 1 and x.shape[1] > 1:
+        x = x.contiguous()
+    return x, x.data_ptr(), x.stride(0)
+
+
+def _head_checks(what, hidden, weight, reduction, *others):
+    index = hidden.get_device()
+    _one_gpu(what, index, weight, *others)
+    if hidden.dtype not in _DTYPES or weight.dtype != hidden.dtype:
+        raise TypeError(f"{what}: hidden and weight must share dtype float32, bfloat16 or float16, got {hidden.dtype}, "
+                        f"{weight.dtype}")
+    if hidden.dim() < 1 or weight.dim() != 2 or weight.shape[1] != hidden.shape[-1] or 0 in weight.shape:
+        raise ValueError(f"{what}: hidden (..., d) and weight (V, d) expected, got {tuple(hidden.shape)}, "
+                         f"{tuple(weight.shape)}")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"{what}: reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
+
+
+def _head_args(hidden, weight, ids, teacher, temperature, ignore_index, reduction, state, loss, dloss, dhidden, dweight,
+               workspace=None):
+    """msa_head_args of 2-D hidden (N, d), ids (N, K) and teacher (N, K) or None."""
+    N, K = ids.shape
+    V, d = weight.shape
+
+    def at(x):
+        return 0 if x is None else x.data_ptr()
+
+    return _native.pack_head_args(
+        hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), ids.data_ptr(), ids.stride(0),
+        at(teacher), 0 if teacher is None else teacher.stride(0), at(state), 0 if state is None else state.numel(),
+        at(loss), at(dloss), at(dhidden), at(dweight), at(workspace), 0 if workspace is None else workspace.numel(),
+        N, d, V, K, _DTYPES[hidden.dtype], 0 if teacher is None else _DTYPES[teacher.dtype], _REDUCTIONS[reduction],
+        ignore_index, temperature)
+
+
+def _head_call(what, fn, index, backward, *args):
+    L = _native.lib()
+    need = L.msa_head_workspace_bytes(_head_args(*args), backward)
+    workspace = torch.empty((need,), dtype=torch.uint8, device=args[0].device)
+    _launch(what, fn, index, _head_args(*args, workspace))
+
+
+class _HeadLoss(torch.autograd.Function):
+    """forward = msa_head_fwd, backward = msa_head_bwd, on 2-D rows."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, ids, teacher, temperature, ignore_index, reduction):
+        L = _native.lib()
+        N, K = ids.shape
+        dev = hidden.device
+        state = torch.empty((L.msa_head_state_bytes(N, K),), dtype=torch.uint8, device=dev)
+        loss = torch.empty((N,) if reduction == "none" else (), dtype=torch.float32, device=dev)
+        _head_call("msa_head_fwd", L.msa_head_fwd, hidden.get_device(), 0, hidden, weight, ids, teacher, temperature,
+                   ignore_index, reduction, state, loss, None, None, None)
+        if any(ctx.needs_input_grad[:2]):
+            ctx.save_for_backward(hidden, weight, ids, teacher, state)
+            ctx.options = temperature, ignore_index, reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        hidden, weight, ids, teacher, state = ctx.saved_tensors
+        dloss = dloss.to(torch.float32).contiguous()
+        dh = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if ctx.needs_input_grad[0] else None
+        dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if ctx.needs_input_grad[1] else None
+        # the pass keeps scales in the state's header: one of its own, so that two passes may run at once
+        _head_call("msa_head_bwd", _native.lib().msa_head_bwd, hidden.get_device(), 1, hidden, weight, ids, teacher,
+                   *ctx.options, state.clone(), None, dloss, dh, dw)
+        return dh, dw, None, None, None, None, None
+
+
+def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="mean"):
+    """Cross entropy of the logits hidden @ weight.T without the logits.
+
+    hidden (..., d), weight (V, d) float32, bfloat16 or float16 of one type
+    (autocast's under it); labels (...) int64.  Rows whose label is ignore_index
+    do not count: their loss and gradient are 0, whatever hidden holds there.
+    Other labels outside [0, V) give NaN.
+    reduction "mean" (over the rows that count; NaN if none does), "sum", or
+    "none": a loss per row, shaped as labels, of which N = 1 and a few rows are the
+    scores of a decoding step.  float32; sums and softmax statistics are too.
+    The backward pass forms the logits again, in pieces of the vocabulary of at
+    most 256 MB; their gradient is rounded to hidden's type (float32: 22 bits).
+    """
+    hidden, weight = _autocast(hidden, weight)
+    _head_checks("linear_cross_entropy", hidden, weight, reduction, labels)
+    if labels.dtype != torch.int64 or labels.shape != hidden.shape[:-1]:
+        raise ValueError(f"linear_cross_entropy: labels must be int64 {tuple(hidden.shape[:-1])}, got {labels.dtype} "
+                         f"{tuple(labels.shape)}")
+    ids = labels.reshape(-1, 1)
+    loss = _HeadLoss.apply(_rows_2d(hidden)[0], _rows_2d(weight)[0], ids, None, 1.0, int(ignore_index), reduction)
+    return loss.view(labels.shape) if reduction == "none" else loss
+
+
+def linear_distillation(hidden, weight, teacher_logits, teacher_ids, temperature=1.0, reduction="mean"):
+    """Divergence of the softmax of hidden @ weight.T from a teacher's, of which
+    each row holds its largest logits, without the logits:
+
+        p = softmax(teacher_logits / T) over the row's entries
+        q = softmax(hidden @ weight.T / T) over the vocabulary
+        loss = T^2 sum_k p_k (log p_k - log q[teacher_ids_k])
+
+    hidden (..., d), weight (V, d) as in linear_cross_entropy; teacher_logits
+    (..., K) float32, bfloat16 or float16, teacher_ids (..., K) int64, 1 <= K <=
+    256 (MultiscreenLM.top_logits).  An entry with a negative id or a logit of -inf
+    is none; rows without an entry do not count.  An id named twice is two entries;
+    ids of V and above give NaN.  reduction as in linear_cross_entropy.  No gradient
+    flows to the teacher.
+    """
+    hidden, weight = _autocast(hidden, weight)
+    _head_checks("linear_distillation", hidden, weight, reduction, teacher_logits, teacher_ids)
+    shape = teacher_ids.shape
+    if teacher_ids.dtype != torch.int64 or len(shape) < 1 or shape[:-1] != hidden.shape[:-1]:
+        raise ValueError(f"linear_distillation: teacher_ids must be int64 ({tuple(hidden.shape[:-1])}, K), got "
+                         f"{teacher_ids.dtype} {tuple(shape)}")
+    if teacher_logits.dtype not in _DTYPES or teacher_logits.shape != shape:
+        raise TypeError(f"linear_distillation: teacher_logits must be float32, bfloat16 or float16 {tuple(shape)}, got "
+                        f"{teacher_logits.dtype} {tuple(teacher_logits.shape)}")
+    if not 1 <= shape[-1] <= _native.HEAD_MAX_K:
+        raise ValueError(f"linear_distillation: a row holds 1 to {_native.HEAD_MAX_K} teacher logits, got {shape[-1]}")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"linear_distillation: temperature must be positive and finite, got {temperature}")
+    loss = _HeadLoss.apply(_rows_2d(hidden)[0], _rows_2d(weight)[0], _rows_2d(teacher_ids)[0],
+                           _rows_2d(teacher_logits.detach())[0], float(temperature), 0, reduction)
+    return loss.view(shape[:-1]) if reduction == "none" else loss
+
+
+def _gated_args(x, gate, up, act, h, dh, dx, dgate, dup, workspace=None):
+    N, d = x.shape
+
+    def at(t):
+        return 0 if t is None else t.data_ptr()
+
+    return _native.pack_gated_args(
+        x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0), up.data_ptr(), up.stride(0), at(h), at(dh),
+        0 if dh is None else dh.stride(0), at(dx), at(dgate), at(dup), at(workspace),
+        0 if workspace is None else workspace.numel(), N, d, gate.shape[0], _DTYPES[x.dtype], act)
+
+
+def _gated_call(what, fn, backward, *args):
+    x = args[0]
+    need = _native.lib().msa_gated_workspace_bytes(_gated_args(*args), backward)
+    workspace = torch.empty((need,), dtype=torch.uint8, device=x.device)
+    _launch(what, fn, x.get_device(), _gated_args(*args, workspace))
+
+
+class _GatedLinear(torch.autograd.Function):
+    """forward = msa_gated_fwd, backward = msa_gated_bwd, on 2-D rows."""
+
+    @staticmethod
+    def forward(ctx, x, gate, up, act):
+        h = torch.empty((x.shape[0], gate.shape[0]), dtype=x.dtype, device=x.device)
+        _gated_call("msa_gated_fwd", _native.lib().msa_gated_fwd, 0, x, gate, up, act, h, None, None, None, None)
+        if any(ctx.needs_input_grad[:3]):
+            ctx.save_for_backward(x, gate, up)
+            ctx.act = act
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        x, gate, up = ctx.saved_tensors
+        dh = _rows_2d(dh)[0]
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[0] else None
+        dgate = dup = None
+        if any(ctx.needs_input_grad[1:3]):
+            dgate, dup = (torch.empty(gate.shape, dtype=x.dtype, device=x.device) for _ in range(2))
+        _gated_call("msa_gated_bwd", _native.lib().msa_gated_bwd, 1, x, gate, up, ctx.act, None, dh, dx, dgate, dup)
+        return dx, dgate if ctx.needs_input_grad[1] else None, dup if ctx.needs_input_grad[2] else None, None
+
+
+def gated_linear(x, w_gate, w_up, activation="silu"):
+    """act(x @ w_gate.T) * (x @ w_up.T), the first half of a gated feed-forward, in
+    one kernel: neither product is written.
+
+    x (..., d), w_gate and w_up (F, d) float32, bfloat16 or float16 of one type
+    (autocast's under it); activation "silu" or "gelu" (the exact one, by erf).
+    Returns (..., F); activation and product are taken in float32 and rounded once.
+    The backward pass forms both products again; their gradients are rounded to
+    x's type (float32: 22 bits), sums are float32.
+    """
+    x, w_gate, w_up = _autocast(x, w_gate, w_up)
+    _one_gpu("gated_linear", x.get_device(), w_gate, w_up)
+    if x.dtype not in _DTYPES or w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
+        raise TypeError(f"gated_linear: x, w_gate and w_up must share dtype float32, bfloat16 or float16, got {x.dtype}, "
+                        f"{w_gate.dtype}, {w_up.dtype}")
+    if x.dim() < 1 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_gate.shape[1] != x.shape[-1] \
+            or 0 in w_gate.shape:
+        raise ValueError(f"gated_linear: x (..., d), w_gate and w_up (F, d) expected, got {tuple(x.shape)}, "
+                         f"{tuple(w_gate.shape)}, {tuple(w_up.shape)}")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"gated_linear: activation must be 'silu' or 'gelu', got {activation!r}")
+    h = _GatedLinear.apply(_rows_2d(x)[0], _rows_2d(w_gate)[0], _rows_2d(w_up)[0], _ACTIVATIONS[activation])
+    return h.view(*x.shape[:-1], w_gate.shape[0])
