@@ -59,13 +59,20 @@ struct MmTile {
   static constexpr int NWAVES = WM * WN;
   static constexpr int AI = ABYTES / 1024 / NWAVES, BI = BBYTES / 1024 / NWAVES;  // copies of 1 KiB a wave issues
   static_assert(AI * NWAVES * 1024 == ABYTES && BI * NWAVES * 1024 == BBYTES, "a stage is whole copies of every wave");
+  static_assert(MB <= 4 && NB <= 4, "blocks are found by two address bits");
   static_assert(!DUAL || (!AMN && NWAVES == 4 && BM % 128 == 0), "alternating rows are laid out for four waves");
 
   typedef f32x16 Acc[MB][NB];
 
-  // One operand's copies.  K-contiguous: rows of 64 bytes, a copy is 16 rows; the 16-byte chunks of row R are
-  // XOR-swizzled by (R >> 1) & 3.  Otherwise: k rows of W columns; chunks are swizzled by (k & 3) << 1, so that the
-  // four rows that a transposed read takes lie in different banks.
+  // Places of 16-byte chunks are XOR-swizzled so that reads are free of bank conflicts whether the LDS serves 128 or 256
+  // bytes a cycle.  K-contiguous rows R of 4 chunks: by (b1 ^ b3, b2) of R, one-to-one on rows 0, 2, 4, 6 (which
+  // share a half of 128 bytes) and on 0, 4, 8, 12 (a quarter of 256).  k rows of the other order: a transposed read
+  // takes 4 neighbours k at 2 chunks (128 bytes) or 4 (256): by bits 1 to 3 (k1, k0, k1).  (With half of the banks at
+  // a time in mind only, half of all LDS cycles were conflicts.)
+  __device__ static constexpr int swz_row(int R) { return (((R >> 1) ^ (R >> 3)) & 1) | (((R >> 2) & 1) << 1); }
+  __device__ static constexpr int swz_k(int k) { return ((k & 2) * 5) | ((k & 1) << 2); }
+
+  // One operand's copies.  K-contiguous: rows of 64 bytes, a copy is 16 rows.  Otherwise: k rows of W columns.
   template <bool MN, int W, int NI, bool ALT>
   struct Loader {
     uint32_t off[NI];
@@ -79,7 +86,7 @@ struct MmTile {
       ld = (uint32_t)stride_bytes;
       rows = krows;
       if constexpr (!MN) {
-        const int lr = lane >> 2, chunk = (lane & 3) ^ ((lane >> 3) & 3);
+        const int lr = lane >> 2, chunk = (lane & 3) ^ swz_row(lr);
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
           int r = ALT ? (j >> 1) * 64 + 16 * wave + lr : (j * NWAVES + wave) * 16 + lr;
@@ -91,7 +98,7 @@ struct MmTile {
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
           const int p = (j * NWAVES + wave) * 64 + lane, k = p / CPR;
-          int col = ((p % CPR) ^ ((k & 3) << 1)) * 8;
+          int col = ((p % CPR) ^ swz_k(k)) * 8;
           col = col < count ? col : count - 8;  // count is a multiple of 8
           off[j] = (uint32_t)k * ld + (uint32_t)col * 2u;
         }
@@ -131,10 +138,10 @@ struct MmTile {
       const int half = lane >> 5;
       if constexpr (!MN) {
         const int R = lane & 31;
-        at = (uint32_t)((first + R) * 64 + ((half ^ ((R >> 1) & 3)) << 4));
+        at = (uint32_t)((first + R) * 64 + ((half ^ swz_row(R)) << 4));
       } else {
         const int kk = (lane & 15) >> 2, q = lane & 3, gg = (lane >> 4) & 1;
-        at = (uint32_t)((8 * half + kk) * (W * 2) + first * 2 + (((2 * gg + (q >> 1)) ^ (kk << 1)) << 4) + 8 * (q & 1));
+        at = (uint32_t)((8 * half + kk) * (W * 2) + (((first / 8 + 2 * gg + (q >> 1)) ^ swz_k(kk)) << 4) + 8 * (q & 1));
       }
     }
     __device__ inline frag read(const LdsChar* tile, int i, int c) const {
@@ -146,7 +153,7 @@ struct MmTile {
         s16x8 v;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const LdsChar* p = tile + (at ^ (uint32_t)((i & 1) << 6)) + (i >> 1) * 128 + (16 * c + 4 * j) * (W * 2);
+          const LdsChar* p = tile + (at ^ (uint32_t)(i << 6)) + (16 * c + 4 * j) * (W * 2);  // `first` is a multiple of 32 times the wave's blocks, which are at most 4
           const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)const_cast<LdsChar*>(p));
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[4 * j + e] = x[e];
@@ -205,49 +212,67 @@ struct MmTile {
     };
     int filled = 0;
 #pragma unroll
-    for (int u = 0; u < NST - 1; ++u)
+    for (int u = 0; u < NST; ++u)
       if (u < total) { issue(u); ++filled; }
     const int low = steps * segs.low;
-    int rs = 0, ws = NST - 1;
-    for (int t = 0; t < total; ++t) {
-      // stage t has landed once only the younger ones are outstanding
-      if (filled - t > NST - 2) arrive<(NST - 2) * (AI + BI)>();
-      else if (NST > 3 && filled - t == NST - 2) arrive<(NST > 3 ? NST - 3 : 0) * (AI + BI)>();
+    frag a[2][MB], b[2][NB];
+    auto fetch = [&](int slot, auto C) {  // fragments of half C of a landed stage
+      constexpr int c = decltype(C)::value;
+      const LdsChar* at = lds + slot * STAGE;
+#pragma unroll
+      for (int i = 0; i < MB; ++i) a[c][i] = ra.read(at, i, c);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) b[c][j] = rb.read(at + ABYTES, j, c);
+    };
+    auto multiply = [&](auto C) {
+      constexpr int c = decltype(C)::value;
+      // MB * NB independent sums: an accumulator comes again only after all the others, so no MFMA waits for the
+      // one before it and none reads its operands late (see the source-operand guard in msa_device.h)
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = M::mma_ng(a[c][i], b[c][j], acc[i][j]);
+      if constexpr (MB * NB < 4) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int j = 0; j < NB; ++j) asm volatile(MSA_NOP16 : "+v"(a[c][i]), "+v"(b[c][j]));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    typedef std::integral_constant<int, 0> First;
+    typedef std::integral_constant<int, 1> Second;
+    if (filled == NST) arrive<(NST - 1) * (AI + BI)>();
+    else arrive<0>();
+    fetch(0, First());
+    fetch(0, Second());
+    auto scale_low = [&]() {
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] *= kLowTerm;
+    };
+    int slot = 0;  // of stage t
+    for (int t = 0; t < total - 1; ++t) {
+      if (low != 0 && t == low) scale_low();
+      multiply(First());
+      // Between the halves: stage t + 1 has landed once only the younger ones are outstanding, and every wave holds the
+      // fragments of stage t, so its slot takes the next copy.
+      if (filled - t >= NST) arrive<(NST - 2) * (AI + BI)>();
       else arrive<0>();
-      if (filled < total) { issue(ws); ++filled; }
-      const LdsChar* at = lds + rs * STAGE;
-      const LdsChar* bt = at + ABYTES;
-      rs = rs + 1 == NST ? 0 : rs + 1;
-      ws = ws + 1 == NST ? 0 : ws + 1;
-      if (low != 0 && t == low) {
-#pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int j = 0; j < NB; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] *= kLowTerm;
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        frag a[MB], b[NB];
-#pragma unroll
-        for (int i = 0; i < MB; ++i) a[i] = ra.read(at, i, c);
-#pragma unroll
-        for (int j = 0; j < NB; ++j) b[j] = rb.read(bt, j, c);
-        // MB * NB independent sums: an accumulator comes again only after all the others, so no MFMA waits for the
-        // one before it and none reads its operands late (see the source-operand guard in msa_device.h)
-#pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int j = 0; j < NB; ++j) acc[i][j] = M::mma_ng(a[i], b[j], acc[i][j]);
-        if constexpr (MB * NB < 4) {
-#pragma unroll
-          for (int i = 0; i < MB; ++i)
-#pragma unroll
-            for (int j = 0; j < NB; ++j) asm volatile(MSA_NOP16 : "+v"(a[i]), "+v"(b[j]));
-        }
-      }
+      if (filled < total) { issue(slot); ++filled; }
+      slot = slot + 1 == NST ? 0 : slot + 1;
+      fetch(slot, First());
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(Second());
+      fetch(slot, Second());
+      __builtin_amdgcn_sched_barrier(0);
     }
+    if (low != 0 && total - 1 == low) scale_low();
+    multiply(First());
+    multiply(Second());
     arrive<0>();
   }
 

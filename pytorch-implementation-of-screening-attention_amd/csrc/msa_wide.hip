@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, 2) products_kernel(ProductArgs p) {
     TX::clear(acc);
     const typename TX::Side A{p.w + (int64_t)m0 * 2, (int)(p.dp - m0), p.w_ld, p.w_rows, 0};
     const typename TX::Side B{p.g + (int64_t)n0 * p.C * 2, (int)(p.n_pad - n0), p.C * 2, 0, 0};
-    TX::run(acc, lds, A, B, p.dx_segs, from * 32, to - from);
+    if (to > from) TX::run(acc, lds, A, B, p.dx_segs, from * 32, to - from);
     float* out = p.dx_part + ((int64_t)split * p.n_pad + n0) * p.dp + m0;
     auto fn = [&](int i, int j, int g) { return quad<float>([&](int e) { return acc[i][j][4 * g + e]; }); };
     const int rows = (int)(N - n0 < 128 ? N - n0 : 128);
