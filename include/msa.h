@@ -391,9 +391,8 @@ int msa_verify(const msa_verify_args* args, void* stream);
  * A row that counts and names a token outside [0, V) has loss NaN and gradient
  * NaN.  Rows that do not count are not read beyond their ids (and teacher): their
  * hidden may hold anything, and their gradient is 0.
- * msa_head_bwd takes the same arguments, state as msa_head_fwd left it (its pass
- * only writes the header's scales there) and dloss, fp32: (N) for reduction 0,
- * one value else.  dhidden (N, d) and dweight (V, d) contiguous, of type dtype;
+ * msa_head_bwd takes the same arguments, state as msa_head_fwd left it (read
+ * only) and dloss, fp32: (N) for reduction 0, one value else.  dhidden (N, d) and dweight (V, d) contiguous, of type dtype;
  * either may be null.  The gradient of the logits is formed in pieces of the
  * vocabulary, rounded to dtype (fp32: to two fp16 terms, 22 bits) and multiplied
  * with fp32 sums.

@@ -173,7 +173,7 @@ struct GatedPlan {
     char* p = (char*)c.workspace;
     size_t o = 0;
     auto take = [&](int64_t bytes) { char* q = p + o; o += (size_t)round_up(bytes, 256); return q; };
-    hdr = (WideHdr*)take(256);
+    hdr = (WideHdr*)take(sizeof(WideHdr));
     x = direct(c, c.x, c.x_ld) ? nullptr : take(planes * x_plane);
     w = direct(c, c.w[0], c.w_ld[0]) && direct(c, c.w[1], c.w_ld[1]) && c.w_ld[0] == c.w_ld[1] ? nullptr : take(2 * planes * w_plane);
     C = g_plane = 0;
@@ -201,25 +201,20 @@ struct GatedPlan {
 struct GatedOperands { const char *x, *w[2]; int64_t x_ld, w_ld; int x_rows; MmSegs segs; };
 
 hipError_t operands(const GatedCall& c, const GatedPlan& p, int backward, GatedOperands* o) {
-  RowsCopy x{c.x, c.x_ld, c.N, c.d, c.dtype, p.x, p.x_plane, nullptr, p.hdr, 0};
-  RowsCopy w[2];
+  RowsCopies all = {}, copies = {};
+  all.dtype = copies.dtype = c.dtype;
+  all.hdr = copies.hdr = p.hdr;
+  all.add(RowsCopy{c.x, c.x_ld, c.N, c.d, p.x, p.x_plane, nullptr, 0, backward});
   for (int i = 0; i < 2; ++i)
-    w[i] = RowsCopy{c.w[i], c.w_ld[i], c.F, c.d, c.dtype, p.w + (p.w == nullptr ? 0 : i * p.planes * p.w_plane), p.w_plane, nullptr, p.hdr, 1};
+    all.add(RowsCopy{c.w[i], c.w_ld[i], c.F, c.d, p.w + (p.w == nullptr ? 0 : i * p.planes * p.w_plane), p.w_plane, nullptr, 1, backward});
+  if (p.x != nullptr) copies.add(all.m[0]);
+  if (p.w != nullptr) { copies.add(all.m[1]); copies.add(all.m[2]); }
   if (p.planes == 2 || (backward && c.dtype == 2)) {  // scales of the operands, and of dg and du
+    if (backward) all.add(RowsCopy{c.dh, c.dh_ld, c.N, c.F, nullptr, 0, nullptr, 2, 0});
     GATED_TRY(launch_hdr_clear(p.hdr, c.stream));
-    GATED_TRY(launch_rows_max(x, backward, c.stream));
-    GATED_TRY(launch_rows_max(w[0], backward, c.stream));
-    GATED_TRY(launch_rows_max(w[1], backward, c.stream));
-    if (backward) {
-      const RowsCopy dh{c.dh, c.dh_ld, c.N, c.F, c.dtype, nullptr, 0, nullptr, p.hdr, 2};
-      GATED_TRY(launch_rows_max(dh, 0, c.stream));
-    }
+    GATED_TRY(launch_rows_max(all, c.stream));
   }
-  if (p.x != nullptr) GATED_TRY(launch_rows_copy(x, c.stream));
-  if (p.w != nullptr) {
-    GATED_TRY(launch_rows_copy(w[0], c.stream));
-    GATED_TRY(launch_rows_copy(w[1], c.stream));
-  }
+  if (copies.n > 0) GATED_TRY(launch_rows_copy(copies, c.stream));
   o->x = p.x != nullptr ? p.x : (const char*)c.x;
   o->x_ld = p.x != nullptr ? p.dp * 2 : c.x_ld * 2;
   o->x_rows = (int)c.N;
@@ -296,11 +291,11 @@ hipError_t gated_bwd(const GatedCall& c) {
     q.w_ld = o.w_ld; q.w_plane = p.w_plane; q.w_rows = (int)(c.F - f0);
     q.g = p.g; q.g_plane = p.g_plane; q.g_half = p.planes * p.g_plane;
     q.dx_part = p.dx_part; q.dx_add = f0 > 0; q.dw_part = p.dw_part;
-    q.dx_split = p.dx_split; q.dw_split = p.dw_split; q.hdr = p.hdr; q.use_live = 0;
+    q.dx_split = p.dx_split; q.dw_split = p.dw_split; q.hdr = p.hdr; q.unit.mode = 3; q.use_live = 0;
     GATED_TRY(launch_wide_products(q, c.stream));
   }
   if (c.dx != nullptr) {
-    const WideFinish f{c.dtype, 1, c.N, p.n_pad, c.d, p.dp, p.dx_split, p.dx_part, nullptr, p.hdr, c.dx};
+    const WideFinish f{c.dtype, 1, c.N, p.n_pad, c.d, p.dp, p.dx_split, p.dx_part, nullptr, p.hdr, GradUnit{nullptr, 1.0f, 3}, nullptr, c.dx};
     GATED_TRY(launch_wide_finish(f, c.stream));
   }
   return hipSuccess;

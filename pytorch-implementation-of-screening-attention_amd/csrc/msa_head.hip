@@ -27,7 +27,7 @@ struct HeadState {
   size_t bytes;
   HeadState(void* p, int64_t N, int K) {
     char* c = (char*)p;
-    size_t o = 256;
+    size_t o = (size_t)round_up(sizeof(WideHdr), 256);
     hdr = (WideHdr*)c;
     pos = (int*)(c + o); o += (size_t)round_up(N * 4, 256);
     lse2 = (float*)(c + o); o += (size_t)round_up(round_up(N, 128) * 4, 256);
@@ -39,30 +39,37 @@ struct HeadState {
 // ---------------------------------------------------------------------------
 // Which rows count
 // ---------------------------------------------------------------------------
-// One block: pos[n] = how many rows before n count, or -1.  A thread takes neighbouring rows twice: to count and to
-// number them.  32768 rows take about 10 us beside products of milliseconds.
+// One block: pos[n] = how many rows before n count, or -1.  A thread takes up to 64 neighbouring rows at a time and keeps
+// which count as bits; 65536 rows are one round.
 template <typename Fn>
 __device__ inline int number_rows(int64_t N, int* pos, Fn counts) {
   __shared__ int sums[16];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t per = (N + 1023) / 1024, from = tid * per, to = from + per < N ? from + per : N;
-  int c = 0;
-  for (int64_t n = from; n < to; ++n) c += counts(n) ? 1 : 0;
-  int incl = c;
+  const int per = (int)(N >= 65536 ? 64 : (N + 1023) / 1024);
+  int total = 0;
+  for (int64_t base = 0; base < N; base += (int64_t)per * 1024) {
+    const int64_t from = base + (int64_t)tid * per;
+    const int here = from >= N ? 0 : (int)(N - from < per ? N - from : per);
+    unsigned long long bits = 0;
+#pragma unroll 8
+    for (int i = 0; i < here; ++i) bits |= (unsigned long long)(counts(from + i) ? 1 : 0) << i;
+    const int c = __popcll(bits);
+    int incl = c;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int v = __shfl_up(incl, o);
-    if (lane >= o) incl += v;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(incl, o);
+      if (lane >= o) incl += v;
+    }
+    __syncthreads();
+    if (lane == 63) sums[wave] = incl;
+    __syncthreads();
+    int at = total + incl - c;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) at += sums[w];
+      total += sums[w];
+    }
+    for (int i = 0; i < here; ++i) pos[from + i] = (bits >> i) & 1 ? at++ : -1;
   }
-  if (lane == 63) sums[wave] = incl;
-  __syncthreads();
-  int before = 0, total = 0;
-  for (int w = 0; w < 16; ++w) {
-    if (w < wave) before += sums[w];
-    total += sums[w];
-  }
-  int at = before + incl - c;
-  for (int64_t n = from; n < to; ++n) pos[n] = counts(n) ? at++ : -1;
   return total;
 }
 
@@ -70,11 +77,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const int64_t* ids, int64_t 
                                                     const uint8_t* live, int64_t N, int* pos, WideHdr* hdr) {
   const int total = live != nullptr ? number_rows(N, pos, [&](int64_t n) { return live[n] != 0; })
                                     : number_rows(N, pos, [&](int64_t n) { return ids[n * ids_ld] != ignore; });
-  if (threadIdx.x == 0) {
-    *hdr = WideHdr{};
-    hdr->live = total;
-    hdr->cmax = 1.0f;
-  }
+  for (int i = (int)threadIdx.x; i < kHdrWords; i += 1024) reinterpret_cast<uint32_t*>(hdr)[i] = i == 0 ? (uint32_t)total : 0u;
 }
 
 // A teacher's record of a row: entries with an id >= 0 and a logit above -inf; p = their softmax at 1/T.  A wave per
@@ -213,8 +216,9 @@ __global__ void __launch_bounds__(kThreads, 2) stats_kernel(StatsArgs a) {
 
 // ---------------------------------------------------------------------------
 // A row's sum over the tiles, its targets' logits and its loss.  A block takes 8 rows: first 32 groups of 8 lanes
-// share the tiles, then a wave takes a target at a time (a dot product of d terms).
+// share the tiles, then 16 lanes take a target at a time (a dot product of d terms).
 // ---------------------------------------------------------------------------
+constexpr int kRows = 8;
 struct RowsArgs {
   const void* x; int64_t x_ld;
   const void* w; int64_t w_ld;
@@ -228,52 +232,53 @@ struct RowsArgs {
   float* lse2; float* t; float* loss;
 };
 
-// x . w in one order of the sum however the rows are aligned.
+// PER neighbours of a row, zeros past its end.
 template <typename T>
-__device__ inline float row_dot_of(const T* x, const T* w, int d, int vec, int lane) {
+__device__ inline void load_vec(const T* p, int c, int d, bool vec, T (&v)[16 / sizeof(T)]) {
   constexpr int PER = 16 / (int)sizeof(T);
-  typedef __attribute__((__vector_size__(16))) T TV;
-  float s = 0.0f;
-  for (int c = lane * PER; c < d; c += 64 * PER) {
-    TV a, b;
-    if (vec) {
-      a = *reinterpret_cast<const TV*>(x + c);
-      b = *reinterpret_cast<const TV*>(w + c);
-    } else {
+  if (vec) {
+    typedef __attribute__((__vector_size__(16))) T TV;
+    const TV t = *reinterpret_cast<const TV*>(p + c);
 #pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        const int at = c + e < d ? c + e : d - 1;
-        a[e] = c + e < d ? x[at] : (T)0.0f;
-        b[e] = c + e < d ? w[at] : (T)0.0f;
-      }
+    for (int e = 0; e < PER; ++e) v[e] = t[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const T t = p[c + e < d ? c + e : d - 1];
+      v[e] = c + e < d ? t : (T)0.0f;
     }
-#pragma unroll
-    for (int e = 0; e < PER; ++e) s = fmaf((float)a[e], (float)b[e], s);
   }
-  return wave_sum(s);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
-  __shared__ float2 red[32][8];
-  __shared__ float2 stat[8];     // the row's maximum and log2 of its sum
-  __shared__ float part_loss[8][4];
+  __shared__ float2 red[32][kRows];
+  __shared__ float2 stat[kRows];  // the row's maximum and log2 of its sum
+  __shared__ int place[kRows];    // the row's place in the operand, -1: it does not count
+  __shared__ float terms[kRows][kHeadMaxK];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t first = (int64_t)blockIdx.x * 8;
+  const int64_t first = (int64_t)blockIdx.x * kRows;
   {
     const int r = tid & 7, g = tid >> 3;
     const int at = first + r < a.N ? a.pos[first + r] : -1;
     float m = -INFINITY, s = 0.0f;
-    if (at >= 0)
-      for (int t = g; t < a.tiles; t += 32) {
-        const float2 p = a.part[(int64_t)t * a.part_ld + at];
-        const float mn = fmaxf(m, p.x), b = mn == -INFINITY ? 0.0f : mn;
-        s = s * __builtin_amdgcn_exp2f(m - b) + p.y * __builtin_amdgcn_exp2f(p.x - b);
-        m = mn;
+    if (at >= 0) {
+      for (int t = g; t < a.tiles; t += 32 * 4) {
+        float2 p[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) p[q] = t + 32 * q < a.tiles ? a.part[(int64_t)(t + 32 * q) * a.part_ld + at] : float2{-INFINITY, 0.0f};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float mn = fmaxf(m, p[q].x), b = mn == -INFINITY ? 0.0f : mn;
+          s = s * __builtin_amdgcn_exp2f(m - b) + p[q].y * __builtin_amdgcn_exp2f(p[q].x - b);
+          m = mn;
+        }
       }
+    }
     red[g][r] = float2{m, s};
+    if (g == 0) place[r] = at;
     __syncthreads();
-    if (tid < 8) {
+    if (tid < kRows) {
       float mm = -INFINITY, ss = 0.0f;
       for (int q = 0; q < 32; ++q) mm = fmaxf(mm, red[q][tid].x);
       const float b = mm == -INFINITY ? 0.0f : mm;
@@ -283,77 +288,90 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
     __syncthreads();
   }
   const float to_log2 = kLog2e / a.temperature;
-  for (int r = 0; r < 8; ++r) {
-    const int64_t n = first + r;
-    const int at = n < a.N ? a.pos[n] : -1;
-    float sum = 0.0f;
-    if (at >= 0) {
-      const float2 st = stat[r];
-      for (int k = wave; k < a.K; k += 4) {
-        const int64_t id = a.ids[n * a.ids_ld + k];
-        const float2 p = a.tp == nullptr ? float2{1.0f, 1.0f} : a.tp[n * a.K + k];
-        const bool none = a.tp != nullptr && id < 0;
-        float t = 0.0f, part = 0.0f;
-        if (!none) {
-          if (id >= 0 && id < a.V) {
-            const float z2 = to_log2 * row_dot_of((const T*)a.x + n * a.x_ld, (const T*)a.w + id * a.w_ld, a.d, a.vec, lane);
-            const float away = (st.x - z2) + st.y;  // lse2 - z2
-            t = __builtin_amdgcn_exp2f(-away) - p.y;
-            part = p.x > 0.0f || !(p.x == p.x) ? p.x * away : 0.0f;
-          } else {
-            t = part = NAN;
-          }
+  constexpr int PER = 16 / (int)sizeof(T);
+  const int l16 = lane & 15;
+  for (int e = tid >> 4; e < kRows * a.K; e += 16) {
+    const int r = e / a.K, k = e - r * a.K;
+    if (place[r] < 0) continue;  // alike in the 16 lanes
+    const int64_t n = first + r, id = a.ids[n * a.ids_ld + k];
+    const float2 p = a.tp == nullptr ? float2{1.0f, 1.0f} : a.tp[n * a.K + k];
+    float t = 0.0f, term = 0.0f;
+    if (a.tp == nullptr || id >= 0) {
+      if (id >= 0 && id < a.V) {
+        const T* xr = (const T*)a.x + n * a.x_ld;
+        const T* wr = (const T*)a.w + id * a.w_ld;
+        float dot = 0.0f;
+#pragma unroll 4
+        for (int c = l16 * PER; c < a.d; c += 16 * PER) {
+          T xv[PER], wv[PER];
+          load_vec(xr, c, a.d, a.vec != 0, xv);
+          load_vec(wr, c, a.d, a.vec != 0, wv);
+#pragma unroll
+          for (int q = 0; q < PER; ++q) dot = fmaf((float)xv[q], (float)wv[q], dot);
         }
-        sum += part;
-        if (lane == 0) a.t[n * a.K + k] = t;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor(dot, o);
+        const float away = (stat[r].x - to_log2 * dot) + stat[r].y;  // lse2 - z2
+        t = __builtin_amdgcn_exp2f(-away) - p.y;
+        term = p.x > 0.0f || !(p.x == p.x) ? p.x * away : 0.0f;
+      } else {
+        t = term = NAN;
       }
     }
-    if (lane == 0) part_loss[r][wave] = sum;
+    if (l16 == 0) {
+      terms[r][k] = term;
+      a.t[n * a.K + k] = t;
+    }
   }
   __syncthreads();
-  if (tid < 8) {
-    const int64_t n = first + tid;
+  {
+    const int r = tid >> 5, l = tid & 31;
+    const int64_t n = first + r;
     if (n < a.N) {
-      const int at = a.pos[n];
-      const float away = (part_loss[tid][0] + part_loss[tid][1]) + (part_loss[tid][2] + part_loss[tid][3]);
-      float loss = kLn2 * away;
-      if (a.tp != nullptr && at >= 0) loss = a.temperature * a.temperature * (loss + a.ent[n]);
-      a.loss[n] = at >= 0 ? loss : 0.0f;
-      // a target outside the vocabulary makes the row NaN, its gradient too
-      if (at >= 0) a.lse2[at] = away == away ? stat[tid].x + stat[tid].y : NAN;
+      const int at = place[r];
+      float away = 0.0f;
+      if (at >= 0)
+        for (int k = l; k < a.K; k += 32) away += terms[r][k];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) away += __shfl_xor(away, o);
+      if (l == 0) {
+        float loss = kLn2 * away;
+        if (a.tp != nullptr && at >= 0) loss = a.temperature * a.temperature * (loss + a.ent[n]);
+        a.loss[n] = at >= 0 ? loss : 0.0f;
+        // a target outside the vocabulary makes the row NaN, its gradient too
+        if (at >= 0) a.lse2[at] = away == away ? stat[r].x + stat[r].y : NAN;
+      }
     }
   }
 }
 
-// One block: the mean or the sum of the rows' losses, in 64 bits.
+// One block: the mean or the sum of the rows' losses, in 64 bits.  (The last block of rows_kernel could do it; but making
+// each block's rows visible to it writes back its L2: 160 -> 390 us for 8192 rows of 64 targets.)
 __global__ void __launch_bounds__(1024) total_kernel(const float* rows, int64_t N, const WideHdr* hdr, int mean, float* out) {
-  __shared__ double sums[1024];
+  __shared__ double sums[16];
   double s = 0.0;
+#pragma unroll 4
   for (int64_t n = threadIdx.x; n < N; n += 1024) s += (double)rows[n];
-  sums[threadIdx.x] = s;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
   __syncthreads();
-  for (int o = 512; o > 0; o >>= 1) {
-    if ((int)threadIdx.x < o) sums[threadIdx.x] += sums[threadIdx.x + o];
-    __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) s += sums[w];
+    out[0] = (float)(mean ? s / (double)hdr->live : s);
   }
-  if (threadIdx.x == 0) out[0] = (float)(mean ? sums[0] / (double)hdr->live : sums[0]);
 }
 
 // ---------------------------------------------------------------------------
 // Backward
 // ---------------------------------------------------------------------------
-// One block: coefficients of the rows of the operand, as g_n / cmax; zero behind the last row up to the next multiple
-// of 128.  A mean or a sum has one coefficient: cmax is it and every row's is 1, so that G is rounded from the
-// probabilities themselves.  Else cmax is a power of two, at least the largest finite |g_n|.
-__global__ void __launch_bounds__(1024) coef_kernel(const float* dloss, int reduction, float factor, int64_t N, int64_t n_pad,
-                                                    const int* pos, WideHdr* hdr, float* coef) {
+// Coefficients of the rows of the operand where each row's loss has a gradient of its own, as g_n / cmax with a power of
+// two cmax, at least the largest finite |g_n|; zero behind the last row up to the next multiple of 128.  One block.  (A mean
+// or a sum has one coefficient for all: G is formed for 1 and so rounded from the probabilities themselves.)
+__global__ void __launch_bounds__(1024) coef_kernel(const float* dloss, float factor, int64_t N, int64_t n_pad, const int* pos,
+                                                    const WideHdr* hdr, float* cmax, float* coef) {
   const int tid = (int)threadIdx.x;
   const int live = hdr->live;
-  if (reduction != 0) {
-    if (tid == 0) hdr->cmax = reduction == 1 ? dloss[0] * factor / (float)live : dloss[0] * factor;
-    for (int64_t i = tid; i < n_pad; i += 1024) coef[i] = i < live ? 1.0f : 0.0f;
-    return;
-  }
   __shared__ float red[16];
   float mx = 0.0f;
   for (int64_t n = tid; n < N; n += 1024) {
@@ -366,7 +384,7 @@ __global__ void __launch_bounds__(1024) coef_kernel(const float* dloss, int redu
   __syncthreads();
   for (int w = 0; w < 16; ++w) mx = fmaxf(mx, red[w]);
   const float inv = pow2_to(mx, 0);  // mx inv in [0.5, 1)
-  if (tid == 0) hdr->cmax = 1.0f / inv;
+  if (tid == 0) *cmax = 1.0f / inv;
   for (int64_t n = tid; n < N; n += 1024)
     if (pos[n] >= 0) coef[pos[n]] = dloss[n] * factor * inv;
   for (int64_t i = live + tid; i < n_pad; i += 1024) coef[i] = 0.0f;
@@ -410,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
     const int64_t n = n0 + Tl::n_of(wn, lane, j);
     const bool ok = n < live;
     // a row behind the last one has an operand of zeros, lse2 of infinity and so a gradient of zeros
-    const float l = ok ? a.lse2[n] : INFINITY, c = ok ? a.coef[n] * sg : 0.0f;
+    const float l = ok ? a.lse2[n] : INFINITY, c = !ok ? 0.0f : a.coef != nullptr ? a.coef[n] * sg : sg;
 #pragma unroll
     for (int i = 0; i < Tl::MB; ++i)
 #pragma unroll
@@ -447,7 +465,7 @@ __global__ void __launch_bounds__(kThreads) scatter_kernel(const int64_t* ids, i
   const int at = pos[n];
   const int64_t v = ids[n * ids_ld + (e - n * K)] - v0;
   if (at < 0 || v < 0 || v >= cols) return;
-  const float x = t[e] * coef[at] * scale_g<T>(hdr, 0);
+  const float x = (coef != nullptr ? t[e] * coef[at] : t[e]) * scale_g<T>(hdr, 0);
   E* p = reinterpret_cast<E*>(g) + (int64_t)at * C + v;
   if constexpr (Wide<T>::P == 2) {
     const Terms<float> w(x);
@@ -480,7 +498,7 @@ struct HeadPlan {
   bool distill;
   char *x, *w, *g;
   float2 *part, *tp;
-  float *ent, *rows, *coef, *dx_part, *dw_part;
+  float *ent, *rows, *coef, *cmax, *dx_part, *dw_part;
   uint8_t* live;
   size_t bytes;
   HeadPlan(const HeadCall& c, int backward) {
@@ -499,7 +517,7 @@ struct HeadPlan {
     w = w_direct(c) ? nullptr : take(planes * w_plane);
     C = g_plane = 0;
     dx_split = dw_split = 1;
-    part = tp = nullptr; ent = rows = coef = dx_part = dw_part = nullptr; live = nullptr; g = nullptr;
+    part = tp = nullptr; ent = rows = coef = cmax = dx_part = dw_part = nullptr; live = nullptr; g = nullptr;
     if (!backward) {
       part = (float2*)take((int64_t)tiles_v * n_pad * 8);
       if (c.reduction != 0) rows = (float*)take(c.N * 4);
@@ -517,7 +535,10 @@ struct HeadPlan {
       C = round_up((all + pieces - 1) / pieces, 256);
       g_plane = round_up(n_pad * C * 2, 256);
       g = take(planes * g_plane);
-      coef = (float*)take(n_pad * 4);
+      if (c.reduction == 0) {
+        coef = (float*)take(n_pad * 4);
+        cmax = (float*)take(4);
+      }
       wide_splits(c.N, c.d, C, 1, c.dx != nullptr, c.dw != nullptr, &dx_split, &dw_split);
       if (c.dx != nullptr) dx_part = (float*)take((int64_t)dx_split * n_pad * dp * 4);
       if (c.dw != nullptr && dw_split > 1) dw_part = (float*)take((int64_t)dw_split * C * dp * 4);
@@ -540,18 +561,15 @@ struct HeadPlan {
 
 #define HEAD_TRY(call) do { const hipError_t e_ = (call); if (e_ != hipSuccess) return e_; } while (0)
 
-// hidden's counting rows and the weight as operands
-template <typename T>
-hipError_t operands(const HeadCall& c, const HeadPlan& p, const HeadState& st) {
-  RowsCopy x{c.x, c.x_ld, c.N, c.d, c.dtype, p.x, p.x_plane, st.pos, st.hdr, 0};
-  RowsCopy w{c.w, c.w_ld, c.V, c.d, c.dtype, p.w, p.w_plane, nullptr, st.hdr, 1};
-  if (p.planes == 2) {
-    HEAD_TRY(launch_rows_max(x, 0, c.stream));
-    HEAD_TRY(launch_rows_max(w, 0, c.stream));
-  }
-  HEAD_TRY(launch_rows_copy(x, c.stream));
-  if (p.w != nullptr) HEAD_TRY(launch_rows_copy(w, c.stream));
-  return hipSuccess;
+// hidden's counting rows and the weight as operands; the forward pass finds fp32's scales for both passes
+hipError_t operands(const HeadCall& c, const HeadPlan& p, const HeadState& st, bool find) {
+  RowsCopies all = {};
+  all.dtype = c.dtype;
+  all.hdr = st.hdr;
+  all.add(RowsCopy{c.x, c.x_ld, c.N, c.d, p.x, p.x_plane, st.pos, 0, 0});
+  if (p.w != nullptr) all.add(RowsCopy{c.w, c.w_ld, c.V, c.d, p.w, p.w_plane, nullptr, 1, 0});
+  if (p.planes == 2 && find) HEAD_TRY(launch_rows_max(all, c.stream));
+  return launch_rows_copy(all, c.stream);
 }
 
 template <typename T>
@@ -571,9 +589,8 @@ hipError_t head_fwd(const HeadCall& c) {
   }
   hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, c.stream, c.ids, c.ids_ld, c.ignore_index, p.live, c.N, st.pos, st.hdr);
   HEAD_TRY(hipGetLastError());
-  float* rows = c.reduction == 0 ? c.loss : p.rows;
   if (c.N > 0) {
-    HEAD_TRY(operands<T>(c, p, st));
+    HEAD_TRY(operands(c, p, st, true));
     StatsArgs a;
     a.x = p.x; a.x_ld = p.dp * 2; a.n_pad = p.n_pad;
     a.w = p.w != nullptr ? p.w : (const char*)c.w; a.w_ld = p.w != nullptr ? p.dp * 2 : c.w_ld * 2; a.V = c.V;
@@ -584,12 +601,12 @@ hipError_t head_fwd(const HeadCall& c) {
     RowsArgs r;
     r.x = c.x; r.x_ld = c.x_ld; r.w = c.w; r.w_ld = c.w_ld; r.ids = c.ids; r.ids_ld = c.ids_ld; r.tp = p.tp; r.ent = p.ent;
     r.part = p.part; r.part_ld = p.n_pad; r.tiles = p.tiles_v; r.N = c.N; r.V = c.V; r.d = c.d; r.K = c.K; r.vec = rows_vec(c);
-    r.temperature = c.temperature; r.pos = st.pos; r.lse2 = st.lse2; r.t = st.t; r.loss = rows;
-    hipLaunchKernelGGL(rows_kernel<T>, dim3((unsigned)((c.N + 7) / 8)), dim3(kThreads), 0, c.stream, r);
+    r.temperature = c.temperature; r.pos = st.pos; r.lse2 = st.lse2; r.t = st.t; r.loss = c.reduction == 0 ? c.loss : p.rows;
+    hipLaunchKernelGGL(rows_kernel<T>, dim3((unsigned)((c.N + kRows - 1) / kRows)), dim3(kThreads), 0, c.stream, r);
     HEAD_TRY(hipGetLastError());
   }
   if (c.reduction != 0) {
-    hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, c.stream, rows, c.N, st.hdr, c.reduction == 1, c.loss);
+    hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, c.stream, p.rows, c.N, st.hdr, c.reduction == 1, c.loss);
     HEAD_TRY(hipGetLastError());
   }
   return hipSuccess;
@@ -605,9 +622,12 @@ hipError_t head_bwd(const HeadCall& c) {
     return hipGetLastError();
   }
   const float factor = p.distill ? c.temperature : 1.0f;  // T^2 of the loss, 1/T of z
-  hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, c.stream, c.dloss, c.reduction, factor, c.N, p.n_pad, st.pos, st.hdr, p.coef);
-  HEAD_TRY(hipGetLastError());
-  HEAD_TRY(operands<T>(c, p, st));
+  const GradUnit unit{c.dloss, factor, c.reduction};
+  if (c.reduction == 0) {
+    hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, c.stream, c.dloss, factor, c.N, p.n_pad, st.pos, st.hdr, p.cmax, p.coef);
+    HEAD_TRY(hipGetLastError());
+  }
+  HEAD_TRY(operands(c, p, st, false));
   const char* w = p.w != nullptr ? p.w : (const char*)c.w;
   const int64_t w_ld = p.w != nullptr ? p.dp * 2 : c.w_ld * 2;
   for (int64_t v0 = 0; v0 < c.V; v0 += p.C) {
@@ -629,11 +649,11 @@ hipError_t head_bwd(const HeadCall& c) {
     q.g = p.g; q.g_plane = p.g_plane; q.g_half = 0;
     q.dx_part = p.dx_part; q.dx_add = v0 > 0;
     q.dw[0] = c.dw == nullptr ? nullptr : (char*)c.dw + v0 * c.d * es_of(c.dtype); q.dw_part = p.dw_part;
-    q.dx_split = p.dx_split; q.dw_split = p.dw_split; q.hdr = st.hdr; q.use_live = 1;
+    q.dx_split = p.dx_split; q.dw_split = p.dw_split; q.hdr = st.hdr; q.unit = unit; q.cmax = p.cmax; q.use_live = 1;
     HEAD_TRY(launch_wide_products(q, c.stream));
   }
   if (c.dx != nullptr) {
-    const WideFinish f{c.dtype, 0, c.N, p.n_pad, c.d, p.dp, p.dx_split, p.dx_part, st.pos, st.hdr, c.dx};
+    const WideFinish f{c.dtype, 0, c.N, p.n_pad, c.d, p.dp, p.dx_split, p.dx_part, st.pos, st.hdr, unit, p.cmax, c.dx};
     HEAD_TRY(launch_wide_finish(f, c.stream));
   }
   return hipSuccess;

@@ -16,15 +16,18 @@ namespace msa {
 template <typename T> struct Wide { typedef T E; static constexpr int P = 1; };
 template <> struct Wide<float> { typedef f16 E; static constexpr int P = 2; };
 
-// Device-side facts of a call.  max_*: bits of the largest finite |entry| (of counting rows), norm_*: of the largest
-// finite squared row norm; floats of one sign compare as integers, so atomicMax gives the same whatever the order.
+// Device-side facts of a call.  max: bits of the largest finite |entry| of x (rows that count), w, dh, and of the largest
+// finite squared row norm of x and w; floats of one sign compare as integers, so atomicMax gives the same whatever the
+// order.  Each has kSlots places a cache line apart (blocks in turn), which a reader takes the largest of: 2700 atomics to
+// one place take 40 us.
+constexpr int kSlots = 16;
+enum WideMax { kMaxX = 0, kMaxW = 1, kMaxDh = 2, kNormX = 3, kNormW = 4, kMaxes = 5 };
 struct WideHdr {
   int live;  // rows that count
-  uint32_t max_x, max_w, max_dh, norm_x, norm_w;
-  float cmax;  // what the rows' gradient coefficients are divided by: their common value, or a power of two
-  int pad[9];
+  int pad[15];
+  uint32_t max[kMaxes][kSlots][16];
 };
-static_assert(sizeof(WideHdr) == 64, "header size");
+constexpr int kHdrWords = (int)(sizeof(WideHdr) / 4);
 
 __device__ inline float pow2_to(float mx, int top) {  // p with mx p in [2^(top-1), 2^top); 1 for 0
   if (!(mx > 0.0f)) return 1.0f;
@@ -34,16 +37,28 @@ __device__ inline float pow2_to(float mx, int top) {  // p with mx p in [2^(top-
   e = e > 120 ? 120 : (e < -120 ? -120 : e);
   return ldexpf(1.0f, e);
 }
-__device__ inline float finite_max(uint32_t bits) { return __uint_as_float(bits); }
+// Every lane of the wave calls it.
+__device__ inline float wide_max(const WideHdr* h, int which) {
+  float v = __uint_as_float(h->max[which][threadIdx.x & (kSlots - 1)][0]);
+#pragma unroll
+  for (int o = kSlots / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
 
-// Scales of the operands.  fp16 gradients of logits lie in [-1, 1] and are kept times 2^15; those of the gated
-// projections are bounded by max|dh| 1.13 max|x| max|w| (|act(g)| <= |g|, |act'| < 1.13).
-template <typename T> __device__ inline float scale_x(const WideHdr* h) { return Wide<T>::P == 2 ? pow2_to(finite_max(h->max_x), 15) : 1.0f; }
-template <typename T> __device__ inline float scale_w(const WideHdr* h) { return Wide<T>::P == 2 ? pow2_to(finite_max(h->max_w), 15) : 1.0f; }
+// Scales of the operands (every lane of the wave calls these).  fp16 gradients of logits lie in [-1, 1] and are kept times
+// 2^15; those of the gated projections are bounded by max|dh| 1.13 max|x| max|w| (|act(g)| <= |g|, |act'| < 1.13).
+template <typename T> __device__ inline float scale_x(const WideHdr* h) {
+  if constexpr (Wide<T>::P == 2) return pow2_to(wide_max(h, kMaxX), 15);
+  return 1.0f;
+}
+template <typename T> __device__ inline float scale_w(const WideHdr* h) {
+  if constexpr (Wide<T>::P == 2) return pow2_to(wide_max(h, kMaxW), 15);
+  return 1.0f;
+}
 template <typename T> __device__ inline float scale_g(const WideHdr* h, int gated) {
   if constexpr (__is_same(T, bf16)) return 1.0f;
   if (!gated) return 32768.0f;
-  return pow2_to(1.15f * finite_max(h->max_dh) * sqrtf(finite_max(h->norm_x)) * sqrtf(finite_max(h->norm_w)), 15);
+  return pow2_to(1.15f * wide_max(h, kMaxDh) * sqrtf(wide_max(h, kNormX)) * sqrtf(wide_max(h, kNormW)), 15);
 }
 
 // The terms of v (already scaled).  v is held in a register first: formed inside, a product that makes v may be rounded
@@ -60,18 +75,37 @@ template <> struct Terms<float> {
 
 inline int64_t wide_dp(int64_t d) { return round_up(d, 32); }
 
-// Rows of a matrix (rows x d, type dtype) as operand rows of dp columns: `planes` matrices of plane_bytes each.
-// pos: null, or which row of the operand each row becomes (-1: none); rows from *live up to the next multiple of 128
-// are then zeroed.  hdr, slot (0: x, 1: w): fp32's scale.
+// Matrices as operand rows of dp columns: `planes` matrices of plane_bytes each.  pos: null, or which row of the
+// operand each row becomes (-1: none); rows from *live up to the next multiple of 128 are then zeroed.  slot (0: x, 1: w, 2:
+// dh): whose maxima it adds to, and whose scale it takes.
 struct RowsCopy {
-  const void* src; int64_t ld; int64_t rows; int d, dtype;
+  const void* src; int64_t ld; int64_t rows; int d;
   char* dst; int64_t plane_bytes;
-  const int* pos; WideHdr* hdr; int slot;
+  const int* pos; int slot, norms;
 };
-hipError_t launch_rows_copy(const RowsCopy& c, hipStream_t s);
-// max|entry| and, with `norms`, the largest squared row norm of a matrix into hdr (slot 0: x, 1: w, 2: dh).
-hipError_t launch_rows_max(const RowsCopy& c, int norms, hipStream_t s);
+constexpr int kCopies = 4;
+struct RowsCopies {
+  RowsCopy m[kCopies];
+  int n, dtype;
+  WideHdr* hdr;
+  void add(const RowsCopy& c) { m[n++] = c; }
+};
+hipError_t launch_rows_copy(const RowsCopies& c, hipStream_t s);
+// max|entry| and, where asked for, the largest squared row norm of the matrices, into hdr.
+hipError_t launch_rows_max(const RowsCopies& c, hipStream_t s);
 hipError_t launch_hdr_clear(WideHdr* hdr, hipStream_t s);
+
+// What G is to be multiplied with: *cmax; or dloss[0] factor, over the number of rows that count for a mean; or 1.
+struct GradUnit {
+  const float* dloss;
+  float factor;
+  int mode;  // 0: cmax, 1: mean, 2: sum, 3: one
+};
+__device__ inline float unit_of(const GradUnit& u, const WideHdr* h, const float* cmax) {
+  if (u.mode == 3) return 1.0f;
+  if (u.mode == 0) return *cmax;
+  return u.mode == 1 ? u.dloss[0] * u.factor / (float)h->live : u.dloss[0] * u.factor;
+}
 
 // The backward products of one piece of the weight's rows.
 struct WideProducts {
@@ -90,6 +124,7 @@ struct WideProducts {
   float* dw_part;                                             // [dw_split][halves][C][dp] where dw_split > 1
   int dx_split, dw_split;
   const WideHdr* hdr;
+  GradUnit unit; const float* cmax;
   int use_live;  // tokens are hdr->live
 };
 hipError_t launch_wide_products(const WideProducts& p, hipStream_t s);
@@ -107,6 +142,7 @@ struct WideFinish {
   const float* part;
   const int* pos;
   const WideHdr* hdr;
+  GradUnit unit; const float* cmax;
   void* dx;
 };
 hipError_t launch_wide_finish(const WideFinish& f, hipStream_t s);

@@ -7,33 +7,67 @@ namespace {
 constexpr int kThreads = 256;
 
 __global__ void hdr_clear_kernel(WideHdr* h) {
-  if (threadIdx.x < sizeof(WideHdr) / 4) reinterpret_cast<uint32_t*>(h)[threadIdx.x] = 0u;
+  for (int i = (int)threadIdx.x; i < kHdrWords; i += kThreads) reinterpret_cast<uint32_t*>(h)[i] = 0u;
 }
 
+// 8 neighbours of a row, zeros past its end.
 template <typename T>
-__device__ inline void atomic_max_finite(uint32_t* slot, float v) {
-  v = fabsf(v);
-  if (v < INFINITY && v > 0.0f) atomicMax(slot, __float_as_uint(v));
+__device__ inline void load8(const T* in, int c, int d, bool vec, T (&x)[8]) {
+  if (vec && c + 8 <= d) {
+    typedef __attribute__((__vector_size__(16))) T T16;
+    constexpr int PER = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int q = 0; q < 8 / PER; ++q) {
+      const T16 t = *reinterpret_cast<const T16*>(in + c + q * PER);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) x[q * PER + e] = t[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const T v = in[c + e < d ? c + e : d - 1];
+      x[e] = c + e < d ? v : (T)0.0f;
+    }
+  }
 }
 
-// A wave per row, rows in turn.
+struct RowsArgs {
+  RowsCopy m[kCopies];
+  int64_t first[kCopies + 1];  // blocks of each matrix
+  int vec[kCopies];
+  WideHdr* hdr;
+};
+__device__ inline int matrix_of(const RowsArgs& a, int64_t block) {
+  int i = 0;
+#pragma unroll
+  for (int k = 1; k < kCopies; ++k) i += block >= a.first[k] ? 1 : 0;
+  return i;
+}
+
+// A wave takes rows in turn, of the matrix that its block belongs to.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) rows_max_kernel(const T* src, int64_t ld, int64_t rows, int d, const int* pos,
-                                                            uint32_t* mslot, uint32_t* nslot) {
-  const int lane = (int)threadIdx.x & 63;
+__global__ void __launch_bounds__(kThreads) rows_max_kernel(RowsArgs a) {
+  const int i = matrix_of(a, blockIdx.x), lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  const RowsCopy m = a.m[i];
+  const int64_t step = (a.first[i + 1] - a.first[i]) * 4;
   float mx = 0.0f, nx = 0.0f;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
-    if (pos != nullptr && pos[r] < 0) continue;
-    const T* p = src + r * ld;
+  for (int64_t r = ((int64_t)blockIdx.x - a.first[i]) * 4 + wave; r < m.rows; r += step) {
+    if (m.pos != nullptr && m.pos[r] < 0) continue;
+    const T* p = (const T*)m.src + r * m.ld;
     float ss = 0.0f;
-    for (int c = lane; c < d; c += 64) {
-      const float v = fabsf(to_f(p[c]));
-      if (v < INFINITY) {
-        mx = fmaxf(mx, v);
-        ss = fmaf(v, v, ss);
+    for (int c = lane * 8; c < m.d; c += 512) {
+      T x[8];
+      load8(p, c, m.d, a.vec[i] != 0, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = fabsf(to_f(x[e]));
+        if (v < INFINITY) {
+          mx = fmaxf(mx, v);
+          ss = fmaf(v, v, ss);
+        }
       }
     }
-    if (nslot != nullptr) {
+    if (m.norms) {
       ss = wave_sum(ss);
       if (ss < INFINITY) nx = fmaxf(nx, ss);
     }
@@ -41,54 +75,47 @@ __global__ void __launch_bounds__(kThreads) rows_max_kernel(const T* src, int64_
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
   __shared__ float sm[4], sn[4];
-  if (lane == 0) { sm[threadIdx.x >> 6] = mx; sn[threadIdx.x >> 6] = nx; }
+  if (lane == 0) { sm[wave] = mx; sn[wave] = nx; }
   __syncthreads();
   if (threadIdx.x == 0) {
-    atomic_max_finite<T>(mslot, fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])));
-    if (nslot != nullptr) atomic_max_finite<T>(nslot, fmaxf(fmaxf(sn[0], sn[1]), fmaxf(sn[2], sn[3])));
+    const int at = (int)blockIdx.x & (kSlots - 1);
+    atomicMax(&a.hdr->max[m.slot][at][0], __float_as_uint(fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]))));
+    if (m.norms) atomicMax(&a.hdr->max[kNormX + m.slot][at][0], __float_as_uint(fmaxf(fmaxf(sn[0], sn[1]), fmaxf(sn[2], sn[3]))));
   }
 }
 
-// Rows to operand rows.  A wave per row, 8 columns a lane; the last blocks zero the rows behind the last one that
+// Rows to operand rows.  A wave per row, 8 columns a lane; a matrix's last blocks zero the rows behind the last one that
 // counts, up to the next multiple of 128.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) rows_copy_kernel(const T* src, int64_t ld, int64_t rows, int d, int dp,
-                                                             char* dst, int64_t plane, const int* pos,
-                                                             const WideHdr* hdr, int slot) {
+template <typename T>
+__global__ void __launch_bounds__(kThreads) rows_copy_kernel(RowsArgs a, int dp) {
   using E = typename Wide<T>::E;
-  const int lane = (int)threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int i = matrix_of(a, blockIdx.x), lane = (int)threadIdx.x & 63;
+  const RowsCopy m = a.m[i];
+  const int64_t r = ((int64_t)blockIdx.x - a.first[i]) * 4 + (threadIdx.x >> 6);
   int64_t to = r;
   bool zero = false;
-  if (r >= rows) {
-    if (pos == nullptr) return;
-    const int64_t live = hdr->live;
-    to = live + (r - rows);
+  if (r >= m.rows) {
+    if (m.pos == nullptr) return;
+    const int64_t live = a.hdr->live;
+    to = live + (r - m.rows);
     if (to >= (live + 127) / 128 * 128) return;
     zero = true;
-  } else if (pos != nullptr) {
-    to = pos[r];
+  } else if (m.pos != nullptr) {
+    to = m.pos[r];
     if (to < 0) return;
   }
   float s = 1.0f;
-  if constexpr (Wide<T>::P == 2) s = slot == 0 ? scale_x<T>(hdr) : scale_w<T>(hdr);
-  E* out = reinterpret_cast<E*>(dst) + to * dp;
-  const T* in = src + r * ld;
+  if constexpr (Wide<T>::P == 2) s = m.slot == 0 ? scale_x<T>(a.hdr) : scale_w<T>(a.hdr);
+  E* out = reinterpret_cast<E*>(m.dst) + to * dp;
+  const T* in = (const T*)m.src + r * m.ld;
   typedef __attribute__((__vector_size__(16))) E E8;
   for (int c = lane * 8; c < dp; c += 512) {
     T x[8];
-    if (VEC && !zero && c + 8 <= d) {
-      typedef __attribute__((__vector_size__(16))) T T16;
-      constexpr int PER = 16 / (int)sizeof(T);
+    if (zero || c >= m.d) {
 #pragma unroll
-      for (int q = 0; q < 8 / PER; ++q) {
-        const T16 t = *reinterpret_cast<const T16*>(in + c + q * PER);
-#pragma unroll
-        for (int e = 0; e < PER; ++e) x[q * PER + e] = t[e];
-      }
+      for (int e = 0; e < 8; ++e) x[e] = (T)0.0f;
     } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = !zero && c + e < d ? in[c + e] : (T)0.0f;
+      load8(in, c, m.d, a.vec[i] != 0, x);
     }
     E8 h;
     if constexpr (Wide<T>::P == 2) {
@@ -99,7 +126,7 @@ __global__ void __launch_bounds__(kThreads) rows_copy_kernel(const T* src, int64
         h[e] = t.h;
         l[e] = t.l;
       }
-      *reinterpret_cast<E8*>(reinterpret_cast<char*>(out + c) + plane) = l;
+      *reinterpret_cast<E8*>(reinterpret_cast<char*>(out + c) + m.plane_bytes) = l;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[e] = x[e];
@@ -123,6 +150,7 @@ struct ProductArgs {
   void* dw0; void* dw1;
   float* dw_part;
   const WideHdr* hdr;
+  GradUnit unit; const float* cmax;
   int use_live, gated, vec;
 };
 
@@ -137,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, 2) products_kernel(ProductArgs p) {
   LdsChar* lds = (LdsChar*)smem;
   const int64_t N = p.use_live ? p.hdr->live : p.N;
   const bool is_dx = (int)blockIdx.x < p.dx_blocks;
-  const float out_g = (p.gated ? 1.0f : p.hdr->cmax) / scale_g<T>(p.hdr, p.gated);
+  const float out_g = unit_of(p.unit, p.hdr, p.cmax) / scale_g<T>(p.hdr, p.gated);
   if (is_dx) {
     int64_t t = xcd_order(blockIdx.x, p.dx_blocks);
     const int split = (int)(t % p.dx_split);
@@ -189,15 +217,21 @@ __global__ void __launch_bounds__(kThreads, 2) products_kernel(ProductArgs p) {
 // Sums of split tiles in split order, scaled, as rows of T.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) parts_kernel(const float* part, int64_t part_stride, int split, int64_t rows,
-                                                         int d, int dp, const int* pos, const WideHdr* hdr, int gated,
-                                                         int by_x, T* out) {
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= rows) return;
+                                                         int64_t half_stride, int d, int dp, const int* pos, const WideHdr* hdr,
+                                                         GradUnit unit, const float* cmax, int gated, int by_x, T* out0, T* out1) {
+  int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  T* out = out0;
+  if (r >= rows) {  // the second weight's rows follow the first's
+    if (out1 == nullptr || (r -= rows) >= rows) return;
+    out = out1;
+    part += half_stride;
+  }
   const int64_t at = pos == nullptr ? r : pos[r];
-  const float f = (gated ? 1.0f : hdr->cmax) / scale_g<T>(hdr, gated), f2 = 1.0f / (by_x ? scale_x<T>(hdr) : scale_w<T>(hdr));
+  const float f = unit_of(unit, hdr, cmax) / scale_g<T>(hdr, gated), f2 = 1.0f / (by_x ? scale_x<T>(hdr) : scale_w<T>(hdr));
   for (int c = ((int)threadIdx.x & 63) * 4; c < d; c += 256) {
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     if (at >= 0) {
+#pragma unroll 4
       for (int s = 0; s < split; ++s) v += *reinterpret_cast<const f32x4*>(part + s * part_stride + at * dp + c);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = v[e] * f * f2;
@@ -212,25 +246,41 @@ __global__ void __launch_bounds__(kThreads) parts_kernel(const float* part, int6
   }
 }
 
+// Blocks of each matrix: a wave per row, at most `most` blocks.
+RowsArgs rows_args(const RowsCopies& c, int64_t most, bool zeros, int64_t* blocks) {
+  RowsArgs a = {};
+  const int64_t es = c.dtype == 0 ? 4 : 2;
+  int64_t at = 0;
+  for (int i = 0; i < kCopies; ++i) {
+    a.first[i] = at;
+    if (i >= c.n) continue;
+    a.m[i] = c.m[i];
+    a.vec[i] = ((uintptr_t)c.m[i].src & 15) == 0 && c.m[i].ld * es % 16 == 0;
+    const int64_t b = (c.m[i].rows + (zeros && c.m[i].pos != nullptr ? 128 : 0) + 3) / 4;
+    at += b < most ? b : most;
+  }
+  a.first[kCopies] = at;
+  for (int i = c.n; i < kCopies; ++i) a.first[i] = at;
+  a.hdr = c.hdr;
+  *blocks = at;
+  return a;
+}
+
 template <typename T>
-hipError_t rows_copy(const RowsCopy& c, hipStream_t s) {
-  const bool vec = ((uintptr_t)c.src & 15) == 0 && c.ld * (int64_t)sizeof(T) % 16 == 0;
-  const int64_t blocks = (c.rows + (c.pos != nullptr ? 128 : 0) + 3) / 4;
+hipError_t rows_copy(const RowsCopies& c, hipStream_t s) {
+  int64_t blocks;
+  const RowsArgs a = rows_args(c, (int64_t)1 << 40, true, &blocks);
   if (blocks == 0) return hipSuccess;
-  auto* k = vec ? rows_copy_kernel<T, true> : rows_copy_kernel<T, false>;
-  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(kThreads), 0, s, (const T*)c.src, c.ld, c.rows, c.d,
-                     (int)wide_dp(c.d), c.dst, c.plane_bytes, c.pos, c.hdr, c.slot);
+  hipLaunchKernelGGL(rows_copy_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, s, a, (int)wide_dp(c.m[0].d));
   return hipGetLastError();
 }
 
 template <typename T>
-hipError_t rows_max(const RowsCopy& c, int norms, hipStream_t s) {
-  const int64_t blocks = (c.rows + 3) / 4 < 1024 ? (c.rows + 3) / 4 : 1024;
+hipError_t rows_max(const RowsCopies& c, hipStream_t s) {
+  int64_t blocks;
+  const RowsArgs a = rows_args(c, 1024, false, &blocks);
   if (blocks == 0) return hipSuccess;
-  uint32_t* m = c.slot == 0 ? &c.hdr->max_x : c.slot == 1 ? &c.hdr->max_w : &c.hdr->max_dh;
-  uint32_t* n = !norms ? nullptr : c.slot == 0 ? &c.hdr->norm_x : &c.hdr->norm_w;
-  hipLaunchKernelGGL(rows_max_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, s, (const T*)c.src, c.ld, c.rows,
-                     c.d, c.pos, m, n);
+  hipLaunchKernelGGL(rows_max_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
   return hipGetLastError();
 }
 
@@ -268,7 +318,7 @@ hipError_t products(const WideProducts& p, hipStream_t s) {
   a.g = p.g; a.g_half = p.g_half;
   a.dx_part = p.dx_part; a.dx_add = p.dx_add;
   a.dw0 = p.dw[0]; a.dw1 = p.dw[1]; a.dw_part = p.dw_part;
-  a.hdr = p.hdr; a.use_live = p.use_live; a.gated = p.gated;
+  a.hdr = p.hdr; a.unit = p.unit; a.cmax = p.cmax; a.use_live = p.use_live; a.gated = p.gated;
   a.vec = (int64_t)p.d * sizeof(T) % 16 == 0 && ((uintptr_t)p.dw[0] & 15) == 0 && ((uintptr_t)p.dw[1] & 15) == 0;
   const int64_t dw_blocks = p.dw[0] != nullptr ? (int64_t)a.dw_tm * a.dw_tn * p.dw_split * p.halves : 0;
   const int64_t blocks = a.dx_blocks + dw_blocks;
@@ -276,34 +326,31 @@ hipError_t products(const WideProducts& p, hipStream_t s) {
   hipLaunchKernelGGL(products_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || dw_blocks == 0 || p.dw_split == 1) return e;
-  for (int half = 0; half < p.halves; ++half) {
-    hipLaunchKernelGGL(parts_kernel<T>, dim3((unsigned)((p.cols + 3) / 4)), dim3(kThreads), 0, s,
-                       p.dw_part + (int64_t)half * p.C * p.dp, (int64_t)p.halves * p.C * p.dp, p.dw_split, (int64_t)p.cols, p.d,
-                       (int)p.dp, (const int*)nullptr, p.hdr, p.gated, 1, (T*)p.dw[half]);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-  }
-  return hipSuccess;
+  hipLaunchKernelGGL(parts_kernel<T>, dim3((unsigned)(((int64_t)p.cols * p.halves + 3) / 4)), dim3(kThreads), 0, s, p.dw_part,
+                     (int64_t)p.halves * p.C * p.dp, p.dw_split, (int64_t)p.cols, (int64_t)p.C * p.dp, p.d, (int)p.dp,
+                     (const int*)nullptr, p.hdr, p.unit, p.cmax, p.gated, 1, (T*)p.dw[0], (T*)(p.halves == 2 ? p.dw[1] : nullptr));
+  return hipGetLastError();
 }
 
 template <typename T>
 hipError_t finish(const WideFinish& f, hipStream_t s) {
   if (f.N == 0) return hipSuccess;
   hipLaunchKernelGGL(parts_kernel<T>, dim3((unsigned)((f.N + 3) / 4)), dim3(kThreads), 0, s, f.part, f.n_pad * f.dp,
-                     f.split, f.N, f.d, (int)f.dp, f.pos, f.hdr, f.gated, 0, (T*)f.dx);
+                     f.split, f.N, (int64_t)0, f.d, (int)f.dp, f.pos, f.hdr, f.unit, f.cmax, f.gated, 0, (T*)f.dx, (T*)nullptr);
   return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_hdr_clear(WideHdr* hdr, hipStream_t s) {
-  hipLaunchKernelGGL(hdr_clear_kernel, dim3(1), dim3(64), 0, s, hdr);
+  hipLaunchKernelGGL(hdr_clear_kernel, dim3(1), dim3(kThreads), 0, s, hdr);
   return hipGetLastError();
 }
-hipError_t launch_rows_copy(const RowsCopy& c, hipStream_t s) {
+hipError_t launch_rows_copy(const RowsCopies& c, hipStream_t s) {
   return c.dtype == 0 ? rows_copy<float>(c, s) : c.dtype == 1 ? rows_copy<bf16>(c, s) : rows_copy<f16>(c, s);
 }
-hipError_t launch_rows_max(const RowsCopy& c, int norms, hipStream_t s) {
-  return c.dtype == 0 ? rows_max<float>(c, norms, s) : c.dtype == 1 ? rows_max<bf16>(c, norms, s) : rows_max<f16>(c, norms, s);
+hipError_t launch_rows_max(const RowsCopies& c, hipStream_t s) {
+  return c.dtype == 0 ? rows_max<float>(c, s) : c.dtype == 1 ? rows_max<bf16>(c, s) : rows_max<f16>(c, s);
 }
 hipError_t launch_wide_products(const WideProducts& p, hipStream_t s) {
   return p.dtype == 0 ? products<float>(p, s) : p.dtype == 1 ? products<bf16>(p, s) : products<f16>(p, s);

@@ -622,12 +622,11 @@ class _HeadLoss(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dloss):
         hidden, weight, ids, teacher, state = ctx.saved_tensors
-        dloss = dloss.to(torch.float32).contiguous()
+        dloss = dloss.contiguous()
         dh = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if ctx.needs_input_grad[0] else None
         dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if ctx.needs_input_grad[1] else None
-        # the pass keeps scales in the state's header: one of its own, so that two passes may run at once
         _head_call("msa_head_bwd", _native.lib().msa_head_bwd, hidden.get_device(), 1, hidden, weight, ids, teacher,
-                   *ctx.options, state.clone(), None, dloss, dh, dw)
+                   *ctx.options, state, None, dloss, dh, dw)
         return dh, dw, None, None, None, None, None
 
 
