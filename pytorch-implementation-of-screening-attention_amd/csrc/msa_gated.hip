@@ -2,7 +2,7 @@
 //   dg = dh u act'(g), du = dh act(g);  dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x
 // A tile's A rows alternate between the two weights by 64, so that a wave holds a feature's g and u of the same token
 // and the activation and the product happen in registers: h is written once, g and u never.  The backward pass forms g
-// and u again (keeping them rounded would cost 4 N F bytes and a rounding), in pieces of the features (256 MB of dg and
+// and u again (keeping them rounded would cost 4 N F bytes and a rounding), in pieces of the features (1 GB of dg and
 // du, or 256 features), then takes the two products of msa_wide.hip.
 #include "msa_wide.h"
 
@@ -10,7 +10,6 @@ namespace msa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int64_t kPieceBytes = (int64_t)256 << 20;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // act(g) and act'(g): silu g / (1 + e^-g); gelu g (1 + erf(g / sqrt 2)) / 2, with erfc(x) = (a1 t + ... + a5 t^5) e^-x^2,
@@ -159,7 +158,8 @@ bool direct(const GatedCall& c, const void* p, int64_t ld) {
 
 struct GatedPlan {
   int64_t n_pad, dp, x_plane, w_plane, C, g_plane;
-  int planes, dx_split, dw_split;
+  int planes;
+  WideShare share;
   char *x, *w, *g;
   float *dx_part, *dw_part;
   WideHdr* hdr;
@@ -177,20 +177,14 @@ struct GatedPlan {
     x = direct(c, c.x, c.x_ld) ? nullptr : take(planes * x_plane);
     w = direct(c, c.w[0], c.w_ld[0]) && direct(c, c.w[1], c.w_ld[1]) && c.w_ld[0] == c.w_ld[1] ? nullptr : take(2 * planes * w_plane);
     C = g_plane = 0;
-    dx_split = dw_split = 1;
+    share = WideShare{};
     g = nullptr; dx_part = dw_part = nullptr;
     if (backward) {
-      C = kPieceBytes / (2 * planes * 2 * n_pad) / 256 * 256;
-      C = C < 256 ? 256 : C;
-      const int64_t all = round_up(c.F, 256);
-      C = C > all ? all : C;
-      const int64_t pieces = (all + C - 1) / C;
-      C = round_up((all + pieces - 1) / pieces, 256);
+      C = wide_piece(c.N, c.d, c.F, 2, planes, c.dx != nullptr, c.dw[0] != nullptr, 2 * planes * 2 * n_pad, &share);
       g_plane = round_up(n_pad * C * 2, 256);
       g = take(2 * planes * g_plane);
-      wide_splits(c.N, c.d, C, 2, c.dx != nullptr, c.dw[0] != nullptr, &dx_split, &dw_split);
-      if (c.dx != nullptr) dx_part = (float*)take((int64_t)dx_split * n_pad * dp * 4);
-      if (c.dw[0] != nullptr && dw_split > 1) dw_part = (float*)take((int64_t)dw_split * 2 * C * dp * 4);
+      if (c.dx != nullptr) dx_part = (float*)take((int64_t)share.dx_split * n_pad * dp * 4);
+      if (c.dw[0] != nullptr && share.dw_split > 1) dw_part = (float*)take((int64_t)share.dw_split * 2 * C * dp * 4);
     }
     bytes = o;
   }
@@ -291,11 +285,11 @@ hipError_t gated_bwd(const GatedCall& c) {
     q.w_ld = o.w_ld; q.w_plane = p.w_plane; q.w_rows = (int)(c.F - f0);
     q.g = p.g; q.g_plane = p.g_plane; q.g_half = p.planes * p.g_plane;
     q.dx_part = p.dx_part; q.dx_add = f0 > 0; q.dw_part = p.dw_part;
-    q.dx_split = p.dx_split; q.dw_split = p.dw_split; q.hdr = p.hdr; q.unit.mode = 3; q.use_live = 0;
+    q.share = p.share; q.hdr = p.hdr; q.unit.mode = 3; q.use_live = 0;
     GATED_TRY(launch_wide_products(q, c.stream));
   }
   if (c.dx != nullptr) {
-    const WideFinish f{c.dtype, 1, c.N, p.n_pad, c.d, p.dp, p.dx_split, p.dx_part, nullptr, p.hdr, GradUnit{nullptr, 1.0f, 3}, nullptr, c.dx};
+    const WideFinish f{c.dtype, 1, c.N, p.n_pad, c.d, p.dp, p.share.dx_split, p.dx_part, nullptr, p.hdr, GradUnit{nullptr, 1.0f, 3}, nullptr, c.dx};
     GATED_TRY(launch_wide_finish(f, c.stream));
   }
   return hipSuccess;

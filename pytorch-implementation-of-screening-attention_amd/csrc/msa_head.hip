@@ -5,7 +5,7 @@
 //   both           dL_n/dz_nv = T (2^(z2_nv - lse2_n) - sum_{k: id(k) = v} p_k)        (z: logits before 1/T)
 // Forward: one product over all of the vocabulary whose tiles leave each row's maximum and sum; a row's own logits are
 // K dot products.  Backward, in pieces of the vocabulary: the product again, now with lse2 known, gives the piece's
-// gradient G in the operand type (256 MB at most, or 256 columns); then dx += G W and dW = G^T x (msa_wide.hip).
+// gradient G in the operand type (1 GB at most, or 256 columns); then dx += G W and dW = G^T x (msa_wide.hip).
 // Rows that do not count are taken out before the products: their x may hold anything.
 #include "msa_wide.h"
 
@@ -15,7 +15,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kHeadMaxK = 256;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int64_t kPieceBytes = (int64_t)256 << 20;
 
 // What the backward pass needs: header, pos[N] (row of the operand, -1: does not count), lse2[N rows of the operand],
 // t[N][K]: 2^(z2 - lse2) - p of the targets (p summed over equal ids).
@@ -417,6 +416,7 @@ __global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
   typename Tl::Acc acc;
   Tl::clear(acc);
   const int vleft = (int)(a.cols - v0 < 256 ? a.cols - v0 : 256);
+  E* out = reinterpret_cast<E*>(a.g) + n0 * a.C + v0;
   const typename Tl::Side A{a.w + v0 * a.w_ld, vleft, a.w_ld, 0, 0};
   const typename Tl::Side B{a.x + n0 * a.x_ld, (int)(a.n_pad - n0 < 128 ? a.n_pad - n0 : 128), a.x_ld, 0, 0};
   Tl::run(acc, lds, A, B, a.segs, 0, a.ksteps);
@@ -436,7 +436,6 @@ __global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
         acc[i][j][r] = c * __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], f, -l));
       }
   }
-  E* out = reinterpret_cast<E*>(a.g) + n0 * a.C + v0;
   if constexpr (Wide<T>::P == 2) {
     Tl::template store_rows<E, false>(lds, out, a.C, 128, 256, true, [&](int i, int j, int g) {
       return quad<E>([&](int e) { return (float)Terms<float>(acc[i][j][4 * g + e]).h; });
@@ -494,7 +493,8 @@ bool rows_vec(const HeadCall& c) {
 
 struct HeadPlan {
   int64_t n_pad, dp, x_plane, w_plane, C, g_plane;
-  int planes, tiles_n, tiles_v, dx_split, dw_split;
+  int planes, tiles_n, tiles_v;
+  WideShare share;
   bool distill;
   char *x, *w, *g;
   float2 *part, *tp;
@@ -516,7 +516,7 @@ struct HeadPlan {
     x = take(planes * x_plane);
     w = w_direct(c) ? nullptr : take(planes * w_plane);
     C = g_plane = 0;
-    dx_split = dw_split = 1;
+    share = WideShare{};
     part = tp = nullptr; ent = rows = coef = cmax = dx_part = dw_part = nullptr; live = nullptr; g = nullptr;
     if (!backward) {
       part = (float2*)take((int64_t)tiles_v * n_pad * 8);
@@ -527,21 +527,15 @@ struct HeadPlan {
         live = (uint8_t*)take(c.N);
       }
     } else {
-      C = kPieceBytes / (planes * 2 * n_pad) / 256 * 256;
-      C = C < 256 ? 256 : C;
-      const int64_t all = round_up(c.V, 256);
-      C = C > all ? all : C;
-      const int64_t pieces = (all + C - 1) / C;  // of equal size
-      C = round_up((all + pieces - 1) / pieces, 256);
+      C = wide_piece(c.N, c.d, c.V, 1, planes, c.dx != nullptr, c.dw != nullptr, planes * 2 * n_pad, &share);
       g_plane = round_up(n_pad * C * 2, 256);
       g = take(planes * g_plane);
       if (c.reduction == 0) {
         coef = (float*)take(n_pad * 4);
         cmax = (float*)take(4);
       }
-      wide_splits(c.N, c.d, C, 1, c.dx != nullptr, c.dw != nullptr, &dx_split, &dw_split);
-      if (c.dx != nullptr) dx_part = (float*)take((int64_t)dx_split * n_pad * dp * 4);
-      if (c.dw != nullptr && dw_split > 1) dw_part = (float*)take((int64_t)dw_split * C * dp * 4);
+      if (c.dx != nullptr) dx_part = (float*)take((int64_t)share.dx_split * n_pad * dp * 4);
+      if (c.dw != nullptr && share.dw_split > 1) dw_part = (float*)take((int64_t)share.dw_split * C * dp * 4);
     }
     bytes = o;
   }
@@ -649,11 +643,11 @@ hipError_t head_bwd(const HeadCall& c) {
     q.g = p.g; q.g_plane = p.g_plane; q.g_half = 0;
     q.dx_part = p.dx_part; q.dx_add = v0 > 0;
     q.dw[0] = c.dw == nullptr ? nullptr : (char*)c.dw + v0 * c.d * es_of(c.dtype); q.dw_part = p.dw_part;
-    q.dx_split = p.dx_split; q.dw_split = p.dw_split; q.hdr = st.hdr; q.unit = unit; q.cmax = p.cmax; q.use_live = 1;
+    q.share = p.share; q.hdr = st.hdr; q.unit = unit; q.cmax = p.cmax; q.use_live = 1;
     HEAD_TRY(launch_wide_products(q, c.stream));
   }
   if (c.dx != nullptr) {
-    const WideFinish f{c.dtype, 0, c.N, p.n_pad, c.d, p.dp, p.dx_split, p.dx_part, st.pos, st.hdr, unit, p.cmax, c.dx};
+    const WideFinish f{c.dtype, 0, c.N, p.n_pad, c.d, p.dp, p.share.dx_split, p.dx_part, st.pos, st.hdr, unit, p.cmax, c.dx};
     HEAD_TRY(launch_wide_finish(f, c.stream));
   }
   return hipSuccess;

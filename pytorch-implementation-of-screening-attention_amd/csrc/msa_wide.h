@@ -107,6 +107,17 @@ __device__ inline float unit_of(const GradUnit& u, const WideHdr* h, const float
   return u.mode == 1 ? u.dloss[0] * u.factor / (float)h->live : u.dloss[0] * u.factor;
 }
 
+// How the two products of a piece are cut: each of dx's tiles into dx_split ranges of its k, dW's into dw_split, a block
+// each.  cost: stages (32 k of a tile) until the last of 512 blocks in flight (two a CU) has ended, as wide_share reckons.
+struct WideShare {
+  int dx_split, dw_split;
+  bool dx_first;
+  int64_t cost;
+};
+WideShare wide_share(int64_t N, int d, int64_t C, int halves, int planes, bool dx, bool dw);
+// The columns of a piece of `rows` weight rows whose G takes `bytes_of_column` a column: 1 GB of G, 512 or 256 MB, by cost.
+int64_t wide_piece(int64_t N, int d, int64_t rows, int halves, int planes, bool dx, bool dw, int64_t bytes_of_column, WideShare* share);
+
 // The backward products of one piece of the weight's rows.
 struct WideProducts {
   int dtype, gated;
@@ -119,18 +130,15 @@ struct WideProducts {
   const char* x; int64_t x_ld, x_plane; int x_rows;           // bytes from row to row, to the second term; readable rows
   const char* w[2]; int64_t w_ld, w_plane; int w_rows;        // the piece's first rows; readable rows from there
   const char* g; int64_t g_plane, g_half;                     // [half][term][n_pad][C]
-  float* dx_part; int dx_add;                                 // [dx_split][n_pad][dp], or null: no dx
+  float* dx_part; int dx_add;                                 // [share.dx_split][n_pad][dp], or null: no dx
   void* dw[2];                                                // the piece's rows of the gradients, or null
-  float* dw_part;                                             // [dw_split][halves][C][dp] where dw_split > 1
-  int dx_split, dw_split;
+  float* dw_part;                                             // [share.dw_split][halves][C][dp] where that is over 1
+  WideShare share;
   const WideHdr* hdr;
   GradUnit unit; const float* cmax;
   int use_live;  // tokens are hdr->live
 };
 hipError_t launch_wide_products(const WideProducts& p, hipStream_t s);
-
-// Blocks that share the k of each tile, for tiles of 256 x 128 of which a CU holds two.
-void wide_splits(int64_t N, int d, int64_t C, int halves, bool dx, bool dw, int* dx_split, int* dw_split);
 
 // dx[n] = factor * sum of the parts' rows pos[n] (pos null: n); rows with pos < 0 are zero.
 struct WideFinish {

@@ -1,6 +1,8 @@
 // Operand rows, scales and the backward products of the wide layers (msa_wide.h).
 #include "msa_wide.h"
 
+#include <string.h>
+
 namespace msa {
 namespace {
 
@@ -139,9 +141,9 @@ struct ProductArgs {
   int64_t N, n_pad;
   int d;
   int64_t dp;
-  int dx_tm, dx_tn, dx_split, dw_tm, dw_tn, dw_split, halves, cols;
-  int dx_blocks;
+  int tm, dx_blocks, dw_blocks, dx_steps, dw_tn, halves, cols;
   int64_t C;
+  WideShare share;
   MmSegs dx_segs, dw_segs;
   const char* x; int64_t x_ld; int x_rows;
   const char* w; int64_t w_ld; int w_rows;
@@ -154,8 +156,10 @@ struct ProductArgs {
   int use_live, gated, vec;
 };
 
-// A block per tile and split: the first dx_blocks take dx[n][m] = sum_v G[n][v] W[v][m], the others dW[v][m] = sum_n
-// G[n][v] x[n][m].  Both in one launch, so that neither leaves CUs idle at its end.
+// A block per tile and range of its k: dx[n][m] = sum_v G[n][v] W[v][m], and dW[v][m] = sum_n G[n][v] x[n][m].  Both in one
+// launch, the longer blocks first, so that neither leaves CUs idle at its end.  Ranges of one tile, and tiles of one block
+// of rows or columns of G, stand side by side: an XCD's blocks then read the same rows of W or x at the same time.  (Cut
+// where 512 equal shares end instead, the blocks start at places of their own in W: 12% slower at 8192 rows.)
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) products_kernel(ProductArgs p) {
   using E = typename Wide<T>::E;
@@ -164,17 +168,17 @@ __global__ void __launch_bounds__(kThreads, 2) products_kernel(ProductArgs p) {
   __shared__ char smem[TX::LDS];
   LdsChar* lds = (LdsChar*)smem;
   const int64_t N = p.use_live ? p.hdr->live : p.N;
-  const bool is_dx = (int)blockIdx.x < p.dx_blocks;
-  const float out_g = unit_of(p.unit, p.hdr, p.cmax) / scale_g<T>(p.hdr, p.gated);
+  const int first = p.share.dx_first ? p.dx_blocks : p.dw_blocks;
+  const bool head = (int)blockIdx.x < first, is_dx = head == p.share.dx_first;
+  const int64_t at = head ? blockIdx.x : (int64_t)blockIdx.x - first;
   if (is_dx) {
-    int64_t t = xcd_order(blockIdx.x, p.dx_blocks);
-    const int split = (int)(t % p.dx_split);
-    t /= p.dx_split;
-    const int tm = (int)(t % p.dx_tm), tn = (int)(t / p.dx_tm);
+    int64_t t = xcd_order(at, p.dx_blocks);
+    const int split = (int)(t % p.share.dx_split);
+    t /= p.share.dx_split;
+    const int tm = (int)(t % p.tm), tn = (int)(t / p.tm);
     const int n0 = tn * 128, m0 = tm * 256;
     if (n0 >= N) return;
-    const int steps = (p.cols + 127) / 128 * 4, from = (int)((int64_t)steps * split / p.dx_split),
-              to = (int)((int64_t)steps * (split + 1) / p.dx_split);
+    const int from = (int)((int64_t)p.dx_steps * split / p.share.dx_split), to = (int)((int64_t)p.dx_steps * (split + 1) / p.share.dx_split);
     typename TX::Acc acc;
     TX::clear(acc);
     const typename TX::Side A{p.w + (int64_t)m0 * 2, (int)(p.dp - m0), p.w_ld, p.w_rows, 0};
@@ -186,27 +190,27 @@ __global__ void __launch_bounds__(kThreads, 2) products_kernel(ProductArgs p) {
     if (p.dx_add) TX::template store_rows<float, true>(lds, out, p.dp, rows, (int)(p.dp - m0), true, fn);
     else TX::template store_rows<float, false>(lds, out, p.dp, rows, (int)(p.dp - m0), true, fn);
   } else {
-    int64_t t = xcd_order((int64_t)blockIdx.x - p.dx_blocks, (int64_t)gridDim.x - p.dx_blocks);
-    const int split = (int)(t % p.dw_split);
-    t /= p.dw_split;
-    const int tm = (int)(t % p.dw_tm);
-    t /= p.dw_tm;
+    int64_t t = xcd_order(at, p.dw_blocks);
+    const int split = (int)(t % p.share.dw_split);
+    t /= p.share.dw_split;
+    const int tm = (int)(t % p.tm);
+    t /= p.tm;
     const int tn = (int)(t % p.dw_tn), half = (int)(t / p.dw_tn);
     const int n0 = tn * 128, m0 = tm * 256;
-    const int steps = (int)((N + 31) / 32), from = (int)((int64_t)steps * split / p.dw_split),
-              to = (int)((int64_t)steps * (split + 1) / p.dw_split);
+    const int steps = (int)((N + 31) / 32), from = (int)((int64_t)steps * split / p.share.dw_split),
+              to = (int)((int64_t)steps * (split + 1) / p.share.dw_split);
     typename TW::Acc acc;
     TW::clear(acc);
     const typename TW::Side A{p.x + (int64_t)m0 * 2, (int)(p.dp - m0), p.x_ld, p.x_rows, 0};
     const typename TW::Side B{p.g + half * p.g_half + (int64_t)n0 * 2, (int)(p.C - n0), p.C * 2, (int)p.n_pad, 0};
     if (to > from) TW::run(acc, lds, A, B, p.dw_segs, from * 32, to - from);
     const int rows = p.cols - n0 < 128 ? p.cols - n0 : 128;
-    const float f = out_g, fx = 1.0f / scale_x<T>(p.hdr);
-    if (p.dw_split > 1) {
+    if (p.share.dw_split > 1) {
       float* out = p.dw_part + (((int64_t)split * p.halves + half) * p.C + n0) * p.dp + m0;
       TW::template store_rows<float, false>(lds, out, p.dp, rows, (int)(p.dp - m0), true,
                                             [&](int i, int j, int g) { return quad<float>([&](int e) { return acc[i][j][4 * g + e]; }); });
     } else {
+      const float f = unit_of(p.unit, p.hdr, p.cmax) / scale_g<T>(p.hdr, p.gated), fx = 1.0f / scale_x<T>(p.hdr);
       T* out = (T*)(half ? p.dw1 : p.dw0) + (int64_t)n0 * p.d + m0;
       TW::template store_rows<T, false>(lds, out, p.d, rows, p.d - m0, p.vec != 0,
                                         [&](int i, int j, int g) { return quad<T>([&](int e) { return acc[i][j][4 * g + e] * f * fx; }); });
@@ -214,34 +218,44 @@ __global__ void __launch_bounds__(kThreads, 2) products_kernel(ProductArgs p) {
   }
 }
 
-// Sums of split tiles in split order, scaled, as rows of T.
+// Sums of parts in their order, scaled, as rows of T.  A wave per row; the second matrix's rows follow the first's.
+struct PartArgs {
+  const float* part; int64_t part_stride, half_stride;
+  int split;
+  int64_t rows;
+  int d, dp;
+  const int* pos;
+  const WideHdr* hdr;
+  GradUnit unit; const float* cmax;
+  int gated, by_x;
+  void* out0; void* out1;
+};
 template <typename T>
-__global__ void __launch_bounds__(kThreads) parts_kernel(const float* part, int64_t part_stride, int split, int64_t rows,
-                                                         int64_t half_stride, int d, int dp, const int* pos, const WideHdr* hdr,
-                                                         GradUnit unit, const float* cmax, int gated, int by_x, T* out0, T* out1) {
+__global__ void __launch_bounds__(kThreads) parts_kernel(PartArgs a) {
   int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  T* out = out0;
-  if (r >= rows) {  // the second weight's rows follow the first's
-    if (out1 == nullptr || (r -= rows) >= rows) return;
-    out = out1;
-    part += half_stride;
+  T* out = (T*)a.out0;
+  const float* part = a.part;
+  if (r >= a.rows) {
+    if (a.out1 == nullptr || (r -= a.rows) >= a.rows) return;
+    out = (T*)a.out1;
+    part += a.half_stride;
   }
-  const int64_t at = pos == nullptr ? r : pos[r];
-  const float f = unit_of(unit, hdr, cmax) / scale_g<T>(hdr, gated), f2 = 1.0f / (by_x ? scale_x<T>(hdr) : scale_w<T>(hdr));
-  for (int c = ((int)threadIdx.x & 63) * 4; c < d; c += 256) {
+  const int64_t at = a.pos == nullptr ? r : a.pos[r];
+  const float f = unit_of(a.unit, a.hdr, a.cmax) / scale_g<T>(a.hdr, a.gated), f2 = 1.0f / (a.by_x ? scale_x<T>(a.hdr) : scale_w<T>(a.hdr));
+  for (int c = ((int)threadIdx.x & 63) * 4; c < a.d; c += 256) {
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     if (at >= 0) {
 #pragma unroll 4
-      for (int s = 0; s < split; ++s) v += *reinterpret_cast<const f32x4*>(part + s * part_stride + at * dp + c);
+      for (int s = 0; s < a.split; ++s) v += *reinterpret_cast<const f32x4*>(part + s * a.part_stride + at * a.dp + c);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = v[e] * f * f2;
     }
-    T* o = out + r * d + c;
-    if (c + 4 <= d && d % 4 == 0) store4(o, v[0], v[1], v[2], v[3]);
+    T* o = out + r * a.d + c;
+    if (c + 4 <= a.d && a.d % 4 == 0) store4(o, v[0], v[1], v[2], v[3]);
     else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (c + e < d) o[e] = from_f<T>(v[e]);
+        if (c + e < a.d) o[e] = from_f<T>(v[e]);
     }
   }
 }
@@ -287,11 +301,16 @@ hipError_t rows_max(const RowsCopies& c, hipStream_t s) {
 template <typename T>
 hipError_t products(const WideProducts& p, hipStream_t s) {
   constexpr int P = Wide<T>::P;
+  const bool dx = p.dx_part != nullptr, dw = p.dw[0] != nullptr;
+  if (!dx && !dw) return hipSuccess;
   ProductArgs a;
-  a.N = p.N; a.n_pad = p.n_pad; a.d = p.d; a.dp = p.dp;
-  a.dx_tm = (int)((p.dp + 255) / 256); a.dx_tn = (int)(p.n_pad / 128); a.dx_split = p.dx_split;
-  a.dw_tm = a.dx_tm; a.dw_tn = (p.cols + 127) / 128; a.dw_split = p.dw_split; a.halves = p.halves; a.cols = p.cols;
-  a.dx_blocks = p.dx_part != nullptr ? a.dx_tm * a.dx_tn * p.dx_split : 0;
+  a.N = p.N; a.n_pad = p.n_pad; a.d = p.d; a.dp = p.dp; a.share = p.share;
+  a.tm = (int)((p.dp + 255) / 256);
+  a.dx_blocks = dx ? a.tm * (int)(p.n_pad / 128) * p.share.dx_split : 0;
+  a.dx_steps = (p.cols + 127) / 128 * 4;
+  a.dw_tn = (p.cols + 127) / 128;
+  a.dw_blocks = dw ? a.tm * a.dw_tn * p.halves * p.share.dw_split : 0;
+  a.halves = p.halves; a.cols = p.cols;
   a.C = p.C;
   // (first, second) terms: low ones first
   int n = 0;
@@ -320,23 +339,25 @@ hipError_t products(const WideProducts& p, hipStream_t s) {
   a.dw0 = p.dw[0]; a.dw1 = p.dw[1]; a.dw_part = p.dw_part;
   a.hdr = p.hdr; a.unit = p.unit; a.cmax = p.cmax; a.use_live = p.use_live; a.gated = p.gated;
   a.vec = (int64_t)p.d * sizeof(T) % 16 == 0 && ((uintptr_t)p.dw[0] & 15) == 0 && ((uintptr_t)p.dw[1] & 15) == 0;
-  const int64_t dw_blocks = p.dw[0] != nullptr ? (int64_t)a.dw_tm * a.dw_tn * p.dw_split * p.halves : 0;
-  const int64_t blocks = a.dx_blocks + dw_blocks;
-  if (blocks == 0) return hipSuccess;
-  hipLaunchKernelGGL(products_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(products_kernel<T>, dim3((unsigned)(a.dx_blocks + a.dw_blocks)), dim3(kThreads), 0, s, a);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || dw_blocks == 0 || p.dw_split == 1) return e;
-  hipLaunchKernelGGL(parts_kernel<T>, dim3((unsigned)(((int64_t)p.cols * p.halves + 3) / 4)), dim3(kThreads), 0, s, p.dw_part,
-                     (int64_t)p.halves * p.C * p.dp, p.dw_split, (int64_t)p.cols, (int64_t)p.C * p.dp, p.d, (int)p.dp,
-                     (const int*)nullptr, p.hdr, p.unit, p.cmax, p.gated, 1, (T*)p.dw[0], (T*)(p.halves == 2 ? p.dw[1] : nullptr));
+  if (e != hipSuccess || !dw || p.share.dw_split == 1) return e;
+  PartArgs q = {};
+  q.part = p.dw_part; q.part_stride = (int64_t)p.halves * p.C * p.dp; q.half_stride = p.C * p.dp; q.split = p.share.dw_split;
+  q.rows = p.cols; q.d = p.d; q.dp = (int)p.dp; q.hdr = p.hdr; q.unit = p.unit; q.cmax = p.cmax; q.gated = p.gated; q.by_x = 1;
+  q.out0 = p.dw[0]; q.out1 = p.halves == 2 ? p.dw[1] : nullptr;
+  hipLaunchKernelGGL(parts_kernel<T>, dim3((unsigned)((q.rows * p.halves + 3) / 4)), dim3(kThreads), 0, s, q);
   return hipGetLastError();
 }
 
 template <typename T>
 hipError_t finish(const WideFinish& f, hipStream_t s) {
   if (f.N == 0) return hipSuccess;
-  hipLaunchKernelGGL(parts_kernel<T>, dim3((unsigned)((f.N + 3) / 4)), dim3(kThreads), 0, s, f.part, f.n_pad * f.dp,
-                     f.split, f.N, (int64_t)0, f.d, (int)f.dp, f.pos, f.hdr, f.unit, f.cmax, f.gated, 0, (T*)f.dx, (T*)nullptr);
+  PartArgs q = {};
+  q.part = f.part; q.part_stride = f.n_pad * f.dp; q.split = f.split;
+  q.rows = f.N; q.d = f.d; q.dp = (int)f.dp; q.pos = f.pos; q.hdr = f.hdr; q.unit = f.unit; q.cmax = f.cmax; q.gated = f.gated;
+  q.out0 = f.dx;
+  hipLaunchKernelGGL(parts_kernel<T>, dim3((unsigned)((f.N + 3) / 4)), dim3(kThreads), 0, s, q);
   return hipGetLastError();
 }
 
@@ -359,16 +380,76 @@ hipError_t launch_wide_finish(const WideFinish& f, hipStream_t s) {
   return f.dtype == 0 ? finish<float>(f, s) : f.dtype == 1 ? finish<bf16>(f, s) : finish<f16>(f, s);
 }
 
-void wide_splits(int64_t N, int d, int64_t C, int halves, bool dx, bool dw, int* dx_split, int* dw_split) {
-  const int64_t tm = (wide_dp(d) + 255) / 256;
-  const int64_t bx = dx ? tm * ((N + 127) / 128) : 0, bw = dw ? tm * (C / 128) * halves : 0;
-  // k of the products in steps of 32, shared so that about 512 blocks have equal parts of at least 8 steps
-  const int64_t kx = halves * (C / 32), kw = (N + 31) / 32;
-  int64_t each = (bx * kx + bw * kw) / 512;
-  if (each < 8) each = 8;
-  const int64_t sx = (kx + each / 2) / each, sw = (kw + each / 2) / each;
-  *dx_split = (int)(sx < 1 ? 1 : sx > 16 ? 16 : sx);
-  *dw_split = (int)(sw < 1 ? 1 : sw > 16 ? 16 : sw);
+// Blocks in flight take the next block of the grid as they end: the time until all `n2` blocks of length l2 have ended that
+// follow n1 of length l1.
+static int64_t two_kinds(int64_t n1, int64_t l1, int64_t n2, int64_t l2) {
+  constexpr int64_t kInFlight = 512;
+  const int64_t r = n1 / kInFlight, more = n1 - r * kInFlight, few = kInFlight - more;
+  const int64_t a = r * l1, b = a + l1;  // `more` places are free at b, the `few` others at a
+  const int64_t end1 = more > 0 ? b : a;
+  if (n2 == 0) return end1;
+  auto fits = [&](int64_t t) { return few * ((t - a) / l2) + (t > b ? more * ((t - b) / l2) : 0) >= n2; };
+  // without a remainder, then the next ends of both groups of places
+  int64_t t = a + (n2 * l2 + few - 1) / few;
+  if (t > b) t = (n2 * l2 + few * a + more * b + kInFlight - 1) / kInFlight;
+  const int64_t ta = a + (t - a + l2 - 1) / l2 * l2, tb = t <= b ? b + l2 : b + (t - b + l2 - 1) / l2 * l2;
+  int64_t lo = ta < tb ? ta : tb, hi = ta < tb ? tb : ta;
+  if (more == 0) lo = hi = ta;
+  t = fits(lo) ? lo : fits(hi) ? hi : lo + l2;
+  return t > end1 ? t : end1;
+}
+
+WideShare wide_share(int64_t N, int d, int64_t C, int halves, int planes, bool dx, bool dw) {
+  // What a block costs beside its stages, in stages: 6 to fill and drain its pipeline, 12 to store a tile rounded, 25 to
+  // store it in fp32 and as much, over all of the card, to add it up (64 MB of 512 tiles at 4 TB/s are 16 us, a stage 0.7).
+  constexpr int64_t kFill = 6, kRounded = 12, kFloat = 25;
+  const int64_t tm = (wide_dp(d) + 255) / 256, segs = planes == 2 ? 3 : 1;
+  const int64_t tx = dx ? tm * ((N + 127) / 128) : 0, kx = C / 32 * segs * halves;
+  const int64_t tw = dw ? tm * (C / 128) * halves : 0, kw = (N + 31) / 32 * segs;
+  constexpr int kCuts[] = {1, 2, 3, 4, 5, 6, 8, 11, 16};
+  WideShare best = {1, 1, true, -1};
+  for (const int sx : kCuts) {
+    if (sx > 1 && (!dx || kx / sx < 8)) break;
+    const int64_t lx = (kx + sx - 1) / sx + kFill + kFloat;
+    for (const int sw : kCuts) {
+      if (sw > 1 && (!dw || kw / sw < 8)) break;
+      const int64_t lw = (kw + sw - 1) / sw + kFill + (sw > 1 ? kFloat : kRounded);
+      const bool first = lx >= lw;
+      const int64_t sum = kFloat * (tx * sx + (sw > 1 ? tw * sw : 0)) / 512;
+      const int64_t cost = sum + (first ? two_kinds(tx * sx, lx, tw * sw, lw) : two_kinds(tw * sw, lw, tx * sx, lx));
+      if (best.cost < 0 || cost < best.cost) best = WideShare{sx, sw, first, cost};
+    }
+  }
+  return best;
+}
+
+int64_t wide_piece(int64_t N, int d, int64_t rows, int halves, int planes, bool dx, bool dw, int64_t bytes_of_column, WideShare* share) {
+  // the sizes of the last call: a backward pass asks twice, for its workspace and for its launches
+  struct Memo { int64_t key[8], C; WideShare share; };
+  static thread_local Memo memo = {{-1}, 0, {}};
+  const int64_t key[8] = {N, d, rows, halves, planes, dx, dw, bytes_of_column};
+  if (memcmp(memo.key, key, sizeof(key)) == 0) {
+    *share = memo.share;
+    return memo.C;
+  }
+  const int64_t all = round_up(rows, 256);
+  int64_t chosen = 0, cost = -1;
+  for (int s = 30; s >= 28; --s) {
+    int64_t C = ((int64_t)1 << s) / bytes_of_column / 256 * 256;
+    C = C < 256 ? 256 : C > all ? all : C;
+    const int64_t pieces = (all + C - 1) / C;  // of equal size
+    C = round_up((all + pieces - 1) / pieces, 256);
+    const WideShare w = wide_share(N, d, C, halves, planes, dx, dw);
+    if (cost < 0 || w.cost * pieces < cost) {
+      cost = w.cost * pieces;
+      chosen = C;
+      *share = w;
+    }
+  }
+  memcpy(memo.key, key, sizeof(key));
+  memo.C = chosen;
+  memo.share = *share;
+  return chosen;
 }
 
 }  // namespace msa

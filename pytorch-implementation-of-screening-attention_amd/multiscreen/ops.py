@@ -641,7 +641,7 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="m
     "none": a loss per row, shaped as labels, of which N = 1 and a few rows are the
     scores of a decoding step.  float32; sums and softmax statistics are too.
     The backward pass forms the logits again, in pieces of the vocabulary of at
-    most 256 MB; their gradient is rounded to hidden's type (float32: 22 bits).
+    most 1 GB; their gradient is rounded to hidden's type (float32: 22 bits).
     """
     hidden, weight = _autocast(hidden, weight)
     _head_checks("linear_cross_entropy", hidden, weight, reduction, labels)
