@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_kernel(GatedArgs a) {
         }
         *reinterpret_cast<LdsTV*>(lds + row * ROW + f * (int)sizeof(T)) = v;
       }
-      __syncthreads();
+      Tl::sync_lds();
       typename Quad<E>::V grads[2][Wide<T>::P][8];  // [dg, du][term], rounded as they are made
       const LdsChar* at = lds + (wn * 32 + (lane & 31)) * ROW + (wm * 64 + 4 * (lane >> 5)) * (int)sizeof(T);
 #pragma unroll
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_kernel(GatedArgs a) {
           }
         }
       }
-      __syncthreads();
+      Tl::sync_lds();
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll

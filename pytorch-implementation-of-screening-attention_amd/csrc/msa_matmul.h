@@ -276,11 +276,19 @@ struct MmTile {
     arrive<0>();
   }
 
+  // The block's barrier for LDS alone: __syncthreads would also wait for the wave's stores to memory.
+  __device__ static inline void sync_lds() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+
   // The block's barrier, with this wave's LDS reads done and at most N of its copies outstanding.
   template <int N>
   __device__ static inline void arrive() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(N) : "memory");
     __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   }
 
   // Writes rows of an output: dst[n ld + m .. + 3] = fn(i, j, g) of registers 4 g .. 4 g + 3 of blocks (i, j), i < MS, for
@@ -309,7 +317,7 @@ struct MmTile {
         const typename Quad<O>::V v = fn(i, g);
         *reinterpret_cast<LdsQuad*>(to + (32 * i + 8 * g) * (int)sizeof(O)) = v;
       }
-    __syncthreads();
+    sync_lds();
 #pragma unroll 4
     for (int u = tid; u < R * CPR; u += NT) {
       const int r = u / CPR, c = (u - r * CPR) * PER, n = (r >> 5) * (BN / WN) + 32 * j + (r & 31);
@@ -327,7 +335,7 @@ struct MmTile {
         }
       }
     }
-    __syncthreads();
+    sync_lds();
   }
 
   // Hides the values from the compiler, which would otherwise keep what it formed from them for a second use.
