@@ -191,16 +191,15 @@ __global__ void __launch_bounds__(kThreads, 2) stats_kernel(StatsArgs a) {
     for (int i = 0; i < Tl::MB; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        acc[i][j][r] *= f;
         mx = fmaxf(mx, acc[i][j][r]);
       }
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    mx = f * fmaxf(mx, __shfl_xor(mx, 32));  // f > 0
     const float at = mx == -INFINITY ? 0.0f : mx;
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < Tl::MB; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(acc[i][j][r] - at);
+      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], f, -at));
     s += __shfl_xor(s, 32);
     if (lane < 32) red[wm][Tl::n_of(wn, lane, j)] = float2{mx, s};
   }
@@ -420,21 +419,27 @@ __global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
   const typename Tl::Side A{a.w + v0 * a.w_ld, vleft, a.w_ld, 0, 0};
   const typename Tl::Side B{a.x + n0 * a.x_ld, (int)(a.n_pad - n0 < 128 ? a.n_pad - n0 : 128), a.x_ld, 0, 0};
   Tl::run(acc, lds, A, B, a.segs, 0, a.ksteps);
-  const float f = a.to_log2 / scale_x<T>(a.hdr) / scale_w<T>(a.hdr), sg = scale_g<T>(a.hdr, 0);
+  const float f = a.to_log2 / scale_x<T>(a.hdr) / scale_w<T>(a.hdr), lg = __is_same(T, bf16) ? 0.0f : 15.0f;  // log2 of scale_g
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
   if (vleft < 256) mask_features<Tl>(acc, vleft, wm, lane, -INFINITY);
 #pragma unroll
   for (int j = 0; j < Tl::NB; ++j) {
     const int64_t n = n0 + Tl::n_of(wn, lane, j);
     const bool ok = n < live;
-    // a row behind the last one has an operand of zeros, lse2 of infinity and so a gradient of zeros
-    const float l = ok ? a.lse2[n] : INFINITY, c = !ok ? 0.0f : a.coef != nullptr ? a.coef[n] * sg : sg;
+    // a row behind the last one has an operand of zeros, lse2 of infinity and so a gradient of zeros; the power of two sg
+    // goes into the exponent
+    const float l = ok ? a.lse2[n] - lg : INFINITY;
 #pragma unroll
     for (int i = 0; i < Tl::MB; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        acc[i][j][r] = c * __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], f, -l));
-      }
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], f, -l));
+    if (a.coef != nullptr) {
+      const float c = ok ? a.coef[n] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < Tl::MB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] *= c;
+    }
   }
   if constexpr (Wide<T>::P == 2) {
     Tl::template store_rows<E, false>(lds, out, a.C, 128, 256, true, [&](int i, int j, int g) {

@@ -55,7 +55,8 @@ struct MmTile {
   static constexpr int NT = 64 * WM * WN;                    // threads
   static constexpr int MB = BM / WM / 32, NB = BN / WN / 32;  // 32x32 blocks of a wave
   static constexpr int ABYTES = BM * kMmK * 2, BBYTES = BN * kMmK * 2, STAGE = ABYTES + BBYTES;
-  static constexpr int LDS = NST * STAGE;
+  static constexpr int STAGED = 32 * WN * (BM * 4 + 16);  // store_tokens of fp32
+  static constexpr int LDS = NST * STAGE > STAGED ? NST * STAGE : STAGED;
   static constexpr int NWAVES = WM * WN;
   static constexpr int AI = ABYTES / 1024 / NWAVES, BI = BBYTES / 1024 / NWAVES;  // copies of 1 KiB a wave issues
   static_assert(AI * NWAVES * 1024 == ABYTES && BI * NWAVES * 1024 == BBYTES, "a stage is whole copies of every wave");

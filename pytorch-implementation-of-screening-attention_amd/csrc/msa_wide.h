@@ -108,7 +108,7 @@ __device__ inline float unit_of(const GradUnit& u, const WideHdr* h, const float
 }
 
 // How the two products of a piece are cut: each of dx's tiles into dx_split ranges of its k, dW's into dw_split, a block
-// each.  cost: stages (32 k of a tile) until the last of 512 blocks in flight (two a CU) has ended, as wide_share reckons.
+// each.  cost: stages (32 k of a tile) until the last of 256 blocks in flight (one a CU) has ended, as wide_share reckons.
 struct WideShare {
   int dx_split, dw_split;
   bool dx_first;

@@ -7,6 +7,11 @@ namespace msa {
 namespace {
 
 constexpr int kThreads = 256;
+// Tokens (or weight rows) of a product's tile.  256 by 256, one block of 8 waves a CU, against two blocks of 256 by 128: a
+// third less goes through LDS for each flop, and its one epilogue behind a long k costs little (the losses' own products,
+// whose k is d, are better off with two blocks, one in its epilogue while the other multiplies).  us of a whole training
+// pass, 128 / 256: 8192 x 50257 x 512 bf16 1855 / 1805, 32768 rows 7640 / 7270, 2867 fp32 rows 2500 / 2260.
+constexpr int kTileN = 256, kProductThreads = 512;
 
 __global__ void hdr_clear_kernel(WideHdr* h) {
   for (int i = (int)threadIdx.x; i < kHdrWords; i += kThreads) reinterpret_cast<uint32_t*>(h)[i] = 0u;
@@ -161,10 +166,10 @@ struct ProductArgs {
 // of rows or columns of G, stand side by side: an XCD's blocks then read the same rows of W or x at the same time.  (Cut
 // where 512 equal shares end instead, the blocks start at places of their own in W: 12% slower at 8192 rows.)
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) products_kernel(ProductArgs p) {
+__global__ void __launch_bounds__(kProductThreads, 2) products_kernel(ProductArgs p) {
   using E = typename Wide<T>::E;
-  using TX = MmTile<E, 256, 128, 2, 2, true, false, false, 3>;
-  using TW = MmTile<E, 256, 128, 2, 2, true, true, false, 3>;
+  using TX = MmTile<E, 256, kTileN, 2, 4, true, false, false, 4>;
+  using TW = MmTile<E, 256, kTileN, 2, 4, true, true, false, 4>;
   __shared__ char smem[TX::LDS];
   LdsChar* lds = (LdsChar*)smem;
   const int64_t N = p.use_live ? p.hdr->live : p.N;
@@ -176,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, 2) products_kernel(ProductArgs p) {
     const int split = (int)(t % p.share.dx_split);
     t /= p.share.dx_split;
     const int tm = (int)(t % p.tm), tn = (int)(t / p.tm);
-    const int n0 = tn * 128, m0 = tm * 256;
+    const int n0 = tn * kTileN, m0 = tm * 256;
     if (n0 >= N) return;
     const int from = (int)((int64_t)p.dx_steps * split / p.share.dx_split), to = (int)((int64_t)p.dx_steps * (split + 1) / p.share.dx_split);
     typename TX::Acc acc;
@@ -186,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 2) products_kernel(ProductArgs p) {
     if (to > from) TX::run(acc, lds, A, B, p.dx_segs, from * 32, to - from);
     float* out = p.dx_part + ((int64_t)split * p.n_pad + n0) * p.dp + m0;
     auto fn = [&](int i, int j, int g) { return quad<float>([&](int e) { return acc[i][j][4 * g + e]; }); };
-    const int rows = (int)(N - n0 < 128 ? N - n0 : 128);
+    const int rows = (int)(N - n0 < kTileN ? N - n0 : kTileN);
     if (p.dx_add) TX::template store_rows<float, true>(lds, out, p.dp, rows, (int)(p.dp - m0), true, fn);
     else TX::template store_rows<float, false>(lds, out, p.dp, rows, (int)(p.dp - m0), true, fn);
   } else {
@@ -196,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 2) products_kernel(ProductArgs p) {
     const int tm = (int)(t % p.tm);
     t /= p.tm;
     const int tn = (int)(t % p.dw_tn), half = (int)(t / p.dw_tn);
-    const int n0 = tn * 128, m0 = tm * 256;
+    const int n0 = tn * kTileN, m0 = tm * 256;
     const int steps = (int)((N + 31) / 32), from = (int)((int64_t)steps * split / p.share.dw_split),
               to = (int)((int64_t)steps * (split + 1) / p.share.dw_split);
     typename TW::Acc acc;
@@ -204,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 2) products_kernel(ProductArgs p) {
     const typename TW::Side A{p.x + (int64_t)m0 * 2, (int)(p.dp - m0), p.x_ld, p.x_rows, 0};
     const typename TW::Side B{p.g + half * p.g_half + (int64_t)n0 * 2, (int)(p.C - n0), p.C * 2, (int)p.n_pad, 0};
     if (to > from) TW::run(acc, lds, A, B, p.dw_segs, from * 32, to - from);
-    const int rows = p.cols - n0 < 128 ? p.cols - n0 : 128;
+    const int rows = p.cols - n0 < kTileN ? p.cols - n0 : kTileN;
     if (p.share.dw_split > 1) {
       float* out = p.dw_part + (((int64_t)split * p.halves + half) * p.C + n0) * p.dp + m0;
       TW::template store_rows<float, false>(lds, out, p.dp, rows, (int)(p.dp - m0), true,
@@ -306,9 +311,9 @@ hipError_t products(const WideProducts& p, hipStream_t s) {
   ProductArgs a;
   a.N = p.N; a.n_pad = p.n_pad; a.d = p.d; a.dp = p.dp; a.share = p.share;
   a.tm = (int)((p.dp + 255) / 256);
-  a.dx_blocks = dx ? a.tm * (int)(p.n_pad / 128) * p.share.dx_split : 0;
+  a.dx_blocks = dx ? a.tm * (int)((p.n_pad + kTileN - 1) / kTileN) * p.share.dx_split : 0;
   a.dx_steps = (p.cols + 127) / 128 * 4;
-  a.dw_tn = (p.cols + 127) / 128;
+  a.dw_tn = (p.cols + kTileN - 1) / kTileN;
   a.dw_blocks = dw ? a.tm * a.dw_tn * p.halves * p.share.dw_split : 0;
   a.halves = p.halves; a.cols = p.cols;
   a.C = p.C;
@@ -339,7 +344,7 @@ hipError_t products(const WideProducts& p, hipStream_t s) {
   a.dw0 = p.dw[0]; a.dw1 = p.dw[1]; a.dw_part = p.dw_part;
   a.hdr = p.hdr; a.unit = p.unit; a.cmax = p.cmax; a.use_live = p.use_live; a.gated = p.gated;
   a.vec = (int64_t)p.d * sizeof(T) % 16 == 0 && ((uintptr_t)p.dw[0] & 15) == 0 && ((uintptr_t)p.dw[1] & 15) == 0;
-  hipLaunchKernelGGL(products_kernel<T>, dim3((unsigned)(a.dx_blocks + a.dw_blocks)), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(products_kernel<T>, dim3((unsigned)(a.dx_blocks + a.dw_blocks)), dim3(kProductThreads), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !dw || p.share.dw_split == 1) return e;
   PartArgs q = {};
@@ -382,8 +387,8 @@ hipError_t launch_wide_finish(const WideFinish& f, hipStream_t s) {
 
 // Blocks in flight take the next block of the grid as they end: the time until all `n2` blocks of length l2 have ended that
 // follow n1 of length l1.
+constexpr int64_t kInFlight = 256;  // a block a CU
 static int64_t two_kinds(int64_t n1, int64_t l1, int64_t n2, int64_t l2) {
-  constexpr int64_t kInFlight = 512;
   const int64_t r = n1 / kInFlight, more = n1 - r * kInFlight, few = kInFlight - more;
   const int64_t a = r * l1, b = a + l1;  // `more` places are free at b, the `few` others at a
   const int64_t end1 = more > 0 ? b : a;
@@ -400,12 +405,12 @@ static int64_t two_kinds(int64_t n1, int64_t l1, int64_t n2, int64_t l2) {
 }
 
 WideShare wide_share(int64_t N, int d, int64_t C, int halves, int planes, bool dx, bool dw) {
-  // What a block costs beside its stages, in stages: 6 to fill and drain its pipeline, 12 to store a tile rounded, 25 to
-  // store it in fp32 and as much, over all of the card, to add it up (64 MB of 512 tiles at 4 TB/s are 16 us, a stage 0.7).
-  constexpr int64_t kFill = 6, kRounded = 12, kFloat = 25;
+  // What a block costs beside its stages, in stages: 12 to fill and drain its pipeline, 12 to store a tile rounded, 25 to
+  // store it in fp32 and as much, over all of the card, to add it up (64 MB of 256 tiles at 4 TB/s are 16 us, a stage 0.7).
+  constexpr int64_t kFill = 12, kRounded = 12, kFloat = 25;
   const int64_t tm = (wide_dp(d) + 255) / 256, segs = planes == 2 ? 3 : 1;
-  const int64_t tx = dx ? tm * ((N + 127) / 128) : 0, kx = C / 32 * segs * halves;
-  const int64_t tw = dw ? tm * (C / 128) * halves : 0, kw = (N + 31) / 32 * segs;
+  const int64_t tx = dx ? tm * ((N + kTileN - 1) / kTileN) : 0, kx = C / 32 * segs * halves;
+  const int64_t tw = dw ? tm * (C / kTileN) * halves : 0, kw = (N + 31) / 32 * segs;
   constexpr int kCuts[] = {1, 2, 3, 4, 5, 6, 8, 11, 16};
   WideShare best = {1, 1, true, -1};
   for (const int sx : kCuts) {
@@ -415,7 +420,7 @@ WideShare wide_share(int64_t N, int d, int64_t C, int halves, int planes, bool d
       if (sw > 1 && (!dw || kw / sw < 8)) break;
       const int64_t lw = (kw + sw - 1) / sw + kFill + (sw > 1 ? kFloat : kRounded);
       const bool first = lx >= lw;
-      const int64_t sum = kFloat * (tx * sx + (sw > 1 ? tw * sw : 0)) / 512;
+      const int64_t sum = kFloat * (tx * sx + (sw > 1 ? tw * sw : 0)) / kInFlight;
       const int64_t cost = sum + (first ? two_kinds(tx * sx, lx, tw * sw, lw) : two_kinds(tw * sw, lw, tx * sx, lx));
       if (best.cost < 0 || cost < best.cost) best = WideShare{sx, sw, first, cost};
     }
