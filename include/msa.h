@@ -396,9 +396,10 @@ int msa_verify(const msa_verify_args* args, void* stream);
  * either may be null.  The gradient of the logits is formed in pieces of the
  * vocabulary, rounded to dtype (fp32: to two fp16 terms, 22 bits) and multiplied
  * with fp32 sums.
- * state: msa_head_state_bytes, kept from forward to backward.  workspace:
- * msa_head_workspace_bytes of the same arguments (backward 0 or 1; state,
- * loss, dloss and workspace are not looked at), scratch of the call.
+ * state: msa_head_state_bytes, kept from forward to backward, or null for a forward
+ * pass that no backward pass follows.  workspace: msa_head_workspace_bytes of the
+ * same arguments (backward 0 or 1; of state only whether it is null; loss, dloss
+ * and workspace are not looked at), scratch of the call.
  * 1 <= d <= 65536, V < 2^26, N <= 2^24, N K < 2^32, N d <= 2^38, V d <= 2^37, (N / 128)
  * (V / 128) < 2^24.  No atomics on sums: equal calls give bitwise equal results.
  */

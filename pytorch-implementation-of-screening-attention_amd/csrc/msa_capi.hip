@@ -719,7 +719,8 @@ static int head_run(const msa_head_args* a, int backward, void* stream) {
   msa::HeadCall c;
   const int rc = head_call(a, &c);
   if (rc != MSA_OK) return rc;
-  if (a->state == nullptr || a->state_bytes < msa::head_state_bytes(c.N, c.K))
+  if (backward ? a->state == nullptr || a->state_bytes < msa::head_state_bytes(c.N, c.K)
+               : a->state != nullptr && a->state_bytes < msa::head_state_bytes(c.N, c.K))
     return fail(MSA_ERR_WORKSPACE, "head state holds %zu bytes, %zu needed", (size_t)a->state_bytes, msa::head_state_bytes(c.N, c.K));
   const size_t need = msa::head_workspace_bytes(c, backward);
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need))

@@ -1,7 +1,6 @@
 // Gated feed-forward: h = act(x Wg^T) * (x Wu^T) in one kernel, and its gradients.
 //   dg = dh u act'(g), du = dh act(g);  dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x
-// A tile's A rows alternate between the two weights by 64, so that a wave holds a feature's g and u of the same token
-// and the activation and the product happen in registers: h is written once, g and u never.  The backward pass forms g
+// A tile's A rows alternate between the two weights by 16, so that a lane holds a feature's g and u of the same token and the activation and the product happen in registers: h is written once, g and u never.  The backward pass forms g
 // and u again (keeping them rounded would cost 4 N F bytes and a rounding), in pieces of the features (1 GB of dg and
 // du, or 256 features), then takes the two products of msa_wide.hip.
 #include "msa_wide.h"
@@ -54,20 +53,25 @@ struct GatedArgs {
   char* g; int64_t C, plane, half;
 };
 
-template <typename T, int ACT, bool BWD>
-__global__ void __launch_bounds__(kThreads, 2) gated_kernel(GatedArgs a) {
+// Tl: 128 features of 128 tokens, or 32 of 32 for few tokens (forward only).
+template <typename E> using GatedTile = MmTile<E, 256, 128, 2, 2, false, false, true, 3>;
+template <typename E> using GatedFew = MmTile<E, 64, 32, 2, 1, false, false, true, 8>;
+constexpr int kFew = 32;
+
+template <typename T, int ACT, bool BWD, typename Tl>
+__global__ void __launch_bounds__(Tl::THREADS, 2) gated_kernel(GatedArgs a) {
   using E = typename Wide<T>::E;
-  using Tl = MmTile<E, 256, 128, 2, 2, false, false, true, 3>;
+  constexpr int BF = Tl::TILE_M / 2, BN = Tl::TILE_N;
   __shared__ char smem[Tl::LDS];
   LdsChar* lds = (LdsChar*)smem;
   int tf, tn;
   patch_order(xcd_order(blockIdx.x, gridDim.x), a.tiles_f, a.tiles_n, 8, tf, tn);
-  const int64_t n0 = (int64_t)tn * 128;
-  const int f0 = tf * 128;
+  const int64_t n0 = (int64_t)tn * BN;
+  const int f0 = tf * BF;
   typename Tl::Acc acc;
   Tl::clear(acc);
-  const int fleft = a.cols - f0 < 128 ? a.cols - f0 : 128;
-  const int rows = (int)(a.N - n0 < 128 ? a.N - n0 : 128);
+  const int fleft = a.cols - f0 < BF ? a.cols - f0 : BF;
+  const int rows = (int)(a.N - n0 < BN ? a.N - n0 : BN);
   const typename Tl::Side A{a.w + f0 * a.w_ld, fleft, a.w_ld, 0, a.up};
   const typename Tl::Side B{a.x + n0 * a.x_ld, rows, a.x_ld, 0, 0};
   Tl::run(acc, lds, A, B, a.segs, 0, a.ksteps);
@@ -78,8 +82,8 @@ __global__ void __launch_bounds__(kThreads, 2) gated_kernel(GatedArgs a) {
   }
   if constexpr (!BWD) {
     T* out = (T*)a.h + n0 * a.h_ld + f0;
-    Tl::template store_rows<T, false, 2>(lds, out, a.h_ld, rows, fleft, a.vec != 0, [&](int i, int j, int q) {
-      return quad<T>([&](int e) { return act_of<ACT>(acc[i][j][4 * q + e] * f1 * f2) * (acc[i + 2][j][4 * q + e] * f1 * f2); });
+    Tl::store_dual(lds, out, a.h_ld, rows, fleft, a.vec != 0, [&](int i, int j, int q) {
+      return quad<T>([&](int e) { return act_of<ACT>(acc[i][j][4 * q + e] * f1 * f2) * (acc[i][j][4 * q + e + 8] * f1 * f2); });
     });
   } else {
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
@@ -115,8 +119,8 @@ __global__ void __launch_bounds__(kThreads, 2) gated_kernel(GatedArgs a) {
         const T4 d = *reinterpret_cast<const LdsT4*>(at + 8 * q * (int)sizeof(T));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int i = q >> 2, r = 4 * (q & 3) + e;
-          const float g = acc[i][j][r] * f1 * f2, u = acc[i + 2][j][r] * f1 * f2;
+          const int i = q >> 1, r = 4 * (q & 1) + e;  // features 16 i + 8 (q & 1) + ...: 8 q
+          const float g = acc[i][j][r] * f1 * f2, u = acc[i][j][r + 8] * f1 * f2;
           float act, slope;
           act_slope<ACT>(g, act, slope);
           const float ds = (float)d[e] * sg;
@@ -173,7 +177,7 @@ struct GatedPlan {
     char* p = (char*)c.workspace;
     size_t o = 0;
     auto take = [&](int64_t bytes) { char* q = p + o; o += (size_t)round_up(bytes, 256); return q; };
-    hdr = (WideHdr*)take(sizeof(WideHdr));
+    hdr = planes == 2 || (backward && c.dtype == 2) ? (WideHdr*)take(sizeof(WideHdr)) : nullptr;  // scales: not of bf16
     x = direct(c, c.x, c.x_ld) ? nullptr : take(planes * x_plane);
     w = direct(c, c.w[0], c.w_ld[0]) && direct(c, c.w[1], c.w_ld[1]) && c.w_ld[0] == c.w_ld[1] ? nullptr : take(2 * planes * w_plane);
     C = g_plane = 0;
@@ -231,15 +235,18 @@ GatedArgs args_of(const GatedCall& c, const GatedPlan& p, const GatedOperands& o
   GatedArgs a = {};
   a.x = o.x; a.x_ld = o.x_ld; a.N = c.N; a.n_pad = p.n_pad;
   a.w = o.w[0] + f0 * o.w_ld; a.w_ld = o.w_ld; a.up = o.w[1] - o.w[0]; a.cols = cols;
-  a.segs = o.segs; a.ksteps = (int)(p.dp / 32); a.tiles_f = (cols + 127) / 128; a.tiles_n = (int)(p.n_pad / 128);
+  a.segs = o.segs; a.ksteps = (int)(p.dp / 32);
   a.hdr = p.hdr;
   return a;
 }
 
-template <typename T, bool BWD>
-hipError_t launch(const GatedArgs& a, int act, hipStream_t s) {
-  auto* k = act == 0 ? gated_kernel<T, 0, BWD> : gated_kernel<T, 1, BWD>;
-  hipLaunchKernelGGL(k, dim3((unsigned)((int64_t)a.tiles_f * a.tiles_n)), dim3(kThreads), 0, s, a);
+template <typename T, bool BWD, template <typename> class Tile>
+hipError_t launch(GatedArgs a, int act, hipStream_t s) {
+  using Tl = Tile<typename Wide<T>::E>;
+  a.tiles_f = (a.cols + Tl::TILE_M / 2 - 1) / (Tl::TILE_M / 2);
+  a.tiles_n = (int)((a.N + Tl::TILE_N - 1) / Tl::TILE_N);
+  auto* k = act == 0 ? gated_kernel<T, 0, BWD, Tl> : gated_kernel<T, 1, BWD, Tl>;
+  hipLaunchKernelGGL(k, dim3((unsigned)((int64_t)a.tiles_f * a.tiles_n)), dim3(Tl::THREADS), 0, s, a);
   return hipGetLastError();
 }
 
@@ -252,7 +259,7 @@ hipError_t gated_fwd(const GatedCall& c) {
   GatedArgs a = args_of(c, p, o, 0, c.F);
   a.h = c.h; a.h_ld = c.F;
   a.vec = (int64_t)c.F * sizeof(T) % 16 == 0 && ((uintptr_t)c.h & 15) == 0;
-  return launch<T, false>(a, c.act, c.stream);
+  return c.N <= kFew ? launch<T, false, GatedFew>(a, c.act, c.stream) : launch<T, false, GatedTile>(a, c.act, c.stream);
 }
 
 template <typename T>
@@ -274,7 +281,7 @@ hipError_t gated_bwd(const GatedCall& c) {
     a.dh = (const T*)c.dh + f0; a.dh_ld = c.dh_ld;
     a.vec = c.dh_ld * sizeof(T) % 16 == 0 && ((uintptr_t)c.dh & 15) == 0;
     a.g = p.g; a.C = p.C; a.plane = p.g_plane; a.half = p.planes * p.g_plane;
-    GATED_TRY((launch<T, true>(a, c.act, c.stream)));
+    GATED_TRY((launch<T, true, GatedTile>(a, c.act, c.stream)));
     WideProducts q = {};
     q.dtype = c.dtype; q.gated = 1; q.N = c.N; q.n_pad = p.n_pad; q.d = c.d; q.dp = p.dp; q.halves = 2; q.cols = cols; q.C = p.C;
     q.x = o.x; q.x_ld = o.x_ld; q.x_plane = p.x_plane; q.x_rows = o.x_rows;

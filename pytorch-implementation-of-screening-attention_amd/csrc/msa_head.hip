@@ -142,13 +142,13 @@ __global__ void __launch_bounds__(kThreads) teacher_kernel(const L* logits, int6
 // The product's maxima and sums
 // ---------------------------------------------------------------------------
 struct StatsArgs {
-  const char* x; int64_t x_ld; int64_t n_pad;
+  const char* x; int64_t x_ld; int64_t rows;  // readable rows
   const char* w; int64_t w_ld; int64_t V;
   MmSegs segs;
   int ksteps, tiles_v, tiles_n;
   float to_log2;  // log2(e) / T
   const WideHdr* hdr;
-  float2* part;  // [tiles_v][n_pad]
+  float2* part; int64_t part_ld;  // [tiles_v][part_ld]
 };
 
 // Features from `left` on become v: only the last tile along the vocabulary pays for the comparisons.
@@ -164,35 +164,42 @@ __device__ inline void mask_features(typename Tl::Acc& acc, int left, int wm, in
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) stats_kernel(StatsArgs a) {
-  using E = typename Wide<T>::E;
-  using Tl = MmTile<E, 256, 128, 2, 2, false, false, false, 3>;
+// 256 tokens of the vocabulary by 128 rows, or 64 by 32 for few rows, whose time is the weight's stream: small tiles in all
+// CUs with seven stages ahead.  16 rows of 512 over 50257 tokens take 16 us with either (51 MB: 10 us of stream behind a
+// launch and a first load), but only the small one reads a row's part of x once a tile.
+template <typename E> using HeadTile = MmTile<E, 256, 128, 2, 2, false, false, false, 3>;
+template <typename E> using HeadFew = MmTile<E, 64, 32, 2, 1, false, false, false, 8>;
+constexpr int kFew = 32;
+
+template <typename T, typename Tl>
+__global__ void __launch_bounds__(Tl::THREADS, 2) stats_kernel(StatsArgs a) {
+  constexpr int BM = Tl::TILE_M, BN = Tl::TILE_N, WM = Tl::WAVES_M;
   __shared__ char smem[Tl::LDS];
   LdsChar* lds = (LdsChar*)smem;
   int tv, tn;
   patch_order(xcd_order(blockIdx.x, gridDim.x), a.tiles_v, a.tiles_n, 8, tv, tn);
-  const int64_t v0 = (int64_t)tv * 256, n0 = (int64_t)tn * 128;
-  if (n0 >= a.hdr->live) return;
+  const int64_t v0 = (int64_t)tv * BM, n0 = (int64_t)tn * BN;
+  const int64_t rows = a.hdr != nullptr ? a.hdr->live : a.rows;  // null: the rows as they are
+  if (n0 >= rows) return;
   typename Tl::Acc acc;
   Tl::clear(acc);
-  const int vleft = (int)(a.V - v0 < 256 ? a.V - v0 : 256);
+  const int vleft = (int)(a.V - v0 < BM ? a.V - v0 : BM);
+  const int readable = (int)(a.rows - n0 < BN ? a.rows - n0 : BN);
   const typename Tl::Side A{a.w + v0 * a.w_ld, vleft, a.w_ld, 0, 0};
-  const typename Tl::Side B{a.x + n0 * a.x_ld, (int)(a.n_pad - n0 < 128 ? a.n_pad - n0 : 128), a.x_ld, 0, 0};
+  const typename Tl::Side B{a.x + n0 * a.x_ld, readable, a.x_ld, 0, 0};
   Tl::run(acc, lds, A, B, a.segs, 0, a.ksteps);
-  const float f = a.to_log2 / scale_x<T>(a.hdr) / scale_w<T>(a.hdr);
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
-  __shared__ float2 red[2][128];
-  if (vleft < 256) mask_features<Tl>(acc, vleft, wm, lane, -INFINITY);
+  float f = a.to_log2;
+  if constexpr (Wide<T>::P == 2) f = f / scale_x<T>(a.hdr) / scale_w<T>(a.hdr);
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave % WM, wn = wave / WM;
+  __shared__ float2 red[WM][BN];
+  if (vleft < BM) mask_features<Tl>(acc, vleft, wm, lane, -INFINITY);
 #pragma unroll
   for (int j = 0; j < Tl::NB; ++j) {
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < Tl::MB; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        mx = fmaxf(mx, acc[i][j][r]);
-      }
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc[i][j][r]);
     mx = f * fmaxf(mx, __shfl_xor(mx, 32));  // f > 0
     const float at = mx == -INFINITY ? 0.0f : mx;
     float s = 0.0f;
@@ -204,19 +211,21 @@ __global__ void __launch_bounds__(kThreads, 2) stats_kernel(StatsArgs a) {
     if (lane < 32) red[wm][Tl::n_of(wn, lane, j)] = float2{mx, s};
   }
   __syncthreads();
-  if (threadIdx.x < 128) {
+  if ((int)threadIdx.x < BN && (int)threadIdx.x < readable) {
     const float2 p = red[0][threadIdx.x], q = red[1][threadIdx.x];
+    static_assert(WM == 2, "two waves share a row's features");
     const float m = fmaxf(p.x, q.x), at = m == -INFINITY ? 0.0f : m;
-    a.part[(int64_t)tv * a.n_pad + n0 + threadIdx.x] =
+    a.part[(int64_t)tv * a.part_ld + n0 + threadIdx.x] =
         float2{m, p.y * __builtin_amdgcn_exp2f(p.x - at) + q.y * __builtin_amdgcn_exp2f(q.x - at)};
   }
 }
 
 // ---------------------------------------------------------------------------
-// A row's sum over the tiles, its targets' logits and its loss.  A block takes 8 rows: first 32 groups of 8 lanes
+// A row's sum over the tiles, its targets' logits and its loss.  A block takes up to 8 rows: first its threads
 // share the tiles, then 16 lanes take a target at a time (a dot product of d terms).
+// Few rows are spread over more blocks.
 // ---------------------------------------------------------------------------
-constexpr int kRows = 8;
+constexpr int kRows = 8;  // of a block, at most
 struct RowsArgs {
   const void* x; int64_t x_ld;
   const void* w; int64_t w_ld;
@@ -224,10 +233,10 @@ struct RowsArgs {
   const float2* tp;  // null: cross entropy
   const float* ent;
   const float2* part; int64_t part_ld; int tiles;
-  int64_t N, V; int d, K, vec;
+  int64_t N, V, ignore; int d, K, vec, rows;
   float temperature;
-  const int* pos;
-  float* lse2; float* t; float* loss;
+  const int* pos;  // null: every row whose id is not `ignore`, in its own place
+  float* lse2; float* t; float* loss;  // lse2, t: null where no gradient follows
 };
 
 // PER neighbours of a row, zeros past its end.
@@ -250,45 +259,49 @@ __device__ inline void load_vec(const T* p, int c, int d, bool vec, T (&v)[16 / 
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
-  __shared__ float2 red[32][kRows];
+  __shared__ float2 red[kThreads];
   __shared__ float2 stat[kRows];  // the row's maximum and log2 of its sum
   __shared__ int place[kRows];    // the row's place in the operand, -1: it does not count
   __shared__ float terms[kRows][kHeadMaxK];
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t first = (int64_t)blockIdx.x * kRows;
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  const int64_t first = (int64_t)blockIdx.x * a.rows;
   {
-    const int r = tid & 7, g = tid >> 3;
-    const int at = first + r < a.N ? a.pos[first + r] : -1;
+    const int r = tid & (a.rows - 1), g = tid / a.rows, groups = kThreads / a.rows;  // rows is a power of two
+    int at = -1;
+    if (first + r < a.N) at = a.pos != nullptr ? a.pos[first + r] : a.ids[(first + r) * a.ids_ld] == a.ignore ? -1 : (int)(first + r);
     float m = -INFINITY, s = 0.0f;
+    auto add = [&](float2 p) {
+      const float mn = fmaxf(m, p.x), b = mn == -INFINITY ? 0.0f : mn;
+      s = s * __builtin_amdgcn_exp2f(m - b) + p.y * __builtin_amdgcn_exp2f(p.x - b);
+      m = mn;
+    };
     if (at >= 0) {
-      for (int t = g; t < a.tiles; t += 32 * 4) {
+      for (int t = g; t < a.tiles; t += groups * 4) {
         float2 p[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) p[q] = t + 32 * q < a.tiles ? a.part[(int64_t)(t + 32 * q) * a.part_ld + at] : float2{-INFINITY, 0.0f};
+        for (int q = 0; q < 4; ++q) p[q] = t + groups * q < a.tiles ? a.part[(int64_t)(t + groups * q) * a.part_ld + at] : float2{-INFINITY, 0.0f};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float mn = fmaxf(m, p[q].x), b = mn == -INFINITY ? 0.0f : mn;
-          s = s * __builtin_amdgcn_exp2f(m - b) + p[q].y * __builtin_amdgcn_exp2f(p[q].x - b);
-          m = mn;
-        }
+        for (int q = 0; q < 4; ++q) add(p[q]);
       }
     }
-    red[g][r] = float2{m, s};
-    if (g == 0) place[r] = at;
+    red[tid] = float2{m, s};
+    if (tid < kRows) place[tid] = -1;
     __syncthreads();
-    if (tid < kRows) {
-      float mm = -INFINITY, ss = 0.0f;
-      for (int q = 0; q < 32; ++q) mm = fmaxf(mm, red[q][tid].x);
-      const float b = mm == -INFINITY ? 0.0f : mm;
-      for (int q = 0; q < 32; ++q) ss += red[q][tid].y * __builtin_amdgcn_exp2f(red[q][tid].x - b);
-      stat[tid] = float2{mm, log2f(ss)};
+    if (g == 0) place[r] = at;
+    for (int o = kThreads / 2; o >= a.rows; o >>= 1) {
+      if (tid < o) {
+        add(red[tid + o]);
+        red[tid] = float2{m, s};
+      }
+      __syncthreads();
     }
+    if (tid < a.rows) stat[tid] = float2{m, log2f(s)};
     __syncthreads();
   }
   const float to_log2 = kLog2e / a.temperature;
   constexpr int PER = 16 / (int)sizeof(T);
   const int l16 = lane & 15;
-  for (int e = tid >> 4; e < kRows * a.K; e += 16) {
+  for (int e = tid >> 4; e < a.rows * a.K; e += 16) {
     const int r = e / a.K, k = e - r * a.K;
     if (place[r] < 0) continue;  // alike in the 16 lanes
     const int64_t n = first + r, id = a.ids[n * a.ids_ld + k];
@@ -318,14 +331,14 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
     }
     if (l16 == 0) {
       terms[r][k] = term;
-      a.t[n * a.K + k] = t;
+      if (a.t != nullptr) a.t[n * a.K + k] = t;
     }
   }
   __syncthreads();
   {
     const int r = tid >> 5, l = tid & 31;
     const int64_t n = first + r;
-    if (n < a.N) {
+    if (r < a.rows && n < a.N) {
       const int at = place[r];
       float away = 0.0f;
       if (at >= 0)
@@ -337,7 +350,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
         if (a.tp != nullptr && at >= 0) loss = a.temperature * a.temperature * (loss + a.ent[n]);
         a.loss[n] = at >= 0 ? loss : 0.0f;
         // a target outside the vocabulary makes the row NaN, its gradient too
-        if (at >= 0) a.lse2[at] = away == away ? stat[r].x + stat[r].y : NAN;
+        if (at >= 0 && a.lse2 != nullptr) a.lse2[at] = away == away ? stat[r].x + stat[r].y : NAN;
       }
     }
   }
@@ -496,12 +509,19 @@ bool rows_vec(const HeadCall& c) {
   return c.d % per == 0 && c.x_ld % per == 0 && c.w_ld % per == 0 && (((uintptr_t)c.x | (uintptr_t)c.w) & 15) == 0;
 }
 
+// Scores of a few rows without a gradient: the rows are operands as they are, and none is taken out.
+constexpr int64_t kDirectRows = 1024;
+bool x_direct(const HeadCall& c) {
+  return c.state == nullptr && c.teacher == nullptr && c.reduction == 0 && c.N <= kDirectRows && w_direct(c) &&
+         ((uintptr_t)c.x & 15) == 0 && c.x_ld % 8 == 0 && c.x_ld * 2 * 256 < ((int64_t)1 << 32);
+}
+
 struct HeadPlan {
   int64_t n_pad, dp, x_plane, w_plane, C, g_plane;
   int planes, tiles_n, tiles_v;
   WideShare share;
-  bool distill;
-  char *x, *w, *g;
+  bool distill, few, direct;  // direct: x is used as it is
+  char *x, *w, *g, *state = nullptr;
   float2 *part, *tp;
   float *ent, *rows, *coef, *cmax, *dx_part, *dw_part;
   uint8_t* live;
@@ -514,17 +534,20 @@ struct HeadPlan {
     x_plane = round_up(n_pad * dp * 2, 256);
     w_plane = round_up(c.V * dp * 2, 256);
     tiles_n = (int)(n_pad / 128);
-    tiles_v = (int)((c.V + 255) / 256);
+    few = c.N <= kFew;
+    tiles_v = (int)(few ? (c.V + 63) / 64 : (c.V + 255) / 256);
     char* p = (char*)c.workspace;
     size_t o = 0;
     auto take = [&](int64_t bytes) { char* q = p + o; o += (size_t)round_up(bytes, 256); return q; };
-    x = take(planes * x_plane);
+    direct = !backward && x_direct(c);
+    x = direct ? nullptr : take(planes * x_plane);
     w = w_direct(c) ? nullptr : take(planes * w_plane);
     C = g_plane = 0;
     share = WideShare{};
     part = tp = nullptr; ent = rows = coef = cmax = dx_part = dw_part = nullptr; live = nullptr; g = nullptr;
     if (!backward) {
       part = (float2*)take((int64_t)tiles_v * n_pad * 8);
+      state = c.state == nullptr && !direct ? take((int64_t)HeadState(nullptr, c.N, c.K).bytes) : (char*)c.state;
       if (c.reduction != 0) rows = (float*)take(c.N * 4);
       if (distill) {
         tp = (float2*)take(c.N * c.K * 8);
@@ -574,7 +597,7 @@ hipError_t operands(const HeadCall& c, const HeadPlan& p, const HeadState& st, b
 template <typename T>
 hipError_t head_fwd(const HeadCall& c) {
   const HeadPlan p(c, 0);
-  const HeadState st(c.state, c.N, c.K);
+  const HeadState st(p.state, c.N, c.K);
   const unsigned row_blocks = (unsigned)((c.N + 3) / 4);
   const float inv_t = 1.0f / c.temperature;
   if (p.distill && c.N > 0) {
@@ -586,22 +609,30 @@ hipError_t head_fwd(const HeadCall& c) {
       hipLaunchKernelGGL(teacher_kernel<f16>, dim3(row_blocks), dim3(kThreads), 0, c.stream, (const f16*)c.teacher, c.teacher_ld, c.ids, c.ids_ld, c.N, c.K, inv_t, p.tp, p.ent, p.live);
     HEAD_TRY(hipGetLastError());
   }
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, c.stream, c.ids, c.ids_ld, c.ignore_index, p.live, c.N, st.pos, st.hdr);
-  HEAD_TRY(hipGetLastError());
+  const bool direct = p.direct;
+  if (!direct) {
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, c.stream, c.ids, c.ids_ld, c.ignore_index, p.live, c.N, st.pos, st.hdr);
+    HEAD_TRY(hipGetLastError());
+  }
   if (c.N > 0) {
-    HEAD_TRY(operands(c, p, st, true));
+    if (!direct) HEAD_TRY(operands(c, p, st, true));
     StatsArgs a;
-    a.x = p.x; a.x_ld = p.dp * 2; a.n_pad = p.n_pad;
+    a.x = direct ? (const char*)c.x : p.x; a.x_ld = direct ? c.x_ld * 2 : p.dp * 2; a.rows = direct ? c.N : p.n_pad;
     a.w = p.w != nullptr ? p.w : (const char*)c.w; a.w_ld = p.w != nullptr ? p.dp * 2 : c.w_ld * 2; a.V = c.V;
-    a.segs = p.logits(); a.ksteps = (int)(p.dp / 32); a.tiles_v = p.tiles_v; a.tiles_n = p.tiles_n;
-    a.to_log2 = kLog2e / c.temperature; a.hdr = st.hdr; a.part = p.part;
-    hipLaunchKernelGGL(stats_kernel<T>, dim3((unsigned)((int64_t)p.tiles_v * p.tiles_n)), dim3(kThreads), 0, c.stream, a);
+    a.segs = p.logits(); a.ksteps = (int)(p.dp / 32); a.tiles_v = p.tiles_v; a.tiles_n = p.few ? 1 : p.tiles_n;
+    a.to_log2 = kLog2e / c.temperature; a.hdr = direct ? nullptr : st.hdr; a.part = p.part; a.part_ld = p.n_pad;
+    using E = typename Wide<T>::E;
+    const unsigned blocks = (unsigned)((int64_t)a.tiles_v * a.tiles_n);
+    if (p.few) hipLaunchKernelGGL((stats_kernel<T, HeadFew<E>>), dim3(blocks), dim3(HeadFew<E>::THREADS), 0, c.stream, a);
+    else hipLaunchKernelGGL((stats_kernel<T, HeadTile<E>>), dim3(blocks), dim3(HeadTile<E>::THREADS), 0, c.stream, a);
     HEAD_TRY(hipGetLastError());
     RowsArgs r;
     r.x = c.x; r.x_ld = c.x_ld; r.w = c.w; r.w_ld = c.w_ld; r.ids = c.ids; r.ids_ld = c.ids_ld; r.tp = p.tp; r.ent = p.ent;
-    r.part = p.part; r.part_ld = p.n_pad; r.tiles = p.tiles_v; r.N = c.N; r.V = c.V; r.d = c.d; r.K = c.K; r.vec = rows_vec(c);
-    r.temperature = c.temperature; r.pos = st.pos; r.lse2 = st.lse2; r.t = st.t; r.loss = c.reduction == 0 ? c.loss : p.rows;
-    hipLaunchKernelGGL(rows_kernel<T>, dim3((unsigned)((c.N + kRows - 1) / kRows)), dim3(kThreads), 0, c.stream, r);
+    r.part = p.part; r.part_ld = p.n_pad; r.tiles = p.tiles_v; r.N = c.N; r.V = c.V; r.ignore = c.ignore_index; r.d = c.d; r.K = c.K;
+    r.vec = rows_vec(c); r.rows = c.N > 2048 ? 8 : c.N > 1024 ? 4 : c.N > 512 ? 2 : 1;
+    r.temperature = c.temperature; r.pos = direct ? nullptr : st.pos; r.lse2 = direct ? nullptr : st.lse2; r.t = direct ? nullptr : st.t;
+    r.loss = c.reduction == 0 ? c.loss : p.rows;
+    hipLaunchKernelGGL(rows_kernel<T>, dim3((unsigned)((c.N + r.rows - 1) / r.rows)), dim3(kThreads), 0, c.stream, r);
     HEAD_TRY(hipGetLastError());
   }
   if (c.reduction != 0) {

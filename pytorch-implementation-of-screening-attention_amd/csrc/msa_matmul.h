@@ -46,8 +46,8 @@ __device__ inline typename Quad<O>::V quad(Fn fn) {
 }
 
 // E: operand type.  BM x BN: the block's tile; WM x WN waves share it.  AMN, BMN: the operand's m or n is
-// contiguous.  DUAL: A is two matrices, whose rows alternate by 64 (m = 128 i + j: row 64 i + j of the first for j <
-// 64, row 64 i + j - 64 of the second above).  NST: stages.
+// contiguous.  DUAL: A is two matrices, whose rows alternate by 16 (m = 32 i + j: row 16 i + j of the first for j < 16, row
+// 16 i + j - 16 of the second above): registers r and r + 8 of a lane are the same row of both, r < 8.  NST: stages.
 template <typename E, int BM, int BN, int WM, int WN, bool AMN, bool BMN, bool DUAL, int NST>
 struct MmTile {
   using M = Mma<E>;
@@ -55,13 +55,14 @@ struct MmTile {
   static constexpr int NT = 64 * WM * WN;                    // threads
   static constexpr int MB = BM / WM / 32, NB = BN / WN / 32;  // 32x32 blocks of a wave
   static constexpr int ABYTES = BM * kMmK * 2, BBYTES = BN * kMmK * 2, STAGE = ABYTES + BBYTES;
+  static constexpr int TILE_M = BM, TILE_N = BN, THREADS = NT, WAVES_M = WM;
   static constexpr int STAGED = 32 * WN * (BM * 4 + 16);  // store_tokens of fp32
   static constexpr int LDS = NST * STAGE > STAGED ? NST * STAGE : STAGED;
   static constexpr int NWAVES = WM * WN;
   static constexpr int AI = ABYTES / 1024 / NWAVES, BI = BBYTES / 1024 / NWAVES;  // copies of 1 KiB a wave issues
   static_assert(AI * NWAVES * 1024 == ABYTES && BI * NWAVES * 1024 == BBYTES, "a stage is whole copies of every wave");
   static_assert(MB <= 4 && NB <= 4, "blocks are found by two address bits");
-  static_assert(!DUAL || (!AMN && NWAVES == 4 && BM % 128 == 0), "alternating rows are laid out for four waves");
+  static_assert(!DUAL || (!AMN && NWAVES % 2 == 0), "a wave's copies are one matrix's");
 
   typedef f32x16 Acc[MB][NB];
 
@@ -90,7 +91,8 @@ struct MmTile {
         const int lr = lane >> 2, chunk = (lane & 3) ^ swz_row(lr);
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
-          int r = ALT ? (j >> 1) * 64 + 16 * wave + lr : (j * NWAVES + wave) * 16 + lr;
+          const int g = j * NWAVES + wave;  // a copy's 16 rows
+          int r = (ALT ? g >> 1 : g) * 16 + lr;
           r = r < count ? r : count - 1;
           off[j] = (uint32_t)r * ld + (uint32_t)chunk * 16u;
         }
@@ -125,7 +127,7 @@ struct MmTile {
             if (k > last) o -= (uint32_t)(k - last) * ld;
           }
         }
-        const char* b = ALT && (j & 1) ? base + alt : base;
+        const char* b = ALT && (wave & 1) ? base + alt : base;
         mm_copy(b, o, (uint32_t)(uintptr_t)lds + (uint32_t)((j * NWAVES + wave) * 1024));
       }
     }
@@ -292,6 +294,14 @@ struct MmTile {
     asm volatile("" ::: "memory");
   }
 
+  // A DUAL tile's rows of an output: fn(i, j, g) of registers 4 g .. 4 g + 3 and 8 more, g < 2.
+  template <typename O, typename Fn>
+  __device__ static inline void store_dual(LdsChar* lds, O* dst, int64_t ld, int rows, int cols, bool vec, Fn fn) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      store_tokens<O, false, (MB + 1) / 2>(lds, dst, ld, rows, cols, vec, j, [&](int i, int g) { return fn(2 * i + (g >> 1), j, g & 1); });
+  }
+
   // Writes rows of an output: dst[n ld + m .. + 3] = fn(i, j, g) of registers 4 g .. 4 g + 3 of blocks (i, j), i < MS, for
   // n < rows and m < cols; ADD: added to what is there (O float).  A wave's MS blocks are neighbours (MS = MB: the tile itself).  vec:
   // dst and ld allow 16-byte accesses.  The values go through the block's LDS (free on entry and on return), 32
@@ -305,16 +315,16 @@ struct MmTile {
   // The part of it for the tokens of blocks (., j).
   template <typename O, bool ADD, int MS, typename Fn>
   __device__ static inline void store_tokens(LdsChar* lds, O* dst, int64_t ld, int rows, int cols, bool vec, int j, Fn fn) {
-    constexpr int W = 32 * MS * WM;
+    constexpr int QUADS = DUAL && MB == 1 ? 2 : 4, W = 8 * QUADS * MS * WM;  // a lone DUAL block is 16 features
     constexpr int ROW = W * (int)sizeof(O) + 16, PER = 16 / (int)sizeof(O), CPR = W / PER, R = 32 * WN;
     static_assert(R * ROW <= LDS, "the staged rows fit the tile's LDS");
     typedef __attribute__((address_space(3))) typename Quad<O>::V LdsQuad;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave % WM, wn = wave / WM;
-    LdsChar* to = lds + (wn * 32 + (lane & 31)) * ROW + (wm * 32 * MS + 4 * (lane >> 5)) * (int)sizeof(O);
+    LdsChar* to = lds + (wn * 32 + (lane & 31)) * ROW + (wm * 8 * QUADS * MS + 4 * (lane >> 5)) * (int)sizeof(O);
 #pragma unroll
     for (int i = 0; i < MS; ++i)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
+      for (int g = 0; g < QUADS; ++g) {
         const typename Quad<O>::V v = fn(i, g);
         *reinterpret_cast<LdsQuad*>(to + (32 * i + 8 * g) * (int)sizeof(O)) = v;
       }

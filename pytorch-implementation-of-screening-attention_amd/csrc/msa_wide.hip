@@ -411,7 +411,7 @@ WideShare wide_share(int64_t N, int d, int64_t C, int halves, int planes, bool d
   const int64_t tm = (wide_dp(d) + 255) / 256, segs = planes == 2 ? 3 : 1;
   const int64_t tx = dx ? tm * ((N + kTileN - 1) / kTileN) : 0, kx = C / 32 * segs * halves;
   const int64_t tw = dw ? tm * (C / kTileN) * halves : 0, kw = (N + 31) / 32 * segs;
-  constexpr int kCuts[] = {1, 2, 3, 4, 5, 6, 8, 11, 16};
+  constexpr int kCuts[] = {1, 2, 3, 4, 5, 6, 8, 11, 16, 24, 32, 48, 64};
   WideShare best = {1, 1, true, -1};
   for (const int sx : kCuts) {
     if (sx > 1 && (!dx || kx / sx < 8)) break;

@@ -557,11 +557,10 @@ def _autocast(*tensors):
 
 
 def _rows_2d(x):
-    """x (..., n) as rows with unit stride: the 2-D tensor, its pointer and its row stride."""
-    x = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if x.stride(1) != 1 and x.shape[1] > 1:
-        x = x.contiguous()
-    return x, x.data_ptr(), x.stride(0)
+    """x (..., n) as 2-D rows with unit stride."""
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
 def _head_checks(what, hidden, weight, reduction, *others):
@@ -601,22 +600,33 @@ def _head_call(what, fn, index, backward, *args):
     _launch(what, fn, index, _head_args(*args, workspace))
 
 
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(x.requires_grad for x in tensors)
+
+
+def _head_forward(hidden, weight, ids, teacher, temperature, ignore_index, reduction, state):
+    loss = torch.empty((ids.shape[0],) if reduction == "none" else (), dtype=torch.float32, device=hidden.device)
+    _head_call("msa_head_fwd", _native.lib().msa_head_fwd, hidden.get_device(), 0, hidden, weight, ids, teacher, temperature,
+               ignore_index, reduction, state, loss, None, None, None)
+    return loss
+
+
+def _head_loss(hidden, weight, *args):
+    """The loss of 2-D rows; without a gradient to follow, without the state that it takes."""
+    if _wants_grad(hidden, weight):
+        return _HeadLoss.apply(hidden, weight, *args)
+    return _head_forward(hidden, weight, *args, None)
+
+
 class _HeadLoss(torch.autograd.Function):
     """forward = msa_head_fwd, backward = msa_head_bwd, on 2-D rows."""
 
     @staticmethod
     def forward(ctx, hidden, weight, ids, teacher, temperature, ignore_index, reduction):
-        L = _native.lib()
-        N, K = ids.shape
-        dev = hidden.device
-        state = torch.empty((L.msa_head_state_bytes(N, K),), dtype=torch.uint8, device=dev)
-        loss = torch.empty((N,) if reduction == "none" else (), dtype=torch.float32, device=dev)
-        _head_call("msa_head_fwd", L.msa_head_fwd, hidden.get_device(), 0, hidden, weight, ids, teacher, temperature,
-                   ignore_index, reduction, state, loss, None, None, None)
-        if any(ctx.needs_input_grad[:2]):
-            ctx.save_for_backward(hidden, weight, ids, teacher, state)
-            ctx.options = temperature, ignore_index, reduction
-        return loss
+        state = torch.empty((_native.lib().msa_head_state_bytes(*ids.shape),), dtype=torch.uint8, device=hidden.device)
+        ctx.save_for_backward(hidden, weight, ids, teacher, state)
+        ctx.options = temperature, ignore_index, reduction
+        return _head_forward(hidden, weight, ids, teacher, temperature, ignore_index, reduction, state)
 
     @staticmethod
     @once_differentiable
@@ -649,7 +659,7 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="m
         raise ValueError(f"linear_cross_entropy: labels must be int64 {tuple(hidden.shape[:-1])}, got {labels.dtype} "
                          f"{tuple(labels.shape)}")
     ids = labels.reshape(-1, 1)
-    loss = _HeadLoss.apply(_rows_2d(hidden)[0], _rows_2d(weight)[0], ids, None, 1.0, int(ignore_index), reduction)
+    loss = _head_loss(_rows_2d(hidden), _rows_2d(weight), ids, None, 1.0, int(ignore_index), reduction)
     return loss.view(labels.shape) if reduction == "none" else loss
 
 
@@ -681,8 +691,8 @@ def linear_distillation(hidden, weight, teacher_logits, teacher_ids, temperature
         raise ValueError(f"linear_distillation: a row holds 1 to {_native.HEAD_MAX_K} teacher logits, got {shape[-1]}")
     if not 0.0 < temperature < float("inf"):
         raise ValueError(f"linear_distillation: temperature must be positive and finite, got {temperature}")
-    loss = _HeadLoss.apply(_rows_2d(hidden)[0], _rows_2d(weight)[0], _rows_2d(teacher_ids)[0],
-                           _rows_2d(teacher_logits.detach())[0], float(temperature), 0, reduction)
+    loss = _head_loss(_rows_2d(hidden), _rows_2d(weight), _rows_2d(teacher_ids), _rows_2d(teacher_logits.detach()),
+                      float(temperature), 0, reduction)
     return loss.view(shape[:-1]) if reduction == "none" else loss
 
 
@@ -699,10 +709,18 @@ def _gated_args(x, gate, up, act, h, dh, dx, dgate, dup, workspace=None):
 
 
 def _gated_call(what, fn, backward, *args):
-    x = args[0]
-    need = _native.lib().msa_gated_workspace_bytes(_gated_args(*args), backward)
-    workspace = torch.empty((need,), dtype=torch.uint8, device=x.device)
-    _launch(what, fn, x.get_device(), _gated_args(*args, workspace))
+    x, packed = args[0], _gated_args(*args)
+    need = _native.lib().msa_gated_workspace_bytes(packed, backward)
+    if need:
+        workspace = torch.empty((need,), dtype=torch.uint8, device=x.device)
+        packed = _gated_args(*args, workspace)
+    _launch(what, fn, x.get_device(), packed)
+
+
+def _gated_forward(x, gate, up, act):
+    h = torch.empty((x.shape[0], gate.shape[0]), dtype=x.dtype, device=x.device)
+    _gated_call("msa_gated_fwd", _native.lib().msa_gated_fwd, 0, x, gate, up, act, h, None, None, None, None)
+    return h
 
 
 class _GatedLinear(torch.autograd.Function):
@@ -710,18 +728,15 @@ class _GatedLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, gate, up, act):
-        h = torch.empty((x.shape[0], gate.shape[0]), dtype=x.dtype, device=x.device)
-        _gated_call("msa_gated_fwd", _native.lib().msa_gated_fwd, 0, x, gate, up, act, h, None, None, None, None)
-        if any(ctx.needs_input_grad[:3]):
-            ctx.save_for_backward(x, gate, up)
-            ctx.act = act
-        return h
+        ctx.save_for_backward(x, gate, up)
+        ctx.act = act
+        return _gated_forward(x, gate, up, act)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
         x, gate, up = ctx.saved_tensors
-        dh = _rows_2d(dh)[0]
+        dh = _rows_2d(dh)
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[0] else None
         dgate = dup = None
         if any(ctx.needs_input_grad[1:3]):
@@ -751,5 +766,6 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
                          f"{tuple(w_gate.shape)}, {tuple(w_up.shape)}")
     if activation not in _ACTIVATIONS:
         raise ValueError(f"gated_linear: activation must be 'silu' or 'gelu', got {activation!r}")
-    h = _GatedLinear.apply(_rows_2d(x)[0], _rows_2d(w_gate)[0], _rows_2d(w_up)[0], _ACTIVATIONS[activation])
-    return h.view(*x.shape[:-1], w_gate.shape[0])
+    fn = _GatedLinear.apply if _wants_grad(x, w_gate, w_up) else _gated_forward
+    h = fn(_rows_2d(x), _rows_2d(w_gate), _rows_2d(w_up), _ACTIVATIONS[activation])
+    return h if x.dim() == 2 else h.view(*x.shape[:-1], w_gate.shape[0])

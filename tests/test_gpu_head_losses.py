@@ -384,3 +384,22 @@ def test_refusals():
             (ValueError, lambda: kd(x, w, t, ids, math.inf))]:
         with pytest.raises(error):
             call()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [1, 16, 32, 33, 200, 1025])
+def test_scores_without_a_gradient_are_the_training_passs(N, dtype):
+    # a forward pass alone takes the rows as they are, where it can; others and masked rows go through a copy
+    x, w, y, g = _data(N, 128, 999, dtype, 16)
+    y[torch.rand(N, device=DEV, generator=g) < 0.2] = -100
+    a, b = _leaf(x, w)
+    want = ops.linear_cross_entropy(a, b, y, reduction="none").detach()
+    assert torch.equal(ops.linear_cross_entropy(x, w, y, reduction="none"), want)
+    odd = torch.empty(N * 128 + 1, device=DEV, dtype=dtype)[1:].view(N, 128)
+    odd.copy_(x)
+    assert torch.equal(ops.linear_cross_entropy(odd, w, y, reduction="none"), want)
+    ids, p, live = R.targets_of_labels(y)
+    value, bound = R.head(x, w, ids, p, live, 1.0, torch.ones(N, device=DEV).double())["loss"]
+    R.check("loss", want, value, bound)
+    x[y == -100] = math.nan
+    assert torch.equal(ops.linear_cross_entropy(x, w, y, reduction="none"), want)

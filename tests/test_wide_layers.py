@@ -154,12 +154,17 @@ def _head(fn="msa_head_fwd", **kw):
     (dict(t=1 << 22, t_ld=300, K=257, ids_ld=300), 1, "K must be"), (dict(t=1 << 22, tdt=3), 1, "teacher_dtype"),
     (dict(t=1 << 22, t_ld=256, K=256, ids_ld=256, N=1 << 24), 1, "N * K"), (dict(red=3), 1, "reduction"), (dict(T=0.0), 1, "temperature"),
     (dict(T=math.nan), 1, "temperature"), (dict(T=math.inf), 1, "temperature"), (dict(x=0), 1, "hidden is null"), (dict(x=(1 << 20) + 1), 1, "hidden"),
-    (dict(w=0), 1, "weight is null"), (dict(ids=0), 1, "ids is null"), (dict(x_ld=-64), 1, "stride"), (dict(state=0), 2, "state"),
+    (dict(w=0), 1, "weight is null"), (dict(ids=0), 1, "ids is null"), (dict(x_ld=-64), 1, "stride"),
     (dict(sb=10), 2, "state"), (dict(ws=0), 2, "workspace"), (dict(wsb=10), 2, "workspace"), (dict(ws=(1 << 27) + 8), 1, "aligned"),
     (dict(loss=0, dloss=0), 1, "null"), (dict(dx=(1 << 25) + 2), 1, "aligned")])
 def test_head_refusals(fn, kw, code, msg):
     rc, said = _head(fn, **kw)
     assert rc == code and msg in said
+
+
+def test_head_backward_needs_the_forwards_state():
+    rc, said = _head("msa_head_bwd", state=0)
+    assert rc == 2 and "state" in said
 
 
 def test_head_sizes():
