@@ -400,8 +400,8 @@ int msa_verify(const msa_verify_args* args, void* stream);
  * pass that no backward pass follows.  workspace: msa_head_workspace_bytes of the
  * same arguments (backward 0 or 1; of state only whether it is null; loss, dloss
  * and workspace are not looked at), scratch of the call.
- * 1 <= d <= 65536, V < 2^26, N <= 2^24, N K < 2^32, N d <= 2^38, V d <= 2^37, (N / 128)
- * (V / 128) < 2^24.  No atomics on sums: equal calls give bitwise equal results.
+ * 1 <= d <= 65536, V <= 2^23, N <= 2^23, N d <= 2^38, V d <= 2^37, (N / 128) (V / 128)
+ * < 2^24.  No atomics on sums: equal calls give bitwise equal results.
  */
 #define MSA_HEAD_MAX_K 256
 typedef struct {
@@ -445,7 +445,7 @@ int msa_head_bwd(const msa_head_args* args, void* stream);
  * fp32.
  * Operands are used in place under the conditions of msa_head_args' weight.
  * workspace: msa_gated_workspace_bytes of the same arguments.  1 <= d <= 65536, 1 <= F
- * <= 2^24, N <= 2^24, N d <= 2^38, F d <= 2^37, (N / 128) (F / 128) < 2^24.  Equal calls
+ * <= 2^23, N <= 2^23, N d <= 2^38, F d <= 2^37, (N / 128) (F / 128) < 2^24.  Equal calls
  * give bitwise equal results.
  */
 typedef struct {

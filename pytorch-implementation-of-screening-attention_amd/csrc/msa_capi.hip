@@ -662,7 +662,8 @@ int msa_verify(const msa_verify_args* a, void* stream) {
 static int check_wide(const char* what, int64_t N, int64_t d, int64_t rows, int64_t most, int64_t dtype) {
   if (dtype != MSA_F32 && dtype != MSA_BF16 && dtype != MSA_F16)
     return fail(MSA_ERR_INVALID, "dtype must be MSA_F32, MSA_BF16 or MSA_F16");
-  if (N < 0 || N > (int64_t)1 << 24) return fail(MSA_ERR_INVALID, "%s: 0 to 2^24 rows, got %lld", what, (long long)N);
+  // 8 blocks of 32 columns by all rows are addressed in 32 bits
+  if (N < 0 || N > (int64_t)1 << 23) return fail(MSA_ERR_INVALID, "%s: 0 to 2^23 rows, got %lld", what, (long long)N);
   if (d < 1 || d > 65536) return fail(MSA_ERR_INVALID, "%s: rows of 1 to 65536 columns, got %lld", what, (long long)d);
   if (rows < 1 || rows > most)
     return fail(MSA_ERR_INVALID, "%s: 1 to %lld weight rows, got %lld", what, (long long)most, (long long)rows);
@@ -682,13 +683,12 @@ static int check_rows(const char* name, const void* p, int64_t ld, int64_t cols,
 
 static int head_call(const msa_head_args* a, msa::HeadCall* c) {
   if (a == nullptr) return fail(MSA_ERR_INVALID, "args is null");
-  int rc = check_wide("head", a->N, a->d, a->V, ((int64_t)1 << 26) - 1, a->dtype);
+  int rc = check_wide("head", a->N, a->d, a->V, (int64_t)1 << 23, a->dtype);
   if (rc != MSA_OK) return rc;
   if (a->teacher == nullptr ? a->K != 1 : a->K < 1 || a->K > MSA_HEAD_MAX_K)
     return fail(MSA_ERR_INVALID, "K must be 1 without a teacher and 1 to %d with one, got %lld", MSA_HEAD_MAX_K, (long long)a->K);
   if (a->teacher != nullptr && a->teacher_dtype != MSA_F32 && a->teacher_dtype != MSA_BF16 && a->teacher_dtype != MSA_F16)
     return fail(MSA_ERR_INVALID, "teacher_dtype must be MSA_F32, MSA_BF16 or MSA_F16");
-  if (a->N * a->K >= (int64_t)1 << 32) return fail(MSA_ERR_INVALID, "N * K = %lld exceeds 2^32 - 1", (long long)(a->N * a->K));
   if (a->reduction < 0 || a->reduction > 2) return fail(MSA_ERR_INVALID, "reduction must be 0, 1 or 2");
   if (!(a->temperature > 0.0) || !((float)a->temperature > 1e-30f) || !((float)a->temperature < 1e30f))
     return fail(MSA_ERR_INVALID, "temperature must be positive and finite");
@@ -707,7 +707,7 @@ static int head_call(const msa_head_args* a, msa::HeadCall* c) {
 }
 
 size_t msa_head_state_bytes(int64_t N, int64_t K) {
-  return N < 0 || N > (int64_t)1 << 24 || K < 1 || K > MSA_HEAD_MAX_K ? 0 : msa::head_state_bytes(N, (int)K);
+  return N < 0 || N > (int64_t)1 << 23 || K < 1 || K > MSA_HEAD_MAX_K ? 0 : msa::head_state_bytes(N, (int)K);
 }
 
 size_t msa_head_workspace_bytes(const msa_head_args* a, int backward) {
@@ -739,7 +739,7 @@ int msa_head_bwd(const msa_head_args* a, void* stream) { return head_run(a, 1, s
 
 static int gated_call(const msa_gated_args* a, int backward, msa::GatedCall* c) {
   if (a == nullptr) return fail(MSA_ERR_INVALID, "args is null");
-  int rc = check_wide("gated", a->N, a->d, a->F, (int64_t)1 << 24, a->dtype);
+  int rc = check_wide("gated", a->N, a->d, a->F, (int64_t)1 << 23, a->dtype);
   if (rc != MSA_OK) return rc;
   if (a->act != 0 && a->act != 1) return fail(MSA_ERR_INVALID, "act must be 0 (silu) or 1 (gelu)");
   if (a->N > 0 && (rc = check_rows("x", a->x, a->x_ld, a->d, a->dtype)) != MSA_OK) return rc;

@@ -42,24 +42,26 @@ __device__ inline float act_of(float g) {
 }
 
 struct GatedArgs {
-  const char* x; int64_t x_ld; int64_t N, n_pad;
-  const char* w; int64_t w_ld, up;  // the gate's first row of the piece; from there to the other weight's
+  const char* x; int64_t x_ld, x_blk; int64_t N, n_pad;
+  const char* w; int64_t w_ld, w_blk, up;  // the gate's first row of the piece; from there to the other weight's
   int cols;                         // features of the piece
   MmSegs segs;
   int ksteps, tiles_f, tiles_n;
   const WideHdr* hdr;
   void* h; int64_t h_ld; int vec;   // forward
   const void* dh; int64_t dh_ld;    // backward: the piece's first column
-  char* g; int64_t C, plane, half;
+  char* g; int64_t plane, half;
 };
 
-// Tl: 128 features of 128 tokens, or 32 of 32 for few tokens (forward only).
+// Tl: 128 features of 128 tokens, 64 of 128 where that shares the work better (smaller_tiles), or 32 of 32 for few tokens
+// (forward only).
 template <typename E> using GatedTile = MmTile<E, 256, 128, 2, 2, false, false, true, 3>;
+template <typename E> using GatedHalf = MmTile<E, 128, 128, 2, 2, false, false, true, 3>;
 template <typename E> using GatedFew = MmTile<E, 64, 32, 2, 1, false, false, true, 8>;
 constexpr int kFew = 32;
 
 template <typename T, int ACT, bool BWD, typename Tl>
-__global__ void __launch_bounds__(Tl::THREADS, 2) gated_kernel(GatedArgs a) {
+__global__ void __launch_bounds__(Tl::THREADS, Tl::TILE_M == 128 ? 3 : 2) gated_kernel(GatedArgs a) {
   using E = typename Wide<T>::E;
   constexpr int BF = Tl::TILE_M / 2, BN = Tl::TILE_N;
   __shared__ char smem[Tl::LDS];
@@ -72,8 +74,8 @@ __global__ void __launch_bounds__(Tl::THREADS, 2) gated_kernel(GatedArgs a) {
   Tl::clear(acc);
   const int fleft = a.cols - f0 < BF ? a.cols - f0 : BF;
   const int rows = (int)(a.N - n0 < BN ? a.N - n0 : BN);
-  const typename Tl::Side A{a.w + f0 * a.w_ld, fleft, a.w_ld, 0, a.up};
-  const typename Tl::Side B{a.x + n0 * a.x_ld, rows, a.x_ld, 0, 0};
+  const typename Tl::Side A{a.w + f0 * a.w_ld, fleft, a.w_ld, a.w_blk, 0, a.up};
+  const typename Tl::Side B{a.x + n0 * a.x_ld, rows, a.x_ld, a.x_blk, 0, 0};
   Tl::run(acc, lds, A, B, a.segs, 0, a.ksteps);
   float f1 = 1.0f, f2 = 1.0f;
   if constexpr (Wide<T>::P == 2) {
@@ -90,7 +92,7 @@ __global__ void __launch_bounds__(Tl::THREADS, 2) gated_kernel(GatedArgs a) {
     const float sg = scale_g<T>(a.hdr, 1);
     // dh goes through LDS in whole rows, 32 tokens of each wave at a time; places outside are zeros, so that dg and du
     // are zeros there.
-    constexpr int PER = 16 / (int)sizeof(T), CPR = 128 / PER, ROW = 128 * (int)sizeof(T) + 16;
+    constexpr int PER = 16 / (int)sizeof(T), CPR = BF / PER, ROW = BF * (int)sizeof(T) + 16, NQ = 2 * Tl::MB;
     static_assert(64 * ROW <= Tl::LDS, "the staged rows of dh fit the tile's LDS");
     typedef __attribute__((__vector_size__(16))) T TV;
     typedef __attribute__((address_space(3))) TV LdsTV;
@@ -112,10 +114,10 @@ __global__ void __launch_bounds__(Tl::THREADS, 2) gated_kernel(GatedArgs a) {
         *reinterpret_cast<LdsTV*>(lds + row * ROW + f * (int)sizeof(T)) = v;
       }
       Tl::sync_lds();
-      typename Quad<E>::V grads[2][Wide<T>::P][8];  // [dg, du][term], rounded as they are made
-      const LdsChar* at = lds + (wn * 32 + (lane & 31)) * ROW + (wm * 64 + 4 * (lane >> 5)) * (int)sizeof(T);
+      typename Quad<E>::V grads[2][Wide<T>::P][NQ];  // [dg, du][term], rounded as they are made
+      const LdsChar* at = lds + (wn * 32 + (lane & 31)) * ROW + (wm * (BF / 2) + 4 * (lane >> 5)) * (int)sizeof(T);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
+      for (int q = 0; q < NQ; ++q) {
         const T4 d = *reinterpret_cast<const LdsT4*>(at + 8 * q * (int)sizeof(T));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -142,8 +144,8 @@ __global__ void __launch_bounds__(Tl::THREADS, 2) gated_kernel(GatedArgs a) {
       for (int half = 0; half < 2; ++half)
 #pragma unroll
         for (int t = 0; t < Wide<T>::P; ++t)
-          Tl::template store_tokens<E, false, 2>(lds, reinterpret_cast<E*>(a.g + half * a.half + t * a.plane) + n0 * a.C + f0, a.C,
-                                                 128, 128, true, j, [&](int i, int q) { return grads[half][t][4 * i + q]; });
+          Tl::template store_operand_tokens<Tl::MB / 2>(lds, reinterpret_cast<E*>(a.g + half * a.half + t * a.plane) + (f0 >> 5) * (a.n_pad * 32) + n0 * 32,
+                                                        a.n_pad * 32, j, [&](int i, int q) { return grads[half][t][4 * i + q]; });
     }
   }
 }
@@ -196,29 +198,31 @@ struct GatedPlan {
 
 #define GATED_TRY(call) do { const hipError_t e_ = (call); if (e_ != hipSuccess) return e_; } while (0)
 
-struct GatedOperands { const char *x, *w[2]; int64_t x_ld, w_ld; int x_rows; MmSegs segs; };
+struct GatedOperands { const char *x, *w[2]; int64_t x_ld, x_blk, w_ld, w_blk; int x_rows; MmSegs segs; };
 
 hipError_t operands(const GatedCall& c, const GatedPlan& p, int backward, GatedOperands* o) {
   RowsCopies all = {}, copies = {};
   all.dtype = copies.dtype = c.dtype;
   all.hdr = copies.hdr = p.hdr;
-  all.add(RowsCopy{c.x, c.x_ld, c.N, c.d, p.x, p.x_plane, nullptr, 0, backward});
+  all.add(RowsCopy{c.x, c.x_ld, c.N, c.d, p.x, p.x_plane, p.n_pad * 64, nullptr, 0, backward});
   for (int i = 0; i < 2; ++i)
-    all.add(RowsCopy{c.w[i], c.w_ld[i], c.F, c.d, p.w + (p.w == nullptr ? 0 : i * p.planes * p.w_plane), p.w_plane, nullptr, 1, backward});
+    all.add(RowsCopy{c.w[i], c.w_ld[i], c.F, c.d, p.w + (p.w == nullptr ? 0 : i * p.planes * p.w_plane), p.w_plane, c.F * (int64_t)64, nullptr, 1, backward});
   if (p.x != nullptr) copies.add(all.m[0]);
   if (p.w != nullptr) { copies.add(all.m[1]); copies.add(all.m[2]); }
   if (p.planes == 2 || (backward && c.dtype == 2)) {  // scales of the operands, and of dg and du
-    if (backward) all.add(RowsCopy{c.dh, c.dh_ld, c.N, c.F, nullptr, 0, nullptr, 2, 0});
+    if (backward) all.add(RowsCopy{c.dh, c.dh_ld, c.N, c.F, nullptr, 0, 0, nullptr, 2, 0});
     GATED_TRY(launch_hdr_clear(p.hdr, c.stream));
     GATED_TRY(launch_rows_max(all, c.stream));
   }
   if (copies.n > 0) GATED_TRY(launch_rows_copy(copies, c.stream));
   o->x = p.x != nullptr ? p.x : (const char*)c.x;
-  o->x_ld = p.x != nullptr ? p.dp * 2 : c.x_ld * 2;
+  o->x_ld = p.x != nullptr ? 64 : c.x_ld * 2;
+  o->x_blk = p.x != nullptr ? p.n_pad * 64 : 64;
   o->x_rows = (int)c.N;
   o->w[0] = p.w != nullptr ? p.w : (const char*)c.w[0];
   o->w[1] = p.w != nullptr ? p.w + p.planes * p.w_plane : (const char*)c.w[1];
-  o->w_ld = p.w != nullptr ? p.dp * 2 : c.w_ld[0] * 2;
+  o->w_ld = p.w != nullptr ? 64 : c.w_ld[0] * 2;
+  o->w_blk = p.w != nullptr ? c.F * (int64_t)64 : 64;
   o->segs = MmSegs{};
   if (p.planes == 2) {
     o->segs.b[0] = p.x_plane;
@@ -233,21 +237,29 @@ hipError_t operands(const GatedCall& c, const GatedPlan& p, int backward, GatedO
 
 GatedArgs args_of(const GatedCall& c, const GatedPlan& p, const GatedOperands& o, int64_t f0, int cols) {
   GatedArgs a = {};
-  a.x = o.x; a.x_ld = o.x_ld; a.N = c.N; a.n_pad = p.n_pad;
-  a.w = o.w[0] + f0 * o.w_ld; a.w_ld = o.w_ld; a.up = o.w[1] - o.w[0]; a.cols = cols;
+  a.x = o.x; a.x_ld = o.x_ld; a.x_blk = o.x_blk; a.N = c.N; a.n_pad = p.n_pad;
+  a.w = o.w[0] + f0 * o.w_ld; a.w_ld = o.w_ld; a.w_blk = o.w_blk; a.up = o.w[1] - o.w[0]; a.cols = cols;
   a.segs = o.segs; a.ksteps = (int)(p.dp / 32);
   a.hdr = p.hdr;
   return a;
 }
 
 template <typename T, bool BWD, template <typename> class Tile>
-hipError_t launch(GatedArgs a, int act, hipStream_t s) {
+hipError_t launch_tiles(GatedArgs a, int act, hipStream_t s) {
   using Tl = Tile<typename Wide<T>::E>;
   a.tiles_f = (a.cols + Tl::TILE_M / 2 - 1) / (Tl::TILE_M / 2);
   a.tiles_n = (int)((a.N + Tl::TILE_N - 1) / Tl::TILE_N);
   auto* k = act == 0 ? gated_kernel<T, 0, BWD, Tl> : gated_kernel<T, 1, BWD, Tl>;
   hipLaunchKernelGGL(k, dim3((unsigned)((int64_t)a.tiles_f * a.tiles_n)), dim3(Tl::THREADS), 0, s, a);
   return hipGetLastError();
+}
+
+template <typename T, bool BWD>
+hipError_t launch(const GatedArgs& a, int act, hipStream_t s) {
+  if (!BWD && a.N <= kFew) return launch_tiles<T, false, GatedFew>(a, act, s);
+  const int64_t tiles_n = (a.N + 127) / 128;
+  return smaller_tiles((a.cols + 127) / 128, tiles_n, (a.cols + 63) / 64) ? launch_tiles<T, BWD, GatedHalf>(a, act, s)
+                                                                        : launch_tiles<T, BWD, GatedTile>(a, act, s);
 }
 
 template <typename T>
@@ -259,7 +271,7 @@ hipError_t gated_fwd(const GatedCall& c) {
   GatedArgs a = args_of(c, p, o, 0, c.F);
   a.h = c.h; a.h_ld = c.F;
   a.vec = (int64_t)c.F * sizeof(T) % 16 == 0 && ((uintptr_t)c.h & 15) == 0;
-  return c.N <= kFew ? launch<T, false, GatedFew>(a, c.act, c.stream) : launch<T, false, GatedTile>(a, c.act, c.stream);
+  return launch<T, false>(a, c.act, c.stream);
 }
 
 template <typename T>
@@ -280,16 +292,16 @@ hipError_t gated_bwd(const GatedCall& c) {
     GatedArgs a = args_of(c, p, o, f0, cols);
     a.dh = (const T*)c.dh + f0; a.dh_ld = c.dh_ld;
     a.vec = c.dh_ld * sizeof(T) % 16 == 0 && ((uintptr_t)c.dh & 15) == 0;
-    a.g = p.g; a.C = p.C; a.plane = p.g_plane; a.half = p.planes * p.g_plane;
-    GATED_TRY((launch<T, true, GatedTile>(a, c.act, c.stream)));
+    a.g = p.g; a.plane = p.g_plane; a.half = p.planes * p.g_plane;
+    GATED_TRY((launch<T, true>(a, c.act, c.stream)));
     WideProducts q = {};
     q.dtype = c.dtype; q.gated = 1; q.N = c.N; q.n_pad = p.n_pad; q.d = c.d; q.dp = p.dp; q.halves = 2; q.cols = cols; q.C = p.C;
-    q.x = o.x; q.x_ld = o.x_ld; q.x_plane = p.x_plane; q.x_rows = o.x_rows;
+    q.x = o.x; q.x_ld = o.x_ld; q.x_blk = o.x_blk; q.x_plane = p.x_plane; q.x_rows = o.x_rows;
     for (int i = 0; i < 2; ++i) {
       q.w[i] = o.w[i] + f0 * o.w_ld;
       q.dw[i] = c.dw[i] == nullptr ? nullptr : (char*)c.dw[i] + f0 * c.d * es_of(c.dtype);
     }
-    q.w_ld = o.w_ld; q.w_plane = p.w_plane; q.w_rows = (int)(c.F - f0);
+    q.w_ld = o.w_ld; q.w_blk = o.w_blk; q.w_plane = p.w_plane; q.w_rows = (int)(c.F - f0);
     q.g = p.g; q.g_plane = p.g_plane; q.g_half = p.planes * p.g_plane;
     q.dx_part = p.dx_part; q.dx_add = f0 > 0; q.dw_part = p.dw_part;
     q.share = p.share; q.hdr = p.hdr; q.unit.mode = 3; q.use_live = 0;

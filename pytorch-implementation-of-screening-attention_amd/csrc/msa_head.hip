@@ -142,8 +142,8 @@ __global__ void __launch_bounds__(kThreads) teacher_kernel(const L* logits, int6
 // The product's maxima and sums
 // ---------------------------------------------------------------------------
 struct StatsArgs {
-  const char* x; int64_t x_ld; int64_t rows;  // readable rows
-  const char* w; int64_t w_ld; int64_t V;
+  const char* x; int64_t x_ld, x_blk; int64_t rows;  // readable rows
+  const char* w; int64_t w_ld, w_blk; int64_t V;
   MmSegs segs;
   int ksteps, tiles_v, tiles_n;
   float to_log2;  // log2(e) / T
@@ -185,8 +185,8 @@ __global__ void __launch_bounds__(Tl::THREADS, 2) stats_kernel(StatsArgs a) {
   Tl::clear(acc);
   const int vleft = (int)(a.V - v0 < BM ? a.V - v0 : BM);
   const int readable = (int)(a.rows - n0 < BN ? a.rows - n0 : BN);
-  const typename Tl::Side A{a.w + v0 * a.w_ld, vleft, a.w_ld, 0, 0};
-  const typename Tl::Side B{a.x + n0 * a.x_ld, readable, a.x_ld, 0, 0};
+  const typename Tl::Side A{a.w + v0 * a.w_ld, vleft, a.w_ld, a.w_blk, 0, 0};
+  const typename Tl::Side B{a.x + n0 * a.x_ld, readable, a.x_ld, a.x_blk, 0, 0};
   Tl::run(acc, lds, A, B, a.segs, 0, a.ksteps);
   float f = a.to_log2;
   if constexpr (Wide<T>::P == 2) f = f / scale_x<T>(a.hdr) / scale_w<T>(a.hdr);
@@ -402,15 +402,15 @@ __global__ void __launch_bounds__(1024) coef_kernel(const float* dloss, float fa
 }
 
 struct GradArgs {
-  const char* x; int64_t x_ld; int64_t n_pad;
-  const char* w; int64_t w_ld;  // the piece's first row
+  const char* x; int64_t n_pad;
+  const char* w; int64_t w_ld, w_blk;  // the piece's first row
   int cols;                     // its rows
   MmSegs segs;
   int ksteps, tiles_v, tiles_n;
   float to_log2;
   const WideHdr* hdr;
   const float* lse2; const float* coef;
-  char* g; int64_t C, plane;
+  char* g; int64_t plane;
 };
 
 // G of one tile: c_n 2^(z2 - lse2), without the targets, which scatter_kernel puts in their place.
@@ -428,9 +428,10 @@ __global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
   typename Tl::Acc acc;
   Tl::clear(acc);
   const int vleft = (int)(a.cols - v0 < 256 ? a.cols - v0 : 256);
-  E* out = reinterpret_cast<E*>(a.g) + n0 * a.C + v0;
-  const typename Tl::Side A{a.w + v0 * a.w_ld, vleft, a.w_ld, 0, 0};
-  const typename Tl::Side B{a.x + n0 * a.x_ld, (int)(a.n_pad - n0 < 128 ? a.n_pad - n0 : 128), a.x_ld, 0, 0};
+  const int64_t blk = a.n_pad * 32;
+  E* out = reinterpret_cast<E*>(a.g) + (v0 >> 5) * blk + n0 * 32;
+  const typename Tl::Side A{a.w + v0 * a.w_ld, vleft, a.w_ld, a.w_blk, 0, 0};
+  const typename Tl::Side B{a.x + n0 * 64, (int)(a.n_pad - n0 < 128 ? a.n_pad - n0 : 128), 64, a.n_pad * 64, 0, 0};
   Tl::run(acc, lds, A, B, a.segs, 0, a.ksteps);
   const float f = a.to_log2 / scale_x<T>(a.hdr) / scale_w<T>(a.hdr), lg = __is_same(T, bf16) ? 0.0f : 15.0f;  // log2 of scale_g
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
@@ -455,16 +456,16 @@ __global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
     }
   }
   if constexpr (Wide<T>::P == 2) {
-    Tl::template store_rows<E, false>(lds, out, a.C, 128, 256, true, [&](int i, int j, int g) {
+    Tl::store_operand(lds, out, blk, [&](int i, int j, int g) {
       return quad<E>([&](int e) { return (float)Terms<float>(acc[i][j][4 * g + e]).h; });
     });
     Tl::renew(acc);
-    Tl::template store_rows<E, false>(lds, reinterpret_cast<E*>(reinterpret_cast<char*>(out) + a.plane), a.C, 128, 256, true,
+    Tl::store_operand(lds, reinterpret_cast<E*>(reinterpret_cast<char*>(out) + a.plane), blk,
                                       [&](int i, int j, int g) {
                                         return quad<E>([&](int e) { return (float)Terms<float>(acc[i][j][4 * g + e]).l; });
                                       });
   } else {
-    Tl::template store_rows<E, false>(lds, out, a.C, 128, 256, true, [&](int i, int j, int g) {
+    Tl::store_operand(lds, out, blk, [&](int i, int j, int g) {
       return quad<E>([&](int e) { return acc[i][j][4 * g + e]; });
     });
   }
@@ -474,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) scatter_kernel(const int64_t* ids, int64_t ids_ld, int64_t N, int K, const int* pos,
                                                            const float* t, const float* coef, const WideHdr* hdr, int64_t v0,
-                                                           int cols, char* g, int64_t C, int64_t plane) {
+                                                           int cols, char* g, int64_t n_pad, int64_t plane) {
   using E = typename Wide<T>::E;
   const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   const int64_t n = e / K;
@@ -483,7 +484,7 @@ __global__ void __launch_bounds__(kThreads) scatter_kernel(const int64_t* ids, i
   const int64_t v = ids[n * ids_ld + (e - n * K)] - v0;
   if (at < 0 || v < 0 || v >= cols) return;
   const float x = (coef != nullptr ? t[e] * coef[at] : t[e]) * scale_g<T>(hdr, 0);
-  E* p = reinterpret_cast<E*>(g) + (int64_t)at * C + v;
+  E* p = reinterpret_cast<E*>(g) + (v >> 5) * (n_pad * 32) + (int64_t)at * 32 + (v & 31);
   if constexpr (Wide<T>::P == 2) {
     const Terms<float> w(x);
     *p = w.h;
@@ -588,8 +589,8 @@ hipError_t operands(const HeadCall& c, const HeadPlan& p, const HeadState& st, b
   RowsCopies all = {};
   all.dtype = c.dtype;
   all.hdr = st.hdr;
-  all.add(RowsCopy{c.x, c.x_ld, c.N, c.d, p.x, p.x_plane, st.pos, 0, 0});
-  if (p.w != nullptr) all.add(RowsCopy{c.w, c.w_ld, c.V, c.d, p.w, p.w_plane, nullptr, 1, 0});
+  all.add(RowsCopy{c.x, c.x_ld, c.N, c.d, p.x, p.x_plane, p.n_pad * 64, st.pos, 0, 0});
+  if (p.w != nullptr) all.add(RowsCopy{c.w, c.w_ld, c.V, c.d, p.w, p.w_plane, c.V * 64, nullptr, 1, 0});
   if (p.planes == 2 && find) HEAD_TRY(launch_rows_max(all, c.stream));
   return launch_rows_copy(all, c.stream);
 }
@@ -617,8 +618,8 @@ hipError_t head_fwd(const HeadCall& c) {
   if (c.N > 0) {
     if (!direct) HEAD_TRY(operands(c, p, st, true));
     StatsArgs a;
-    a.x = direct ? (const char*)c.x : p.x; a.x_ld = direct ? c.x_ld * 2 : p.dp * 2; a.rows = direct ? c.N : p.n_pad;
-    a.w = p.w != nullptr ? p.w : (const char*)c.w; a.w_ld = p.w != nullptr ? p.dp * 2 : c.w_ld * 2; a.V = c.V;
+    a.x = direct ? (const char*)c.x : p.x; a.x_ld = direct ? c.x_ld * 2 : 64; a.x_blk = direct ? 64 : p.n_pad * 64; a.rows = direct ? c.N : p.n_pad;
+    a.w = p.w != nullptr ? p.w : (const char*)c.w; a.w_ld = p.w != nullptr ? 64 : c.w_ld * 2; a.w_blk = p.w != nullptr ? c.V * 64 : 64; a.V = c.V;
     a.segs = p.logits(); a.ksteps = (int)(p.dp / 32); a.tiles_v = p.tiles_v; a.tiles_n = p.few ? 1 : p.tiles_n;
     a.to_log2 = kLog2e / c.temperature; a.hdr = direct ? nullptr : st.hdr; a.part = p.part; a.part_ld = p.n_pad;
     using E = typename Wide<T>::E;
@@ -659,23 +660,23 @@ hipError_t head_bwd(const HeadCall& c) {
   }
   HEAD_TRY(operands(c, p, st, false));
   const char* w = p.w != nullptr ? p.w : (const char*)c.w;
-  const int64_t w_ld = p.w != nullptr ? p.dp * 2 : c.w_ld * 2;
+  const int64_t w_ld = p.w != nullptr ? 64 : c.w_ld * 2, w_blk = p.w != nullptr ? c.V * 64 : 64;
   for (int64_t v0 = 0; v0 < c.V; v0 += p.C) {
     const int cols = (int)(c.V - v0 < p.C ? c.V - v0 : p.C);
     GradArgs a;
-    a.x = p.x; a.x_ld = p.dp * 2; a.n_pad = p.n_pad; a.w = w + v0 * w_ld; a.w_ld = w_ld; a.cols = cols;
+    a.x = p.x; a.n_pad = p.n_pad; a.w = w + v0 * w_ld; a.w_ld = w_ld; a.w_blk = w_blk; a.cols = cols;
     a.segs = p.logits(); a.ksteps = (int)(p.dp / 32); a.tiles_v = (int)(round_up(cols, 256) / 256); a.tiles_n = p.tiles_n;
-    a.to_log2 = kLog2e / c.temperature; a.hdr = st.hdr; a.lse2 = st.lse2; a.coef = p.coef; a.g = p.g; a.C = p.C; a.plane = p.g_plane;
+    a.to_log2 = kLog2e / c.temperature; a.hdr = st.hdr; a.lse2 = st.lse2; a.coef = p.coef; a.g = p.g; a.plane = p.g_plane;
     hipLaunchKernelGGL(grad_kernel<T>, dim3((unsigned)((int64_t)a.tiles_v * a.tiles_n)), dim3(kThreads), 0, c.stream, a);
     HEAD_TRY(hipGetLastError());
     hipLaunchKernelGGL(scatter_kernel<T>, dim3((unsigned)((c.N * c.K + kThreads - 1) / kThreads)), dim3(kThreads), 0, c.stream,
-                       c.ids, c.ids_ld, c.N, c.K, st.pos, st.t, p.coef, st.hdr, v0, cols, p.g, p.C, p.g_plane);
+                       c.ids, c.ids_ld, c.N, c.K, st.pos, st.t, p.coef, st.hdr, v0, cols, p.g, p.n_pad, p.g_plane);
     HEAD_TRY(hipGetLastError());
     WideProducts q = {};
     q.dtype = c.dtype; q.gated = 0; q.N = c.N; q.n_pad = p.n_pad; q.d = c.d; q.dp = p.dp; q.halves = 1; q.cols = cols;
     q.C = p.C;
-    q.x = p.x; q.x_ld = p.dp * 2; q.x_plane = p.x_plane; q.x_rows = (int)p.n_pad;
-    q.w[0] = w + v0 * w_ld; q.w_ld = w_ld; q.w_plane = p.w_plane; q.w_rows = (int)(c.V - v0);
+    q.x = p.x; q.x_ld = 64; q.x_blk = p.n_pad * 64; q.x_plane = p.x_plane; q.x_rows = (int)p.n_pad;
+    q.w[0] = w + v0 * w_ld; q.w_ld = w_ld; q.w_blk = w_blk; q.w_plane = p.w_plane; q.w_rows = (int)(c.V - v0);
     q.g = p.g; q.g_plane = p.g_plane; q.g_half = 0;
     q.dx_part = p.dx_part; q.dx_add = v0 > 0;
     q.dw[0] = c.dw == nullptr ? nullptr : (char*)c.dw + v0 * c.d * es_of(c.dtype); q.dw_part = p.dw_part;

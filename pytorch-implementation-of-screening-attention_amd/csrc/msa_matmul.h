@@ -84,7 +84,7 @@ struct MmTile {
     static constexpr int RPI = 64 / CPR;         // MN: rows of a copy (W <= 512)
     // first: the tile's first row (K-contiguous) or column (MN); count: rows or columns of the matrix from there on.
     // ALT: count of each of the two matrices.
-    __device__ inline void init(int64_t stride_bytes, int count, int wave, int lane, int krows) {
+    __device__ inline void init(int64_t stride_bytes, int64_t blk, int count, int wave, int lane, int krows) {
       ld = (uint32_t)stride_bytes;
       rows = krows;
       if constexpr (!MN) {
@@ -103,7 +103,7 @@ struct MmTile {
           const int p = (j * NWAVES + wave) * 64 + lane, k = p / CPR;
           int col = ((p % CPR) ^ swz_k(k)) * 8;
           col = col < count ? col : count - 8;  // count is a multiple of 8
-          off[j] = (uint32_t)k * ld + (uint32_t)col * 2u;
+          off[j] = (uint32_t)k * ld + (uint32_t)(col >> 5) * (uint32_t)blk + (uint32_t)(col & 31) * 2u;
         }
         r0 = wave * RPI + lane / CPR;
       }
@@ -167,11 +167,13 @@ struct MmTile {
   };
 
   // The tile's operands: where (first row or column, k = 0) lies, rows or columns there are from it on, bytes from
-  // row to row, bytes that 32 k advance, k rows (MN).
+  // row to row and from 32 columns to the next 32, k rows (MN).  Rows as they are in a tensor: blk = 64.  Operands that a
+  // kernel writes lie in blocks of 32 columns, row behind row (ld = 64): a stage is then whole kilobytes, where 64 bytes of
+  // a long row are half a cache line and a request of its own.
   struct Side {
     const char* p;
     int count;
-    int64_t ld;
+    int64_t ld, blk;
     int krows;
     int64_t alt;  // DUAL: to the second matrix
   };
@@ -185,15 +187,15 @@ struct MmTile {
     const int wm = wave % WM, wn = wave / WM;
     Loader<AMN, BM, AI, DUAL> la;
     Loader<BMN, BN, BI, false> lb;
-    la.init(A.ld, A.count, wave, lane, A.krows);
-    lb.init(B.ld, B.count, wave, lane, B.krows);
+    la.init(A.ld, A.blk, A.count, wave, lane, A.krows);
+    lb.init(B.ld, B.blk, B.count, wave, lane, B.krows);
     Reader<AMN, BM> ra;
     Reader<BMN, BN> rb;
     ra.init(wm * (BM / WM), lane);
     rb.init(wn * (BN / WN), lane);
-    const int64_t astep = AMN ? A.ld * kMmK : kMmK * 2, bstep = BMN ? B.ld * kMmK : kMmK * 2;
-    const char* const a0 = A.p + (AMN ? A.ld * k0 : (int64_t)k0 * 2);
-    const char* const b0 = B.p + (BMN ? B.ld * k0 : (int64_t)k0 * 2);
+    const int64_t astep = AMN ? A.ld * kMmK : A.blk, bstep = BMN ? B.ld * kMmK : B.blk;
+    const char* const a0 = A.p + astep * (k0 / kMmK);
+    const char* const b0 = B.p + bstep * (k0 / kMmK);
 
     const int total = steps * segs.n;
     int iseg = 0, istep = 0;  // the next stage to copy
@@ -294,6 +296,46 @@ struct MmTile {
     asm volatile("" ::: "memory");
   }
 
+  // Operand rows for a later product, in blocks of 32 columns (Side): dst is the tile's first row in its first block, blk
+  // elements from block to block; the tile's rows and columns are all there.
+  template <typename Fn>
+  __device__ static inline void store_operand(LdsChar* lds, E* dst, int64_t blk, Fn fn) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) store_operand_tokens<MB>(lds, dst, blk, j, [&](int i, int g) { return fn(i, j, g); });
+  }
+  template <int MS, typename Fn>
+  __device__ static inline void store_operand_tokens(LdsChar* lds, E* dst, int64_t blk, int j, Fn fn) {
+    constexpr int W = 32 * MS * WM, R = 32 * WN, ROW = W * 2 + 16;
+    stage_tokens<E, MS>(lds, j, fn);
+    const int tid = (int)threadIdx.x;
+#pragma unroll 4
+    for (int u = tid; u < R * W / 8; u += NT) {
+      const int c4 = u & 3, r = (u >> 2) % R, b = (u >> 2) / R, n = (r >> 5) * (BN / WN) + 32 * j + (r & 31);
+      typedef __attribute__((__vector_size__(16))) E EV;
+      const EV v = *reinterpret_cast<const __attribute__((address_space(3))) EV*>(lds + r * ROW + b * 64 + c4 * 16);
+      *reinterpret_cast<EV*>(dst + b * blk + (int64_t)n * 32 + c4 * 8) = v;
+    }
+    sync_lds();
+  }
+  // Registers of the blocks (., j) as rows of 32 tokens of each wave in LDS.
+  template <typename O, int MS, typename Fn>
+  __device__ static inline void stage_tokens(LdsChar* lds, int j, Fn fn) {
+    constexpr int QUADS = DUAL && MB == 1 ? 2 : 4, W = 8 * QUADS * MS * WM;  // a lone DUAL block is 16 features
+    constexpr int ROW = W * (int)sizeof(O) + 16;
+    static_assert(32 * WN * ROW <= LDS, "the staged rows fit the tile's LDS");
+    typedef __attribute__((address_space(3))) typename Quad<O>::V LdsQuad;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave % WM, wn = wave / WM;
+    LdsChar* to = lds + (wn * 32 + (lane & 31)) * ROW + (wm * 8 * QUADS * MS + 4 * (lane >> 5)) * (int)sizeof(O);
+#pragma unroll
+    for (int i = 0; i < MS; ++i)
+#pragma unroll
+      for (int g = 0; g < QUADS; ++g) {
+        const typename Quad<O>::V v = fn(i, g);
+        *reinterpret_cast<LdsQuad*>(to + (32 * i + 8 * g) * (int)sizeof(O)) = v;
+      }
+    sync_lds();
+  }
+
   // A DUAL tile's rows of an output: fn(i, j, g) of registers 4 g .. 4 g + 3 and 8 more, g < 2.
   template <typename O, typename Fn>
   __device__ static inline void store_dual(LdsChar* lds, O* dst, int64_t ld, int rows, int cols, bool vec, Fn fn) {
@@ -315,20 +357,10 @@ struct MmTile {
   // The part of it for the tokens of blocks (., j).
   template <typename O, bool ADD, int MS, typename Fn>
   __device__ static inline void store_tokens(LdsChar* lds, O* dst, int64_t ld, int rows, int cols, bool vec, int j, Fn fn) {
-    constexpr int QUADS = DUAL && MB == 1 ? 2 : 4, W = 8 * QUADS * MS * WM;  // a lone DUAL block is 16 features
+    constexpr int QUADS = DUAL && MB == 1 ? 2 : 4, W = 8 * QUADS * MS * WM;
     constexpr int ROW = W * (int)sizeof(O) + 16, PER = 16 / (int)sizeof(O), CPR = W / PER, R = 32 * WN;
-    static_assert(R * ROW <= LDS, "the staged rows fit the tile's LDS");
-    typedef __attribute__((address_space(3))) typename Quad<O>::V LdsQuad;
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave % WM, wn = wave / WM;
-    LdsChar* to = lds + (wn * 32 + (lane & 31)) * ROW + (wm * 8 * QUADS * MS + 4 * (lane >> 5)) * (int)sizeof(O);
-#pragma unroll
-    for (int i = 0; i < MS; ++i)
-#pragma unroll
-      for (int g = 0; g < QUADS; ++g) {
-        const typename Quad<O>::V v = fn(i, g);
-        *reinterpret_cast<LdsQuad*>(to + (32 * i + 8 * g) * (int)sizeof(O)) = v;
-      }
-    sync_lds();
+    stage_tokens<O, MS>(lds, j, fn);
+    const int tid = (int)threadIdx.x;
 #pragma unroll 4
     for (int u = tid; u < R * CPR; u += NT) {
       const int r = u / CPR, c = (u - r * CPR) * PER, n = (r >> 5) * (BN / WN) + 32 * j + (r & 31);
@@ -370,6 +402,12 @@ struct MmTile {
   __device__ static inline int m_of(int wm, int lane, int i, int g) { return wm * (BM / WM) + 32 * i + 8 * g + 4 * (lane >> 5); }
   __device__ static inline int n_of(int wn, int lane, int j) { return wn * (BN / WN) + 32 * j + (lane & 31); }
 };
+
+// Whether a grid of tiles of 256 by 128 (two a CU at a time) is better cut into twice as many of 128 by 128: those take
+// about 12% longer for the same work, but the CU with most of them may have less of it.
+inline bool smaller_tiles(int64_t tiles_m, int64_t tiles_n, int64_t small_m) {
+  return (small_m * tiles_n + 255) / 256 * 112 < (tiles_m * tiles_n + 255) / 256 * 200;
+}
 
 // Blocks of a grid go to the eight XCDs in turn, each with an L2 of its own: block id -> position in an order whose
 // consecutive eighths are an XCD's.

@@ -75,12 +75,13 @@ template <> struct Terms<float> {
 
 inline int64_t wide_dp(int64_t d) { return round_up(d, 32); }
 
-// Matrices as operand rows of dp columns: `planes` matrices of plane_bytes each.  pos: null, or which row of the
+// Matrices as operand rows of dp columns, in blocks of 32 columns (MmTile::Side) with blk bytes from block to block, one
+// or two terms plane_bytes apart.  pos: null, or which row of the
 // operand each row becomes (-1: none); rows from *live up to the next multiple of 128 are then zeroed.  slot (0: x, 1: w, 2:
 // dh): whose maxima it adds to, and whose scale it takes.
 struct RowsCopy {
   const void* src; int64_t ld; int64_t rows; int d;
-  char* dst; int64_t plane_bytes;
+  char* dst; int64_t plane_bytes, blk;
   const int* pos; int slot, norms;
 };
 constexpr int kCopies = 4;
@@ -127,9 +128,9 @@ struct WideProducts {
   int halves;        // weights: 1, or 2 (gate and up)
   int cols;          // weight rows of the piece
   int64_t C;         // columns of g: cols rounded up to 256
-  const char* x; int64_t x_ld, x_plane; int x_rows;           // bytes from row to row, to the second term; readable rows
-  const char* w[2]; int64_t w_ld, w_plane; int w_rows;        // the piece's first rows; readable rows from there
-  const char* g; int64_t g_plane, g_half;                     // [half][term][n_pad][C]
+  const char* x; int64_t x_ld, x_blk, x_plane; int x_rows;    // bytes from row to row, from 32 columns on, to the second term; readable rows
+  const char* w[2]; int64_t w_ld, w_blk, w_plane; int w_rows;        // the piece's first rows; readable rows from there
+  const char* g; int64_t g_plane, g_half;                     // [half][term][C / 32][n_pad][32]
   float* dx_part; int dx_add;                                 // [share.dx_split][n_pad][dp], or null: no dx
   void* dw[2];                                                // the piece's rows of the gradients, or null
   float* dw_part;                                             // [share.dw_split][halves][C][dp] where that is over 1

@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kThreads) rows_copy_kernel(RowsArgs a, int dp)
   }
   float s = 1.0f;
   if constexpr (Wide<T>::P == 2) s = m.slot == 0 ? scale_x<T>(a.hdr) : scale_w<T>(a.hdr);
-  E* out = reinterpret_cast<E*>(m.dst) + to * dp;
+  char* const out = m.dst + to * 64;
   const T* in = (const T*)m.src + r * m.ld;
   typedef __attribute__((__vector_size__(16))) E E8;
   for (int c = lane * 8; c < dp; c += 512) {
@@ -133,12 +133,12 @@ __global__ void __launch_bounds__(kThreads) rows_copy_kernel(RowsArgs a, int dp)
         h[e] = t.h;
         l[e] = t.l;
       }
-      *reinterpret_cast<E8*>(reinterpret_cast<char*>(out + c) + m.plane_bytes) = l;
+      *reinterpret_cast<E8*>(out + (c >> 5) * m.blk + (c & 31) * 2 + m.plane_bytes) = l;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[e] = x[e];
     }
-    *reinterpret_cast<E8*>(out + c) = h;
+    *reinterpret_cast<E8*>(out + (c >> 5) * m.blk + (c & 31) * 2) = h;
   }
 }
 
@@ -150,8 +150,8 @@ struct ProductArgs {
   int64_t C;
   WideShare share;
   MmSegs dx_segs, dw_segs;
-  const char* x; int64_t x_ld; int x_rows;
-  const char* w; int64_t w_ld; int w_rows;
+  const char* x; int64_t x_ld, x_blk; int x_rows;
+  const char* w; int64_t w_ld, w_blk; int w_rows;
   const char* g; int64_t g_half;
   float* dx_part; int dx_add;
   void* dw0; void* dw1;
@@ -186,8 +186,8 @@ __global__ void __launch_bounds__(kProductThreads, 2) products_kernel(ProductArg
     const int from = (int)((int64_t)p.dx_steps * split / p.share.dx_split), to = (int)((int64_t)p.dx_steps * (split + 1) / p.share.dx_split);
     typename TX::Acc acc;
     TX::clear(acc);
-    const typename TX::Side A{p.w + (int64_t)m0 * 2, (int)(p.dp - m0), p.w_ld, p.w_rows, 0};
-    const typename TX::Side B{p.g + (int64_t)n0 * p.C * 2, (int)(p.n_pad - n0), p.C * 2, 0, 0};
+    const typename TX::Side A{p.w + (m0 >> 5) * p.w_blk, (int)(p.dp - m0), p.w_ld, p.w_blk, p.w_rows, 0};
+    const typename TX::Side B{p.g + (int64_t)n0 * 64, (int)(p.n_pad - n0), 64, p.n_pad * 64, 0, 0};
     if (to > from) TX::run(acc, lds, A, B, p.dx_segs, from * 32, to - from);
     float* out = p.dx_part + ((int64_t)split * p.n_pad + n0) * p.dp + m0;
     auto fn = [&](int i, int j, int g) { return quad<float>([&](int e) { return acc[i][j][4 * g + e]; }); };
@@ -206,8 +206,8 @@ __global__ void __launch_bounds__(kProductThreads, 2) products_kernel(ProductArg
               to = (int)((int64_t)steps * (split + 1) / p.share.dw_split);
     typename TW::Acc acc;
     TW::clear(acc);
-    const typename TW::Side A{p.x + (int64_t)m0 * 2, (int)(p.dp - m0), p.x_ld, p.x_rows, 0};
-    const typename TW::Side B{p.g + half * p.g_half + (int64_t)n0 * 2, (int)(p.C - n0), p.C * 2, (int)p.n_pad, 0};
+    const typename TW::Side A{p.x + (m0 >> 5) * p.x_blk, (int)(p.dp - m0), p.x_ld, p.x_blk, p.x_rows, 0};
+    const typename TW::Side B{p.g + half * p.g_half + (n0 >> 5) * p.n_pad * 64, (int)(p.C - n0), 64, p.n_pad * 64, (int)p.n_pad, 0};
     if (to > from) TW::run(acc, lds, A, B, p.dw_segs, from * 32, to - from);
     const int rows = p.cols - n0 < kTileN ? p.cols - n0 : kTileN;
     if (p.share.dw_split > 1) {
@@ -312,7 +312,7 @@ hipError_t products(const WideProducts& p, hipStream_t s) {
   a.N = p.N; a.n_pad = p.n_pad; a.d = p.d; a.dp = p.dp; a.share = p.share;
   a.tm = (int)((p.dp + 255) / 256);
   a.dx_blocks = dx ? a.tm * (int)((p.n_pad + kTileN - 1) / kTileN) * p.share.dx_split : 0;
-  a.dx_steps = (p.cols + 127) / 128 * 4;
+  a.dx_steps = (p.cols + 63) / 64 * 2;  // columns of G that are there: the gated kernel fills 64 at a time
   a.dw_tn = (p.cols + kTileN - 1) / kTileN;
   a.dw_blocks = dw ? a.tm * a.dw_tn * p.halves * p.share.dw_split : 0;
   a.halves = p.halves; a.cols = p.cols;
@@ -337,8 +337,8 @@ hipError_t products(const WideProducts& p, hipStream_t s) {
   }
   a.dw_segs.a[n] = 0; a.dw_segs.b[n++] = 0;
   a.dw_segs.n = n; a.dw_segs.low = n - 1;
-  a.x = p.x; a.x_ld = p.x_ld; a.x_rows = p.x_rows;
-  a.w = p.w[0]; a.w_ld = p.w_ld; a.w_rows = p.w_rows;
+  a.x = p.x; a.x_ld = p.x_ld; a.x_blk = p.x_blk; a.x_rows = p.x_rows;
+  a.w = p.w[0]; a.w_ld = p.w_ld; a.w_blk = p.w_blk; a.w_rows = p.w_rows;
   a.g = p.g; a.g_half = p.g_half;
   a.dx_part = p.dx_part; a.dx_add = p.dx_add;
   a.dw0 = p.dw[0]; a.dw1 = p.dw[1]; a.dw_part = p.dw_part;
@@ -405,9 +405,9 @@ static int64_t two_kinds(int64_t n1, int64_t l1, int64_t n2, int64_t l2) {
 }
 
 WideShare wide_share(int64_t N, int d, int64_t C, int halves, int planes, bool dx, bool dw) {
-  // What a block costs beside its stages, in stages: 12 to fill and drain its pipeline, 12 to store a tile rounded, 25 to
-  // store it in fp32 and as much, over all of the card, to add it up (64 MB of 256 tiles at 4 TB/s are 16 us, a stage 0.7).
-  constexpr int64_t kFill = 12, kRounded = 12, kFloat = 25;
+  // What a block costs beside its stages, in stages of 0.7 us: 12 to fill and drain its pipeline, 5 to store a tile, and
+  // where all CUs store fp32 tiles at once 20 more (64 MB at 4 TB/s); adding them up takes a launch, 8, and as much again.
+  constexpr int64_t kFill = 12, kStore = 5, kFloat = 20, kLaunch = 8;
   const int64_t tm = (wide_dp(d) + 255) / 256, segs = planes == 2 ? 3 : 1;
   const int64_t tx = dx ? tm * ((N + kTileN - 1) / kTileN) : 0, kx = C / 32 * segs * halves;
   const int64_t tw = dw ? tm * (C / kTileN) * halves : 0, kw = (N + 31) / 32 * segs;
@@ -415,13 +415,15 @@ WideShare wide_share(int64_t N, int d, int64_t C, int halves, int planes, bool d
   WideShare best = {1, 1, true, -1};
   for (const int sx : kCuts) {
     if (sx > 1 && (!dx || kx / sx < 8)) break;
-    const int64_t lx = (kx + sx - 1) / sx + kFill + kFloat;
+    const int64_t nx = tx * sx;
     for (const int sw : kCuts) {
       if (sw > 1 && (!dw || kw / sw < 8)) break;
-      const int64_t lw = (kw + sw - 1) / sw + kFill + (sw > 1 ? kFloat : kRounded);
+      const int64_t nw = tw * sw, floats = nx + (sw > 1 ? nw : 0), busy = kFloat * (floats < kInFlight ? floats : kInFlight) / kInFlight;
+      const int64_t lx = (kx + sx - 1) / sx + kFill + kStore + busy;
+      const int64_t lw = (kw + sw - 1) / sw + kFill + kStore + (sw > 1 ? busy : 0);
       const bool first = lx >= lw;
-      const int64_t sum = kFloat * (tx * sx + (sw > 1 ? tw * sw : 0)) / kInFlight;
-      const int64_t cost = sum + (first ? two_kinds(tx * sx, lx, tw * sw, lw) : two_kinds(tw * sw, lw, tx * sx, lx));
+      const int64_t sum = kFloat * floats / kInFlight + (sw > 1 ? kLaunch : 0);
+      const int64_t cost = sum + (first ? two_kinds(nx, lx, nw, lw) : two_kinds(nw, lw, nx, lx));
       if (best.cost < 0 || cost < best.cost) best = WideShare{sx, sw, first, cost};
     }
   }
