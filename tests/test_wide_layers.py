@@ -189,7 +189,7 @@ def _gated(fn="msa_gated_fwd", **kw):
 @pytest.mark.parametrize("kw,code,msg", [
     (dict(dt=4), 1, "dtype"), (dict(N=-1), 1, "rows"), (dict(d=0), 1, "columns"), (dict(F=0), 1, "weight rows"), (dict(F=(1 << 23) + 1), 1, "weight rows"),
     (dict(N=1 << 23, F=1 << 20), 1, "too many"), (dict(act=2), 1, "act"), (dict(x=0), 1, "x is null"), (dict(g=0), 1, "gate is null"),
-    (dict(u=3), 1, "up is not aligned"), (dict(x_ld=-1), 1, "stride"), (dict(wsb=10), 2, "workspace"), (dict(ws=8), 1, "aligned"),
+    (dict(u=3), 1, "up is not aligned"), (dict(x_ld=-1), 1, "stride"), (dict(wsb=10, dt=0), 2, "workspace"), (dict(ws=8), 1, "aligned"),
     (dict(dx=8), 1, "aligned")])
 def test_gated_refusals(fn, kw, code, msg):
     rc, said = _gated(fn, **kw)
