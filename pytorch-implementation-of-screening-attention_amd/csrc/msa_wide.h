@@ -108,12 +108,16 @@ __device__ inline float unit_of(const GradUnit& u, const WideHdr* h, const float
   return u.mode == 1 ? u.dloss[0] * u.factor / (float)h->live : u.dloss[0] * u.factor;
 }
 
-// How the two products of a piece are cut: each of dx's tiles into dx_split ranges of its k, dW's into dw_split, a block
-// each.  cost: stages (32 k of a tile) until the last of 256 blocks in flight (one a CU) has ended, as wide_share reckons.
+// How the two products of a piece are cut: each of dx's tiles into dx_split ranges of its k, dW's into dw_split.  cost:
+// stages (32 k of a tile) until the last of 256 blocks in flight (one a CU) has ended, as wide_share reckons.  Either a
+// block for each range, the longer kind first; or, `slots` > 0, as many blocks as CUs: block s takes dW's ranges s, s + slots,
+// ... and then range s / tiles of dx's tile s % tiles, the first n_a ranges `a` steps long (behind one more of dW's) and
+// the others b.
 struct WideShare {
   int dx_split, dw_split;
   bool dx_first;
   int64_t cost;
+  int slots, n_a, a, b;
 };
 WideShare wide_share(int64_t N, int d, int64_t C, int halves, int planes, bool dx, bool dw);
 // The columns of a piece of `rows` weight rows whose G takes `bytes_of_column` a column: 1 GB of G, 512 or 256 MB, by cost.

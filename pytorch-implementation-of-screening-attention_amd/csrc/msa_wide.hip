@@ -146,7 +146,7 @@ struct ProductArgs {
   int64_t N, n_pad;
   int d;
   int64_t dp;
-  int tm, dx_blocks, dw_blocks, dx_steps, dw_tn, halves, cols;
+  int tm, dx_tiles, dx_blocks, dw_blocks, dx_steps, dw_tn, halves, cols;
   int64_t C;
   WideShare share;
   MmSegs dx_segs, dw_segs;
@@ -164,38 +164,31 @@ struct ProductArgs {
 // A block per tile and range of its k: dx[n][m] = sum_v G[n][v] W[v][m], and dW[v][m] = sum_n G[n][v] x[n][m].  Both in one
 // launch, the longer blocks first, so that neither leaves CUs idle at its end.  Ranges of one tile, and tiles of one block
 // of rows or columns of G, stand side by side: an XCD's blocks then read the same rows of W or x at the same time.  (Cut
-// where 512 equal shares end instead, the blocks start at places of their own in W: 12% slower at 8192 rows.)
+// where equal shares end instead, the blocks start at places of their own in W: 12% slower at 8192 rows.)
 template <typename T>
-__global__ void __launch_bounds__(kProductThreads, 2) products_kernel(ProductArgs p) {
+struct Products {
   using E = typename Wide<T>::E;
   using TX = MmTile<E, 256, kTileN, 2, 4, true, false, false, 4>;
   using TW = MmTile<E, 256, kTileN, 2, 4, true, true, false, 4>;
-  __shared__ char smem[TX::LDS];
-  LdsChar* lds = (LdsChar*)smem;
-  const int64_t N = p.use_live ? p.hdr->live : p.N;
-  const int first = p.share.dx_first ? p.dx_blocks : p.dw_blocks;
-  const bool head = (int)blockIdx.x < first, is_dx = head == p.share.dx_first;
-  const int64_t at = head ? blockIdx.x : (int64_t)blockIdx.x - first;
-  if (is_dx) {
-    int64_t t = xcd_order(at, p.dx_blocks);
-    const int split = (int)(t % p.share.dx_split);
-    t /= p.share.dx_split;
-    const int tm = (int)(t % p.tm), tn = (int)(t / p.tm);
+
+  // Steps [from, to) of dx's tile (tm, tn), as its part `part`.
+  __device__ static inline void dx(const ProductArgs& p, LdsChar* lds, int64_t N, int tm, int tn, int part, int from, int to) {
     const int n0 = tn * kTileN, m0 = tm * 256;
     if (n0 >= N) return;
-    const int from = (int)((int64_t)p.dx_steps * split / p.share.dx_split), to = (int)((int64_t)p.dx_steps * (split + 1) / p.share.dx_split);
     typename TX::Acc acc;
     TX::clear(acc);
     const typename TX::Side A{p.w + (m0 >> 5) * p.w_blk, (int)(p.dp - m0), p.w_ld, p.w_blk, p.w_rows, 0};
     const typename TX::Side B{p.g + (int64_t)n0 * 64, (int)(p.n_pad - n0), 64, p.n_pad * 64, 0, 0};
     if (to > from) TX::run(acc, lds, A, B, p.dx_segs, from * 32, to - from);
-    float* out = p.dx_part + ((int64_t)split * p.n_pad + n0) * p.dp + m0;
+    float* out = p.dx_part + ((int64_t)part * p.n_pad + n0) * p.dp + m0;
     auto fn = [&](int i, int j, int g) { return quad<float>([&](int e) { return acc[i][j][4 * g + e]; }); };
     const int rows = (int)(N - n0 < kTileN ? N - n0 : kTileN);
     if (p.dx_add) TX::template store_rows<float, true>(lds, out, p.dp, rows, (int)(p.dp - m0), true, fn);
     else TX::template store_rows<float, false>(lds, out, p.dp, rows, (int)(p.dp - m0), true, fn);
-  } else {
-    int64_t t = xcd_order(at, p.dw_blocks);
+  }
+
+  // Range t % dw_split of a tile of dW.
+  __device__ static inline void dw(const ProductArgs& p, LdsChar* lds, int64_t N, int64_t t) {
     const int split = (int)(t % p.share.dw_split);
     t /= p.share.dw_split;
     const int tm = (int)(t % p.tm);
@@ -221,6 +214,43 @@ __global__ void __launch_bounds__(kProductThreads, 2) products_kernel(ProductArg
                                         [&](int i, int j, int g) { return quad<T>([&](int e) { return acc[i][j][4 * g + e] * f * fx; }); });
     }
   }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kProductThreads, 2) products_kernel(ProductArgs p) {
+  __shared__ char smem[Products<T>::TX::LDS];
+  LdsChar* lds = (LdsChar*)smem;
+  const int64_t N = p.use_live ? p.hdr->live : p.N;
+  const int first = p.share.dx_first ? p.dx_blocks : p.dw_blocks;
+  const bool head = (int)blockIdx.x < first;
+  const int64_t at = head ? blockIdx.x : (int64_t)blockIdx.x - first;
+  if (head == p.share.dx_first) {
+    int64_t t = xcd_order(at, p.dx_blocks);
+    const int split = (int)(t % p.share.dx_split);
+    t /= p.share.dx_split;
+    const int from = (int)((int64_t)p.dx_steps * split / p.share.dx_split), to = (int)((int64_t)p.dx_steps * (split + 1) / p.share.dx_split);
+    Products<T>::dx(p, lds, N, (int)(t % p.tm), (int)(t / p.tm), split, from, to);
+  } else {
+    Products<T>::dw(p, lds, N, xcd_order(at, p.dw_blocks));
+  }
+}
+
+// As many blocks as CUs, each with its share of both products (WideShare).  Blocks of an XCD hold one range of many tiles,
+// so that they read the same rows of W at the same time.
+template <typename T>
+__global__ void __launch_bounds__(kProductThreads, 2) shares_kernel(ProductArgs p) {
+  __shared__ char smem[Products<T>::TX::LDS];
+  LdsChar* lds = (LdsChar*)smem;
+  const int64_t N = p.use_live ? p.hdr->live : p.N;
+  const int slot = (int)xcd_order(blockIdx.x, p.share.slots);
+  for (int t = slot; t < p.dw_blocks; t += p.share.slots) Products<T>::dw(p, lds, N, t);
+  const int part = slot / p.dx_tiles, tile = slot - part * p.dx_tiles;
+  if (part >= p.share.dx_split) return;
+  const int a = p.share.a, b = p.share.b, n = p.share.n_a;
+  int from = part < n ? part * a : n * a + (part - n) * b, to = part < n ? from + a : from + b;
+  if (part == p.share.dx_split - 1 || to > p.dx_steps) to = p.dx_steps;
+  if (from > to) from = to;
+  Products<T>::dx(p, lds, N, tile % p.tm, tile / p.tm, part, from, to);
 }
 
 // Sums of parts in their order, scaled, as rows of T.  A wave per row; the second matrix's rows follow the first's.
@@ -311,7 +341,8 @@ hipError_t products(const WideProducts& p, hipStream_t s) {
   ProductArgs a;
   a.N = p.N; a.n_pad = p.n_pad; a.d = p.d; a.dp = p.dp; a.share = p.share;
   a.tm = (int)((p.dp + 255) / 256);
-  a.dx_blocks = dx ? a.tm * (int)((p.n_pad + kTileN - 1) / kTileN) * p.share.dx_split : 0;
+  a.dx_tiles = dx ? a.tm * (int)((p.n_pad + kTileN - 1) / kTileN) : 0;
+  a.dx_blocks = a.dx_tiles * p.share.dx_split;
   a.dx_steps = (p.cols + 63) / 64 * 2;  // columns of G that are there: the gated kernel fills 64 at a time
   a.dw_tn = (p.cols + kTileN - 1) / kTileN;
   a.dw_blocks = dw ? a.tm * a.dw_tn * p.halves * p.share.dw_split : 0;
@@ -344,7 +375,8 @@ hipError_t products(const WideProducts& p, hipStream_t s) {
   a.dw0 = p.dw[0]; a.dw1 = p.dw[1]; a.dw_part = p.dw_part;
   a.hdr = p.hdr; a.unit = p.unit; a.cmax = p.cmax; a.use_live = p.use_live; a.gated = p.gated;
   a.vec = (int64_t)p.d * sizeof(T) % 16 == 0 && ((uintptr_t)p.dw[0] & 15) == 0 && ((uintptr_t)p.dw[1] & 15) == 0;
-  hipLaunchKernelGGL(products_kernel<T>, dim3((unsigned)(a.dx_blocks + a.dw_blocks)), dim3(kProductThreads), 0, s, a);
+  if (p.share.slots > 0) hipLaunchKernelGGL(shares_kernel<T>, dim3((unsigned)p.share.slots), dim3(kProductThreads), 0, s, a);
+  else hipLaunchKernelGGL(products_kernel<T>, dim3((unsigned)(a.dx_blocks + a.dw_blocks)), dim3(kProductThreads), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !dw || p.share.dw_split == 1) return e;
   PartArgs q = {};
@@ -412,7 +444,7 @@ WideShare wide_share(int64_t N, int d, int64_t C, int halves, int planes, bool d
   const int64_t tx = dx ? tm * ((N + kTileN - 1) / kTileN) : 0, kx = C / 32 * segs * halves;
   const int64_t tw = dw ? tm * (C / kTileN) * halves : 0, kw = (N + 31) / 32 * segs;
   constexpr int kCuts[] = {1, 2, 3, 4, 5, 6, 8, 11, 16, 24, 32, 48, 64};
-  WideShare best = {1, 1, true, -1};
+  WideShare best = {1, 1, true, -1, 0, 0, 0, 0};
   for (const int sx : kCuts) {
     if (sx > 1 && (!dx || kx / sx < 8)) break;
     const int64_t nx = tx * sx;
@@ -424,8 +456,28 @@ WideShare wide_share(int64_t N, int d, int64_t C, int halves, int planes, bool d
       const bool first = lx >= lw;
       const int64_t sum = kFloat * floats / kInFlight + (sw > 1 ? kLaunch : 0);
       const int64_t cost = sum + (first ? two_kinds(nx, lx, nw, lw) : two_kinds(nw, lw, nx, lx));
-      if (best.cost < 0 || cost < best.cost) best = WideShare{sx, sw, first, cost};
+      if (best.cost < 0 || cost < best.cost) best = WideShare{sx, sw, first, cost, 0, 0, 0, 0};
     }
+  }
+  // shares of both: `ranges` of dx's tiles for each CU's block, and what dW's leave over
+  const int64_t ranges = tx > 0 && tw > 0 ? kInFlight / tx : 0, xw = segs * halves, steps = C / 32;
+  if (ranges < 2 || ranges > 64) return best;
+  for (const int sw : kCuts) {
+    if (sw > 1 && kw / sw < 8) break;
+    const int64_t nw = tw * sw, floats = ranges * tx + (sw > 1 ? nw : 0), busy = kFloat * (floats < kInFlight ? floats : kInFlight) / kInFlight;
+    const int64_t lw = (kw + sw - 1) / sw + kFill + kStore + (sw > 1 ? busy : 0), lx = kFill + kStore + busy;
+    const int64_t q = nw / kInFlight, more = nw - q * kInFlight;  // `more` blocks have q + 1 ranges of dW
+    int64_t n_a = (more + tx - 1) / tx;
+    n_a = n_a < ranges ? n_a : ranges;
+    const int64_t goal = (kx + (n_a * (q + 1) + (ranges - n_a) * q) * lw + ranges - 1) / ranges;
+    const int64_t a = n_a > 0 ? (goal - (q + 1) * lw) / xw : 0;
+    if (n_a > 0 && a * xw < 16) continue;
+    const int64_t rest = n_a < ranges ? (steps - n_a * a + ranges - n_a - 1) / (ranges - n_a) : 0;
+    if (n_a < ranges && (rest < 1 || steps - n_a * a < 1)) continue;
+    const int64_t a_all = n_a == ranges ? (steps + ranges - 1) / ranges : a;
+    const int64_t cost = goal + xw + lx + kFloat * floats / kInFlight + (sw > 1 ? kLaunch : 0);
+    if (cost < best.cost)
+      best = WideShare{(int)ranges, sw, false, cost, (int)kInFlight, (int)n_a, (int)a_all, (int)(rest > 0 ? rest : 1)};
   }
   return best;
 }
