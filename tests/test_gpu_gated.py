@@ -147,6 +147,15 @@ def test_pieces_of_the_features():
         R.check(name, got[name], value, bound)
 
 
+@pytest.mark.parametrize("dtype,N", [(torch.bfloat16, 1999), (torch.float16, 1999), (torch.float32, 1100)])
+def test_blocks_that_share_both_products(dtype, N):
+    # sizes at which each CU's block takes ranges of dWg and dWu and then one of dx
+    x, wg, wu, dh = _data(N, 520, 7001, dtype, 9)
+    got = _run(x, wg, wu, dh, "silu")
+    for name, (value, bound) in R.gated(x, wg, wu, "silu", dh).items():
+        R.check(name, got[name], value, bound)
+
+
 def test_equal_calls_streams_and_graph():
     x, wg, wu, dh = _data(500, 128, 700, torch.float16, 7)
     first = _run(x, wg, wu, dh, "silu")
