@@ -387,7 +387,8 @@ int msa_verify(const msa_verify_args* args, void* stream);
  *              without an entry do not count.  A token that is named twice is
  *              two entries.
  *   reduction: 0: loss (N) fp32, rows that do not count 0; 1: their mean over
- *              the rows that count (NaN if none does); 2: their sum.
+ *              the rows that count (NaN if none does, with
+ *              gradients of zeros); 2: their sum.
  * A row that counts and names a token outside [0, V) has loss NaN and gradient
  * NaN.  Rows that do not count are not read beyond their ids (and teacher): their
  * hidden may hold anything, and their gradient is 0.

@@ -105,7 +105,8 @@ struct GradUnit {
 __device__ inline float unit_of(const GradUnit& u, const WideHdr* h, const float* cmax) {
   if (u.mode == 3) return 1.0f;
   if (u.mode == 0) return *cmax;
-  return u.mode == 1 ? u.dloss[0] * u.factor / (float)h->live : u.dloss[0] * u.factor;
+  if (u.mode == 2) return u.dloss[0] * u.factor;
+  return h->live > 0 ? u.dloss[0] * u.factor / (float)h->live : 0.0f;  // a mean over no rows: gradients of zeros
 }
 
 // How the two products of a piece are cut: each of dx's tiles into dx_split ranges of its k, dW's into dw_split.  cost:

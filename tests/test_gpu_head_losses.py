@@ -157,6 +157,8 @@ def test_no_row_counts():
     loss = ops.linear_cross_entropy(a, b, y, reduction="sum")
     dx, dw = _grads(loss, a, b)
     assert float(loss.detach()) == 0.0 and not dx.any() and not dw.any()
+    dx, dw = _grads(ops.linear_cross_entropy(a, b, y), a, b)  # a mean of none is NaN, its gradients are zeros
+    assert not dx.any() and not dw.any()
     rows = ops.linear_cross_entropy(x, w, y, reduction="none")
     assert not rows.any()
     none = ops.linear_distillation(x, w, torch.zeros(20, 3, device=DEV), torch.full((20, 3), -1, device=DEV), reduction="sum")

@@ -31,6 +31,13 @@ def test_cross_entropy_is_torchs(reduction):
         _dense.linear_cross_entropy_dense(x, w, y, -100, "batch")
 
 
+def test_a_mean_of_no_rows_has_gradients_of_zeros():
+    x, w = torch.randn(5, 8, requires_grad=True), torch.randn(11, 8, requires_grad=True)
+    loss = _dense.linear_cross_entropy_dense(x, w, torch.full((5,), -100))
+    loss.backward()
+    assert bool(torch.isnan(loss)) and not x.grad.any() and not w.grad.any()
+
+
 def test_distillation_over_the_whole_vocabulary_is_kl():
     torch.manual_seed(2)
     x, w, t = torch.randn(9, 16), torch.randn(13, 16), torch.randn(9, 13)
