@@ -80,7 +80,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const int64_t* ids, int64_t 
 }
 
 // A teacher's record of a row: entries with an id >= 0 and a logit above -inf; p = their softmax at 1/T.  A wave per
-// row.  tp[n][k] = (p, p summed over the row's entries of the same id); ent[n] = sum p ln p.  NaN logits, or +inf, give NaN.
+// row.  tp[n][k] = (p, p summed over the row's entries of the same id), p = -1: no entry; ent[n] = sum p ln p.
+// NaN logits, or +inf, give NaN.
 template <typename L>
 __global__ void __launch_bounds__(kThreads) teacher_kernel(const L* logits, int64_t lld, const int64_t* ids,
                                                            int64_t ids_ld, int64_t N, int K, float inv_t, float2* tp,
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(kThreads) teacher_kernel(const L* logits, int6
       const int k = q * 64 + lane;
       const float lp = t[q] - mx - ls, p = t[q] == -INFINITY ? 0.0f : expf(lp);
       h += p > 0.0f ? p * lp : p;  // 0 ln 0 = 0; NaN stays
-      t[q] = p;
+      t[q] = t[q] == -INFINITY ? -1.0f : p;
       sid[wave][k] = id[q];
       sp[wave][k] = p;
     }
@@ -325,8 +326,8 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
         const float away = (stat[r].x - to_log2 * dot) + stat[r].y;  // lse2 - z2
         t = __builtin_amdgcn_exp2f(-away) - p.y;
         term = p.x > 0.0f || !(p.x == p.x) ? p.x * away : 0.0f;
-      } else {
-        t = term = NAN;
+      } else if (!(p.x < 0.0f)) {
+        t = term = NAN;  // an entry outside the vocabulary
       }
     }
     if (l16 == 0) {

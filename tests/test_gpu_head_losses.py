@@ -149,6 +149,26 @@ def test_rows_that_do_not_count_may_hold_anything(dtype):
         assert torch.equal(a, b) and bool(torch.isfinite(a).all())
 
 
+def test_entries_that_are_none_may_name_any_token():
+    N, d, V = 70, 64, 300
+    x, w, _, g = _data(N, d, V, torch.bfloat16, 21)
+    t, ids = _teacher(N, V, 6, g)
+    t[:, 2] = -math.inf
+    t[5] = -math.inf  # no entry at all
+    ids[:, 2] = -7
+    ids[5] = -7
+    far = ids.clone()
+    far[::2, 2] = V + 5
+    far[5] = V
+    out = []
+    for i in (ids, far):
+        a, b = _leaf(x, w)
+        loss = ops.linear_distillation(a, b, t, i, 1.5)
+        out.append((loss.detach(), *_grads(loss, a, b)))
+    for a, b in zip(*out):
+        assert torch.equal(a, b) and bool(torch.isfinite(a).all())
+
+
 def test_no_row_counts():
     x, w, _, _ = _data(20, 64, 100, torch.bfloat16)
     y = torch.full((20,), -100, device=DEV)
