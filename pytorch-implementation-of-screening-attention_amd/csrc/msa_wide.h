@@ -17,7 +17,7 @@ template <typename T> struct Wide { typedef T E; static constexpr int P = 1; };
 template <> struct Wide<float> { typedef f16 E; static constexpr int P = 2; };
 
 // Device-side facts of a call.  max: bits of the largest finite |entry| of x (rows that count), w, dh, and of the largest
-// finite squared row norm of x and w; floats of one sign compare as integers, so atomicMax gives the same whatever the
+// row norm of x and w (of their finite entries); floats of one sign compare as integers, so atomicMax gives the same whatever the
 // order.  Each has kSlots places a cache line apart (blocks in turn), which a reader takes the largest of: 2700 atomics to
 // one place take 40 us.
 constexpr int kSlots = 16;
@@ -29,14 +29,17 @@ struct WideHdr {
 };
 constexpr int kHdrWords = (int)(sizeof(WideHdr) / 4);
 
-__device__ inline float pow2_to(float mx, int top) {  // p with mx p in [2^(top-1), 2^top); 1 for 0
-  if (!(mx > 0.0f)) return 1.0f;
-  int ex;
-  (void)frexpf(mx, &ex);
-  int e = top - ex;
+// p with a b c p in [2^(top-1), 2^top); 1 for 0.  The product itself may be too large or too small for a float.
+__device__ inline float pow2_to(float a, float b, float c, int top) {
+  if (!(a > 0.0f) || !(b > 0.0f) || !(c > 0.0f)) return 1.0f;
+  int ea, eb, ec, em;
+  const float m = frexpf(a, &ea) * frexpf(b, &eb) * frexpf(c, &ec);
+  (void)frexpf(m, &em);
+  int e = top - (ea + eb + ec + em);
   e = e > 120 ? 120 : (e < -120 ? -120 : e);
   return ldexpf(1.0f, e);
 }
+__device__ inline float pow2_to(float mx, int top) { return pow2_to(mx, 1.0f, 1.0f, top); }
 // Every lane of the wave calls it.
 __device__ inline float wide_max(const WideHdr* h, int which) {
   float v = __uint_as_float(h->max[which][threadIdx.x & (kSlots - 1)][0]);
@@ -58,7 +61,7 @@ template <typename T> __device__ inline float scale_w(const WideHdr* h) {
 template <typename T> __device__ inline float scale_g(const WideHdr* h, int gated) {
   if constexpr (__is_same(T, bf16)) return 1.0f;
   if (!gated) return 32768.0f;
-  return pow2_to(1.15f * wide_max(h, kMaxDh) * sqrtf(wide_max(h, kNormX)) * sqrtf(wide_max(h, kNormW)), 15);
+  return pow2_to(1.15f * fminf(wide_max(h, kMaxDh), 1e38f), wide_max(h, kNormX), wide_max(h, kNormW), 15);
 }
 
 // The terms of v (already scaled).  v is held in a register first: formed inside, a product that makes v may be rounded
@@ -92,7 +95,7 @@ struct RowsCopies {
   void add(const RowsCopy& c) { m[n++] = c; }
 };
 hipError_t launch_rows_copy(const RowsCopies& c, hipStream_t s);
-// max|entry| and, where asked for, the largest squared row norm of the matrices, into hdr.
+// max|entry| and, where asked for, the largest row norm of the matrices, into hdr.
 hipError_t launch_rows_max(const RowsCopies& c, hipStream_t s);
 hipError_t launch_hdr_clear(WideHdr* hdr, hipStream_t s);
 

@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(kThreads) rows_max_kernel(RowsArgs a) {
   for (int64_t r = ((int64_t)blockIdx.x - a.first[i]) * 4 + wave; r < m.rows; r += step) {
     if (m.pos != nullptr && m.pos[r] < 0) continue;
     const T* p = (const T*)m.src + r * m.ld;
-    float ss = 0.0f;
+    float ss = 0.0f, rx = 0.0f;
     for (int c = lane * 8; c < m.d; c += 512) {
       T x[8];
       load8(p, c, m.d, a.vec[i] != 0, x);
@@ -69,14 +69,21 @@ __global__ void __launch_bounds__(kThreads) rows_max_kernel(RowsArgs a) {
       for (int e = 0; e < 8; ++e) {
         const float v = fabsf(to_f(x[e]));
         if (v < INFINITY) {
-          mx = fmaxf(mx, v);
+          rx = fmaxf(rx, v);
           ss = fmaf(v, v, ss);
         }
       }
     }
+    mx = fmaxf(mx, rx);
     if (m.norms) {
       ss = wave_sum(ss);
-      if (ss < INFINITY) nx = fmaxf(nx, ss);
+      if (ss > 1e-30f && ss < INFINITY) {
+        nx = fmaxf(nx, sqrtf(ss));
+      } else {  // squares left fp32's range: a bound that does not
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) rx = fmaxf(rx, __shfl_xor(rx, o));
+        nx = fmaxf(nx, fminf(rx * sqrtf((float)m.d), 3e38f));
+      }
     }
   }
 #pragma unroll

@@ -64,6 +64,19 @@ def test_scales_of_gradients(dtype):
             R.check(name, got[name], value, bound)
 
 
+@pytest.mark.parametrize("up", [66, -66])
+def test_operands_whose_squares_leave_the_range(up):
+    # x and the weights far from 1 in opposite directions, in fp32: the products are ordinary, the rows' squares are not, and
+    # the bound of a row's norm is its largest entry times sqrt(d)
+    x, wg, wu, dh = _data(150, 64, 200, torch.float32, 5)
+    x, wg, wu, dh = x * 2.0 ** up, wg * 2.0 ** -up, wu * 2.0 ** -up, dh * 2.0 ** -20
+    got = _run(x, wg, wu, dh, "silu")
+    w = torch.cat([wg, wu])
+    spread = math.prod(8.0 * float(t.abs().amax()) / float(t.double().norm(dim=1).amax()) for t in (x, w))
+    for name, (value, bound) in R.gated(x, wg, wu, "silu", dh, spread).items():
+        R.check(name, got[name], value, bound)
+
+
 def test_zero_gradient_and_no_rows():
     for dtype in TYPES:
         x, wg, wu, dh = _data(70, 64, 100, dtype)

@@ -91,7 +91,7 @@ def act_slope(g, activation):
     return g * c, c + g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
 
 
-def gated(x, wg, wu, activation, dh=None):
+def gated(x, wg, wu, activation, dh=None, spread=1.0):
     dtype = x.dtype
     X, G, U = x.flatten(0, -2).double(), wg.double(), wu.double()
     d = X.shape[1]
@@ -116,9 +116,10 @@ def gated(x, wg, wu, activation, dh=None):
     dg_b = D.abs() * (u_off * (s.abs() + s_off) + u.abs() * s_off)
     du_b = D.abs() * a_off
     # one rounding of dg and du, relative, or of the smallest number kept: fp16 keeps 2^-24 beside a bound of 2^15
-    # over every |dg| and |du|, max|dh| 1.15 max|x| max|w| (and a factor of two of the power of two)
+    # over every |dg| and |du|, max|dh| 1.15 max|x| max|w| (and a factor of two of the power of two); spread: how far the
+    # kernel's max|x| max|w| lies over the norms
     floor = 2.0 ** -39 * 2 * 1.15 * float(D.abs().amax()) * float(X.norm(dim=1).amax()) * float(
-        max(G.norm(dim=1).amax(), U.norm(dim=1).amax())) * 0.5 if dtype != torch.bfloat16 else 0.0
+        max(G.norm(dim=1).amax(), U.norm(dim=1).amax())) * 0.5 * spread if dtype != torch.bfloat16 else 0.0
     dg_b = dg_b + (ug + 8 * U32) * (dg.abs() + dg_b) + floor
     du_b = du_b + (ug + 8 * U32) * (du.abs() + du_b) + floor
 
