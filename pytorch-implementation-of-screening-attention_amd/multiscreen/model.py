@@ -120,8 +120,6 @@ class MultiscreenLM(nn.Module):
         positions' logits exist at a time."""
         rows = self.hidden_states(input_ids, key_padding_mask).flatten(0, 1)
         parts = [self.lm_head(x).topk(k, -1) for x in rows.split(1024)]
-        if not parts:
-            parts = [self.lm_head(rows).topk(k, -1)]
         values, ids = (torch.cat(p).view(*input_ids.shape, k) for p in zip(*parts))
         return values, ids
 

@@ -648,10 +648,14 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="m
     do not count: their loss and gradient are 0, whatever hidden holds there.
     Other labels outside [0, V) give NaN.
     reduction "mean" (over the rows that count; NaN if none does, with gradients of
-    zeros), "sum", or "none": a loss per row, shaped as labels, of which N = 1 and a few rows are the
-    scores of a decoding step.  float32; sums and softmax statistics are too.
+    zeros), "sum", or "none": a loss per row, shaped as labels, of which N = 1 and a
+    few rows are the scores of a decoding step.  float32; sums and softmax
+    statistics are too.
     The backward pass forms the logits again, in pieces of the vocabulary of at
     most 1 GB; their gradient is rounded to hidden's type (float32: 22 bits).
+    Forward and backward pass can be captured into a HIP graph together, once no
+    autograd graph of an eager call on the same leaves is alive (torch's rule for
+    every backward pass).
     """
     hidden, weight = _autocast(hidden, weight)
     _head_checks("linear_cross_entropy", hidden, weight, reduction, labels)
