@@ -395,8 +395,8 @@ int msa_verify(const msa_verify_args* args, void* stream);
  * msa_head_bwd takes the same arguments, state as msa_head_fwd left it (read
  * only) and dloss, fp32: (N) for reduction 0, one value else.  dhidden (N, d) and dweight (V, d) contiguous, of type dtype;
  * either may be null.  The gradient of the logits is formed in pieces of the
- * vocabulary, rounded to dtype (fp32: to two fp16 terms, 22 bits) and multiplied
- * with fp32 sums.
+ * vocabulary, rounded to dtype (fp32: to two fp16 terms, 22 bits; the others up to
+ * 256 rows: to two terms of their own) and multiplied with fp32 sums.
  * state: msa_head_state_bytes, kept from forward to backward, or null for a forward
  * pass that no backward pass follows.  workspace: msa_head_workspace_bytes of the
  * same arguments (backward 0 or 1; of state only whether it is null; loss, dloss
@@ -442,7 +442,7 @@ int msa_head_bwd(const msa_head_args* args, void* stream);
  * msa_gated_bwd: dh (N, F), unit stride over F, dh_ld from row to row; dx (N, d),
  * dgate, dup (F, d) contiguous, of type dtype.  dx may be null, or dgate and dup
  * both.  The gradients of x Wg^T and x Wu^T are formed in pieces of the features,
- * rounded to dtype behind a power of two (fp32: to two fp16 terms), sums are
+ * rounded to dtype behind a power of two (two terms as in msa_head_bwd), sums are
  * fp32.
  * Operands are used in place under the conditions of msa_head_args' weight.
  * workspace: msa_gated_workspace_bytes of the same arguments.  1 <= d <= 65536, 1 <= F

@@ -60,7 +60,7 @@ template <typename E> using GatedHalf = MmTile<E, 128, 128, 2, 2, false, false, 
 template <typename E> using GatedFew = MmTile<E, 64, 32, 2, 1, false, false, true, 8>;
 constexpr int kFew = 32;
 
-template <typename T, int ACT, bool BWD, typename Tl>
+template <typename T, int ACT, int TERMS, typename Tl>  // TERMS: of dg and du; 0: forward
 __global__ void __launch_bounds__(Tl::THREADS, Tl::TILE_M == 128 ? 3 : 2) gated_kernel(GatedArgs a) {
   using E = typename Wide<T>::E;
   constexpr int BF = Tl::TILE_M / 2, BN = Tl::TILE_N;
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(Tl::THREADS, Tl::TILE_M == 128 ? 3 : 2) gated_
     f1 = 1.0f / scale_x<T>(a.hdr);
     f2 = 1.0f / scale_w<T>(a.hdr);
   }
-  if constexpr (!BWD) {
+  if constexpr (TERMS == 0) {
     T* out = (T*)a.h + n0 * a.h_ld + f0;
     Tl::store_dual(lds, out, a.h_ld, rows, fleft, a.vec != 0, [&](int i, int j, int q) {
       return quad<T>([&](int e) { return act_of<ACT>(acc[i][j][4 * q + e] * f1 * f2) * (acc[i][j][4 * q + e + 8] * f1 * f2); });
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(Tl::THREADS, Tl::TILE_M == 128 ? 3 : 2) gated_
         *reinterpret_cast<LdsTV*>(lds + row * ROW + f * (int)sizeof(T)) = v;
       }
       Tl::sync_lds();
-      typename Quad<E>::V grads[2][Wide<T>::P][NQ];  // [dg, du][term], rounded as they are made
+      typename Quad<E>::V grads[2][TERMS][NQ];  // [dg, du][term], rounded as they are made
       const LdsChar* at = lds + (wn * 32 + (lane & 31)) * ROW + (wm * (BF / 2) + 4 * (lane >> 5)) * (int)sizeof(T);
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
@@ -129,8 +129,8 @@ __global__ void __launch_bounds__(Tl::THREADS, Tl::TILE_M == 128 ? 3 : 2) gated_
           const float v[2] = {ds * u * slope, ds * act};
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            if constexpr (Wide<T>::P == 2) {
-              const Terms<float> t(v[half]);
+            if constexpr (TERMS == 2) {
+              const Terms<E> t(v[half]);
               grads[half][0][q][e] = t.h;
               grads[half][1][q][e] = t.l;
             } else {
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(Tl::THREADS, Tl::TILE_M == 128 ? 3 : 2) gated_
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int t = 0; t < Wide<T>::P; ++t)
+        for (int t = 0; t < TERMS; ++t)
           Tl::template store_operand_tokens<Tl::MB / 2>(lds, reinterpret_cast<E*>(a.g + half * a.half + t * a.plane) + (f0 >> 5) * (a.n_pad * 32) + n0 * 32,
                                                         a.n_pad * 32, j, [&](int i, int q) { return grads[half][t][4 * i + q]; });
     }
@@ -164,7 +164,7 @@ bool direct(const GatedCall& c, const void* p, int64_t ld) {
 
 struct GatedPlan {
   int64_t n_pad, dp, x_plane, w_plane, C, g_plane;
-  int planes;
+  int planes, g_terms;
   WideShare share;
   char *x, *w, *g;
   float *dx_part, *dw_part;
@@ -172,6 +172,7 @@ struct GatedPlan {
   size_t bytes;
   GatedPlan(const GatedCall& c, int backward) {
     planes = c.dtype == 0 ? 2 : 1;
+    g_terms = terms_of_g(c.dtype, c.N);
     n_pad = round_up(c.N > 0 ? c.N : 1, 128);
     dp = wide_dp(c.d);
     x_plane = round_up(n_pad * dp * 2, 256);
@@ -186,9 +187,9 @@ struct GatedPlan {
     share = WideShare{};
     g = nullptr; dx_part = dw_part = nullptr;
     if (backward) {
-      C = wide_piece(c.N, c.d, c.F, 2, planes, c.dx != nullptr, c.dw[0] != nullptr, 2 * planes * 2 * n_pad, &share);
+      C = wide_piece(c.N, c.d, c.F, 2, planes == 2 ? 3 : g_terms, c.dx != nullptr, c.dw[0] != nullptr, 2 * g_terms * 2 * n_pad, &share);
       g_plane = round_up(n_pad * C * 2, 256);
-      g = take(2 * planes * g_plane);
+      g = take(2 * g_terms * g_plane);
       if (c.dx != nullptr) dx_part = (float*)take((int64_t)share.dx_split * n_pad * dp * 4);
       if (c.dw[0] != nullptr && share.dw_split > 1) dw_part = (float*)take((int64_t)share.dw_split * 2 * C * dp * 4);
     }
@@ -244,22 +245,22 @@ GatedArgs args_of(const GatedCall& c, const GatedPlan& p, const GatedOperands& o
   return a;
 }
 
-template <typename T, bool BWD, template <typename> class Tile>
+template <typename T, int TERMS, template <typename> class Tile>
 hipError_t launch_tiles(GatedArgs a, int act, hipStream_t s) {
   using Tl = Tile<typename Wide<T>::E>;
   a.tiles_f = (a.cols + Tl::TILE_M / 2 - 1) / (Tl::TILE_M / 2);
   a.tiles_n = (int)((a.N + Tl::TILE_N - 1) / Tl::TILE_N);
-  auto* k = act == 0 ? gated_kernel<T, 0, BWD, Tl> : gated_kernel<T, 1, BWD, Tl>;
+  auto* k = act == 0 ? gated_kernel<T, 0, TERMS, Tl> : gated_kernel<T, 1, TERMS, Tl>;
   hipLaunchKernelGGL(k, dim3((unsigned)((int64_t)a.tiles_f * a.tiles_n)), dim3(Tl::THREADS), 0, s, a);
   return hipGetLastError();
 }
 
-template <typename T, bool BWD>
+template <typename T, int TERMS>
 hipError_t launch(const GatedArgs& a, int act, hipStream_t s) {
-  if (!BWD && a.N <= kFew) return launch_tiles<T, false, GatedFew>(a, act, s);
+  if (TERMS == 0 && a.N <= kFew) return launch_tiles<T, 0, GatedFew>(a, act, s);
   const int64_t tiles_n = (a.N + 127) / 128;
-  return smaller_tiles((a.cols + 127) / 128, tiles_n, (a.cols + 63) / 64) ? launch_tiles<T, BWD, GatedHalf>(a, act, s)
-                                                                        : launch_tiles<T, BWD, GatedTile>(a, act, s);
+  return smaller_tiles((a.cols + 127) / 128, tiles_n, (a.cols + 63) / 64) ? launch_tiles<T, TERMS, GatedHalf>(a, act, s)
+                                                                        : launch_tiles<T, TERMS, GatedTile>(a, act, s);
 }
 
 template <typename T>
@@ -271,7 +272,7 @@ hipError_t gated_fwd(const GatedCall& c) {
   GatedArgs a = args_of(c, p, o, 0, c.F);
   a.h = c.h; a.h_ld = c.F;
   a.vec = (int64_t)c.F * sizeof(T) % 16 == 0 && ((uintptr_t)c.h & 15) == 0;
-  return launch<T, false>(a, c.act, c.stream);
+  return launch<T, 0>(a, c.act, c.stream);
 }
 
 template <typename T>
@@ -292,8 +293,8 @@ hipError_t gated_bwd(const GatedCall& c) {
     GatedArgs a = args_of(c, p, o, f0, cols);
     a.dh = (const T*)c.dh + f0; a.dh_ld = c.dh_ld;
     a.vec = c.dh_ld * sizeof(T) % 16 == 0 && ((uintptr_t)c.dh & 15) == 0;
-    a.g = p.g; a.plane = p.g_plane; a.half = p.planes * p.g_plane;
-    GATED_TRY((launch<T, true>(a, c.act, c.stream)));
+    a.g = p.g; a.plane = p.g_plane; a.half = p.g_terms * p.g_plane;
+    GATED_TRY((p.g_terms == 2 ? launch<T, 2>(a, c.act, c.stream) : launch<T, Wide<T>::P>(a, c.act, c.stream)));
     WideProducts q = {};
     q.dtype = c.dtype; q.gated = 1; q.N = c.N; q.n_pad = p.n_pad; q.d = c.d; q.dp = p.dp; q.halves = 2; q.cols = cols; q.C = p.C;
     q.x = o.x; q.x_ld = o.x_ld; q.x_blk = o.x_blk; q.x_plane = p.x_plane; q.x_rows = o.x_rows;
@@ -302,7 +303,7 @@ hipError_t gated_bwd(const GatedCall& c) {
       q.dw[i] = c.dw[i] == nullptr ? nullptr : (char*)c.dw[i] + f0 * c.d * es_of(c.dtype);
     }
     q.w_ld = o.w_ld; q.w_blk = o.w_blk; q.w_plane = p.w_plane; q.w_rows = (int)(c.F - f0);
-    q.g = p.g; q.g_plane = p.g_plane; q.g_half = p.planes * p.g_plane;
+    q.g = p.g; q.g_plane = p.g_plane; q.g_half = p.g_terms * p.g_plane; q.g_terms = p.g_terms;
     q.dx_part = p.dx_part; q.dx_add = f0 > 0; q.dw_part = p.dw_part;
     q.share = p.share; q.hdr = p.hdr; q.unit.mode = 3; q.use_live = 0;
     GATED_TRY(launch_wide_products(q, c.stream));

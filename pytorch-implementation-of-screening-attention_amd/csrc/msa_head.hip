@@ -415,7 +415,7 @@ struct GradArgs {
 };
 
 // G of one tile: c_n 2^(z2 - lse2), without the targets, which scatter_kernel puts in their place.
-template <typename T>
+template <typename T, int TERMS>
 __global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
   using E = typename Wide<T>::E;
   using Tl = MmTile<E, 256, 128, 2, 2, false, false, false, 3>;
@@ -456,14 +456,14 @@ __global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
         for (int r = 0; r < 16; ++r) acc[i][j][r] *= c;
     }
   }
-  if constexpr (Wide<T>::P == 2) {
+  if constexpr (TERMS == 2) {
     Tl::store_operand(lds, out, blk, [&](int i, int j, int g) {
-      return quad<E>([&](int e) { return (float)Terms<float>(acc[i][j][4 * g + e]).h; });
+      return quad<E>([&](int e) { return (float)Terms<E>(acc[i][j][4 * g + e]).h; });
     });
     Tl::renew(acc);
     Tl::store_operand(lds, reinterpret_cast<E*>(reinterpret_cast<char*>(out) + a.plane), blk,
                                       [&](int i, int j, int g) {
-                                        return quad<E>([&](int e) { return (float)Terms<float>(acc[i][j][4 * g + e]).l; });
+                                        return quad<E>([&](int e) { return (float)Terms<E>(acc[i][j][4 * g + e]).l; });
                                       });
   } else {
     Tl::store_operand(lds, out, blk, [&](int i, int j, int g) {
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) scatter_kernel(const int64_t* ids, int64_t ids_ld, int64_t N, int K, const int* pos,
                                                            const float* t, const float* coef, const WideHdr* hdr, int64_t v0,
-                                                           int cols, char* g, int64_t n_pad, int64_t plane) {
+                                                           int cols, char* g, int64_t n_pad, int64_t plane, int terms) {
   using E = typename Wide<T>::E;
   const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   const int64_t n = e / K;
@@ -486,13 +486,9 @@ __global__ void __launch_bounds__(kThreads) scatter_kernel(const int64_t* ids, i
   if (at < 0 || v < 0 || v >= cols) return;
   const float x = (coef != nullptr ? t[e] * coef[at] : t[e]) * scale_g<T>(hdr, 0);
   E* p = reinterpret_cast<E*>(g) + (v >> 5) * (n_pad * 32) + (int64_t)at * 32 + (v & 31);
-  if constexpr (Wide<T>::P == 2) {
-    const Terms<float> w(x);
-    *p = w.h;
-    *reinterpret_cast<E*>(reinterpret_cast<char*>(p) + plane) = w.l;
-  } else {
-    *p = (E)x;
-  }
+  const Terms<E> w(x);
+  *p = w.h;
+  if (terms == 2) *reinterpret_cast<E*>(reinterpret_cast<char*>(p) + plane) = w.l;
 }
 
 __global__ void zero_kernel(uint16_t* p, int64_t n) {
@@ -520,7 +516,7 @@ bool x_direct(const HeadCall& c) {
 
 struct HeadPlan {
   int64_t n_pad, dp, x_plane, w_plane, C, g_plane;
-  int planes, tiles_n, tiles_v;
+  int planes, g_terms, tiles_n, tiles_v;
   WideShare share;
   bool distill, few, direct;  // direct: x is used as it is
   char *x, *w, *g, *state = nullptr;
@@ -531,6 +527,7 @@ struct HeadPlan {
   HeadPlan(const HeadCall& c, int backward) {
     distill = c.teacher != nullptr;
     planes = c.dtype == 0 ? 2 : 1;
+    g_terms = terms_of_g(c.dtype, c.N);
     n_pad = round_up(c.N > 0 ? c.N : 1, 128);
     dp = wide_dp(c.d);
     x_plane = round_up(n_pad * dp * 2, 256);
@@ -557,9 +554,9 @@ struct HeadPlan {
         live = (uint8_t*)take(c.N);
       }
     } else {
-      C = wide_piece(c.N, c.d, c.V, 1, planes, c.dx != nullptr, c.dw != nullptr, planes * 2 * n_pad, &share);
+      C = wide_piece(c.N, c.d, c.V, 1, planes == 2 ? 3 : g_terms, c.dx != nullptr, c.dw != nullptr, g_terms * 2 * n_pad, &share);
       g_plane = round_up(n_pad * C * 2, 256);
-      g = take(planes * g_plane);
+      g = take(g_terms * g_plane);
       if (c.reduction == 0) {
         coef = (float*)take(n_pad * 4);
         cmax = (float*)take(4);
@@ -668,17 +665,18 @@ hipError_t head_bwd(const HeadCall& c) {
     a.x = p.x; a.n_pad = p.n_pad; a.w = w + v0 * w_ld; a.w_ld = w_ld; a.w_blk = w_blk; a.cols = cols;
     a.segs = p.logits(); a.ksteps = (int)(p.dp / 32); a.tiles_v = (int)(round_up(cols, 256) / 256); a.tiles_n = p.tiles_n;
     a.to_log2 = kLog2e / c.temperature; a.hdr = st.hdr; a.lse2 = st.lse2; a.coef = p.coef; a.g = p.g; a.plane = p.g_plane;
-    hipLaunchKernelGGL(grad_kernel<T>, dim3((unsigned)((int64_t)a.tiles_v * a.tiles_n)), dim3(kThreads), 0, c.stream, a);
+    auto* grad = p.g_terms == 2 ? grad_kernel<T, 2> : grad_kernel<T, Wide<T>::P>;
+    hipLaunchKernelGGL(grad, dim3((unsigned)((int64_t)a.tiles_v * a.tiles_n)), dim3(kThreads), 0, c.stream, a);
     HEAD_TRY(hipGetLastError());
     hipLaunchKernelGGL(scatter_kernel<T>, dim3((unsigned)((c.N * c.K + kThreads - 1) / kThreads)), dim3(kThreads), 0, c.stream,
-                       c.ids, c.ids_ld, c.N, c.K, st.pos, st.t, p.coef, st.hdr, v0, cols, p.g, p.n_pad, p.g_plane);
+                       c.ids, c.ids_ld, c.N, c.K, st.pos, st.t, p.coef, st.hdr, v0, cols, p.g, p.n_pad, p.g_plane, p.g_terms);
     HEAD_TRY(hipGetLastError());
     WideProducts q = {};
     q.dtype = c.dtype; q.gated = 0; q.N = c.N; q.n_pad = p.n_pad; q.d = c.d; q.dp = p.dp; q.halves = 1; q.cols = cols;
     q.C = p.C;
     q.x = p.x; q.x_ld = 64; q.x_blk = p.n_pad * 64; q.x_plane = p.x_plane; q.x_rows = (int)p.n_pad;
     q.w[0] = w + v0 * w_ld; q.w_ld = w_ld; q.w_blk = w_blk; q.w_plane = p.w_plane; q.w_rows = (int)(c.V - v0);
-    q.g = p.g; q.g_plane = p.g_plane; q.g_half = 0;
+    q.g = p.g; q.g_plane = p.g_plane; q.g_half = 0; q.g_terms = p.g_terms;
     q.dx_part = p.dx_part; q.dx_add = v0 > 0;
     q.dw[0] = c.dw == nullptr ? nullptr : (char*)c.dw + v0 * c.d * es_of(c.dtype); q.dw_part = p.dw_part;
     q.share = p.share; q.hdr = st.hdr; q.unit = unit; q.cmax = p.cmax; q.use_live = 1;

@@ -64,17 +64,24 @@ template <typename T> __device__ inline float scale_g(const WideHdr* h, int gate
   return pow2_to(1.15f * fminf(wide_max(h, kMaxDh), 1e38f), wide_max(h, kNormX), wide_max(h, kNormW), 15);
 }
 
-// The terms of v (already scaled).  v is held in a register first: formed inside, a product that makes v may be rounded
+// The terms of v (already scaled) in an operand type.  v is held in a register first: formed inside, a product that makes v may be rounded
 // to h straight from its exact value in one place and from the rounded one in another, and l belongs to one h only.
-template <typename T> struct Terms;
-template <> struct Terms<float> {
-  f16 h, l;
+template <typename E> struct Terms {
+  E h, l;
   __device__ explicit Terms(float v) {
     asm("" : "+v"(v));
-    h = (f16)v;
-    l = (f16)((v - (float)h) * 2048.0f);
+    h = (E)v;
+    l = (E)((v - (float)h) * 2048.0f);
   }
 };
+
+// Terms of G.  2-byte types keep one, in their own type: beside the rounding of dx and dW themselves that makes their error
+// sqrt(2) times as large on average, as any training that keeps such gradients.  Few rows average over few roundings, and
+// their products are short: two terms up to 256 rows.  Error of dx and dW over that of their own rounding, one term / two: 1.79
+// / 1.00 for 2 rows, 1.48 / 1.00 for 18, 1.24 to 1.41 / 1.00 for 100 and more.  Time: 84 rows of 1024 by 51364 bf16 191 / 226 us,
+// shorter calls alike (their launches).
+constexpr int64_t kTwoTerms = 256;
+inline int terms_of_g(int dtype, int64_t N) { return dtype == 0 || N <= kTwoTerms ? 2 : 1; }
 
 inline int64_t wide_dp(int64_t d) { return round_up(d, 32); }
 
@@ -123,9 +130,10 @@ struct WideShare {
   int64_t cost;
   int slots, n_a, a, b;
 };
-WideShare wide_share(int64_t N, int d, int64_t C, int halves, int planes, bool dx, bool dw);
+// segs: products that each tile adds up of one weight (MmSegs).
+WideShare wide_share(int64_t N, int d, int64_t C, int halves, int segs, bool dx, bool dw);
 // The columns of a piece of `rows` weight rows whose G takes `bytes_of_column` a column: 1 GB of G, 512 or 256 MB, by cost.
-int64_t wide_piece(int64_t N, int d, int64_t rows, int halves, int planes, bool dx, bool dw, int64_t bytes_of_column, WideShare* share);
+int64_t wide_piece(int64_t N, int d, int64_t rows, int halves, int segs, bool dx, bool dw, int64_t bytes_of_column, WideShare* share);
 
 // The backward products of one piece of the weight's rows.
 struct WideProducts {
@@ -138,7 +146,7 @@ struct WideProducts {
   int64_t C;         // columns of g: cols rounded up to 256
   const char* x; int64_t x_ld, x_blk, x_plane; int x_rows;    // bytes from row to row, from 32 columns on, to the second term; readable rows
   const char* w[2]; int64_t w_ld, w_blk, w_plane; int w_rows;        // the piece's first rows; readable rows from there
-  const char* g; int64_t g_plane, g_half;                     // [half][term][C / 32][n_pad][32]
+  const char* g; int64_t g_plane, g_half; int g_terms;        // [half][term][C / 32][n_pad][32]
   float* dx_part; int dx_add;                                 // [share.dx_split][n_pad][dp], or null: no dx
   void* dw[2];                                                // the piece's rows of the gradients, or null
   float* dw_part;                                             // [share.dw_split][halves][C][dp] where that is over 1

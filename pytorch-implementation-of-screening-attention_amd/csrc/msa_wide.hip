@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kThreads) rows_copy_kernel(RowsArgs a, int dp)
       E8 l;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const Terms<float> t(x[e] * s);
+        const Terms<E> t(x[e] * s);
         h[e] = t.h;
         l[e] = t.l;
       }
@@ -345,7 +345,7 @@ hipError_t products(const WideProducts& p, hipStream_t s) {
   constexpr int P = Wide<T>::P;
   const bool dx = p.dx_part != nullptr, dw = p.dw[0] != nullptr;
   if (!dx && !dw) return hipSuccess;
-  ProductArgs a;
+  ProductArgs a = {};
   a.N = p.N; a.n_pad = p.n_pad; a.d = p.d; a.dp = p.dp; a.share = p.share;
   a.tm = (int)((p.dp + 255) / 256);
   a.dx_tiles = dx ? a.tm * (int)((p.n_pad + kTileN - 1) / kTileN) : 0;
@@ -357,24 +357,23 @@ hipError_t products(const WideProducts& p, hipStream_t s) {
   a.C = p.C;
   // (first, second) terms: low ones first
   int n = 0;
-  for (int t = P - 1; t >= 0; --t)
+  for (int t = p.g_terms - 1; t >= 0; --t) {
     for (int half = 0; half < p.halves; ++half) {
       const int64_t wh = half ? p.w[1] - p.w[0] : 0, gh = half * p.g_half;
-      if (t == 1) {
-        a.dx_segs.a[n] = wh; a.dx_segs.b[n++] = gh + p.g_plane;
-        a.dx_segs.a[n] = wh + p.w_plane; a.dx_segs.b[n++] = gh;
-      } else {
-        a.dx_segs.a[n] = wh; a.dx_segs.b[n++] = gh;
-      }
+      a.dx_segs.a[n] = wh; a.dx_segs.b[n++] = gh + t * p.g_plane;
+      if (t == 1 && P == 2) { a.dx_segs.a[n] = wh + p.w_plane; a.dx_segs.b[n++] = gh; }
     }
-  a.dx_segs.n = n; a.dx_segs.low = n - p.halves;
-  n = 0;
-  if (P == 2) {
-    a.dw_segs.a[n] = 0; a.dw_segs.b[n++] = p.g_plane;
-    a.dw_segs.a[n] = p.x_plane; a.dw_segs.b[n++] = 0;
+    if (t == 1) a.dx_segs.low = n;
   }
+  a.dx_segs.n = n;
+  n = 0;
+  if (p.g_terms == 2) {
+    a.dw_segs.a[n] = 0; a.dw_segs.b[n++] = p.g_plane;
+    if (P == 2) { a.dw_segs.a[n] = p.x_plane; a.dw_segs.b[n++] = 0; }
+  }
+  a.dw_segs.low = n;
   a.dw_segs.a[n] = 0; a.dw_segs.b[n++] = 0;
-  a.dw_segs.n = n; a.dw_segs.low = n - 1;
+  a.dw_segs.n = n;
   a.x = p.x; a.x_ld = p.x_ld; a.x_blk = p.x_blk; a.x_rows = p.x_rows;
   a.w = p.w[0]; a.w_ld = p.w_ld; a.w_blk = p.w_blk; a.w_rows = p.w_rows;
   a.g = p.g; a.g_half = p.g_half;
@@ -443,11 +442,11 @@ static int64_t two_kinds(int64_t n1, int64_t l1, int64_t n2, int64_t l2) {
   return t > end1 ? t : end1;
 }
 
-WideShare wide_share(int64_t N, int d, int64_t C, int halves, int planes, bool dx, bool dw) {
+WideShare wide_share(int64_t N, int d, int64_t C, int halves, int segs, bool dx, bool dw) {
   // What a block costs beside its stages, in stages of 0.7 us: 12 to fill and drain its pipeline, 5 to store a tile, and
   // where all CUs store fp32 tiles at once 20 more (64 MB at 4 TB/s); adding them up takes a launch, 8, and as much again.
   constexpr int64_t kFill = 12, kStore = 5, kFloat = 20, kLaunch = 8;
-  const int64_t tm = (wide_dp(d) + 255) / 256, segs = planes == 2 ? 3 : 1;
+  const int64_t tm = (wide_dp(d) + 255) / 256;
   const int64_t tx = dx ? tm * ((N + kTileN - 1) / kTileN) : 0, kx = C / 32 * segs * halves;
   const int64_t tw = dw ? tm * (C / kTileN) * halves : 0, kw = (N + 31) / 32 * segs;
   constexpr int kCuts[] = {1, 2, 3, 4, 5, 6, 8, 11, 16, 24, 32, 48, 64};
@@ -489,11 +488,11 @@ WideShare wide_share(int64_t N, int d, int64_t C, int halves, int planes, bool d
   return best;
 }
 
-int64_t wide_piece(int64_t N, int d, int64_t rows, int halves, int planes, bool dx, bool dw, int64_t bytes_of_column, WideShare* share) {
+int64_t wide_piece(int64_t N, int d, int64_t rows, int halves, int segs, bool dx, bool dw, int64_t bytes_of_column, WideShare* share) {
   // the sizes of the last call: a backward pass asks twice, for its workspace and for its launches
   struct Memo { int64_t key[8], C; WideShare share; };
   static thread_local Memo memo = {{-1}, 0, {}};
-  const int64_t key[8] = {N, d, rows, halves, planes, dx, dw, bytes_of_column};
+  const int64_t key[8] = {N, d, rows, halves, segs, dx, dw, bytes_of_column};
   if (memcmp(memo.key, key, sizeof(key)) == 0) {
     *share = memo.share;
     return memo.C;
@@ -505,7 +504,7 @@ int64_t wide_piece(int64_t N, int d, int64_t rows, int halves, int planes, bool 
     C = C < 256 ? 256 : C > all ? all : C;
     const int64_t pieces = (all + C - 1) / C;  // of equal size
     C = round_up((all + pieces - 1) / pieces, 256);
-    const WideShare w = wide_share(N, d, C, halves, planes, dx, dw);
+    const WideShare w = wide_share(N, d, C, halves, segs, dx, dw);
     if (cost < 0 || w.cost * pieces < cost) {
       cost = w.cost * pieces;
       chosen = C;

@@ -22,9 +22,12 @@ def product_slack(n, dtype):
     return n * U32 + (3 * 2.0 ** -22 if dtype == torch.float32 else 0.0)
 
 
-def gradient_unit(dtype):
-    """Relative rounding of the gradient that the backward products take: the operands' type, 22 bits for fp32."""
-    return 2.0 ** -22 if dtype == torch.float32 else u_of(dtype)
+def gradient_unit(dtype, rows):
+    """Relative rounding of the gradient that the backward products take: the operands' type, or two terms of it (fp32: of
+    fp16; the others: up to 256 rows)."""
+    if dtype == torch.float32:
+        return 2.0 ** -22
+    return u_of(dtype) ** 2 if rows <= 256 else u_of(dtype)
 
 
 def targets_of_labels(labels, ignore_index=-100):
@@ -49,7 +52,7 @@ def head(hidden, weight, ids, p, live, temperature, coef):
     X = torch.where(live[:, None], hidden.flatten(0, -2).double(), 0.0)
     W = weight.double()
     N, d = X.shape
-    u, ug = u_of(dtype), gradient_unit(dtype)
+    u, ug = u_of(dtype), gradient_unit(dtype, N)
     z = X @ W.T / temperature
     lse = torch.logsumexp(z, -1, keepdim=True)
     log_q = z - lse
@@ -95,7 +98,7 @@ def gated(x, wg, wu, activation, dh=None, spread=1.0):
     dtype = x.dtype
     X, G, U = x.flatten(0, -2).double(), wg.double(), wu.double()
     d = X.shape[1]
-    u_t, ug = u_of(dtype), gradient_unit(dtype)
+    u_t, ug = u_of(dtype), gradient_unit(dtype, X.shape[0])
     g, u = X @ G.T, X @ U.T
     slack = product_slack(d, dtype)
     g_off, u_off = slack * (X.abs() @ G.abs().T), slack * (X.abs() @ U.abs().T)
