@@ -169,6 +169,25 @@ def test_blocks_that_share_both_products(dtype, N):
         R.check(name, got[name], value, bound)
 
 
+def test_weights_past_32_bits():
+    # 4.4 GB of each weight, of its copy and of its gradient: the reference takes the features in parts
+    N, d, F = 4, 1040, 2 ** 21 + 77
+    x, wg, wu, dh = _data(N, d, F, torch.bfloat16, 10)
+    got = _run(x, wg, wu, dh, "silu")
+    value = bound = reach = 0.0
+    for at in range(0, F, 2 ** 18):
+        c = slice(at, at + 2 ** 18)
+        want = R.gated(x, wg[c], wu[c], "silu", dh[:, c])
+        R.check("h", got["h"][:, c], *want["h"])
+        R.check("dgate", got["dgate"][c], *want["dgate"])
+        R.check("dup", got["dup"][c], *want["dup"])
+        value, bound = value + want["dx"][0], bound + want["dx"][1]
+        # of the sums over all features: |dg| and |du| are at most 1.15 |dh| max|x| max|w|
+        top = 1.15 * float(x.double().norm(dim=1).amax()) * float(torch.cat([wg[c], wu[c]]).float().norm(dim=1).amax())
+        reach = reach + top * (dh[:, c].double().abs() @ (wg[c].double().abs() + wu[c].double().abs()))
+    R.check("dx", got["dx"], value, bound + R.product_slack(2 * F, torch.bfloat16) * reach)
+
+
 def test_equal_calls_streams_and_graph():
     x, wg, wu, dh = _data(500, 128, 700, torch.float16, 7)
     first = _run(x, wg, wu, dh, "silu")

@@ -394,6 +394,29 @@ def test_blocks_that_share_both_products(dtype, N, d, V, gone):
     _check_head(x, w, ids, p, live, 1.0, torch.full((N,), 1.0 / int(live.sum()), device=DEV).double(), loss, dx, dw, "mean")
 
 
+def test_rows_past_32_bits():
+    # 4.4 GB of rows, of their copies and of dx: the reference takes them in parts, whose bounds add up
+    N, d, V = 2 ** 21 + 77, 1040, 70
+    x, w, y, g = _data(N, d, V, torch.bfloat16, 18)
+    y[::5] = -100
+    x, w = _leaf(x, w)
+    loss = ops.linear_cross_entropy(x, w, y, reduction="none")
+    coef = torch.rand(N, device=DEV, generator=g)
+    dx, dw = _grads(loss, x, w, coef)
+    value = bound = 0.0
+    for at in range(0, N, 2 ** 18):
+        rows = slice(at, at + 2 ** 18)
+        ids, p, live = R.targets_of_labels(y[rows])
+        want = R.head(x.detach()[rows], w.detach(), ids, p, live, 1.0, coef[rows].double(), N)
+        R.check("loss", loss[rows], *want["loss"])
+        R.check("dhidden", dx[rows], *want["dhidden"])
+        value, bound = value + want["dweight"][0], bound + want["dweight"][1]
+    # fp32 sums over all rows, not over a part's
+    ids, p, live = R.targets_of_labels(y)
+    reach = sum(x.detach()[at: at + 2 ** 18].double().abs().sum(0) for at in range(0, N, 2 ** 18))
+    R.check("dweight", dw, value, bound + R.product_slack(N, torch.bfloat16) * reach)
+
+
 def test_autocast():
     x, w, y, _ = _data(100, 64, 300, torch.float32, 15)
     a, b = _leaf(x, w)

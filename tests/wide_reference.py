@@ -46,13 +46,14 @@ def targets_of_teacher(logits, ids, temperature):
     return torch.where(held, i, 0), p, live
 
 
-def head(hidden, weight, ids, p, live, temperature, coef):
-    """Loss per row and gradients for sum_n coef[n] loss[n], with bounds: {name: (value, bound)}."""
+def head(hidden, weight, ids, p, live, temperature, coef, rows=None):
+    """Loss per row and gradients for sum_n coef[n] loss[n], with bounds: {name: (value, bound)}.  rows: of the call that
+    these are a part of."""
     dtype = hidden.dtype
     X = torch.where(live[:, None], hidden.flatten(0, -2).double(), 0.0)
     W = weight.double()
     N, d = X.shape
-    u, ug = u_of(dtype), gradient_unit(dtype, N)
+    u, ug = u_of(dtype), gradient_unit(dtype, rows or N)
     z = X @ W.T / temperature
     lse = torch.logsumexp(z, -1, keepdim=True)
     log_q = z - lse
