@@ -7,6 +7,9 @@
 // K dot products.  Backward, in pieces of the vocabulary: the product again, now with lse2 known, gives the piece's
 // gradient G in the operand type (1 GB at most, or 256 columns); then dx += G W and dW = G^T x (msa_wide.hip).
 // Rows that do not count are taken out before the products: their x may hold anything.
+// Matrix units bound it, at the clock that the card's power allows: 8192 rows of 512 by 50257 bf16, a training pass 1780 us =
+// logits 400 to 480 (870 to 1020 TFLOP/s), G 580 to 605 (its 823 MB store beside the product), both products 970 to 1030
+// (820 to 870), all else 65.
 #include "msa_wide.h"
 
 namespace msa {
@@ -519,7 +522,8 @@ bool rows_vec(const HeadCall& c) {
   return c.d % per == 0 && c.x_ld % per == 0 && c.w_ld % per == 0 && (((uintptr_t)c.x | (uintptr_t)c.w) & 15) == 0;
 }
 
-// Scores of a few rows without a gradient: the rows are operands as they are, and none is taken out.
+// Scores of a few rows without a gradient: the rows are operands as they are, and none is taken out.  16 rows of 512 by 50257
+// bf16: 28.0 us with the plan and the copy, 21.6 without; from 1024 rows on products of rows that do not count cost more.
 constexpr int64_t kDirectRows = 1024;
 bool x_direct(const HeadCall& c) {
   return c.state == nullptr && c.teacher == nullptr && c.reduction == 0 && c.N <= kDirectRows && w_direct(c) &&
