@@ -523,8 +523,9 @@ bool rows_vec(const HeadCall& c) {
 }
 
 // Scores of a few rows without a gradient: the rows are operands as they are, and none is taken out.  16 rows of 512 by 50257
-// bf16: 28.0 us with the plan and the copy, 21.6 without; from 1024 rows on products of rows that do not count cost more.
-constexpr int64_t kDirectRows = 1024;
+// bf16: 28.0 us with the plan and the copy, 21.6 without.  But rows that do not count are then multiplied as well; us with /
+// without: 512 rows 49.6 / 43.2, of which 40% do not count 43.1 / 42.6; 1024 rows 76.5 / 70.6 and 53.5 / 69.3.
+constexpr int64_t kDirectRows = 512;
 bool x_direct(const HeadCall& c) {
   return c.state == nullptr && c.teacher == nullptr && c.reduction == 0 && c.N <= kDirectRows && w_direct(c) &&
          ((uintptr_t)c.x & 15) == 0 && c.x_ld % 8 == 0 && c.x_ld * 2 * 256 < ((int64_t)1 << 32);
