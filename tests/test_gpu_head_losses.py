@@ -369,6 +369,36 @@ def test_captured_forward_and_backward():
             assert torch.equal(p, q)
 
 
+def test_two_captured_calls_at_once():
+    sides, graphs, outs, wants = [torch.cuda.Stream() for _ in range(2)], [], [], []
+    kept = []  # a graph reads its inputs where they were: they have to live as long
+    for seed in range(2):
+        x, w, y, _ = _data(700, 64, 3000, torch.float32 if seed else torch.bfloat16, 30 + seed)
+        a, b = _leaf(x, w)
+
+        def body():
+            loss = ops.linear_cross_entropy(a, b, y)
+            return (loss.detach(), *_grads(loss, a, b))
+
+        wants.append(body())
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = body()
+        graphs.append(graph)
+        outs.append(out)
+        kept.append((a, b, y))
+    for _ in range(3):
+        for side, graph, out in zip(sides, graphs, outs):
+            with torch.cuda.stream(side):
+                for t in out:
+                    t.zero_()
+                graph.replay()
+        torch.cuda.synchronize()
+        for out, want in zip(outs, wants):
+            assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
 def test_pieces_of_the_vocabulary():
     # rows enough for several pieces (1 GB of 2 N bytes a column): 300000 rows take at most 1536 columns a piece
     N, d, V = 300000, 32, 2000
