@@ -395,8 +395,14 @@ int msa_verify(const msa_verify_args* args, void* stream);
  * msa_head_bwd takes the same arguments, state as msa_head_fwd left it (read
  * only) and dloss, fp32: (N) for reduction 0, one value else.  dhidden (N, d) and dweight (V, d) contiguous, of type dtype;
  * either may be null.  The gradient of the logits is formed in pieces of the
- * vocabulary, rounded to dtype (fp32: to two fp16 terms, 22 bits; the others up to
+ * vocabulary, rounded to dtype (fp32: to terms, below; the others up to
  * 256 rows: to two terms of their own) and multiplied with fp32 sums.
+ * fp32 is taken in terms that the matrix core multiplies.  Where the rows that count,
+ * the weight and the rows' coefficients are even (rows' largest entries within 2^10
+ * of each other, fewer entries below 2^-18 of their row's largest than a quarter of a
+ * column has; coefficients within 2^20): two fp16 terms, 22 bits, of G down to 2^-28
+ * of the largest coefficient.  Else three bf16 terms, 24 bits over fp32's range, in
+ * about twice the time.  The call finds out on the device.
  * state: msa_head_state_bytes, kept from forward to backward, or null for a forward
  * pass that no backward pass follows.  workspace: msa_head_workspace_bytes of the
  * same arguments (backward 0 or 1; of state only whether it is null; loss, dloss
@@ -442,8 +448,9 @@ int msa_head_bwd(const msa_head_args* args, void* stream);
  * msa_gated_bwd: dh (N, F), unit stride over F, dh_ld from row to row; dx (N, d),
  * dgate, dup (F, d) contiguous, of type dtype.  dx may be null, or dgate and dup
  * both.  The gradients of x Wg^T and x Wu^T are formed in pieces of the features,
- * rounded to dtype behind a power of two (two terms as in msa_head_bwd), sums are
- * fp32.
+ * rounded to dtype behind a power of two (terms as in msa_head_bwd; fp32 is even where
+ * x and the weights are and, backward, the largest entries of their rows and of dh's
+ * lie within 2^24 together), sums are fp32.
  * Operands are used in place under the conditions of msa_head_args' weight.
  * workspace: msa_gated_workspace_bytes of the same arguments.  1 <= d <= 65536, 1 <= F
  * <= 2^23, N <= 2^23, N d <= 2^38, F d <= 2^37, (N / 128) (F / 128) < 2^24.  Equal calls

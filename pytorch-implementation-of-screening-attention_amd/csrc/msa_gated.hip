@@ -48,9 +48,9 @@ struct GatedArgs {
   const char* x; int64_t x_ld, x_blk; int64_t N, n_pad;
   const char* w; int64_t w_ld, w_blk, up;  // the gate's first row of the piece; from there to the other weight's
   int cols;                         // features of the piece
-  MmSegs segs;
+  MmSegs segs[2];                   // of the narrow and the wide format
   int ksteps, tiles_f, tiles_n;
-  const WideHdr* hdr;
+  const WideMode* mode;
   void* h; int64_t h_ld; int vec;   // forward
   const void* dh; int64_t dh_ld;    // backward: the piece's first column
   char* g; int64_t plane, half;
@@ -63,12 +63,10 @@ template <typename E> using GatedHalf = MmTile<E, 128, 128, 2, 2, false, false, 
 template <typename E> using GatedFew = MmTile<E, 64, 32, 2, 1, false, false, true, 8>;
 constexpr int kFew = 32;
 
-template <typename T, int ACT, int TERMS, typename Tl>  // TERMS: of dg and du; 0: forward
-__global__ void __launch_bounds__(Tl::THREADS, Tl::TILE_M == 128 ? 3 : 2) gated_kernel(GatedArgs a) {
-  using E = typename Wide<T>::E;
+template <typename T, bool WIDE, int ACT, int TERMS, typename Tl>  // TERMS: of dg and du; 0: forward
+__device__ inline void gated_tile(const GatedArgs& a, LdsChar* lds) {
+  using E = typename Wide<T, WIDE>::E;
   constexpr int BF = Tl::TILE_M / 2, BN = Tl::TILE_N;
-  __shared__ char smem[Tl::LDS];
-  LdsChar* lds = (LdsChar*)smem;
   int tf, tn;
   patch_order(xcd_order(blockIdx.x, gridDim.x), a.tiles_f, a.tiles_n, 8, tf, tn);
   const int64_t n0 = (int64_t)tn * BN;
@@ -79,11 +77,11 @@ __global__ void __launch_bounds__(Tl::THREADS, Tl::TILE_M == 128 ? 3 : 2) gated_
   const int rows = (int)(a.N - n0 < BN ? a.N - n0 : BN);
   const typename Tl::Side A{a.w + f0 * a.w_ld, fleft, a.w_ld, a.w_blk, 0, a.up};
   const typename Tl::Side B{a.x + n0 * a.x_ld, rows, a.x_ld, a.x_blk, 0, 0};
-  Tl::run(acc, lds, A, B, a.segs, 0, a.ksteps);
+  Tl::run(acc, lds, A, B, a.segs[WIDE], 0, a.ksteps);
   float f1 = 1.0f, f2 = 1.0f;
-  if constexpr (Wide<T>::P == 2) {
-    f1 = 1.0f / scale_x<T>(a.hdr);
-    f2 = 1.0f / scale_w<T>(a.hdr);
+  if constexpr (__is_same(T, float)) {
+    f1 = 1.0f / scale_x<T>(a.mode);
+    f2 = 1.0f / scale_w<T>(a.mode);
   }
   if constexpr (TERMS == 0) {
     T* out = (T*)a.h + n0 * a.h_ld + f0;
@@ -92,7 +90,7 @@ __global__ void __launch_bounds__(Tl::THREADS, Tl::TILE_M == 128 ? 3 : 2) gated_
     });
   } else {
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
-    const float sg = scale_g<T>(a.hdr, 1);
+    const float sg = scale_g<T>(a.mode, 1);
     // dh goes through LDS in whole rows, 32 tokens of each wave at a time; places outside are zeros, so that dg and du
     // are zeros there.
     constexpr int PER = 16 / (int)sizeof(T), CPR = BF / PER, ROW = BF * (int)sizeof(T) + 16, NQ = 2 * Tl::MB;
@@ -117,7 +115,10 @@ __global__ void __launch_bounds__(Tl::THREADS, Tl::TILE_M == 128 ? 3 : 2) gated_
         *reinterpret_cast<LdsTV*>(lds + row * ROW + f * (int)sizeof(T)) = v;
       }
       Tl::sync_lds();
-      typename Quad<E>::V grads[2][TERMS][NQ];  // [dg, du][term], rounded as they are made
+      // dg and du: two terms at most as they are made; three would be more registers than the values themselves
+      constexpr bool SPLIT = TERMS < 3;
+      typename Quad<E>::V grads[2][SPLIT ? TERMS : 1][NQ];  // [dg, du][term]
+      f32x4 values[2][SPLIT ? 1 : NQ];
       const LdsChar* at = lds + (wn * 32 + (lane & 31)) * ROW + (wm * (BF / 2) + 4 * (lane >> 5)) * (int)sizeof(T);
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
@@ -132,12 +133,12 @@ __global__ void __launch_bounds__(Tl::THREADS, Tl::TILE_M == 128 ? 3 : 2) gated_
           const float v[2] = {ds * u * slope, ds * act};
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            if constexpr (TERMS == 2) {
-              const Terms<E> t(v[half]);
-              grads[half][0][q][e] = t.h;
-              grads[half][1][q][e] = t.l;
+            if constexpr (SPLIT) {
+              const Terms<E, TERMS> t(v[half]);
+#pragma unroll
+              for (int k = 0; k < TERMS; ++k) grads[half][k][q][e] = t.t[k];
             } else {
-              grads[half][0][q][e] = (E)v[half];
+              values[half][q][e] = v[half];
             }
           }
         }
@@ -147,10 +148,22 @@ __global__ void __launch_bounds__(Tl::THREADS, Tl::TILE_M == 128 ? 3 : 2) gated_
       for (int half = 0; half < 2; ++half)
 #pragma unroll
         for (int t = 0; t < TERMS; ++t)
-          Tl::template store_operand_tokens<Tl::MB / 2>(lds, reinterpret_cast<E*>(a.g + half * a.half + t * a.plane) + (f0 >> 5) * (a.n_pad * 32) + n0 * 32,
-                                                        a.n_pad * 32, j, [&](int i, int q) { return grads[half][t][4 * i + q]; });
+          Tl::template store_operand_tokens<Tl::MB / 2>(
+              lds, reinterpret_cast<E*>(a.g + half * a.half + t * a.plane) + (f0 >> 5) * (a.n_pad * 32) + n0 * 32, a.n_pad * 32, j, [&](int i, int q) {
+                if constexpr (SPLIT) return grads[half][t][4 * i + q];
+                else return quad<E>([&](int e) { return (float)Terms<E, TERMS>(values[half][4 * i + q][e]).t[t]; });
+              });
     }
   }
+}
+
+template <typename T, int ACT, int TERMS, template <typename> class Tile>
+__global__ void __launch_bounds__(Tile<T>::THREADS, Tile<T>::TILE_M == 128 ? 3 : 2) gated_kernel(GatedArgs a) {
+  __shared__ char smem[Tile<typename Wide<T>::E>::LDS];  // the sizes are the same in both formats
+  by_format<T>(a.mode, [&](auto wide) {
+    constexpr bool WIDE = decltype(wide)::value;
+    gated_tile<T, WIDE, ACT, (WIDE && TERMS > 0 ? 3 : TERMS), Tile<typename Wide<T, WIDE>::E>>(a, (LdsChar*)smem);
+  });
 }
 
 __global__ void zero_kernel(uint16_t* p, int64_t n) {
@@ -171,10 +184,11 @@ struct GatedPlan {
   WideShare share;
   char *x, *w, *g;
   float *dx_part, *dw_part;
-  WideHdr* hdr;
+  WideMode* mode;
+  WidePart* parts;
   size_t bytes;
   GatedPlan(const GatedCall& c, int backward) {
-    planes = c.dtype == 0 ? 2 : 1;
+    planes = planes_of(c.dtype);
     g_terms = terms_of_g(c.dtype, c.N);
     n_pad = round_up(c.N > 0 ? c.N : 1, 128);
     dp = wide_dp(c.d);
@@ -183,16 +197,18 @@ struct GatedPlan {
     char* p = (char*)c.workspace;
     size_t o = 0;
     auto take = [&](int64_t bytes) { char* q = p + o; o += (size_t)round_up(bytes, 256); return q; };
-    hdr = planes == 2 || (backward && c.dtype == 2) ? (WideHdr*)take(sizeof(WideHdr)) : nullptr;  // scales: not of bf16
+    const bool scales = c.dtype == 0 || (backward && c.dtype == 2);  // bf16 has none
+    mode = scales ? (WideMode*)take(sizeof(WideMode)) : nullptr;
+    parts = scales ? (WidePart*)take(kPartBytes) : nullptr;
     x = direct(c, c.x, c.x_ld) ? nullptr : take(planes * x_plane);
     w = direct(c, c.w[0], c.w_ld[0]) && direct(c, c.w[1], c.w_ld[1]) && c.w_ld[0] == c.w_ld[1] ? nullptr : take(2 * planes * w_plane);
     C = g_plane = 0;
     share = WideShare{};
     g = nullptr; dx_part = dw_part = nullptr;
     if (backward) {
-      C = wide_piece(c.N, c.d, c.F, 2, planes == 2 ? 3 : g_terms, c.dx != nullptr, c.dw[0] != nullptr, 2 * g_terms * 2 * n_pad, &share);
+      C = wide_piece(c.N, c.d, c.F, 2, c.dtype == 0 ? 3 : g_terms, c.dx != nullptr, c.dw[0] != nullptr, 2 * g_terms * 2 * n_pad, &share);
       g_plane = round_up(n_pad * C * 2, 256);
-      g = take(2 * g_terms * g_plane);
+      g = take(2 * g_planes(c.dtype, c.N) * g_plane);
       if (c.dx != nullptr) dx_part = (float*)take((int64_t)share.dx_split * n_pad * dp * 4);
       if (c.dw[0] != nullptr && share.dw_split > 1) dw_part = (float*)take((int64_t)share.dw_split * 2 * C * dp * 4);
     }
@@ -202,21 +218,20 @@ struct GatedPlan {
 
 #define GATED_TRY(call) do { const hipError_t e_ = (call); if (e_ != hipSuccess) return e_; } while (0)
 
-struct GatedOperands { const char *x, *w[2]; int64_t x_ld, x_blk, w_ld, w_blk; int x_rows; MmSegs segs; };
+struct GatedOperands { const char *x, *w[2]; int64_t x_ld, x_blk, w_ld, w_blk; int x_rows; MmSegs segs[2]; };
 
 hipError_t operands(const GatedCall& c, const GatedPlan& p, int backward, GatedOperands* o) {
   RowsCopies all = {}, copies = {};
   all.dtype = copies.dtype = c.dtype;
-  all.hdr = copies.hdr = p.hdr;
+  all.mode = copies.mode = p.mode;
   all.add(RowsCopy{c.x, c.x_ld, c.N, c.d, p.x, p.x_plane, p.n_pad * 64, nullptr, 0, backward});
   for (int i = 0; i < 2; ++i)
     all.add(RowsCopy{c.w[i], c.w_ld[i], c.F, c.d, p.w + (p.w == nullptr ? 0 : i * p.planes * p.w_plane), p.w_plane, c.F * (int64_t)64, nullptr, 1, backward});
   if (p.x != nullptr) copies.add(all.m[0]);
   if (p.w != nullptr) { copies.add(all.m[1]); copies.add(all.m[2]); }
-  if (p.planes == 2 || (backward && c.dtype == 2)) {  // scales of the operands, and of dg and du
+  if (p.mode != nullptr) {  // scales of the operands, and of dg and du
     if (backward) all.add(RowsCopy{c.dh, c.dh_ld, c.N, c.F, nullptr, 0, 0, nullptr, 2, 0});
-    GATED_TRY(launch_hdr_clear(p.hdr, c.stream));
-    GATED_TRY(launch_rows_max(all, c.stream));
+    GATED_TRY(launch_wide_mode(all, p.parts, p.mode, 1, c.stream));
   }
   if (copies.n > 0) GATED_TRY(launch_rows_copy(copies, c.stream));
   o->x = p.x != nullptr ? p.x : (const char*)c.x;
@@ -227,14 +242,14 @@ hipError_t operands(const GatedCall& c, const GatedPlan& p, int backward, GatedO
   o->w[1] = p.w != nullptr ? p.w + p.planes * p.w_plane : (const char*)c.w[1];
   o->w_ld = p.w != nullptr ? 64 : c.w_ld[0] * 2;
   o->w_blk = p.w != nullptr ? c.F * (int64_t)64 : 64;
-  o->segs = MmSegs{};
-  if (p.planes == 2) {
-    o->segs.b[0] = p.x_plane;
-    o->segs.a[1] = p.w_plane;
-    o->segs.n = 3;
-    o->segs.low = 2;
-  } else {
-    o->segs.n = 1;
+  o->segs[0] = o->segs[1] = MmSegs{};
+  o->segs[0].n = 1;
+  if (p.planes > 1) {
+    o->segs[0].b[0] = p.x_plane;
+    o->segs[0].a[1] = p.w_plane;
+    o->segs[0].n = 3;
+    o->segs[0].low = 2;
+    for (int order = 2; order >= 0; --order) add_wide_segs(o->segs[1], order, 0, p.w_plane, 0, p.x_plane);
   }
   return hipSuccess;
 }
@@ -243,8 +258,9 @@ GatedArgs args_of(const GatedCall& c, const GatedPlan& p, const GatedOperands& o
   GatedArgs a = {};
   a.x = o.x; a.x_ld = o.x_ld; a.x_blk = o.x_blk; a.N = c.N; a.n_pad = p.n_pad;
   a.w = o.w[0] + f0 * o.w_ld; a.w_ld = o.w_ld; a.w_blk = o.w_blk; a.up = o.w[1] - o.w[0]; a.cols = cols;
-  a.segs = o.segs; a.ksteps = (int)(p.dp / 32);
-  a.hdr = p.hdr;
+  for (int i = 0; i < 2; ++i) a.segs[i] = o.segs[i];
+  a.ksteps = (int)(p.dp / 32);
+  a.mode = p.mode;
   return a;
 }
 
@@ -253,7 +269,7 @@ hipError_t launch_tiles(GatedArgs a, int act, hipStream_t s) {
   using Tl = Tile<typename Wide<T>::E>;
   a.tiles_f = (a.cols + Tl::TILE_M / 2 - 1) / (Tl::TILE_M / 2);
   a.tiles_n = (int)((a.N + Tl::TILE_N - 1) / Tl::TILE_N);
-  auto* k = act == 0 ? gated_kernel<T, 0, TERMS, Tl> : gated_kernel<T, 1, TERMS, Tl>;
+  auto* k = act == 0 ? gated_kernel<T, 0, TERMS, Tile> : gated_kernel<T, 1, TERMS, Tile>;
   hipLaunchKernelGGL(k, dim3((unsigned)((int64_t)a.tiles_f * a.tiles_n)), dim3(Tl::THREADS), 0, s, a);
   return hipGetLastError();
 }
@@ -296,8 +312,8 @@ hipError_t gated_bwd(const GatedCall& c) {
     GatedArgs a = args_of(c, p, o, f0, cols);
     a.dh = (const T*)c.dh + f0; a.dh_ld = c.dh_ld;
     a.vec = c.dh_ld * sizeof(T) % 16 == 0 && ((uintptr_t)c.dh & 15) == 0;
-    a.g = p.g; a.plane = p.g_plane; a.half = p.g_terms * p.g_plane;
-    GATED_TRY((p.g_terms == 2 ? launch<T, 2>(a, c.act, c.stream) : launch<T, Wide<T>::P>(a, c.act, c.stream)));
+    a.g = p.g; a.plane = p.g_plane; a.half = g_planes(c.dtype, c.N) * p.g_plane;
+    GATED_TRY((p.g_terms == 2 ? launch<T, 2>(a, c.act, c.stream) : launch<T, __is_same(T, float) ? 2 : 1>(a, c.act, c.stream)));
     WideProducts q = {};
     q.dtype = c.dtype; q.gated = 1; q.N = c.N; q.n_pad = p.n_pad; q.d = c.d; q.dp = p.dp; q.halves = 2; q.cols = cols; q.C = p.C;
     q.x = o.x; q.x_ld = o.x_ld; q.x_blk = o.x_blk; q.x_plane = p.x_plane; q.x_rows = o.x_rows;
@@ -306,13 +322,13 @@ hipError_t gated_bwd(const GatedCall& c) {
       q.dw[i] = c.dw[i] == nullptr ? nullptr : (char*)c.dw[i] + f0 * c.d * es_of(c.dtype);
     }
     q.w_ld = o.w_ld; q.w_blk = o.w_blk; q.w_plane = p.w_plane; q.w_rows = (int)(c.F - f0);
-    q.g = p.g; q.g_plane = p.g_plane; q.g_half = p.g_terms * p.g_plane; q.g_terms = p.g_terms;
+    q.g = p.g; q.g_plane = p.g_plane; q.g_half = g_planes(c.dtype, c.N) * p.g_plane; q.g_terms = p.g_terms;
     q.dx_part = p.dx_part; q.dx_add = f0 > 0; q.dw_part = p.dw_part;
-    q.share = p.share; q.hdr = p.hdr; q.unit.mode = 3; q.use_live = 0;
+    q.share = p.share; q.mode = p.mode; q.unit.mode = 3; q.use_live = 0;
     GATED_TRY(launch_wide_products(q, c.stream));
   }
   if (c.dx != nullptr) {
-    const WideFinish f{c.dtype, 1, c.N, p.n_pad, c.d, p.dp, p.share.dx_split, p.dx_part, nullptr, p.hdr, GradUnit{nullptr, 1.0f, 3}, nullptr, c.dx};
+    const WideFinish f{c.dtype, 1, c.N, p.n_pad, c.d, p.dp, p.share.dx_split, p.dx_part, nullptr, p.mode, GradUnit{nullptr, 1.0f, 3}, nullptr, c.dx};
     GATED_TRY(launch_wide_finish(f, c.stream));
   }
   return hipSuccess;

@@ -19,18 +19,18 @@ constexpr int kThreads = 256;
 constexpr int kHeadMaxK = 256;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// What the backward pass needs: header, pos[N] (row of the operand, -1: does not count), lse2[N rows of the operand],
+// What the backward pass needs: mode, pos[N] (row of the operand, -1: does not count), lse2[N rows of the operand],
 // t[N][K]: 2^(z2 - lse2) - p of the targets (p summed over equal ids).
 struct HeadState {
-  WideHdr* hdr;
+  WideMode* mode;
   int* pos;
   float* lse2;
   float* t;
   size_t bytes;
   HeadState(void* p, int64_t N, int K) {
     char* c = (char*)p;
-    size_t o = (size_t)round_up(sizeof(WideHdr), 256);
-    hdr = (WideHdr*)c;
+    size_t o = (size_t)round_up(sizeof(WideMode), 256);
+    mode = (WideMode*)c;
     pos = (int*)(c + o); o += (size_t)round_up(N * 4, 256);
     lse2 = (float*)(c + o); o += (size_t)round_up(round_up(N, 128) * 4, 256);
     t = (float*)(c + o); o += (size_t)round_up(N * K * 4, 256);
@@ -88,10 +88,10 @@ __device__ inline int number_rows(int64_t N, int* pos, Fn counts) {
 }
 
 __global__ void __launch_bounds__(1024) plan_kernel(const int64_t* ids, int64_t ids_ld, int64_t ignore,
-                                                    const uint8_t* live, int64_t N, int* pos, WideHdr* hdr) {
+                                                    const uint8_t* live, int64_t N, int* pos, WideMode* mode) {
   const int total = live != nullptr ? number_rows(N, pos, [&](int64_t n) { return live[n] != 0; })
                                     : number_rows(N, pos, [&](int64_t n) { return ids[n * ids_ld] != ignore; });
-  for (int i = (int)threadIdx.x; i < kHdrWords; i += 1024) reinterpret_cast<uint32_t*>(hdr)[i] = i == 0 ? (uint32_t)total : 0u;
+  if (threadIdx.x == 0) *mode = WideMode{total, 0, 1.0f, 1.0f, 1.0f};
 }
 
 // A teacher's record of a row: entries with an id >= 0 and a logit above -inf; p = their softmax at 1/T.  A wave per
@@ -160,10 +160,10 @@ __global__ void __launch_bounds__(kThreads) teacher_kernel(const L* logits, int6
 struct StatsArgs {
   const char* x; int64_t x_ld, x_blk; int64_t rows;  // readable rows
   const char* w; int64_t w_ld, w_blk; int64_t V;
-  MmSegs segs;
+  MmSegs segs[2];                   // of the narrow and the wide format
   int ksteps, tiles_v, tiles_n;
   float to_log2;  // log2(e) / T
-  const WideHdr* hdr;
+  const WideMode* mode;             // null: the rows as they are
   float2* part; int64_t part_ld;  // [tiles_v][part_ld]
 };
 
@@ -187,15 +187,13 @@ template <typename E> using HeadTile = MmTile<E, 256, 128, 2, 2, false, false, f
 template <typename E> using HeadFew = MmTile<E, 64, 32, 2, 1, false, false, false, 8>;
 constexpr int kFew = 32;
 
-template <typename T, typename Tl>
-__global__ void __launch_bounds__(Tl::THREADS, 2) stats_kernel(StatsArgs a) {
+template <typename T, bool WIDE, typename Tl>
+__device__ inline void stats_tile(const StatsArgs& a, LdsChar* lds, float2 (*red)[Tl::TILE_N]) {
   constexpr int BM = Tl::TILE_M, BN = Tl::TILE_N, WM = Tl::WAVES_M;
-  __shared__ char smem[Tl::LDS];
-  LdsChar* lds = (LdsChar*)smem;
   int tv, tn;
   patch_order(xcd_order(blockIdx.x, gridDim.x), a.tiles_v, a.tiles_n, 8, tv, tn);
   const int64_t v0 = (int64_t)tv * BM, n0 = (int64_t)tn * BN;
-  const int64_t rows = a.hdr != nullptr ? a.hdr->live : a.rows;  // null: the rows as they are
+  const int64_t rows = a.mode != nullptr ? a.mode->live : a.rows;
   if (n0 >= rows) return;
   typename Tl::Acc acc;
   Tl::clear(acc);
@@ -203,11 +201,10 @@ __global__ void __launch_bounds__(Tl::THREADS, 2) stats_kernel(StatsArgs a) {
   const int readable = (int)(a.rows - n0 < BN ? a.rows - n0 : BN);
   const typename Tl::Side A{a.w + v0 * a.w_ld, vleft, a.w_ld, a.w_blk, 0, 0};
   const typename Tl::Side B{a.x + n0 * a.x_ld, readable, a.x_ld, a.x_blk, 0, 0};
-  Tl::run(acc, lds, A, B, a.segs, 0, a.ksteps);
+  Tl::run(acc, lds, A, B, a.segs[WIDE], 0, a.ksteps);
   float f = a.to_log2;
-  if constexpr (Wide<T>::P == 2) f = f / scale_x<T>(a.hdr) / scale_w<T>(a.hdr);
+  if constexpr (__is_same(T, float)) f = f / scale_x<T>(a.mode) / scale_w<T>(a.mode);
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave % WM, wn = wave / WM;
-  __shared__ float2 red[WM][BN];
   if (vleft < BM) mask_features<Tl>(acc, vleft, wm, lane, -INFINITY);
 #pragma unroll
   for (int j = 0; j < Tl::NB; ++j) {
@@ -234,6 +231,16 @@ __global__ void __launch_bounds__(Tl::THREADS, 2) stats_kernel(StatsArgs a) {
     a.part[(int64_t)tv * a.part_ld + n0 + threadIdx.x] =
         float2{m, p.y * __builtin_amdgcn_exp2f(p.x - at) + q.y * __builtin_amdgcn_exp2f(q.x - at)};
   }
+}
+
+template <typename T, template <typename> class Tile>
+__global__ void __launch_bounds__(Tile<T>::THREADS, 2) stats_kernel(StatsArgs a) {
+  using Any = Tile<typename Wide<T>::E>;  // the sizes are the same in both formats
+  __shared__ char smem[Any::LDS];
+  __shared__ float2 red[Any::WAVES_M][Any::TILE_N];
+  by_format<T>(a.mode, [&](auto wide) {
+    stats_tile<T, decltype(wide)::value, Tile<typename Wide<T, decltype(wide)::value>::E>>(a, (LdsChar*)smem, red);
+  });
 }
 
 // ---------------------------------------------------------------------------
@@ -374,7 +381,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
 
 // One block: the mean or the sum of the rows' losses, in 64 bits.  (The last block of rows_kernel could do it; but making
 // each block's rows visible to it writes back its L2: 160 -> 390 us for 8192 rows of 64 targets.)
-__global__ void __launch_bounds__(1024) total_kernel(const float* rows, int64_t N, const WideHdr* hdr, int mean, float* out) {
+__global__ void __launch_bounds__(1024) total_kernel(const float* rows, int64_t N, const WideMode* mode, int mean, float* out) {
   __shared__ double sums[16];
   double s = 0.0;
 #pragma unroll 4
@@ -385,7 +392,7 @@ __global__ void __launch_bounds__(1024) total_kernel(const float* rows, int64_t 
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 16; ++w) s += sums[w];
-    out[0] = (float)(mean ? s / (double)hdr->live : s);
+    out[0] = (float)(mean ? s / (double)mode->live : s);
   }
 }
 
@@ -394,24 +401,37 @@ __global__ void __launch_bounds__(1024) total_kernel(const float* rows, int64_t 
 // ---------------------------------------------------------------------------
 // Coefficients of the rows of the operand where each row's loss has a gradient of its own, as g_n / cmax with a power of
 // two cmax, at least the largest finite |g_n|; zero behind the last row up to the next multiple of 128.  One block.  (A mean
-// or a sum has one coefficient for all: G is formed for 1 and so rounded from the probabilities themselves.)
+// or a sum has one coefficient for all: G is formed for 1 and so rounded from the probabilities themselves.)  fp32: rows of G
+// are as uneven as the coefficients, and past 2^kEvenCoef the pass takes the wide format, whichever the forward pass took.
+constexpr int kEvenCoef = 20;
 __global__ void __launch_bounds__(1024) coef_kernel(const float* dloss, float factor, int64_t N, int64_t n_pad, const int* pos,
-                                                    const WideHdr* hdr, float* cmax, float* coef) {
+                                                    const WideMode* fwd, WideMode* mode, float* cmax, float* coef) {
   const int tid = (int)threadIdx.x;
-  const int live = hdr->live;
-  __shared__ float red[16];
-  float mx = 0.0f;
+  const int live = fwd->live;
+  __shared__ float red[16], least[16];
+  float mx = 0.0f, mn = INFINITY;
   for (int64_t n = tid; n < N; n += 1024) {
     const float g = pos[n] >= 0 ? fabsf(dloss[n] * factor) : 0.0f;
     if (g < INFINITY) mx = fmaxf(mx, g);
+    if (g > 0.0f) mn = fminf(mn, g);
   }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-  if ((tid & 63) == 0) red[tid >> 6] = mx;
+  for (int o = 32; o > 0; o >>= 1) {
+    mx = fmaxf(mx, __shfl_xor(mx, o));
+    mn = fminf(mn, __shfl_xor(mn, o));
+  }
+  if ((tid & 63) == 0) { red[tid >> 6] = mx; least[tid >> 6] = mn; }
   __syncthreads();
-  for (int w = 0; w < 16; ++w) mx = fmaxf(mx, red[w]);
+  for (int w = 0; w < 16; ++w) {
+    mx = fmaxf(mx, red[w]);
+    mn = fminf(mn, least[w]);
+  }
   const float inv = pow2_to(mx, 0);  // mx inv in [0.5, 1)
-  if (tid == 0) *cmax = 1.0f / inv;
+  if (tid == 0) {
+    *cmax = 1.0f / inv;
+    const bool wide = fwd->wide || mn < mx * (1.0f / (1 << kEvenCoef));
+    *mode = WideMode{live, wide ? 1 : 0, wide ? 1.0f : fwd->sx, wide ? 1.0f : fwd->sw, wide ? 1.0f : fwd->sg};
+  }
   for (int64_t n = tid; n < N; n += 1024)
     if (pos[n] >= 0) coef[pos[n]] = dloss[n] * factor * inv;
   for (int64_t i = live + tid; i < n_pad; i += 1024) coef[i] = 0.0f;
@@ -421,25 +441,23 @@ struct GradArgs {
   const char* x; int64_t n_pad;
   const char* w; int64_t w_ld, w_blk;  // the piece's first row
   int cols;                     // its rows
-  MmSegs segs;
+  MmSegs segs[2];               // of the narrow and the wide format
   int ksteps, tiles_v, tiles_n;
   float to_log2;
-  const WideHdr* hdr;
+  const WideMode* mode;
   const float* lse2; const float* coef;
   char* g; int64_t plane;
 };
 
 // G of one tile: c_n 2^(z2 - lse2), without the targets, which scatter_kernel puts in their place.
-template <typename T, int TERMS>
-__global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
-  using E = typename Wide<T>::E;
-  using Tl = MmTile<E, 256, 128, 2, 2, false, false, false, 3>;
-  __shared__ char smem[Tl::LDS];
-  LdsChar* lds = (LdsChar*)smem;
+template <typename T, bool WIDE, int TERMS>
+__device__ inline void grad_tile(const GradArgs& a, LdsChar* lds) {
+  using E = typename Wide<T, WIDE>::E;
+  using Tl = HeadTile<E>;
   int tv, tn;
   patch_order(xcd_order(blockIdx.x, gridDim.x), a.tiles_v, a.tiles_n, 8, tv, tn);
   const int64_t v0 = (int64_t)tv * 256, n0 = (int64_t)tn * 128;
-  const int64_t live = a.hdr->live;
+  const int64_t live = a.mode->live;
   if (n0 >= live) return;
   typename Tl::Acc acc;
   Tl::clear(acc);
@@ -448,8 +466,8 @@ __global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
   E* out = reinterpret_cast<E*>(a.g) + (v0 >> 5) * blk + n0 * 32;
   const typename Tl::Side A{a.w + v0 * a.w_ld, vleft, a.w_ld, a.w_blk, 0, 0};
   const typename Tl::Side B{a.x + n0 * 64, (int)(a.n_pad - n0 < 128 ? a.n_pad - n0 : 128), 64, a.n_pad * 64, 0, 0};
-  Tl::run(acc, lds, A, B, a.segs, 0, a.ksteps);
-  const float f = a.to_log2 / scale_x<T>(a.hdr) / scale_w<T>(a.hdr), lg = __is_same(T, bf16) ? 0.0f : 15.0f;  // log2 of scale_g
+  Tl::run(acc, lds, A, B, a.segs[WIDE], 0, a.ksteps);
+  const float f = a.to_log2 / scale_x<T>(a.mode) / scale_w<T>(a.mode), lg = __is_same(E, bf16) ? 0.0f : 15.0f;  // log2 of scale_g
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
   if (vleft < 256) mask_features<Tl>(acc, vleft, wm, lane, -INFINITY);
 #pragma unroll
@@ -471,39 +489,50 @@ __global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
         for (int r = 0; r < 16; ++r) acc[i][j][r] *= c;
     }
   }
-  if constexpr (TERMS == 2) {
-    Tl::store_operand(lds, out, blk, [&](int i, int j, int g) {
-      return quad<E>([&](int e) { return (float)Terms<E>(acc[i][j][4 * g + e]).h; });
-    });
-    Tl::renew(acc);
-    Tl::store_operand(lds, reinterpret_cast<E*>(reinterpret_cast<char*>(out) + a.plane), blk,
-                                      [&](int i, int j, int g) {
-                                        return quad<E>([&](int e) { return (float)Terms<E>(acc[i][j][4 * g + e]).l; });
-                                      });
-  } else {
-    Tl::store_operand(lds, out, blk, [&](int i, int j, int g) {
-      return quad<E>([&](int e) { return acc[i][j][4 * g + e]; });
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) {
+    if (t > 0) Tl::renew(acc);
+    Tl::store_operand(lds, reinterpret_cast<E*>(reinterpret_cast<char*>(out) + t * a.plane), blk, [&](int i, int j, int g) {
+      return quad<E>([&](int e) { return (float)Terms<E, TERMS>(acc[i][j][4 * g + e]).t[t]; });
     });
   }
+}
+
+template <typename T, int TERMS>
+__global__ void __launch_bounds__(kThreads, 2) grad_kernel(GradArgs a) {
+  __shared__ char smem[HeadTile<typename Wide<T>::E>::LDS];
+  by_format<T>(a.mode, [&](auto wide) {
+    constexpr bool WIDE = decltype(wide)::value;
+    grad_tile<T, WIDE, WIDE ? Wide<T, WIDE>::P : TERMS>(a, (LdsChar*)smem);
+  });
 }
 
 // The targets' entries of a piece's G.  Entries of equal ids write equal values.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) scatter_kernel(const int64_t* ids, int64_t ids_ld, int64_t N, int K, const int* pos,
-                                                           const float* t, const float* coef, const WideHdr* hdr, int64_t v0,
+                                                           const float* t, const float* coef, const WideMode* mode, int64_t v0,
                                                            int cols, char* g, int64_t n_pad, int64_t plane, int terms) {
-  using E = typename Wide<T>::E;
   const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   const int64_t n = e / K;
   if (n >= N) return;
   const int at = pos[n];
   const int64_t v = ids[n * ids_ld + (e - n * K)] - v0;
   if (at < 0 || v < 0 || v >= cols) return;
-  const float x = (coef != nullptr ? t[e] * coef[at] : t[e]) * scale_g<T>(hdr, 0);
-  E* p = reinterpret_cast<E*>(g) + (v >> 5) * (n_pad * 32) + (int64_t)at * 32 + (v & 31);
-  const Terms<E> w(x);
-  *p = w.h;
-  if (terms == 2) *reinterpret_cast<E*>(reinterpret_cast<char*>(p) + plane) = w.l;
+  const float x = (coef != nullptr ? t[e] * coef[at] : t[e]) * scale_g<T>(mode, 0);
+  char* const p = g + ((v >> 5) * (n_pad * 32) + (int64_t)at * 32 + (v & 31)) * 2;
+  by_format<T>(mode, [&](auto wide) {
+    constexpr bool WIDE = decltype(wide)::value;
+    using E = typename Wide<T, WIDE>::E;
+    if constexpr (WIDE) {
+      const Terms<E, 3> w(x);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<E*>(p + k * plane) = w.t[k];
+    } else {
+      const Terms<E, 2> w(x);
+      *reinterpret_cast<E*>(p) = w.t[0];
+      if (terms == 2) *reinterpret_cast<E*>(p + plane) = w.t[1];
+    }
+  });
 }
 
 __global__ void zero_kernel(uint16_t* p, int64_t n) {
@@ -536,14 +565,16 @@ struct HeadPlan {
   int planes, g_terms, tiles_n, tiles_v;
   WideShare share;
   bool distill, few, direct;  // direct: x is used as it is
+  WideMode* mode;             // backward, a coefficient a row: the format that they need
   char *x, *w, *g, *state = nullptr;
   float2 *part, *tp;
+  WidePart* parts;
   float *ent, *rows, *coef, *cmax, *dx_part, *dw_part;
   uint8_t* live;
   size_t bytes;
   HeadPlan(const HeadCall& c, int backward) {
     distill = c.teacher != nullptr;
-    planes = c.dtype == 0 ? 2 : 1;
+    planes = planes_of(c.dtype);
     g_terms = terms_of_g(c.dtype, c.N);
     n_pad = round_up(c.N > 0 ? c.N : 1, 128);
     dp = wide_dp(c.d);
@@ -560,10 +591,11 @@ struct HeadPlan {
     w = w_direct(c) ? nullptr : take(planes * w_plane);
     C = g_plane = 0;
     share = WideShare{};
-    part = tp = nullptr; ent = rows = coef = cmax = dx_part = dw_part = nullptr; live = nullptr; g = nullptr;
+    mode = nullptr; parts = nullptr; part = tp = nullptr; ent = rows = coef = cmax = dx_part = dw_part = nullptr; live = nullptr; g = nullptr;
     if (!backward) {
       part = (float2*)take((int64_t)tiles_v * n_pad * 8);
       state = c.state == nullptr && !direct ? take((int64_t)HeadState(nullptr, c.N, c.K).bytes) : (char*)c.state;
+      if (c.dtype == 0) parts = (WidePart*)take(kPartBytes);
       if (c.reduction != 0) rows = (float*)take(c.N * 4);
       if (distill) {
         tp = (float2*)take(c.N * c.K * 8);
@@ -571,42 +603,42 @@ struct HeadPlan {
         live = (uint8_t*)take(c.N);
       }
     } else {
-      C = wide_piece(c.N, c.d, c.V, 1, planes == 2 ? 3 : g_terms, c.dx != nullptr, c.dw != nullptr, g_terms * 2 * n_pad, &share);
+      C = wide_piece(c.N, c.d, c.V, 1, c.dtype == 0 ? 3 : g_terms, c.dx != nullptr, c.dw != nullptr, g_terms * 2 * n_pad, &share);
       g_plane = round_up(n_pad * C * 2, 256);
-      g = take(g_terms * g_plane);
+      g = take(g_planes(c.dtype, c.N) * g_plane);
       if (c.reduction == 0) {
         coef = (float*)take(n_pad * 4);
         cmax = (float*)take(4);
+        mode = (WideMode*)take(sizeof(WideMode));
       }
       if (c.dx != nullptr) dx_part = (float*)take((int64_t)share.dx_split * n_pad * dp * 4);
       if (c.dw != nullptr && share.dw_split > 1) dw_part = (float*)take((int64_t)share.dw_split * C * dp * 4);
     }
     bytes = o;
   }
-  MmSegs logits() const {
-    MmSegs s = {};
-    if (planes == 2) {
-      s.b[0] = x_plane;
-      s.a[1] = w_plane;
-      s.n = 3;
-      s.low = 2;
-    } else {
-      s.n = 1;
+  void logits(MmSegs (&s)[2]) const {
+    s[0] = s[1] = MmSegs{};
+    s[0].n = 1;
+    if (planes > 1) {
+      s[0].b[0] = x_plane;
+      s[0].a[1] = w_plane;
+      s[0].n = 3;
+      s[0].low = 2;
+      for (int order = 2; order >= 0; --order) add_wide_segs(s[1], order, 0, w_plane, 0, x_plane);
     }
-    return s;
   }
 };
 
 #define HEAD_TRY(call) do { const hipError_t e_ = (call); if (e_ != hipSuccess) return e_; } while (0)
 
-// hidden's counting rows and the weight as operands; the forward pass finds fp32's scales for both passes
-hipError_t operands(const HeadCall& c, const HeadPlan& p, const HeadState& st, bool find) {
+// hidden's counting rows and the weight as operands; the forward pass finds fp32's scales and format for both passes
+hipError_t operands(const HeadCall& c, const HeadPlan& p, const HeadState& st, const WideMode* mode, bool find) {
   RowsCopies all = {};
   all.dtype = c.dtype;
-  all.hdr = st.hdr;
+  all.mode = mode;
   all.add(RowsCopy{c.x, c.x_ld, c.N, c.d, p.x, p.x_plane, p.n_pad * 64, st.pos, 0, 0});
   if (p.w != nullptr) all.add(RowsCopy{c.w, c.w_ld, c.V, c.d, p.w, p.w_plane, c.V * 64, nullptr, 1, 0});
-  if (p.planes == 2 && find) HEAD_TRY(launch_rows_max(all, c.stream));
+  if (c.dtype == 0 && find) HEAD_TRY(launch_wide_mode(all, p.parts, st.mode, 0, c.stream));
   return launch_rows_copy(all, c.stream);
 }
 
@@ -627,20 +659,20 @@ hipError_t head_fwd(const HeadCall& c) {
   }
   const bool direct = p.direct;
   if (!direct) {
-    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, c.stream, c.ids, c.ids_ld, c.ignore_index, p.live, c.N, st.pos, st.hdr);
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, c.stream, c.ids, c.ids_ld, c.ignore_index, p.live, c.N, st.pos, st.mode);
     HEAD_TRY(hipGetLastError());
   }
   if (c.N > 0) {
-    if (!direct) HEAD_TRY(operands(c, p, st, true));
+    if (!direct) HEAD_TRY(operands(c, p, st, st.mode, true));
     StatsArgs a;
     a.x = direct ? (const char*)c.x : p.x; a.x_ld = direct ? c.x_ld * 2 : 64; a.x_blk = direct ? 64 : p.n_pad * 64; a.rows = direct ? c.N : p.n_pad;
     a.w = p.w != nullptr ? p.w : (const char*)c.w; a.w_ld = p.w != nullptr ? 64 : c.w_ld * 2; a.w_blk = p.w != nullptr ? c.V * 64 : 64; a.V = c.V;
-    a.segs = p.logits(); a.ksteps = (int)(p.dp / 32); a.tiles_v = p.tiles_v; a.tiles_n = p.few ? 1 : p.tiles_n;
-    a.to_log2 = kLog2e / c.temperature; a.hdr = direct ? nullptr : st.hdr; a.part = p.part; a.part_ld = p.n_pad;
+    p.logits(a.segs); a.ksteps = (int)(p.dp / 32); a.tiles_v = p.tiles_v; a.tiles_n = p.few ? 1 : p.tiles_n;
+    a.to_log2 = kLog2e / c.temperature; a.mode = direct ? nullptr : st.mode; a.part = p.part; a.part_ld = p.n_pad;
     using E = typename Wide<T>::E;
     const unsigned blocks = (unsigned)((int64_t)a.tiles_v * a.tiles_n);
-    if (p.few) hipLaunchKernelGGL((stats_kernel<T, HeadFew<E>>), dim3(blocks), dim3(HeadFew<E>::THREADS), 0, c.stream, a);
-    else hipLaunchKernelGGL((stats_kernel<T, HeadTile<E>>), dim3(blocks), dim3(HeadTile<E>::THREADS), 0, c.stream, a);
+    if (p.few) hipLaunchKernelGGL((stats_kernel<T, HeadFew>), dim3(blocks), dim3(HeadFew<E>::THREADS), 0, c.stream, a);
+    else hipLaunchKernelGGL((stats_kernel<T, HeadTile>), dim3(blocks), dim3(HeadTile<E>::THREADS), 0, c.stream, a);
     HEAD_TRY(hipGetLastError());
     RowsArgs r;
     r.x = c.x; r.x_ld = c.x_ld; r.w = c.w; r.w_ld = c.w_ld; r.ids = c.ids; r.ids_ld = c.ids_ld; r.tp = p.tp; r.ent = p.ent;
@@ -652,7 +684,7 @@ hipError_t head_fwd(const HeadCall& c) {
     HEAD_TRY(hipGetLastError());
   }
   if (c.reduction != 0) {
-    hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, c.stream, p.rows, c.N, st.hdr, c.reduction == 1, c.loss);
+    hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, c.stream, p.rows, c.N, st.mode, c.reduction == 1, c.loss);
     HEAD_TRY(hipGetLastError());
   }
   return hipSuccess;
@@ -669,24 +701,25 @@ hipError_t head_bwd(const HeadCall& c) {
   }
   const float factor = p.distill ? c.temperature : 1.0f;  // T^2 of the loss, 1/T of z
   const GradUnit unit{c.dloss, factor, c.reduction};
+  const WideMode* const mode = c.reduction == 0 ? p.mode : st.mode;
   if (c.reduction == 0) {
-    hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, c.stream, c.dloss, factor, c.N, p.n_pad, st.pos, st.hdr, p.cmax, p.coef);
+    hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, c.stream, c.dloss, factor, c.N, p.n_pad, st.pos, st.mode, p.mode, p.cmax, p.coef);
     HEAD_TRY(hipGetLastError());
   }
-  HEAD_TRY(operands(c, p, st, false));
+  HEAD_TRY(operands(c, p, st, mode, false));
   const char* w = p.w != nullptr ? p.w : (const char*)c.w;
   const int64_t w_ld = p.w != nullptr ? 64 : c.w_ld * 2, w_blk = p.w != nullptr ? c.V * 64 : 64;
   for (int64_t v0 = 0; v0 < c.V; v0 += p.C) {
     const int cols = (int)(c.V - v0 < p.C ? c.V - v0 : p.C);
     GradArgs a;
     a.x = p.x; a.n_pad = p.n_pad; a.w = w + v0 * w_ld; a.w_ld = w_ld; a.w_blk = w_blk; a.cols = cols;
-    a.segs = p.logits(); a.ksteps = (int)(p.dp / 32); a.tiles_v = (int)(round_up(cols, 256) / 256); a.tiles_n = p.tiles_n;
-    a.to_log2 = kLog2e / c.temperature; a.hdr = st.hdr; a.lse2 = st.lse2; a.coef = p.coef; a.g = p.g; a.plane = p.g_plane;
-    auto* grad = p.g_terms == 2 ? grad_kernel<T, 2> : grad_kernel<T, Wide<T>::P>;
+    p.logits(a.segs); a.ksteps = (int)(p.dp / 32); a.tiles_v = (int)(round_up(cols, 256) / 256); a.tiles_n = p.tiles_n;
+    a.to_log2 = kLog2e / c.temperature; a.mode = mode; a.lse2 = st.lse2; a.coef = p.coef; a.g = p.g; a.plane = p.g_plane;
+    auto* grad = p.g_terms == 2 ? grad_kernel<T, 2> : grad_kernel<T, __is_same(T, float) ? 2 : 1>;
     hipLaunchKernelGGL(grad, dim3((unsigned)((int64_t)a.tiles_v * a.tiles_n)), dim3(kThreads), 0, c.stream, a);
     HEAD_TRY(hipGetLastError());
     hipLaunchKernelGGL(scatter_kernel<T>, dim3((unsigned)((c.N * c.K + kThreads - 1) / kThreads)), dim3(kThreads), 0, c.stream,
-                       c.ids, c.ids_ld, c.N, c.K, st.pos, st.t, p.coef, st.hdr, v0, cols, p.g, p.n_pad, p.g_plane, p.g_terms);
+                       c.ids, c.ids_ld, c.N, c.K, st.pos, st.t, p.coef, mode, v0, cols, p.g, p.n_pad, p.g_plane, p.g_terms);
     HEAD_TRY(hipGetLastError());
     WideProducts q = {};
     q.dtype = c.dtype; q.gated = 0; q.N = c.N; q.n_pad = p.n_pad; q.d = c.d; q.dp = p.dp; q.halves = 1; q.cols = cols;
@@ -696,11 +729,11 @@ hipError_t head_bwd(const HeadCall& c) {
     q.g = p.g; q.g_plane = p.g_plane; q.g_half = 0; q.g_terms = p.g_terms;
     q.dx_part = p.dx_part; q.dx_add = v0 > 0;
     q.dw[0] = c.dw == nullptr ? nullptr : (char*)c.dw + v0 * c.d * es_of(c.dtype); q.dw_part = p.dw_part;
-    q.share = p.share; q.hdr = st.hdr; q.unit = unit; q.cmax = p.cmax; q.use_live = 1;
+    q.share = p.share; q.mode = mode; q.unit = unit; q.cmax = p.cmax; q.use_live = 1;
     HEAD_TRY(launch_wide_products(q, c.stream));
   }
   if (c.dx != nullptr) {
-    const WideFinish f{c.dtype, 0, c.N, p.n_pad, c.d, p.dp, p.share.dx_split, p.dx_part, st.pos, st.hdr, unit, p.cmax, c.dx};
+    const WideFinish f{c.dtype, 0, c.N, p.n_pad, c.d, p.dp, p.share.dx_split, p.dx_part, st.pos, mode, unit, p.cmax, c.dx};
     HEAD_TRY(launch_wide_finish(f, c.stream));
   }
   return hipSuccess;

@@ -15,10 +15,11 @@
 namespace msa {
 
 constexpr int kMmK = 32;      // k of a stage
-constexpr int kMmSegs = 6;    // products that one tile adds up
+constexpr int kMmSegs = 12;   // products that one tile adds up
 
 // A sum over up to kMmSegs operand pairs of the same shape (byte offsets to A and B).  fp32 operands enter as two
-// fp16 terms, x s = h + 2^-11 l with a power of two s: three products h l + l h, then 2^-11 of their sum, then h h.
+// fp16 terms, x s = h + 2^-11 l with a power of two s: three products h l + l h, then 2^-11 of their sum, then h h; or as
+// three bf16 terms, x = h + m + l: h l + l h + m m, then h m + m h, then h h (what is left out is 2^-26 of x).
 struct MmSegs {
   int64_t a[kMmSegs], b[kMmSegs];
   int n, low;  // products; the first `low` are of order 2^-11 (0: none)

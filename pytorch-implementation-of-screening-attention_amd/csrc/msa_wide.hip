@@ -13,10 +13,6 @@ constexpr int kThreads = 256;
 // pass, 128 / 256: 8192 x 50257 x 512 bf16 1855 / 1805, 32768 rows 7640 / 7270, 2867 fp32 rows 2500 / 2260.
 constexpr int kTileN = 256, kProductThreads = 512;
 
-__global__ void hdr_clear_kernel(WideHdr* h) {
-  for (int i = (int)threadIdx.x; i < kHdrWords; i += kThreads) reinterpret_cast<uint32_t*>(h)[i] = 0u;
-}
-
 // 8 neighbours of a row, zeros past its end.
 template <typename T>
 __device__ inline void load8(const T* in, int c, int d, bool vec, T (&x)[8]) {
@@ -42,7 +38,7 @@ struct RowsArgs {
   RowsCopy m[kCopies];
   int64_t first[kCopies + 1];  // blocks of each matrix
   int vec[kCopies];
-  WideHdr* hdr;
+  const WideMode* mode;
 };
 __device__ inline int matrix_of(const RowsArgs& a, int64_t block) {
   int i = 0;
@@ -51,58 +47,160 @@ __device__ inline int matrix_of(const RowsArgs& a, int64_t block) {
   return i;
 }
 
-// A wave takes rows in turn, of the matrix that its block belongs to.
+// Below 2^-digits of its row's largest entry an entry is small (fp32): with rows' largest entries within 2^kEven of each other
+// the rest keep their 22 bits in the narrow format.  dh is no operand, but rows and columns of G are as uneven as its own, and G
+// keeps as many bits: G has the digits, and dh's share of kEvenG, to itself.
+constexpr int kDigits = 18, kDigitsDh = 24, kEven = 10, kEvenG = 24;
+
+// A wave takes rows in turn, of the matrix that its block belongs to.  Which entries of fp32 rows are small is seen once the
+// largest is known: rows of up to 2048 are still in registers then, longer ones in the cache.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) rows_max_kernel(RowsArgs a) {
+__global__ void __launch_bounds__(kThreads) rows_max_kernel(RowsArgs a, WidePart* parts) {
+  constexpr bool EVEN = __is_same(T, float);
+  constexpr int HELD = EVEN ? 4 : 1;
   const int i = matrix_of(a, blockIdx.x), lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   const RowsCopy m = a.m[i];
   const int64_t step = (a.first[i + 1] - a.first[i]) * 4;
+  const float digits = m.slot == 2 ? 1.0f / (1 << kDigitsDh) : 1.0f / (1 << kDigits);
   float mx = 0.0f, nx = 0.0f;
+  int low = 0, small = 0;
   for (int64_t r = ((int64_t)blockIdx.x - a.first[i]) * 4 + wave; r < m.rows; r += step) {
     if (m.pos != nullptr && m.pos[r] < 0) continue;
     const T* p = (const T*)m.src + r * m.ld;
     float ss = 0.0f, rx = 0.0f;
-    for (int c = lane * 8; c < m.d; c += 512) {
-      T x[8];
-      load8(p, c, m.d, a.vec[i] != 0, x);
+    T x[HELD][8];
+    auto load = [&](int c0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = fabsf(to_f(x[e]));
-        if (v < INFINITY) {
-          rx = fmaxf(rx, v);
-          ss = fmaf(v, v, ss);
+      for (int q = 0; q < HELD; ++q) {
+        const int c = c0 + q * 512 + lane * 8;
+        if (c0 + q * 512 >= m.d) break;
+        if (c < m.d) {
+          load8(p, c, m.d, a.vec[i] != 0, x[q]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[q][e] = (T)0.0f;
+        }
+      }
+    };
+    for (int c0 = 0; c0 < m.d; c0 += HELD * 512) {
+      load(c0);
+#pragma unroll
+      for (int q = 0; q < HELD; ++q) {
+        if (c0 + q * 512 >= m.d) break;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = fabsf(to_f(x[q][e]));
+          if (v < INFINITY) {
+            rx = fmaxf(rx, v);
+            ss = fmaf(v, v, ss);
+          }
         }
       }
     }
     mx = fmaxf(mx, rx);
+    if (m.norms || EVEN) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) rx = fmaxf(rx, __shfl_xor(rx, o));
+    }
     if (m.norms) {
       ss = wave_sum(ss);
-      if (ss > 1e-30f && ss < INFINITY) {
-        nx = fmaxf(nx, sqrtf(ss));
-      } else {  // squares left fp32's range: a bound that does not
+      if (ss > 1e-30f && ss < INFINITY) nx = fmaxf(nx, sqrtf(ss));
+      else nx = fmaxf(nx, fminf(rx * sqrtf((float)m.d), 3e38f));  // squares left fp32's range: a bound that does not
+    }
+    if (EVEN && rx > 0.0f) {
+      const int at = 255 - (int)(__float_as_uint(rx) >> 23);
+      low = at > low ? at : low;
+      const float least = rx * digits;
+      for (int c0 = 0; c0 < m.d; c0 += HELD * 512) {
+        if (m.d > HELD * 512) load(c0);
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) rx = fmaxf(rx, __shfl_xor(rx, o));
-        nx = fmaxf(nx, fminf(rx * sqrtf((float)m.d), 3e38f));
+        for (int q = 0; q < HELD; ++q) {
+          if (c0 + q * 512 >= m.d) break;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float v = fabsf(to_f(x[q][e]));
+            small += v < least && v > 0.0f ? 1 : 0;
+          }
+        }
       }
     }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-  __shared__ float sm[4], sn[4];
-  if (lane == 0) { sm[wave] = mx; sn[wave] = nx; }
+  if constexpr (EVEN) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) small += __shfl_xor(small, o);
+  }
+  __shared__ WidePart found[4];
+  if (lane == 0) found[wave] = WidePart{mx, nx, low, small};
   __syncthreads();
   if (threadIdx.x == 0) {
-    const int at = (int)blockIdx.x & (kSlots - 1);
-    atomicMax(&a.hdr->max[m.slot][at][0], __float_as_uint(fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]))));
-    if (m.norms) atomicMax(&a.hdr->max[kNormX + m.slot][at][0], __float_as_uint(fmaxf(fmaxf(sn[0], sn[1]), fmaxf(sn[2], sn[3]))));
+    WidePart f = found[0];
+    for (int w = 1; w < 4; ++w)
+      f = WidePart{fmaxf(f.max, found[w].max), fmaxf(f.norm, found[w].norm), f.low > found[w].low ? f.low : found[w].low, f.small + found[w].small};
+    parts[blockIdx.x] = f;
   }
+}
+
+// The scales and the format.  Narrow is what has rows within 2^kEven of each other and fewer small entries than a quarter of
+// a column would hold; with the gradient's rows besides, 2^kEvenG.  Model data lies far from both: rows behind a norm are
+// within 2^3, and of normal entries 1e-5 are small, of which a quarter of a column is 1 / 4 d.  One block, four waves to a matrix.
+template <typename T>
+__global__ void __launch_bounds__(64 * 4 * kCopies) wide_mode_kernel(RowsArgs a, const WidePart* parts, WideMode* mode, int gated,
+                                                                     int64_t rows_x, int64_t rows_w, int64_t rows_dh) {
+  struct Sum { float max, norm; int low; long long small; };
+  __shared__ Sum sums[4 * kCopies];
+  auto join = [](Sum& x, float max, float norm, int low, long long small) {
+    x = Sum{fmaxf(x.max, max), fmaxf(x.norm, norm), x.low > low ? x.low : low, x.small + small};
+  };
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  Sum s = {0.0f, 0.0f, 0, 0};
+  {
+    const int64_t end = a.first[wave / 4 + 1], b = a.first[wave / 4] + wave % 4 * 64 + lane;
+    constexpr int PER = (int)(kMaxBlocks / 256);
+    WidePart p[PER];
+#pragma unroll
+    for (int q = 0; q < PER; ++q) p[q] = b + q * 256 < end ? parts[b + q * 256] : WidePart{0.0f, 0.0f, 0, 0};
+#pragma unroll
+    for (int q = 0; q < PER; ++q) join(s, p[q].max, p[q].norm, p[q].low, p[q].small);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) join(s, __shfl_xor(s.max, o), __shfl_xor(s.norm, o), __shfl_xor(s.low, o), __shfl_xor(s.small, o));
+  if (lane == 0) sums[wave] = s;
+  __syncthreads();
+  if (threadIdx.x > 0) return;
+  Sum f[3] = {};
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    Sum m = sums[4 * i];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) join(m, sums[4 * i + w].max, sums[4 * i + w].norm, sums[4 * i + w].low, sums[4 * i + w].small);
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (a.m[i].slot == k) join(f[k], m.max, m.norm, m.low, m.small);  // a place without a matrix has zeros
+  }
+  bool wide = false;
+  if constexpr (__is_same(T, float)) {
+    const int64_t rows[3] = {rows_x >= 0 ? rows_x : mode->live, rows_w, rows_dh};  // -1: those that count
+    int sum = 0;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const int uneven = f[k].low > 0 ? (int)(__float_as_uint(f[k].max) >> 23) + f[k].low - 255 : 0;
+      wide = wide || f[k].small * 4 > rows[k] || (k < 2 && uneven > kEven);
+      sum += uneven;
+    }
+    wide = wide || (rows_dh > 0 && sum > kEvenG);
+  }
+  mode->wide = wide ? 1 : 0;
+  mode->sx = wide ? 1.0f : pow2_to(f[0].max, 15);
+  mode->sw = wide ? 1.0f : pow2_to(f[1].max, 15);
+  mode->sg = wide ? 1.0f : gated ? pow2_to(1.15f * fminf(f[2].max, 1e38f), f[0].norm, f[1].norm, 15) : 32768.0f;
 }
 
 // Rows to operand rows.  A wave per row, 8 columns a lane; a matrix's last blocks zero the rows behind the last one that
 // counts, up to the next multiple of 128.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) rows_copy_kernel(RowsArgs a, int dp) {
-  using E = typename Wide<T>::E;
   const int i = matrix_of(a, blockIdx.x), lane = (int)threadIdx.x & 63;
   const RowsCopy m = a.m[i];
   const int64_t r = ((int64_t)blockIdx.x - a.first[i]) * 4 + (threadIdx.x >> 6);
@@ -110,7 +208,7 @@ __global__ void __launch_bounds__(kThreads) rows_copy_kernel(RowsArgs a, int dp)
   bool zero = false;
   if (r >= m.rows) {
     if (m.pos == nullptr) return;
-    const int64_t live = a.hdr->live;
+    const int64_t live = a.mode->live;
     to = live + (r - m.rows);
     if (to >= (live + 127) / 128 * 128) return;
     zero = true;
@@ -118,11 +216,9 @@ __global__ void __launch_bounds__(kThreads) rows_copy_kernel(RowsArgs a, int dp)
     to = m.pos[r];
     if (to < 0) return;
   }
-  float s = 1.0f;
-  if constexpr (Wide<T>::P == 2) s = m.slot == 0 ? scale_x<T>(a.hdr) : scale_w<T>(a.hdr);
+  const float s = m.slot == 0 ? scale_x<T>(a.mode) : scale_w<T>(a.mode);
   char* const out = m.dst + to * 64;
   const T* in = (const T*)m.src + r * m.ld;
-  typedef __attribute__((__vector_size__(16))) E E8;
   for (int c = lane * 8; c < dp; c += 512) {
     T x[8];
     if (zero || c >= m.d) {
@@ -131,21 +227,24 @@ __global__ void __launch_bounds__(kThreads) rows_copy_kernel(RowsArgs a, int dp)
     } else {
       load8(in, c, m.d, a.vec[i] != 0, x);
     }
-    E8 h;
-    if constexpr (Wide<T>::P == 2) {
-      E8 l;
+    by_format<T>(a.mode, [&](auto wide) {
+      using F = Wide<T, decltype(wide)::value>;
+      using E = typename F::E;
+      typedef __attribute__((__vector_size__(16))) E E8;
+      E8 t[F::P];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const Terms<E> t(x[e] * s);
-        h[e] = t.h;
-        l[e] = t.l;
-      }
-      *reinterpret_cast<E8*>(out + (c >> 5) * m.blk + (c & 31) * 2 + m.plane_bytes) = l;
-    } else {
+        if constexpr (F::P == 1) {
+          t[0][e] = x[e];
+        } else {
+          const Terms<E, F::P> v(x[e] * s);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = x[e];
-    }
-    *reinterpret_cast<E8*>(out + (c >> 5) * m.blk + (c & 31) * 2) = h;
+          for (int k = 0; k < F::P; ++k) t[k][e] = v.t[k];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < F::P; ++k) *reinterpret_cast<E8*>(out + (c >> 5) * m.blk + (c & 31) * 2 + k * m.plane_bytes) = t[k];
+    });
   }
 }
 
@@ -156,14 +255,14 @@ struct ProductArgs {
   int tm, dx_tiles, dx_blocks, dw_blocks, dx_steps, dw_tn, halves, cols;
   int64_t C;
   WideShare share;
-  MmSegs dx_segs, dw_segs;
+  MmSegs dx_segs[2], dw_segs[2];  // of the narrow and the wide format
   const char* x; int64_t x_ld, x_blk; int x_rows;
   const char* w; int64_t w_ld, w_blk; int w_rows;
   const char* g; int64_t g_half;
   float* dx_part; int dx_add;
   void* dw0; void* dw1;
   float* dw_part;
-  const WideHdr* hdr;
+  const WideMode* mode;
   GradUnit unit; const float* cmax;
   int use_live, gated, vec;
 };
@@ -172,9 +271,9 @@ struct ProductArgs {
 // launch, the longer blocks first, so that neither leaves CUs idle at its end.  Ranges of one tile, and tiles of one block
 // of rows or columns of G, stand side by side: an XCD's blocks then read the same rows of W or x at the same time.  (Cut
 // where equal shares end instead, the blocks start at places of their own in W: 12% slower at 8192 rows.)
-template <typename T>
+template <typename T, bool WIDE>
 struct Products {
-  using E = typename Wide<T>::E;
+  using E = typename Wide<T, WIDE>::E;
   using TX = MmTile<E, 256, kTileN, 2, 4, true, false, false, 4>;
   using TW = MmTile<E, 256, kTileN, 2, 4, true, true, false, 4>;
 
@@ -186,7 +285,7 @@ struct Products {
     TX::clear(acc);
     const typename TX::Side A{p.w + (m0 >> 5) * p.w_blk, (int)(p.dp - m0), p.w_ld, p.w_blk, p.w_rows, 0};
     const typename TX::Side B{p.g + (int64_t)n0 * 64, (int)(p.n_pad - n0), 64, p.n_pad * 64, 0, 0};
-    if (to > from) TX::run(acc, lds, A, B, p.dx_segs, from * 32, to - from);
+    if (to > from) TX::run(acc, lds, A, B, p.dx_segs[WIDE], from * 32, to - from);
     float* out = p.dx_part + ((int64_t)part * p.n_pad + n0) * p.dp + m0;
     auto fn = [&](int i, int j, int g) { return quad<float>([&](int e) { return acc[i][j][4 * g + e]; }); };
     const int rows = (int)(N - n0 < kTileN ? N - n0 : kTileN);
@@ -208,14 +307,14 @@ struct Products {
     TW::clear(acc);
     const typename TW::Side A{p.x + (m0 >> 5) * p.x_blk, (int)(p.dp - m0), p.x_ld, p.x_blk, p.x_rows, 0};
     const typename TW::Side B{p.g + half * p.g_half + (n0 >> 5) * p.n_pad * 64, (int)(p.C - n0), 64, p.n_pad * 64, (int)p.n_pad, 0};
-    if (to > from) TW::run(acc, lds, A, B, p.dw_segs, from * 32, to - from);
+    if (to > from) TW::run(acc, lds, A, B, p.dw_segs[WIDE], from * 32, to - from);
     const int rows = p.cols - n0 < kTileN ? p.cols - n0 : kTileN;
     if (p.share.dw_split > 1) {
       float* out = p.dw_part + (((int64_t)split * p.halves + half) * p.C + n0) * p.dp + m0;
       TW::template store_rows<float, false>(lds, out, p.dp, rows, (int)(p.dp - m0), true,
                                             [&](int i, int j, int g) { return quad<float>([&](int e) { return acc[i][j][4 * g + e]; }); });
     } else {
-      const float f = unit_of(p.unit, p.hdr, p.cmax) / scale_g<T>(p.hdr, p.gated), fx = 1.0f / scale_x<T>(p.hdr);
+      const float f = unit_of(p.unit, p.mode, p.cmax) / scale_g<T>(p.mode, p.gated), fx = 1.0f / scale_x<T>(p.mode);
       T* out = (T*)(half ? p.dw1 : p.dw0) + (int64_t)n0 * p.d + m0;
       TW::template store_rows<T, false>(lds, out, p.d, rows, p.d - m0, p.vec != 0,
                                         [&](int i, int j, int g) { return quad<T>([&](int e) { return acc[i][j][4 * g + e] * f * fx; }); });
@@ -225,39 +324,45 @@ struct Products {
 
 template <typename T>
 __global__ void __launch_bounds__(kProductThreads, 2) products_kernel(ProductArgs p) {
-  __shared__ char smem[Products<T>::TX::LDS];
+  __shared__ char smem[Products<T, false>::TX::LDS];
   LdsChar* lds = (LdsChar*)smem;
-  const int64_t N = p.use_live ? p.hdr->live : p.N;
+  const int64_t N = p.use_live ? p.mode->live : p.N;
   const int first = p.share.dx_first ? p.dx_blocks : p.dw_blocks;
   const bool head = (int)blockIdx.x < first;
   const int64_t at = head ? blockIdx.x : (int64_t)blockIdx.x - first;
-  if (head == p.share.dx_first) {
-    int64_t t = xcd_order(at, p.dx_blocks);
-    const int split = (int)(t % p.share.dx_split);
-    t /= p.share.dx_split;
-    const int from = (int)((int64_t)p.dx_steps * split / p.share.dx_split), to = (int)((int64_t)p.dx_steps * (split + 1) / p.share.dx_split);
-    Products<T>::dx(p, lds, N, (int)(t % p.tm), (int)(t / p.tm), split, from, to);
-  } else {
-    Products<T>::dw(p, lds, N, xcd_order(at, p.dw_blocks));
-  }
+  by_format<T>(p.mode, [&](auto wide) {
+    using P = Products<T, decltype(wide)::value>;
+    if (head == p.share.dx_first) {
+      int64_t t = xcd_order(at, p.dx_blocks);
+      const int split = (int)(t % p.share.dx_split);
+      t /= p.share.dx_split;
+      const int from = (int)((int64_t)p.dx_steps * split / p.share.dx_split), to = (int)((int64_t)p.dx_steps * (split + 1) / p.share.dx_split);
+      P::dx(p, lds, N, (int)(t % p.tm), (int)(t / p.tm), split, from, to);
+    } else {
+      P::dw(p, lds, N, xcd_order(at, p.dw_blocks));
+    }
+  });
 }
 
 // As many blocks as CUs, each with its share of both products (WideShare).  Blocks of an XCD hold one range of many tiles,
 // so that they read the same rows of W at the same time.
 template <typename T>
 __global__ void __launch_bounds__(kProductThreads, 2) shares_kernel(ProductArgs p) {
-  __shared__ char smem[Products<T>::TX::LDS];
+  __shared__ char smem[Products<T, false>::TX::LDS];
   LdsChar* lds = (LdsChar*)smem;
-  const int64_t N = p.use_live ? p.hdr->live : p.N;
+  const int64_t N = p.use_live ? p.mode->live : p.N;
   const int slot = (int)xcd_order(blockIdx.x, p.share.slots);
-  for (int t = slot; t < p.dw_blocks; t += p.share.slots) Products<T>::dw(p, lds, N, t);
-  const int part = slot / p.dx_tiles, tile = slot - part * p.dx_tiles;
-  if (part >= p.share.dx_split) return;
-  const int a = p.share.a, b = p.share.b, n = p.share.n_a;
-  int from = part < n ? part * a : n * a + (part - n) * b, to = part < n ? from + a : from + b;
-  if (part == p.share.dx_split - 1 || to > p.dx_steps) to = p.dx_steps;
-  if (from > to) from = to;
-  Products<T>::dx(p, lds, N, tile % p.tm, tile / p.tm, part, from, to);
+  by_format<T>(p.mode, [&](auto wide) {
+    using P = Products<T, decltype(wide)::value>;
+    for (int t = slot; t < p.dw_blocks; t += p.share.slots) P::dw(p, lds, N, t);
+    const int part = slot / p.dx_tiles, tile = slot - part * p.dx_tiles;
+    if (part >= p.share.dx_split) return;
+    const int a = p.share.a, b = p.share.b, n = p.share.n_a;
+    int from = part < n ? part * a : n * a + (part - n) * b, to = part < n ? from + a : from + b;
+    if (part == p.share.dx_split - 1 || to > p.dx_steps) to = p.dx_steps;
+    if (from > to) from = to;
+    P::dx(p, lds, N, tile % p.tm, tile / p.tm, part, from, to);
+  });
 }
 
 // Sums of parts in their order, scaled, as rows of T.  A wave per row; the second matrix's rows follow the first's.
@@ -267,7 +372,7 @@ struct PartArgs {
   int64_t rows;
   int d, dp;
   const int* pos;
-  const WideHdr* hdr;
+  const WideMode* mode;
   GradUnit unit; const float* cmax;
   int gated, by_x;
   void* out0; void* out1;
@@ -283,7 +388,7 @@ __global__ void __launch_bounds__(kThreads) parts_kernel(PartArgs a) {
     part += a.half_stride;
   }
   const int64_t at = a.pos == nullptr ? r : a.pos[r];
-  const float f = unit_of(a.unit, a.hdr, a.cmax) / scale_g<T>(a.hdr, a.gated), f2 = 1.0f / (a.by_x ? scale_x<T>(a.hdr) : scale_w<T>(a.hdr));
+  const float f = unit_of(a.unit, a.mode, a.cmax) / scale_g<T>(a.mode, a.gated), f2 = 1.0f / (a.by_x ? scale_x<T>(a.mode) : scale_w<T>(a.mode));
   for (int c = ((int)threadIdx.x & 63) * 4; c < a.d; c += 256) {
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     if (at >= 0) {
@@ -317,7 +422,7 @@ RowsArgs rows_args(const RowsCopies& c, int64_t most, bool zeros, int64_t* block
   }
   a.first[kCopies] = at;
   for (int i = c.n; i < kCopies; ++i) a.first[i] = at;
-  a.hdr = c.hdr;
+  a.mode = c.mode;
   *blocks = at;
   return a;
 }
@@ -332,11 +437,16 @@ hipError_t rows_copy(const RowsCopies& c, hipStream_t s) {
 }
 
 template <typename T>
-hipError_t rows_max(const RowsCopies& c, hipStream_t s) {
-  int64_t blocks;
-  const RowsArgs a = rows_args(c, 1024, false, &blocks);
-  if (blocks == 0) return hipSuccess;
-  hipLaunchKernelGGL(rows_max_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
+hipError_t wide_mode(const RowsCopies& c, WidePart* parts, WideMode* mode, int gated, hipStream_t s) {
+  int64_t blocks, rows[3] = {0, 0, 0};
+  const RowsArgs a = rows_args(c, kMaxBlocks, false, &blocks);
+  if (blocks > 0) {
+    hipLaunchKernelGGL(rows_max_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, s, a, parts);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  for (int i = 0; i < c.n; ++i) rows[c.m[i].slot] += c.m[i].pos != nullptr ? -1 : c.m[i].rows;
+  hipLaunchKernelGGL(wide_mode_kernel<T>, dim3(1), dim3(1024), 0, s, a, parts, mode, gated, rows[0], rows[1], rows[2]);
   return hipGetLastError();
 }
 
@@ -360,26 +470,32 @@ hipError_t products(const WideProducts& p, hipStream_t s) {
   for (int t = p.g_terms - 1; t >= 0; --t) {
     for (int half = 0; half < p.halves; ++half) {
       const int64_t wh = half ? p.w[1] - p.w[0] : 0, gh = half * p.g_half;
-      a.dx_segs.a[n] = wh; a.dx_segs.b[n++] = gh + t * p.g_plane;
-      if (t == 1 && P == 2) { a.dx_segs.a[n] = wh + p.w_plane; a.dx_segs.b[n++] = gh; }
+      a.dx_segs[0].a[n] = wh; a.dx_segs[0].b[n++] = gh + t * p.g_plane;
+      if (t == 1 && P == 2) { a.dx_segs[0].a[n] = wh + p.w_plane; a.dx_segs[0].b[n++] = gh; }
     }
-    if (t == 1) a.dx_segs.low = n;
+    if (t == 1) a.dx_segs[0].low = n;
   }
-  a.dx_segs.n = n;
+  a.dx_segs[0].n = n;
   n = 0;
   if (p.g_terms == 2) {
-    a.dw_segs.a[n] = 0; a.dw_segs.b[n++] = p.g_plane;
-    if (P == 2) { a.dw_segs.a[n] = p.x_plane; a.dw_segs.b[n++] = 0; }
+    a.dw_segs[0].a[n] = 0; a.dw_segs[0].b[n++] = p.g_plane;
+    if (P == 2) { a.dw_segs[0].a[n] = p.x_plane; a.dw_segs[0].b[n++] = 0; }
   }
-  a.dw_segs.low = n;
-  a.dw_segs.a[n] = 0; a.dw_segs.b[n++] = 0;
-  a.dw_segs.n = n;
+  a.dw_segs[0].low = n;
+  a.dw_segs[0].a[n] = 0; a.dw_segs[0].b[n++] = 0;
+  a.dw_segs[0].n = n;
+  if (P == 2) {
+    for (int order = 2; order >= 0; --order)
+      for (int half = 0; half < p.halves; ++half)
+        add_wide_segs(a.dx_segs[1], order, half ? p.w[1] - p.w[0] : 0, p.w_plane, half * p.g_half, p.g_plane);
+    for (int order = 2; order >= 0; --order) add_wide_segs(a.dw_segs[1], order, 0, p.x_plane, 0, p.g_plane);
+  }
   a.x = p.x; a.x_ld = p.x_ld; a.x_blk = p.x_blk; a.x_rows = p.x_rows;
   a.w = p.w[0]; a.w_ld = p.w_ld; a.w_blk = p.w_blk; a.w_rows = p.w_rows;
   a.g = p.g; a.g_half = p.g_half;
   a.dx_part = p.dx_part; a.dx_add = p.dx_add;
   a.dw0 = p.dw[0]; a.dw1 = p.dw[1]; a.dw_part = p.dw_part;
-  a.hdr = p.hdr; a.unit = p.unit; a.cmax = p.cmax; a.use_live = p.use_live; a.gated = p.gated;
+  a.mode = p.mode; a.unit = p.unit; a.cmax = p.cmax; a.use_live = p.use_live; a.gated = p.gated;
   a.vec = (int64_t)p.d * sizeof(T) % 16 == 0 && ((uintptr_t)p.dw[0] & 15) == 0 && ((uintptr_t)p.dw[1] & 15) == 0;
   if (p.share.slots > 0) hipLaunchKernelGGL(shares_kernel<T>, dim3((unsigned)p.share.slots), dim3(kProductThreads), 0, s, a);
   else hipLaunchKernelGGL(products_kernel<T>, dim3((unsigned)(a.dx_blocks + a.dw_blocks)), dim3(kProductThreads), 0, s, a);
@@ -387,7 +503,7 @@ hipError_t products(const WideProducts& p, hipStream_t s) {
   if (e != hipSuccess || !dw || p.share.dw_split == 1) return e;
   PartArgs q = {};
   q.part = p.dw_part; q.part_stride = (int64_t)p.halves * p.C * p.dp; q.half_stride = p.C * p.dp; q.split = p.share.dw_split;
-  q.rows = p.cols; q.d = p.d; q.dp = (int)p.dp; q.hdr = p.hdr; q.unit = p.unit; q.cmax = p.cmax; q.gated = p.gated; q.by_x = 1;
+  q.rows = p.cols; q.d = p.d; q.dp = (int)p.dp; q.mode = p.mode; q.unit = p.unit; q.cmax = p.cmax; q.gated = p.gated; q.by_x = 1;
   q.out0 = p.dw[0]; q.out1 = p.halves == 2 ? p.dw[1] : nullptr;
   hipLaunchKernelGGL(parts_kernel<T>, dim3((unsigned)((q.rows * p.halves + 3) / 4)), dim3(kThreads), 0, s, q);
   return hipGetLastError();
@@ -398,7 +514,7 @@ hipError_t finish(const WideFinish& f, hipStream_t s) {
   if (f.N == 0) return hipSuccess;
   PartArgs q = {};
   q.part = f.part; q.part_stride = f.n_pad * f.dp; q.split = f.split;
-  q.rows = f.N; q.d = f.d; q.dp = (int)f.dp; q.pos = f.pos; q.hdr = f.hdr; q.unit = f.unit; q.cmax = f.cmax; q.gated = f.gated;
+  q.rows = f.N; q.d = f.d; q.dp = (int)f.dp; q.pos = f.pos; q.mode = f.mode; q.unit = f.unit; q.cmax = f.cmax; q.gated = f.gated;
   q.out0 = f.dx;
   hipLaunchKernelGGL(parts_kernel<T>, dim3((unsigned)((f.N + 3) / 4)), dim3(kThreads), 0, s, q);
   return hipGetLastError();
@@ -406,15 +522,11 @@ hipError_t finish(const WideFinish& f, hipStream_t s) {
 
 }  // namespace
 
-hipError_t launch_hdr_clear(WideHdr* hdr, hipStream_t s) {
-  hipLaunchKernelGGL(hdr_clear_kernel, dim3(1), dim3(kThreads), 0, s, hdr);
-  return hipGetLastError();
-}
 hipError_t launch_rows_copy(const RowsCopies& c, hipStream_t s) {
   return c.dtype == 0 ? rows_copy<float>(c, s) : c.dtype == 1 ? rows_copy<bf16>(c, s) : rows_copy<f16>(c, s);
 }
-hipError_t launch_rows_max(const RowsCopies& c, hipStream_t s) {
-  return c.dtype == 0 ? rows_max<float>(c, s) : c.dtype == 1 ? rows_max<bf16>(c, s) : rows_max<f16>(c, s);
+hipError_t launch_wide_mode(const RowsCopies& c, WidePart* parts, WideMode* mode, int gated, hipStream_t s) {
+  return c.dtype == 0 ? wide_mode<float>(c, parts, mode, gated, s) : wide_mode<f16>(c, parts, mode, gated, s);
 }
 hipError_t launch_wide_products(const WideProducts& p, hipStream_t s) {
   return p.dtype == 0 ? products<float>(p, s) : p.dtype == 1 ? products<bf16>(p, s) : products<f16>(p, s);

@@ -652,8 +652,10 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="m
     few rows are the scores of a decoding step.  float32; sums and softmax
     statistics are too.
     The backward pass forms the logits again, in pieces of the vocabulary of at
-    most 1 GB; their gradient is rounded to hidden's type (float32: 22 bits; up to
-    256 rows: two terms of the type).
+    most 1 GB; their gradient is rounded to hidden's type (up to 256 rows: two terms
+    of the type).  float32 is multiplied in 22 bits where rows and weights are even,
+    as behind a norm, and in 24 bits over its whole range, in twice the time, where
+    some rows or columns lie 2^10 and more above others.
     Forward and backward pass can be captured into a HIP graph together, once no
     autograd graph of an eager call on the same leaves is alive (torch's rule for
     every backward pass).
@@ -758,7 +760,8 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
     (autocast's under it); activation "silu" or "gelu" (the exact one, by erf).
     Returns (..., F); activation and product are taken in float32 and rounded once.
     The backward pass forms both products again; their gradients are rounded to
-    x's type (float32: 22 bits; up to 256 rows: two terms), sums are float32.
+    x's type (up to 256 rows: two terms; float32: as in linear_cross_entropy), sums
+    are float32.
     """
     x, w_gate, w_up = _autocast(x, w_gate, w_up)
     _one_gpu("gated_linear", x.get_device(), w_gate, w_up)
