@@ -19,12 +19,13 @@ constexpr int kThreads = 256;
 constexpr int kHeadMaxK = 256;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// What the backward pass needs: mode, pos[N] (row of the operand, -1: does not count), lse2[N rows of the operand],
-// t[N][K]: 2^(z2 - lse2) - p of the targets (p summed over equal ids).
+// What the backward pass needs: mode, pos[N] (row of the operand, -1: does not count), lse[N rows of the operand]: the
+// largest of x_n . W_v, and log2 of the sum of 2^z2 over its own; t[N][K]: 2^(z2 - lse2) - p of the targets (p summed over
+// equal ids).
 struct HeadState {
   WideMode* mode;
   int* pos;
-  float* lse2;
+  float2* lse;
   float* t;
   size_t bytes;
   HeadState(void* p, int64_t N, int K) {
@@ -32,7 +33,7 @@ struct HeadState {
     size_t o = (size_t)round_up(sizeof(WideMode), 256);
     mode = (WideMode*)c;
     pos = (int*)(c + o); o += (size_t)round_up(N * 4, 256);
-    lse2 = (float*)(c + o); o += (size_t)round_up(round_up(N, 128) * 4, 256);
+    lse = (float2*)(c + o); o += (size_t)round_up(round_up(N, 128) * 8, 256);
     t = (float*)(c + o); o += (size_t)round_up(N * K * 4, 256);
     bytes = o;
   }
@@ -167,6 +168,11 @@ struct StatsArgs {
   float2* part; int64_t part_ld;  // [tiles_v][part_ld]
 };
 
+// Logits as the product leaves them, a, times f > 0 are z2.  Statistics keep a row's largest a itself and a sum over
+// 2^(f (a - max)), and G takes a - max too, so that the largest one's term is 1 whatever its size.  One fma with f max rounded
+// would be off by up to half a step of it: 2^(1/32) at z2 = 2^20, past any number at 2^31.  It would save 5 us of
+// 1780 (ce_train_8k_bf16: stats 4, G 1).
+
 // Features from `left` on become v: only the last tile along the vocabulary pays for the comparisons.
 template <typename Tl>
 __device__ inline void mask_features(typename Tl::Acc& acc, int left, int wm, int lane, float v) {
@@ -213,13 +219,13 @@ __device__ inline void stats_tile(const StatsArgs& a, LdsChar* lds, float2 (*red
     for (int i = 0; i < Tl::MB; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc[i][j][r]);
-    mx = f * fmaxf(mx, __shfl_xor(mx, 32));  // f > 0
-    const float at = mx == -INFINITY ? 0.0f : mx;
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const float top = mx == -INFINITY ? 0.0f : mx;
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < Tl::MB; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], f, -at));
+      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - top) * f);
     s += __shfl_xor(s, 32);
     if (lane < 32) red[wm][Tl::n_of(wn, lane, j)] = float2{mx, s};
   }
@@ -229,7 +235,7 @@ __device__ inline void stats_tile(const StatsArgs& a, LdsChar* lds, float2 (*red
     static_assert(WM == 2, "two waves share a row's features");
     const float m = fmaxf(p.x, q.x), at = m == -INFINITY ? 0.0f : m;
     a.part[(int64_t)tv * a.part_ld + n0 + threadIdx.x] =
-        float2{m, p.y * __builtin_amdgcn_exp2f(p.x - at) + q.y * __builtin_amdgcn_exp2f(q.x - at)};
+        float2{m, p.y * __builtin_amdgcn_exp2f((p.x - at) * f) + q.y * __builtin_amdgcn_exp2f((q.x - at) * f)};
   }
 }
 
@@ -259,7 +265,8 @@ struct RowsArgs {
   int64_t N, V, ignore; int d, K, vec, rows;
   float temperature;
   const int* pos;  // null: every row whose id is not `ignore`, in its own place
-  float* lse2; float* t; float* loss;  // lse2, t: null where no gradient follows
+  const WideMode* mode;
+  float2* lse; float* t; float* loss;  // lse, t: null where no gradient follows
 };
 
 // PER neighbours of a row, zeros past its end.
@@ -283,11 +290,17 @@ __device__ inline void load_vec(const T* p, int c, int d, bool vec, T (&v)[16 / 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
   __shared__ float2 red[kThreads];
-  __shared__ float2 stat[kRows];  // the row's maximum and log2 of its sum
+  __shared__ float2 stat[kRows];  // the row's largest logit and log2 of its sum
   __shared__ int place[kRows];    // the row's place in the operand, -1: it does not count
   __shared__ float terms[kRows][kHeadMaxK];
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int64_t first = (int64_t)blockIdx.x * a.rows;
+  const float to_log2 = kLog2e / a.temperature;
+  float f = to_log2, unscale = 1.0f;  // of the product's own numbers, and to x . W
+  if constexpr (__is_same(T, float)) {
+    f = f / scale_x<T>(a.mode) / scale_w<T>(a.mode);
+    unscale = 1.0f / scale_x<T>(a.mode) / scale_w<T>(a.mode);
+  }
   {
     const int r = tid & (a.rows - 1), g = tid / a.rows, groups = kThreads / a.rows;  // rows is a power of two
     int at = -1;
@@ -295,7 +308,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
     float m = -INFINITY, s = 0.0f;
     auto add = [&](float2 p) {
       const float mn = fmaxf(m, p.x), b = mn == -INFINITY ? 0.0f : mn;
-      s = s * __builtin_amdgcn_exp2f(m - b) + p.y * __builtin_amdgcn_exp2f(p.x - b);
+      s = s * __builtin_amdgcn_exp2f((m - b) * f) + p.y * __builtin_amdgcn_exp2f((p.x - b) * f);
       m = mn;
     };
     if (at >= 0) {
@@ -321,7 +334,6 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
     if (tid < a.rows) stat[tid] = float2{m, log2f(s)};
     __syncthreads();
   }
-  const float to_log2 = kLog2e / a.temperature;
   constexpr int PER = 16 / (int)sizeof(T);
   const int l16 = lane & 15;
   for (int e = tid >> 4; e < a.rows * a.K; e += 16) {
@@ -345,7 +357,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
         }
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor(dot, o);
-        const float away = (stat[r].x - to_log2 * dot) + stat[r].y;  // lse2 - z2
+        const float away = to_log2 * (stat[r].x * unscale - dot) + stat[r].y;  // lse2 - z2
         t = __builtin_amdgcn_exp2f(-away) - p.y;
         term = p.x > 0.0f || !(p.x == p.x) ? p.x * away : 0.0f;
       } else if (!(p.x < 0.0f)) {
@@ -373,7 +385,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
         if (a.tp != nullptr && at >= 0) loss = a.temperature * a.temperature * (loss + a.ent[n]);
         a.loss[n] = at >= 0 ? loss : 0.0f;
         // a target outside the vocabulary makes the row NaN, its gradient too
-        if (at >= 0 && a.lse2 != nullptr) a.lse2[at] = away == away ? stat[r].x + stat[r].y : NAN;
+        if (at >= 0 && a.lse != nullptr) a.lse[at] = float2{stat[r].x * unscale, away == away ? stat[r].y : NAN};
       }
     }
   }
@@ -445,7 +457,7 @@ struct GradArgs {
   int ksteps, tiles_v, tiles_n;
   float to_log2;
   const WideMode* mode;
-  const float* lse2; const float* coef;
+  const float2* lse; const float* coef;
   char* g; int64_t plane;
 };
 
@@ -474,13 +486,14 @@ __device__ inline void grad_tile(const GradArgs& a, LdsChar* lds) {
   for (int j = 0; j < Tl::NB; ++j) {
     const int64_t n = n0 + Tl::n_of(wn, lane, j);
     const bool ok = n < live;
-    // a row behind the last one has an operand of zeros, lse2 of infinity and so a gradient of zeros; the power of two sg
+    // a row behind the last one has an operand of zeros, lse of infinity and so a gradient of zeros; the power of two sg
     // goes into the exponent
-    const float l = ok ? a.lse2[n] - lg : INFINITY;
+    const float2 lse = ok ? a.lse[n] : float2{0.0f, INFINITY};
+    const float top = lse.x * scale_x<T>(a.mode) * scale_w<T>(a.mode), l = lse.y - lg;
 #pragma unroll
     for (int i = 0; i < Tl::MB; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], f, -l));
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r] - top, f, -l));
     if (a.coef != nullptr) {
       const float c = ok ? a.coef[n] : 0.0f;
 #pragma unroll
@@ -678,7 +691,7 @@ hipError_t head_fwd(const HeadCall& c) {
     r.x = c.x; r.x_ld = c.x_ld; r.w = c.w; r.w_ld = c.w_ld; r.ids = c.ids; r.ids_ld = c.ids_ld; r.tp = p.tp; r.ent = p.ent;
     r.part = p.part; r.part_ld = p.n_pad; r.tiles = p.tiles_v; r.N = c.N; r.V = c.V; r.ignore = c.ignore_index; r.d = c.d; r.K = c.K;
     r.vec = rows_vec(c); r.rows = c.N > 2048 ? 8 : c.N > 1024 ? 4 : c.N > 512 ? 2 : 1;
-    r.temperature = c.temperature; r.pos = direct ? nullptr : st.pos; r.lse2 = direct ? nullptr : st.lse2; r.t = direct ? nullptr : st.t;
+    r.temperature = c.temperature; r.pos = direct ? nullptr : st.pos; r.mode = direct ? nullptr : st.mode; r.lse = direct ? nullptr : st.lse; r.t = direct ? nullptr : st.t;
     r.loss = c.reduction == 0 ? c.loss : p.rows;
     hipLaunchKernelGGL(rows_kernel<T>, dim3((unsigned)((c.N + r.rows - 1) / r.rows)), dim3(kThreads), 0, c.stream, r);
     HEAD_TRY(hipGetLastError());
@@ -714,7 +727,7 @@ hipError_t head_bwd(const HeadCall& c) {
     GradArgs a;
     a.x = p.x; a.n_pad = p.n_pad; a.w = w + v0 * w_ld; a.w_ld = w_ld; a.w_blk = w_blk; a.cols = cols;
     p.logits(a.segs); a.ksteps = (int)(p.dp / 32); a.tiles_v = (int)(round_up(cols, 256) / 256); a.tiles_n = p.tiles_n;
-    a.to_log2 = kLog2e / c.temperature; a.mode = mode; a.lse2 = st.lse2; a.coef = p.coef; a.g = p.g; a.plane = p.g_plane;
+    a.to_log2 = kLog2e / c.temperature; a.mode = mode; a.lse = st.lse; a.coef = p.coef; a.g = p.g; a.plane = p.g_plane;
     auto* grad = p.g_terms == 2 ? grad_kernel<T, 2> : grad_kernel<T, __is_same(T, float) ? 2 : 1>;
     hipLaunchKernelGGL(grad, dim3((unsigned)((int64_t)a.tiles_v * a.tiles_n)), dim3(kThreads), 0, c.stream, a);
     HEAD_TRY(hipGetLastError());
