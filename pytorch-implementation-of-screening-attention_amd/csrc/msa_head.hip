@@ -4,7 +4,7 @@
 //   distillation   L_n = T^2 (sum_k p_k ln p_k - ln2 sum_k p_k (z2_n,id(k) - lse2_n)),  p = softmax of the row's entries
 //   both           dL_n/dz_nv = T (2^(z2_nv - lse2_n) - sum_{k: id(k) = v} p_k)        (z: logits before 1/T)
 // Forward: one product over all of the vocabulary whose tiles leave each row's maximum and sum; a row's own logits are
-// K dot products.  Backward, in pieces of the vocabulary: the product again, now with lse2 known, gives the piece's
+// K dot products in the same order.  Backward, in pieces of the vocabulary: the product again, now with lse2 known, gives the piece's
 // gradient G in the operand type (1 GB at most, or 256 columns); then dx += G W and dW = G^T x (msa_wide.hip).
 // Rows that do not count are taken out before the products: their x may hold anything.
 // Matrix units bound it, at the clock that the card's power allows: 8192 rows of 512 by 50257 bf16, a training pass 1780 us =
@@ -250,44 +250,75 @@ __global__ void __launch_bounds__(Tile<T>::THREADS, 2) stats_kernel(StatsArgs a)
 }
 
 // ---------------------------------------------------------------------------
-// A row's sum over the tiles, its targets' logits and its loss.  A block takes up to 8 rows: first its threads
-// share the tiles, then 16 lanes take a target at a time (a dot product of d terms).
-// Few rows are spread over more blocks.
+// A row's targets' logits, its sum over the tiles and its loss.  A block takes up to 8 rows: its waves form 32 targets'
+// logits at a time, its threads share the tiles, then each thread has a target.  Few rows are spread over more blocks.
+//
+// Logits are formed as the product formed them, by the same MFMA in the same order, so that a target's is bitwise the one in
+// its row's sum: away = lse2 - z2 is then log2 of a sum that has 1 in it, and neither that nor 1 - q hides behind the logits'
+// own rounding.  (By another order they are off by 1e-5 at logits of 120: losses below that come out negative and their
+// gradients of either sign.)  32 targets and their rows are A and B; of the 32 x 32 results the diagonal counts.
+// Bound by the latency of what it gathers: 8192 rows of 64 targets at d = 256 (537 MB) 61 us, 8192 rows of one at 512 21 us.  A
+// lone pair is one wave's, 8 steps in flight instead of 4 (16 scores: a call 23.1 -> 22.4 us with the tiles' loads ahead of it);
+// with more pairs a CU holds one block of those instead of three (8192 rows 35 us).
 // ---------------------------------------------------------------------------
 constexpr int kRows = 8;  // of a block, at most
 struct RowsArgs {
-  const void* x; int64_t x_ld;
-  const void* w; int64_t w_ld;
+  const char* x; int64_t x_ld, x_blk;  // operands, as in StatsArgs
+  const char* w; int64_t w_ld, w_blk;
+  MmSegs segs[2];
+  int ksteps;
   const int64_t* ids; int64_t ids_ld;
   const float2* tp;  // null: cross entropy
   const float* ent;
   const float2* part; int64_t part_ld; int tiles;
-  int64_t N, V, ignore; int d, K, vec, rows;
+  int64_t N, V, ignore; int K, rows;
   float temperature;
   const int* pos;  // null: every row whose id is not `ignore`, in its own place
   const WideMode* mode;
   float2* lse; float* t; float* loss;  // lse, t: null where no gradient follows
 };
 
-// PER neighbours of a row, zeros past its end.
-template <typename T>
-__device__ inline void load_vec(const T* p, int c, int d, bool vec, T (&v)[16 / sizeof(T)]) {
-  constexpr int PER = 16 / (int)sizeof(T);
-  if (vec) {
-    typedef __attribute__((__vector_size__(16))) T TV;
-    const TV t = *reinterpret_cast<const TV*>(p + c);
+// The products of 32 pairs of rows, U steps of 32 k in flight, a lane holding its pair's (that of lane & 31, in one of the two lanes).
+template <typename E, int U>
+__device__ inline float pair_products(const char* a, const char* b, int64_t a_blk, int64_t b_blk, const MmSegs& segs, int steps) {
+  using M = Mma<E>;
+  const int n = (int)threadIdx.x & 31, half = ((int)threadIdx.x >> 5) & 1;
+  f32x16 acc;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) v[e] = t[e];
-  } else {
+  for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+  for (int seg = 0; seg < segs.n; ++seg) {
+    if (segs.low != 0 && seg == segs.low) {
 #pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const T t = p[c + e < d ? c + e : d - 1];
-      v[e] = c + e < d ? t : (T)0.0f;
+      for (int r = 0; r < 16; ++r) acc[r] *= kLowTerm;
+    }
+    const char* pa = a + segs.a[seg] + half * 16;
+    const char* pb = b + segs.b[seg] + half * 16;
+    for (int s = 0; s < steps; s += U) {
+      typename M::frag fa[2 * U], fb[2 * U];
+#pragma unroll
+      for (int u = 0; u < 2 * U; ++u) {
+        if (s + u / 2 < steps) {
+          fa[u] = M::load(reinterpret_cast<const E*>(pa + (u / 2) * a_blk + (u & 1) * 32));
+          fb[u] = M::load(reinterpret_cast<const E*>(pb + (u / 2) * b_blk + (u & 1) * 32));
+        } else {
+          fa[u] = fb[u] = M::zero();
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2 * U; ++u) acc = M::mma_ng(fa[u], fb[u], acc);
+      guard_run(fa, acc);
+      guard_keep(fb);
+      pa += U * a_blk;
+      pb += U * b_blk;
     }
   }
+  float z = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z = 8 * (r >> 2) + 4 * half + (r & 3) == n ? acc[r] : z;
+  return z;
 }
 
-template <typename T>
+template <typename T, int U>
 __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
   __shared__ float2 red[kThreads];
   __shared__ float2 stat[kRows];  // the row's largest logit and log2 of its sum
@@ -301,29 +332,53 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
     f = f / scale_x<T>(a.mode) / scale_w<T>(a.mode);
     unscale = 1.0f / scale_x<T>(a.mode) / scale_w<T>(a.mode);
   }
-  {
-    const int r = tid & (a.rows - 1), g = tid / a.rows, groups = kThreads / a.rows;  // rows is a power of two
+  if (tid < kRows) {
     int at = -1;
-    if (first + r < a.N) at = a.pos != nullptr ? a.pos[first + r] : a.ids[(first + r) * a.ids_ld] == a.ignore ? -1 : (int)(first + r);
+    if (tid < a.rows && first + tid < a.N)
+      at = a.pos != nullptr ? a.pos[first + tid] : a.ids[(first + tid) * a.ids_ld] == a.ignore ? -1 : (int)(first + tid);
+    place[tid] = at;
+  }
+  __syncthreads();
+  const int r_of = tid & (a.rows - 1), g = tid / a.rows, groups = kThreads / a.rows;  // rows is a power of two
+  const int at_of = place[r_of];
+  float2 p[4];
+  auto load = [&](int t) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      p[q] = at_of >= 0 && t + groups * q < a.tiles ? a.part[(int64_t)(t + groups * q) * a.part_ld + at_of] : float2{-INFINITY, 0.0f};
+  };
+  load(g);  // all there are where rows are few, on their way beside the targets'
+  by_format<T>(a.mode, [&](auto wide) {
+    constexpr bool WIDE = decltype(wide)::value;
+    for (int e0 = (3 - (tid >> 6)) * 32; e0 < a.rows * a.K; e0 += 128) {
+      const int e = e0 + (lane & 31), r = e / a.K, k = e - r * a.K;
+      int at = 0;
+      int64_t id = 0;
+      bool is = false;
+      if (e < a.rows * a.K && place[r] >= 0) {
+        const int64_t v = a.ids[(first + r) * a.ids_ld + k];
+        is = v >= 0 && v < a.V;
+        if (is) { id = v; at = place[r]; }
+      }
+      if (__ballot(is) == 0ull) continue;  // a pair that is none takes rows that are there
+      const float z = pair_products<typename Wide<T, WIDE>::E, U>(a.w + id * a.w_ld, a.x + (int64_t)at * a.x_ld, a.w_blk, a.x_blk, a.segs[WIDE], a.ksteps);
+      if (is && (lane >> 5) == ((lane >> 2) & 1)) terms[r][k] = z;
+    }
+  });
+  {
     float m = -INFINITY, s = 0.0f;
     auto add = [&](float2 p) {
       const float mn = fmaxf(m, p.x), b = mn == -INFINITY ? 0.0f : mn;
       s = s * __builtin_amdgcn_exp2f((m - b) * f) + p.y * __builtin_amdgcn_exp2f((p.x - b) * f);
       m = mn;
     };
-    if (at >= 0) {
-      for (int t = g; t < a.tiles; t += groups * 4) {
-        float2 p[4];
+    for (int t = g; t < a.tiles; t += groups * 4) {
+      if (t > g) load(t);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) p[q] = t + groups * q < a.tiles ? a.part[(int64_t)(t + groups * q) * a.part_ld + at] : float2{-INFINITY, 0.0f};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) add(p[q]);
-      }
+      for (int q = 0; q < 4; ++q) add(p[q]);
     }
     red[tid] = float2{m, s};
-    if (tid < kRows) place[tid] = -1;
     __syncthreads();
-    if (g == 0) place[r] = at;
     for (int o = kThreads / 2; o >= a.rows; o >>= 1) {
       if (tid < o) {
         add(red[tid + o]);
@@ -334,40 +389,22 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsArgs a) {
     if (tid < a.rows) stat[tid] = float2{m, log2f(s)};
     __syncthreads();
   }
-  constexpr int PER = 16 / (int)sizeof(T);
-  const int l16 = lane & 15;
-  for (int e = tid >> 4; e < a.rows * a.K; e += 16) {
+  for (int e = tid; e < a.rows * a.K; e += kThreads) {
     const int r = e / a.K, k = e - r * a.K;
-    if (place[r] < 0) continue;  // alike in the 16 lanes
+    if (place[r] < 0) continue;
     const int64_t n = first + r, id = a.ids[n * a.ids_ld + k];
     const float2 p = a.tp == nullptr ? float2{1.0f, 1.0f} : a.tp[n * a.K + k];
     float t = 0.0f, term = 0.0f;
-    if (a.tp == nullptr || id >= 0) {
-      if (id >= 0 && id < a.V) {
-        const T* xr = (const T*)a.x + n * a.x_ld;
-        const T* wr = (const T*)a.w + id * a.w_ld;
-        float dot = 0.0f;
-#pragma unroll 4
-        for (int c = l16 * PER; c < a.d; c += 16 * PER) {
-          T xv[PER], wv[PER];
-          load_vec(xr, c, a.d, a.vec != 0, xv);
-          load_vec(wr, c, a.d, a.vec != 0, wv);
-#pragma unroll
-          for (int q = 0; q < PER; ++q) dot = fmaf((float)xv[q], (float)wv[q], dot);
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor(dot, o);
-        const float away = to_log2 * (stat[r].x * unscale - dot) + stat[r].y;  // lse2 - z2
-        t = __builtin_amdgcn_exp2f(-away) - p.y;
-        term = p.x > 0.0f || !(p.x == p.x) ? p.x * away : 0.0f;
-      } else if (!(p.x < 0.0f)) {
-        t = term = NAN;  // an entry outside the vocabulary
-      }
+    if (id >= 0 && id < a.V) {
+      float away = fmaf(stat[r].x - terms[r][k], f, stat[r].y);  // lse2 - z2
+      away = away < 0.0f ? 0.0f : away;  // a rounding of the sum; NaN stays
+      t = __builtin_amdgcn_exp2f(-away) - p.y;
+      term = p.x > 0.0f || !(p.x == p.x) ? p.x * away : 0.0f;
+    } else if (a.tp == nullptr || (id >= 0 && !(p.x < 0.0f))) {
+      t = term = NAN;  // an entry outside the vocabulary
     }
-    if (l16 == 0) {
-      terms[r][k] = term;
-      if (a.t != nullptr) a.t[n * a.K + k] = t;
-    }
+    terms[r][k] = term;
+    if (a.t != nullptr) a.t[n * a.K + k] = t;
   }
   __syncthreads();
   {
@@ -559,11 +596,6 @@ int64_t es_of(int dtype) { return dtype == 0 ? 4 : 2; }
 bool w_direct(const HeadCall& c) {
   return c.dtype != 0 && c.d % 32 == 0 && ((uintptr_t)c.w & 15) == 0 && c.w_ld % 8 == 0 && c.w_ld * 2 * 256 < ((int64_t)1 << 32);
 }
-bool rows_vec(const HeadCall& c) {
-  const int64_t per = 16 / es_of(c.dtype);
-  return c.d % per == 0 && c.x_ld % per == 0 && c.w_ld % per == 0 && (((uintptr_t)c.x | (uintptr_t)c.w) & 15) == 0;
-}
-
 // Scores of a few rows without a gradient: the rows are operands as they are, and none is taken out.  16 rows of 512 by 50257
 // bf16: 28.0 us with the plan and the copy, 21.6 without.  But rows that do not count are then multiplied as well; us with /
 // without: 512 rows 49.6 / 43.2, of which 40% do not count 43.1 / 42.6; 1024 rows 76.5 / 70.6 and 53.5 / 69.3.
@@ -688,12 +720,14 @@ hipError_t head_fwd(const HeadCall& c) {
     else hipLaunchKernelGGL((stats_kernel<T, HeadTile>), dim3(blocks), dim3(HeadTile<E>::THREADS), 0, c.stream, a);
     HEAD_TRY(hipGetLastError());
     RowsArgs r;
-    r.x = c.x; r.x_ld = c.x_ld; r.w = c.w; r.w_ld = c.w_ld; r.ids = c.ids; r.ids_ld = c.ids_ld; r.tp = p.tp; r.ent = p.ent;
-    r.part = p.part; r.part_ld = p.n_pad; r.tiles = p.tiles_v; r.N = c.N; r.V = c.V; r.ignore = c.ignore_index; r.d = c.d; r.K = c.K;
-    r.vec = rows_vec(c); r.rows = c.N > 2048 ? 8 : c.N > 1024 ? 4 : c.N > 512 ? 2 : 1;
+    r.x = a.x; r.x_ld = a.x_ld; r.x_blk = a.x_blk; r.w = a.w; r.w_ld = a.w_ld; r.w_blk = a.w_blk; r.ksteps = a.ksteps;
+    for (int i = 0; i < 2; ++i) r.segs[i] = a.segs[i];
+    r.ids = c.ids; r.ids_ld = c.ids_ld; r.tp = p.tp; r.ent = p.ent;
+    r.part = p.part; r.part_ld = p.n_pad; r.tiles = p.tiles_v; r.N = c.N; r.V = c.V; r.ignore = c.ignore_index; r.K = c.K;
+    r.rows = c.N > 2048 ? 8 : c.N > 1024 ? 4 : c.N > 512 ? 2 : 1;
     r.temperature = c.temperature; r.pos = direct ? nullptr : st.pos; r.mode = direct ? nullptr : st.mode; r.lse = direct ? nullptr : st.lse; r.t = direct ? nullptr : st.t;
     r.loss = c.reduction == 0 ? c.loss : p.rows;
-    hipLaunchKernelGGL(rows_kernel<T>, dim3((unsigned)((c.N + r.rows - 1) / r.rows)), dim3(kThreads), 0, c.stream, r);
+    hipLaunchKernelGGL((r.rows * r.K > 1 ? rows_kernel<T, 4> : rows_kernel<T, 8>), dim3((unsigned)((c.N + r.rows - 1) / r.rows)), dim3(kThreads), 0, c.stream, r);
     HEAD_TRY(hipGetLastError());
   }
   if (c.reduction != 0) {

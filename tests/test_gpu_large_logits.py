@@ -101,3 +101,61 @@ def test_a_row_of_large_logits_leaves_the_others(dtype):
         g = q.scatter_add(1, y[others].unsqueeze(1), -torch.ones(N - 1, 1, device=DEV).double()).abs()
         reach = (2 * off * (q + g)).T @ X.abs() + N * 2.0 ** -24 * (g.T @ X.abs()) + 2.0 ** -39 * X.abs().sum(0)
         assert bool(((dw.double() - want[2].double()).abs() <= 2 * reach + 2 * step * want[2].double().abs())[away].all())
+
+
+@pytest.mark.parametrize("up", [4, 6, 10, 20, 30])
+@pytest.mark.parametrize("N", [30, 700])
+def test_the_largest_logit_of_all_bits(up, N):
+    # as above, with rows that fp32's two terms hold to 22 bits only: the target's logit is the one in the sum
+    x, w, _ = _rows(up, torch.float32, N)
+    g = torch.Generator(device=DEV).manual_seed(up)
+    x = x * (1.0 + 2.0 ** -9 * torch.rand(N, 1, device=DEV, generator=g))
+    at = torch.arange(N, device=DEV) % 64
+    loss, dx, _ = _grads(x, w, at, N)
+    a = x.double()[torch.arange(N), at]
+    rest = 299 * torch.exp(-a)  # beside the largest
+    one = 8 * 2.0 ** -24
+    off = a * 2.0 ** -21  # of a logit
+    assert bool((loss >= 0).all())
+    assert bool(((loss.double() - torch.log1p(rest)).abs() <= one + 2 * off.clamp(max=1) * rest).all())
+    # dx = -(1 - q) W_at + sum of the others' q W
+    left = rest / (1 + rest)
+    expect = (torch.exp(-a) / (1 + rest)).unsqueeze(1).repeat(1, 64)
+    expect[torch.arange(N), at] = -left
+    assert bool(((dx.double() - expect).abs() <= one + (2 * off.clamp(max=1) * left + 2.0 ** -21 * left).unsqueeze(1)).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,d,V,top", [(8, 512, 300, 120.0), (150, 512, 1000, 30.0), (600, 512, 3000, 60.0), (20, 333, 4001, 100.0), (700, 100, 500, 16.0)])
+def test_confident_rows(N, d, V, top, dtype):
+    # each row's own token is `top` above the others: what is left of 1 is the loss and the gradient
+    g = torch.Generator(device=DEV).manual_seed(N)
+    w = (torch.randn(V, d, device=DEV, generator=g) / math.sqrt(d)).to(dtype)
+    y = torch.randint(0, V, (N,), device=DEV, generator=g)
+    x = (top * w.double()[y] + 0.2 * torch.randn(N, d, device=DEV, generator=g)).to(dtype)
+    loss, dx, dw = _grads(x, w, y, N)
+    X, W = x.double(), w.double()
+    z = X @ W.T
+    z = z - z.gather(1, y.unsqueeze(1))
+    q = torch.exp(z)
+    q[torch.arange(N), y] = 0
+    rest = q.sum(1)
+    q = q / (1 + rest).unsqueeze(1)
+    # Differences of two logits of one product: both of their errors, and per term e^-z of the sum one of 2^-23 (exp2) and two
+    # of 2^-24 z (the difference and its factor; z < 64 where a term counts beside the largest): 130 2^-24.  A sum of 1 + rest: 64
+    # additions in a lane, 2 of lanes and waves, 12 of tiles at most 4 x 256 of them, and 8 of its logarithm: 96, each
+    # at most 2^-24 of it.
+    off = 2 * (d * 2.0 ** -24 + (3 * 2.0 ** -22 if dtype == torch.float32 else 0)) * (X.abs() @ W.abs().T).amax(1)
+    off = torch.expm1(off) + 130 * 2.0 ** -24
+    one = 96 * 2.0 ** -24 * (1 + rest)
+    assert bool((loss >= 0).all())
+    assert bool(((loss.double() - torch.log1p(rest)).abs() <= one + off * rest).all())
+    ug = torch.finfo(dtype).eps / 2 if N > 256 and dtype != torch.float32 else 2.0 ** -16
+    G, B = q.clone(), q * (2 * off.unsqueeze(1) + ug) + 2.0 ** -39
+    G[torch.arange(N), y] = -rest / (1 + rest)
+    B[torch.arange(N), y] = one + 2 * off * rest + ug * rest
+    u = torch.finfo(dtype).eps
+    for got, a, b, m in ((dx, G, B, W), (dw, G.T, B.T, X)):
+        want, reach = a @ m, b @ m.abs() + a.shape[1] * 2.0 ** -24 * (a.abs() @ m.abs())
+        tiny = torch.finfo(dtype).smallest_normal * u
+        assert bool(((got.double() - want).abs() <= reach + u * (want.abs() + reach) + tiny).all())
