@@ -19,6 +19,7 @@ GPU tensors only: a CPU tensor, or a missing libmsa.so, raises.
 """
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native
@@ -556,6 +557,12 @@ def _autocast(*tensors):
     return tensors
 
 
+def _no_tangents(what, *tensors):
+    """Refuses dual tensors: a call without a gradient to follow does not pass autograd, which would refuse them."""
+    if any(forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise NotImplementedError(f"{what}: no forward-mode derivatives")
+
+
 def _rows_2d(x):
     """x (..., n) as 2-D rows with unit stride."""
     if x.dim() != 2:
@@ -660,6 +667,7 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="m
     autograd graph of an eager call on the same leaves is alive (torch's rule for
     every backward pass).
     """
+    _no_tangents("linear_cross_entropy", hidden, weight)
     hidden, weight = _autocast(hidden, weight)
     _head_checks("linear_cross_entropy", hidden, weight, reduction, labels)
     if labels.dtype != torch.int64 or labels.shape != hidden.shape[:-1]:
@@ -685,6 +693,7 @@ def linear_distillation(hidden, weight, teacher_logits, teacher_ids, temperature
     ids of V and above give NaN.  reduction as in linear_cross_entropy.  No gradient
     flows to the teacher.
     """
+    _no_tangents("linear_distillation", hidden, weight, teacher_logits)
     hidden, weight = _autocast(hidden, weight)
     _head_checks("linear_distillation", hidden, weight, reduction, teacher_logits, teacher_ids)
     shape = teacher_ids.shape
@@ -763,6 +772,7 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
     x's type (up to 256 rows: two terms; float32: as in linear_cross_entropy), sums
     are float32.
     """
+    _no_tangents("gated_linear", x, w_gate, w_up)
     x, w_gate, w_up = _autocast(x, w_gate, w_up)
     _one_gpu("gated_linear", x.get_device(), w_gate, w_up)
     if x.dtype not in _DTYPES or w_gate.dtype != x.dtype or w_up.dtype != x.dtype:

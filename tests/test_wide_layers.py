@@ -138,6 +138,29 @@ def test_generation_with_gated_feed_forward():
             assert torch.equal(lm(out[:, :n])["logits"][:, -1].argmax(-1), out[:, n])
 
 
+@pytest.mark.parametrize("place", [0, 1])
+def test_forward_mode_derivatives_are_refused_or_right(place):
+    # the kernels have none: refused before any check of devices, also where no weight requires a gradient
+    import torch.autograd.forward_ad as ad
+
+    from multiscreen import ops
+    torch.manual_seed(5)
+    x, w, y = torch.randn(6, 8), torch.randn(11, 8), torch.randint(0, 11, (6,))
+    t, ids = torch.randn(6, 3), torch.randint(0, 11, (6, 3))
+    with ad.dual_level():
+        args = [x, w]
+        args[place] = ad.make_dual(args[place], torch.randn(args[place].shape))
+        for call in (lambda: ops.linear_cross_entropy(*args, y), lambda: ops.linear_distillation(*args, t, ids),
+                     lambda: ops.linear_distillation(x, w, ad.make_dual(t, t), ids), lambda: ops.gated_linear(*args, w),
+                     lambda: ops.gated_linear(x, w, ad.make_dual(w, w))):
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        # the CPU's forms have them
+        got = ad.unpack_dual(_dense.linear_cross_entropy_dense(*args, y)).tangent
+        want = ad.unpack_dual(F.cross_entropy(args[0] @ args[1].T, y)).tangent
+        torch.testing.assert_close(got, want)
+
+
 # ---------------------------------------------------------------------------
 # The C entry points refuse on the host, before any GPU call.
 # ---------------------------------------------------------------------------
