@@ -183,28 +183,41 @@ def _check_tokens(ids, V):
         raise IndexError(f"token ids must be in [0, {V})")
 
 
+def _product(weight):
+    return lambda rows: rows.float() @ weight.float().T
+
+
 def linear_cross_entropy_dense(hidden, weight, labels, ignore_index=-100, reduction="mean"):
+    return cross_entropy_dense(hidden, _product(weight), labels, ignore_index, reduction)
+
+
+def cross_entropy_dense(hidden, head, labels, ignore_index=-100, reduction="mean"):
+    """head: what makes logits of rows."""
     live = labels != ignore_index
-    _check_tokens(labels[live], weight.shape[0])
-    rows = torch.where(live.unsqueeze(-1), hidden, 0.0).float()  # rows that do not count may hold anything
-    z = rows @ weight.float().T
+    z = head(torch.where(live.unsqueeze(-1), hidden, 0.0)).float()  # rows that do not count may hold anything
+    _check_tokens(labels[live], z.shape[-1])
     at = torch.where(live, labels, 0).unsqueeze(-1)
     loss = torch.logsumexp(z, -1) - z.gather(-1, at).squeeze(-1)
     return _reduce_rows(torch.where(live, loss, 0.0), live, reduction)
 
 
 def linear_distillation_dense(hidden, weight, teacher_logits, teacher_ids, temperature=1.0, reduction="mean"):
+    return distillation_dense(hidden, _product(weight), teacher_logits, teacher_ids, temperature, reduction)
+
+
+def distillation_dense(hidden, head, teacher_logits, teacher_ids, temperature=1.0, reduction="mean"):
+    """head: what makes logits of rows."""
     if not 0.0 < temperature < math.inf:
         raise ValueError(f"temperature must be positive and finite, got {temperature}")
     t = teacher_logits.detach().float() / temperature
     held = (teacher_ids >= 0) & (t != -math.inf)
-    _check_tokens(teacher_ids[held], weight.shape[0])
     live = held.any(-1)
     t = torch.where(held, t, -math.inf)
     log_p = torch.log_softmax(torch.where(live.unsqueeze(-1), t, 0.0), -1)
     p = torch.where(held, log_p.exp(), 0.0)
-    rows = torch.where(live.unsqueeze(-1), hidden, 0.0).float()
-    log_q = torch.log_softmax(rows @ weight.float().T / temperature, -1).gather(-1, torch.where(held, teacher_ids, 0))
+    z = head(torch.where(live.unsqueeze(-1), hidden, 0.0)).float()
+    _check_tokens(teacher_ids[held], z.shape[-1])
+    log_q = torch.log_softmax(z / temperature, -1).gather(-1, torch.where(held, teacher_ids, 0))
     loss = temperature ** 2 * torch.where(p > 0, p * (log_p - log_q), p).sum(-1)
     return _reduce_rows(torch.where(live, loss, 0.0), live, reduction)
 

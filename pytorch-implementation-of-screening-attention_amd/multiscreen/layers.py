@@ -18,6 +18,7 @@ cache, used by MultiscreenLM.generate and generate_speculative.
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
 from . import ops
 from ._dense import gated_linear_dense
@@ -26,9 +27,18 @@ from .attention import ScreeningAttention
 _GATED = {"swiglu": "silu", "geglu": "gelu"}
 
 
+def plain_linears(*modules) -> bool:
+    """Whether using the modules' weights is what calling them does: bias-free nn.Linear without hooks of either
+    direction or a forward of their own.  Replaced, adapted or observed modules are called."""
+    from torch.nn.modules import module as _m
+    return ScreeningAttention._plain(modules) and not (_m._global_backward_hooks or _m._global_backward_pre_hooks) and not any(
+        m._backward_hooks or m._backward_pre_hooks or "forward" in m.__dict__ for m in modules)
+
+
 class GatedFFN(nn.Module):
     """down(dropout(act(gate(x)) * up(x))), dropout behind it: both products, the
-    activation and their product are one kernel on the GPU (ops.gated_linear)."""
+    activation and their product are one kernel on the GPU (ops.gated_linear), unless
+    gate or up is not a plain nn.Linear (plain_linears)."""
 
     def __init__(self, d_model: int, ffn_dim: int, dropout: float = 0.0, activation: str = "silu"):
         super().__init__()
@@ -39,8 +49,12 @@ class GatedFFN(nn.Module):
         self.activation = activation
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        gated = ops.gated_linear if x.is_cuda else gated_linear_dense
-        h = gated(x, self.gate.weight, self.up.weight, self.activation)
+        if plain_linears(self.gate, self.up):
+            gated = ops.gated_linear if x.is_cuda else gated_linear_dense
+            h = gated(x, self.gate.weight, self.up.weight, self.activation)
+        else:
+            act = F.silu if self.activation == "silu" else F.gelu
+            h = act(self.gate(x)) * self.up(x)
         return self.dropout(self.down(self.dropout(h)))
 
 

@@ -29,9 +29,10 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import ops
-from ._dense import linear_cross_entropy_dense, linear_distillation_dense, tree_relations, verify_dense
+from ._dense import (cross_entropy_dense, distillation_dense, linear_cross_entropy_dense, linear_distillation_dense,
+                     tree_relations, verify_dense)
 from .attention import KVCache
-from .layers import MultiscreenBlock
+from .layers import MultiscreenBlock, plain_linears
 
 
 class MultiscreenLM(nn.Module):
@@ -99,9 +100,16 @@ class MultiscreenLM(nn.Module):
              reduction: str = "mean") -> torch.Tensor:
         """forward()'s loss (un-shifted, -100 ignored) without its (B, T, vocab) logits
         (ops.linear_cross_entropy).  float32; reduction "none": (B, T), each token's
-        score with its sign changed."""
+        score with its sign changed.  An lm_head that is not a plain nn.Linear
+        (replaced, adapted, with a bias or hooks) is called, and its logits are formed.
+
+        Not behind forward(): a wrapper that works there (DistributedDataParallel)
+        needs a module around the model whose forward calls this."""
+        hidden = self.hidden_states(input_ids, key_padding_mask)
+        if not plain_linears(self.lm_head):
+            return cross_entropy_dense(hidden, self.lm_head, labels, -100, reduction)
         fn = ops.linear_cross_entropy if input_ids.is_cuda else linear_cross_entropy_dense
-        return fn(self.hidden_states(input_ids, key_padding_mask), self.lm_head.weight, labels, -100, reduction)
+        return fn(hidden, self.lm_head.weight, labels, -100, reduction)
 
     def distillation_loss(self, input_ids: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
                           temperature: float = 1.0, key_padding_mask: torch.Tensor | None = None,
@@ -109,10 +117,12 @@ class MultiscreenLM(nn.Module):
         """Divergence from a teacher of the same vocabulary that gave teacher_logits,
         teacher_ids (B, T, K) = teacher.top_logits(input_ids, K): what a drafting model
         learns for generate_speculative (ops.linear_distillation).  Positions whose ids
-        are all -1 do not count."""
+        are all -1 do not count.  lm_head and wrappers: as loss()."""
+        hidden = self.hidden_states(input_ids, key_padding_mask)
+        if not plain_linears(self.lm_head):
+            return distillation_dense(hidden, self.lm_head, teacher_logits, teacher_ids, temperature, reduction)
         fn = ops.linear_distillation if input_ids.is_cuda else linear_distillation_dense
-        return fn(self.hidden_states(input_ids, key_padding_mask), self.lm_head.weight, teacher_logits, teacher_ids,
-                  temperature, reduction)
+        return fn(hidden, self.lm_head.weight, teacher_logits, teacher_ids, temperature, reduction)
 
     @torch.no_grad()
     def top_logits(self, input_ids: torch.Tensor, k: int, key_padding_mask: torch.Tensor | None = None):

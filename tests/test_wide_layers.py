@@ -161,6 +161,88 @@ def test_forward_mode_derivatives_are_refused_or_right(place):
         torch.testing.assert_close(got, want)
 
 
+class _Adapted(torch.nn.Module):
+    """A low-rank adapter around a Linear, with the weight that the Linear has."""
+
+    def __init__(self, base, scale=0.5):
+        super().__init__()
+        self.base = base
+        self.a = torch.nn.Parameter(scale * torch.randn(3, base.in_features) / math.sqrt(base.in_features))
+        self.b = torch.nn.Parameter(scale * torch.randn(base.out_features, 3))
+
+    @property
+    def weight(self):
+        return self.base.weight
+
+    def forward(self, x):
+        return self.base(x) + x @ self.a.T @ self.b.T
+
+
+def _adapt(kind, owner, name):
+    m = getattr(owner, name)
+    if kind == "adapter":
+        setattr(owner, name, _Adapted(m))
+    elif kind == "bias":
+        new = torch.nn.Linear(m.in_features, m.out_features)
+        new.weight = m.weight
+        setattr(owner, name, new)
+    elif kind == "hook":
+        m.register_forward_hook(lambda mod, args, out: out * 0.5)
+    elif kind == "pre-hook":
+        m.register_forward_pre_hook(lambda mod, args: (args[0] * 0.5,))
+    elif kind == "own forward":
+        m.forward = lambda x: 0.5 * F.linear(x, m.weight)
+
+
+KINDS = ["adapter", "bias", "hook", "pre-hook", "own forward"]
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("ffn", ["swiglu", "geglu"])
+def test_an_adapted_feed_forward_is_called(kind, ffn, device):
+    for name in ("gate", "up"):
+        block = MultiscreenBlock(32, 2, 40, ffn=ffn)
+        f = block.ffn.to(device)
+        _adapt(kind, f, name)
+        f.to(device)
+        x = torch.randn(2, 5, 32, device=device)
+        want = f.down((F.silu if ffn == "swiglu" else F.gelu)(f.gate(x)) * f.up(x))
+        torch.testing.assert_close(f(x), want, rtol=1e-5, atol=1e-6)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_an_adapted_head_is_called(kind, device):
+    lm = _lm().to(device)
+    _adapt(kind, lm, "lm_head")
+    lm.to(device)
+    ids, y = torch.randint(0, 61, (2, 9), device=device), torch.randint(0, 61, (2, 9), device=device)
+    y[1, 6:] = -100
+    want = lm(ids, labels=y)
+    torch.testing.assert_close(lm.loss(ids, y), want["loss"], rtol=1e-5, atol=1e-6)
+    assert not lm.loss(ids, y, reduction="none")[1, 6:].any()
+    t, at = lm.top_logits(ids, 61)  # of its own logits a model has no divergence
+    assert abs(float(lm.distillation_loss(ids, t, at).detach())) < 1e-6
+    for got, loss in ((lm.loss(ids, y), want["loss"]),):
+        a, b = (torch.autograd.grad(v, list(lm.parameters()), allow_unused=True) for v in (got, loss))
+        for p, q in zip(a, b):
+            assert (p is None) == (q is None)
+            if p is not None:
+                torch.testing.assert_close(p, q, rtol=1e-4, atol=1e-6)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_hooks_of_the_backward_pass_see_it(device):
+    lm = _lm(ffn="swiglu").to(device)
+    seen = []
+    for m in (lm.lm_head, lm.blocks[0].ffn.gate, lm.blocks[1].ffn.up):
+        m.register_full_backward_hook(lambda mod, gi, go: seen.append(mod))
+    ids = torch.randint(0, 61, (2, 9), device=device)
+    lm.loss(ids, ids).backward()
+    assert len(seen) == 3
+
+
 # ---------------------------------------------------------------------------
 # The C entry points refuse on the host, before any GPU call.
 # ---------------------------------------------------------------------------
