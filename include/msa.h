@@ -370,7 +370,9 @@ int msa_verify(const msa_verify_args* args, void* stream);
  * kept.  The reference forms them all (its loss is F.cross_entropy of lm_head's
  * output, model.py:101-106); its distillation has no counterpart.
  *   hidden   : (N, d) of type dtype, unit stride over d, hidden_ld elements
- *              from row to row (any alignment: rows that count are copied).
+ *              from row to row (any alignment: rows that count are copied, but
+ *              scores of up to 512 aligned rows of the 2-byte types, reduction 0
+ *              without state, take them in place).  All N rows are readable.
  *   weight   : (V, d) of type dtype, unit stride over d, weight_ld from row to
  *              row.  Used in place where its rows are 16-byte aligned, d % 32
  *              == 0 and dtype is not MSA_F32; else copied once a call.
@@ -390,8 +392,8 @@ int msa_verify(const msa_verify_args* args, void* stream);
  *              the rows that count (NaN if none does, with
  *              gradients of zeros); 2: their sum.
  * A row that counts and names a token outside [0, V) has loss NaN and gradient
- * NaN.  Rows that do not count are not read beyond their ids (and teacher): their
- * hidden may hold anything, and their gradient is 0.
+ * NaN.  Rows that do not count have a gradient of 0, and nothing depends on their
+ * hidden, which may hold anything (but may be read).
  * msa_head_bwd takes the same arguments, state as msa_head_fwd left it (read
  * only) and dloss, fp32: (N) for reduction 0, one value else.  dhidden (N, d) and dweight (V, d) contiguous, of type dtype;
  * either may be null.  The gradient of the logits is formed in pieces of the

@@ -6,7 +6,8 @@
 // Forward: one product over all of the vocabulary whose tiles leave each row's maximum and sum; a row's own logits are
 // K dot products in the same order.  Backward, in pieces of the vocabulary: the product again, now with lse2 known, gives the piece's
 // gradient G in the operand type (1 GB at most, or 256 columns); then dx += G W and dW = G^T x (msa_wide.hip).
-// Rows that do not count are taken out before the products: their x may hold anything.
+// Rows that do not count are taken out before the products, but for a few rows' scores, which leave them unused
+// (x_direct): their x may hold anything.
 // Matrix units bound it, at the clock that the card's power allows: 8192 rows of 512 by 50257 bf16, a training pass 1780 us =
 // logits 400 to 480 (870 to 1020 TFLOP/s), G 580 to 605 (its 823 MB store beside the product), both products 970 to 1030
 // (820 to 870), all else 65.
