@@ -397,7 +397,7 @@ int msa_verify(const msa_verify_args* args, void* stream);
  * msa_head_bwd takes the same arguments, state as msa_head_fwd left it (read
  * only) and dloss, fp32: (N) for reduction 0, one value else.  dhidden (N, d) and dweight (V, d) contiguous, of type dtype;
  * either may be null.  The gradient of the logits is formed in pieces of the
- * vocabulary, rounded to dtype (fp32: to terms, below; the others up to
+ * vocabulary (up to 1 GB, fp32 1.5 GB, or 256 columns of it, whichever is more), rounded to dtype (fp32: to terms, below; the others up to
  * 256 rows: to two terms of their own) and multiplied with fp32 sums.
  * fp32 is taken in terms that the matrix core multiplies.  Where the rows that count,
  * the weight and the rows' coefficients are even (rows' largest entries within 2^10

@@ -2,8 +2,8 @@
 //   dg = dh u act'(g), du = dh act(g);  dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x
 // A tile's A rows alternate between the two weights by 16, so that a lane holds a feature's g and u of the same token and
 // the activation and the product happen in registers: h is written once, g and u never.  The backward pass forms g
-// and u again (keeping them rounded would cost 4 N F bytes and a rounding), in pieces of the features (1 GB of dg and
-// du, or 256 features), then takes the two products of msa_wide.hip.
+// and u again (keeping them rounded would cost 4 N F bytes and a rounding), in pieces of the features (up to 1 GB of dg and
+// du, fp32 1.5 GB, or 256 features, whichever is more), then takes the two products of msa_wide.hip.
 // Matrix units bound it: 32768 rows of 512 to 2048 features, bf16: forward 163 us (840 TFLOP/s), dg and du 235, products 285
 // (960).  16 rows: latency, 7 us of kernel.
 #include "msa_wide.h"

@@ -5,7 +5,7 @@
 //   both           dL_n/dz_nv = T (2^(z2_nv - lse2_n) - sum_{k: id(k) = v} p_k)        (z: logits before 1/T)
 // Forward: one product over all of the vocabulary whose tiles leave each row's maximum and sum; a row's own logits are
 // K dot products in the same order.  Backward, in pieces of the vocabulary: the product again, now with lse2 known, gives the piece's
-// gradient G in the operand type (1 GB at most, or 256 columns); then dx += G W and dW = G^T x (msa_wide.hip).
+// gradient G in the operand type (up to 1 GB, fp32 1.5 GB, or 256 columns, whichever is more); then dx += G W and dW = G^T x (msa_wide.hip).
 // Rows that do not count are taken out before the products, but for a few rows' scores, which leave them unused
 // (x_direct): their x may hold anything.
 // Matrix units bound it, at the clock that the card's power allows: 8192 rows of 512 by 50257 bf16, a training pass 1780 us =

@@ -168,7 +168,7 @@ struct WideShare {
 };
 // segs: products that each tile adds up of one weight (MmSegs).
 WideShare wide_share(int64_t N, int d, int64_t C, int halves, int segs, bool dx, bool dw);
-// The columns of a piece of `rows` weight rows whose G takes `bytes_of_column` a column: 1 GB of G, 512 or 256 MB, by cost.
+// The columns of a piece of `rows` weight rows whose G takes `bytes_of_column` a column (fp32: of the narrow format): 1 GB of G, 512 or 256 MB, by cost, and 256 at least.
 int64_t wide_piece(int64_t N, int d, int64_t rows, int halves, int segs, bool dx, bool dw, int64_t bytes_of_column, WideShare* share);
 
 // The backward products of one piece of the weight's rows.

@@ -658,9 +658,11 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="m
     zeros), "sum", or "none": a loss per row, shaped as labels, of which N = 1 and a
     few rows are the scores of a decoding step.  float32; sums and softmax
     statistics are too.
-    The backward pass forms the logits again, in pieces of the vocabulary of at
-    most 1 GB; their gradient is rounded to hidden's type (up to 256 rows: two terms
-    of the type).  float32 is multiplied in 22 bits where rows and weights are even,
+    Nothing of (rows, V) is kept for the backward pass, which forms the logits again.
+    Its scratch holds their gradient in pieces of the vocabulary of up to 1 GB
+    (float32 1.5 GB) or 256 tokens, whichever is more (all of it where it is less), and float32
+    sums of hidden's gradient, up to 64 of them where rows are few.  The gradient is rounded
+    to hidden's type (up to 256 rows: two terms of the type).  float32 is multiplied in 22 bits where rows and weights are even,
     as behind a norm, and in 24 bits over its whole range, in twice the time, where
     some rows or columns lie 2^10 and more above others.
     Forward and backward pass can be captured into a HIP graph together, once no
