@@ -13,6 +13,8 @@
 // (820 to 870), all else 65.
 #include "msa_wide.h"
 
+#include <float.h>
+
 namespace msa {
 namespace {
 
@@ -117,7 +119,8 @@ __global__ void __launch_bounds__(kThreads) teacher_kernel(const L* logits, int6
     for (int q = 0; q < R; ++q) {
       const int k = q * 64 + lane;
       id[q] = k < K ? ids[n * ids_ld + k] : -1;
-      t[q] = id[q] >= 0 ? to_f(logits[n * lld + k]) * inv_t : -INFINITY;
+      const float raw = id[q] >= 0 ? to_f(logits[n * lld + k]) : -INFINITY;
+      t[q] = fabsf(raw) < INFINITY ? fminf(fmaxf(raw * inv_t, -FLT_MAX), FLT_MAX) : raw;  // a finite logit stays an entry
       any = any || !(t[q] == -INFINITY);
       mx = fmaxf(mx, t[q]);
     }

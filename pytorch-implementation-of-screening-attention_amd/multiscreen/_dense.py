@@ -209,8 +209,10 @@ def distillation_dense(hidden, head, teacher_logits, teacher_ids, temperature=1.
     """head: what makes logits of rows."""
     if not 0.0 < temperature < math.inf:
         raise ValueError(f"temperature must be positive and finite, got {temperature}")
-    t = teacher_logits.detach().float() / temperature
+    t = teacher_logits.detach().float()
     held = (teacher_ids >= 0) & (t != -math.inf)
+    most = torch.finfo(torch.float32).max  # a finite logit stays an entry
+    t = torch.where(t.isfinite(), (t / temperature).clamp(-most, most), t)
     live = held.any(-1)
     t = torch.where(held, t, -math.inf)
     log_p = torch.log_softmax(torch.where(live.unsqueeze(-1), t, 0.0), -1)

@@ -161,6 +161,30 @@ def test_forward_mode_derivatives_are_refused_or_right(place):
         torch.testing.assert_close(got, want)
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_teacher_logits_at_the_ends_of_the_type(dtype, device):
+    # a finite logit is an entry whatever the temperature makes of it
+    from multiscreen import ops
+    fn = ops.linear_distillation if device == "cuda" else _dense.linear_distillation_dense
+    torch.manual_seed(6)
+    x, w, ids = torch.randn(5, 32, device=device), torch.randn(40, 32, device=device), torch.arange(10, 14, device=device).repeat(5, 1)
+    t = torch.randn(5, 4, device=device).to(dtype)
+    info = torch.finfo(dtype)
+    t[1] = info.min                       # all as low as can be: as equal logits
+    t[2, 1:] = info.min                   # all on the first
+    t[3] = info.max
+    t[4] = -math.inf                      # none
+    log_q = torch.log_softmax(x.double() @ w.double().T / 0.5, -1)[:, 10:14]
+    p = torch.softmax(t.double() / 0.5, -1)
+    p[1] = p[3] = 0.25
+    want = 0.25 * (torch.special.xlogy(p, p) - p * log_q).sum(-1)
+    want[4] = 0
+    got = fn(x, w, t, ids, 0.5, reduction="none")
+    torch.testing.assert_close(got.double(), want, rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(fn(x, w, t, ids, 0.5).double(), want.sum() / 4, rtol=1e-5, atol=1e-5)
+
+
 class _Adapted(torch.nn.Module):
     """A low-rank adapter around a Linear, with the weight that the Linear has."""
 
