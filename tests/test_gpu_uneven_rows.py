@@ -195,3 +195,37 @@ def test_gated_gradient_far_above_the_others(up):
     want = R.gated(x, wg[others], wu[others], "silu", dh[:, others])
     for name in ("dgate", "dup"):
         R.check(name, got[name][others], *want[name])
+
+
+def test_a_captured_call_finds_the_format_of_each_replays_data():
+    N, d, V = 300, 64, 1000
+    x, w, y, _ = _head(N, d, V, 6)
+    a, b = _leaf(x, w)
+    xg, wg, wu, dh = _gated(N, d, 200, 7)
+
+    def body():
+        loss = ops.linear_cross_entropy(a, b, y)
+        return {"loss": loss.detach(), **dict(zip(("dhidden", "dweight"), torch.autograd.grad(loss, (a, b)))), **_run(xg, wg, wu, dh, "silu")}
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        body()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = body()
+    for up in (0, 40, 0, 25):
+        with torch.no_grad():
+            a.copy_(x)
+            a[3] *= 2.0 ** -up
+            xg[3] *= 2.0 ** -up
+        graph.replay()
+        torch.cuda.synchronize()
+        got = {k: v.clone() for k, v in out.items()}
+        want = body()
+        for k in want:
+            assert torch.equal(got[k], want[k]), (up, k)
+        with torch.no_grad():
+            xg[3] *= 2.0 ** up
