@@ -553,7 +553,7 @@ def _autocast(*tensors):
     if torch.is_autocast_enabled("cuda") and tensors[0].is_cuda:
         dtype = torch.get_autocast_dtype("cuda")
         if dtype in _DTYPES:
-            return tuple(x.to(dtype) for x in tensors)
+            return tuple(x.to(dtype) if x.dtype in _DTYPES else x for x in tensors)
     return tensors
 
 

@@ -354,3 +354,16 @@ def test_structs_match_the_header():
         fields = [f for line in body.split(";") for f in line.split(",") if f.strip()]
         assert len(pack(*values)) == 8 * len(fields) == 8 * len(values)
     assert f"MSA_HEAD_MAX_K {_native.HEAD_MAX_K}" in text
+
+
+@pytest.mark.gpu
+def test_autocast_leaves_float64_alone():
+    # as torch's own: refused with a type of its own, not narrowed to 8 bits
+    from multiscreen import ops
+    x, w, y = torch.randn(4, 32, device="cuda"), torch.randn(9, 32, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        for call in (lambda: ops.linear_cross_entropy(x.double(), w.double(), y), lambda: ops.gated_linear(x.double(), w.double(), w.double()),
+                     lambda: ops.linear_distillation(x.double(), w, x[:, :2], y.unsqueeze(1).repeat(1, 2))):
+            with pytest.raises(TypeError):
+                call()
+        assert ops.linear_cross_entropy(x, w.half(), y).dtype == torch.float32
