@@ -56,12 +56,14 @@ struct GatedArgs {
   char* g; int64_t plane, half;
 };
 
-// Tl: 128 features of 128 tokens, 64 of 128 where that shares the work better (smaller_tiles), or 32 of 32 for few tokens
-// (forward only: 16 rows of 512 to 2048 features 16.0 -> 11.0 us a call).
+// Tl: 128 features of 128 tokens, 64 of 128 where that shares the work better (smaller_tiles), or forward 32 of 32 where that
+// makes at most two tiles a CU.  us of a forward kernel, 32 of 32 / the better of the others, bf16: 16 rows of 512 to 2048 features
+// 5.7 / 7.6, 64 5.8 / 7.7, 256 (512 tiles) 6.5 / 7.7; 64 rows of 2048 to 8192 (512) 18.1 / 21.4, of 4096 to 11008 (688) 42.4 / 39.7, 96
+// rows of 512 to 8192 (768) 7.4 / 8.0, 128 (1024) 11.2 / 8.3.
 template <typename E> using GatedTile = MmTile<E, 256, 128, 2, 2, false, false, true, 3>;
 template <typename E> using GatedHalf = MmTile<E, 128, 128, 2, 2, false, false, true, 3>;
 template <typename E> using GatedFew = MmTile<E, 64, 32, 2, 1, false, false, true, 8>;
-constexpr int kFew = 32;
+constexpr int64_t kFewTiles = 2 * 256;
 
 template <typename T, bool WIDE, int ACT, int TERMS, typename Tl>  // TERMS: of dg and du; 0: forward
 __device__ inline void gated_tile(const GatedArgs& a, LdsChar* lds) {
@@ -276,7 +278,7 @@ hipError_t launch_tiles(GatedArgs a, int act, hipStream_t s) {
 
 template <typename T, int TERMS>
 hipError_t launch(const GatedArgs& a, int act, hipStream_t s) {
-  if (TERMS == 0 && a.N <= kFew) return launch_tiles<T, 0, GatedFew>(a, act, s);
+  if (TERMS == 0 && (a.cols + 31) / 32 * ((a.N + 31) / 32) <= kFewTiles) return launch_tiles<T, 0, GatedFew>(a, act, s);
   const int64_t tiles_n = (a.N + 127) / 128;
   return smaller_tiles((a.cols + 127) / 128, tiles_n, (a.cols + 63) / 64) ? launch_tiles<T, TERMS, GatedHalf>(a, act, s)
                                                                         : launch_tiles<T, TERMS, GatedTile>(a, act, s);

@@ -190,12 +190,13 @@ __device__ inline void mask_features(typename Tl::Acc& acc, int left, int wm, in
     }
 }
 
-// 256 tokens of the vocabulary by 128 rows, or 64 by 32 for few rows, whose time is the weight's stream: small tiles in all
-// CUs with seven stages ahead.  16 rows of 512 over 50257 tokens take 16 us with either (51 MB: 10 us of stream behind a
-// launch and a first load), but only the small one reads a row's part of x once a tile.
+// 256 tokens of the vocabulary by 128 rows, or 64 by 32 for up to 32 rows, whose time is the weight's stream: small tiles in all
+// CUs with seven stages ahead.  Only up to three of them a CU, which LDS holds at once: a fourth comes late, and large tiles
+// leave fewer partial sums.  us of 16 scores, small / large, bf16, d = 512: V 8003 12.3 / 17.7, 24000 13.1 / 17.9, 40000 17.8 / 20.3,
+// 50257 22.3 / 21.1, 100000 30.0 / 29.0; d = 1024: 40000 25.5 / 29.2, 50257 33.3 / 30.0; fp32, d = 512: 40000 85.0 / 88.7, 50257 105.1 / 98.7.
 template <typename E> using HeadTile = MmTile<E, 256, 128, 2, 2, false, false, false, 3>;
 template <typename E> using HeadFew = MmTile<E, 64, 32, 2, 1, false, false, false, 8>;
-constexpr int kFew = 32;
+constexpr int kFew = 32, kFewTiles = 3 * 256;
 
 template <typename T, bool WIDE, typename Tl>
 __device__ inline void stats_tile(const StatsArgs& a, LdsChar* lds, float2 (*red)[Tl::TILE_N]) {
@@ -630,7 +631,7 @@ struct HeadPlan {
     x_plane = round_up(n_pad * dp * 2, 256);
     w_plane = round_up(c.V * dp * 2, 256);
     tiles_n = (int)(n_pad / 128);
-    few = c.N <= kFew;
+    few = c.N <= kFew && (c.V + 63) / 64 <= kFewTiles;
     tiles_v = (int)(few ? (c.V + 63) / 64 : (c.V + 255) / 256);
     char* p = (char*)c.workspace;
     size_t o = 0;
