@@ -4,8 +4,9 @@
 // the activation and the product happen in registers: h is written once, g and u never.  The backward pass forms g
 // and u again (keeping them rounded would cost 4 N F bytes and a rounding), in pieces of the features (up to 1 GB of dg and
 // du, fp32 1.5 GB, or 256 features, whichever is more), then takes the two products of msa_wide.hip.
-// Matrix units bound it: 32768 rows of 512 to 2048 features, bf16: forward 163 us (840 TFLOP/s), dg and du 235, products 285
-// (960).  16 rows: latency, 7 us of kernel.
+// The products bound it: 32768 rows of 512 to 2048 features, bf16: forward 161 us (850 TFLOP/s, matrix units busy 40% of the
+// cycles: an epilogue for each 16 stages), dg and du 237 (27%: dh's loads and two stores), products 284 (965, 48%).  16 rows:
+// latency, 6 to 7 us of kernel.
 #include "msa_wide.h"
 
 namespace msa {

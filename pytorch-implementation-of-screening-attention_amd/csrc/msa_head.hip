@@ -8,9 +8,10 @@
 // gradient G in the operand type (up to 1 GB, fp32 1.5 GB, or 256 columns, whichever is more); then dx += G W and dW = G^T x (msa_wide.hip).
 // Rows that do not count are taken out before the products, but for a few rows' scores, which leave them unused
 // (x_direct): their x may hold anything.
-// Matrix units bound it, at the clock that the card's power allows: 8192 rows of 512 by 50257 bf16, a training pass 1780 us =
-// logits 400 to 480 (870 to 1020 TFLOP/s), G 580 to 605 (its 823 MB store beside the product), both products 970 to 1030
-// (820 to 870), all else 65.
+// The products bound it: 8192 rows of 512 by 50257 bf16, a training pass 1800 us = logits 400 to 480 (870 to 1020 TFLOP/s),
+// G 580 to 600 (its 823 MB store beside the product), both products 970 to 1030 (820 to 870), all else 75.  Their matrix units are
+// busy 53, 41 and 49% of the cycles, at 1.7 to 2.0 GHz that the card's power allows; the rest are waits for copies and at
+// the barrier of every 32 k, and G's store.
 #include "msa_wide.h"
 
 #include <float.h>
