@@ -452,7 +452,8 @@ int msa_head_bwd(const msa_head_args* args, void* stream);
  * both.  The gradients of x Wg^T and x Wu^T are formed in pieces of the features,
  * rounded to dtype behind a power of two (terms as in msa_head_bwd; fp32 is even where
  * x and the weights are and, backward, the largest entries of their rows and of dh's
- * lie within 2^24 together), sums are fp32.
+ * lie within 2^24 together; fp16's are rounded to 11 bits down to 2^-29, and to 2^-39, of
+ * a bound on all of them, 1.15 max|dh| max|x row| max|weight row|), sums are fp32.
  * Operands are used in place under the conditions of msa_head_args' weight.
  * workspace: msa_gated_workspace_bytes of the same arguments.  1 <= d <= 65536, 1 <= F
  * <= 2^23, N <= 2^23, N d <= 2^38, F d <= 2^37, (N / 128) (F / 128) < 2^24.  Equal calls
