@@ -106,7 +106,7 @@ template <typename E, int N> struct Terms {
 // Terms of G.  2-byte types keep one, in their own type: beside the rounding of dx and dW themselves that makes their error
 // sqrt(2) times as large on average (bf16 2.1e-3 where theirs alone is 1.7e-3; torch's products and cross entropy in the type,
 // which round the logits too, 3.8e-3).  Two terms for all rows make dx and dW twice as long: 8192 rows of 512 by 50257 bf16 1.77 ->
-// 2.86 ms a pass (torch's 2.90).  Few rows average over few roundings, and
+// 2.86 ms a pass (torch's 2.90); a captured pass of less than 10 GFLOP a product 12 to 20% longer.  Few rows average over few roundings, and
 // their products are short: two terms up to 256 rows.  Error of dx and dW over that of their own rounding, one term / two: 1.79
 // / 1.00 for 2 rows, 1.48 / 1.00 for 18, 1.24 to 1.41 / 1.00 for 100 and more.  Time: 84 rows of 1024 by 51364 bf16 191 / 226 us,
 // shorter calls alike (their launches).
